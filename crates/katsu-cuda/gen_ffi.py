@@ -18,6 +18,8 @@ TYPES = {
     "int32_t": "i32", "uint64_t": "u64", "size_t": "usize", "float": "f32",
     "int32_t *": "*mut i32", "uint64_t *": "*mut u64", "float *": "*mut f32", "const float *": "*const f32",
     "float **": "*mut *mut f32", "void **": "*mut *mut c_void", "size_t *": "*mut usize",
+    "int8_t *": "*mut i8", "const int8_t *": "*const i8", "const size_t *": "*const usize",
+    "float *const *": "*const *mut f32", "const float *const *": "*const *const f32",
     "katsu_cuda_ctx *": "*mut Ctx", "katsu_cuda_ctx **": "*mut *mut Ctx",
     "katsu_cuda_event *": "*mut Event", "katsu_cuda_event **": "*mut *mut Event",
 }

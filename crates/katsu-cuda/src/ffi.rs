@@ -25,6 +25,16 @@ pub const KATSU_ERR_UNSUPPORTED: i32 = 7;
 pub const KATSU_MODE_3XTF32: i32 = 0;
 pub const KATSU_MODE_TF32: i32 = 1;
 pub const KATSU_MODE_FP32: i32 = 2;
+pub const KATSU_NORM_RMS: i32 = 0;
+pub const KATSU_NORM_LAYER: i32 = 1;
+pub const KATSU_BLOCK_DX: i32 = 1;
+pub const KATSU_BLOCK_DH: i32 = 2;
+pub const KATSU_BLOCK_DGATE: i32 = 4;
+pub const KATSU_BLOCK_DPOST_W: i32 = 8;
+pub const KATSU_BLOCK_DPOST_B: i32 = 16;
+pub const KATSU_BLOCK_DPRE_W: i32 = 32;
+pub const KATSU_BLOCK_DPRE_B: i32 = 64;
+pub const KATSU_INT8_MAX_K: i32 = 133144;
 pub const KATSU_COMM_ID_BYTES: usize = 128;
 pub const KATSU_SUM_STATIC_MAX_COUNT: usize = 1 << 30;
 
@@ -61,6 +71,16 @@ extern "C" {
     pub fn katsu_cuda_sgd_step(ctx: *mut Ctx, w: *mut f32, dw: *const f32, lr: f32, count: usize) -> i32;
     pub fn katsu_cuda_matmul_fwd(ctx: *mut Ctx, a: *const f32, b: *const f32, c: *mut f32, m: usize, k: usize, n: usize) -> i32;
     pub fn katsu_cuda_matmul_bwd(ctx: *mut Ctx, a: *const f32, b: *const f32, g: *const f32, da: *mut f32, db: *mut f32, m: usize, k: usize, n: usize, accumulate: i32) -> i32;
+    pub fn katsu_cuda_block_norm_fwd(ctx: *mut Ctx, x: *const f32, h: *const f32, gate: *const f32, gate_rows: usize, post_w: *const f32, post_b: *const f32, pre_w: *const f32, pre_b: *const f32, scale: f32, eps: f32, kind: i32, r: *mut f32, n: *mut f32, rows: usize, cols: usize) -> i32;
+    pub fn katsu_cuda_block_norm_bwd(ctx: *mut Ctx, r: *const f32, h: *const f32, gate: *const f32, gate_rows: usize, post_w: *const f32, post_b: *const f32, pre_w: *const f32, scale: f32, eps: f32, kind: i32, dr: *const f32, dn: *const f32, dx: *mut f32, dh: *mut f32, dgate: *mut f32, dpost_w: *mut f32, dpost_b: *mut f32, dpre_w: *mut f32, dpre_b: *mut f32, rows: usize, cols: usize, accumulate: i32) -> i32;
+    pub fn katsu_cuda_int8_row_bytes(k: usize, out_bytes: *mut usize) -> i32;
+    pub fn katsu_cuda_int8_quantize_weights(ctx: *mut Ctx, w: *const f32, q: *mut i8, scale: *mut f32, k: usize, n: usize) -> i32;
+    pub fn katsu_cuda_int8_quantize_rows(ctx: *mut Ctx, x: *const f32, q: *mut i8, scale: *mut f32, m: usize, k: usize) -> i32;
+    pub fn katsu_cuda_int8_matmul(ctx: *mut Ctx, xq: *const i8, xs: *const f32, wq: *const i8, ws: *const f32, bias: *const f32, y: *mut f32, m: usize, k: usize, n: usize) -> i32;
+    pub fn katsu_cuda_int8_linear(ctx: *mut Ctx, x: *const f32, wq: *const i8, ws: *const f32, bias: *const f32, y: *mut f32, m: usize, k: usize, n: usize) -> i32;
+    pub fn katsu_cuda_grad_norm(ctx: *mut Ctx, grads: *const *const f32, counts: *const usize, tensors: usize, norm: *mut f32) -> i32;
+    pub fn katsu_cuda_clip_grads(ctx: *mut Ctx, grads: *const *const f32, out: *const *mut f32, counts: *const usize, tensors: usize, max_norm: f32, norm: *mut f32) -> i32;
+    pub fn katsu_cuda_sgd_step_clipped(ctx: *mut Ctx, weights: *const *mut f32, grads: *const *const f32, counts: *const usize, tensors: usize, lr: f32, max_norm: f32, norm: *mut f32) -> i32;
     pub fn katsu_cuda_add(ctx: *mut Ctx, a: *const f32, b: *const f32, out: *mut f32, count: usize) -> i32;
     pub fn katsu_cuda_mul(ctx: *mut Ctx, a: *const f32, b: *const f32, out: *mut f32, count: usize) -> i32;
     pub fn katsu_cuda_sum(ctx: *mut Ctx, a: *const f32, out: *mut f32, count: usize) -> i32;

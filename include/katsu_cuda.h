@@ -11,8 +11,9 @@
  *  - every function returns an int32_t status (KATSU_OK == 0); nothing throws,
  *    aborts or prints.  katsu_cuda_last_error_string() describes the most
  *    recent failure on the calling thread.
- *  - all tensors are contiguous row-major f32; device pointers come from
- *    katsu_cuda_alloc (or any cudaMalloc'ed memory on the context's device).
+ *  - all tensors are contiguous row-major f32 (the 8-bit matrices of the integer
+ *    product apart); device pointers come from katsu_cuda_alloc (or any
+ *    cudaMalloc'ed memory on the context's device).
  *  - sizes are size_t like the reference's usize; the caller has already run
  *    the reference's shape validation (Geometry::new, matmul rank checks);
  *    the library re-checks what it needs and never launches on bad input.
@@ -194,6 +195,91 @@ int32_t katsu_cuda_matmul_fwd(katsu_cuda_ctx *ctx, const float *a, const float *
  * then receives g @ b^T + a^T @ g (added to its contents when accumulate != 0). */
 int32_t katsu_cuda_matmul_bwd(katsu_cuda_ctx *ctx, const float *a, const float *b, const float *g,
                               float *da, float *db, size_t m, size_t k, size_t n, int32_t accumulate);
+
+/* ---- norms around a block ------------------------------------------------
+ * No counterpart in the reference.  With N(v; w, b) = (v - mean) / sqrt(var + eps) * w + b over the last axis
+ * (KATSU_NORM_LAYER; var = mean((v - mean)^2)) or v / sqrt(mean(v^2) + eps) * w + b (KATSU_NORM_RMS), for every
+ * row of `cols` values:
+ *     r = x + scale * gate * N(h; post)      the residual stream behind a block with output h
+ *     n = N(r; pre)                          the input of the next block
+ * Parts that are left out:
+ *     h null        r = x is not written: only n = N(x; pre); gate, post_w, post_b and r are null
+ *     post_w null   h itself in place of N(h; post); post_b is null
+ *     gate null     1 in its place (gate_rows 0)
+ *     n null        no norm behind the sum; pre_w and pre_b are null
+ * post_b and pre_b may be null (no bias).  gate is [gate_rows, cols], gate_rows a divisor of rows: 1 (one value a
+ * channel), rows (each row its own), or one row of the gate for every rows / gate_rows rows (sequences of one
+ * length).  cols is at least 1; without rows nothing is written.  Outputs alias neither inputs nor each other.
+ * Sums are f32: squares above the f32 range (values above 1.8e19) overflow to a norm of 0. */
+#define KATSU_NORM_RMS 0
+#define KATSU_NORM_LAYER 1
+int32_t katsu_cuda_block_norm_fwd(katsu_cuda_ctx *ctx, const float *x, const float *h, const float *gate,
+                                  size_t gate_rows, const float *post_w, const float *post_b, const float *pre_w,
+                                  const float *pre_b, float scale, float eps, int32_t kind, float *r, float *n,
+                                  size_t rows, size_t cols);
+/* Backward.  r is what the forward wrote (x where h is null); dr and dn are the gradients of r and n (dr null:
+ * zeros; dn is null exactly where pre_w is).  The statistics of the rows are taken again from r and h.
+ *     dx = dr + [gradient through N(r; pre)]        dh = [gradient through the gate and N(h; post)] of dx
+ *     dgate [gate_rows, cols], dpost_w, dpost_b, dpre_w, dpre_b [cols]: sums over rows, in an order that the
+ *     shape fixes
+ * Any output may be null.  `accumulate` is a sum of KATSU_BLOCK_*: those outputs are added to their contents. */
+#define KATSU_BLOCK_DX 1
+#define KATSU_BLOCK_DH 2
+#define KATSU_BLOCK_DGATE 4
+#define KATSU_BLOCK_DPOST_W 8
+#define KATSU_BLOCK_DPOST_B 16
+#define KATSU_BLOCK_DPRE_W 32
+#define KATSU_BLOCK_DPRE_B 64
+int32_t katsu_cuda_block_norm_bwd(katsu_cuda_ctx *ctx, const float *r, const float *h, const float *gate,
+                                  size_t gate_rows, const float *post_w, const float *post_b, const float *pre_w,
+                                  float scale, float eps, int32_t kind, const float *dr, const float *dn, float *dx,
+                                  float *dh, float *dgate, float *dpost_w, float *dpost_b, float *dpre_w,
+                                  float *dpre_b, size_t rows, size_t cols, int32_t accumulate);
+
+/* ---- matrix product in 8-bit integers --------------------------------------
+ * For a model that is served: y = x w + bias from weights and rows of x in 8 bits, with one scale for every
+ * output channel and one for every row (token).  No counterpart in the reference.
+ *     scale = max |v| / 127, rounded to f32;  q = v / scale to the nearest whole number, halves to the even one;
+ *     y[i][j] = (sum_p q_x[i][p] q_w[p][j]) * scale_x[i] * scale_w[j] + bias[j]
+ * The sum is exact (32-bit integers; k is at most KATSU_INT8_MAX_K), so y differs from the real-number formula
+ * by the roundings of its conversion, products and sum to f32 only, and no result depends on the other rows.
+ * A row (column of w) of zeros has scale 0; one that holds an infinity or a NaN has a NaN for its scale, and so
+ * for its results.
+ * A quantised matrix of `rows` rows of k values is int8_t [rows][katsu_cuda_int8_row_bytes], the bytes behind k
+ * zero, at a 16-byte aligned address; w [k, n] is kept transposed, one row for an output channel. */
+#define KATSU_INT8_MAX_K 133144
+/* k rounded up to whole 16-byte units. */
+int32_t katsu_cuda_int8_row_bytes(size_t k, size_t *out_bytes);
+/* w f32 [k, n] -> q int8_t [n][row bytes], scale f32 [n]; done once. */
+int32_t katsu_cuda_int8_quantize_weights(katsu_cuda_ctx *ctx, const float *w, int8_t *q, float *scale, size_t k,
+                                         size_t n);
+/* x f32 [m, k] -> q int8_t [m][row bytes], scale f32 [m]: for several products of the same x. */
+int32_t katsu_cuda_int8_quantize_rows(katsu_cuda_ctx *ctx, const float *x, int8_t *q, float *scale, size_t m,
+                                      size_t k);
+/* y f32 [m, n] from both matrices quantised; bias [n] may be null. */
+int32_t katsu_cuda_int8_matmul(katsu_cuda_ctx *ctx, const int8_t *xq, const float *xs, const int8_t *wq,
+                               const float *ws, const float *bias, float *y, size_t m, size_t k, size_t n);
+/* y f32 [m, n] from x f32 [m, k], whose rows are quantised on the way: the same bits as katsu_cuda_int8_quantize_rows
+ * and katsu_cuda_int8_matmul one after the other. */
+int32_t katsu_cuda_int8_linear(katsu_cuda_ctx *ctx, const float *x, const int8_t *wq, const float *ws,
+                               const float *bias, float *y, size_t m, size_t k, size_t n);
+
+/* ---- the norm over all gradients, and clipping ------------------------------
+ * norm = sqrt of the sum of all squares over `tensors` buffers of counts[i] floats (counts of 0 are fine), summed
+ * in 64 bits in an order that the counts fix; norm[0] is f32 device memory.  The arrays of addresses and counts
+ * are host memory, read before the call returns.  No counterpart in the reference. */
+int32_t katsu_cuda_grad_norm(katsu_cuda_ctx *ctx, const float *const *grads, const size_t *counts, size_t tensors,
+                             float *norm);
+/* out[i] = grads[i] * min(1, max_norm / norm); out[i] may be grads[i] itself, other overlaps of an output are
+ * refused.  Where norm <= max_norm the values stay as they are, bit for bit; so they do where a gradient is
+ * infinite or NaN, which norm[0] then shows.  max_norm is 0 or more. */
+int32_t katsu_cuda_clip_grads(katsu_cuda_ctx *ctx, const float *const *grads, float *const *out, const size_t *counts,
+                              size_t tensors, float max_norm, float *norm);
+/* weights[i] -= lr * (grads[i] * min(1, max_norm / norm)): katsu_cuda_clip_grads and katsu_cuda_sgd_step in one,
+ * without the clipped gradients being stored (the same bits; grads stay as they are).  Where a gradient is infinite
+ * or NaN no weight changes.  Weights overlap neither gradients nor each other. */
+int32_t katsu_cuda_sgd_step_clipped(katsu_cuda_ctx *ctx, float *const *weights, const float *const *grads,
+                                    const size_t *counts, size_t tensors, float lr, float max_norm, float *norm);
 
 /* ---- streaming ops that keep the autograd graph on the device ---------- */
 /* out = a + b / out = a * b; Tensor::elementwise, tensor.rs:226-233. */

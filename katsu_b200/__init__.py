@@ -22,9 +22,9 @@ HOST_LIB_PATH = os.path.join(_PKG, "lib", "libkatsu_host.so")
 USIZE_MAX = (1 << 64) - 1
 
 __all__ = [
-    "Tensor", "Conv2D", "Op", "TensorError", "ShapeOverflow", "InvalidConv", "MissingForward",
+    "Tensor", "Conv2D", "Norm", "BlockNorm", "Int8Linear", "grad_norm", "clip_grad_norm", "sgd_step_clipped", "Op", "TensorError", "ShapeOverflow", "InvalidConv", "MissingForward",
     "NonScalarBackward", "GradientBorrowed", "DataLength", "ShapeMismatch", "RankMismatch",
-    "MatmulMismatch", "Allocation", "DeviceError", "set_device", "set_precision", "synchronize",
+    "MatmulMismatch", "Allocation", "DeviceError", "InvalidOperand", "set_device", "set_precision", "synchronize",
     "set_loss_fusion", "loss_fusion",
     "context", "MODE_3XTF32", "MODE_TF32", "MODE_FP32",
 ]
@@ -106,8 +106,13 @@ class DeviceError(TensorError):
     """CUDA / library failure; has no counterpart in the CPU-only reference."""
 
 
+class InvalidOperand(TensorError):
+    """An operand that a norm, the 8-bit product or clipping does not take (an addition, like these)."""
+
+
 _ERRORS = {1: ShapeOverflow, 2: InvalidConv, 3: MissingForward, 4: NonScalarBackward, 5: GradientBorrowed,
-           6: DataLength, 7: ShapeMismatch, 8: RankMismatch, 9: MatmulMismatch, 10: Allocation, 11: DeviceError}
+           6: DataLength, 7: ShapeMismatch, 8: RankMismatch, 9: MatmulMismatch, 10: Allocation, 11: DeviceError,
+           12: InvalidOperand}
 
 # ---------------------------------------------------------------------------
 # library
@@ -154,6 +159,14 @@ def _load():
             "kh_conv_forward": [_vp, _vp, ctypes.POINTER(_vp)],
             "kh_conv_backward": [_vp, _vp, ctypes.POINTER(_vp), ctypes.POINTER(_vp)],
             "kh_conv_activation_map": [_vp, ctypes.POINTER(_vp)],
+            "kh_norm_new": [_vp, _vp, ctypes.c_float, ctypes.c_int, ctypes.POINTER(_vp)],
+            "kh_norm_forward": [_vp, _vp, ctypes.POINTER(_vp)],
+            "kh_block_norm_new": [_vp, _vp, ctypes.c_float, ctypes.POINTER(_vp)],
+            "kh_block_norm_forward": [_vp, _vp, _vp, _vp, ctypes.POINTER(_vp), ctypes.POINTER(_vp)],
+            "kh_int8_from_weights": [_vp, _vp, ctypes.POINTER(_vp)], "kh_int8_forward": [_vp, _vp, ctypes.POINTER(_vp)],
+            "kh_grad_norm": [ctypes.POINTER(_vp), _sz, ctypes.POINTER(_vp)],
+            "kh_clip_grad_norm": [ctypes.POINTER(_vp), _sz, ctypes.c_float, ctypes.POINTER(_vp)],
+            "kh_sgd_step_clipped": [ctypes.POINTER(_vp), _sz, ctypes.c_float, ctypes.c_float, ctypes.POINTER(_vp)],
         }
         for name, argtypes in sigs.items():
             fn = getattr(lib, name)
@@ -166,6 +179,9 @@ def _load():
             ("kh_conv_free", [_vp], None), ("kh_conv_stride", [_vp], _sz), ("kh_conv_padding", [_vp], _sz),
             ("kh_conv_clear_cache", [_vp], None), ("kh_set_loss_fusion", [ctypes.c_int], None),
             ("kh_tensor_op_flags", [_vp, ctypes.POINTER(ctypes.c_int), ctypes.POINTER(ctypes.c_int)], None),
+            ("kh_tensor_op_norm", [_vp] + [ctypes.POINTER(ctypes.c_float)] * 2 + [ctypes.POINTER(ctypes.c_int)] * 3, None),
+            ("kh_norm_free", [_vp], None), ("kh_block_norm_free", [_vp], None), ("kh_int8_free", [_vp], None),
+            ("kh_int8_features", [_vp, _szp, _szp], None),
         ]:
             fn = getattr(lib, name)
             fn.argtypes, fn.restype = argtypes, restype
@@ -222,16 +238,18 @@ def context() -> int:
 
 
 # ---------------------------------------------------------------------------
-# Op (tensor.rs:85-93, plus Reshape)
+# Op (tensor.rs:85-93, plus Reshape, Norm and BlockSum)
 # ---------------------------------------------------------------------------
 class Op:
-    _KINDS = ["Leaf", "Add", "Mul", "Matmul", "Conv2D", "Sum", "Reshape"]
+    _KINDS = ["Leaf", "Add", "Mul", "Matmul", "Conv2D", "Sum", "Reshape", "Norm", "BlockSum"]
 
-    def __init__(self, kind, stride=None, padding=None, bias=False, relu=False):
+    def __init__(self, kind, stride=None, padding=None, bias=False, relu=False, scale=None, eps=None, layer=False, gate=False,
+                 post=False):
         self.kind, self.stride, self.padding, self.bias, self.relu = kind, stride, padding, bias, relu
+        self.scale, self.eps, self.layer, self.gate, self.post = scale, eps, layer, gate, post
 
     def _key(self):
-        return (self.kind, self.stride, self.padding, self.bias, self.relu)
+        return (self.kind, self.stride, self.padding, self.bias, self.relu, self.scale, self.eps, self.layer, self.gate, self.post)
 
     def __eq__(self, other):
         return isinstance(other, Op) and self._key() == other._key()
@@ -243,6 +261,10 @@ class Op:
         if self.kind == "Conv2D":
             extra = (", bias" if self.bias else "") + (", relu" if self.relu else "")
             return f"Conv2D {{ stride: {self.stride}, padding: {self.padding}{extra} }}"
+        if self.kind in ("Norm", "BlockSum"):
+            flags = "".join(f", {name}" for name in ("layer", "gate", "post", "bias") if getattr(self, name))
+            scale = f"scale: {self.scale}, " if self.kind == "BlockSum" else ""
+            return f"{self.kind} {{ {scale}eps: {self.eps}{flags} }}"
         return self.kind
 
     @staticmethod
@@ -338,10 +360,16 @@ class Tensor:
         kind, stride, padding = ctypes.c_int(), _sz(), _sz()
         _lib.kh_tensor_op(self._h, ctypes.byref(kind), ctypes.byref(stride), ctypes.byref(padding))
         name = Op._KINDS[kind.value]
-        if name != "Conv2D":
+        if name not in ("Conv2D", "Norm", "BlockSum"):
             return Op(name)
         bias, relu = ctypes.c_int(), ctypes.c_int()
         _lib.kh_tensor_op_flags(self._h, ctypes.byref(bias), ctypes.byref(relu))
+        if name != "Conv2D":
+            scale, eps = ctypes.c_float(), ctypes.c_float()
+            layer, gate, post = ctypes.c_int(), ctypes.c_int(), ctypes.c_int()
+            _lib.kh_tensor_op_norm(self._h, *(ctypes.byref(v) for v in (scale, eps, layer, gate, post)))
+            return Op(name, bias=bool(bias.value), scale=scale.value if name == "BlockSum" else None, eps=eps.value,
+                      layer=bool(layer.value), gate=bool(gate.value), post=bool(post.value))
         return Op.Conv2D(stride.value, padding.value, bool(bias.value), bool(relu.value))
 
     def parents(self):
@@ -507,3 +535,112 @@ class Conv2D:
 
     def clear_cache(self):
         _lib.kh_conv_clear_cache(self._h)
+
+
+# ---------------------------------------------------------------------------
+# Additions: what surrounds the products of a block
+# ---------------------------------------------------------------------------
+class Norm:
+    """v / sqrt(mean(v^2) + eps) * weight + bias over the last axis, or with the mean taken off first (layer).
+    weight and bias (may be None) are rank-1 Tensors and take part in autograd."""
+
+    def __init__(self, weight, bias=None, eps=1e-6, layer=False):
+        out = _vp()
+        _check(_load().kh_norm_new(weight._h, bias._h if bias is not None else None, float(eps), 1 if layer else 0,
+                                   ctypes.byref(out)))
+        self._h = out.value
+
+    def __del__(self):
+        h = getattr(self, "_h", None)
+        if h and _lib is not None:
+            _lib.kh_norm_free(h)
+            self._h = None
+
+    def forward(self, x):
+        out = _vp()
+        _check(_lib.kh_norm_forward(self._h, x._h, ctypes.byref(out)))
+        return Tensor._wrap(out.value)
+
+
+class BlockNorm:
+    """The residual sum behind a block with the norms around it, in one pass forward and one backward:
+    r = x + scale * gate * post(h), n = pre(r).  post and pre are Norms of one kind and eps, or None."""
+
+    def __init__(self, post=None, pre=None, scale=1.0):
+        out = _vp()
+        _check(_load().kh_block_norm_new(post._h if post is not None else None, pre._h if pre is not None else None,
+                                         float(scale), ctypes.byref(out)))
+        self._h = out.value
+
+    def __del__(self):
+        h = getattr(self, "_h", None)
+        if h and _lib is not None:
+            _lib.kh_block_norm_free(h)
+            self._h = None
+
+    def forward(self, x, h, gate=None):
+        """(r, n); n is None without pre.  gate: [..., channels] with a row for every one or more rows of x."""
+        r, n = _vp(), _vp()
+        _check(_lib.kh_block_norm_forward(self._h, x._h, h._h, gate._h if gate is not None else None, ctypes.byref(r),
+                                          ctypes.byref(n)))
+        return Tensor._wrap(r.value), Tensor._wrap(n.value) if n.value else None
+
+
+class Int8Linear:
+    """x @ weights + bias in 8-bit integers with a scale for every row of x and every output channel, for serving.  The
+    weights [k, n] are quantised here, once; forward returns a leaf that no gradient passes."""
+
+    def __init__(self, weights, bias=None):
+        out = _vp()
+        _check(_load().kh_int8_from_weights(weights._h, bias._h if bias is not None else None, ctypes.byref(out)))
+        self._h = out.value
+
+    def __del__(self):
+        h = getattr(self, "_h", None)
+        if h and _lib is not None:
+            _lib.kh_int8_free(h)
+            self._h = None
+
+    def _features(self):
+        k, n = _sz(), _sz()
+        _lib.kh_int8_features(self._h, ctypes.byref(k), ctypes.byref(n))
+        return k.value, n.value
+
+    def in_features(self):
+        return self._features()[0]
+
+    def out_features(self):
+        return self._features()[1]
+
+    def forward(self, x):
+        out = _vp()
+        _check(_lib.kh_int8_forward(self._h, x._h, ctypes.byref(out)))
+        return Tensor._wrap(out.value)
+
+
+def _handles(tensors):
+    tensors = list(tensors)
+    return (_vp * len(tensors))(*(t._h for t in tensors)), len(tensors)
+
+
+def grad_norm(tensors):
+    """The norm over the gradients of all `tensors`, as a Tensor of one element that stays on the device until it is read."""
+    lib, out = _load(), _vp()
+    _check(lib.kh_grad_norm(*_handles(tensors), ctypes.byref(out)))
+    return Tensor._wrap(out.value)
+
+
+def clip_grad_norm(tensors, max_norm):
+    """Scales the gradients of all `tensors` in place so that their norm is at most max_norm; returns the norm before.
+    Gradients that hold an infinity or a NaN stay as they are."""
+    lib, out = _load(), _vp()
+    _check(lib.kh_clip_grad_norm(*_handles(tensors), float(max_norm), ctypes.byref(out)))
+    return Tensor._wrap(out.value)
+
+
+def sgd_step_clipped(tensors, lr, max_norm):
+    """clip_grad_norm and sgd_step of all `tensors` in two launches; the gradients stay as they are.  Returns the norm.
+    Where a gradient holds an infinity or a NaN no tensor changes."""
+    lib, out = _load(), _vp()
+    _check(lib.kh_sgd_step_clipped(*_handles(tensors), float(lr), float(max_norm), ctypes.byref(out)))
+    return Tensor._wrap(out.value)

@@ -20,12 +20,16 @@ ERR_INVALID_ARG, ERR_ALLOC, ERR_CUDA, ERR_NCCL, ERR_TIMEOUT, ERR_NO_DEVICE, ERR_
 MODE_3XTF32, MODE_TF32, MODE_FP32 = 0, 1, 2
 SUM_STATIC_MAX_COUNT = 1 << 30
 COMM_ID_BYTES = 128
+NORM_RMS, NORM_LAYER = 0, 1
+BLOCK_DX, BLOCK_DH, BLOCK_DGATE, BLOCK_DPOST_W, BLOCK_DPOST_B, BLOCK_DPRE_W, BLOCK_DPRE_B = (1 << i for i in range(7))
+INT8_MAX_K = 133144
 
 _c_float_p = ctypes.POINTER(ctypes.c_float)
 _sz = ctypes.c_size_t
 _i32 = ctypes.c_int32
 _ctx = ctypes.c_void_p
 _ptr = ctypes.c_void_p  # device pointers travel as integers
+_f32 = ctypes.c_float
 
 # name -> argtypes (restype is int32 for all but last_error_string)
 SIGNATURES = {
@@ -62,6 +66,16 @@ SIGNATURES = {
     "katsu_cuda_square_vjp": [_ctx, _ptr, _ptr, _ptr, _sz, _i32],
     "katsu_cuda_matmul_fwd": [_ctx, _ptr, _ptr, _ptr, _sz, _sz, _sz],
     "katsu_cuda_matmul_bwd": [_ctx, _ptr, _ptr, _ptr, _ptr, _ptr, _sz, _sz, _sz, _i32],
+    "katsu_cuda_block_norm_fwd": [_ctx, _ptr, _ptr, _ptr, _sz] + [_ptr] * 4 + [_f32, _f32, _i32, _ptr, _ptr, _sz, _sz],
+    "katsu_cuda_block_norm_bwd": [_ctx, _ptr, _ptr, _ptr, _sz] + [_ptr] * 3 + [_f32, _f32, _i32] + [_ptr] * 9 + [_sz, _sz, _i32],
+    "katsu_cuda_int8_row_bytes": [_sz, ctypes.POINTER(_sz)],
+    "katsu_cuda_int8_quantize_weights": [_ctx, _ptr, _ptr, _ptr, _sz, _sz],
+    "katsu_cuda_int8_quantize_rows": [_ctx, _ptr, _ptr, _ptr, _sz, _sz],
+    "katsu_cuda_int8_matmul": [_ctx] + [_ptr] * 6 + [_sz] * 3,
+    "katsu_cuda_int8_linear": [_ctx] + [_ptr] * 5 + [_sz] * 3,
+    "katsu_cuda_grad_norm": [_ctx, ctypes.POINTER(_ptr), ctypes.POINTER(_sz), _sz, _ptr],
+    "katsu_cuda_clip_grads": [_ctx, ctypes.POINTER(_ptr), ctypes.POINTER(_ptr), ctypes.POINTER(_sz), _sz, _f32, _ptr],
+    "katsu_cuda_sgd_step_clipped": [_ctx, ctypes.POINTER(_ptr), ctypes.POINTER(_ptr), ctypes.POINTER(_sz), _sz, _f32, _f32, _ptr],
     "katsu_cuda_add": [_ctx, _ptr, _ptr, _ptr, _sz],
     "katsu_cuda_mul": [_ctx, _ptr, _ptr, _ptr, _sz],
     "katsu_cuda_sum": [_ctx, _ptr, _ptr, _sz],
@@ -256,3 +270,59 @@ class Context:
 
     def matmul_bwd(self, a, b, g, da, db, m, k, n, accumulate=0) -> None:
         self.call("katsu_cuda_matmul_bwd", a, b, g, da, db, m, k, n, accumulate)
+
+    # -- norms around a block -----------------------------------------------------
+    def block_norm_fwd(self, x, h, gate, gate_rows, post_w, post_b, pre_w, pre_b, scale, eps, kind, r, n, rows, cols) -> None:
+        self.call("katsu_cuda_block_norm_fwd", x, h, gate, gate_rows, post_w, post_b, pre_w, pre_b, scale, eps, kind, r, n,
+                  rows, cols)
+
+    def block_norm_bwd(self, r, h, gate, gate_rows, post_w, post_b, pre_w, scale, eps, kind, dr, dn, dx, dh, dgate, dpost_w,
+                       dpost_b, dpre_w, dpre_b, rows, cols, accumulate=0) -> None:
+        self.call("katsu_cuda_block_norm_bwd", r, h, gate, gate_rows, post_w, post_b, pre_w, scale, eps, kind, dr, dn, dx, dh,
+                  dgate, dpost_w, dpost_b, dpre_w, dpre_b, rows, cols, accumulate)
+
+    # -- 8-bit integers --------------------------------------------------------------
+    def int8_row_bytes(self, k) -> int:
+        """Bytes of a row of k values of a quantised matrix."""
+        out = ctypes.c_size_t(0)
+        check(self.lib.katsu_cuda_int8_row_bytes(k, ctypes.byref(out)))
+        return int(out.value)
+
+    def int8_quantize_weights(self, w, q, scale, k, n) -> None:
+        self.call("katsu_cuda_int8_quantize_weights", w, q, scale, k, n)
+
+    def int8_quantize_rows(self, x, q, scale, m, k) -> None:
+        self.call("katsu_cuda_int8_quantize_rows", x, q, scale, m, k)
+
+    def int8_matmul(self, xq, xs, wq, ws, bias, y, m, k, n) -> None:
+        self.call("katsu_cuda_int8_matmul", xq, xs, wq, ws, bias, y, m, k, n)
+
+    def int8_linear(self, x, wq, ws, bias, y, m, k, n) -> None:
+        self.call("katsu_cuda_int8_linear", x, wq, ws, bias, y, m, k, n)
+
+    # -- all gradients of a step --------------------------------------------------------
+    @staticmethod
+    def _addresses(pointers):
+        return (_ptr * len(pointers))(*map(int, pointers))
+
+    @staticmethod
+    def _counts(counts, tensors):
+        if len(counts) != tensors:
+            raise ValueError(f"{tensors} addresses, but {len(counts)} counts")
+        return (_sz * tensors)(*map(int, counts))
+
+    def grad_norm(self, grads, counts, norm) -> None:
+        """norm[0] = norm over all of `grads` (device addresses, counts[i] floats each)."""
+        self.call("katsu_cuda_grad_norm", self._addresses(grads), self._counts(counts, len(grads)), len(grads), norm)
+
+    def clip_grads(self, grads, out, counts, max_norm, norm) -> None:
+        if len(out) != len(grads):
+            raise ValueError(f"{len(grads)} gradients, but {len(out)} outputs")
+        self.call("katsu_cuda_clip_grads", self._addresses(grads), self._addresses(out), self._counts(counts, len(grads)),
+                  len(grads), max_norm, norm)
+
+    def sgd_step_clipped(self, weights, grads, counts, lr, max_norm, norm) -> None:
+        if len(weights) != len(grads):
+            raise ValueError(f"{len(grads)} gradients, but {len(weights)} weights")
+        self.call("katsu_cuda_sgd_step_clipped", self._addresses(weights), self._addresses(grads),
+                  self._counts(counts, len(grads)), len(grads), lr, max_norm, norm)

@@ -10,7 +10,10 @@
 
 #include "katsu.hpp"
 
+using katsu::BlockNorm;
 using katsu::Conv2D;
+using katsu::Int8Linear;
+using katsu::Norm;
 using katsu::Tensor;
 using katsu::TensorError;
 
@@ -52,6 +55,12 @@ std::vector<size_t> shape_vec(const size_t *shape, size_t rank) { return std::ve
 Tensor &T(void *h) { return *static_cast<Tensor *>(h); }
 Conv2D &C(void *h) { return *static_cast<Conv2D *>(h); }
 void *box(Tensor t) { return new Tensor(std::move(t)); }
+Tensor optional_tensor(void *h) { return h ? T(h) : Tensor(); }
+std::vector<Tensor> tensor_vec(void *const *handles, size_t count) {
+    std::vector<Tensor> tensors;
+    for (size_t i = 0; i < count; ++i) tensors.push_back(T(handles[i]));
+    return tensors;
+}
 
 struct GradBorrow {
     katsu::GradRef ref;
@@ -136,6 +145,15 @@ void kh_tensor_op_flags(void *h, int *bias, int *relu) {
     const katsu::Op op = T(h).op();
     *bias = op.bias ? 1 : 0;
     *relu = op.relu ? 1 : 0;
+}
+
+void kh_tensor_op_norm(void *h, float *scale, float *eps, int *layer, int *gate, int *post) {
+    const katsu::Op op = T(h).op();
+    *scale = op.scale;
+    *eps = op.eps;
+    *layer = op.layer ? 1 : 0;
+    *gate = op.gate ? 1 : 0;
+    *post = op.post ? 1 : 0;
 }
 
 size_t kh_tensor_parent_count(void *h) { return T(h).parents().size(); }
@@ -248,5 +266,57 @@ int kh_conv_activation_map(void *h, void **out) {
     });
 }
 void kh_conv_clear_cache(void *h) { C(h).clear_cache(); }
+
+// ---- Norm, BlockNorm --------------------------------------------------------
+// bias may be NULL.
+int kh_norm_new(void *weight, void *bias, float eps, int layer, void **out) {
+    return guarded([&] { *out = new Norm(T(weight), optional_tensor(bias), eps, layer != 0); });
+}
+void kh_norm_free(void *h) { delete static_cast<Norm *>(h); }
+int kh_norm_forward(void *h, void *x, void **out) {
+    return guarded([&] { *out = box(static_cast<Norm *>(h)->forward(T(x))); });
+}
+// post and pre are Norm handles or NULL; the layer keeps copies.
+int kh_block_norm_new(void *post, void *pre, float scale, void **out) {
+    return guarded([&] {
+        std::optional<Norm> a, b;
+        if (post) a = *static_cast<Norm *>(post);
+        if (pre) b = *static_cast<Norm *>(pre);
+        *out = new BlockNorm(std::move(a), std::move(b), scale);
+    });
+}
+void kh_block_norm_free(void *h) { delete static_cast<BlockNorm *>(h); }
+// gate may be NULL; *out_n = NULL when the layer has no norm behind the sum.
+int kh_block_norm_forward(void *h, void *x, void *block, void *gate, void **out_r, void **out_n) {
+    return guarded([&] {
+        auto [r, n] = static_cast<BlockNorm *>(h)->forward(T(x), T(block), optional_tensor(gate));
+        *out_n = n.defined() ? box(std::move(n)) : nullptr;
+        *out_r = box(std::move(r));
+    });
+}
+
+// ---- Int8Linear ---------------------------------------------------------------
+int kh_int8_from_weights(void *weights, void *bias, void **out) {
+    return guarded([&] { *out = new Int8Linear(Int8Linear::from_weights(T(weights), optional_tensor(bias))); });
+}
+void kh_int8_free(void *h) { delete static_cast<Int8Linear *>(h); }
+int kh_int8_forward(void *h, void *x, void **out) {
+    return guarded([&] { *out = box(static_cast<Int8Linear *>(h)->forward(T(x))); });
+}
+void kh_int8_features(void *h, size_t *in, size_t *out) {
+    *in = static_cast<Int8Linear *>(h)->in_features();
+    *out = static_cast<Int8Linear *>(h)->out_features();
+}
+
+// ---- all gradients of a step ----------------------------------------------------
+int kh_grad_norm(void *const *tensors, size_t count, void **out) {
+    return guarded([&] { *out = box(katsu::grad_norm(tensor_vec(tensors, count))); });
+}
+int kh_clip_grad_norm(void *const *tensors, size_t count, float max_norm, void **out) {
+    return guarded([&] { *out = box(katsu::clip_grad_norm(tensor_vec(tensors, count), max_norm)); });
+}
+int kh_sgd_step_clipped(void *const *tensors, size_t count, float lr, float max_norm, void **out) {
+    return guarded([&] { *out = box(katsu::sgd_step_clipped(tensor_vec(tensors, count), lr, max_norm)); });
+}
 
 }  // extern "C"

@@ -30,6 +30,7 @@ std::string TensorError::to_string() const {
             return "matmul inner dimensions differ: " + std::to_string(a) + " and " + std::to_string(b);
         case ErrorKind::Allocation: return "tensor allocation failed: " + detail;
         case ErrorKind::Device: return "device error: " + detail;
+        case ErrorKind::InvalidOperand: return "invalid operand: " + detail;
     }
     return "unknown error";
 }
@@ -110,6 +111,9 @@ DeviceBuffer::~DeviceBuffer() {
 //   Bcast   every element is scalar[0]                       (Sum VJP into a fresh adjoint)
 //   Scaled  element i is t + t with t = fl(scalar[0] * source[i])   (both Mul edges of y * y into y's fresh adjoint)
 // `scalar` is another node's one-element adjoint (shared, see share()), `source` the node's own immutable values.
+//
+// Beside either there may be a part that the fused backward of BlockSum will add (see Op::Norm in op_backward): the adjoint
+// `tail_grad` of the node `tail`, a norm of this node's values.
 struct Adjoint {
     enum Kind { Dense, Bcast, Scaled };
     Kind kind = Dense;
@@ -117,6 +121,8 @@ struct Adjoint {
     std::shared_ptr<DeviceBuffer> dense;   // Dense: null until first needed (then zeros)
     std::shared_ptr<DeviceBuffer> scalar;  // Bcast, Scaled
     std::shared_ptr<DeviceBuffer> source;  // Scaled
+    Tensor tail;
+    std::shared_ptr<DeviceBuffer> tail_grad;
 
     // Writes the values out (a no-op for an allocated dense adjoint) and returns the buffer.
     float *to_dense() {
@@ -488,6 +494,96 @@ std::shared_ptr<DeviceBuffer> device_one() {
     return *one;
 }
 
+// Rows and columns of a norm's values: the last axis is normalised.
+size_t last_axis(const std::vector<size_t> &shape) { return shape.back(); }
+size_t rows_of(const Tensor &t) { return t.numel() ? t.numel() / last_axis(t.shape()) : 0; }
+
+// A norm fits into the backward pass of the sum in front of it: one kind and eps for both (a sum without a norm behind its
+// block takes any).
+bool same_norms(const Op &sum, const Op &norm) { return !sum.post || (sum.layer == norm.layer && sum.eps == norm.eps); }
+
+// One katsu_cuda_block_norm_bwd: of a norm alone (`sum` null; `values` is what it normalises), of a sum alone (`norm` null) or of
+// both.  dr is the adjoint of the sum without the norm's part (null: zeros), dn the norm's.  `own` is the adjoint of the node
+// that is being processed; of a sum it is complete afterwards.
+void block_backward(const Tensor &values, const Tensor *sum, const Tensor *norm, const float *dr, const float *dn, Adjoint &own,
+                    Pending &pending, Touched &touched) {
+    if (values.numel() == 0) return;  // adjoints that nothing is added to are zeros
+    katsu_cuda_ctx *ctx = device_context();
+    const size_t cols = last_axis(values.shape()), rows = rows_of(values);
+    int accumulate = 0;
+    std::unordered_set<const TensorNode *> used;
+    std::vector<std::pair<Tensor, std::shared_ptr<DeviceBuffer>>> again;  // a tensor in a second role: added behind the call
+    auto sink = [&](const Tensor &t, int bit) -> float * {
+        if (!used.insert(t.id()).second) {
+            again.emplace_back(t, uninit_buffer(t.numel()));
+            return again.back().second->ptr;
+        }
+        if (touched.count(t.id())) {
+            accumulate |= bit;
+            return pending.at(t.id()).to_add();
+        }
+        return pending.at(t.id()).to_overwrite();
+    };
+    const float *h = nullptr, *gate = nullptr, *post_w = nullptr, *post_b = nullptr, *pre_w = nullptr;
+    float *dx = nullptr, *dh = nullptr, *dgate = nullptr, *dpost_w = nullptr, *dpost_b = nullptr, *dpre_w = nullptr, *dpre_b = nullptr;
+    size_t gate_rows = 0;
+    float scale = 1.f;
+    std::shared_ptr<DeviceBuffer> full;
+    if (sum) {
+        const Op op = sum->op();
+        const auto &parents = sum->parents();
+        scale = op.scale;
+        if (norm) {
+            full = uninit_buffer(sum->numel());
+            dx = full->ptr;
+        }
+        size_t i = 1;
+        h = parents[i].device_data();
+        dh = sink(parents[i++], KATSU_BLOCK_DH);
+        if (op.gate) {
+            gate = parents[i].device_data();
+            gate_rows = rows_of(parents[i]);
+            dgate = sink(parents[i++], KATSU_BLOCK_DGATE);
+        }
+        if (op.post) {
+            post_w = parents[i].device_data();
+            dpost_w = sink(parents[i++], KATSU_BLOCK_DPOST_W);
+        }
+        if (op.bias) {
+            post_b = parents[i].device_data();
+            dpost_b = sink(parents[i++], KATSU_BLOCK_DPOST_B);
+        }
+    }
+    if (norm) {
+        const auto &parents = norm->parents();
+        pre_w = parents[1].device_data();
+        if (!sum) dx = sink(parents[0], KATSU_BLOCK_DX);
+        dpre_w = sink(parents[1], KATSU_BLOCK_DPRE_W);
+        if (norm->op().bias) dpre_b = sink(parents[2], KATSU_BLOCK_DPRE_B);
+    }
+    const Op kind = norm ? norm->op() : sum->op();
+    check(katsu_cuda_block_norm_bwd(ctx, values.device_data(), h, gate, gate_rows, post_w, post_b, pre_w, scale, kind.eps,
+                                    kind.layer ? KATSU_NORM_LAYER : KATSU_NORM_RMS, dr, dn, dx, dh, dgate, dpost_w, dpost_b,
+                                    dpre_w, dpre_b, rows, cols, accumulate));
+    for (const TensorNode *t : used) touched.insert(t);
+    for (auto &[t, buffer] : again)
+        if (t.numel()) check(katsu_cuda_axpy_acc(ctx, pending.at(t.id()).to_add(), buffer->ptr, t.numel()));
+    if (!sum) return;
+    if (full) {
+        own.dense = full;
+        own.kind = Adjoint::Dense;
+        own.scalar.reset();
+        own.source.reset();
+    }
+    const Tensor &x = sum->parents()[0];  // the sum's adjoint reaches x as it is
+    if (touched.count(x.id())) {
+        if (x.numel()) check(katsu_cuda_axpy_acc(ctx, pending.at(x.id()).to_add(), own.to_dense(), x.numel()));
+    } else {
+        pending.at(x.id()).share(own);
+    }
+    touched.insert(x.id());
+}
+
 // Op::backward, tensor.rs:365-449: adds this node's contribution to the
 // pending adjoint of each parent.  `own` is the node's own (complete) adjoint.
 void op_backward(const Tensor &node, Adjoint &own, Pending &pending, Touched &touched) {
@@ -621,6 +717,31 @@ void op_backward(const Tensor &node, Adjoint &own, Pending &pending, Touched &to
                 pending.at(parents[0].id()).share(own);
             touched.insert(parents[0].id());
             return;
+        case Op::Norm: {
+            const Tensor &x = parents[0];
+            bool leaves = true;
+            for (size_t i = 1; i < parents.size(); ++i) leaves = leaves && parents[i].op().kind == Op::Leaf;
+            Adjoint &target = pending.at(x.id());
+            if (x.op().kind == Op::BlockSum && leaves && !target.tail.defined() && same_norms(x.op(), op)) {
+                // The sum in front takes this norm's part into its own pass.  Until then its adjoint is without it, and the
+                // weights are leaves: nobody asks for theirs before the end.
+                own.to_dense();
+                target.tail = node;
+                target.tail_grad = own.dense;
+                return;
+            }
+            block_backward(x, nullptr, &node, nullptr, own.to_dense(), own, pending, touched);
+            return;
+        }
+        case Op::BlockSum: {
+            const float *dr = touched.count(node.id()) || !own.tail.defined() ? own.to_dense() : nullptr;
+            const Tensor tail = own.tail;
+            const std::shared_ptr<DeviceBuffer> dn = own.tail_grad;
+            own.tail = Tensor();
+            own.tail_grad.reset();
+            block_backward(node, &node, tail.defined() ? &tail : nullptr, dr, dn ? dn->ptr : nullptr, own, pending, touched);
+            return;
+        }
         case Op::Matmul: {
             const Tensor &a = parents[0], &b = parents[1];
             const size_t m = a.shape()[0], k = a.shape()[1], n = b.shape()[1];
@@ -838,5 +959,208 @@ std::optional<Tensor> Conv2D::get_activation_map() const {
 }
 
 void Conv2D::clear_cache() { last_forward_.reset(); }
+
+// ---------------------------------------------------------------------------
+// norms around a block
+// ---------------------------------------------------------------------------
+namespace {
+
+// Shapes of x and h behind Norm and BlockNorm: at least one axis, the last one not empty.
+size_t normed_axis(const Tensor &x) {
+    if (x.rank() == 0 || x.shape().back() == 0) fail(ErrorKind::InvalidOperand, "a norm needs a last axis of at least one value");
+    return x.shape().back();
+}
+
+void check_weight(const Norm &norm, size_t cols) {
+    if (norm.weight().shape()[0] != cols) fail(ErrorKind::InvalidOperand, "a norm's weight must have one value per channel of the last axis");
+}
+
+const float *data_or_null(const Tensor &t) { return t.defined() ? t.device_data() : nullptr; }
+
+Op norm_op(const Norm &norm) {
+    Op op;
+    op.kind = Op::Norm;
+    op.eps = norm.eps();
+    op.layer = norm.layer();
+    op.bias = norm.bias().defined();
+    return op;
+}
+
+Tensor norm_node(std::shared_ptr<DeviceBuffer> values, const Norm &norm, const Tensor &of) {
+    std::vector<Tensor> parents = {of, norm.weight()};
+    if (norm.bias().defined()) parents.push_back(norm.bias());
+    return Tensor::make_node(std::move(values), of.shape(), norm_op(norm), std::move(parents));
+}
+
+int kind_of(bool layer) { return layer ? KATSU_NORM_LAYER : KATSU_NORM_RMS; }
+
+}  // namespace
+
+Norm::Norm(Tensor weight, Tensor bias, float eps, bool layer)
+    : weight_(std::move(weight)), bias_(std::move(bias)), eps_(eps), layer_(layer) {
+    if (weight_.rank() != 1) fail(ErrorKind::InvalidOperand, "a norm's weight must have rank 1");
+    if (bias_.defined() && bias_.shape() != weight_.shape()) fail(ErrorKind::InvalidOperand, "a norm's bias must have its weight's shape");
+    if (!(eps >= 0.f) || std::isinf(eps)) fail(ErrorKind::InvalidOperand, "a norm's eps must be 0 or more, and finite");
+}
+
+Tensor Norm::forward(const Tensor &x) const {
+    const size_t cols = normed_axis(x);
+    check_weight(*this, cols);
+    auto n = uninit_buffer(x.numel());
+    if (x.numel())
+        check(katsu_cuda_block_norm_fwd(device_context(), x.device_data(), nullptr, nullptr, 0, nullptr, nullptr,
+                                        weight_.device_data(), data_or_null(bias_), 1.f, eps_, kind_of(layer_), nullptr, n->ptr,
+                                        x.numel() / cols, cols));
+    return norm_node(std::move(n), *this, x);
+}
+
+BlockNorm::BlockNorm(std::optional<Norm> post, std::optional<Norm> pre, float scale)
+    : post_(std::move(post)), pre_(std::move(pre)), scale_(scale) {
+    if (post_ && pre_ && (post_->layer() != pre_->layer() || post_->eps() != pre_->eps()))
+        fail(ErrorKind::InvalidOperand, "the norms around a block must be of one kind and eps");
+}
+
+std::pair<Tensor, Tensor> BlockNorm::forward(const Tensor &x, const Tensor &h, const Tensor &gate) const {
+    if (x.shape() != h.shape()) fail(ErrorKind::ShapeMismatch);
+    const size_t cols = normed_axis(x), rows = x.numel() / cols;
+    if (post_) check_weight(*post_, cols);
+    if (pre_) check_weight(*pre_, cols);
+    size_t gate_rows = 0;
+    if (gate.defined()) {
+        if (gate.rank() == 0 || gate.shape().back() != cols || gate.numel() == 0 || rows % (gate.numel() / cols) != 0)
+            fail(ErrorKind::InvalidOperand, "a gate's last axis must be that of x, and its rows must divide those of x");
+        gate_rows = gate.numel() / cols;
+    }
+    auto r = uninit_buffer(x.numel());
+    std::shared_ptr<DeviceBuffer> n = pre_ ? uninit_buffer(x.numel()) : nullptr;
+    const Norm *any = pre_ ? &*pre_ : post_ ? &*post_ : nullptr;
+    if (x.numel())
+        check(katsu_cuda_block_norm_fwd(device_context(), x.device_data(), h.device_data(), data_or_null(gate), gate_rows,
+                                        post_ ? post_->weight().device_data() : nullptr, post_ ? data_or_null(post_->bias()) : nullptr,
+                                        pre_ ? pre_->weight().device_data() : nullptr, pre_ ? data_or_null(pre_->bias()) : nullptr,
+                                        scale_, any ? any->eps() : 0.f, kind_of(any && any->layer()), r->ptr, n ? n->ptr : nullptr,
+                                        rows, cols));
+    Op op;
+    op.kind = Op::BlockSum;
+    op.scale = scale_;
+    op.gate = gate.defined();
+    std::vector<Tensor> parents = {x, h};
+    if (op.gate) parents.push_back(gate);
+    if (post_) {
+        op.post = true;
+        op.eps = post_->eps();
+        op.layer = post_->layer();
+        op.bias = post_->bias().defined();
+        parents.push_back(post_->weight());
+        if (op.bias) parents.push_back(post_->bias());
+    }
+    Tensor sum = Tensor::make_node(std::move(r), x.shape(), op, std::move(parents));
+    Tensor normed = pre_ ? norm_node(std::move(n), *pre_, sum) : Tensor();
+    return {std::move(sum), std::move(normed)};
+}
+
+// ---------------------------------------------------------------------------
+// the product in 8-bit integers
+// ---------------------------------------------------------------------------
+Int8Linear Int8Linear::from_weights(const Tensor &weights, const Tensor &bias) {
+    if (weights.rank() != 2) fail(ErrorKind::RankMismatch, "", 2, weights.rank());
+    Int8Linear layer;
+    layer.k_ = weights.shape()[0];
+    layer.n_ = weights.shape()[1];
+    if (bias.defined() && (bias.rank() != 1 || bias.shape()[0] != layer.n_))
+        fail(ErrorKind::InvalidOperand, "bias must have one value per output channel");
+    if (layer.k_ == 0 || layer.k_ > KATSU_INT8_MAX_K)
+        fail(ErrorKind::InvalidOperand, "the 8-bit product sums 1 to " + std::to_string(KATSU_INT8_MAX_K) + " values");
+    layer.bias_ = bias;
+    size_t pitch = 0;
+    check(katsu_cuda_int8_row_bytes(layer.k_, &pitch));
+    layer.q_ = uninit_buffer(element_count({layer.n_, pitch / sizeof(float)}));
+    layer.scale_ = uninit_buffer(layer.n_);
+    if (layer.n_)
+        check(katsu_cuda_int8_quantize_weights(device_context(), weights.device_data(), reinterpret_cast<int8_t *>(layer.q_->ptr),
+                                               layer.scale_->ptr, layer.k_, layer.n_));
+    return layer;
+}
+
+Tensor Int8Linear::forward(const Tensor &x) const {
+    if (x.rank() != 2) fail(ErrorKind::RankMismatch, "", x.rank(), 2);
+    const size_t m = x.shape()[0];
+    if (x.shape()[1] != k_) fail(ErrorKind::MatmulMismatch, "", x.shape()[1], k_);
+    auto out = uninit_buffer(element_count({m, n_}));
+    if (out->count)
+        check(katsu_cuda_int8_linear(device_context(), x.device_data(), reinterpret_cast<const int8_t *>(q_->ptr), scale_->ptr,
+                                     data_or_null(bias_), out->ptr, m, k_, n_));
+    return Tensor::make_node(std::move(out), {m, n_}, Op{}, {});
+}
+
+// ---------------------------------------------------------------------------
+// all gradients of a step
+// ---------------------------------------------------------------------------
+namespace {
+
+// Every check before anything changes.
+void check_gradients(const std::vector<Tensor> &tensors, const char *what) {
+    std::unordered_set<const TensorNode *> seen;
+    for (const Tensor &t : tensors) {
+        if (!seen.insert(t.id()).second) fail(ErrorKind::InvalidOperand, std::string(what) + " takes every tensor once");
+        if (t.node()->borrows != 0) fail(ErrorKind::GradientBorrowed);
+        if (!t.node()->has_grad()) fail(ErrorKind::Device, std::string(what) + " needs a gradient of every tensor: run backward first");
+    }
+}
+
+void check_max_norm(float max_norm) {
+    if (!(max_norm >= 0.f)) fail(ErrorKind::InvalidOperand, "max_norm must be 0 or more");
+}
+
+}  // namespace
+
+Tensor grad_norm(const std::vector<Tensor> &tensors) {
+    check_gradients(tensors, "grad_norm");
+    std::vector<const float *> grads;
+    std::vector<size_t> counts;
+    for (const Tensor &t : tensors) {
+        grads.push_back(t.node()->dense_grad()->ptr);
+        counts.push_back(t.numel());
+    }
+    auto norm = uninit_buffer(1);
+    check(katsu_cuda_grad_norm(device_context(), grads.data(), counts.data(), tensors.size(), norm->ptr));
+    return Tensor::make_node(std::move(norm), {}, Op{}, {});
+}
+
+Tensor clip_grad_norm(const std::vector<Tensor> &tensors, float max_norm) {
+    check_max_norm(max_norm);
+    check_gradients(tensors, "clip_grad_norm");
+    std::vector<float *> grads;
+    std::vector<size_t> counts;
+    for (const Tensor &t : tensors) {
+        grads.push_back(t.node()->own_grad());
+        counts.push_back(t.numel());
+    }
+    auto norm = uninit_buffer(1);
+    check(katsu_cuda_clip_grads(device_context(), grads.data(), grads.data(), counts.data(), tensors.size(), max_norm, norm->ptr));
+    for (const Tensor &t : tensors) t.node()->grad_host_valid = false;
+    return Tensor::make_node(std::move(norm), {}, Op{}, {});
+}
+
+Tensor sgd_step_clipped(const std::vector<Tensor> &tensors, float lr, float max_norm) {
+    check_max_norm(max_norm);
+    check_gradients(tensors, "sgd_step_clipped");
+    std::vector<const float *> grads;
+    std::vector<float *> weights;
+    std::vector<size_t> counts;
+    for (const Tensor &t : tensors) {
+        grads.push_back(t.node()->dense_grad()->ptr);
+        weights.push_back(const_cast<float *>(t.node()->device()));
+        counts.push_back(t.numel());
+    }
+    auto norm = uninit_buffer(1);
+    check(katsu_cuda_sgd_step_clipped(device_context(), weights.data(), grads.data(), counts.data(), tensors.size(), lr, max_norm,
+                                      norm->ptr));
+    for (const Tensor &t : tensors) {
+        t.node()->host_valid = false;
+        t.node()->staged.reset();
+    }
+    return Tensor::make_node(std::move(norm), {}, Op{}, {});
+}
 
 }  // namespace katsu

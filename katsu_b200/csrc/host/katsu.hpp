@@ -40,11 +40,12 @@ enum class ErrorKind : int {
     MatmulMismatch,
     Allocation,
     Device,  // addition: a CUDA / library failure (no counterpart in the CPU-only reference)
+    InvalidOperand,  // addition: an operand that a norm, the 8-bit product or clipping does not take
 };
 
 // tensor.rs:9-82.  `a` and `b` carry the two numbers of DataLength
 // {expected, actual}, RankMismatch {left, right} and MatmulMismatch
-// {left_columns, right_rows}; `detail` the &'static str of InvalidConv.
+// {left_columns, right_rows}; `detail` the &'static str of InvalidConv (and the reason of InvalidOperand).
 struct TensorError {
     ErrorKind kind;
     size_t a = 0, b = 0;
@@ -52,16 +53,21 @@ struct TensorError {
     std::string to_string() const;  // the reference's Display text
 };
 
-// tensor.rs:85-93 plus Reshape (the reference has no view op).
+// tensor.rs:85-93 plus Reshape (the reference has no view op), Norm and BlockSum (class Norm, class BlockNorm).
 struct Op {
-    enum Kind : int { Leaf = 0, Add, Mul, Matmul, Conv2D, Sum, Reshape };
+    enum Kind : int { Leaf = 0, Add, Mul, Matmul, Conv2D, Sum, Reshape, Norm, BlockSum };
     Kind kind = Leaf;
     size_t stride = 0, padding = 0;  // Conv2D only
     // Conv2D only, additions (docs/roadmap.md:18-26 names bias and ReLU as the next layer features):
     // the node's third parent is a bias of one value per output channel; the output went through max(., 0).
     bool bias = false, relu = false;
+    // Norm (parents: values, weight and, with `bias`, a bias) and BlockSum (parents: x, h, with `gate` the gate, with `post` the
+    // weight of the norm behind the block and, with `bias`, its bias).
+    float scale = 1.f, eps = 0.f;
+    bool layer = false, gate = false, post = false;
     bool operator==(const Op &o) const {
-        return kind == o.kind && stride == o.stride && padding == o.padding && bias == o.bias && relu == o.relu;
+        return kind == o.kind && stride == o.stride && padding == o.padding && bias == o.bias && relu == o.relu &&
+               scale == o.scale && eps == o.eps && layer == o.layer && gate == o.gate && post == o.post;
     }
 };
 
@@ -207,6 +213,65 @@ class Conv2D {
     size_t stride_ = 1, padding_ = 0;
     std::optional<std::pair<Tensor, Tensor>> last_forward_;
 };
+
+// Additions: what surrounds the products of a block.
+//
+// A norm over the last axis with a weight and, if defined, a bias a channel: v / sqrt(mean(v^2) + eps) * weight + bias, or with
+// the mean taken off first (layer).
+class Norm {
+   public:
+    Norm(Tensor weight, Tensor bias, float eps, bool layer);
+    const Tensor &weight() const { return weight_; }
+    const Tensor &bias() const { return bias_; }  // undefined: none
+    float eps() const { return eps_; }
+    bool layer() const { return layer_; }
+    Tensor forward(const Tensor &x) const;
+
+   private:
+    Tensor weight_, bias_;
+    float eps_;
+    bool layer_;
+};
+
+// The residual sum behind a block with the norms around it, in one pass: r = x + scale * gate * post(h), n = pre(r).  Either
+// norm may be left out; both are of one kind and eps.  The backward pass of the two nodes is one pass too, where the weights
+// of `pre` are leaves.
+class BlockNorm {
+   public:
+    BlockNorm(std::optional<Norm> post, std::optional<Norm> pre, float scale);
+    const std::optional<Norm> &post() const { return post_; }
+    const std::optional<Norm> &pre() const { return pre_; }
+    float scale() const { return scale_; }
+    // gate: undefined, or [..., cols] whose rows divide those of x (katsu_cuda_block_norm_fwd).  The second tensor is
+    // undefined without `pre`.
+    std::pair<Tensor, Tensor> forward(const Tensor &x, const Tensor &h, const Tensor &gate) const;
+
+   private:
+    std::optional<Norm> post_, pre_;
+    float scale_;
+};
+
+// x w + bias with w [k, n] and the rows of x [m, k] in 8 bits (katsu_cuda_int8_linear), for serving: the weights are quantised
+// once, later changes of the tensor are not seen, and what forward returns is a leaf that no gradient passes.
+class Int8Linear {
+   public:
+    static Int8Linear from_weights(const Tensor &weights, const Tensor &bias);
+    Tensor forward(const Tensor &x) const;
+    size_t in_features() const { return k_; }
+    size_t out_features() const { return n_; }
+
+   private:
+    size_t k_ = 0, n_ = 0;
+    std::shared_ptr<DeviceBuffer> q_, scale_;
+    Tensor bias_;
+};
+
+// The norm over the gradients of all `tensors`, each listed once, as a leaf of one element; clipping them to max_norm in place;
+// and the SGD step with clipped gradients, which stay as they are (katsu_cuda_grad_norm, _clip_grads, _sgd_step_clipped).
+// Without a gradient somewhere they fail as sgd_step does, and change nothing.
+Tensor grad_norm(const std::vector<Tensor> &tensors);
+Tensor clip_grad_norm(const std::vector<Tensor> &tensors, float max_norm);
+Tensor sgd_step_clipped(const std::vector<Tensor> &tensors, float lr, float max_norm);
 
 // Geometry::new (conv2d.rs:183-224): validation + output size, integer only.
 struct Geometry {

@@ -1,0 +1,175 @@
+// Matrices to 8 bits: rows of x (one scale a token) and columns of w (one scale an output channel, kept transposed).
+//
+// Rows: a warp (up to 1024 values) or a block takes a row, holds its first 8192 values in registers between the largest
+// magnitude and the quotients and reads the rest again.  Bound: HBM, 4 bytes in and 1 out a value.
+#include "int8.cuh"
+
+namespace {
+
+constexpr int kHeld = 8;  // 16-byte pieces of a row that a thread holds
+
+// Values j .. j + 3 of a row, zeros behind its end.
+template <bool VEC>
+__device__ __forceinline__ void load4(const float *row, size_t j, size_t k, float (&v)[4]) {
+    if (VEC && j + 4 <= k) {
+        const float4 f = __ldg(reinterpret_cast<const float4 *>(row + j));
+        v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = j + i < k ? __ldg(row + j + i) : 0.f;
+    }
+}
+
+__device__ __forceinline__ unsigned largest4(const float (&v)[4]) {
+    return max(max(katsu_magnitude(v[0]), katsu_magnitude(v[1])), max(katsu_magnitude(v[2]), katsu_magnitude(v[3])));
+}
+
+template <int T, bool VEC>
+__global__ void __launch_bounds__(256) quantize_rows_kernel(const float *__restrict__ x, int8_t *q, float *scale,
+                                                            unsigned long long rows, size_t k, size_t pitch) {
+    __shared__ unsigned sh[2][8];
+    launch_next();
+    launch_wait();
+    constexpr int per_block = 256 / T;
+    const int t = threadIdx.x % T;
+    int turn = 0;
+    for (unsigned long long row = (unsigned long long)blockIdx.x * per_block + threadIdx.x / T; row < rows;
+         row += (unsigned long long)gridDim.x * per_block, turn ^= 1) {
+        const float *src = x + row * k;
+        float v[kHeld][4];
+        unsigned most = 0;
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) load4<VEC>(src, 4 * size_t(t + i * T), k, v[i]);
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) most = max(most, largest4(v[i]));
+        for (size_t j = 4 * size_t(t + kHeld * T); j < k; j += 4 * T) {
+            float w[4];
+            load4<VEC>(src, j, k, w);
+            most = max(most, largest4(w));
+        }
+        most = __reduce_max_sync(0xffffffffu, most);
+        if (T > 32) {  // (two sets of places: the row behind this one does not wait for its readers)
+            if ((threadIdx.x & 31) == 0) sh[turn][threadIdx.x >> 5] = most;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < 8; ++w) most = max(most, sh[turn][w]);
+        }
+        const KatsuInt8Scale s = katsu_int8_scale(__uint_as_float(most));
+        if (t == 0) scale[row] = s.scale;
+        unsigned *dst = reinterpret_cast<unsigned *>(q + row * pitch);
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) {
+            const size_t j = 4 * size_t(t + i * T);
+            if (j < pitch) dst[j / 4] = katsu_int8_pack(v[i], s);
+        }
+        for (size_t j = 4 * size_t(t + kHeld * T); j < pitch; j += 4 * T) {
+            float w[4];
+            load4<VEC>(src, j, k, w);
+            dst[j / 4] = katsu_int8_pack(w, s);
+        }
+    }
+}
+
+// Largest magnitude of every column of w [k, n], as bits, over k rows cut into gridDim.y pieces; `most` starts at zero.
+// (The largest of a set does not depend on the order of the atomics.)
+__global__ void __launch_bounds__(256) column_largest_kernel(const float *__restrict__ w, unsigned *most, size_t k, size_t n) {
+    launch_next();
+    launch_wait();
+    const size_t col = size_t(blockIdx.x) * 32 + (threadIdx.x & 31);
+    const size_t begin = k * blockIdx.y / gridDim.y, end = k * (blockIdx.y + 1) / gridDim.y;
+    unsigned m = 0;
+    if (col < n)
+#pragma unroll 8
+        for (size_t p = begin + (threadIdx.x >> 5); p < end; p += 8) m = max(m, katsu_magnitude(__ldg(w + p * n + col)));
+    __shared__ unsigned sh[8][33];
+    sh[threadIdx.x >> 5][threadIdx.x & 31] = m;
+    __syncthreads();
+    if (threadIdx.x < 32 && col < n) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m = max(m, sh[i][threadIdx.x]);
+        atomicMax(most + col, m);
+    }
+}
+
+// A tile of 128 rows of w by 32 columns, through shared memory, to 32 rows of q.
+__global__ void __launch_bounds__(256) quantize_columns_kernel(const float *__restrict__ w, const unsigned *most, int8_t *q,
+                                                               float *scale, size_t k, size_t n, size_t pitch) {
+    __shared__ float tile[128][33];
+    launch_next();
+    launch_wait();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const size_t p0 = size_t(blockIdx.y) * 128, col0 = size_t(blockIdx.x) * 32;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const size_t p = p0 + warp + 8 * i;
+        tile[warp + 8 * i][lane] = p < k && col0 + lane < n ? __ldg(w + p * n + col0 + lane) : 0.f;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const size_t col = col0 + warp + 8 * i;
+        if (col >= n) break;
+        const KatsuInt8Scale s = katsu_int8_scale(__uint_as_float(__ldcg(most + col)));
+        if (blockIdx.y == 0 && lane == 0) scale[col] = s.scale;
+        const size_t p = p0 + 4 * lane;
+        if (p >= pitch) continue;
+        const float v[4] = {tile[4 * lane][warp + 8 * i], tile[4 * lane + 1][warp + 8 * i], tile[4 * lane + 2][warp + 8 * i],
+                            tile[4 * lane + 3][warp + 8 * i]};
+        *reinterpret_cast<unsigned *>(q + col * pitch + p) = katsu_int8_pack(v, s);
+    }
+}
+
+}  // namespace
+
+int32_t katsu_int8_quantize(katsu_cuda_ctx *ctx, const float *x, int8_t *q, float *scale, size_t m, size_t k) {
+    const bool vec = k % 4 == 0 && (reinterpret_cast<uintptr_t>(x) & 15u) == 0;
+    // A row of up to 1024 values is one warp's: eight rows to a block, and no barrier between the largest and the quotients.
+    const bool small = k <= 32 * 4 * kHeld;
+    const size_t need = small ? katsu_div_up(m, 8) : m, most = size_t(ctx->num_sms) * 8;
+    auto kernel = small ? (vec ? quantize_rows_kernel<32, true> : quantize_rows_kernel<32, false>)
+                        : (vec ? quantize_rows_kernel<256, true> : quantize_rows_kernel<256, false>);
+    KATSU_TRY(katsu_prepare_kernel(ctx, (const void *)kernel, 0));
+    return katsu_launch_chained(ctx, kernel, (unsigned)(need < most ? need : most), 256, 0, 1, x, q, scale, m, k,
+                                katsu_int8_pitch(k));
+}
+
+extern "C" int32_t katsu_cuda_int8_row_bytes(size_t k, size_t *out_bytes) {
+    KATSU_REQUIRE(out_bytes != nullptr, "out_bytes is null");
+    KATSU_REQUIRE(k >= 1 && k <= KATSU_INT8_MAX_K, "k must be 1 to KATSU_INT8_MAX_K");
+    *out_bytes = katsu_int8_pitch(k);
+    return KATSU_OK;
+}
+
+extern "C" int32_t katsu_cuda_int8_quantize_rows(katsu_cuda_ctx *ctx, const float *x, int8_t *q, float *scale, size_t m,
+                                                 size_t k) {
+    KATSU_REQUIRE(ctx != nullptr, "null context");
+    KATSU_REQUIRE(k >= 1 && k <= KATSU_INT8_MAX_K, "k must be 1 to KATSU_INT8_MAX_K");
+    KATSU_REQUIRE(m <= 0x7fffffff, "too many rows");
+    if (m == 0) return katsu_bind(ctx);
+    KATSU_REQUIRE(x != nullptr && q != nullptr && scale != nullptr, "null buffer");
+    KATSU_REQUIRE((reinterpret_cast<uintptr_t>(q) & 15u) == 0, "a quantised matrix must be 16-byte aligned");
+    KATSU_TRY(katsu_bind(ctx));
+    return katsu_int8_quantize(ctx, x, q, scale, m, k);
+}
+
+extern "C" int32_t katsu_cuda_int8_quantize_weights(katsu_cuda_ctx *ctx, const float *w, int8_t *q, float *scale, size_t k,
+                                                    size_t n) {
+    KATSU_REQUIRE(ctx != nullptr, "null context");
+    KATSU_REQUIRE(k >= 1 && k <= KATSU_INT8_MAX_K, "k must be 1 to KATSU_INT8_MAX_K");
+    KATSU_REQUIRE(n <= 0x7fffffff, "too many columns");
+    if (n == 0) return katsu_bind(ctx);
+    KATSU_REQUIRE(w != nullptr && q != nullptr && scale != nullptr, "null buffer");
+    KATSU_REQUIRE((reinterpret_cast<uintptr_t>(q) & 15u) == 0, "a quantised matrix must be 16-byte aligned");
+    KATSU_TRY(katsu_bind(ctx));
+    float *most = nullptr;
+    KATSU_TRY(katsu_scratch(ctx, n, &most));
+    KATSU_CUDA_TRY(cudaMemsetAsync(most, 0, n * sizeof(float), ctx->stream));
+    const unsigned tiles = (unsigned)katsu_div_up(n, 32);
+    // pieces of at least 64 rows, about eight blocks to an SM
+    size_t pieces = katsu_div_up(size_t(ctx->num_sms) * 8, tiles);
+    if (pieces > katsu_div_up(k, 64)) pieces = katsu_div_up(k, 64);
+    KATSU_LAUNCH(ctx, column_largest_kernel, dim3(tiles, (unsigned)pieces), 256, 0, w, reinterpret_cast<unsigned *>(most), k, n);
+    KATSU_LAUNCH(ctx, quantize_columns_kernel, dim3(tiles, (unsigned)katsu_div_up(k, 128)), 256, 0, w,
+                 reinterpret_cast<const unsigned *>(most), q, scale, k, n, katsu_int8_pitch(k));
+    return KATSU_OK;
+}

@@ -173,6 +173,13 @@ __device__ __forceinline__ void tma_load_4d(void *smem_dst, const CUtensorMap *m
         : "memory");
 }
 
+// `bytes` contiguous bytes (16-byte aligned addresses, a multiple of 16) to this block's shared memory.
+__device__ __forceinline__ void bulk_load(void *smem_dst, const void *src, uint32_t bytes, uint64_t *bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(smem_u32(smem_dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar))
+                 : "memory");
+}
+
 // Tensor store shared -> global (bulk async group).  Out-of-range parts of the box are
 // clipped.  The issuing thread must commit the group and, before the shared buffer is
 // overwritten, wait until the group has finished reading it.
@@ -305,7 +312,12 @@ __host__ __device__ constexpr uint32_t idesc_f16(int m, int n, bool a_mn_major, 
            | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
 }
 
-// Same with the A operand in tensor memory (lane = row, one 32-bit column per K element;
+// Instruction descriptor for kind::i8: signed 8-bit K-major operands, 32-bit integer accumulator.
+__host__ __device__ constexpr uint32_t idesc_i8(int m, int n) {
+    return (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
+}
+
+// kind::tf32 with the A operand in tensor memory (lane = row, one 32-bit column per K element;
 // A is always K-major in this form).
 __device__ __forceinline__ void mma_tf32_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc,
                                             bool accumulate) {

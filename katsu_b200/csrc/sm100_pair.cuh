@@ -21,6 +21,13 @@ __device__ __forceinline__ uint32_t map_to_rank(const void *local, uint32_t rank
     return out;
 }
 
+// The variable at this place in block `rank`'s shared memory (ordered by a cluster barrier behind the write).
+__device__ __forceinline__ float ld_shared_of_rank(const float *local, uint32_t rank) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(map_to_rank(local, rank)) : "memory");
+    return v;
+}
+
 // Arrival on a barrier of the other block.  Relaxed: what these arrivals publish lives in tensor memory and is
 // ordered by tcgen05.wait / tcgen05.fence around them, not by the memory model; a release at cluster scope made
 // every arrival wait for the thread's earlier global and shared writes to drain (measured: ~2 000 clk per k-block).
@@ -74,6 +81,18 @@ __device__ __forceinline__ void mma_f16_pair(uint32_t tmem_d, uint64_t desc_a, u
         ".reg .pred p;\n"
         "setp.ne.b32 p, %4, 0;\n"
         "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n"
+        "}\n"
+        ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate ? 1u : 0u)
+        : "memory");
+}
+
+// The same with signed 8-bit operands and a 32-bit integer accumulator: 256 x N x 32 per instruction.
+__device__ __forceinline__ void mma_i8_pair(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, bool accumulate) {
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "setp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n"
         "}\n"
         ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate ? 1u : 0u)
         : "memory");

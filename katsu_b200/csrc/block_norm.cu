@@ -17,8 +17,14 @@
 // row whose mean is a thousand times its spread.
 #include <math.h>
 
+#include <initializer_list>
+
 #include "common.cuh"
 #include "launch.cuh"
+#include "sm100.cuh"
+#include "sm100_pair.cuh"
+
+using namespace sm100;
 
 namespace {
 
@@ -44,6 +50,7 @@ struct Backward {
     // Rows go to blocks in groups of equal length: `groups` of them, cut into `slices` blocks each, or several to a block.
     unsigned long long groups;
     int slices, gate_of_row, add_dx, add_dh, add_dgate;
+    int *status;
 };
 
 constexpr int kThreads = 256;
@@ -67,6 +74,361 @@ __device__ __forceinline__ void block_sums(float (&v)[K], float (*sh)[32]) {
         for (int q = 0; q < T / 32; ++q) t += sh[k][q];
         v[k] = t;
     }
+}
+
+// ---- rows that a block holds ------------------------------------------------------------------------------------------
+// N values of a row for each of T threads: pieces of four, T pieces apart (VEC: 16-byte accesses, the row's pieces are whole), or
+// single values T apart.  `width` values from `at` on; what lies behind them is 0 and not stored.
+template <int N, bool VEC>
+__device__ __forceinline__ void load_row(float (&v)[N], const float *at, int t, int T, int width) {
+#pragma unroll
+    for (int i = 0; i < N; i += VEC ? 4 : 1) {
+        if (VEC) {
+            const int j = 4 * (t + i / 4 * T);
+            const float4 f = j < width ? *reinterpret_cast<const float4 *>(at + j) : make_float4(0.f, 0.f, 0.f, 0.f);
+            v[i] = f.x; v[i + 1] = f.y; v[i + 2] = f.z; v[i + 3] = f.w;
+        } else {
+            const int j = t + i * T;
+            v[i] = j < width ? at[j] : 0.f;
+        }
+    }
+}
+
+template <int N, bool VEC>
+__device__ __forceinline__ void store_row(const float (&v)[N], float *at, int t, int T, int width, bool add) {
+#pragma unroll
+    for (int i = 0; i < N; i += VEC ? 4 : 1) {
+        if (VEC) {
+            const int j = 4 * (t + i / 4 * T);
+            if (j >= width) break;
+            float4 f = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+            if (add) {
+                const float4 old = *reinterpret_cast<const float4 *>(at + j);
+                f.x += old.x; f.y += old.y; f.z += old.z; f.w += old.w;
+            }
+            *reinterpret_cast<float4 *>(at + j) = f;
+        } else {
+            const int j = t + i * T;
+            if (j >= width) break;
+            at[j] = add ? at[j] + v[i] : v[i];
+        }
+    }
+}
+
+// Whether value i of this thread is one of the row's.
+template <bool VEC>
+__device__ __forceinline__ bool in_row(int i, int t, int T, int width) {
+    return (VEC ? 4 * (t + i / 4 * T) : t + i * T) < width;
+}
+
+constexpr int kMostThreads = 512;
+
+// Sums over the threads of a row; WARP: the row is a warp's.  Rounds take the two sets of places in turn: a thread that
+// writes to a set again has passed the barrier of the round between, and so have that set's readers.
+template <bool WARP>
+struct Rounds {
+    float (*places)[4][kMostThreads / 32];
+    int turn;
+    template <int K>
+    __device__ __forceinline__ void sums(float (&v)[K]) {
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+        if (WARP) return;
+        const int warps = blockDim.x >> 5;
+        if ((threadIdx.x & 31) == 0)
+#pragma unroll
+            for (int k = 0; k < K; ++k) places[turn][k][threadIdx.x >> 5] = v[k];
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            float t = 0.f;
+            for (int q = 0; q < warps; ++q) t += places[turn][k][q];
+            v[k] = t;
+        }
+        turn ^= 1;
+    }
+};
+
+template <int N, bool VEC, bool WARP, bool LAYER>
+__global__ void __launch_bounds__(kMostThreads) norm_fwd_kernel(const __grid_constant__ Forward p) {
+    __shared__ float places[2][4][kMostThreads / 32];
+    launch_next();
+    launch_wait();
+    Rounds<WARP> rounds = {places, 0};
+    const int T = WARP ? 32 : blockDim.x, t = WARP ? threadIdx.x & 31 : threadIdx.x;
+    const unsigned per_block = WARP ? blockDim.x >> 5 : 1;
+    const float inv = 1.f / float(p.cols);
+    for (unsigned long long row = (unsigned long long)blockIdx.x * per_block + (WARP ? threadIdx.x >> 5 : 0); row < p.rows;
+         row += (unsigned long long)gridDim.x * per_block) {
+        const size_t at = row * size_t(p.cols);
+        float v[N], u[N], w[N];
+        load_row<N, VEC>(v, p.x + at, t, T, p.cols);
+        if (p.h) {
+            load_row<N, VEC>(u, p.h + at, t, T, p.cols);
+            float g[N];
+            if (p.gate) load_row<N, VEC>(g, p.gate + row / p.rows_per_gate * p.cols, t, T, p.cols);
+            if (p.post_w) {
+                float m[1] = {0.f}, sq[1] = {0.f};
+                if (LAYER) {
+#pragma unroll
+                    for (int i = 0; i < N; ++i) m[0] += u[i];
+                    rounds.sums(m);
+                    m[0] *= inv;
+                }
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    if (LAYER) u[i] = in_row<VEC>(i, t, T, p.cols) ? u[i] - m[0] : 0.f;
+                    sq[0] += u[i] * u[i];
+                }
+                load_row<N, VEC>(w, p.post_w, t, T, p.cols);
+                rounds.sums(sq);
+                const float rstd = 1.f / sqrtf(sq[0] * inv + p.eps);
+#pragma unroll
+                for (int i = 0; i < N; ++i) u[i] *= rstd * w[i];
+                if (p.post_b) {
+                    load_row<N, VEC>(w, p.post_b, t, T, p.cols);
+#pragma unroll
+                    for (int i = 0; i < N; ++i) u[i] += w[i];
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] += p.scale * (p.gate ? g[i] * u[i] : u[i]);
+            store_row<N, VEC>(v, p.r + at, t, T, p.cols, false);
+        }
+        if (!p.n) continue;
+        float m[1] = {0.f}, sq[1] = {0.f};
+        if (LAYER) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) m[0] += v[i];
+            rounds.sums(m);
+            m[0] *= inv;
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if (LAYER) v[i] = in_row<VEC>(i, t, T, p.cols) ? v[i] - m[0] : 0.f;
+            sq[0] += v[i] * v[i];
+        }
+        load_row<N, VEC>(w, p.pre_w, t, T, p.cols);
+        rounds.sums(sq);
+        const float rstd = 1.f / sqrtf(sq[0] * inv + p.eps);
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] *= rstd * w[i];
+        if (p.pre_b) {
+            load_row<N, VEC>(w, p.pre_b, t, T, p.cols);
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] += w[i];
+        }
+        store_row<N, VEC>(v, p.n + at, t, T, p.cols, false);
+    }
+}
+
+// First and last row of the block's share; a block has one piece of a group or several whole groups.
+__device__ __forceinline__ void rows_of_block(const Backward &p, unsigned block, unsigned blocks, unsigned long long *begin, unsigned long long *end) {
+    const unsigned long long length = p.rows / p.groups;
+    if (p.slices > 1) {
+        const unsigned long long group = block / p.slices, s = block % p.slices;
+        *begin = group * length + length * s / p.slices;
+        *end = group * length + length * (s + 1) / p.slices;
+    } else {
+        *begin = p.groups * block / blocks * length;
+        *end = p.groups * (block + 1) / blocks * length;
+    }
+}
+
+// Backward of rows that a block (or a cluster of blocks, each with a slab of the columns) holds, eight values a thread.
+//
+// The arrays of a row are brought to shared memory some rows ahead (RING: one bulk copy an array; else plain loads of the row
+// itself), and a thread keeps its columns' sums over the block's rows in registers.  A row costs two or three rounds of sums,
+// about 300 clocks each, beside the 2000 that HBM takes for a row of 2048 values on every SM, so one block's rounds hide
+// behind its own copies.
+constexpr int kValues = 8;
+
+struct Slab {
+    int width, arrays, stages;  // columns to a block; arrays of the ring and its depth in rows
+};
+
+template <bool LAYER, bool RING, bool CLUSTER>
+__global__ void __launch_bounds__(kMostThreads) norm_bwd_kernel(const __grid_constant__ Backward p, const __grid_constant__ Slab slab) {
+    constexpr bool VEC = RING;
+    constexpr int N = kValues;
+    extern __shared__ __align__(128) float ring[];
+    __shared__ float places[2][4][kMostThreads / 32];
+    __shared__ float shared_sums[2][4];  // CLUSTER: this block's sums of a round
+    __shared__ uint64_t full[8];
+    const int T = blockDim.x, t = threadIdx.x;
+    const unsigned rank = CLUSTER ? cluster_ctarank() : 0, blocks_a_row = CLUSTER ? unsigned(p.cols + slab.width - 1) / unsigned(slab.width) : 1;
+    const int c0 = int(rank) * slab.width, width = min(slab.width, p.cols - c0);
+    launch_next();
+    if (RING && t == 0) {
+        for (int s = 0; s < slab.stages; ++s) mbar_init(&full[s], 1);
+        mbar_init_fence();
+    }
+    __syncthreads();
+    launch_wait();
+
+    const float inv = 1.f / float(p.cols);
+    const unsigned block = blockIdx.x / blocks_a_row, blocks = gridDim.x / blocks_a_row;
+    const unsigned long long length = p.rows / p.groups;
+    unsigned long long begin, end;
+    rows_of_block(p, block, blocks, &begin, &end);
+    const bool gate_each = p.gate && p.rows_per_gate == 1;
+    // arrays in the ring: r, then those of h, dn, dr and a gate for each row that there are
+    auto fetch = [&](unsigned long long row) {
+        const int s = int((row - begin) % slab.stages);
+        const uint32_t bytes = uint32_t(width) * 4;
+        float *to = ring + size_t(s) * slab.arrays * slab.width;
+        const size_t at = row * size_t(p.cols) + c0;
+        mbar_arrive_expect_tx(&full[s], bytes * slab.arrays);
+        for (const float *src : {p.r, p.h, p.dn, p.dr, gate_each ? p.gate : nullptr})
+            if (src) {
+                bulk_load(to, src + at, bytes, &full[s]);
+                to += slab.width;
+            }
+    };
+    if (RING && t == 0)
+        for (unsigned long long row = begin; row < end && row < begin + slab.stages; ++row) fetch(row);
+
+    int turn = 0;
+    auto round = [&](auto &v) {  // sums over the row
+        constexpr int K = sizeof(v) / sizeof(v[0]);
+        Rounds<false> r = {places, turn};
+        r.sums(v);
+        if (CLUSTER) {
+            if (t == 0)
+#pragma unroll
+                for (int k = 0; k < K; ++k) shared_sums[turn][k] = v[k];
+            cluster_sync_all();
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                float sum = 0.f;
+                for (unsigned q = 0; q < blocks_a_row; ++q) sum += ld_shared_of_rank(&shared_sums[turn][k], q);
+                v[k] = sum;
+            }
+        }
+        turn ^= 1;
+    };
+
+    float gate[N] = {}, sum_gate[N] = {}, sum_pre_w[N] = {}, sum_pre_b[N] = {}, sum_post_w[N] = {}, sum_post_b[N] = {};
+    for (unsigned long long row = begin; row < end; ++row) {
+        const size_t at = row * size_t(p.cols) + c0;
+        float r[N], h[N], dn[N] = {}, dr[N] = {}, w[N];
+        if (RING) {
+            const unsigned long long i = row - begin;
+            const int s = int(i % slab.stages);
+            // (a wait that gives up leaves wrong values behind, which the next synchronising call reports)
+            mbar_wait_warp(&full[s], uint32_t(i / slab.stages) & 1u, p.status, 191);
+            const float *from = ring + size_t(s) * slab.arrays * slab.width;
+            load_row<N, VEC>(r, from, t, T, width);
+            if (p.h) load_row<N, VEC>(h, from += slab.width, t, T, width);
+            if (p.dn) load_row<N, VEC>(dn, from += slab.width, t, T, width);
+            if (p.dr) load_row<N, VEC>(dr, from += slab.width, t, T, width);
+            if (gate_each) load_row<N, VEC>(gate, from += slab.width, t, T, width);
+            fence_proxy_async_smem();  // in front of the copies behind the first round's barrier
+        } else {
+            load_row<N, VEC>(r, p.r + at, t, T, width);
+            if (p.h) load_row<N, VEC>(h, p.h + at, t, T, width);
+            if (p.dn) load_row<N, VEC>(dn, p.dn + at, t, T, width);
+            if (p.dr) load_row<N, VEC>(dr, p.dr + at, t, T, width);
+            if (gate_each) load_row<N, VEC>(gate, p.gate + at, t, T, width);
+        }
+        if (p.gate && !gate_each && (row == begin || row % p.rows_per_gate == 0))
+            load_row<N, VEC>(gate, p.gate + row / p.rows_per_gate * p.cols + c0, t, T, width);
+        if (!p.h)
+#pragma unroll
+            for (int i = 0; i < N; ++i) h[i] = 0.f;
+        if (LAYER) {
+            float m[2] = {0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                m[0] += r[i];
+                m[1] += h[i];
+            }
+            round(m);
+            const float mr = m[0] * inv, mh = p.post_w ? m[1] * inv : 0.f;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const bool in = in_row<VEC>(i, t, T, width);
+                r[i] = in ? r[i] - mr : 0.f;
+                h[i] = in ? h[i] - mh : 0.f;
+            }
+        }
+        float a[N], v[4] = {0.f, 0.f, 0.f, 0.f};  // squares of r and h, a (r - m) and a
+        if (p.dn) load_row<N, VEC>(w, p.pre_w + c0, t, T, width);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            a[i] = p.dn ? dn[i] * w[i] : 0.f;
+            v[0] += r[i] * r[i];
+            v[1] += h[i] * h[i];
+            v[2] += a[i] * r[i];
+            v[3] += a[i];
+        }
+        round(v);
+        if (RING && t == 0 && row + slab.stages < end) fetch(row + slab.stages);
+        const float rs = 1.f / sqrtf(v[0] * inv + p.eps), hs = 1.f / sqrtf(v[1] * inv + p.eps);
+        const float c_hat = v[2] * rs * inv, c_one = LAYER ? v[3] * inv : 0.f;
+        if (p.dn)
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const float hat = r[i] * rs;
+                dr[i] += rs * (a[i] - hat * c_hat - c_one);  // all of r's gradient from here on
+                sum_pre_w[i] += dn[i] * hat;
+                sum_pre_b[i] += dn[i];
+            }
+        if (p.dx) store_row<N, VEC>(dr, p.dx + at, t, T, width, p.add_dx);
+        if (!p.h) continue;
+        float q[2] = {0.f, 0.f}, b[N];  // b h^ and b behind the block
+        if (p.post_w) {
+            load_row<N, VEC>(w, p.post_w + c0, t, T, width);
+            float bias[N] = {};
+            if (p.post_b && (p.dgate || p.partial[DGATE])) load_row<N, VEC>(bias, p.post_b + c0, t, T, width);
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const float sd = p.scale * dr[i], du = p.gate ? gate[i] * sd : sd;
+                h[i] *= hs;
+                b[i] = in_row<VEC>(i, t, T, width) ? du * w[i] : 0.f;
+                q[0] += b[i] * h[i];
+                q[1] += b[i];
+                sum_post_w[i] += du * h[i];
+                sum_post_b[i] += du;
+                dr[i] = sd * (h[i] * w[i] + bias[i]);  // the gate's
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const float sd = p.scale * dr[i], u = h[i];
+                b[i] = p.gate ? gate[i] * sd : sd;
+                dr[i] = sd * u;
+            }
+        }
+        if (p.gate_of_row) {
+            store_row<N, VEC>(dr, p.dgate + at, t, T, width, p.add_dgate);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) sum_gate[i] += dr[i];
+            if (p.dgate && (row + 1) % length == 0) {
+                store_row<N, VEC>(sum_gate, p.dgate + row / length * p.cols + c0, t, T, width, p.add_dgate);
+#pragma unroll
+                for (int i = 0; i < N; ++i) sum_gate[i] = 0.f;
+            }
+        }
+        if (!p.dh) continue;
+        if (p.post_w) {
+            round(q);
+            const float q_hat = q[0] * inv, q_one = LAYER ? q[1] * inv : 0.f;
+#pragma unroll
+            for (int i = 0; i < N; ++i) b[i] = hs * (b[i] - h[i] * q_hat - q_one);
+        }
+        store_row<N, VEC>(b, p.dh + at, t, T, width, p.add_dh);
+    }
+    const size_t mine = size_t(block) * p.cols + c0;
+    if (p.partial[DPRE_W]) store_row<N, VEC>(sum_pre_w, p.partial[DPRE_W] + mine, t, T, width, false);
+    if (p.partial[DPRE_B]) store_row<N, VEC>(sum_pre_b, p.partial[DPRE_B] + mine, t, T, width, false);
+    if (p.partial[DPOST_W]) store_row<N, VEC>(sum_post_w, p.partial[DPOST_W] + mine, t, T, width, false);
+    if (p.partial[DPOST_B]) store_row<N, VEC>(sum_post_b, p.partial[DPOST_B] + mine, t, T, width, false);
+    if (p.partial[DGATE]) store_row<N, VEC>(sum_gate, p.partial[DGATE] + mine, t, T, width, false);
+    if (CLUSTER) cluster_sync_all();  // no block leaves while another may read its sums
 }
 
 // ---- rows of any length: every round of sums reads its row again (from L2, mostly) ---------------------------------
@@ -117,19 +479,6 @@ __global__ void __launch_bounds__(kThreads) norm_fwd_long_kernel(const __grid_co
     }
 }
 
-// First and last row of the block's share; a block has one piece of a group or several whole groups.
-__device__ __forceinline__ void rows_of_block(const Backward &p, unsigned long long *begin, unsigned long long *end) {
-    const unsigned long long length = p.rows / p.groups;
-    if (p.slices > 1) {
-        const unsigned long long group = blockIdx.x / p.slices, s = blockIdx.x % p.slices;
-        *begin = group * length + length * s / p.slices;
-        *end = group * length + length * (s + 1) / p.slices;
-    } else {
-        *begin = p.groups * blockIdx.x / gridDim.x * length;
-        *end = p.groups * (blockIdx.x + 1) / gridDim.x * length;
-    }
-}
-
 template <bool LAYER>
 __global__ void __launch_bounds__(kThreads) norm_bwd_long_kernel(const __grid_constant__ Backward p) {
     __shared__ float sh[2][32], sh4[4][32], sh2[2][32];
@@ -138,7 +487,7 @@ __global__ void __launch_bounds__(kThreads) norm_bwd_long_kernel(const __grid_co
     const float inv = 1.f / float(p.cols);
     const unsigned long long length = p.rows / p.groups;
     unsigned long long begin, end;
-    rows_of_block(p, &begin, &end);
+    rows_of_block(p, blockIdx.x, gridDim.x, &begin, &end);
     const size_t mine = size_t(blockIdx.x) * p.cols;
     auto add = [&](Sum s, int j, float v, bool first) {
         float *q = p.partial[s] + mine + j;
@@ -278,6 +627,72 @@ int32_t start(katsu_cuda_ctx *ctx, void (*kernel)(Params...), unsigned grid, uns
     return katsu_launch_chained(ctx, kernel, grid, block, 0, 1, args...);
 }
 
+// Whether rows are whole 16-byte pieces at 16-byte addresses.
+bool pieces(int cols, std::initializer_list<const void *> pointers) {
+    uintptr_t at = uintptr_t(cols) * sizeof(float);
+    for (const void *q : pointers) at |= reinterpret_cast<uintptr_t>(q);
+    return (at & 15u) == 0;
+}
+
+template <int N, bool LAYER>
+int32_t start_forward_of(katsu_cuda_ctx *ctx, const Forward &p, bool vec, bool warp, unsigned grid, unsigned block) {
+    if (warp) return start(ctx, vec ? norm_fwd_kernel<16, true, true, LAYER> : norm_fwd_kernel<16, false, true, LAYER>, grid, block, p);
+    return start(ctx, vec ? norm_fwd_kernel<N, true, false, LAYER> : norm_fwd_kernel<N, false, false, LAYER>, grid, block, p);
+}
+
+template <bool LAYER>
+int32_t start_forward(katsu_cuda_ctx *ctx, const Forward &p) {
+    const bool vec = pieces(p.cols, {p.x, p.h, p.gate, p.post_w, p.post_b, p.pre_w, p.pre_b, p.r, p.n});
+    const unsigned long long sms = ctx->num_sms;
+    if (p.cols > kMostThreads * 32)
+        return start(ctx, norm_fwd_long_kernel<LAYER>, unsigned(p.rows < sms * 8 ? p.rows : sms * 8), kThreads, p);
+    // 16 values a thread, 32 where that would take more than 512 threads; up to 512 values are one warp's
+    const bool warp = p.cols <= 512, wide = p.cols > kMostThreads * 16;
+    const unsigned threads = warp ? 128 : unsigned(katsu_div_up(katsu_div_up(p.cols, wide ? 32 : 16), 32)) * 32;
+    const unsigned long long need = warp ? katsu_div_up(p.rows, 4) : p.rows, most = sms * (2048 / threads);
+    const unsigned grid = unsigned(need < most ? need : most);
+    return wide ? start_forward_of<32, LAYER>(ctx, p, vec, warp, grid, threads) : start_forward_of<16, LAYER>(ctx, p, vec, warp, grid, threads);
+}
+
+// Which kernel a backward pass takes, and how many blocks (or clusters) go round at once.
+struct BackwardShape {
+    Slab slab;  // arrays 0: no ring; width 0: the kernel for rows of any length
+    unsigned threads, cluster;
+    size_t smem, most_blocks;
+};
+
+BackwardShape backward_shape(const katsu_cuda_ctx *ctx, const Backward &p, std::initializer_list<const void *> pointers) {
+    BackwardShape s = {};
+    const int most = kMostThreads * kValues;  // columns to a block
+    const bool vec = pieces(p.cols, pointers);
+    if (p.cols > (vec ? 4 : 1) * most) {
+        s.most_blocks = size_t(ctx->num_sms) * 4;
+        return s;
+    }
+    s.cluster = p.cols > 2 * most ? 4 : p.cols > most ? 2 : 1;
+    s.slab.width = int(katsu_div_up(katsu_div_up(p.cols, s.cluster), 4)) * 4;
+    s.threads = unsigned(katsu_div_up(katsu_div_up(s.slab.width, kValues), 32)) * 32;
+    unsigned resident = 512 / s.threads;  // registers: 512 threads to an SM
+    if (resident > 8) resident = 8;
+    if (vec) {
+        s.slab.arrays = 1 + (p.h != nullptr) + (p.dn != nullptr) + (p.dr != nullptr) + (p.gate && p.rows_per_gate == 1);
+        const size_t row = size_t(s.slab.arrays) * s.slab.width * sizeof(float), room = size_t(216) * 1024 / resident - 1024;
+        s.slab.stages = int(room / row < 4 ? room / row : 4);
+        s.smem = s.slab.stages * row;
+    }
+    s.most_blocks = size_t(ctx->num_sms) * resident / s.cluster;
+    return s;
+}
+
+template <bool LAYER>
+int32_t start_backward(katsu_cuda_ctx *ctx, const Backward &p, const BackwardShape &s, size_t blocks) {
+    if (s.slab.width == 0) return start(ctx, norm_bwd_long_kernel<LAYER>, (unsigned)blocks, kThreads, p);
+    auto kernel = s.cluster > 1 ? norm_bwd_kernel<LAYER, true, true>
+                  : s.slab.arrays ? norm_bwd_kernel<LAYER, true, false> : norm_bwd_kernel<LAYER, false, false>;
+    KATSU_TRY(katsu_prepare_kernel(ctx, (const void *)kernel, s.smem));
+    return katsu_launch_chained(ctx, kernel, (unsigned)blocks * s.cluster, s.threads, s.smem, s.cluster, p, s.slab);
+}
+
 int32_t check_sizes(size_t rows, size_t cols, const float *gate, size_t gate_rows, int32_t kind, float eps) {
     KATSU_REQUIRE(kind == KATSU_NORM_RMS || kind == KATSU_NORM_LAYER, "unknown kind of norm");
     KATSU_REQUIRE(eps >= 0.f && eps < INFINITY, "eps must be 0 or more, and finite");
@@ -308,10 +723,7 @@ extern "C" int32_t katsu_cuda_block_norm_fwd(katsu_cuda_ctx *ctx, const float *x
     KATSU_REQUIRE(r != n, "r and n are the same buffer");
     KATSU_TRY(katsu_bind(ctx));
     Forward p = {x, h, gate, post_w, post_b, pre_w, pre_b, r, n, scale, eps, rows, gate ? rows / gate_rows : 1, (int)cols};
-    const size_t most = size_t(ctx->num_sms) * 8;
-    const unsigned blocks = unsigned(rows < most ? rows : most);
-    auto kernel = kind == KATSU_NORM_LAYER ? norm_fwd_long_kernel<true> : norm_fwd_long_kernel<false>;
-    return start(ctx, kernel, blocks, kThreads, p);
+    return kind == KATSU_NORM_LAYER ? start_forward<true>(ctx, p) : start_forward<false>(ctx, p);
 }
 
 extern "C" int32_t katsu_cuda_block_norm_bwd(katsu_cuda_ctx *ctx, const float *r, const float *h, const float *gate,
@@ -354,8 +766,9 @@ extern "C" int32_t katsu_cuda_block_norm_bwd(katsu_cuda_ctx *ctx, const float *r
     p.add_dx = accumulate & KATSU_BLOCK_DX; p.add_dh = accumulate & KATSU_BLOCK_DH; p.add_dgate = adds[DGATE];
     p.gate_of_row = dgate && gate_rows == rows;
     p.groups = dgate && !p.gate_of_row ? gate_rows : 1;
-    // one block a row at first, then more rows to a block: a block's sums over rows are written and read once more
-    const size_t want = size_t(ctx->num_sms) * 4 < rows ? size_t(ctx->num_sms) * 4 : rows;
+    p.status = ctx->status;
+    const BackwardShape shape = backward_shape(ctx, p, {r, h, gate, post_w, post_b, pre_w, dr, dn, dx, dh, dgate});
+    const size_t want = shape.most_blocks < rows ? shape.most_blocks : rows;
     size_t blocks;
     if (p.gate_of_row || dgate == nullptr || p.groups < want) {
         p.slices = (int)katsu_div_up(want, p.groups);
@@ -382,8 +795,7 @@ extern "C" int32_t katsu_cuda_block_norm_bwd(katsu_cuda_ctx *ctx, const float *r
             scratch += blocks * cols;
         }
     }
-    auto kernel = kind == KATSU_NORM_LAYER ? norm_bwd_long_kernel<true> : norm_bwd_long_kernel<false>;
-    KATSU_TRY(start(ctx, kernel, (unsigned)blocks, kThreads, p));
+    KATSU_TRY(kind == KATSU_NORM_LAYER ? start_backward<true>(ctx, p, shape, blocks) : start_backward<false>(ctx, p, shape, blocks));
     if (folds.folds == 0) return KATSU_OK;
     unsigned long long items = 0;
     for (int k = 0; k < folds.folds; ++k) items += folds.f[k].results * katsu_div_up(cols, 32);

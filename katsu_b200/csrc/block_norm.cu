@@ -125,36 +125,71 @@ constexpr int kMostThreads = 512;
 
 // Sums over the threads of a row; WARP: the row is a warp's.  Rounds take the two sets of places in turn: a thread that
 // writes to a set again has passed the barrier of the round between, and so have that set's readers.
+//
+// Up to four sums share one butterfly: each step halves the lanes that carry a sum instead of repeating itself for every sum,
+// 6 exchanges for four sums instead of 20 (with those, and every thread adding up all warps' sums, the two rounds were half of
+// the backward's 890 instructions a row and warp, which bound it: 207 us at 16384 x 2048).
+template <int K>
+__device__ __forceinline__ float packed_sum(const float (&v)[K]) {  // of v[lane / (32 / K)], over the lanes
+    static_assert(K == 1 || K == 2 || K == 4, "sums to a round");
+    const int lane = threadIdx.x & 31;
+    float x;
+    if constexpr (K == 4) {
+        const bool high = lane & 16, odd = lane & 8;
+        const float a = (high ? v[2] : v[0]) + __shfl_xor_sync(0xffffffffu, high ? v[0] : v[2], 16);
+        const float b = (high ? v[3] : v[1]) + __shfl_xor_sync(0xffffffffu, high ? v[1] : v[3], 16);
+        x = (odd ? b : a) + __shfl_xor_sync(0xffffffffu, odd ? a : b, 8);
+    } else if constexpr (K == 2) {
+        const bool high = lane & 16;
+        x = (high ? v[1] : v[0]) + __shfl_xor_sync(0xffffffffu, high ? v[0] : v[1], 16);
+    } else {
+        x = v[0];
+    }
+#pragma unroll
+    for (int o = 16 / K; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+    return x;
+}
+
+using Places = float[2][4][32];  // sums of up to 32 warps, zeros where there are fewer
+
+__device__ __forceinline__ void clear_places(Places &places) {
+    if (threadIdx.x < 32)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) places[i >> 2][i & 3][threadIdx.x] = 0.f;
+}
+
 template <bool WARP>
 struct Rounds {
-    float (*places)[4][kMostThreads / 32];
+    Places &places;
     int turn;
     template <int K>
     __device__ __forceinline__ void sums(float (&v)[K]) {
+        constexpr int L = 32 / K;  // lanes to a sum
+        float x = packed_sum(v);
+        const int lane = threadIdx.x & 31;
+        if (!WARP) {
+            if (lane % L == 0) places[turn][lane / L][threadIdx.x >> 5] = x;
+            __syncthreads();
+            x = 0.f;
 #pragma unroll
-        for (int k = 0; k < K; ++k)
+            for (int q = 0; q < kMostThreads / 32; q += L) x += places[turn][lane / L][q + lane % L];
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
-        if (WARP) return;
-        const int warps = blockDim.x >> 5;
-        if ((threadIdx.x & 31) == 0)
-#pragma unroll
-            for (int k = 0; k < K; ++k) places[turn][k][threadIdx.x >> 5] = v[k];
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < K; ++k) {
-            float t = 0.f;
-            for (int q = 0; q < warps; ++q) t += places[turn][k][q];
-            v[k] = t;
+            for (int o = (L < 16 ? L : 16) / 2; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+            turn ^= 1;
         }
-        turn ^= 1;
+#pragma unroll
+        for (int k = 0; k < K; ++k) v[k] = __shfl_sync(0xffffffffu, x, k * L);
     }
 };
 
 template <int N, bool VEC, bool WARP, bool LAYER>
 __global__ void __launch_bounds__(kMostThreads) norm_fwd_kernel(const __grid_constant__ Forward p) {
-    __shared__ float places[2][4][kMostThreads / 32];
+    __shared__ Places places;
     launch_next();
+    if (!WARP) {
+        clear_places(places);
+        __syncthreads();
+    }
     launch_wait();
     Rounds<WARP> rounds = {places, 0};
     const int T = WARP ? 32 : blockDim.x, t = WARP ? threadIdx.x & 31 : threadIdx.x;
@@ -245,16 +280,19 @@ __device__ __forceinline__ void rows_of_block(const Backward &p, unsigned block,
 // behind its own copies.
 constexpr int kValues = 8;
 
+// What a kernel adds up: without biases a row takes fewer instructions and registers.
+enum Sums { RMS, RMS_BIAS, LAYER_BIAS };
+
 struct Slab {
     int width, arrays, stages;  // columns to a block; arrays of the ring and its depth in rows
 };
 
-template <bool LAYER, bool RING, bool CLUSTER>
+template <Sums MODE, bool RING, bool CLUSTER>
 __global__ void __launch_bounds__(kMostThreads) norm_bwd_kernel(const __grid_constant__ Backward p, const __grid_constant__ Slab slab) {
-    constexpr bool VEC = RING;
+    constexpr bool VEC = RING, LAYER = MODE == LAYER_BIAS, BIAS = MODE != RMS;
     constexpr int N = kValues;
     extern __shared__ __align__(128) float ring[];
-    __shared__ float places[2][4][kMostThreads / 32];
+    __shared__ Places places;
     __shared__ float shared_sums[2][4];  // CLUSTER: this block's sums of a round
     __shared__ uint64_t full[8];
     const int T = blockDim.x, t = threadIdx.x;
@@ -265,6 +303,7 @@ __global__ void __launch_bounds__(kMostThreads) norm_bwd_kernel(const __grid_con
         for (int s = 0; s < slab.stages; ++s) mbar_init(&full[s], 1);
         mbar_init_fence();
     }
+    clear_places(places);
     __syncthreads();
     launch_wait();
 
@@ -362,7 +401,7 @@ __global__ void __launch_bounds__(kMostThreads) norm_bwd_kernel(const __grid_con
             v[0] += r[i] * r[i];
             v[1] += h[i] * h[i];
             v[2] += a[i] * r[i];
-            v[3] += a[i];
+            if (LAYER) v[3] += a[i];
         }
         round(v);
         if (RING && t == 0 && row + slab.stages < end) fetch(row + slab.stages);
@@ -374,24 +413,24 @@ __global__ void __launch_bounds__(kMostThreads) norm_bwd_kernel(const __grid_con
                 const float hat = r[i] * rs;
                 dr[i] += rs * (a[i] - hat * c_hat - c_one);  // all of r's gradient from here on
                 sum_pre_w[i] += dn[i] * hat;
-                sum_pre_b[i] += dn[i];
+                if (BIAS) sum_pre_b[i] += dn[i];
             }
         if (p.dx) store_row<N, VEC>(dr, p.dx + at, t, T, width, p.add_dx);
         if (!p.h) continue;
-        float q[2] = {0.f, 0.f}, b[N];  // b h^ and b behind the block
+        float q[LAYER ? 2 : 1] = {}, b[N];  // b h^ and b behind the block
         if (p.post_w) {
             load_row<N, VEC>(w, p.post_w + c0, t, T, width);
             float bias[N] = {};
-            if (p.post_b && (p.dgate || p.partial[DGATE])) load_row<N, VEC>(bias, p.post_b + c0, t, T, width);
+            if (BIAS && p.post_b && (p.dgate || p.partial[DGATE])) load_row<N, VEC>(bias, p.post_b + c0, t, T, width);
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 const float sd = p.scale * dr[i], du = p.gate ? gate[i] * sd : sd;
                 h[i] *= hs;
                 b[i] = in_row<VEC>(i, t, T, width) ? du * w[i] : 0.f;
                 q[0] += b[i] * h[i];
-                q[1] += b[i];
+                if constexpr (LAYER) q[1] += b[i];
                 sum_post_w[i] += du * h[i];
-                sum_post_b[i] += du;
+                if (BIAS) sum_post_b[i] += du;
                 dr[i] = sd * (h[i] * w[i] + bias[i]);  // the gate's
             }
         } else {
@@ -416,7 +455,9 @@ __global__ void __launch_bounds__(kMostThreads) norm_bwd_kernel(const __grid_con
         if (!p.dh) continue;
         if (p.post_w) {
             round(q);
-            const float q_hat = q[0] * inv, q_one = LAYER ? q[1] * inv : 0.f;
+            float q_one = 0.f;
+            if constexpr (LAYER) q_one = q[1] * inv;
+            const float q_hat = q[0] * inv;
 #pragma unroll
             for (int i = 0; i < N; ++i) b[i] = hs * (b[i] - h[i] * q_hat - q_one);
         }
@@ -424,9 +465,9 @@ __global__ void __launch_bounds__(kMostThreads) norm_bwd_kernel(const __grid_con
     }
     const size_t mine = size_t(block) * p.cols + c0;
     if (p.partial[DPRE_W]) store_row<N, VEC>(sum_pre_w, p.partial[DPRE_W] + mine, t, T, width, false);
-    if (p.partial[DPRE_B]) store_row<N, VEC>(sum_pre_b, p.partial[DPRE_B] + mine, t, T, width, false);
+    if (BIAS && p.partial[DPRE_B]) store_row<N, VEC>(sum_pre_b, p.partial[DPRE_B] + mine, t, T, width, false);
     if (p.partial[DPOST_W]) store_row<N, VEC>(sum_post_w, p.partial[DPOST_W] + mine, t, T, width, false);
-    if (p.partial[DPOST_B]) store_row<N, VEC>(sum_post_b, p.partial[DPOST_B] + mine, t, T, width, false);
+    if (BIAS && p.partial[DPOST_B]) store_row<N, VEC>(sum_post_b, p.partial[DPOST_B] + mine, t, T, width, false);
     if (p.partial[DGATE]) store_row<N, VEC>(sum_gate, p.partial[DGATE] + mine, t, T, width, false);
     if (CLUSTER) cluster_sync_all();  // no block leaves while another may read its sums
 }
@@ -589,8 +630,10 @@ struct Folds {
     int cols, folds;
 };
 
-__global__ void __launch_bounds__(kThreads) norm_fold_kernel(const __grid_constant__ Folds p) {
-    __shared__ float sh[8][33];
+constexpr int kFoldThreads = 1024;  // 32 columns by 32 parts at a time: one round of loads for 300 blocks' sums
+
+__global__ void __launch_bounds__(kFoldThreads) norm_fold_kernel(const __grid_constant__ Folds p) {
+    __shared__ float sh[32][33];
     launch_next();
     launch_wait();
     const int lane = threadIdx.x & 31, part = threadIdx.x >> 5;
@@ -604,15 +647,17 @@ __global__ void __launch_bounds__(kThreads) norm_fold_kernel(const __grid_consta
             const float *src = f.partial + result * f.parts * p.cols;
             float s = 0.f;
             if (col < p.cols)
-#pragma unroll 8
-                for (int q = part; q < f.parts; q += 8) s += __ldcg(src + size_t(q) * p.cols + col);
+#pragma unroll 10
+                for (int q = part; q < f.parts; q += 32) s += __ldcg(src + size_t(q) * p.cols + col);
             sh[part][lane] = s;
             __syncthreads();
-            if (part == 0 && col < p.cols) {
-                float t = 0.f;
+            // warp `part` adds up column `part` of the tile
+            float t = sh[lane][part];
 #pragma unroll
-                for (int q = 0; q < 8; ++q) t += sh[q][lane];
-                float *o = f.out + result * p.cols + col;
+            for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+            const int mine = int(item - result * tiles) * 32 + part;
+            if (lane == 0 && mine < p.cols) {
+                float *o = f.out + result * p.cols + mine;
                 *o = f.add ? *o + t : t;
             }
             __syncthreads();
@@ -684,13 +729,20 @@ BackwardShape backward_shape(const katsu_cuda_ctx *ctx, const Backward &p, std::
     return s;
 }
 
+template <Sums MODE>
+int32_t start_backward_of(katsu_cuda_ctx *ctx, const Backward &p, const BackwardShape &s, size_t blocks) {
+    auto kernel = s.cluster > 1 ? norm_bwd_kernel<MODE, true, true>
+                  : s.slab.arrays ? norm_bwd_kernel<MODE, true, false> : norm_bwd_kernel<MODE, false, false>;
+    KATSU_TRY(katsu_prepare_kernel(ctx, (const void *)kernel, s.smem));
+    return katsu_launch_chained(ctx, kernel, (unsigned)blocks * s.cluster, s.threads, s.smem, s.cluster, p, s.slab);
+}
+
 template <bool LAYER>
 int32_t start_backward(katsu_cuda_ctx *ctx, const Backward &p, const BackwardShape &s, size_t blocks) {
     if (s.slab.width == 0) return start(ctx, norm_bwd_long_kernel<LAYER>, (unsigned)blocks, kThreads, p);
-    auto kernel = s.cluster > 1 ? norm_bwd_kernel<LAYER, true, true>
-                  : s.slab.arrays ? norm_bwd_kernel<LAYER, true, false> : norm_bwd_kernel<LAYER, false, false>;
-    KATSU_TRY(katsu_prepare_kernel(ctx, (const void *)kernel, s.smem));
-    return katsu_launch_chained(ctx, kernel, (unsigned)blocks * s.cluster, s.threads, s.smem, s.cluster, p, s.slab);
+    const bool bias = p.post_b || p.partial[DPRE_B] || p.partial[DPOST_B];
+    return LAYER ? start_backward_of<LAYER_BIAS>(ctx, p, s, blocks)
+                 : bias ? start_backward_of<RMS_BIAS>(ctx, p, s, blocks) : start_backward_of<RMS>(ctx, p, s, blocks);
 }
 
 int32_t check_sizes(size_t rows, size_t cols, const float *gate, size_t gate_rows, int32_t kind, float eps) {
@@ -771,7 +823,7 @@ extern "C" int32_t katsu_cuda_block_norm_bwd(katsu_cuda_ctx *ctx, const float *r
     const size_t want = shape.most_blocks < rows ? shape.most_blocks : rows;
     size_t blocks;
     if (p.gate_of_row || dgate == nullptr || p.groups < want) {
-        p.slices = (int)katsu_div_up(want, p.groups);
+        p.slices = (int)(want / p.groups);  // (a block more than go round at once would double the time)
         const size_t length = rows / p.groups;
         if ((size_t)p.slices > length) p.slices = (int)length;
         blocks = p.groups * p.slices;
@@ -799,6 +851,6 @@ extern "C" int32_t katsu_cuda_block_norm_bwd(katsu_cuda_ctx *ctx, const float *r
     if (folds.folds == 0) return KATSU_OK;
     unsigned long long items = 0;
     for (int k = 0; k < folds.folds; ++k) items += folds.f[k].results * katsu_div_up(cols, 32);
-    const unsigned long long most = (unsigned long long)ctx->num_sms * 8;
-    return start(ctx, norm_fold_kernel, unsigned(items < most ? items : most), kThreads, folds);
+    const unsigned long long most = (unsigned long long)ctx->num_sms * 2;
+    return start(ctx, norm_fold_kernel, unsigned(items < most ? items : most), kFoldThreads, folds);
 }

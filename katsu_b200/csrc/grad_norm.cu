@@ -21,7 +21,7 @@
 namespace {
 
 constexpr int kThreads = 256;
-constexpr unsigned kChunk = 8192;  // values a block takes at a time: eight 16-byte loads a thread
+constexpr unsigned kChunk = 4096;  // values a block takes at a time: four 16-byte loads a thread
 constexpr int kMaxTensors = 512;   // a launch (14 KiB of parameters)
 constexpr int kFewTensors = 32;    // (1 KiB: the launch of a large parameter block takes longer)
 
@@ -145,32 +145,29 @@ __global__ void __launch_bounds__(kThreads) apply_kernel(const __grid_constant__
         const float *sb = src - lead;
         float *db = dst - lead;
         if (lead_of(dst) == lead) {
+            constexpr int loads = kChunk / 4 / kThreads;
+            float4 g[loads], w[loads];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                constexpr int half = kChunk / 8 / kThreads;
-                float4 g[half], w[half];
-#pragma unroll
-                for (int j = 0; j < half; ++j) {
-                    const unsigned long long a = begin + 4ull * (threadIdx.x + (h * half + j) * kThreads);
-                    if (a >= lead && a + 4 <= end) {
-                        g[j] = *reinterpret_cast<const float4 *>(sb + a);
-                        if (OP == STEP) w[j] = *reinterpret_cast<const float4 *>(db + a);
-                    }
+            for (int j = 0; j < loads; ++j) {
+                const unsigned long long a = begin + 4ull * (threadIdx.x + j * kThreads);
+                if (a >= lead && a + 4 <= end) {
+                    g[j] = *reinterpret_cast<const float4 *>(sb + a);
+                    if (OP == STEP) w[j] = *reinterpret_cast<const float4 *>(db + a);
                 }
+            }
 #pragma unroll
-                for (int j = 0; j < half; ++j) {
-                    const unsigned long long a = begin + 4ull * (threadIdx.x + (h * half + j) * kThreads);
-                    if (a >= lead && a + 4 <= end) {
-                        float4 o;
-                        o.x = applied<OP>(g[j].x, OP == STEP ? w[j].x : 0.f, c, lr);
-                        o.y = applied<OP>(g[j].y, OP == STEP ? w[j].y : 0.f, c, lr);
-                        o.z = applied<OP>(g[j].z, OP == STEP ? w[j].z : 0.f, c, lr);
-                        o.w = applied<OP>(g[j].w, OP == STEP ? w[j].w : 0.f, c, lr);
-                        *reinterpret_cast<float4 *>(db + a) = o;
-                    } else {
-                        for (unsigned long long b = a; b < a + 4; ++b)
-                            if (b >= lead && b < end) db[b] = applied<OP>(sb[b], OP == STEP ? db[b] : 0.f, c, lr);
-                    }
+            for (int j = 0; j < loads; ++j) {
+                const unsigned long long a = begin + 4ull * (threadIdx.x + j * kThreads);
+                if (a >= lead && a + 4 <= end) {
+                    float4 o;
+                    o.x = applied<OP>(g[j].x, OP == STEP ? w[j].x : 0.f, c, lr);
+                    o.y = applied<OP>(g[j].y, OP == STEP ? w[j].y : 0.f, c, lr);
+                    o.z = applied<OP>(g[j].z, OP == STEP ? w[j].z : 0.f, c, lr);
+                    o.w = applied<OP>(g[j].w, OP == STEP ? w[j].w : 0.f, c, lr);
+                    *reinterpret_cast<float4 *>(db + a) = o;
+                } else {
+                    for (unsigned long long b = a; b < a + 4; ++b)
+                        if (b >= lead && b < end) db[b] = applied<OP>(sb[b], OP == STEP ? db[b] : 0.f, c, lr);
                 }
             }
         } else {

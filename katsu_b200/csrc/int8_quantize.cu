@@ -1,7 +1,8 @@
 // Matrices to 8 bits: rows of x (one scale a token) and columns of w (one scale an output channel, kept transposed).
 //
-// Rows: a warp (up to 1024 values) or a block takes a row, holds its first 8192 values in registers between the largest
-// magnitude and the quotients and reads the rest again.  Bound: HBM, 4 bytes in and 1 out a value.
+// Rows: a warp (up to 1024 values), or a block of 256 (up to 8192) or 512 threads takes a row, holds its first 32 values a
+// thread in registers between the largest magnitude and the quotients and reads the rest again, from L2.  Bound: HBM, 4 bytes
+// in and 1 out a value.
 #include "int8.cuh"
 
 namespace {
@@ -20,41 +21,45 @@ __device__ __forceinline__ void load4(const float *row, size_t j, size_t k, floa
     }
 }
 
-__device__ __forceinline__ unsigned largest4(const float (&v)[4]) {
-    return max(max(katsu_magnitude(v[0]), katsu_magnitude(v[1])), max(katsu_magnitude(v[2]), katsu_magnitude(v[3])));
-}
-
 template <int T, bool VEC>
-__global__ void __launch_bounds__(256) quantize_rows_kernel(const float *__restrict__ x, int8_t *q, float *scale,
-                                                            unsigned long long rows, size_t k, size_t pitch) {
-    __shared__ unsigned sh[2][8];
+__global__ void __launch_bounds__(T < 256 ? 256 : T, T < 256 ? 4 : 1024 / T) quantize_rows_kernel(const float *__restrict__ x, int8_t *q, float *scale,
+                                                                               unsigned long long rows, size_t k, size_t pitch) {
+    __shared__ float sh[2][32];
     launch_next();
     launch_wait();
-    constexpr int per_block = 256 / T;
+    constexpr int per_block = T < 256 ? 256 / T : 1;
     const int t = threadIdx.x % T;
     int turn = 0;
     for (unsigned long long row = (unsigned long long)blockIdx.x * per_block + threadIdx.x / T; row < rows;
          row += (unsigned long long)gridDim.x * per_block, turn ^= 1) {
         const float *src = x + row * k;
         float v[kHeld][4];
-        unsigned most = 0;
+        float most = 0.f;
 #pragma unroll
-        for (int i = 0; i < kHeld; ++i) load4<VEC>(src, 4 * size_t(t + i * T), k, v[i]);
-#pragma unroll
-        for (int i = 0; i < kHeld; ++i) most = max(most, largest4(v[i]));
-        for (size_t j = 4 * size_t(t + kHeld * T); j < k; j += 4 * T) {
-            float w[4];
-            load4<VEC>(src, j, k, w);
-            most = max(most, largest4(w));
+        for (int i = 0; i < kHeld; ++i) {
+            if (size_t(4 * T) * i >= k) break;
+            load4<VEC>(src, 4 * size_t(t + i * T), k, v[i]);
         }
-        most = __reduce_max_sync(0xffffffffu, most);
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) {
+            if (size_t(4 * T) * i >= k) break;
+            most = katsu_larger4(most, v[i]);
+        }
+        for (size_t j = 4 * size_t(kHeld * T); j < k; j += 4 * kHeld * T) {
+            float w[kHeld][4];
+#pragma unroll
+            for (int i = 0; i < kHeld; ++i) load4<VEC>(src, j + 4 * size_t(t + i * T), k, w[i]);
+#pragma unroll
+            for (int i = 0; i < kHeld; ++i) most = katsu_larger4(most, w[i]);
+        }
+        most = katsu_larger_of_warp(most);
         if (T > 32) {  // (two sets of places: the row behind this one does not wait for its readers)
             if ((threadIdx.x & 31) == 0) sh[turn][threadIdx.x >> 5] = most;
             __syncthreads();
 #pragma unroll
-            for (int w = 0; w < 8; ++w) most = max(most, sh[turn][w]);
+            for (int w = 0; w < T / 32; ++w) most = katsu_larger(most, sh[turn][w]);
         }
-        const KatsuInt8Scale s = katsu_int8_scale(__uint_as_float(most));
+        const KatsuInt8Scale s = katsu_int8_scale(most);
         if (t == 0) scale[row] = s.scale;
         unsigned *dst = reinterpret_cast<unsigned *>(q + row * pitch);
 #pragma unroll
@@ -62,32 +67,35 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const float *__restr
             const size_t j = 4 * size_t(t + i * T);
             if (j < pitch) dst[j / 4] = katsu_int8_pack(v[i], s);
         }
-        for (size_t j = 4 * size_t(t + kHeld * T); j < pitch; j += 4 * T) {
-            float w[4];
-            load4<VEC>(src, j, k, w);
-            dst[j / 4] = katsu_int8_pack(w, s);
+        for (size_t j = 4 * size_t(kHeld * T); j < pitch; j += 4 * kHeld * T) {
+            float w[kHeld][4];
+#pragma unroll
+            for (int i = 0; i < kHeld; ++i) load4<VEC>(src, j + 4 * size_t(t + i * T), k, w[i]);
+#pragma unroll
+            for (int i = 0; i < kHeld; ++i)
+                if (j + 4 * size_t(t + i * T) < pitch) dst[(j + 4 * size_t(t + i * T)) / 4] = katsu_int8_pack(w[i], s);
         }
     }
 }
 
 // Largest magnitude of every column of w [k, n], as bits, over k rows cut into gridDim.y pieces; `most` starts at zero.
 // (The largest of a set does not depend on the order of the atomics.)
-__global__ void __launch_bounds__(256) column_largest_kernel(const float *__restrict__ w, unsigned *most, size_t k, size_t n) {
+__global__ void __launch_bounds__(256) column_largest_kernel(const float *__restrict__ w, unsigned *most_of, size_t k, size_t n) {
     launch_next();
     launch_wait();
     const size_t col = size_t(blockIdx.x) * 32 + (threadIdx.x & 31);
     const size_t begin = k * blockIdx.y / gridDim.y, end = k * (blockIdx.y + 1) / gridDim.y;
-    unsigned m = 0;
+    float m = 0.f;
     if (col < n)
 #pragma unroll 8
-        for (size_t p = begin + (threadIdx.x >> 5); p < end; p += 8) m = max(m, katsu_magnitude(__ldg(w + p * n + col)));
-    __shared__ unsigned sh[8][33];
+        for (size_t p = begin + (threadIdx.x >> 5); p < end; p += 8) m = katsu_larger(m, __ldg(w + p * n + col));
+    __shared__ float sh[8][33];
     sh[threadIdx.x >> 5][threadIdx.x & 31] = m;
     __syncthreads();
     if (threadIdx.x < 32 && col < n) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) m = max(m, sh[i][threadIdx.x]);
-        atomicMax(most + col, m);
+        for (int i = 0; i < 8; ++i) m = katsu_larger(m, sh[i][threadIdx.x]);
+        atomicMax(most_of + col, __float_as_uint(m));
     }
 }
 
@@ -123,13 +131,14 @@ __global__ void __launch_bounds__(256) quantize_columns_kernel(const float *__re
 
 int32_t katsu_int8_quantize(katsu_cuda_ctx *ctx, const float *x, int8_t *q, float *scale, size_t m, size_t k) {
     const bool vec = k % 4 == 0 && (reinterpret_cast<uintptr_t>(x) & 15u) == 0;
-    // A row of up to 1024 values is one warp's: eight rows to a block, and no barrier between the largest and the quotients.
-    const bool small = k <= 32 * 4 * kHeld;
-    const size_t need = small ? katsu_div_up(m, 8) : m, most = size_t(ctx->num_sms) * 8;
+    const bool small = k <= 32 * 4 * kHeld, long_rows = k > 256 * 4 * kHeld;
+    const unsigned threads = long_rows ? 512 : 256;
+    const size_t need = small ? katsu_div_up(m, 8) : m, most = size_t(ctx->num_sms) * (2048 / threads);
     auto kernel = small ? (vec ? quantize_rows_kernel<32, true> : quantize_rows_kernel<32, false>)
-                        : (vec ? quantize_rows_kernel<256, true> : quantize_rows_kernel<256, false>);
+                  : long_rows ? (vec ? quantize_rows_kernel<512, true> : quantize_rows_kernel<512, false>)
+                              : (vec ? quantize_rows_kernel<256, true> : quantize_rows_kernel<256, false>);
     KATSU_TRY(katsu_prepare_kernel(ctx, (const void *)kernel, 0));
-    return katsu_launch_chained(ctx, kernel, (unsigned)(need < most ? need : most), 256, 0, 1, x, q, scale, m, k,
+    return katsu_launch_chained(ctx, kernel, (unsigned)(need < most ? need : most), threads, 0, 1, x, q, scale, m, k,
                                 katsu_int8_pitch(k));
 }
 

@@ -16,12 +16,26 @@ __global__ void __launch_bounds__(kWarps * 32) int8_rows_kernel(const float *__r
                                                                 const float *__restrict__ ws, const float *bias, float *y,
                                                                 int m, int k, int n, int pitch, int share) {
     extern __shared__ __align__(16) unsigned char tokens[];  // [M][pitch]
-    __shared__ unsigned largest[M][kWarps];
+    __shared__ float largest[M][kWarps];
     __shared__ float scales[M];
     __shared__ int sums[kWarps][kRows * M];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     launch_next();
     launch_wait();
+    const int pairs = (n + kRows - 1) / kRows, per_block = kWarps / share, part = warp % share;
+    const int units = pitch / 16, begin = int((long long)units * part / share), end = int((long long)units * (part + 1) / share);
+    // 16 bytes a lane of the pair's rows, kUnroll times: all on their way before the first is used
+    int4 v[kUnroll][kRows];
+    auto fetch = [&](int pair, int u0) {
+#pragma unroll
+        for (int r = 0; r < kRows; ++r) {
+            const int4 *w = reinterpret_cast<const int4 *>(wq + size_t(min(pair * kRows + r, n - 1)) * pitch);
+#pragma unroll
+            for (int q = 0; q < kUnroll; ++q)
+                v[q][r] = pair < pairs && u0 + 32 * q < end ? __ldg(w + u0 + 32 * q) : make_int4(0, 0, 0, 0);
+        }
+    };
+    fetch(blockIdx.x * per_block + warp / share, begin + lane);  // the first ones while the tokens are quantised
     // ---- the tokens ----
     if (x != nullptr) {
         const bool vec = (k & 3) == 0 && (reinterpret_cast<uintptr_t>(x) & 15u) == 0;
@@ -37,25 +51,24 @@ __global__ void __launch_bounds__(kWarps * 32) int8_rows_kernel(const float *__r
         };
 #pragma unroll
         for (int i = 0; i < M; ++i) {
-            unsigned most = 0;
+            float most = 0.f;
             if (i < m)
 #pragma unroll 4
                 for (int j = 4 * threadIdx.x; j < pitch; j += 4 * kWarps * 32) {
                     float v[4];
                     load4(i, j, v);
-                    most = max(most, max(max(katsu_magnitude(v[0]), katsu_magnitude(v[1])),
-                                         max(katsu_magnitude(v[2]), katsu_magnitude(v[3]))));
+                    most = katsu_larger4(most, v);
                 }
-            most = __reduce_max_sync(0xffffffffu, most);
+            most = katsu_larger_of_warp(most);
             if (lane == 0) largest[i][warp] = most;
         }
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < M; ++i) {
-            unsigned most = 0;
+            float most = 0.f;
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) most = max(most, largest[i][w]);
-            const KatsuInt8Scale s = katsu_int8_scale(__uint_as_float(most));
+            for (int w = 0; w < kWarps; ++w) most = katsu_larger(most, largest[i][w]);
+            const KatsuInt8Scale s = katsu_int8_scale(most);
             if (threadIdx.x == 0) scales[i] = s.scale;
 #pragma unroll 4
             for (int j = 4 * threadIdx.x; j < pitch; j += 4 * kWarps * 32) {
@@ -72,22 +85,13 @@ __global__ void __launch_bounds__(kWarps * 32) int8_rows_kernel(const float *__r
     }
     __syncthreads();
     // ---- the weights ----
-    const int pairs = (n + kRows - 1) / kRows, per_block = kWarps / share, part = warp % share;
-    const int units = pitch / 16, begin = int((long long)units * part / share), end = int((long long)units * (part + 1) / share);
-    for (int first = blockIdx.x * per_block; first < pairs; first += gridDim.x * per_block) {
+    bool fetched = true;
+    for (int first = blockIdx.x * per_block; first < pairs; first += gridDim.x * per_block, fetched = false) {
         const int pair = first + warp / share;
         int acc[kRows][M] = {};
         if (pair < pairs) {
-            const int4 *w[kRows];
-#pragma unroll
-            for (int r = 0; r < kRows; ++r) w[r] = reinterpret_cast<const int4 *>(wq + size_t(min(pair * kRows + r, n - 1)) * pitch);
-            for (int u0 = begin + lane; u0 < end; u0 += 32 * kUnroll) {
-                int4 v[kUnroll][kRows];
-#pragma unroll
-                for (int q = 0; q < kUnroll; ++q)
-#pragma unroll
-                    for (int r = 0; r < kRows; ++r)
-                        v[q][r] = u0 + 32 * q < end ? __ldg(w[r] + u0 + 32 * q) : make_int4(0, 0, 0, 0);
+            for (int u0 = begin + lane; u0 - lane < end; u0 += 32 * kUnroll, fetched = false) {
+                if (!fetched) fetch(pair, u0);
 #pragma unroll
                 for (int q = 0; q < kUnroll; ++q) {
                     if (u0 + 32 * q >= end) break;

@@ -34,6 +34,7 @@ struct Forward {
     float scale, eps;
     unsigned long long rows, rows_per_gate;
     int cols;
+    int *status;
 };
 
 // Sums over rows, in the order of the partial results.
@@ -77,49 +78,103 @@ __device__ __forceinline__ void block_sums(float (&v)[K], float (*sh)[32]) {
 }
 
 // ---- rows that a block holds ------------------------------------------------------------------------------------------
-// N values of a row for each of T threads: pieces of four, T pieces apart (VEC: 16-byte accesses, the row's pieces are whole), or
-// single values T apart.  `width` values from `at` on; what lies behind them is 0 and not stored.
+// N values of a row for each of T threads, in pieces of four (VEC: 16-byte accesses; the row is whole pieces at 16-byte
+// addresses) or one, the pieces of a thread T pieces apart.  The pieces that lie in the row are a thread's first `live` ones;
+// the others are loaded as zeros and not stored.
 template <int N, bool VEC>
-__device__ __forceinline__ void load_row(float (&v)[N], const float *at, int t, int T, int width) {
-#pragma unroll
-    for (int i = 0; i < N; i += VEC ? 4 : 1) {
-        if (VEC) {
-            const int j = 4 * (t + i / 4 * T);
-            const float4 f = j < width ? *reinterpret_cast<const float4 *>(at + j) : make_float4(0.f, 0.f, 0.f, 0.f);
-            v[i] = f.x; v[i + 1] = f.y; v[i + 2] = f.z; v[i + 3] = f.w;
-        } else {
-            const int j = t + i * T;
-            v[i] = j < width ? at[j] : 0.f;
-        }
+struct Row {
+    static constexpr int W = VEC ? 4 : 1, P = N / W;
+    int t, T, live;
+    __device__ __forceinline__ Row(int t, int T, int width) : t(t), T(T) {
+        const int last = (width + W - 1) / W - 1 - t;  // pieces behind this thread's first one
+        live = last < 0 ? 0 : last / T + 1;
     }
-}
-
-template <int N, bool VEC>
-__device__ __forceinline__ void store_row(const float (&v)[N], float *at, int t, int T, int width, bool add) {
+    template <typename F>
+    __device__ __forceinline__ void each(F f) const {
 #pragma unroll
-    for (int i = 0; i < N; i += VEC ? 4 : 1) {
-        if (VEC) {
-            const int j = 4 * (t + i / 4 * T);
-            if (j >= width) break;
-            float4 f = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-            if (add) {
-                const float4 old = *reinterpret_cast<const float4 *>(at + j);
-                f.x += old.x; f.y += old.y; f.z += old.z; f.w += old.w;
+        for (int i = 0; i < N; ++i) f(i);
+    }
+    // Takes a row's mean off, behind whose end zeros stay.
+    __device__ __forceinline__ void center(float (&v)[N], float mean) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = i / W < live ? v[i] - mean : 0.f;
+    }
+    __device__ __forceinline__ void load(float (&v)[N], const float *at) const {
+        at += W * t;
+#pragma unroll
+        for (int q = 0; q < P; ++q, at += W * T)
+            if constexpr (VEC) {
+                const float4 f = q < live ? *reinterpret_cast<const float4 *>(at) : make_float4(0.f, 0.f, 0.f, 0.f);
+                v[4 * q] = f.x; v[4 * q + 1] = f.y; v[4 * q + 2] = f.z; v[4 * q + 3] = f.w;
+            } else {
+                v[q] = q < live ? *at : 0.f;
             }
-            *reinterpret_cast<float4 *>(at + j) = f;
-        } else {
-            const int j = t + i * T;
-            if (j >= width) break;
-            at[j] = add ? at[j] + v[i] : v[i];
+    }
+    __device__ __forceinline__ void store(const float (&v)[N], float *at, bool add) const {
+        at += W * t;
+#pragma unroll
+        for (int q = 0; q < P; ++q, at += W * T)
+            if (q < live) {
+                if constexpr (VEC) {
+                    float4 f = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+                    if (add) {
+                        const float4 old = *reinterpret_cast<const float4 *>(at);
+                        f.x += old.x; f.y += old.y; f.z += old.z; f.w += old.w;
+                    }
+                    *reinterpret_cast<float4 *>(at) = f;
+                } else {
+                    *at = add ? *at + v[q] : v[q];
+                }
+            }
+    }
+};
+
+// Rows brought to shared memory ahead of their use: `arrays` arrays of `width` columns a row, `stages` rows.
+struct Slab {
+    int width, arrays, stages;
+};
+
+struct Ring {
+    float *data;
+    uint64_t *full;
+    Slab slab;
+    int stage, phase;  // of the row that is read next
+    __device__ __forceinline__ void init(float *at, uint64_t *bars, const Slab &s) {
+        data = at;
+        full = bars;
+        slab = s;
+        stage = phase = 0;
+        if (threadIdx.x == 0) {
+            for (int i = 0; i < s.stages; ++i) mbar_init(&full[i], 1);
+            mbar_init_fence();
         }
     }
-}
+    __device__ __forceinline__ const float *next(int *status) const {  // waits for the next row
+        // (a wait that gives up leaves wrong values behind, which the next synchronising call reports)
+        mbar_wait_warp_ready(&full[stage], phase, status, 191);
+        return data + size_t(stage) * slab.arrays * slab.width;
+    }
+    __device__ __forceinline__ void advance() {
+        if (++stage == slab.stages) {
+            stage = 0;
+            phase ^= 1;
+        }
+    }
+    // By one thread: copies `width` columns of every array that there is, from `at` values behind its start, to a stage.
+    __device__ __forceinline__ void fetch(int to_stage, std::initializer_list<const float *> arrays, size_t at, int width) const {
+        const uint32_t bytes = uint32_t(width) * 4;
+        float *to = data + size_t(to_stage) * slab.arrays * slab.width;
+        mbar_arrive_expect_tx(&full[to_stage], bytes * slab.arrays);
+        for (const float *src : arrays)
+            if (src) {
+                bulk_load(to, src + at, bytes, &full[to_stage]);
+                to += slab.width;
+            }
+    }
+};
 
-// Whether value i of this thread is one of the row's.
-template <bool VEC>
-__device__ __forceinline__ bool in_row(int i, int t, int T, int width) {
-    return (VEC ? 4 * (t + i / 4 * T) : t + i * T) < width;
-}
+constexpr int kMostStages = 8;
+constexpr size_t kRoom = size_t(222) * 1024;  // shared memory of an SM for rings, less 2 KiB a block
 
 constexpr int kMostThreads = 512;
 
@@ -182,80 +237,105 @@ struct Rounds {
     }
 };
 
-template <int N, bool VEC, bool WARP, bool LAYER>
-__global__ void __launch_bounds__(kMostThreads) norm_fwd_kernel(const __grid_constant__ Forward p) {
+// How a row's threads find each other and its values: a warp's own row, a block's by plain loads, a block's by the ring.
+enum Rows { OF_WARP, OF_BLOCK, BY_RING };
+
+template <int N, bool VEC, Rows ROWS, bool LAYER>
+__global__ void __launch_bounds__(kMostThreads) norm_fwd_kernel(const __grid_constant__ Forward p, const __grid_constant__ Slab slab) {
+    constexpr bool WARP = ROWS == OF_WARP, RING = ROWS == BY_RING;
+    extern __shared__ __align__(128) float ring_data[];
     __shared__ Places places;
+    __shared__ uint64_t full[kMostStages];
+    Ring ring;
     launch_next();
+    if (RING) ring.init(ring_data, full, slab);
     if (!WARP) {
         clear_places(places);
         __syncthreads();
     }
     launch_wait();
     Rounds<WARP> rounds = {places, 0};
-    const int T = WARP ? 32 : blockDim.x, t = WARP ? threadIdx.x & 31 : threadIdx.x;
+    const Row<N, VEC> row_of(WARP ? threadIdx.x & 31 : threadIdx.x, WARP ? 32 : blockDim.x, p.cols);
     const unsigned per_block = WARP ? blockDim.x >> 5 : 1;
     const float inv = 1.f / float(p.cols);
-    for (unsigned long long row = (unsigned long long)blockIdx.x * per_block + (WARP ? threadIdx.x >> 5 : 0); row < p.rows;
-         row += (unsigned long long)gridDim.x * per_block) {
+    const bool gate_each = p.gate && p.rows_per_gate == 1;
+    unsigned long long row = (unsigned long long)blockIdx.x * per_block + (WARP ? threadIdx.x >> 5 : 0);
+    const unsigned long long step = (unsigned long long)gridDim.x * per_block;
+    auto fetch = [&](int stage, unsigned long long r) {
+        ring.fetch(stage, {p.x, p.h, gate_each ? p.gate : nullptr}, r * size_t(p.cols), p.cols);
+    };
+    if (RING && threadIdx.x == 0)
+        for (int i = 0; i < slab.stages && row + i * step < p.rows; ++i) fetch(i, row + i * step);
+    for (; row < p.rows; row += step) {
         const size_t at = row * size_t(p.cols);
         float v[N], u[N], w[N];
-        load_row<N, VEC>(v, p.x + at, t, T, p.cols);
+        const float *from = nullptr;
+        bool refill = RING;  // behind the row's first barrier
+        if (RING) from = ring.next(p.status);
+        auto refilled = [&] {
+            if (!RING || !refill) return;
+            refill = false;
+            if (threadIdx.x == 0 && row + slab.stages * step < p.rows) fetch(ring.stage, row + slab.stages * step);
+            ring.advance();
+        };
+        row_of.load(v, RING ? from : p.x + at);
         if (p.h) {
-            load_row<N, VEC>(u, p.h + at, t, T, p.cols);
+            row_of.load(u, RING ? from + slab.width : p.h + at);
             float g[N];
-            if (p.gate) load_row<N, VEC>(g, p.gate + row / p.rows_per_gate * p.cols, t, T, p.cols);
+            if (p.gate)
+                row_of.load(g, RING && gate_each ? from + 2 * slab.width
+                                                 : p.gate + (gate_each ? at : row / p.rows_per_gate * p.cols));
+            if (RING) fence_proxy_async_smem();  // in front of the copies behind the first barrier
             if (p.post_w) {
                 float m[1] = {0.f}, sq[1] = {0.f};
                 if (LAYER) {
-#pragma unroll
-                    for (int i = 0; i < N; ++i) m[0] += u[i];
+                    row_of.each([&](int i) { m[0] += u[i]; });
                     rounds.sums(m);
+                    refilled();
                     m[0] *= inv;
                 }
-#pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    if (LAYER) u[i] = in_row<VEC>(i, t, T, p.cols) ? u[i] - m[0] : 0.f;
-                    sq[0] += u[i] * u[i];
-                }
-                load_row<N, VEC>(w, p.post_w, t, T, p.cols);
+                if (LAYER) row_of.center(u, m[0]);
+                row_of.each([&](int i) { sq[0] += u[i] * u[i]; });
+                row_of.load(w, p.post_w);
                 rounds.sums(sq);
+                refilled();
                 const float rstd = 1.f / sqrtf(sq[0] * inv + p.eps);
-#pragma unroll
-                for (int i = 0; i < N; ++i) u[i] *= rstd * w[i];
+                row_of.each([&](int i) { u[i] *= rstd * w[i]; });
                 if (p.post_b) {
-                    load_row<N, VEC>(w, p.post_b, t, T, p.cols);
-#pragma unroll
-                    for (int i = 0; i < N; ++i) u[i] += w[i];
+                    row_of.load(w, p.post_b);
+                    row_of.each([&](int i) { u[i] += w[i]; });
                 }
             }
-#pragma unroll
-            for (int i = 0; i < N; ++i) v[i] += p.scale * (p.gate ? g[i] * u[i] : u[i]);
-            store_row<N, VEC>(v, p.r + at, t, T, p.cols, false);
+            row_of.each([&](int i) { v[i] += p.scale * (p.gate ? g[i] * u[i] : u[i]); });
+            row_of.store(v, p.r + at, false);
+        } else if (RING) {
+            fence_proxy_async_smem();
         }
-        if (!p.n) continue;
-        float m[1] = {0.f}, sq[1] = {0.f};
-        if (LAYER) {
-#pragma unroll
-            for (int i = 0; i < N; ++i) m[0] += v[i];
-            rounds.sums(m);
-            m[0] *= inv;
+        if (p.n) {
+            float m[1] = {0.f}, sq[1] = {0.f};
+            if (LAYER) {
+                row_of.each([&](int i) { m[0] += v[i]; });
+                rounds.sums(m);
+                refilled();
+                m[0] *= inv;
+            }
+            if (LAYER) row_of.center(v, m[0]);
+            row_of.each([&](int i) { sq[0] += v[i] * v[i]; });
+            row_of.load(w, p.pre_w);
+            rounds.sums(sq);
+            refilled();
+            const float rstd = 1.f / sqrtf(sq[0] * inv + p.eps);
+            row_of.each([&](int i) { v[i] *= rstd * w[i]; });
+            if (p.pre_b) {
+                row_of.load(w, p.pre_b);
+                row_of.each([&](int i) { v[i] += w[i]; });
+            }
+            row_of.store(v, p.n + at, false);
         }
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            if (LAYER) v[i] = in_row<VEC>(i, t, T, p.cols) ? v[i] - m[0] : 0.f;
-            sq[0] += v[i] * v[i];
+        if (RING && refill) {  // no norm, no barrier yet
+            __syncthreads();
+            refilled();
         }
-        load_row<N, VEC>(w, p.pre_w, t, T, p.cols);
-        rounds.sums(sq);
-        const float rstd = 1.f / sqrtf(sq[0] * inv + p.eps);
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] *= rstd * w[i];
-        if (p.pre_b) {
-            load_row<N, VEC>(w, p.pre_b, t, T, p.cols);
-#pragma unroll
-            for (int i = 0; i < N; ++i) v[i] += w[i];
-        }
-        store_row<N, VEC>(v, p.n + at, t, T, p.cols, false);
     }
 }
 
@@ -283,51 +363,36 @@ constexpr int kValues = 8;
 // What a kernel adds up: without biases a row takes fewer instructions and registers.
 enum Sums { RMS, RMS_BIAS, LAYER_BIAS };
 
-struct Slab {
-    int width, arrays, stages;  // columns to a block; arrays of the ring and its depth in rows
-};
-
 template <Sums MODE, bool RING, bool CLUSTER>
 __global__ void __launch_bounds__(kMostThreads) norm_bwd_kernel(const __grid_constant__ Backward p, const __grid_constant__ Slab slab) {
     constexpr bool VEC = RING, LAYER = MODE == LAYER_BIAS, BIAS = MODE != RMS;
     constexpr int N = kValues;
-    extern __shared__ __align__(128) float ring[];
+    extern __shared__ __align__(128) float ring_data[];
     __shared__ Places places;
     __shared__ float shared_sums[2][4];  // CLUSTER: this block's sums of a round
-    __shared__ uint64_t full[8];
-    const int T = blockDim.x, t = threadIdx.x;
-    const unsigned rank = CLUSTER ? cluster_ctarank() : 0, blocks_a_row = CLUSTER ? unsigned(p.cols + slab.width - 1) / unsigned(slab.width) : 1;
+    __shared__ uint64_t full[kMostStages];
+    const unsigned rank = CLUSTER ? cluster_ctarank() : 0;
+    const unsigned blocks_a_row = CLUSTER ? unsigned(p.cols + slab.width - 1) / unsigned(slab.width) : 1;
     const int c0 = int(rank) * slab.width, width = min(slab.width, p.cols - c0);
+    Ring ring;
     launch_next();
-    if (RING && t == 0) {
-        for (int s = 0; s < slab.stages; ++s) mbar_init(&full[s], 1);
-        mbar_init_fence();
-    }
+    if (RING) ring.init(ring_data, full, slab);
     clear_places(places);
     __syncthreads();
     launch_wait();
 
+    const Row<N, VEC> row_of(threadIdx.x, blockDim.x, width);
     const float inv = 1.f / float(p.cols);
     const unsigned block = blockIdx.x / blocks_a_row, blocks = gridDim.x / blocks_a_row;
     const unsigned long long length = p.rows / p.groups;
     unsigned long long begin, end;
     rows_of_block(p, block, blocks, &begin, &end);
     const bool gate_each = p.gate && p.rows_per_gate == 1;
-    // arrays in the ring: r, then those of h, dn, dr and a gate for each row that there are
-    auto fetch = [&](unsigned long long row) {
-        const int s = int((row - begin) % slab.stages);
-        const uint32_t bytes = uint32_t(width) * 4;
-        float *to = ring + size_t(s) * slab.arrays * slab.width;
-        const size_t at = row * size_t(p.cols) + c0;
-        mbar_arrive_expect_tx(&full[s], bytes * slab.arrays);
-        for (const float *src : {p.r, p.h, p.dn, p.dr, gate_each ? p.gate : nullptr})
-            if (src) {
-                bulk_load(to, src + at, bytes, &full[s]);
-                to += slab.width;
-            }
+    auto fetch = [&](int stage, unsigned long long row) {
+        ring.fetch(stage, {p.r, p.h, p.dn, p.dr, gate_each ? p.gate : nullptr}, row * size_t(p.cols) + c0, width);
     };
-    if (RING && t == 0)
-        for (unsigned long long row = begin; row < end && row < begin + slab.stages; ++row) fetch(row);
+    if (RING && threadIdx.x == 0)
+        for (int i = 0; i < slab.stages && begin + i < end; ++i) fetch(i, begin + i);
 
     int turn = 0;
     auto round = [&](auto &v) {  // sums over the row
@@ -335,7 +400,7 @@ __global__ void __launch_bounds__(kMostThreads) norm_bwd_kernel(const __grid_con
         Rounds<false> r = {places, turn};
         r.sums(v);
         if (CLUSTER) {
-            if (t == 0)
+            if (threadIdx.x == 0)
 #pragma unroll
                 for (int k = 0; k < K; ++k) shared_sums[turn][k] = v[k];
             cluster_sync_all();
@@ -349,126 +414,126 @@ __global__ void __launch_bounds__(kMostThreads) norm_bwd_kernel(const __grid_con
         turn ^= 1;
     };
 
-    float gate[N] = {}, sum_gate[N] = {}, sum_pre_w[N] = {}, sum_pre_b[N] = {}, sum_post_w[N] = {}, sum_post_b[N] = {};
-    for (unsigned long long row = begin; row < end; ++row) {
-        const size_t at = row * size_t(p.cols) + c0;
-        float r[N], h[N], dn[N] = {}, dr[N] = {}, w[N];
-        if (RING) {
-            const unsigned long long i = row - begin;
-            const int s = int(i % slab.stages);
-            // (a wait that gives up leaves wrong values behind, which the next synchronising call reports)
-            mbar_wait_warp(&full[s], uint32_t(i / slab.stages) & 1u, p.status, 191);
-            const float *from = ring + size_t(s) * slab.arrays * slab.width;
-            load_row<N, VEC>(r, from, t, T, width);
-            if (p.h) load_row<N, VEC>(h, from += slab.width, t, T, width);
-            if (p.dn) load_row<N, VEC>(dn, from += slab.width, t, T, width);
-            if (p.dr) load_row<N, VEC>(dr, from += slab.width, t, T, width);
-            if (gate_each) load_row<N, VEC>(gate, from += slab.width, t, T, width);
-            fence_proxy_async_smem();  // in front of the copies behind the first round's barrier
-        } else {
-            load_row<N, VEC>(r, p.r + at, t, T, width);
-            if (p.h) load_row<N, VEC>(h, p.h + at, t, T, width);
-            if (p.dn) load_row<N, VEC>(dn, p.dn + at, t, T, width);
-            if (p.dr) load_row<N, VEC>(dr, p.dr + at, t, T, width);
-            if (gate_each) load_row<N, VEC>(gate, p.gate + at, t, T, width);
+    float gate[N], sum_gate[N] = {}, sum_pre_w[N] = {}, sum_pre_b[N] = {}, sum_post_w[N] = {}, sum_post_b[N] = {};
+    // rows until the gate's next row and until the end of the group that dgate is summed over
+    unsigned long long gate_left = 0, group_left = begin < end ? length - begin % length : 0;
+    size_t gate_at = 0;
+    if (p.gate && !gate_each && begin < end) {
+        const unsigned long long q = begin / p.rows_per_gate;
+        gate_left = (q + 1) * p.rows_per_gate - begin;
+        gate_at = q * p.cols + c0;
+        row_of.load(gate, p.gate + gate_at);
+    }
+    size_t at = begin * size_t(p.cols) + c0;
+    for (unsigned long long row = begin; row < end; ++row, at += p.cols) {
+        float r[N], h[N], dn[N], dr[N], w[N];
+        const float *from = RING ? ring.next(p.status) : nullptr;
+        row_of.load(r, RING ? from : p.r + at);
+        if (p.h) row_of.load(h, RING ? from += slab.width : p.h + at);
+        if (p.dn) row_of.load(dn, RING ? from += slab.width : p.dn + at);
+        if (p.dr) row_of.load(dr, RING ? from += slab.width : p.dr + at);
+        if (gate_each) {
+            row_of.load(gate, RING ? from += slab.width : p.gate + at);
+        } else if (p.gate) {
+            if (gate_left == 0) {
+                gate_left = p.rows_per_gate;
+                gate_at += p.cols;
+                row_of.load(gate, p.gate + gate_at);
+            }
+            --gate_left;
         }
-        if (p.gate && !gate_each && (row == begin || row % p.rows_per_gate == 0))
-            load_row<N, VEC>(gate, p.gate + row / p.rows_per_gate * p.cols + c0, t, T, width);
-        if (!p.h)
-#pragma unroll
-            for (int i = 0; i < N; ++i) h[i] = 0.f;
+        if (RING) fence_proxy_async_smem();  // in front of the copies behind the first round's barrier
         if (LAYER) {
             float m[2] = {0.f, 0.f};
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                m[0] += r[i];
-                m[1] += h[i];
-            }
+            row_of.each([&](int i) { m[0] += r[i]; });
+            if (p.post_w) row_of.each([&](int i) { m[1] += h[i]; });
             round(m);
-            const float mr = m[0] * inv, mh = p.post_w ? m[1] * inv : 0.f;
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const bool in = in_row<VEC>(i, t, T, width);
-                r[i] = in ? r[i] - mr : 0.f;
-                h[i] = in ? h[i] - mh : 0.f;
-            }
+            row_of.center(r, m[0] * inv);
+            if (p.post_w) row_of.center(h, m[1] * inv);
         }
         float a[N], v[4] = {0.f, 0.f, 0.f, 0.f};  // squares of r and h, a (r - m) and a
-        if (p.dn) load_row<N, VEC>(w, p.pre_w + c0, t, T, width);
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            a[i] = p.dn ? dn[i] * w[i] : 0.f;
-            v[0] += r[i] * r[i];
-            v[1] += h[i] * h[i];
-            v[2] += a[i] * r[i];
-            if (LAYER) v[3] += a[i];
+        if (p.dn) {
+            row_of.load(w, p.pre_w + c0);
+            row_of.each([&](int i) {
+                a[i] = dn[i] * w[i];
+                v[0] += r[i] * r[i];
+                v[2] += a[i] * r[i];
+                if (LAYER) v[3] += a[i];
+            });
         }
+        if (p.post_w) row_of.each([&](int i) { v[1] += h[i] * h[i]; });
         round(v);
-        if (RING && t == 0 && row + slab.stages < end) fetch(row + slab.stages);
-        const float rs = 1.f / sqrtf(v[0] * inv + p.eps), hs = 1.f / sqrtf(v[1] * inv + p.eps);
-        const float c_hat = v[2] * rs * inv, c_one = LAYER ? v[3] * inv : 0.f;
-        if (p.dn)
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
+        if (RING) {
+            if (threadIdx.x == 0 && row + slab.stages < end) fetch(ring.stage, row + slab.stages);
+            ring.advance();
+        }
+        if (!p.dr) row_of.each([&](int i) { dr[i] = 0.f; });
+        if (p.dn) {
+            const float rs = 1.f / sqrtf(v[0] * inv + p.eps), c_hat = v[2] * rs * inv, c_one = LAYER ? v[3] * inv : 0.f;
+            row_of.each([&](int i) {
                 const float hat = r[i] * rs;
-                dr[i] += rs * (a[i] - hat * c_hat - c_one);  // all of r's gradient from here on
+                dr[i] += rs * (LAYER ? a[i] - hat * c_hat - c_one : a[i] - hat * c_hat);  // all of r's gradient from here on
                 sum_pre_w[i] += dn[i] * hat;
                 if (BIAS) sum_pre_b[i] += dn[i];
-            }
-        if (p.dx) store_row<N, VEC>(dr, p.dx + at, t, T, width, p.add_dx);
+            });
+        }
+        if (p.dx) row_of.store(dr, p.dx + at, p.add_dx);
         if (!p.h) continue;
         float q[LAYER ? 2 : 1] = {}, b[N];  // b h^ and b behind the block
+        const float hs = 1.f / sqrtf(v[1] * inv + p.eps);
+        // gate times gradient; dr turns into the gate's gradient
+        row_of.each([&](int i) {
+            dr[i] *= p.scale;
+            b[i] = p.gate ? gate[i] * dr[i] : dr[i];
+        });
         if (p.post_w) {
-            load_row<N, VEC>(w, p.post_w + c0, t, T, width);
-            float bias[N] = {};
-            if (BIAS && p.post_b && (p.dgate || p.partial[DGATE])) load_row<N, VEC>(bias, p.post_b + c0, t, T, width);
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const float sd = p.scale * dr[i], du = p.gate ? gate[i] * sd : sd;
+            row_of.load(w, p.post_w + c0);
+            row_of.each([&](int i) {
                 h[i] *= hs;
-                b[i] = in_row<VEC>(i, t, T, width) ? du * w[i] : 0.f;
+                sum_post_w[i] += b[i] * h[i];
+                if (BIAS) sum_post_b[i] += b[i];
+                b[i] *= w[i];
                 q[0] += b[i] * h[i];
                 if constexpr (LAYER) q[1] += b[i];
-                sum_post_w[i] += du * h[i];
-                if (BIAS) sum_post_b[i] += du;
-                dr[i] = sd * (h[i] * w[i] + bias[i]);  // the gate's
+            });
+            if (p.gate) {
+                if (BIAS && p.post_b) {
+                    float bias[N];
+                    row_of.load(bias, p.post_b + c0);
+                    row_of.each([&](int i) { dr[i] *= h[i] * w[i] + bias[i]; });
+                } else {
+                    row_of.each([&](int i) { dr[i] *= h[i] * w[i]; });
+                }
             }
         } else {
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const float sd = p.scale * dr[i], u = h[i];
-                b[i] = p.gate ? gate[i] * sd : sd;
-                dr[i] = sd * u;
-            }
+            row_of.each([&](int i) { dr[i] *= h[i]; });
         }
         if (p.gate_of_row) {
-            store_row<N, VEC>(dr, p.dgate + at, t, T, width, p.add_dgate);
-        } else {
-#pragma unroll
-            for (int i = 0; i < N; ++i) sum_gate[i] += dr[i];
-            if (p.dgate && (row + 1) % length == 0) {
-                store_row<N, VEC>(sum_gate, p.dgate + row / length * p.cols + c0, t, T, width, p.add_dgate);
-#pragma unroll
-                for (int i = 0; i < N; ++i) sum_gate[i] = 0.f;
+            row_of.store(dr, p.dgate + at, p.add_dgate);
+        } else if (p.gate) {
+            row_of.each([&](int i) { sum_gate[i] += dr[i]; });
+            if (--group_left == 0 && p.dgate) {
+                group_left = length;
+                row_of.store(sum_gate, p.dgate + row / length * p.cols + c0, p.add_dgate);
+                row_of.each([&](int i) { sum_gate[i] = 0.f; });
             }
         }
         if (!p.dh) continue;
         if (p.post_w) {
             round(q);
+            const float q_hat = q[0] * inv;
             float q_one = 0.f;
             if constexpr (LAYER) q_one = q[1] * inv;
-            const float q_hat = q[0] * inv;
-#pragma unroll
-            for (int i = 0; i < N; ++i) b[i] = hs * (b[i] - h[i] * q_hat - q_one);
+            row_of.each([&](int i) { b[i] = hs * (LAYER ? b[i] - h[i] * q_hat - q_one : b[i] - h[i] * q_hat); });
         }
-        store_row<N, VEC>(b, p.dh + at, t, T, width, p.add_dh);
+        row_of.store(b, p.dh + at, p.add_dh);
     }
     const size_t mine = size_t(block) * p.cols + c0;
-    if (p.partial[DPRE_W]) store_row<N, VEC>(sum_pre_w, p.partial[DPRE_W] + mine, t, T, width, false);
-    if (BIAS && p.partial[DPRE_B]) store_row<N, VEC>(sum_pre_b, p.partial[DPRE_B] + mine, t, T, width, false);
-    if (p.partial[DPOST_W]) store_row<N, VEC>(sum_post_w, p.partial[DPOST_W] + mine, t, T, width, false);
-    if (BIAS && p.partial[DPOST_B]) store_row<N, VEC>(sum_post_b, p.partial[DPOST_B] + mine, t, T, width, false);
-    if (p.partial[DGATE]) store_row<N, VEC>(sum_gate, p.partial[DGATE] + mine, t, T, width, false);
+    if (p.partial[DPRE_W]) row_of.store(sum_pre_w, p.partial[DPRE_W] + mine, false);
+    if (BIAS && p.partial[DPRE_B]) row_of.store(sum_pre_b, p.partial[DPRE_B] + mine, false);
+    if (p.partial[DPOST_W]) row_of.store(sum_post_w, p.partial[DPOST_W] + mine, false);
+    if (BIAS && p.partial[DPOST_B]) row_of.store(sum_post_b, p.partial[DPOST_B] + mine, false);
+    if (p.partial[DGATE]) row_of.store(sum_gate, p.partial[DGATE] + mine, false);
     if (CLUSTER) cluster_sync_all();  // no block leaves while another may read its sums
 }
 
@@ -679,24 +744,48 @@ bool pieces(int cols, std::initializer_list<const void *> pointers) {
     return (at & 15u) == 0;
 }
 
-template <int N, bool LAYER>
-int32_t start_forward_of(katsu_cuda_ctx *ctx, const Forward &p, bool vec, bool warp, unsigned grid, unsigned block) {
-    if (warp) return start(ctx, vec ? norm_fwd_kernel<16, true, true, LAYER> : norm_fwd_kernel<16, false, true, LAYER>, grid, block, p);
-    return start(ctx, vec ? norm_fwd_kernel<N, true, false, LAYER> : norm_fwd_kernel<N, false, false, LAYER>, grid, block, p);
+template <bool LAYER>
+int32_t start_forward_of(katsu_cuda_ctx *ctx, const Forward &p, bool wide, bool vec, Rows rows, const Slab &slab, size_t smem,
+                         unsigned grid, unsigned block) {
+    auto kernel = wide               ? norm_fwd_kernel<32, true, OF_BLOCK, LAYER>
+                  : rows == BY_RING  ? norm_fwd_kernel<16, true, BY_RING, LAYER>
+                  : rows == OF_BLOCK ? (vec ? norm_fwd_kernel<16, true, OF_BLOCK, LAYER> : norm_fwd_kernel<16, false, OF_BLOCK, LAYER>)
+                                     : (vec ? norm_fwd_kernel<16, true, OF_WARP, LAYER> : norm_fwd_kernel<16, false, OF_WARP, LAYER>);
+    KATSU_TRY(katsu_prepare_kernel(ctx, (const void *)kernel, smem));
+    return katsu_launch_chained(ctx, kernel, grid, block, smem, 1, p, slab);
 }
 
 template <bool LAYER>
 int32_t start_forward(katsu_cuda_ctx *ctx, const Forward &p) {
     const bool vec = pieces(p.cols, {p.x, p.h, p.gate, p.post_w, p.post_b, p.pre_w, p.pre_b, p.r, p.n});
     const unsigned long long sms = ctx->num_sms;
-    if (p.cols > kMostThreads * 32)
+    if (p.cols > kMostThreads * (vec ? 32 : 16))
         return start(ctx, norm_fwd_long_kernel<LAYER>, unsigned(p.rows < sms * 8 ? p.rows : sms * 8), kThreads, p);
     // 16 values a thread, 32 where that would take more than 512 threads; up to 512 values are one warp's
-    const bool warp = p.cols <= 512, wide = p.cols > kMostThreads * 16;
-    const unsigned threads = warp ? 128 : unsigned(katsu_div_up(katsu_div_up(p.cols, wide ? 32 : 16), 32)) * 32;
-    const unsigned long long need = warp ? katsu_div_up(p.rows, 4) : p.rows, most = sms * (2048 / threads);
+    const bool wide = p.cols > kMostThreads * 16;
+    Rows rows = p.cols <= 512 ? OF_WARP : OF_BLOCK;
+    const unsigned threads = rows == OF_WARP ? 128 : unsigned(katsu_div_up(katsu_div_up(p.cols, wide ? 32 : 16), 32)) * 32;
+    const unsigned long long need = rows == OF_WARP ? katsu_div_up(p.rows, 4) : p.rows;
+    unsigned long long most = sms * (2048 / threads);
+    Slab slab = {};
+    size_t smem = 0;
+    // A block that takes several rows brings them ahead; a single one arrives sooner by plain loads (one row of 4096: 5.6 us).
+    unsigned resident = 512 / threads;
+    if (resident > 8) resident = 8;
+    if (vec && rows == OF_BLOCK && !wide && p.rows > sms * resident) {
+        slab.width = p.cols;
+        slab.arrays = 1 + (p.h != nullptr) + (p.gate && p.rows_per_gate == 1);
+        const size_t row = size_t(slab.arrays) * p.cols * sizeof(float), room = kRoom / resident - 2048;
+        const size_t stages = room / row < kMostStages ? room / row : kMostStages;
+        if (stages >= 2) {
+            rows = BY_RING;
+            slab.stages = int(stages);
+            smem = slab.stages * row;
+            most = sms * resident;
+        }
+    }
     const unsigned grid = unsigned(need < most ? need : most);
-    return wide ? start_forward_of<32, LAYER>(ctx, p, vec, warp, grid, threads) : start_forward_of<16, LAYER>(ctx, p, vec, warp, grid, threads);
+    return start_forward_of<LAYER>(ctx, p, wide, vec, rows, slab, smem, grid, threads);
 }
 
 // Which kernel a backward pass takes, and how many blocks (or clusters) go round at once.
@@ -721,8 +810,8 @@ BackwardShape backward_shape(const katsu_cuda_ctx *ctx, const Backward &p, std::
     if (resident > 8) resident = 8;
     if (vec) {
         s.slab.arrays = 1 + (p.h != nullptr) + (p.dn != nullptr) + (p.dr != nullptr) + (p.gate && p.rows_per_gate == 1);
-        const size_t row = size_t(s.slab.arrays) * s.slab.width * sizeof(float), room = size_t(216) * 1024 / resident - 1024;
-        s.slab.stages = int(room / row < 4 ? room / row : 4);
+        const size_t row = size_t(s.slab.arrays) * s.slab.width * sizeof(float), room = kRoom / resident - 2048;
+        s.slab.stages = int(room / row < kMostStages ? room / row : kMostStages);
         s.smem = s.slab.stages * row;
     }
     s.most_blocks = size_t(ctx->num_sms) * resident / s.cluster;
@@ -774,7 +863,7 @@ extern "C" int32_t katsu_cuda_block_norm_fwd(katsu_cuda_ctx *ctx, const float *x
         KATSU_REQUIRE(in == nullptr || (in != r && in != n), "an output is an input too");
     KATSU_REQUIRE(r != n, "r and n are the same buffer");
     KATSU_TRY(katsu_bind(ctx));
-    Forward p = {x, h, gate, post_w, post_b, pre_w, pre_b, r, n, scale, eps, rows, gate ? rows / gate_rows : 1, (int)cols};
+    Forward p = {x, h, gate, post_w, post_b, pre_w, pre_b, r, n, scale, eps, rows, gate ? rows / gate_rows : 1, (int)cols, ctx->status};
     return kind == KATSU_NORM_LAYER ? start_forward<true>(ctx, p) : start_forward<false>(ctx, p);
 }
 

@@ -21,18 +21,21 @@
 namespace {
 
 constexpr int kThreads = 256;
-constexpr unsigned kChunk = 4096;  // values a block takes at a time: four 16-byte loads a thread
-constexpr int kMaxTensors = 512;   // a launch (14 KiB of parameters)
-constexpr int kFewTensors = 32;    // (1 KiB: the launch of a large parameter block takes longer)
+constexpr unsigned kUnit = 4 * kThreads;  // values of one 16-byte access a thread
+constexpr int kBatch = 4;                 // units whose loads are on their way together
+constexpr int kMaxTensors = 512;          // a launch (14 KiB of parameters)
+constexpr int kFewTensors = 32;           // (1 KiB: the launch of a large parameter block takes longer)
 
-// Tensors of one launch.  Chunk c of a tensor has the values whose place behind the 16-byte boundary at or in front of the
-// tensor is c * kChunk .. c * kChunk + kChunk - 1, so that 16-byte accesses fit tensors at any address.
+// Tensors of one launch.  Unit u of a tensor has the values whose place behind the 16-byte boundary at or in front of the
+// tensor is u * kUnit .. u * kUnit + kUnit - 1, so that 16-byte accesses fit tensors at any address.  A block takes a run of
+// units, of all tensors counted through: runs differ by one unit, so no block has a chunk more than the others to do, and the
+// tensor of a unit is searched for once a block.
 template <int N>
 struct Tensors {
     const float *src[N];
     float *dst[N];
     unsigned long long count[N];
-    unsigned first[N + 1];  // chunks in front of the tensor
+    unsigned first[N + 1];  // units in front of the tensor
     int tensors;
 };
 
@@ -49,15 +52,35 @@ __device__ __forceinline__ double block_sum(double v, double *sh) {
     return t;
 }
 
-template <int N>
-__device__ __forceinline__ int tensor_of(const Tensors<N> &t, unsigned chunk) {
-    int lo = 0, hi = t.tensors - 1;  // the last tensor whose first chunk is not behind this one (empty ones have none)
+// The block's run of units, in batches of a tensor's own; BACKWARDS: from its last unit to its first.
+template <bool BACKWARDS, int N, typename F>
+__device__ __forceinline__ void each_batch(const Tensors<N> &t, F f) {
+    const unsigned units = t.first[t.tensors];
+    unsigned begin = unsigned((unsigned long long)units * blockIdx.x / gridDim.x);
+    unsigned end = unsigned((unsigned long long)units * (blockIdx.x + 1) / gridDim.x);
+    if (begin >= end) return;
+    const unsigned at = BACKWARDS ? end - 1 : begin;
+    int lo = 0, hi = t.tensors - 1;  // the last tensor whose first unit is not behind this one (empty tensors are left out)
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
-        if (t.first[mid] <= chunk) lo = mid;
+        if (t.first[mid] <= at) lo = mid;
         else hi = mid - 1;
     }
-    return lo;
+    if (BACKWARDS) {
+        for (; end > begin; --lo)
+            while (end > begin && end > t.first[lo]) {
+                const unsigned low = max(begin, t.first[lo]), from = end - low > kBatch ? end - kBatch : low;
+                f(lo, from - t.first[lo], int(end - from));
+                end = from;
+            }
+    } else {
+        for (; begin < end; ++lo)
+            while (begin < end && begin < t.first[lo + 1]) {
+                const unsigned high = min(end, t.first[lo + 1]), to = high - begin > kBatch ? begin + kBatch : high;
+                f(lo, begin - t.first[lo], int(to - begin));
+                begin = to;
+            }
+    }
 }
 
 __device__ __forceinline__ unsigned lead_of(const float *p) { return unsigned(reinterpret_cast<uintptr_t>(p) >> 2) & 3u; }
@@ -68,33 +91,34 @@ __global__ void __launch_bounds__(kThreads) squares_kernel(const __grid_constant
     launch_next();
     launch_wait();
     double acc = 0.0;
-    for (unsigned chunk = blockIdx.x; chunk < t.first[t.tensors]; chunk += gridDim.x) {
-        const int i = tensor_of(t, chunk);
+    each_batch<false>(t, [&](int i, unsigned unit, int units) {
         const float *src = t.src[i];
         const unsigned lead = lead_of(src);
         const float *base = src - lead;
-        const unsigned long long begin = (unsigned long long)(chunk - t.first[i]) * kChunk, end = lead + t.count[i];
-        float4 v[kChunk / 4 / kThreads];
+        const unsigned long long begin = (unsigned long long)unit * kUnit, end = lead + t.count[i];
+        float4 v[kBatch];
 #pragma unroll
-        for (int j = 0; j < int(kChunk / 4 / kThreads); ++j) {
+        for (int j = 0; j < kBatch; ++j) {
             const unsigned long long a = begin + 4ull * (threadIdx.x + j * kThreads);
+            v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (j >= units) continue;
             if (a >= lead && a + 4 <= end) {
                 v[j] = __ldg(reinterpret_cast<const float4 *>(base + a));
             } else {
-                v[j].x = a >= lead && a < end ? __ldg(base + a) : 0.f;
-                v[j].y = a + 1 >= lead && a + 1 < end ? __ldg(base + a + 1) : 0.f;
-                v[j].z = a + 2 >= lead && a + 2 < end ? __ldg(base + a + 2) : 0.f;
-                v[j].w = a + 3 >= lead && a + 3 < end ? __ldg(base + a + 3) : 0.f;
+                if (a >= lead && a < end) v[j].x = __ldg(base + a);
+                if (a + 1 >= lead && a + 1 < end) v[j].y = __ldg(base + a + 1);
+                if (a + 2 >= lead && a + 2 < end) v[j].z = __ldg(base + a + 2);
+                if (a + 3 >= lead && a + 3 < end) v[j].w = __ldg(base + a + 3);
             }
         }
 #pragma unroll
-        for (int j = 0; j < int(kChunk / 4 / kThreads); ++j) {
+        for (int j = 0; j < kBatch; ++j) {
             acc = fma((double)v[j].x, (double)v[j].x, acc);
             acc = fma((double)v[j].y, (double)v[j].y, acc);
             acc = fma((double)v[j].z, (double)v[j].z, acc);
             acc = fma((double)v[j].w, (double)v[j].w, acc);
         }
-    }
+    });
     __shared__ double sh[kThreads / 32];
     acc = block_sum(acc, sh);
     if (threadIdx.x == 0) partial[blockIdx.x] = acc;
@@ -132,32 +156,29 @@ __global__ void __launch_bounds__(kThreads) apply_kernel(const __grid_constant__
     const bool finite = isfinite(sum);
     if (OP == STEP && !finite) return;
     const float c = finite && total > (double)max_norm ? (float)((double)max_norm / total) : 1.f;
-    const unsigned chunks = t.first[t.tensors];
-    // from the last chunk to the first: what the pass over the squares has read last is still in L2
-    for (unsigned q = blockIdx.x; q < chunks; q += gridDim.x) {
-        const unsigned chunk = chunks - 1 - q;
-        const int i = tensor_of(t, chunk);
+    // each block from its last unit to its first: what the pass over the squares has read last is still in L2
+    each_batch<true>(t, [&](int i, unsigned unit, int units) {
         const float *src = t.src[i];
         float *dst = t.dst[i];
-        if (OP == CLIP && c == 1.f && src == dst) continue;
+        if (OP == CLIP && c == 1.f && src == dst) return;
         const unsigned lead = lead_of(src);
-        const unsigned long long begin = (unsigned long long)(chunk - t.first[i]) * kChunk, end = lead + t.count[i];
+        const unsigned long long begin = (unsigned long long)unit * kUnit, end = lead + t.count[i];
         const float *sb = src - lead;
         float *db = dst - lead;
         if (lead_of(dst) == lead) {
-            constexpr int loads = kChunk / 4 / kThreads;
-            float4 g[loads], w[loads];
+            float4 g[kBatch], w[kBatch];
 #pragma unroll
-            for (int j = 0; j < loads; ++j) {
+            for (int j = 0; j < kBatch; ++j) {
                 const unsigned long long a = begin + 4ull * (threadIdx.x + j * kThreads);
-                if (a >= lead && a + 4 <= end) {
+                if (j < units && a >= lead && a + 4 <= end) {
                     g[j] = *reinterpret_cast<const float4 *>(sb + a);
                     if (OP == STEP) w[j] = *reinterpret_cast<const float4 *>(db + a);
                 }
             }
 #pragma unroll
-            for (int j = 0; j < loads; ++j) {
+            for (int j = 0; j < kBatch; ++j) {
                 const unsigned long long a = begin + 4ull * (threadIdx.x + j * kThreads);
+                if (j >= units) continue;
                 if (a >= lead && a + 4 <= end) {
                     float4 o;
                     o.x = applied<OP>(g[j].x, OP == STEP ? w[j].x : 0.f, c, lr);
@@ -171,37 +192,37 @@ __global__ void __launch_bounds__(kThreads) apply_kernel(const __grid_constant__
                 }
             }
         } else {
-            const unsigned long long last = begin + kChunk < end ? begin + kChunk : end;
+            const unsigned long long last = min(begin + (unsigned long long)units * kUnit, end);
             for (unsigned long long b = begin + threadIdx.x; b < last; b += kThreads)
                 if (b >= lead) db[b] = applied<OP>(sb[b], OP == STEP ? db[b] : 0.f, c, lr);
         }
-    }
+    });
 }
 
 template <int N>
 size_t take(Tensors<N> *t, const float *const *src, float *const *dst, const size_t *counts, size_t from, size_t tensors) {
     int k = 0;
-    unsigned long long chunks = 0;
+    unsigned long long units = 0;
     size_t i = from;
     for (; i < tensors && k < N; ++i) {
         if (counts[i] == 0) continue;
         const unsigned long long lead = (reinterpret_cast<uintptr_t>(src[i]) >> 2) & 3u;
-        const unsigned long long more = (lead + counts[i] + kChunk - 1) / kChunk;
-        if (k > 0 && chunks + more > 0xf0000000ull) break;
+        const unsigned long long more = (lead + counts[i] + kUnit - 1) / kUnit;
+        if (k > 0 && units + more > 0xf0000000ull) break;
         t->src[k] = src[i];
         t->dst[k] = dst ? dst[i] : nullptr;
         t->count[k] = counts[i];
-        t->first[k] = (unsigned)chunks;
-        chunks += more;
-        t->first[++k] = (unsigned)chunks;
+        t->first[k] = (unsigned)units;
+        units += more;
+        t->first[++k] = (unsigned)units;
     }
     t->tensors = k;
     return i;
 }
 
-unsigned blocks_for(const katsu_cuda_ctx *ctx, unsigned chunks) {
+unsigned blocks_for(const katsu_cuda_ctx *ctx, unsigned units) {
     const unsigned most = unsigned(ctx->num_sms) * 8;
-    return chunks < most ? chunks : most;
+    return units < most ? units : most;
 }
 
 enum What { NORM_ONLY, CLIPPED, STEPPED };
@@ -280,7 +301,7 @@ int32_t checked(katsu_cuda_ctx *ctx, What what, const float *const *grads, float
     const auto holds_norm = [&](const float *p, size_t count) { return norm + 1 > p && norm < p + count; };
     for (size_t i = 0; i < tensors; ++i) {
         if (counts[i] == 0) continue;
-        KATSU_REQUIRE(counts[i] < (size_t(1) << 43), "count out of range");
+        KATSU_REQUIRE(counts[i] < (size_t(1) << 41), "count out of range");
         KATSU_REQUIRE(grads[i] != nullptr, "null gradient");
         KATSU_REQUIRE(((uintptr_t)grads[i] & 3u) == 0, "a gradient is not at a whole float");
         KATSU_REQUIRE(!holds_norm(grads[i], counts[i]), "norm lies in a gradient");

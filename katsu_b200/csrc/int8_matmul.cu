@@ -211,7 +211,7 @@ __global__ void __launch_bounds__(256) int8_fold_kernel(const int *__restrict__ 
     launch_wait();
     for (size_t i = size_t(blockIdx.x) * blockDim.x + threadIdx.x; i < count; i += size_t(gridDim.x) * blockDim.x) {
         int sum = 0;
-#pragma unroll 8
+#pragma unroll 16
         for (int s = 0; s < splits; ++s) sum += __ldg(partial + size_t(s) * count + i);
         const size_t token = i / channels;
         const unsigned channel = unsigned(i - token * channels);

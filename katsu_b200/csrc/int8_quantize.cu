@@ -1,13 +1,11 @@
 // Matrices to 8 bits: rows of x (one scale a token) and columns of w (one scale an output channel, kept transposed).
 //
-// Rows: a warp (up to 1024 values), or a block of 256 (up to 8192) or 512 threads takes a row, holds its first 32 values a
-// thread in registers between the largest magnitude and the quotients and reads the rest again, from L2.  Bound: HBM, 4 bytes
+// Rows: a warp (up to 1024 values), or a block of 256 (up to 4096) or 512 threads takes a row, holds its first 32 or 16 values
+// a thread in registers between the largest magnitude and the quotients and reads the rest again, from L2.  Bound: HBM, 4 bytes
 // in and 1 out a value.
 #include "int8.cuh"
 
 namespace {
-
-constexpr int kHeld = 8;  // 16-byte pieces of a row that a thread holds
 
 // Values j .. j + 3 of a row, zeros behind its end.
 template <bool VEC>
@@ -21,9 +19,10 @@ __device__ __forceinline__ void load4(const float *row, size_t j, size_t k, floa
     }
 }
 
-template <int T, bool VEC>
-__global__ void __launch_bounds__(T < 256 ? 256 : T, T < 256 ? 4 : 1024 / T) quantize_rows_kernel(const float *__restrict__ x, int8_t *q, float *scale,
-                                                                               unsigned long long rows, size_t k, size_t pitch) {
+// T threads to a row, each of which holds kHeld 16-byte pieces.
+template <int T, int kHeld, bool VEC>
+__global__ void __launch_bounds__(T < 256 ? 256 : T) quantize_rows_kernel(const float *__restrict__ x, int8_t *q, float *scale,
+                                                                          unsigned long long rows, size_t k, size_t pitch) {
     __shared__ float sh[2][32];
     launch_next();
     launch_wait();
@@ -131,12 +130,13 @@ __global__ void __launch_bounds__(256) quantize_columns_kernel(const float *__re
 
 int32_t katsu_int8_quantize(katsu_cuda_ctx *ctx, const float *x, int8_t *q, float *scale, size_t m, size_t k) {
     const bool vec = k % 4 == 0 && (reinterpret_cast<uintptr_t>(x) & 15u) == 0;
-    const bool small = k <= 32 * 4 * kHeld, long_rows = k > 256 * 4 * kHeld;
-    const unsigned threads = long_rows ? 512 : 256;
-    const size_t need = small ? katsu_div_up(m, 8) : m, most = size_t(ctx->num_sms) * (2048 / threads);
-    auto kernel = small ? (vec ? quantize_rows_kernel<32, true> : quantize_rows_kernel<32, false>)
-                  : long_rows ? (vec ? quantize_rows_kernel<512, true> : quantize_rows_kernel<512, false>)
-                              : (vec ? quantize_rows_kernel<256, true> : quantize_rows_kernel<256, false>);
+    const bool small = k <= 1024, medium = k <= 4096;
+    const unsigned threads = medium ? 256 : 512;
+    // a block to every row: the hardware hands them out as others end, and the rounds of one hide behind the loads of others
+    const size_t need = small ? katsu_div_up(m, 8) : m, most = 0x7fffffff;
+    auto kernel = small    ? (vec ? quantize_rows_kernel<32, 8, true> : quantize_rows_kernel<32, 8, false>)
+                  : medium ? (vec ? quantize_rows_kernel<256, 4, true> : quantize_rows_kernel<256, 4, false>)
+                           : (vec ? quantize_rows_kernel<512, 4, true> : quantize_rows_kernel<512, 4, false>);
     KATSU_TRY(katsu_prepare_kernel(ctx, (const void *)kernel, 0));
     return katsu_launch_chained(ctx, kernel, (unsigned)(need < most ? need : most), threads, 0, 1, x, q, scale, m, k,
                                 katsu_int8_pitch(k));

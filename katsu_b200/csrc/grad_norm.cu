@@ -2,8 +2,9 @@
 //
 //   norm = sqrt(sum over all tensors of g^2)      c = max_norm / norm where that is below 1      g' = c g      w -= lr (c g)
 //
-// Two launches whatever the number of tensors (one more pair for every 512): the first leaves a partial sum of squares a
-// block, the blocks of the second fold these for themselves and then scale or step.  The addresses travel as a kernel
+// Two launches (and one more pair for every 512 tensors): the first leaves a partial sum of squares a block, the blocks of the
+// second fold these for themselves and then scale or step.  From 1200 blocks on a launch between the two folds once for all, and
+// the blocks of the last are handed out as others end.  The addresses travel as a kernel
 // parameter, so nothing on the host has to outlive the call and a captured call keeps them.
 //
 // Squares are summed in 64 bits: 1e-30 and 1e30 neither vanish nor overflow, the sum of 1e9 values keeps more bits than the
@@ -27,9 +28,7 @@ constexpr int kMaxTensors = 512;          // a launch (14 KiB of parameters)
 constexpr int kFewTensors = 32;           // (1 KiB: the launch of a large parameter block takes longer)
 
 // Tensors of one launch.  Unit u of a tensor has the values whose place behind the 16-byte boundary at or in front of the
-// tensor is u * kUnit .. u * kUnit + kUnit - 1, so that 16-byte accesses fit tensors at any address.  A block takes a run of
-// units, of all tensors counted through: runs differ by one unit, so no block has a chunk more than the others to do, and the
-// tensor of a unit is searched for once a block.
+// tensor is u * kUnit .. u * kUnit + kUnit - 1, so that 16-byte accesses fit tensors at any address.
 template <int N>
 struct Tensors {
     const float *src[N];
@@ -52,35 +51,34 @@ __device__ __forceinline__ double block_sum(double v, double *sh) {
     return t;
 }
 
-// The block's run of units, in batches of a tensor's own; BACKWARDS: from its last unit to its first.
-template <bool BACKWARDS, int N, typename F>
-__device__ __forceinline__ void each_batch(const Tensors<N> &t, F f) {
-    const unsigned units = t.first[t.tensors];
-    unsigned begin = unsigned((unsigned long long)units * blockIdx.x / gridDim.x);
-    unsigned end = unsigned((unsigned long long)units * (blockIdx.x + 1) / gridDim.x);
-    if (begin >= end) return;
-    const unsigned at = BACKWARDS ? end - 1 : begin;
-    int lo = 0, hi = t.tensors - 1;  // the last tensor whose first unit is not behind this one (empty tensors are left out)
+// Units begin .. end - 1, of all tensors counted through, as batches of one tensor's: the first batch, and the one behind it.
+struct Batch {
+    int tensor, units;  // units 0: none is left
+    unsigned unit;      // first one, of the tensor's
+    unsigned begin, end;
+};
+
+template <int N>
+__device__ __forceinline__ void next_batch(const Tensors<N> &t, Batch *b) {
+    b->units = 0;
+    if (b->begin >= b->end) return;
+    while (b->begin >= t.first[b->tensor + 1]) ++b->tensor;
+    b->unit = b->begin - t.first[b->tensor];
+    b->units = int(min(min(b->end, t.first[b->tensor + 1]) - b->begin, unsigned(kBatch)));
+    b->begin += b->units;
+}
+
+template <int N>
+__device__ __forceinline__ Batch first_batch(const Tensors<N> &t, unsigned begin, unsigned end) {
+    int lo = 0, hi = t.tensors - 1;  // the last tensor whose first unit is not behind `begin` (empty tensors are left out)
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
-        if (t.first[mid] <= at) lo = mid;
+        if (t.first[mid] <= begin) lo = mid;
         else hi = mid - 1;
     }
-    if (BACKWARDS) {
-        for (; end > begin; --lo)
-            while (end > begin && end > t.first[lo]) {
-                const unsigned low = max(begin, t.first[lo]), from = end - low > kBatch ? end - kBatch : low;
-                f(lo, from - t.first[lo], int(end - from));
-                end = from;
-            }
-    } else {
-        for (; begin < end; ++lo)
-            while (begin < end && begin < t.first[lo + 1]) {
-                const unsigned high = min(end, t.first[lo + 1]), to = high - begin > kBatch ? begin + kBatch : high;
-                f(lo, begin - t.first[lo], int(to - begin));
-                begin = to;
-            }
-    }
+    Batch b = {lo, 0, 0, begin, end};
+    next_batch(t, &b);
+    return b;
 }
 
 __device__ __forceinline__ unsigned lead_of(const float *p) { return unsigned(reinterpret_cast<uintptr_t>(p) >> 2) & 3u; }
@@ -91,17 +89,21 @@ __global__ void __launch_bounds__(kThreads) squares_kernel(const __grid_constant
     launch_next();
     launch_wait();
     double acc = 0.0;
-    each_batch<false>(t, [&](int i, unsigned unit, int units) {
+    // runs differ by one unit, so no block has a batch more to do than the others
+    const unsigned long long units = t.first[t.tensors];
+    for (Batch b = first_batch(t, unsigned(units * blockIdx.x / gridDim.x), unsigned(units * (blockIdx.x + 1) / gridDim.x)); b.units;
+         next_batch(t, &b)) {
+        const int i = b.tensor;
         const float *src = t.src[i];
         const unsigned lead = lead_of(src);
         const float *base = src - lead;
-        const unsigned long long begin = (unsigned long long)unit * kUnit, end = lead + t.count[i];
+        const unsigned long long begin = (unsigned long long)b.unit * kUnit, end = lead + t.count[i];
         float4 v[kBatch];
 #pragma unroll
         for (int j = 0; j < kBatch; ++j) {
             const unsigned long long a = begin + 4ull * (threadIdx.x + j * kThreads);
             v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (j >= units) continue;
+            if (j >= b.units) continue;
             if (a >= lead && a + 4 <= end) {
                 v[j] = __ldg(reinterpret_cast<const float4 *>(base + a));
             } else {
@@ -118,7 +120,7 @@ __global__ void __launch_bounds__(kThreads) squares_kernel(const __grid_constant
             acc = fma((double)v[j].z, (double)v[j].z, acc);
             acc = fma((double)v[j].w, (double)v[j].w, acc);
         }
-    });
+    }
     __shared__ double sh[kThreads / 32];
     acc = block_sum(acc, sh);
     if (threadIdx.x == 0) partial[blockIdx.x] = acc;
@@ -132,11 +134,19 @@ __device__ __forceinline__ double fold(const double *partial, int parts) {
     return block_sum(acc, sh);
 }
 
-__global__ void __launch_bounds__(kThreads) norm_kernel(const double *partial, int parts, float *norm) {
+// What gradients are multiplied by; NaN: one of them is no number.
+__device__ __forceinline__ float factor_of(double sum, double norm, float max_norm) {
+    if (!isfinite(sum)) return __int_as_float(0x7fffffff);
+    return norm > (double)max_norm ? (float)((double)max_norm / norm) : 1.f;
+}
+
+__global__ void __launch_bounds__(kThreads) norm_kernel(const double *partial, int parts, float max_norm, float *norm, float *factor) {
     launch_next();
     launch_wait();
-    const double sum = fold(partial, parts);
-    if (threadIdx.x == 0) norm[0] = (float)sqrt(sum);
+    const double sum = fold(partial, parts), total = sqrt(sum);
+    if (threadIdx.x != 0) return;
+    norm[0] = (float)total;
+    if (factor) *factor = factor_of(sum, total, max_norm);
 }
 
 // g and the product are rounded as katsu_cuda_clip_grads followed by katsu_cuda_sgd_step round them.
@@ -146,57 +156,75 @@ __device__ __forceinline__ float applied(float g, float w, float c, float lr) {
     return OP == CLIP ? clipped : w - __fmul_rn(lr, clipped);
 }
 
+// A block takes a batch of units (of several tensors where they are short), the last one first: what the pass over the squares
+// has read last is still in L2.  The first loads are on their way before the block looks at the factor or folds the sums for it
+// (looking first, the 240 tensors' step took 682 us, at 5.3 TB/s).
 template <Apply OP, int N>
 __global__ void __launch_bounds__(kThreads) apply_kernel(const __grid_constant__ Tensors<N> t, const double *partial, int parts,
-                                                         float max_norm, float lr, float *norm) {
+                                                         const float *factor, float max_norm, float lr, float *norm) {
     launch_next();
     launch_wait();
-    const double sum = fold(partial, parts), total = sqrt(sum);
-    if (norm != nullptr && blockIdx.x == 0 && threadIdx.x == 0) norm[0] = (float)total;
-    const bool finite = isfinite(sum);
-    if (OP == STEP && !finite) return;
-    const float c = finite && total > (double)max_norm ? (float)((double)max_norm / total) : 1.f;
-    // each block from its last unit to its first: what the pass over the squares has read last is still in L2
-    each_batch<true>(t, [&](int i, unsigned unit, int units) {
-        const float *src = t.src[i];
-        float *dst = t.dst[i];
-        if (OP == CLIP && c == 1.f && src == dst) return;
+    const unsigned begin_unit = (gridDim.x - 1 - blockIdx.x) * kBatch;
+    Batch b = first_batch(t, begin_unit, min(begin_unit + kBatch, t.first[t.tensors]));
+    // One thread reads the factor: read by all, its one place in L2 had 600 000 requests to answer and held up the rest (633 us).
+    __shared__ float shared_factor;
+    if (factor != nullptr && threadIdx.x == 0) shared_factor = __ldcg(factor);
+    float c = 0.f;
+    bool known = false;
+    for (; b.units; next_batch(t, &b)) {
+        const float *src = t.src[b.tensor];
+        float *dst = t.dst[b.tensor];
         const unsigned lead = lead_of(src);
-        const unsigned long long begin = (unsigned long long)unit * kUnit, end = lead + t.count[i];
+        const unsigned long long begin = (unsigned long long)b.unit * kUnit, end = lead + t.count[b.tensor];
         const float *sb = src - lead;
         float *db = dst - lead;
-        if (lead_of(dst) == lead) {
-            float4 g[kBatch], w[kBatch];
+        const bool whole = lead_of(dst) == lead;
+        float4 g[kBatch], w[kBatch];
+        if (whole)
 #pragma unroll
             for (int j = 0; j < kBatch; ++j) {
                 const unsigned long long a = begin + 4ull * (threadIdx.x + j * kThreads);
-                if (j < units && a >= lead && a + 4 <= end) {
+                if (j < b.units && a >= lead && a + 4 <= end) {
                     g[j] = *reinterpret_cast<const float4 *>(sb + a);
                     if (OP == STEP) w[j] = *reinterpret_cast<const float4 *>(db + a);
                 }
             }
+        if (!known && factor != nullptr) {
+            __syncthreads();
+            c = shared_factor;
+        } else if (!known) {
+            const double sum = fold(partial, parts), total = sqrt(sum);
+            if (norm != nullptr && blockIdx.x == 0 && threadIdx.x == 0) norm[0] = (float)total;
+            c = factor_of(sum, total, max_norm);
+        }
+        known = true;
+        const bool finite = !isnan(c);
+        if (OP == STEP && !finite) return;
+        const float scale = finite ? c : 1.f;
+        if (OP == CLIP && scale == 1.f && src == dst) continue;
+        if (whole) {
 #pragma unroll
             for (int j = 0; j < kBatch; ++j) {
                 const unsigned long long a = begin + 4ull * (threadIdx.x + j * kThreads);
-                if (j >= units) continue;
+                if (j >= b.units) continue;
                 if (a >= lead && a + 4 <= end) {
                     float4 o;
-                    o.x = applied<OP>(g[j].x, OP == STEP ? w[j].x : 0.f, c, lr);
-                    o.y = applied<OP>(g[j].y, OP == STEP ? w[j].y : 0.f, c, lr);
-                    o.z = applied<OP>(g[j].z, OP == STEP ? w[j].z : 0.f, c, lr);
-                    o.w = applied<OP>(g[j].w, OP == STEP ? w[j].w : 0.f, c, lr);
+                    o.x = applied<OP>(g[j].x, OP == STEP ? w[j].x : 0.f, scale, lr);
+                    o.y = applied<OP>(g[j].y, OP == STEP ? w[j].y : 0.f, scale, lr);
+                    o.z = applied<OP>(g[j].z, OP == STEP ? w[j].z : 0.f, scale, lr);
+                    o.w = applied<OP>(g[j].w, OP == STEP ? w[j].w : 0.f, scale, lr);
                     *reinterpret_cast<float4 *>(db + a) = o;
                 } else {
-                    for (unsigned long long b = a; b < a + 4; ++b)
-                        if (b >= lead && b < end) db[b] = applied<OP>(sb[b], OP == STEP ? db[b] : 0.f, c, lr);
+                    for (unsigned long long e = a; e < a + 4; ++e)
+                        if (e >= lead && e < end) db[e] = applied<OP>(sb[e], OP == STEP ? db[e] : 0.f, scale, lr);
                 }
             }
         } else {
-            const unsigned long long last = min(begin + (unsigned long long)units * kUnit, end);
-            for (unsigned long long b = begin + threadIdx.x; b < last; b += kThreads)
-                if (b >= lead) db[b] = applied<OP>(sb[b], OP == STEP ? db[b] : 0.f, c, lr);
+            const unsigned long long last = min(begin + (unsigned long long)b.units * kUnit, end);
+            for (unsigned long long e = begin + threadIdx.x; e < last; e += kThreads)
+                if (e >= lead) db[e] = applied<OP>(sb[e], OP == STEP ? db[e] : 0.f, scale, lr);
         }
-    });
+    }
 }
 
 template <int N>
@@ -220,10 +248,8 @@ size_t take(Tensors<N> *t, const float *const *src, float *const *dst, const siz
     return i;
 }
 
-unsigned blocks_for(const katsu_cuda_ctx *ctx, unsigned units) {
-    const unsigned most = unsigned(ctx->num_sms) * 8;
-    return units < most ? units : most;
-}
+// Blocks with at most a batch of units each.
+unsigned blocks_for(unsigned units) { return units / kBatch + (units % kBatch != 0); }
 
 enum What { NORM_ONLY, CLIPPED, STEPPED };
 
@@ -231,33 +257,42 @@ template <int N>
 int32_t run(katsu_cuda_ctx *ctx, What what, const float *const *grads, float *const *dst, const size_t *counts, size_t tensors,
             float lr, float max_norm, float *norm) {
     static thread_local Tensors<N> t;  // (too large for some hosts' stacks)
-    const size_t most = (size_t)ctx->num_sms * 8;
-    size_t launches = 0;
-    for (size_t i = 0; i < tensors; ++launches) i = take(&t, grads, dst, counts, i, tensors);
+    // Partial sums of a launch: more blocks than go round at once, which the hardware hands out as others end, read 15 % faster
+    // than each SM's share in one piece (1.2 GB: 170 us, 186), and 9 500 numbers are folded in 4 us.
+    const unsigned most = unsigned(ctx->num_sms) * 64;
+    size_t sums = 0, blocks = 0;
+    for (size_t i = 0; i < tensors;) {
+        i = take(&t, grads, dst, counts, i, tensors);
+        blocks += blocks_for(t.first[t.tensors]);
+        sums += std::min(blocks_for(t.first[t.tensors]), most);
+    }
     float *scratch = nullptr;
-    KATSU_TRY(katsu_scratch(ctx, (launches + 1) * most * 2, &scratch));
-    double *partial = reinterpret_cast<double *>(scratch);
+    KATSU_TRY(katsu_scratch(ctx, sums * 2 + 2, &scratch));
+    double *partial = reinterpret_cast<double *>(scratch + 2);
     KATSU_TRY(katsu_prepare_kernel(ctx, (const void *)squares_kernel<N>, 0));
     int parts = 0;
     for (size_t i = 0; i < tensors;) {
         i = take(&t, grads, dst, counts, i, tensors);
         if (t.tensors == 0) break;
-        const unsigned blocks = blocks_for(ctx, t.first[t.tensors]);
-        KATSU_TRY(katsu_launch_chained(ctx, squares_kernel<N>, blocks, kThreads, 0, 1, t, partial + parts));
-        parts += (int)blocks;
+        const unsigned grid = std::min(blocks_for(t.first[t.tensors]), most);
+        KATSU_TRY(katsu_launch_chained(ctx, squares_kernel<N>, grid, kThreads, 0, 1, t, partial + parts));
+        parts += (int)grid;
     }
-    if (what == NORM_ONLY || parts == 0) {
+    const bool between = what != NORM_ONLY && blocks > size_t(ctx->num_sms) * 8;
+    float *factor = between ? scratch : nullptr;
+    if (what == NORM_ONLY || between || parts == 0) {
         KATSU_TRY(katsu_prepare_kernel(ctx, (const void *)norm_kernel, 0));
-        return katsu_launch_chained(ctx, norm_kernel, 1, kThreads, 0, 1, partial, parts, norm);
+        KATSU_TRY(katsu_launch_chained(ctx, norm_kernel, 1, kThreads, 0, 1, partial, parts, max_norm, norm, factor));
     }
+    if (what == NORM_ONLY) return KATSU_OK;
     auto kernel = what == CLIPPED ? apply_kernel<CLIP, N> : apply_kernel<STEP, N>;
     KATSU_TRY(katsu_prepare_kernel(ctx, (const void *)kernel, 0));
     for (size_t i = 0; i < tensors;) {
         const bool first = i == 0;
         i = take(&t, grads, dst, counts, i, tensors);
         if (t.tensors == 0) break;
-        const unsigned blocks = blocks_for(ctx, t.first[t.tensors]);
-        KATSU_TRY(katsu_launch_chained(ctx, kernel, blocks, kThreads, 0, 1, t, partial, parts, max_norm, lr, first ? norm : nullptr));
+        KATSU_TRY(katsu_launch_chained(ctx, kernel, blocks_for(t.first[t.tensors]), kThreads, 0, 1, t, partial, parts, factor,
+                                       max_norm, lr, first ? norm : nullptr));
     }
     return KATSU_OK;
 }

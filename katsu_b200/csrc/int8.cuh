@@ -12,8 +12,7 @@ static inline size_t katsu_int8_pitch(size_t k) { return (k + 15) / 16 * 16; }
 struct KatsuInt8Scale {
     float scale;         // largest magnitude / 127: what results are multiplied by
     float lift, s, inv;  // s = scale * lift, inv = 1 / s
-    float half;          // s / 2
-    bool plain;          // lift is 1 and s a positive number
+    float half;          // s / 2; 0 where the quick way does not do: the scale is 0, no number, or lifted
 };
 
 __device__ __forceinline__ KatsuInt8Scale katsu_int8_scale(float largest) {
@@ -23,8 +22,7 @@ __device__ __forceinline__ KatsuInt8Scale katsu_int8_scale(float largest) {
     q.lift = q.scale < 0x1p-100f ? 0x1p64f : 1.f;
     q.s = q.scale * q.lift;
     q.inv = q.s > 0.f ? __fdiv_rn(1.f, q.s) : 0.f;
-    q.half = 0.5f * q.s;
-    q.plain = q.s > 0.f && q.lift == 1.f;
+    q.half = q.s > 0.f && q.lift == 1.f ? 0.5f * q.s : 0.f;
     return q;
 }
 
@@ -41,21 +39,18 @@ __device__ __forceinline__ int katsu_int8_quotient(float v, const KatsuInt8Scale
     return int(fminf(fmaxf(n, -127.f), 127.f));
 }
 
-// (a call, so that the registers of the quick way are its own)
-static __device__ __noinline__ unsigned katsu_int8_pack_exactly(float a, float b, float c, float d, float scale, float s, float inv) {
-    KatsuInt8Scale q = {};
-    q.scale = scale;
-    q.s = s;
-    q.inv = inv;
-    q.lift = scale < 0x1p-100f ? 0x1p64f : 1.f;
-    const int n[4] = {katsu_int8_quotient(a, q), katsu_int8_quotient(b, q), katsu_int8_quotient(c, q), katsu_int8_quotient(d, q)};
-    return (unsigned(n[0]) & 0xffu) | (unsigned(n[1]) & 0xffu) << 8 | (unsigned(n[2]) & 0xffu) << 16 | unsigned(n[3]) << 24;
+// Four values to four bytes by the definition.
+__device__ __forceinline__ unsigned katsu_int8_pack_exactly(const float (&v)[4], const KatsuInt8Scale &q) {
+    unsigned out = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) out |= (unsigned(katsu_int8_quotient(v[i], q)) & 0xffu) << (8 * i);
+    return out;
 }
 
-// Four values to four bytes.  Almost always the quick way: v / scale rounded by adding 1.5 * 2^23, whose last places are then the
-// whole number, and all four remainders below half a scale.  With a rounding instruction and a comparison for each value the
-// conversions, 16 a clock and SM, took twice the time of the loads (268 MB: 108 us).
-__device__ __forceinline__ unsigned katsu_int8_pack(const float (&v)[4], const KatsuInt8Scale &q) {
+// The same almost always, the quick way: v / scale rounded by adding 1.5 * 2^23, whose last places are then the whole number.
+// *sure turns false where a remainder is not below half a scale; the caller takes such pieces again, by the definition.  (With a
+// rounding instruction and a comparison for each value the conversions, 16 a clock and SM, took twice the time of the loads.)
+__device__ __forceinline__ unsigned katsu_int8_pack(const float (&v)[4], const KatsuInt8Scale &q, bool *sure) {
     constexpr float magic = 12582912.f;
     float n[4], most = 0.f;
 #pragma unroll
@@ -63,10 +58,9 @@ __device__ __forceinline__ unsigned katsu_int8_pack(const float (&v)[4], const K
         n[i] = fmaf(v[i], q.inv, magic);
         most = fmaxf(most, fabsf(fmaf(magic - n[i], q.s, v[i])));
     }
-    if (q.plain && most < q.half)
-        return __byte_perm(__byte_perm(__float_as_uint(n[0]), __float_as_uint(n[1]), 0x0040),
-                           __byte_perm(__float_as_uint(n[2]), __float_as_uint(n[3]), 0x0040), 0x5410);
-    return katsu_int8_pack_exactly(v[0], v[1], v[2], v[3], q.scale, q.s, q.inv);
+    *sure = *sure && most < q.half;
+    return __byte_perm(__byte_perm(__float_as_uint(n[0]), __float_as_uint(n[1]), 0x0040),
+                       __byte_perm(__float_as_uint(n[2]), __float_as_uint(n[3]), 0x0040), 0x5410);
 }
 
 // The larger magnitude; a NaN wins.

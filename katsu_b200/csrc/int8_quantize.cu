@@ -1,7 +1,7 @@
 // Matrices to 8 bits: rows of x (one scale a token) and columns of w (one scale an output channel, kept transposed).
 //
-// Rows: a warp (up to 1024 values), or a block of 256 (up to 4096) or 512 threads takes a row, holds its first 32 or 16 values
-// a thread in registers between the largest magnitude and the quotients and reads the rest again, from L2.  Bound: HBM, 4 bytes
+// Rows: a warp (up to 1024 values) or a block of 256 (up to 8192) or 512 threads takes a row and holds its last 32 values a
+// thread in registers between the largest magnitude and the quotients; what lies in front is read again, from L2.  Bound: HBM, 4 bytes
 // in and 1 out a value.
 #include "int8.cuh"
 
@@ -19,62 +19,62 @@ __device__ __forceinline__ void load4(const float *row, size_t j, size_t k, floa
     }
 }
 
-// T threads to a row, each of which holds kHeld 16-byte pieces.
+// T threads to a row, each of which holds kHeld 16-byte pieces: the row's last ones, loaded behind what is read twice, so that
+// their registers are free until then.
 template <int T, int kHeld, bool VEC>
 __global__ void __launch_bounds__(T < 256 ? 256 : T) quantize_rows_kernel(const float *__restrict__ x, int8_t *q, float *scale,
                                                                           unsigned long long rows, size_t k, size_t pitch) {
-    __shared__ float sh[2][32];
+    __shared__ float sh[T < 256 ? 1 : T / 32];
     launch_next();
     launch_wait();
-    constexpr int per_block = T < 256 ? 256 / T : 1;
+    constexpr int per_block = T < 256 ? 256 / T : 1, batch = 4 * T * kHeld;
     const int t = threadIdx.x % T;
-    int turn = 0;
-    for (unsigned long long row = (unsigned long long)blockIdx.x * per_block + threadIdx.x / T; row < rows;
-         row += (unsigned long long)gridDim.x * per_block, turn ^= 1) {
-        const float *src = x + row * k;
+    const unsigned long long row = (unsigned long long)blockIdx.x * per_block + threadIdx.x / T;
+    if (row >= rows) return;  // (a warp's rows: the others of the block do not wait)
+    const float *src = x + row * k;
+    const size_t twice = (pitch - 1) / batch * batch;  // values in front of the held ones
+    float most = 0.f;
+    for (size_t j0 = 0; j0 < twice; j0 += batch) {
         float v[kHeld][4];
-        float most = 0.f;
 #pragma unroll
-        for (int i = 0; i < kHeld; ++i) {
-            if (size_t(4 * T) * i >= k) break;
-            load4<VEC>(src, 4 * size_t(t + i * T), k, v[i]);
-        }
+        for (int i = 0; i < kHeld; ++i) load4<VEC>(src, j0 + 4 * (t + i * T), k, v[i]);
 #pragma unroll
-        for (int i = 0; i < kHeld; ++i) {
-            if (size_t(4 * T) * i >= k) break;
-            most = katsu_larger4(most, v[i]);
-        }
-        for (size_t j = 4 * size_t(kHeld * T); j < k; j += 4 * kHeld * T) {
-            float w[kHeld][4];
-#pragma unroll
-            for (int i = 0; i < kHeld; ++i) load4<VEC>(src, j + 4 * size_t(t + i * T), k, w[i]);
-#pragma unroll
-            for (int i = 0; i < kHeld; ++i) most = katsu_larger4(most, w[i]);
-        }
-        most = katsu_larger_of_warp(most);
-        if (T > 32) {  // (two sets of places: the row behind this one does not wait for its readers)
-            if ((threadIdx.x & 31) == 0) sh[turn][threadIdx.x >> 5] = most;
-            __syncthreads();
-#pragma unroll
-            for (int w = 0; w < T / 32; ++w) most = katsu_larger(most, sh[turn][w]);
-        }
-        const KatsuInt8Scale s = katsu_int8_scale(most);
-        if (t == 0) scale[row] = s.scale;
-        unsigned *dst = reinterpret_cast<unsigned *>(q + row * pitch);
-#pragma unroll
-        for (int i = 0; i < kHeld; ++i) {
-            const size_t j = 4 * size_t(t + i * T);
-            if (j < pitch) dst[j / 4] = katsu_int8_pack(v[i], s);
-        }
-        for (size_t j = 4 * size_t(kHeld * T); j < pitch; j += 4 * kHeld * T) {
-            float w[kHeld][4];
-#pragma unroll
-            for (int i = 0; i < kHeld; ++i) load4<VEC>(src, j + 4 * size_t(t + i * T), k, w[i]);
-#pragma unroll
-            for (int i = 0; i < kHeld; ++i)
-                if (j + 4 * size_t(t + i * T) < pitch) dst[(j + 4 * size_t(t + i * T)) / 4] = katsu_int8_pack(w[i], s);
-        }
+        for (int i = 0; i < kHeld; ++i) most = katsu_larger4(most, v[i]);
     }
+    float v[kHeld][4];
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) load4<VEC>(src, twice + 4 * (t + i * T), k, v[i]);
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) most = katsu_larger4(most, v[i]);
+    most = katsu_larger_of_warp(most);
+    if (T > 32) {
+        if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = most;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < T / 32; ++w) most = katsu_larger(most, sh[w]);
+    }
+    const KatsuInt8Scale s = katsu_int8_scale(most);
+    if (t == 0) scale[row] = s.scale;
+    unsigned *dst = reinterpret_cast<unsigned *>(q + row * pitch);
+    bool sure = true;
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+        const size_t j = twice + 4 * (t + i * T);
+        const unsigned out = katsu_int8_pack(v[i], s, &sure);
+        if (j < pitch) dst[j / 4] = out;
+    }
+    for (size_t j0 = 0; j0 < twice; j0 += batch) {
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) load4<VEC>(src, j0 + 4 * (t + i * T), k, v[i]);
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) dst[(j0 + 4 * (t + i * T)) / 4] = katsu_int8_pack(v[i], s, &sure);
+    }
+    if (!sure)  // this thread's pieces once more, by the definition
+        for (size_t j = 4 * t; j < pitch; j += 4 * T) {
+            float w[4];
+            load4<VEC>(src, j, k, w);
+            dst[j / 4] = katsu_int8_pack_exactly(w, s);
+        }
 }
 
 // Largest magnitude of every column of w [k, n], as bits, over k rows cut into gridDim.y pieces; `most` starts at zero.
@@ -122,7 +122,10 @@ __global__ void __launch_bounds__(256) quantize_columns_kernel(const float *__re
         if (p >= pitch) continue;
         const float v[4] = {tile[4 * lane][warp + 8 * i], tile[4 * lane + 1][warp + 8 * i], tile[4 * lane + 2][warp + 8 * i],
                             tile[4 * lane + 3][warp + 8 * i]};
-        *reinterpret_cast<unsigned *>(q + col * pitch + p) = katsu_int8_pack(v, s);
+        bool sure = true;
+        unsigned out = katsu_int8_pack(v, s, &sure);
+        if (!sure) out = katsu_int8_pack_exactly(v, s);
+        *reinterpret_cast<unsigned *>(q + col * pitch + p) = out;
     }
 }
 
@@ -130,15 +133,14 @@ __global__ void __launch_bounds__(256) quantize_columns_kernel(const float *__re
 
 int32_t katsu_int8_quantize(katsu_cuda_ctx *ctx, const float *x, int8_t *q, float *scale, size_t m, size_t k) {
     const bool vec = k % 4 == 0 && (reinterpret_cast<uintptr_t>(x) & 15u) == 0;
-    const bool small = k <= 1024, medium = k <= 4096;
-    const unsigned threads = medium ? 256 : 512;
     // a block to every row: the hardware hands them out as others end, and the rounds of one hide behind the loads of others
-    const size_t need = small ? katsu_div_up(m, 8) : m, most = 0x7fffffff;
+    const bool small = k <= 1024, medium = k <= 8192;
+    const unsigned threads = medium ? 256 : 512;
     auto kernel = small    ? (vec ? quantize_rows_kernel<32, 8, true> : quantize_rows_kernel<32, 8, false>)
-                  : medium ? (vec ? quantize_rows_kernel<256, 4, true> : quantize_rows_kernel<256, 4, false>)
-                           : (vec ? quantize_rows_kernel<512, 4, true> : quantize_rows_kernel<512, 4, false>);
+                  : medium ? (vec ? quantize_rows_kernel<256, 8, true> : quantize_rows_kernel<256, 8, false>)
+                           : (vec ? quantize_rows_kernel<512, 8, true> : quantize_rows_kernel<512, 8, false>);
     KATSU_TRY(katsu_prepare_kernel(ctx, (const void *)kernel, 0));
-    return katsu_launch_chained(ctx, kernel, (unsigned)(need < most ? need : most), threads, 0, 1, x, q, scale, m, k,
+    return katsu_launch_chained(ctx, kernel, (unsigned)(small ? katsu_div_up(m, 8) : m), threads, 0, 1, x, q, scale, m, k,
                                 katsu_int8_pitch(k));
 }
 

@@ -74,7 +74,10 @@ __global__ void __launch_bounds__(kWarps * 32) int8_rows_kernel(const float *__r
             for (int j = 4 * threadIdx.x; j < pitch; j += 4 * kWarps * 32) {
                 float v[4] = {0.f, 0.f, 0.f, 0.f};
                 if (i < m) load4(i, j, v);
-                *reinterpret_cast<unsigned *>(tokens + i * pitch + j) = katsu_int8_pack(v, s);
+                bool sure = true;
+                unsigned out = katsu_int8_pack(v, s, &sure);
+                if (!sure) out = katsu_int8_pack_exactly(v, s);
+                *reinterpret_cast<unsigned *>(tokens + i * pitch + j) = out;
             }
         }
     } else {

@@ -733,7 +733,6 @@ __global__ void __launch_bounds__(kFoldThreads) norm_fold_kernel(const __grid_co
 
 template <typename... Params, typename... Args>
 int32_t start(katsu_cuda_ctx *ctx, void (*kernel)(Params...), unsigned grid, unsigned block, Args &&...args) {
-    KATSU_TRY(katsu_prepare_kernel(ctx, (const void *)kernel, 0));
     return katsu_launch_chained(ctx, kernel, grid, block, 0, 1, args...);
 }
 
@@ -751,7 +750,7 @@ int32_t start_forward_of(katsu_cuda_ctx *ctx, const Forward &p, bool wide, bool 
                   : rows == BY_RING  ? norm_fwd_kernel<16, true, BY_RING, LAYER>
                   : rows == OF_BLOCK ? (vec ? norm_fwd_kernel<16, true, OF_BLOCK, LAYER> : norm_fwd_kernel<16, false, OF_BLOCK, LAYER>)
                                      : (vec ? norm_fwd_kernel<16, true, OF_WARP, LAYER> : norm_fwd_kernel<16, false, OF_WARP, LAYER>);
-    KATSU_TRY(katsu_prepare_kernel(ctx, (const void *)kernel, smem));
+    if (smem) KATSU_TRY(katsu_prepare_kernel(ctx, (const void *)kernel, smem));
     return katsu_launch_chained(ctx, kernel, grid, block, smem, 1, p, slab);
 }
 
@@ -822,7 +821,7 @@ template <Sums MODE>
 int32_t start_backward_of(katsu_cuda_ctx *ctx, const Backward &p, const BackwardShape &s, size_t blocks) {
     auto kernel = s.cluster > 1 ? norm_bwd_kernel<MODE, true, true>
                   : s.slab.arrays ? norm_bwd_kernel<MODE, true, false> : norm_bwd_kernel<MODE, false, false>;
-    KATSU_TRY(katsu_prepare_kernel(ctx, (const void *)kernel, s.smem));
+    if (s.smem) KATSU_TRY(katsu_prepare_kernel(ctx, (const void *)kernel, s.smem));
     return katsu_launch_chained(ctx, kernel, (unsigned)blocks * s.cluster, s.threads, s.smem, s.cluster, p, s.slab);
 }
 

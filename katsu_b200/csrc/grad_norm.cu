@@ -269,7 +269,6 @@ int32_t run(katsu_cuda_ctx *ctx, What what, const float *const *grads, float *co
     float *scratch = nullptr;
     KATSU_TRY(katsu_scratch(ctx, sums * 2 + 2, &scratch));
     double *partial = reinterpret_cast<double *>(scratch + 2);
-    KATSU_TRY(katsu_prepare_kernel(ctx, (const void *)squares_kernel<N>, 0));
     int parts = 0;
     for (size_t i = 0; i < tensors;) {
         i = take(&t, grads, dst, counts, i, tensors);
@@ -281,12 +280,10 @@ int32_t run(katsu_cuda_ctx *ctx, What what, const float *const *grads, float *co
     const bool between = what != NORM_ONLY && blocks > size_t(ctx->num_sms) * 8;
     float *factor = between ? scratch : nullptr;
     if (what == NORM_ONLY || between || parts == 0) {
-        KATSU_TRY(katsu_prepare_kernel(ctx, (const void *)norm_kernel, 0));
         KATSU_TRY(katsu_launch_chained(ctx, norm_kernel, 1, kThreads, 0, 1, partial, parts, max_norm, norm, factor));
     }
     if (what == NORM_ONLY) return KATSU_OK;
     auto kernel = what == CLIPPED ? apply_kernel<CLIP, N> : apply_kernel<STEP, N>;
-    KATSU_TRY(katsu_prepare_kernel(ctx, (const void *)kernel, 0));
     for (size_t i = 0; i < tensors;) {
         const bool first = i == 0;
         i = take(&t, grads, dst, counts, i, tensors);

@@ -139,7 +139,6 @@ int32_t katsu_int8_quantize(katsu_cuda_ctx *ctx, const float *x, int8_t *q, floa
     auto kernel = small    ? (vec ? quantize_rows_kernel<32, 8, true> : quantize_rows_kernel<32, 8, false>)
                   : medium ? (vec ? quantize_rows_kernel<256, 8, true> : quantize_rows_kernel<256, 8, false>)
                            : (vec ? quantize_rows_kernel<512, 8, true> : quantize_rows_kernel<512, 8, false>);
-    KATSU_TRY(katsu_prepare_kernel(ctx, (const void *)kernel, 0));
     return katsu_launch_chained(ctx, kernel, (unsigned)(small ? katsu_div_up(m, 8) : m), threads, 0, 1, x, q, scale, m, k,
                                 katsu_int8_pitch(k));
 }

@@ -274,8 +274,8 @@ class Context:
 
     # -- norms around a block -----------------------------------------------------
     def block_norm_fwd(self, x, h, gate, gate_rows, post_w, post_b, pre_w, pre_b, scale, eps, kind, r, n, rows, cols) -> None:
-        self.call("katsu_cuda_block_norm_fwd", x, h, gate, gate_rows, post_w, post_b, pre_w, pre_b, scale, eps, kind, r, n,
-                  rows, cols)
+        check(self.lib.katsu_cuda_block_norm_fwd(self.handle, x, h, gate, gate_rows, post_w, post_b, pre_w, pre_b, scale, eps,
+                                                 kind, r, n, rows, cols))
 
     def block_norm_bwd(self, r, h, gate, gate_rows, post_w, post_b, pre_w, scale, eps, kind, dr, dn, dx, dh, dgate, dpost_w,
                        dpost_b, dpre_w, dpre_b, rows, cols, accumulate=0) -> None:
@@ -299,7 +299,7 @@ class Context:
         self.call("katsu_cuda_int8_matmul", xq, xs, wq, ws, bias, y, m, k, n)
 
     def int8_linear(self, x, wq, ws, bias, y, m, k, n) -> None:
-        self.call("katsu_cuda_int8_linear", x, wq, ws, bias, y, m, k, n)
+        check(self.lib.katsu_cuda_int8_linear(self.handle, x, wq, ws, bias, y, m, k, n))
 
     # -- all gradients of a step --------------------------------------------------------
     # (arrays of 64-bit words take a tenth of the time of ctypes arrays filled one by one: 240 tensors, 90 us a call)

@@ -237,6 +237,23 @@ struct Rounds {
     }
 };
 
+// The ring leaves little of the SM's memory to L1, so what every row needs is kept beside it: a copy of `width` weights, if
+// there are any, in shared memory at `to`, which moves behind it.
+template <bool VEC>
+__device__ __forceinline__ const float *keep_weights(const float *weights, float *&to, int width) {
+    const float *copy = to;
+    if (weights != nullptr) {
+        if (VEC) {
+            for (int j = 4 * threadIdx.x; j < width; j += 4 * blockDim.x)
+                *reinterpret_cast<float4 *>(to + j) = __ldg(reinterpret_cast<const float4 *>(weights + j));
+        } else {
+            for (int j = threadIdx.x; j < width; j += blockDim.x) to[j] = __ldg(weights + j);
+        }
+        to += width;
+    }
+    return copy;
+}
+
 // How a row's threads find each other and its values: a warp's own row, a block's by plain loads, a block's by the ring.
 enum Rows { OF_WARP, OF_BLOCK, BY_RING };
 
@@ -261,6 +278,12 @@ __global__ void __launch_bounds__(kMostThreads) norm_fwd_kernel(const __grid_con
     const bool gate_each = p.gate && p.rows_per_gate == 1;
     unsigned long long row = (unsigned long long)blockIdx.x * per_block + (WARP ? threadIdx.x >> 5 : 0);
     const unsigned long long step = (unsigned long long)gridDim.x * per_block;
+    float *keep_at = ring_data + (RING ? size_t(slab.stages) * slab.arrays * slab.width : 0);
+    const float *post_w = RING ? keep_weights<VEC>(p.post_w, keep_at, p.cols) : p.post_w;
+    const float *post_b = RING ? keep_weights<VEC>(p.post_b, keep_at, p.cols) : p.post_b;
+    const float *pre_w = RING ? keep_weights<VEC>(p.pre_w, keep_at, p.cols) : p.pre_w;
+    const float *pre_b = RING ? keep_weights<VEC>(p.pre_b, keep_at, p.cols) : p.pre_b;
+    if (RING) __syncthreads();
     auto fetch = [&](int stage, unsigned long long r) {
         ring.fetch(stage, {p.x, p.h, gate_each ? p.gate : nullptr}, r * size_t(p.cols), p.cols);
     };
@@ -296,13 +319,13 @@ __global__ void __launch_bounds__(kMostThreads) norm_fwd_kernel(const __grid_con
                 }
                 if (LAYER) row_of.center(u, m[0]);
                 row_of.each([&](int i) { sq[0] += u[i] * u[i]; });
-                row_of.load(w, p.post_w);
+                row_of.load(w, post_w);
                 rounds.sums(sq);
                 refilled();
                 const float rstd = 1.f / sqrtf(sq[0] * inv + p.eps);
                 row_of.each([&](int i) { u[i] *= rstd * w[i]; });
                 if (p.post_b) {
-                    row_of.load(w, p.post_b);
+                    row_of.load(w, post_b);
                     row_of.each([&](int i) { u[i] += w[i]; });
                 }
             }
@@ -321,13 +344,13 @@ __global__ void __launch_bounds__(kMostThreads) norm_fwd_kernel(const __grid_con
             }
             if (LAYER) row_of.center(v, m[0]);
             row_of.each([&](int i) { sq[0] += v[i] * v[i]; });
-            row_of.load(w, p.pre_w);
+            row_of.load(w, pre_w);
             rounds.sums(sq);
             refilled();
             const float rstd = 1.f / sqrtf(sq[0] * inv + p.eps);
             row_of.each([&](int i) { v[i] *= rstd * w[i]; });
             if (p.pre_b) {
-                row_of.load(w, p.pre_b);
+                row_of.load(w, pre_b);
                 row_of.each([&](int i) { v[i] += w[i]; });
             }
             row_of.store(v, p.n + at, false);
@@ -388,6 +411,15 @@ __global__ void __launch_bounds__(kMostThreads) norm_bwd_kernel(const __grid_con
     unsigned long long begin, end;
     rows_of_block(p, block, blocks, &begin, &end);
     const bool gate_each = p.gate && p.rows_per_gate == 1;
+    const bool gate_bias = BIAS && p.post_b && p.gate;
+    const float *post_w = p.post_w + c0, *pre_w = p.pre_w + c0, *post_b = p.post_b + c0;
+    if (RING) {
+        float *keep_at = ring_data + size_t(slab.stages) * slab.arrays * slab.width;
+        post_w = keep_weights<VEC>(p.post_w ? post_w : nullptr, keep_at, width);
+        pre_w = keep_weights<VEC>(p.dn ? pre_w : nullptr, keep_at, width);
+        post_b = keep_weights<VEC>(gate_bias ? post_b : nullptr, keep_at, width);
+        __syncthreads();
+    }
     auto fetch = [&](int stage, unsigned long long row) {
         ring.fetch(stage, {p.r, p.h, p.dn, p.dr, gate_each ? p.gate : nullptr}, row * size_t(p.cols) + c0, width);
     };
@@ -453,7 +485,7 @@ __global__ void __launch_bounds__(kMostThreads) norm_bwd_kernel(const __grid_con
         }
         float a[N], v[4] = {0.f, 0.f, 0.f, 0.f};  // squares of r and h, a (r - m) and a
         if (p.dn) {
-            row_of.load(w, p.pre_w + c0);
+            row_of.load(w, pre_w);
             row_of.each([&](int i) {
                 a[i] = dn[i] * w[i];
                 v[0] += r[i] * r[i];
@@ -487,7 +519,7 @@ __global__ void __launch_bounds__(kMostThreads) norm_bwd_kernel(const __grid_con
             b[i] = p.gate ? gate[i] * dr[i] : dr[i];
         });
         if (p.post_w) {
-            row_of.load(w, p.post_w + c0);
+            row_of.load(w, post_w);
             row_of.each([&](int i) {
                 h[i] *= hs;
                 sum_post_w[i] += b[i] * h[i];
@@ -497,9 +529,9 @@ __global__ void __launch_bounds__(kMostThreads) norm_bwd_kernel(const __grid_con
                 if constexpr (LAYER) q[1] += b[i];
             });
             if (p.gate) {
-                if (BIAS && p.post_b) {
+                if (gate_bias) {
                     float bias[N];
-                    row_of.load(bias, p.post_b + c0);
+                    row_of.load(bias, post_b);
                     row_of.each([&](int i) { dr[i] *= h[i] * w[i] + bias[i]; });
                 } else {
                     row_of.each([&](int i) { dr[i] *= h[i] * w[i]; });
@@ -759,28 +791,29 @@ int32_t start_forward(katsu_cuda_ctx *ctx, const Forward &p) {
     const bool vec = pieces(p.cols, {p.x, p.h, p.gate, p.post_w, p.post_b, p.pre_w, p.pre_b, p.r, p.n});
     const unsigned long long sms = ctx->num_sms;
     if (p.cols > kMostThreads * (vec ? 32 : 16))
-        return start(ctx, norm_fwd_long_kernel<LAYER>, unsigned(p.rows < sms * 8 ? p.rows : sms * 8), kThreads, p);
+        return start(ctx, norm_fwd_long_kernel<LAYER>, unsigned(p.rows < sms * 4 ? p.rows : sms * 4), kThreads, p);
     // 16 values a thread, 32 where that would take more than 512 threads; up to 512 values are one warp's
     const bool wide = p.cols > kMostThreads * 16;
     Rows rows = p.cols <= 512 ? OF_WARP : OF_BLOCK;
     const unsigned threads = rows == OF_WARP ? 128 : unsigned(katsu_div_up(katsu_div_up(p.cols, wide ? 32 : 16), 32)) * 32;
     const unsigned long long need = rows == OF_WARP ? katsu_div_up(p.rows, 4) : p.rows;
-    unsigned long long most = sms * (2048 / threads);
+    unsigned resident = 512 / threads;  // registers: 512 threads to an SM
+    if (resident > 8) resident = 8;
+    const unsigned long long most = sms * resident;
     Slab slab = {};
     size_t smem = 0;
     // A block that takes several rows brings them ahead; a single one arrives sooner by plain loads (one row of 4096: 5.6 us).
-    unsigned resident = 512 / threads;
-    if (resident > 8) resident = 8;
     if (vec && rows == OF_BLOCK && !wide && p.rows > sms * resident) {
         slab.width = p.cols;
         slab.arrays = 1 + (p.h != nullptr) + (p.gate && p.rows_per_gate == 1);
-        const size_t row = size_t(slab.arrays) * p.cols * sizeof(float), room = kRoom / resident - 2048;
+        const size_t row = size_t(slab.arrays) * p.cols * sizeof(float);
+        const size_t kept = size_t((p.post_w != nullptr) + (p.post_b != nullptr) + (p.pre_w != nullptr) + (p.pre_b != nullptr)) * p.cols * sizeof(float);
+        const size_t room = kRoom / resident - 2048 > kept ? kRoom / resident - 2048 - kept : 0;
         const size_t stages = room / row < kMostStages ? room / row : kMostStages;
         if (stages >= 2) {
             rows = BY_RING;
             slab.stages = int(stages);
-            smem = slab.stages * row;
-            most = sms * resident;
+            smem = slab.stages * row + kept;
         }
     }
     const unsigned grid = unsigned(need < most ? need : most);
@@ -809,9 +842,11 @@ BackwardShape backward_shape(const katsu_cuda_ctx *ctx, const Backward &p, std::
     if (resident > 8) resident = 8;
     if (vec) {
         s.slab.arrays = 1 + (p.h != nullptr) + (p.dn != nullptr) + (p.dr != nullptr) + (p.gate && p.rows_per_gate == 1);
-        const size_t row = size_t(s.slab.arrays) * s.slab.width * sizeof(float), room = kRoom / resident - 2048;
+        const size_t row = size_t(s.slab.arrays) * s.slab.width * sizeof(float);
+        const size_t kept = size_t((p.post_w != nullptr) + (p.dn != nullptr) + (p.post_b && p.gate)) * s.slab.width * sizeof(float);
+        const size_t room = kRoom / resident - 2048 - kept;
         s.slab.stages = int(room / row < kMostStages ? room / row : kMostStages);
-        s.smem = s.slab.stages * row;
+        s.smem = s.slab.stages * row + kept;
     }
     s.most_blocks = size_t(ctx->num_sms) * resident / s.cluster;
     return s;

@@ -3,8 +3,8 @@
 //   norm = sqrt(sum over all tensors of g^2)      c = max_norm / norm where that is below 1      g' = c g      w -= lr (c g)
 //
 // Two launches (and one more pair for every 512 tensors): the first leaves a partial sum of squares a block, the blocks of the
-// second fold these for themselves and then scale or step.  From 1200 blocks on a launch between the two folds once for all, and
-// the blocks of the last are handed out as others end.  The addresses travel as a kernel
+// second fold these for themselves and then scale or step.  With more blocks than are resident at once a launch between the two
+// folds once for all.  The addresses travel as a kernel
 // parameter, so nothing on the host has to outlive the call and a captured call keeps them.
 //
 // Squares are summed in 64 bits: 1e-30 and 1e30 neither vanish nor overflow, the sum of 1e9 values keeps more bits than the
@@ -85,8 +85,8 @@ __device__ __forceinline__ unsigned lead_of(const float *p) { return unsigned(re
 
 // partial[block] = the block's sum of squares.
 template <int N>
-__global__ void __launch_bounds__(kThreads) squares_kernel(const __grid_constant__ Tensors<N> t, double *partial) {
-    launch_next();
+__global__ void __launch_bounds__(kThreads) squares_kernel(const __grid_constant__ Tensors<N> t, double *partial, int waves) {
+    if (!waves) launch_next();
     launch_wait();
     double acc = 0.0;
     // runs differ by one unit, so no block has a batch more to do than the others
@@ -162,7 +162,7 @@ __device__ __forceinline__ float applied(float g, float w, float c, float lr) {
 template <Apply OP, int N>
 __global__ void __launch_bounds__(kThreads) apply_kernel(const __grid_constant__ Tensors<N> t, const double *partial, int parts,
                                                          const float *factor, float max_norm, float lr, float *norm) {
-    launch_next();
+    if (factor == nullptr) launch_next();  // (else the grid goes in waves)
     launch_wait();
     const unsigned begin_unit = (gridDim.x - 1 - blockIdx.x) * kBatch;
     Batch b = first_batch(t, begin_unit, min(begin_unit + kBatch, t.first[t.tensors]));
@@ -269,15 +269,16 @@ int32_t run(katsu_cuda_ctx *ctx, What what, const float *const *grads, float *co
     float *scratch = nullptr;
     KATSU_TRY(katsu_scratch(ctx, sums * 2 + 2, &scratch));
     double *partial = reinterpret_cast<double *>(scratch + 2);
+    const bool waves = blocks > size_t(ctx->num_sms) * 4;  // (blocks of the last kernel that are resident at once)
     int parts = 0;
     for (size_t i = 0; i < tensors;) {
         i = take(&t, grads, dst, counts, i, tensors);
         if (t.tensors == 0) break;
         const unsigned grid = std::min(blocks_for(t.first[t.tensors]), most);
-        KATSU_TRY(katsu_launch_chained(ctx, squares_kernel<N>, grid, kThreads, 0, 1, t, partial + parts));
+        KATSU_TRY(katsu_launch(ctx, !waves, squares_kernel<N>, grid, kThreads, 0, 1, t, partial + parts, waves ? 1 : 0));
         parts += (int)grid;
     }
-    const bool between = what != NORM_ONLY && blocks > size_t(ctx->num_sms) * 8;
+    const bool between = what != NORM_ONLY && waves;
     float *factor = between ? scratch : nullptr;
     if (what == NORM_ONLY || between || parts == 0) {
         KATSU_TRY(katsu_launch_chained(ctx, norm_kernel, 1, kThreads, 0, 1, partial, parts, max_norm, norm, factor));
@@ -288,7 +289,7 @@ int32_t run(katsu_cuda_ctx *ctx, What what, const float *const *grads, float *co
         const bool first = i == 0;
         i = take(&t, grads, dst, counts, i, tensors);
         if (t.tensors == 0) break;
-        KATSU_TRY(katsu_launch_chained(ctx, kernel, blocks_for(t.first[t.tensors]), kThreads, 0, 1, t, partial, parts, factor,
+        KATSU_TRY(katsu_launch(ctx, !waves, kernel, blocks_for(t.first[t.tensors]), kThreads, 0, 1, t, partial, parts, factor,
                                        max_norm, lr, first ? norm : nullptr));
     }
     return KATSU_OK;

@@ -293,6 +293,7 @@ int32_t many(katsu_cuda_ctx *ctx, const Plan &plan, int *partial, const int8_t *
     if (plan.splits == 1) return KATSU_OK;
     size_t blocks = katsu_div_up(m * n, 256);
     if (blocks > size_t(ctx->num_sms) * 8) blocks = size_t(ctx->num_sms) * 8;
+    KATSU_TRY(katsu_prepare_kernel(ctx, (const void *)int8_fold_kernel, 0));
     return katsu_launch_chained(ctx, int8_fold_kernel, (unsigned)blocks, 256, 0, 1, partial, plan.splits, xs, ws, bias, y, m * n,
                                 (unsigned)n);
 }

@@ -1,6 +1,6 @@
 // Matrices to 8 bits: rows of x (one scale a token) and columns of w (one scale an output channel, kept transposed).
 //
-// Rows: a warp (up to 1024 values) or a block of 256 (up to 8192) or 512 threads takes a row and holds its last 32 values a
+// Rows: a warp (up to 1024 values) or a block of 256 (up to 8192) or 512 threads takes a row and holds its last 32 (16) values a
 // thread in registers between the largest magnitude and the quotients; what lies in front is read again, from L2.  Bound: HBM, 4 bytes
 // in and 1 out a value.
 #include "int8.cuh"
@@ -20,12 +20,12 @@ __device__ __forceinline__ void load4(const float *row, size_t j, size_t k, floa
 }
 
 // T threads to a row, each of which holds kHeld 16-byte pieces: the row's last ones, loaded behind what is read twice, so that
-// their registers are free until then.
-template <int T, int kHeld, bool VEC>
+// their registers are free until then.  WAVES: more blocks than are resident at once (see katsu_int8_quantize).
+template <int T, int kHeld, bool VEC, bool WAVES>
 __global__ void __launch_bounds__(T < 256 ? 256 : T) quantize_rows_kernel(const float *__restrict__ x, int8_t *q, float *scale,
                                                                           unsigned long long rows, size_t k, size_t pitch) {
     __shared__ float sh[T < 256 ? 1 : T / 32];
-    launch_next();
+    if (!WAVES) launch_next();
     launch_wait();
     constexpr int per_block = T < 256 ? 256 / T : 1, batch = 4 * T * kHeld;
     const int t = threadIdx.x % T;
@@ -131,16 +131,24 @@ __global__ void __launch_bounds__(256) quantize_columns_kernel(const float *__re
 
 }  // namespace
 
+template <bool VEC, bool WAVES>
+static void (*rows_kernel(size_t k))(const float *, int8_t *, float *, unsigned long long, size_t, size_t) {
+    return k <= 1024 ? quantize_rows_kernel<32, 8, VEC, WAVES>
+           : k <= 8192 ? quantize_rows_kernel<256, 8, VEC, WAVES> : quantize_rows_kernel<512, 4, VEC, WAVES>;
+}
+
+// A row to a warp or block.  Few rows: the launch is chained, like that of the product behind it, and takes the largest
+// shared-memory partition as that does.  More rows than go round at once: the hardware hands them out as others end, the rounds
+// of one hide behind the loads of others, and the kernel wants its L1 for the loads in flight (8192 x 8192: 53 us, with the
+// largest partition 80).
 int32_t katsu_int8_quantize(katsu_cuda_ctx *ctx, const float *x, int8_t *q, float *scale, size_t m, size_t k) {
     const bool vec = k % 4 == 0 && (reinterpret_cast<uintptr_t>(x) & 15u) == 0;
-    // a block to every row: the hardware hands them out as others end, and the rounds of one hide behind the loads of others
-    const bool small = k <= 1024, medium = k <= 8192;
-    const unsigned threads = medium ? 256 : 512;
-    auto kernel = small    ? (vec ? quantize_rows_kernel<32, 8, true> : quantize_rows_kernel<32, 8, false>)
-                  : medium ? (vec ? quantize_rows_kernel<256, 8, true> : quantize_rows_kernel<256, 8, false>)
-                           : (vec ? quantize_rows_kernel<512, 8, true> : quantize_rows_kernel<512, 8, false>);
-    return katsu_launch_chained(ctx, kernel, (unsigned)(small ? katsu_div_up(m, 8) : m), threads, 0, 1, x, q, scale, m, k,
-                                katsu_int8_pitch(k));
+    const size_t blocks = k <= 1024 ? katsu_div_up(m, 8) : m;
+    const bool waves = blocks > size_t(ctx->num_sms) * 2;
+    auto kernel = waves ? (vec ? rows_kernel<true, true>(k) : rows_kernel<false, true>(k))
+                         : (vec ? rows_kernel<true, false>(k) : rows_kernel<false, false>(k));
+    if (!waves) KATSU_TRY(katsu_prepare_kernel(ctx, (const void *)kernel, 0));
+    return katsu_launch(ctx, !waves, kernel, (unsigned)blocks, k <= 8192 ? 256u : 512u, 0, 1, x, q, scale, m, k, katsu_int8_pitch(k));
 }
 
 extern "C" int32_t katsu_cuda_int8_row_bytes(size_t k, size_t *out_bytes) {

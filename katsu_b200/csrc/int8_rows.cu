@@ -152,7 +152,7 @@ int32_t katsu_int8_few(katsu_cuda_ctx *ctx, const float *x, const int8_t *xq, co
     while (share < kWarps && pairs * share * 2 <= warps) share *= 2;
     const size_t need = katsu_div_up(pairs, kWarps / share);
     size_t fit = (size_t(224) * 1024) / (smem + 2048);  // blocks that an SM holds
-    if (fit > 4) fit = 4;
+    if (fit > 3) fit = 3;  // (and three by their registers)
     const size_t most = size_t(ctx->num_sms) * fit;
     return katsu_launch_chained(ctx, kernel, (unsigned)(need < most ? need : most), kWarps * 32, smem, 1, x, xq, xs, wq, ws, bias, y,
                                 (int)m, (int)k, (int)n, (int)pitch, share);

@@ -19,9 +19,11 @@ __device__ __forceinline__ void launch_next() { asm volatile("griddepcontrol.lau
 // does when it is idle.
 int32_t katsu_prepare_kernel(katsu_cuda_ctx *ctx, const void *kernel, size_t smem);
 
+// early: the launch may start under its predecessor's end.  Only for grids whose blocks are all resident at once: one that the
+// hardware hands out in waves is launched plainly, and its blocks do not call launch_next().
 template <typename... Params, typename... Args>
-int32_t katsu_launch_chained(katsu_cuda_ctx *ctx, void (*kernel)(Params...), unsigned grid, unsigned block, size_t smem,
-                             unsigned cluster, Args &&...args) {
+int32_t katsu_launch(katsu_cuda_ctx *ctx, bool early, void (*kernel)(Params...), unsigned grid, unsigned block, size_t smem,
+                     unsigned cluster, Args &&...args) {
     cudaLaunchConfig_t config;
     memset(&config, 0, sizeof(config));
     config.gridDim = dim3(grid, 1, 1);
@@ -30,15 +32,17 @@ int32_t katsu_launch_chained(katsu_cuda_ctx *ctx, void (*kernel)(Params...), uns
     config.stream = ctx->stream;
     cudaLaunchAttribute attributes[2];
     memset(attributes, 0, sizeof(attributes));
-    attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attributes[0].val.programmaticStreamSerializationAllowed = 1;
     config.attrs = attributes;
-    config.numAttrs = 1;
+    if (early) {
+        attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attributes[0].val.programmaticStreamSerializationAllowed = 1;
+        config.numAttrs = 1;
+    }
     if (cluster > 1) {
-        attributes[1].id = cudaLaunchAttributeClusterDimension;
-        attributes[1].val.clusterDim.x = cluster;
-        attributes[1].val.clusterDim.y = attributes[1].val.clusterDim.z = 1;
-        config.numAttrs = 2;
+        cudaLaunchAttribute &of_cluster = attributes[config.numAttrs++];
+        of_cluster.id = cudaLaunchAttributeClusterDimension;
+        of_cluster.val.clusterDim.x = cluster;
+        of_cluster.val.clusterDim.y = of_cluster.val.clusterDim.z = 1;
     }
     const cudaError_t err = cudaLaunchKernelEx(&config, kernel, static_cast<Params>(args)...);
     ctx->launches += 1;
@@ -47,4 +51,10 @@ int32_t katsu_launch_chained(katsu_cuda_ctx *ctx, void (*kernel)(Params...), uns
         return katsu_set_error(KATSU_ERR_CUDA, "kernel launch failed: %s", cudaGetErrorString(err));
     }
     return KATSU_OK;
+}
+
+template <typename... Params, typename... Args>
+int32_t katsu_launch_chained(katsu_cuda_ctx *ctx, void (*kernel)(Params...), unsigned grid, unsigned block, size_t smem,
+                             unsigned cluster, Args &&...args) {
+    return katsu_launch(ctx, true, kernel, grid, block, smem, cluster, static_cast<Args &&>(args)...);
 }

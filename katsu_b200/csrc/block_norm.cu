@@ -18,6 +18,7 @@
 #include <math.h>
 
 #include <initializer_list>
+#include <type_traits>
 
 #include "common.cuh"
 #include "launch.cuh"
@@ -33,8 +34,7 @@ struct Forward {
     float *r, *n;
     float scale, eps;
     unsigned long long rows, rows_per_gate;
-    int cols;
-    int *status;
+    int cols, ahead;
 };
 
 // Sums over rows, in the order of the partial results.
@@ -78,43 +78,47 @@ __device__ __forceinline__ void block_sums(float (&v)[K], float (*sh)[32]) {
 }
 
 // ---- rows that a block holds ------------------------------------------------------------------------------------------
-// N values of a row for each of T threads, in pieces of four (VEC: 16-byte accesses; the row is whole pieces at 16-byte
-// addresses) or one, the pieces of a thread T pieces apart.  The pieces that lie in the row are a thread's first `live` ones;
-// the others are loaded as zeros and not stored.
-template <int N, bool VEC>
+// N values of a row for each of T threads, in pieces of one (SINGLES) or four (WHOLE: 16-byte accesses; the row is whole pieces
+// at 16-byte addresses), the pieces of a thread T pieces apart.  The pieces that lie in the row are a thread's first `live` ones;
+// the others are loaded as zeros and not stored.  FULL: whole pieces, and every thread has all of them.
+enum Pieces { SINGLES, WHOLE, FULL };
+
+template <int N, Pieces PIECES>
 struct Row {
+    static constexpr bool VEC = PIECES != SINGLES;
     static constexpr int W = VEC ? 4 : 1, P = N / W;
     int t, T, live;
     __device__ __forceinline__ Row(int t, int T, int width) : t(t), T(T) {
         const int last = (width + W - 1) / W - 1 - t;  // pieces behind this thread's first one
         live = last < 0 ? 0 : last / T + 1;
     }
+    __device__ __forceinline__ bool in(int piece) const { return PIECES == FULL || piece < live; }
     template <typename F>
     __device__ __forceinline__ void each(F f) const {
 #pragma unroll
         for (int i = 0; i < N; ++i) f(i);
     }
-    // Takes a row's mean off, behind whose end zeros stay.
+    // Takes a mean off, behind the row's end zeros stay.
     __device__ __forceinline__ void center(float (&v)[N], float mean) const {
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = i / W < live ? v[i] - mean : 0.f;
+        for (int i = 0; i < N; ++i) v[i] = in(i / W) ? v[i] - mean : 0.f;
     }
     __device__ __forceinline__ void load(float (&v)[N], const float *at) const {
         at += W * t;
 #pragma unroll
         for (int q = 0; q < P; ++q, at += W * T)
             if constexpr (VEC) {
-                const float4 f = q < live ? *reinterpret_cast<const float4 *>(at) : make_float4(0.f, 0.f, 0.f, 0.f);
+                const float4 f = in(q) ? *reinterpret_cast<const float4 *>(at) : make_float4(0.f, 0.f, 0.f, 0.f);
                 v[4 * q] = f.x; v[4 * q + 1] = f.y; v[4 * q + 2] = f.z; v[4 * q + 3] = f.w;
             } else {
-                v[q] = q < live ? *at : 0.f;
+                v[q] = in(q) ? *at : 0.f;
             }
     }
     __device__ __forceinline__ void store(const float (&v)[N], float *at, bool add) const {
         at += W * t;
 #pragma unroll
         for (int q = 0; q < P; ++q, at += W * T)
-            if (q < live) {
+            if (in(q)) {
                 if constexpr (VEC) {
                     float4 f = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
                     if (add) {
@@ -129,52 +133,23 @@ struct Row {
     }
 };
 
-// Rows brought to shared memory ahead of their use: `arrays` arrays of `width` columns a row, `stages` rows.
-struct Slab {
-    int width, arrays, stages;
-};
+// Asks the part of `width` values at `at` that is whole 16-byte units into L2, some rows ahead of its loads: these then wait for
+// L2 and not for HBM, whatever the row's alignment.  (Copies of whole rows to shared memory ahead of their use took as long on
+// the large shapes, longer on rows of 512 to 1024 values, and the shared memory from the loads of everything else.)
+__device__ __forceinline__ void ask_ahead(const float *at, int width) {
+    const uintptr_t begin = (reinterpret_cast<uintptr_t>(at) + 15) & ~uintptr_t(15);
+    const uintptr_t end = reinterpret_cast<uintptr_t>(at + width) & ~uintptr_t(15);
+    if (end > begin) prefetch_l2(reinterpret_cast<const void *>(begin), uint32_t(end - begin));
+}
 
-struct Ring {
-    float *data;
-    uint64_t *full;
-    Slab slab;
-    int stage, phase;  // of the row that is read next
-    __device__ __forceinline__ void init(float *at, uint64_t *bars, const Slab &s) {
-        data = at;
-        full = bars;
-        slab = s;
-        stage = phase = 0;
-        if (threadIdx.x == 0) {
-            for (int i = 0; i < s.stages; ++i) mbar_init(&full[i], 1);
-            mbar_init_fence();
-        }
-    }
-    __device__ __forceinline__ const float *next(int *status) const {  // waits for the next row
-        // (a wait that gives up leaves wrong values behind, which the next synchronising call reports)
-        mbar_wait_warp_ready(&full[stage], phase, status, 191);
-        return data + size_t(stage) * slab.arrays * slab.width;
-    }
-    __device__ __forceinline__ void advance() {
-        if (++stage == slab.stages) {
-            stage = 0;
-            phase ^= 1;
-        }
-    }
-    // By one thread: copies `width` columns of every array that there is, from `at` values behind its start, to a stage.
-    __device__ __forceinline__ void fetch(int to_stage, std::initializer_list<const float *> arrays, size_t at, int width) const {
-        const uint32_t bytes = uint32_t(width) * 4;
-        float *to = data + size_t(to_stage) * slab.arrays * slab.width;
-        mbar_arrive_expect_tx(&full[to_stage], bytes * slab.arrays);
-        for (const float *src : arrays)
-            if (src) {
-                bulk_load(to, src + at, bytes, &full[to_stage]);
-                to += slab.width;
-            }
-    }
-};
-
-constexpr int kMostStages = 8;
-constexpr size_t kRoom = size_t(222) * 1024;  // shared memory of an SM for rings, less 2 KiB a block
+// The same for several arrays (null: none) by the first lanes of the row's warps, in turn.
+template <int COUNT>
+__device__ __forceinline__ void ask_all_ahead(const float *const (&arrays)[COUNT], size_t at, int width, int warp, int warps) {
+    if ((threadIdx.x & 31) != 0) return;
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i)
+        if (i % warps == warp && arrays[i] != nullptr) ask_ahead(arrays[i] + at, width);
+}
 
 constexpr int kMostThreads = 512;
 
@@ -237,127 +212,69 @@ struct Rounds {
     }
 };
 
-// The ring leaves little of the SM's memory to L1, so what every row needs is kept beside it: a copy of `width` weights, if
-// there are any, in shared memory at `to`, which moves behind it.
-template <bool VEC>
-__device__ __forceinline__ const float *keep_weights(const float *weights, float *&to, int width) {
-    const float *copy = to;
-    if (weights != nullptr) {
-        if (VEC) {
-            for (int j = 4 * threadIdx.x; j < width; j += 4 * blockDim.x)
-                *reinterpret_cast<float4 *>(to + j) = __ldg(reinterpret_cast<const float4 *>(weights + j));
-        } else {
-            for (int j = threadIdx.x; j < width; j += blockDim.x) to[j] = __ldg(weights + j);
-        }
-        to += width;
-    }
-    return copy;
-}
-
-// How a row's threads find each other and its values: a warp's own row, a block's by plain loads, a block's by the ring.
-enum Rows { OF_WARP, OF_BLOCK, BY_RING };
-
-template <int N, bool VEC, Rows ROWS, bool LAYER>
-__global__ void __launch_bounds__(kMostThreads) norm_fwd_kernel(const __grid_constant__ Forward p, const __grid_constant__ Slab slab) {
-    constexpr bool WARP = ROWS == OF_WARP, RING = ROWS == BY_RING;
-    extern __shared__ __align__(128) float ring_data[];
+template <int N, Pieces PIECES, bool WARP, bool LAYER>
+__global__ void __launch_bounds__(kMostThreads) norm_fwd_kernel(const __grid_constant__ Forward p) {
     __shared__ Places places;
-    __shared__ uint64_t full[kMostStages];
-    Ring ring;
     launch_next();
-    if (RING) ring.init(ring_data, full, slab);
     if (!WARP) {
         clear_places(places);
         __syncthreads();
     }
     launch_wait();
     Rounds<WARP> rounds = {places, 0};
-    const Row<N, VEC> row_of(WARP ? threadIdx.x & 31 : threadIdx.x, WARP ? 32 : blockDim.x, p.cols);
+    const Row<N, PIECES> row_of(WARP ? threadIdx.x & 31 : threadIdx.x, WARP ? 32 : blockDim.x, p.cols);
     const unsigned per_block = WARP ? blockDim.x >> 5 : 1;
     const float inv = 1.f / float(p.cols);
     const bool gate_each = p.gate && p.rows_per_gate == 1;
     unsigned long long row = (unsigned long long)blockIdx.x * per_block + (WARP ? threadIdx.x >> 5 : 0);
     const unsigned long long step = (unsigned long long)gridDim.x * per_block;
-    float *keep_at = ring_data + (RING ? size_t(slab.stages) * slab.arrays * slab.width : 0);
-    const float *post_w = RING ? keep_weights<VEC>(p.post_w, keep_at, p.cols) : p.post_w;
-    const float *post_b = RING ? keep_weights<VEC>(p.post_b, keep_at, p.cols) : p.post_b;
-    const float *pre_w = RING ? keep_weights<VEC>(p.pre_w, keep_at, p.cols) : p.pre_w;
-    const float *pre_b = RING ? keep_weights<VEC>(p.pre_b, keep_at, p.cols) : p.pre_b;
-    if (RING) __syncthreads();
-    auto fetch = [&](int stage, unsigned long long r) {
-        ring.fetch(stage, {p.x, p.h, gate_each ? p.gate : nullptr}, r * size_t(p.cols), p.cols);
-    };
-    if (RING && threadIdx.x == 0)
-        for (int i = 0; i < slab.stages && row + i * step < p.rows; ++i) fetch(i, row + i * step);
+    const float *const ahead[3] = {p.x, p.h, gate_each ? p.gate : nullptr};
     for (; row < p.rows; row += step) {
         const size_t at = row * size_t(p.cols);
         float v[N], u[N], w[N];
-        const float *from = nullptr;
-        bool refill = RING;  // behind the row's first barrier
-        if (RING) from = ring.next(p.status);
-        auto refilled = [&] {
-            if (!RING || !refill) return;
-            refill = false;
-            if (threadIdx.x == 0 && row + slab.stages * step < p.rows) fetch(ring.stage, row + slab.stages * step);
-            ring.advance();
-        };
-        row_of.load(v, RING ? from : p.x + at);
+        row_of.load(v, p.x + at);
+        if (p.ahead && row + step < p.rows) ask_all_ahead(ahead, (row + step) * size_t(p.cols), p.cols, WARP ? 0 : threadIdx.x >> 5, WARP ? 1 : blockDim.x >> 5);
         if (p.h) {
-            row_of.load(u, RING ? from + slab.width : p.h + at);
+            row_of.load(u, p.h + at);
             float g[N];
-            if (p.gate)
-                row_of.load(g, RING && gate_each ? from + 2 * slab.width
-                                                 : p.gate + (gate_each ? at : row / p.rows_per_gate * p.cols));
-            if (RING) fence_proxy_async_smem();  // in front of the copies behind the first barrier
+            if (p.gate) row_of.load(g, p.gate + (gate_each ? at : row / p.rows_per_gate * p.cols));
             if (p.post_w) {
                 float m[1] = {0.f}, sq[1] = {0.f};
                 if (LAYER) {
                     row_of.each([&](int i) { m[0] += u[i]; });
                     rounds.sums(m);
-                    refilled();
-                    m[0] *= inv;
+                    row_of.center(u, m[0] * inv);
                 }
-                if (LAYER) row_of.center(u, m[0]);
                 row_of.each([&](int i) { sq[0] += u[i] * u[i]; });
-                row_of.load(w, post_w);
+                row_of.load(w, p.post_w);
                 rounds.sums(sq);
-                refilled();
-                const float rstd = 1.f / sqrtf(sq[0] * inv + p.eps);
+                const float rstd = rsqrtf(sq[0] * inv + p.eps);
                 row_of.each([&](int i) { u[i] *= rstd * w[i]; });
                 if (p.post_b) {
-                    row_of.load(w, post_b);
+                    row_of.load(w, p.post_b);
                     row_of.each([&](int i) { u[i] += w[i]; });
                 }
             }
             row_of.each([&](int i) { v[i] += p.scale * (p.gate ? g[i] * u[i] : u[i]); });
             row_of.store(v, p.r + at, false);
-        } else if (RING) {
-            fence_proxy_async_smem();
         }
         if (p.n) {
             float m[1] = {0.f}, sq[1] = {0.f};
             if (LAYER) {
                 row_of.each([&](int i) { m[0] += v[i]; });
                 rounds.sums(m);
-                refilled();
-                m[0] *= inv;
+                row_of.center(v, m[0] * inv);
             }
-            if (LAYER) row_of.center(v, m[0]);
             row_of.each([&](int i) { sq[0] += v[i] * v[i]; });
-            row_of.load(w, pre_w);
+            row_of.load(w, p.pre_w);
             rounds.sums(sq);
-            refilled();
-            const float rstd = 1.f / sqrtf(sq[0] * inv + p.eps);
+            const float rstd = rsqrtf(sq[0] * inv + p.eps);
             row_of.each([&](int i) { v[i] *= rstd * w[i]; });
             if (p.pre_b) {
-                row_of.load(w, pre_b);
+                row_of.load(w, p.pre_b);
                 row_of.each([&](int i) { v[i] += w[i]; });
             }
             row_of.store(v, p.n + at, false);
-        }
-        if (RING && refill) {  // no norm, no barrier yet
-            __syncthreads();
-            refilled();
         }
     }
 }
@@ -375,76 +292,74 @@ __device__ __forceinline__ void rows_of_block(const Backward &p, unsigned block,
     }
 }
 
-// Backward of rows that a block (or a cluster of blocks, each with a slab of the columns) holds, eight values a thread.
-//
-// The arrays of a row are brought to shared memory some rows ahead (RING: one bulk copy an array; else plain loads of the row
-// itself), and a thread keeps its columns' sums over the block's rows in registers.  A row costs two or three rounds of sums,
-// about 300 clocks each, beside the 2000 that HBM takes for a row of 2048 values on every SM, so one block's rounds hide
-// behind its own copies.
-constexpr int kValues = 8;
-
-// What a kernel adds up: without biases a row takes fewer instructions and registers.
+// What a backward kernel adds up: without biases a row takes fewer instructions and registers.
 enum Sums { RMS, RMS_BIAS, LAYER_BIAS };
 
-template <Sums MODE, bool RING, bool CLUSTER>
-__global__ void __launch_bounds__(kMostThreads) norm_bwd_kernel(const __grid_constant__ Backward p, const __grid_constant__ Slab slab) {
-    constexpr bool VEC = RING, LAYER = MODE == LAYER_BIAS, BIAS = MODE != RMS;
+constexpr int kValues = 8;       // a thread's, in the backward
+constexpr int kMostCluster = 4;  // blocks to a row
+
+// Backward of rows that a block (or a cluster of blocks, each with a slab of `width` columns) holds, eight values a thread.  A
+// thread keeps its columns' sums over the block's rows in registers.  What bounds it is the instructions of a row, about 450 a
+// warp at 2048 values and 16 warps to an SM, beside the 2000 clocks that HBM takes for that row on every SM.
+//
+// Layer norms on clusters: the mean is each block's own at first, and the sums about it are moved to the row's mean when the
+// blocks exchange them, so that a row has two exchanges like one of RMS norms and not three.
+template <Sums MODE, Pieces PIECES, bool CLUSTER>
+__global__ void __launch_bounds__(kMostThreads) norm_bwd_kernel(const __grid_constant__ Backward p, int slab) {
+    constexpr bool LAYER = MODE == LAYER_BIAS, BIAS = MODE != RMS;
     constexpr int N = kValues;
-    extern __shared__ __align__(128) float ring_data[];
     __shared__ Places places;
-    __shared__ float shared_sums[2][4];  // CLUSTER: this block's sums of a round
-    __shared__ uint64_t full[kMostStages];
+    __shared__ __align__(16) float exchange[2][kMostCluster][8];  // CLUSTER: the blocks' sums of a round
+    __shared__ uint64_t arrived[2];
     const unsigned rank = CLUSTER ? cluster_ctarank() : 0;
-    const unsigned blocks_a_row = CLUSTER ? unsigned(p.cols + slab.width - 1) / unsigned(slab.width) : 1;
-    const int c0 = int(rank) * slab.width, width = min(slab.width, p.cols - c0);
-    Ring ring;
+    const unsigned blocks_a_row = CLUSTER ? unsigned(p.cols + slab - 1) / unsigned(slab) : 1;
+    const int c0 = int(rank) * slab, width = CLUSTER ? min(slab, p.cols - c0) : p.cols;
     launch_next();
-    if (RING) ring.init(ring_data, full, slab);
     clear_places(places);
     __syncthreads();
+    if (CLUSTER) {
+        if (threadIdx.x == 0) {
+            mbar_init(&arrived[0], 1);
+            mbar_init(&arrived[1], 1);
+            mbar_init_fence();
+        }
+        cluster_sync_all();  // all blocks have begun and have their barriers: their shared memory may be written to
+    }
     launch_wait();
 
-    const Row<N, VEC> row_of(threadIdx.x, blockDim.x, width);
+    const Row<N, PIECES> row_of(threadIdx.x, blockDim.x, width);
+    const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     const float inv = 1.f / float(p.cols);
     const unsigned block = blockIdx.x / blocks_a_row, blocks = gridDim.x / blocks_a_row;
     const unsigned long long length = p.rows / p.groups;
     unsigned long long begin, end;
     rows_of_block(p, block, blocks, &begin, &end);
     const bool gate_each = p.gate && p.rows_per_gate == 1;
-    const bool gate_bias = BIAS && p.post_b && p.gate;
-    const float *post_w = p.post_w + c0, *pre_w = p.pre_w + c0, *post_b = p.post_b + c0;
-    if (RING) {
-        float *keep_at = ring_data + size_t(slab.stages) * slab.arrays * slab.width;
-        post_w = keep_weights<VEC>(p.post_w ? post_w : nullptr, keep_at, width);
-        pre_w = keep_weights<VEC>(p.dn ? pre_w : nullptr, keep_at, width);
-        post_b = keep_weights<VEC>(gate_bias ? post_b : nullptr, keep_at, width);
-        __syncthreads();
-    }
-    auto fetch = [&](int stage, unsigned long long row) {
-        ring.fetch(stage, {p.r, p.h, p.dn, p.dr, gate_each ? p.gate : nullptr}, row * size_t(p.cols) + c0, width);
-    };
-    if (RING && threadIdx.x == 0)
-        for (int i = 0; i < slab.stages && begin + i < end; ++i) fetch(i, begin + i);
+    const float *const ahead[5] = {p.r, p.h, p.dn, p.dr, gate_each ? p.gate : nullptr};
 
+    Rounds<false> rounds = {places, 0};
     int turn = 0;
-    auto round = [&](auto &v) {  // sums over the row
-        constexpr int K = sizeof(v) / sizeof(v[0]);
-        Rounds<false> r = {places, turn};
-        r.sums(v);
-        if (CLUSTER) {
-            if (threadIdx.x == 0)
-#pragma unroll
-                for (int k = 0; k < K; ++k) shared_sums[turn][k] = v[k];
-            cluster_sync_all();
-#pragma unroll
-            for (int k = 0; k < K; ++k) {
-                float sum = 0.f;
-                for (unsigned q = 0; q < blocks_a_row; ++q) sum += ld_shared_of_rank(&shared_sums[turn][k], q);
-                v[k] = sum;
-            }
+    // 4 * QUADS numbers of every block of the cluster, block q's at the result's [q]: a block writes its own to all.  The set of
+    // places and barrier that a block writes to again are free: that block has had the exchange between, to which every block
+    // came behind its reads.  (With cluster barriers, whose release waits for the row's stores, a row of 8192 took 1.6 times as
+    // long.)
+    int phase = 0;
+    auto exchanged = [&](auto quads, const float4 &a, const float4 &b) -> const float (*)[8] {
+        constexpr int QUADS = decltype(quads)::value;
+        if (threadIdx.x == 0) mbar_arrive_expect_tx(&arrived[turn], blocks_a_row * QUADS * 16);
+        if (threadIdx.x < blocks_a_row) {
+            st_async_v4(&exchange[turn][rank][0], &arrived[turn], threadIdx.x, a);
+            if (QUADS > 1) st_async_v4(&exchange[turn][rank][4], &arrived[turn], threadIdx.x, b);
         }
+        mbar_wait_warp_cluster(&arrived[turn], phase, p.status, 191);
+        const float (*const all)[8] = exchange[turn];
+        phase ^= turn;
         turn ^= 1;
+        return all;
     };
+    const float count = float(slab), last_count = float(p.cols - int(blocks_a_row - 1) * slab);  // columns of the blocks
+    using Quads = std::integral_constant<int, LAYER ? 2 : 1>;
+    using Quad = std::integral_constant<int, 1>;
 
     float gate[N], sum_gate[N] = {}, sum_pre_w[N] = {}, sum_pre_b[N] = {}, sum_post_w[N] = {}, sum_post_b[N] = {};
     // rows until the gate's next row and until the end of the group that dgate is summed over
@@ -459,13 +374,12 @@ __global__ void __launch_bounds__(kMostThreads) norm_bwd_kernel(const __grid_con
     size_t at = begin * size_t(p.cols) + c0;
     for (unsigned long long row = begin; row < end; ++row, at += p.cols) {
         float r[N], h[N], dn[N], dr[N], w[N];
-        const float *from = RING ? ring.next(p.status) : nullptr;
-        row_of.load(r, RING ? from : p.r + at);
-        if (p.h) row_of.load(h, RING ? from += slab.width : p.h + at);
-        if (p.dn) row_of.load(dn, RING ? from += slab.width : p.dn + at);
-        if (p.dr) row_of.load(dr, RING ? from += slab.width : p.dr + at);
+        row_of.load(r, p.r + at);
+        if (p.h) row_of.load(h, p.h + at);
+        if (p.dn) row_of.load(dn, p.dn + at);
+        if (p.dr) row_of.load(dr, p.dr + at);
         if (gate_each) {
-            row_of.load(gate, RING ? from += slab.width : p.gate + at);
+            row_of.load(gate, p.gate + at);
         } else if (p.gate) {
             if (gate_left == 0) {
                 gate_left = p.rows_per_gate;
@@ -474,18 +388,21 @@ __global__ void __launch_bounds__(kMostThreads) norm_bwd_kernel(const __grid_con
             }
             --gate_left;
         }
-        if (RING) fence_proxy_async_smem();  // in front of the copies behind the first round's barrier
+        if (row + 1 < end) ask_all_ahead(ahead, at + p.cols, width, warp, warps);
+        float m[2] = {0.f, 0.f};  // means of r and h; on clusters this block's
         if (LAYER) {
-            float m[2] = {0.f, 0.f};
             row_of.each([&](int i) { m[0] += r[i]; });
             if (p.post_w) row_of.each([&](int i) { m[1] += h[i]; });
-            round(m);
-            row_of.center(r, m[0] * inv);
-            if (p.post_w) row_of.center(h, m[1] * inv);
+            rounds.sums(m);
+            const float own = CLUSTER ? 1.f / float(width) : inv;
+            m[0] *= own;
+            m[1] *= own;
+            row_of.center(r, m[0]);
+            if (p.post_w) row_of.center(h, m[1]);
         }
         float a[N], v[4] = {0.f, 0.f, 0.f, 0.f};  // squares of r and h, a (r - m) and a
         if (p.dn) {
-            row_of.load(w, pre_w);
+            row_of.load(w, p.pre_w + c0);
             row_of.each([&](int i) {
                 a[i] = dn[i] * w[i];
                 v[0] += r[i] * r[i];
@@ -494,14 +411,47 @@ __global__ void __launch_bounds__(kMostThreads) norm_bwd_kernel(const __grid_con
             });
         }
         if (p.post_w) row_of.each([&](int i) { v[1] += h[i] * h[i]; });
-        round(v);
-        if (RING) {
-            if (threadIdx.x == 0 && row + slab.stages < end) fetch(ring.stage, row + slab.stages);
-            ring.advance();
+        rounds.sums(v);
+        if (CLUSTER) {
+            const float (*const all)[8] = exchanged(Quads(), make_float4(v[0], v[1], v[2], v[3]), make_float4(m[0], m[1], 0.f, 0.f));
+            float mean[2] = {0.f, 0.f};
+            if (LAYER) {
+#pragma unroll
+                for (unsigned q = 0; q < kMostCluster; ++q)
+                    if (q < blocks_a_row) {
+                        const float share = (q + 1 < blocks_a_row ? count : last_count) * inv;
+                        const float2 own = *reinterpret_cast<const float2 *>(&all[q][4]);
+                        mean[0] += share * own.x;
+                        mean[1] += share * own.y;
+                    }
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = 0.f;
+#pragma unroll
+            for (unsigned q = 0; q < kMostCluster; ++q)
+                if (q < blocks_a_row) {
+                    const float4 sums = *reinterpret_cast<const float4 *>(&all[q][0]);
+                    v[0] += sums.x;
+                    v[1] += sums.y;
+                    v[2] += sums.z;
+                    v[3] += sums.w;
+                    if (LAYER) {
+                        const float n = q + 1 < blocks_a_row ? count : last_count;
+                        const float2 own = *reinterpret_cast<const float2 *>(&all[q][4]);
+                        const float d0 = own.x - mean[0], d1 = own.y - mean[1];
+                        v[0] += n * d0 * d0;
+                        v[1] += n * d1 * d1;
+                        v[2] += d0 * sums.w;
+                    }
+                }
+            if (LAYER) {
+                row_of.center(r, mean[0] - m[0]);
+                if (p.post_w) row_of.center(h, mean[1] - m[1]);
+            }
         }
         if (!p.dr) row_of.each([&](int i) { dr[i] = 0.f; });
         if (p.dn) {
-            const float rs = 1.f / sqrtf(v[0] * inv + p.eps), c_hat = v[2] * rs * inv, c_one = LAYER ? v[3] * inv : 0.f;
+            const float rs = rsqrtf(v[0] * inv + p.eps), c_hat = v[2] * rs * inv, c_one = LAYER ? v[3] * inv : 0.f;
             row_of.each([&](int i) {
                 const float hat = r[i] * rs;
                 dr[i] += rs * (LAYER ? a[i] - hat * c_hat - c_one : a[i] - hat * c_hat);  // all of r's gradient from here on
@@ -512,14 +462,14 @@ __global__ void __launch_bounds__(kMostThreads) norm_bwd_kernel(const __grid_con
         if (p.dx) row_of.store(dr, p.dx + at, p.add_dx);
         if (!p.h) continue;
         float q[LAYER ? 2 : 1] = {}, b[N];  // b h^ and b behind the block
-        const float hs = 1.f / sqrtf(v[1] * inv + p.eps);
+        const float hs = rsqrtf(v[1] * inv + p.eps);
         // gate times gradient; dr turns into the gate's gradient
         row_of.each([&](int i) {
             dr[i] *= p.scale;
             b[i] = p.gate ? gate[i] * dr[i] : dr[i];
         });
         if (p.post_w) {
-            row_of.load(w, post_w);
+            row_of.load(w, p.post_w + c0);
             row_of.each([&](int i) {
                 h[i] *= hs;
                 sum_post_w[i] += b[i] * h[i];
@@ -529,9 +479,9 @@ __global__ void __launch_bounds__(kMostThreads) norm_bwd_kernel(const __grid_con
                 if constexpr (LAYER) q[1] += b[i];
             });
             if (p.gate) {
-                if (gate_bias) {
+                if (BIAS && p.post_b) {
                     float bias[N];
-                    row_of.load(bias, post_b);
+                    row_of.load(bias, p.post_b + c0);
                     row_of.each([&](int i) { dr[i] *= h[i] * w[i] + bias[i]; });
                 } else {
                     row_of.each([&](int i) { dr[i] *= h[i] * w[i]; });
@@ -552,10 +502,22 @@ __global__ void __launch_bounds__(kMostThreads) norm_bwd_kernel(const __grid_con
         }
         if (!p.dh) continue;
         if (p.post_w) {
-            round(q);
-            const float q_hat = q[0] * inv;
-            float q_one = 0.f;
-            if constexpr (LAYER) q_one = q[1] * inv;
+            rounds.sums(q);
+            float q_hat = q[0], q_one = 0.f;
+            if constexpr (LAYER) q_one = q[1];
+            if (CLUSTER) {
+                const float (*const all)[8] = exchanged(Quad(), make_float4(q_hat, q_one, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f));
+                q_hat = q_one = 0.f;
+#pragma unroll
+                for (unsigned k = 0; k < kMostCluster; ++k)
+                    if (k < blocks_a_row) {
+                        const float2 sums = *reinterpret_cast<const float2 *>(&all[k][0]);
+                        q_hat += sums.x;
+                        q_one += sums.y;
+                    }
+            }
+            q_hat *= inv;
+            q_one *= inv;
             row_of.each([&](int i) { b[i] = hs * (LAYER ? b[i] - h[i] * q_hat - q_one : b[i] - h[i] * q_hat); });
         }
         row_of.store(b, p.dh + at, p.add_dh);
@@ -566,7 +528,7 @@ __global__ void __launch_bounds__(kMostThreads) norm_bwd_kernel(const __grid_con
     if (p.partial[DPOST_W]) row_of.store(sum_post_w, p.partial[DPOST_W] + mine, false);
     if (BIAS && p.partial[DPOST_B]) row_of.store(sum_post_b, p.partial[DPOST_B] + mine, false);
     if (p.partial[DGATE]) row_of.store(sum_gate, p.partial[DGATE] + mine, false);
-    if (CLUSTER) cluster_sync_all();  // no block leaves while another may read its sums
+    if (CLUSTER) cluster_sync_all();  // no block leaves while another may still write to it
 }
 
 // ---- rows of any length: every round of sums reads its row again (from L2, mostly) ---------------------------------
@@ -588,7 +550,7 @@ __global__ void __launch_bounds__(kThreads) norm_fwd_long_kernel(const __grid_co
             }
             for (int j = threadIdx.x; j < p.cols; j += kThreads) hs[0] += (h[j] - hm[0]) * (h[j] - hm[0]);
             block_sums<1, kThreads>(hs, sh[1]);
-            hs[0] = 1.f / sqrtf(hs[0] * inv + p.eps);
+            hs[0] = rsqrtf(hs[0] * inv + p.eps);
         }
         for (int j = threadIdx.x; j < p.cols; j += kThreads) {
             float v = x[j];
@@ -609,7 +571,7 @@ __global__ void __launch_bounds__(kThreads) norm_fwd_long_kernel(const __grid_co
                 for (int j = threadIdx.x; j < p.cols; j += kThreads) rs[0] += (r[j] - rm[0]) * (r[j] - rm[0]);
             }
             block_sums<1, kThreads>(rs, sh[3]);
-            rs[0] = 1.f / sqrtf(rs[0] * inv + p.eps);
+            rs[0] = rsqrtf(rs[0] * inv + p.eps);
             for (int j = threadIdx.x; j < p.cols; j += kThreads)
                 p.n[at + j] = (r[j] - rm[0]) * rs[0] * p.pre_w[j] + (p.pre_b ? p.pre_b[j] : 0.f);
         }
@@ -661,7 +623,7 @@ __global__ void __launch_bounds__(kThreads) norm_bwd_long_kernel(const __grid_co
             if (p.post_w) v[1] += (h[j] - m[1]) * (h[j] - m[1]);
         }
         block_sums<4, kThreads>(v, sh4);
-        const float rs = 1.f / sqrtf(v[0] * inv + p.eps), hs = 1.f / sqrtf(v[1] * inv + p.eps);
+        const float rs = rsqrtf(v[0] * inv + p.eps), hs = rsqrtf(v[1] * inv + p.eps);
         const float c_hat = v[2] * rs * inv, c_one = LAYER ? v[3] * inv : 0.f;
         auto full = [&](int j, float *hat) {  // D, and r^
             float d = dr ? dr[j] : 0.f;
@@ -768,6 +730,9 @@ int32_t start(katsu_cuda_ctx *ctx, void (*kernel)(Params...), unsigned grid, uns
     return katsu_launch_chained(ctx, kernel, grid, block, 0, 1, args...);
 }
 
+// Blocks to an SM, by the registers of the kernels that hold rows (up to 128 a thread).
+unsigned resident_blocks(unsigned threads) { return threads >= 64 ? 512 / threads : 8; }
+
 // Whether rows are whole 16-byte pieces at 16-byte addresses.
 bool pieces(int cols, std::initializer_list<const void *> pointers) {
     uintptr_t at = uintptr_t(cols) * sizeof(float);
@@ -776,93 +741,60 @@ bool pieces(int cols, std::initializer_list<const void *> pointers) {
 }
 
 template <bool LAYER>
-int32_t start_forward_of(katsu_cuda_ctx *ctx, const Forward &p, bool wide, bool vec, Rows rows, const Slab &slab, size_t smem,
-                         unsigned grid, unsigned block) {
-    auto kernel = wide               ? norm_fwd_kernel<32, true, OF_BLOCK, LAYER>
-                  : rows == BY_RING  ? norm_fwd_kernel<16, true, BY_RING, LAYER>
-                  : rows == OF_BLOCK ? (vec ? norm_fwd_kernel<16, true, OF_BLOCK, LAYER> : norm_fwd_kernel<16, false, OF_BLOCK, LAYER>)
-                                     : (vec ? norm_fwd_kernel<16, true, OF_WARP, LAYER> : norm_fwd_kernel<16, false, OF_WARP, LAYER>);
-    if (smem) KATSU_TRY(katsu_prepare_kernel(ctx, (const void *)kernel, smem));
-    return katsu_launch_chained(ctx, kernel, grid, block, smem, 1, p, slab);
-}
-
-template <bool LAYER>
-int32_t start_forward(katsu_cuda_ctx *ctx, const Forward &p) {
+int32_t start_forward(katsu_cuda_ctx *ctx, Forward p) {
     const bool vec = pieces(p.cols, {p.x, p.h, p.gate, p.post_w, p.post_b, p.pre_w, p.pre_b, p.r, p.n});
     const unsigned long long sms = ctx->num_sms;
     if (p.cols > kMostThreads * (vec ? 32 : 16))
         return start(ctx, norm_fwd_long_kernel<LAYER>, unsigned(p.rows < sms * 4 ? p.rows : sms * 4), kThreads, p);
     // 16 values a thread, 32 where that would take more than 512 threads; up to 512 values are one warp's
-    const bool wide = p.cols > kMostThreads * 16;
-    Rows rows = p.cols <= 512 ? OF_WARP : OF_BLOCK;
-    const unsigned threads = rows == OF_WARP ? 128 : unsigned(katsu_div_up(katsu_div_up(p.cols, wide ? 32 : 16), 32)) * 32;
-    const unsigned long long need = rows == OF_WARP ? katsu_div_up(p.rows, 4) : p.rows;
-    unsigned resident = 512 / threads;  // registers: 512 threads to an SM
-    if (resident > 8) resident = 8;
-    const unsigned long long most = sms * resident;
-    Slab slab = {};
-    size_t smem = 0;
-    // A block that takes several rows brings them ahead; a single one arrives sooner by plain loads (one row of 4096: 5.6 us).
-    if (vec && rows == OF_BLOCK && !wide && p.rows > sms * resident) {
-        slab.width = p.cols;
-        slab.arrays = 1 + (p.h != nullptr) + (p.gate && p.rows_per_gate == 1);
-        const size_t row = size_t(slab.arrays) * p.cols * sizeof(float);
-        const size_t kept = size_t((p.post_w != nullptr) + (p.post_b != nullptr) + (p.pre_w != nullptr) + (p.pre_b != nullptr)) * p.cols * sizeof(float);
-        const size_t room = kRoom / resident - 2048 > kept ? kRoom / resident - 2048 - kept : 0;
-        const size_t stages = room / row < kMostStages ? room / row : kMostStages;
-        if (stages >= 2) {
-            rows = BY_RING;
-            slab.stages = int(stages);
-            smem = slab.stages * row + kept;
-        }
-    }
-    const unsigned grid = unsigned(need < most ? need : most);
-    return start_forward_of<LAYER>(ctx, p, wide, vec, rows, slab, smem, grid, threads);
+    const bool wide = p.cols > kMostThreads * 16, warp = p.cols <= 512;
+    const unsigned threads = warp ? 128 : unsigned(katsu_div_up(katsu_div_up(p.cols, wide ? 32 : 16), 32)) * 32;
+    const unsigned long long need = warp ? katsu_div_up(p.rows, 4) : p.rows, most = sms * resident_blocks(threads);
+    // Rows are asked into L2 ahead where little else of the SM runs under a row's rounds: layer norms have two more of them
+    // (16384 x 2048: 90 us, 103 without), rows of more than 4096 values leave an SM to one block (8192 x 5120: 108 us, 127).  Two
+    // blocks of RMS norms reach 93 % of HBM's rate without and 87 % with it.
+    p.ahead = !warp && (LAYER || (threads > 256 && !wide));
+    auto kernel = wide   ? norm_fwd_kernel<32, WHOLE, false, LAYER>
+                  : warp ? (vec ? norm_fwd_kernel<16, WHOLE, true, LAYER> : norm_fwd_kernel<16, SINGLES, true, LAYER>)
+                         : (vec ? norm_fwd_kernel<16, WHOLE, false, LAYER> : norm_fwd_kernel<16, SINGLES, false, LAYER>);
+    return start(ctx, kernel, unsigned(need < most ? need : most), threads, p);
 }
 
-// Which kernel a backward pass takes, and how many blocks (or clusters) go round at once.
+// How the kernels' blocks share a row, and how many rows are on their way at once.
 struct BackwardShape {
-    Slab slab;  // arrays 0: no ring; width 0: the kernel for rows of any length
+    int slab;  // columns to a block; 0: the kernel for rows of any length
+    Pieces pieces;
     unsigned threads, cluster;
-    size_t smem, most_blocks;
+    size_t most_blocks;
 };
 
 BackwardShape backward_shape(const katsu_cuda_ctx *ctx, const Backward &p, std::initializer_list<const void *> pointers) {
     BackwardShape s = {};
     const int most = kMostThreads * kValues;  // columns to a block
     const bool vec = pieces(p.cols, pointers);
-    if (p.cols > (vec ? 4 : 1) * most) {
+    if (p.cols > (vec ? kMostCluster * most : most)) {
         s.most_blocks = size_t(ctx->num_sms) * 4;
         return s;
     }
     s.cluster = p.cols > 2 * most ? 4 : p.cols > most ? 2 : 1;
-    s.slab.width = int(katsu_div_up(katsu_div_up(p.cols, s.cluster), 4)) * 4;
-    s.threads = unsigned(katsu_div_up(katsu_div_up(s.slab.width, kValues), 32)) * 32;
-    unsigned resident = 512 / s.threads;  // registers: 512 threads to an SM
-    if (resident > 8) resident = 8;
-    if (vec) {
-        s.slab.arrays = 1 + (p.h != nullptr) + (p.dn != nullptr) + (p.dr != nullptr) + (p.gate && p.rows_per_gate == 1);
-        const size_t row = size_t(s.slab.arrays) * s.slab.width * sizeof(float);
-        const size_t kept = size_t((p.post_w != nullptr) + (p.dn != nullptr) + (p.post_b && p.gate)) * s.slab.width * sizeof(float);
-        const size_t room = kRoom / resident - 2048 - kept;
-        s.slab.stages = int(room / row < kMostStages ? room / row : kMostStages);
-        s.smem = s.slab.stages * row + kept;
-    }
-    s.most_blocks = size_t(ctx->num_sms) * resident / s.cluster;
+    s.slab = int(katsu_div_up(katsu_div_up(p.cols, s.cluster), 4)) * 4;
+    s.threads = unsigned(katsu_div_up(katsu_div_up(s.slab, kValues), 32)) * 32;
+    s.pieces = !vec ? SINGLES : p.cols == int(s.cluster * s.threads) * kValues ? FULL : WHOLE;
+    s.most_blocks = size_t(ctx->num_sms) * resident_blocks(s.threads) / s.cluster;
     return s;
 }
 
 template <Sums MODE>
 int32_t start_backward_of(katsu_cuda_ctx *ctx, const Backward &p, const BackwardShape &s, size_t blocks) {
-    auto kernel = s.cluster > 1 ? norm_bwd_kernel<MODE, true, true>
-                  : s.slab.arrays ? norm_bwd_kernel<MODE, true, false> : norm_bwd_kernel<MODE, false, false>;
-    if (s.smem) KATSU_TRY(katsu_prepare_kernel(ctx, (const void *)kernel, s.smem));
-    return katsu_launch_chained(ctx, kernel, (unsigned)blocks * s.cluster, s.threads, s.smem, s.cluster, p, s.slab);
+    auto kernel = s.cluster > 1       ? (s.pieces == FULL ? norm_bwd_kernel<MODE, FULL, true> : norm_bwd_kernel<MODE, WHOLE, true>)
+                  : s.pieces == FULL  ? norm_bwd_kernel<MODE, FULL, false>
+                  : s.pieces == WHOLE ? norm_bwd_kernel<MODE, WHOLE, false> : norm_bwd_kernel<MODE, SINGLES, false>;
+    return katsu_launch_chained(ctx, kernel, (unsigned)blocks * s.cluster, s.threads, 0, s.cluster, p, s.slab);
 }
 
 template <bool LAYER>
 int32_t start_backward(katsu_cuda_ctx *ctx, const Backward &p, const BackwardShape &s, size_t blocks) {
-    if (s.slab.width == 0) return start(ctx, norm_bwd_long_kernel<LAYER>, (unsigned)blocks, kThreads, p);
+    if (s.slab == 0) return start(ctx, norm_bwd_long_kernel<LAYER>, (unsigned)blocks, kThreads, p);
     const bool bias = p.post_b || p.partial[DPRE_B] || p.partial[DPOST_B];
     return LAYER ? start_backward_of<LAYER_BIAS>(ctx, p, s, blocks)
                  : bias ? start_backward_of<RMS_BIAS>(ctx, p, s, blocks) : start_backward_of<RMS>(ctx, p, s, blocks);
@@ -897,7 +829,7 @@ extern "C" int32_t katsu_cuda_block_norm_fwd(katsu_cuda_ctx *ctx, const float *x
         KATSU_REQUIRE(in == nullptr || (in != r && in != n), "an output is an input too");
     KATSU_REQUIRE(r != n, "r and n are the same buffer");
     KATSU_TRY(katsu_bind(ctx));
-    Forward p = {x, h, gate, post_w, post_b, pre_w, pre_b, r, n, scale, eps, rows, gate ? rows / gate_rows : 1, (int)cols, ctx->status};
+    Forward p = {x, h, gate, post_w, post_b, pre_w, pre_b, r, n, scale, eps, rows, gate ? rows / gate_rows : 1, (int)cols, 0};
     return kind == KATSU_NORM_LAYER ? start_forward<true>(ctx, p) : start_forward<false>(ctx, p);
 }
 
@@ -938,10 +870,10 @@ extern "C" int32_t katsu_cuda_block_norm_bwd(katsu_cuda_ctx *ctx, const float *r
     p.dx = dx; p.dh = dh;
     p.scale = scale; p.eps = eps;
     p.rows = rows; p.rows_per_gate = gate ? rows / gate_rows : 1; p.cols = (int)cols;
+    p.status = ctx->status;
     p.add_dx = accumulate & KATSU_BLOCK_DX; p.add_dh = accumulate & KATSU_BLOCK_DH; p.add_dgate = adds[DGATE];
     p.gate_of_row = dgate && gate_rows == rows;
     p.groups = dgate && !p.gate_of_row ? gate_rows : 1;
-    p.status = ctx->status;
     const BackwardShape shape = backward_shape(ctx, p, {r, h, gate, post_w, post_b, pre_w, dr, dn, dx, dh, dgate});
     const size_t want = shape.most_blocks < rows ? shape.most_blocks : rows;
     size_t blocks;

@@ -21,11 +21,35 @@ __device__ __forceinline__ uint32_t map_to_rank(const void *local, uint32_t rank
     return out;
 }
 
-// The variable at this place in block `rank`'s shared memory (ordered by a cluster barrier behind the write).
-__device__ __forceinline__ float ld_shared_of_rank(const float *local, uint32_t rank) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(map_to_rank(local, rank)) : "memory");
-    return v;
+// Writes to the variable at this place in block `rank`'s shared memory and counts the 16 bytes on the barrier at `bar`'s place
+// there: the data and its signal in one, with nothing of the thread's earlier work waited for.
+__device__ __forceinline__ void st_async_v4(const void *local, uint64_t *bar, uint32_t rank, float4 v) {
+    asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(map_to_rank(local, rank)),
+                 "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w), "r"(map_to_rank(bar, rank))
+                 : "memory");
+}
+
+// Whole-warp bounded wait (mbar_wait_warp) for what other blocks of the cluster have written.
+__device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t *bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+        "selp.u32 %0, 1, 0, p;\n"
+        "}\n"
+        : "=r"(done)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return done != 0;
+}
+
+__device__ __forceinline__ bool mbar_wait_warp_cluster(uint64_t *bar, uint32_t parity, int *status, int code) {
+    // (every lane acquires: each reads the data itself)
+    if (__all_sync(0xffffffffu, mbar_try_wait_cluster(bar, parity) ? 1 : 0)) return true;
+    const bool ok = mbar_wait_warp(bar, parity, status, code);
+    mbar_try_wait_cluster(bar, parity);
+    return ok;
 }
 
 // Arrival on a barrier of the other block.  Relaxed: what these arrivals publish lives in tensor memory and is

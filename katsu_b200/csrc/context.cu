@@ -31,7 +31,7 @@ int32_t katsu_bind(katsu_cuda_ctx *ctx) {
     return KATSU_OK;
 }
 
-int32_t katsu_prepare_kernel(katsu_cuda_ctx *ctx, const void *kernel, size_t smem) {
+int32_t katsu_prepare_kernel(katsu_cuda_ctx *ctx, const void *kernel, size_t smem, bool largest) {
     // contexts of several threads may launch the same kernel for the first time
     static std::mutex lock;
     static std::unordered_map<const void *, size_t> *prepared = new std::unordered_map<const void *, size_t>[64];
@@ -40,7 +40,8 @@ int32_t katsu_prepare_kernel(katsu_cuda_ctx *ctx, const void *kernel, size_t sme
     const auto it = of_device.find(kernel);
     if (it != of_device.end() && it->second >= smem) return KATSU_OK;
     if (smem) KATSU_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    KATSU_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
+    if (largest)
+        KATSU_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
     try {
         of_device[kernel] = smem;
     } catch (...) {  // no host memory for the entry: set again by the next launch

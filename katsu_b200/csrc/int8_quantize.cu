@@ -1,7 +1,7 @@
 // Matrices to 8 bits: rows of x (one scale a token) and columns of w (one scale an output channel, kept transposed).
 //
-// Rows: a warp (up to 1024 values) or a block of 256 (up to 8192) or 512 threads takes a row and holds its last 32 (16) values a
-// thread in registers between the largest magnitude and the quotients; what lies in front is read again, from L2.  Bound: HBM, 4 bytes
+// Rows: a warp (up to 1024 values) or a block of 128 to 1024 threads takes a row and holds it in registers, 32 values a thread,
+// between the largest magnitude and the quotients; of rows above 32768 values what lies in front of these is read again, from L2.  Bound: HBM, 4 bytes
 // in and 1 out a value.
 #include "int8.cuh"
 
@@ -19,15 +19,17 @@ __device__ __forceinline__ void load4(const float *row, size_t j, size_t k, floa
     }
 }
 
+constexpr int kHeld = 8;  // 16-byte pieces
+
 // T threads to a row, each of which holds kHeld 16-byte pieces: the row's last ones, loaded behind what is read twice, so that
 // their registers are free until then.  WAVES: more blocks than are resident at once (see katsu_int8_quantize).
-template <int T, int kHeld, bool VEC, bool WAVES>
-__global__ void __launch_bounds__(T < 256 ? 256 : T) quantize_rows_kernel(const float *__restrict__ x, int8_t *q, float *scale,
+template <int T, bool VEC, bool WAVES>
+__global__ void __launch_bounds__(T == 32 ? 256 : T) quantize_rows_kernel(const float *__restrict__ x, int8_t *q, float *scale,
                                                                           unsigned long long rows, size_t k, size_t pitch) {
-    __shared__ float sh[T < 256 ? 1 : T / 32];
+    __shared__ float sh[T / 32];
     if (!WAVES) launch_next();
     launch_wait();
-    constexpr int per_block = T < 256 ? 256 / T : 1, batch = 4 * T * kHeld;
+    constexpr int per_block = T == 32 ? 8 : 1, batch = 4 * T * kHeld;
     const int t = threadIdx.x % T;
     const unsigned long long row = (unsigned long long)blockIdx.x * per_block + threadIdx.x / T;
     if (row >= rows) return;  // (a warp's rows: the others of the block do not wait)
@@ -133,8 +135,10 @@ __global__ void __launch_bounds__(256) quantize_columns_kernel(const float *__re
 
 template <bool VEC, bool WAVES>
 static void (*rows_kernel(size_t k))(const float *, int8_t *, float *, unsigned long long, size_t, size_t) {
-    return k <= 1024 ? quantize_rows_kernel<32, 8, VEC, WAVES>
-           : k <= 8192 ? quantize_rows_kernel<256, 8, VEC, WAVES> : quantize_rows_kernel<512, 4, VEC, WAVES>;
+    return k <= 1024    ? quantize_rows_kernel<32, VEC, WAVES>
+           : k <= 4096  ? quantize_rows_kernel<128, VEC, WAVES>
+           : k <= 8192  ? quantize_rows_kernel<256, VEC, WAVES>
+           : k <= 16384 ? quantize_rows_kernel<512, VEC, WAVES> : quantize_rows_kernel<1024, VEC, WAVES>;
 }
 
 // A row to a warp or block.  Few rows: the launch is chained, like that of the product behind it, and takes the largest
@@ -143,12 +147,14 @@ static void (*rows_kernel(size_t k))(const float *, int8_t *, float *, unsigned 
 // largest partition 80).
 int32_t katsu_int8_quantize(katsu_cuda_ctx *ctx, const float *x, int8_t *q, float *scale, size_t m, size_t k) {
     const bool vec = k % 4 == 0 && (reinterpret_cast<uintptr_t>(x) & 15u) == 0;
-    const size_t blocks = k <= 1024 ? katsu_div_up(m, 8) : m;
-    const bool waves = blocks > size_t(ctx->num_sms) * 2;
+    const bool warps = k <= 1024;
+    const unsigned threads = warps ? 256 : k <= 4096 ? 128 : k <= 8192 ? 256 : k <= 16384 ? 512 : 1024;
+    const size_t blocks = warps ? katsu_div_up(m, 8) : m;
+    const bool waves = blocks > size_t(ctx->num_sms) * (warps ? 3 : 1024 / threads);  // by the kernels' registers
     auto kernel = waves ? (vec ? rows_kernel<true, true>(k) : rows_kernel<false, true>(k))
                          : (vec ? rows_kernel<true, false>(k) : rows_kernel<false, false>(k));
     if (!waves) KATSU_TRY(katsu_prepare_kernel(ctx, (const void *)kernel, 0));
-    return katsu_launch(ctx, !waves, kernel, (unsigned)blocks, k <= 8192 ? 256u : 512u, 0, 1, x, q, scale, m, k, katsu_int8_pitch(k));
+    return katsu_launch(ctx, !waves, kernel, (unsigned)blocks, threads, 0, 1, x, q, scale, m, k, katsu_int8_pitch(k));
 }
 
 extern "C" int32_t katsu_cuda_int8_row_bytes(size_t k, size_t *out_bytes) {

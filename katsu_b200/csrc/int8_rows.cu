@@ -142,17 +142,22 @@ int32_t katsu_int8_few(katsu_cuda_ctx *ctx, const float *x, const int8_t *xq, co
     const int tokens = m <= 1 ? 1 : m <= 2 ? 2 : m <= 4 ? 4 : 8;
     const size_t smem = tokens * pitch;
     if (m > 8 || smem > size_t(200) * 1024 || n > 0x3fffffff) return KATSU_OK;
-    // rows in 8 bits come to every block as they are, rows in f32 are four times that and read twice
-    if (x != nullptr && m * k > 16384) return KATSU_OK;
+    // Rows in 8 bits come to every block as they are; rows in f32 are four times that, and read twice (2 x 8192 by 8192 x 8192:
+    // 32 us, 19 with a launch that quantises them once).
+    if (x != nullptr && m * k > 8192) return KATSU_OK;
+    // Eight tokens' multiply-adds and their reads of shared memory take about as long as large weights: 8 x 8192 by 8192 x 8192
+    // 27 us, on the tensor cores 22; 8 x 4096 by 4096 x 4096 8.5 and 10.5.
+    if (m > 4 && k * n > (size_t(1) << 25)) return KATSU_OK;
     *handled = 1;
     auto kernel = tokens == 1 ? int8_rows_kernel<1> : tokens == 2 ? int8_rows_kernel<2> : tokens == 4 ? int8_rows_kernel<4> : int8_rows_kernel<8>;
-    KATSU_TRY(katsu_prepare_kernel(ctx, (const void *)kernel, smem));
+    if (smem > size_t(48) * 1024) KATSU_TRY(katsu_prepare_kernel(ctx, (const void *)kernel, smem, false));
     const size_t pairs = katsu_div_up(n, kRows), warps = size_t(ctx->num_sms) * kWarps * 2;
     int share = 1;
     while (share < kWarps && pairs * share * 2 <= warps) share *= 2;
     const size_t need = katsu_div_up(pairs, kWarps / share);
     size_t fit = (size_t(224) * 1024) / (smem + 2048);  // blocks that an SM holds
-    if (fit > 3) fit = 3;  // (and three by their registers)
+    const size_t by_registers = tokens <= 2 ? 4 : 3;
+    if (fit > by_registers) fit = by_registers;
     const size_t most = size_t(ctx->num_sms) * fit;
     return katsu_launch_chained(ctx, kernel, (unsigned)(need < most ? need : most), kWarps * 32, smem, 1, x, xq, xs, wq, ws, bias, y,
                                 (int)m, (int)k, (int)n, (int)pitch, share);

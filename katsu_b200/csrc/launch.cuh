@@ -16,8 +16,9 @@ __device__ __forceinline__ void launch_next() { asm volatile("griddepcontrol.lau
 
 // Once per kernel and device (and whenever more is asked for): its dynamic shared memory, and the largest shared-memory
 // partition of the SM, so that kernels that follow each other do not make the SM re-partition its memory, which it only
-// does when it is idle.
-int32_t katsu_prepare_kernel(katsu_cuda_ctx *ctx, const void *kernel, size_t smem);
+// does when it is idle.  Kernels that live on loads in flight are better off without (largest = false): these take L1, which
+// that partition leaves 28 KiB (a step over 1.2 GB of gradients and weights each: 682 us with it, 506 without).
+int32_t katsu_prepare_kernel(katsu_cuda_ctx *ctx, const void *kernel, size_t smem, bool largest = true);
 
 // early: the launch may start under its predecessor's end.  Only for grids whose blocks are all resident at once: one that the
 // hardware hands out in waves is launched plainly, and its blocks do not call launch_next().

@@ -168,6 +168,30 @@ def test_many_rows_and_gates(ctx, rows, cols, gate_rows):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("layer", [False, True], ids=["rms", "layer"])
+@pytest.mark.parametrize("rows,cols", [(400, 5004), (400, 5120), (160, 9000), (160, 12288), (120, 16384)])
+def test_rows_wider_than_a_block(ctx, rows, cols, layer):
+    """Several rows to each cluster of blocks.  Along a row the values climb by three spreads and more, so that the blocks'
+    own means lie far from the row's: differences from it carry that much more of the values' roundings, a factor of 4."""
+    a = inputs(rows, cols, gate_rows=2, bias=layer, seed=10)
+    climb = np.linspace(-3, 3, cols, dtype=np.float32)
+    a["r"], a["h"] = a.pop("x") + climb, a["h"] - climb
+    want = block_ref.backward(*[a[k] for k in ("r", "h", "gate", "post_w", "post_b", "pre_w")], 0.5, 1e-5, layer, a["dr"], a["dn"])
+    names = [o for o in OUTS if layer or not o.endswith("_b")]
+    with uploaded(ctx, a) as d:
+        for o in names:
+            d.alloc(o, want[o].size, fill=np.nan)
+        bwd(ctx, d, a, (rows, cols), 0.5, 1e-5, layer, {o: d[o] for o in names})
+        got = {o: d.get(o) for o in names}
+        for o in names:
+            assert rel_l2(got[o], want[o].reshape(-1)) <= 4 * tolerance(cols, rows), (o, rel_l2(got[o], want[o].reshape(-1)))
+        for _ in range(3):  # the same bits again
+            bwd(ctx, d, a, (rows, cols), 0.5, 1e-5, layer, {o: d[o] for o in names})
+        for o in names:
+            assert np.array_equal(d.get(o), got[o]), o
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("shift", [1, 2, 3])
 @pytest.mark.parametrize("cols", [64, 1024, 4096, 8192])
 def test_unaligned(ctx, cols, shift):

@@ -12,7 +12,7 @@ U = 2.0 ** -24
 
 SIZES = {"one value": [1], "nothing": [], "empty ones": [0, 5, 0, 0, 3], "one chunk": [8192], "over a chunk": [8193, 8191, 1],
          "small CNN": [864, 18432, 65536 * 10], "many": [1 + (7 * i) % 23 for i in range(33)],
-         "more than a launch takes": [3 + i % 5 for i in range(1100)], "large": [3_000_001, 17, 2_500_000]}
+         "more than a launch takes": [3 + i % 5 for i in range(1100)], "launches in waves": [9001 + 4 * i for i in range(600)], "large": [3_000_001, 17, 2_500_000]}
 
 
 def flat(sizes, seed, std=1.0):
@@ -126,6 +126,16 @@ def test_not_finite(ctx, bad):
         assert np.array_equal(d.get("g"), g, equal_nan=True)
         ctx.sgd_step_clipped(places(d["w"], sizes), gp, sizes, 0.1, 1.0, d["n"])
         assert np.array_equal(d.get("w"), w)
+
+
+@pytest.mark.gpu
+def test_norm_at_the_limit_changes_nothing(ctx):
+    g = np.array([3.0, 4.0], np.float32)
+    with DeviceArrays(ctx, g=g, n=np.zeros(1)) as d:
+        ctx.clip_grads([d["g"]], [d["g"]], [2], 5.0, d["n"])
+        assert d.get("n")[0] == 5 and np.array_equal(d.get("g"), g)
+        ctx.clip_grads([d["g"]], [d["g"]], [2], float(np.nextafter(np.float32(5), np.float32(0))), d["n"])
+        assert not np.array_equal(d.get("g"), g)
 
 
 @pytest.mark.gpu

@@ -1,8 +1,11 @@
 // Matrices to 8 bits: rows of x (one scale a token) and columns of w (one scale an output channel, kept transposed).
 //
 // Rows: a warp (up to 1024 values) or a block of 128 to 1024 threads takes a row and holds it in registers, 32 values a thread,
-// between the largest magnitude and the quotients; of rows above 32768 values what lies in front of these is read again, from L2.  Bound: HBM, 4 bytes
-// in and 1 out a value.
+// between the largest magnitude and the quotients; of rows above 32768 values what lies in front of these is read again, from
+// L2.  Bound: HBM, 4 bytes in and 1 out a value (8192 x 8192: 53 us, its floor 52).
+//
+// Columns: one launch finds the largest magnitudes of pieces of the columns, another folds them and turns tiles of 128 x 32 over
+// in shared memory; w is read twice.
 #include "int8.cuh"
 
 namespace {
@@ -79,47 +82,58 @@ __global__ void __launch_bounds__(T == 32 ? 256 : T) quantize_rows_kernel(const 
         }
 }
 
-// Largest magnitude of every column of w [k, n], as bits, over k rows cut into gridDim.y pieces; `most` starts at zero.
-// (The largest of a set does not depend on the order of the atomics.)
-__global__ void __launch_bounds__(256) column_largest_kernel(const float *__restrict__ w, unsigned *most_of, size_t k, size_t n) {
-    launch_next();
+// Largest magnitude of every column of w [k, n] over each of `pieces` equal pieces of its rows: [pieces][n].  A block has a piece
+// of 32 columns.
+__global__ void __launch_bounds__(256) column_largest_kernel(const float *__restrict__ w, float *largest, size_t k, size_t n,
+                                                             unsigned pieces, unsigned tiles, int waves) {
+    if (!waves) launch_next();
     launch_wait();
-    const size_t col = size_t(blockIdx.x) * 32 + (threadIdx.x & 31);
-    const size_t begin = k * blockIdx.y / gridDim.y, end = k * (blockIdx.y + 1) / gridDim.y;
+    const unsigned piece = blockIdx.x / tiles, lane = threadIdx.x & 31;
+    const size_t col = size_t(blockIdx.x - piece * tiles) * 32 + lane;
+    const size_t begin = k * piece / pieces, end = k * (piece + 1) / pieces;
     float m = 0.f;
     if (col < n)
 #pragma unroll 8
         for (size_t p = begin + (threadIdx.x >> 5); p < end; p += 8) m = katsu_larger(m, __ldg(w + p * n + col));
     __shared__ float sh[8][33];
-    sh[threadIdx.x >> 5][threadIdx.x & 31] = m;
+    sh[threadIdx.x >> 5][lane] = m;
     __syncthreads();
     if (threadIdx.x < 32 && col < n) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) m = katsu_larger(m, sh[i][threadIdx.x]);
-        atomicMax(most_of + col, __float_as_uint(m));
+        for (int i = 0; i < 8; ++i) m = katsu_larger(m, sh[i][lane]);
+        largest[piece * n + col] = m;
     }
 }
 
 // A tile of 128 rows of w by 32 columns, through shared memory, to 32 rows of q.
-__global__ void __launch_bounds__(256) quantize_columns_kernel(const float *__restrict__ w, const unsigned *most, int8_t *q,
-                                                               float *scale, size_t k, size_t n, size_t pitch) {
-    __shared__ float tile[128][33];
-    launch_next();
+__global__ void __launch_bounds__(256) quantize_columns_kernel(const float *__restrict__ w, const float *largest, int8_t *q, float *scale,
+                                                               size_t k, size_t n, size_t pitch, unsigned pieces, unsigned tiles,
+                                                               int waves) {
+    __shared__ float tile[128][33], sh[8][33];
+    if (!waves) launch_next();
     launch_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const size_t p0 = size_t(blockIdx.y) * 128, col0 = size_t(blockIdx.x) * 32;
+    const unsigned part = blockIdx.x / tiles;
+    const size_t p0 = size_t(part) * 128, col0 = size_t(blockIdx.x - part * tiles) * 32;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
         const size_t p = p0 + warp + 8 * i;
         tile[warp + 8 * i][lane] = p < k && col0 + lane < n ? __ldg(w + p * n + col0 + lane) : 0.f;
     }
+    float m = 0.f;
+    if (col0 + lane < n)
+        for (unsigned piece = warp; piece < pieces; piece += 8) m = katsu_larger(m, __ldcg(largest + piece * n + col0 + lane));
+    sh[warp][lane] = m;
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const size_t col = col0 + warp + 8 * i;
         if (col >= n) break;
-        const KatsuInt8Scale s = katsu_int8_scale(__uint_as_float(__ldcg(most + col)));
-        if (blockIdx.y == 0 && lane == 0) scale[col] = s.scale;
+        float most = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) most = katsu_larger(most, sh[j][warp + 8 * i]);
+        const KatsuInt8Scale s = katsu_int8_scale(most);
+        if (part == 0 && lane == 0) scale[col] = s.scale;
         const size_t p = p0 + 4 * lane;
         if (p >= pitch) continue;
         const float v[4] = {tile[4 * lane][warp + 8 * i], tile[4 * lane + 1][warp + 8 * i], tile[4 * lane + 2][warp + 8 * i],
@@ -185,15 +199,18 @@ extern "C" int32_t katsu_cuda_int8_quantize_weights(katsu_cuda_ctx *ctx, const f
     KATSU_REQUIRE(w != nullptr && q != nullptr && scale != nullptr, "null buffer");
     KATSU_REQUIRE((reinterpret_cast<uintptr_t>(q) & 15u) == 0, "a quantised matrix must be 16-byte aligned");
     KATSU_TRY(katsu_bind(ctx));
-    float *most = nullptr;
-    KATSU_TRY(katsu_scratch(ctx, n, &most));
-    KATSU_CUDA_TRY(cudaMemsetAsync(most, 0, n * sizeof(float), ctx->stream));
-    const unsigned tiles = (unsigned)katsu_div_up(n, 32);
+    const size_t tiles = katsu_div_up(n, 32), parts = katsu_div_up(k, 128), resident = size_t(ctx->num_sms) * 8;
     // pieces of at least 64 rows, about eight blocks to an SM
-    size_t pieces = katsu_div_up(size_t(ctx->num_sms) * 8, tiles);
+    size_t pieces = resident / tiles;
     if (pieces > katsu_div_up(k, 64)) pieces = katsu_div_up(k, 64);
-    KATSU_LAUNCH(ctx, column_largest_kernel, dim3(tiles, (unsigned)pieces), 256, 0, w, reinterpret_cast<unsigned *>(most), k, n);
-    KATSU_LAUNCH(ctx, quantize_columns_kernel, dim3(tiles, (unsigned)katsu_div_up(k, 128)), 256, 0, w,
-                 reinterpret_cast<const unsigned *>(most), q, scale, k, n, katsu_int8_pitch(k));
+    if (pieces < 1) pieces = 1;
+    if (parts * tiles > 0x7fffffff) return katsu_set_error(KATSU_ERR_UNSUPPORTED, "too many weights");
+    float *largest = nullptr;
+    KATSU_TRY(katsu_scratch(ctx, pieces * n, &largest));
+    const bool waves_a = pieces * tiles > resident, waves_b = parts * tiles > resident;
+    KATSU_TRY(katsu_launch(ctx, !waves_a, column_largest_kernel, (unsigned)(pieces * tiles), 256, 0, 1, w, largest, k, n,
+                           (unsigned)pieces, (unsigned)tiles, waves_a ? 1 : 0));
+    KATSU_TRY(katsu_launch(ctx, !waves_b, quantize_columns_kernel, (unsigned)(parts * tiles), 256, 0, 1, w, largest, q, scale, k, n,
+                           katsu_int8_pitch(k), (unsigned)pieces, (unsigned)tiles, waves_b ? 1 : 0));
     return KATSU_OK;
 }

@@ -394,6 +394,158 @@ pub fn sgd_step(ctx: &Context, w: &mut DeviceBuf, dw: &DeviceBuf, lr: f32) -> Re
     check(unsafe { ffi::katsu_cuda_sgd_step(ctx.ptr(), w.ptr, dw.ptr, lr, w.len) })
 }
 
+/// A norm's weight and bias, one value per channel.
+#[derive(Clone, Copy)]
+pub struct NormWeights<'a> {
+    pub weight: &'a DeviceBuf,
+    pub bias: Option<&'a DeviceBuf>,
+}
+
+/// Kind and eps of the norms around a block, and the residual scale.
+#[derive(Debug, Clone, Copy)]
+pub struct BlockNorm {
+    pub layer: bool,
+    pub eps: f32,
+    pub scale: f32,
+    pub rows: usize,
+    pub cols: usize,
+}
+
+impl BlockNorm {
+    fn kind(&self) -> i32 {
+        if self.layer { ffi::KATSU_NORM_LAYER } else { ffi::KATSU_NORM_RMS }
+    }
+    fn gate_rows(&self, gate: Option<&DeviceBuf>) -> usize {
+        gate.map_or(0, |g| if self.cols == 0 { 0 } else { g.len / self.cols })
+    }
+    fn weights(&self, w: Option<NormWeights<'_>>) -> Result<(*const f32, *const f32), CudaError> {
+        if let Some(w) = w {
+            length("weight", w.weight, self.cols)?;
+            if let Some(b) = w.bias {
+                length("bias", b, self.cols)?;
+            }
+        }
+        Ok((opt_const(w.map(|w| w.weight)), opt_const(w.and_then(|w| w.bias))))
+    }
+}
+
+/// r = x + scale * gate * N(h; post), n = N(r; pre) in one pass; see katsu_cuda_block_norm_fwd for the parts that may be left out.
+pub fn block_norm_forward(ctx: &Context, x: &DeviceBuf, h: Option<&DeviceBuf>, gate: Option<&DeviceBuf>,
+                          post: Option<NormWeights<'_>>, pre: Option<NormWeights<'_>>, r: Option<&mut DeviceBuf>,
+                          n: Option<&mut DeviceBuf>, g: &BlockNorm) -> Result<(), CudaError> {
+    let count = g.rows * g.cols;
+    for buf in [Some(x), h, r.as_deref(), n.as_deref()].into_iter().flatten() {
+        length("x, h, r or n", buf, count)?;
+    }
+    let ((post_w, post_b), (pre_w, pre_b)) = (g.weights(post)?, g.weights(pre)?);
+    check(unsafe {
+        ffi::katsu_cuda_block_norm_fwd(ctx.ptr(), x.ptr, opt_const(h), opt_const(gate), g.gate_rows(gate), post_w, post_b, pre_w,
+                                       pre_b, g.scale, g.eps, g.kind(), opt_mut(r), opt_mut(n), g.rows, g.cols)
+    })
+}
+
+/// What `block_norm_backward` writes; `None` is skipped.
+#[derive(Default)]
+pub struct BlockNormGrads<'a> {
+    pub x: Option<&'a mut DeviceBuf>,
+    pub h: Option<&'a mut DeviceBuf>,
+    pub gate: Option<&'a mut DeviceBuf>,
+    pub post_weight: Option<&'a mut DeviceBuf>,
+    pub post_bias: Option<&'a mut DeviceBuf>,
+    pub pre_weight: Option<&'a mut DeviceBuf>,
+    pub pre_bias: Option<&'a mut DeviceBuf>,
+}
+
+/// Its backward.  `accumulate` is a sum of `ffi::KATSU_BLOCK_*`: those outputs are added to their contents.
+pub fn block_norm_backward(ctx: &Context, r: &DeviceBuf, h: Option<&DeviceBuf>, gate: Option<&DeviceBuf>,
+                           post: Option<NormWeights<'_>>, pre_weight: Option<&DeviceBuf>, dr: Option<&DeviceBuf>,
+                           dn: Option<&DeviceBuf>, out: BlockNormGrads<'_>, g: &BlockNorm, accumulate: i32)
+                           -> Result<(), CudaError> {
+    let count = g.rows * g.cols;
+    for buf in [Some(r), h, dr, dn, out.x.as_deref(), out.h.as_deref()].into_iter().flatten() {
+        length("r, h, dr, dn or their gradients", buf, count)?;
+    }
+    let per_channel = [pre_weight, out.post_weight.as_deref(), out.post_bias.as_deref(), out.pre_weight.as_deref(), out.pre_bias.as_deref()];
+    for buf in per_channel.into_iter().flatten() {
+        length("weights or their gradients", buf, g.cols)?;
+    }
+    if let (Some(gate), Some(dgate)) = (gate, out.gate.as_deref()) {
+        length("gate gradient", dgate, gate.len)?;
+    }
+    let (post_w, post_b) = g.weights(post)?;
+    check(unsafe {
+        ffi::katsu_cuda_block_norm_bwd(ctx.ptr(), r.ptr, opt_const(h), opt_const(gate), g.gate_rows(gate), post_w, post_b,
+                                       opt_const(pre_weight), g.scale, g.eps, g.kind(), opt_const(dr), opt_const(dn), opt_mut(out.x),
+                                       opt_mut(out.h), opt_mut(out.gate), opt_mut(out.post_weight), opt_mut(out.post_bias),
+                                       opt_mut(out.pre_weight), opt_mut(out.pre_bias), g.rows, g.cols, accumulate)
+    })
+}
+
+/// Weights [k, n] in 8 bits with a scale per output channel, laid out once for `int8_linear`.
+pub struct Int8Weights {
+    q: DeviceBuf,
+    scale: DeviceBuf,
+    k: usize,
+    n: usize,
+}
+
+impl Int8Weights {
+    pub fn new(ctx: &Context, weights: &DeviceBuf, k: usize, n: usize) -> Result<Self, CudaError> {
+        length("weights", weights, k * n)?;
+        let mut bytes = 0usize;
+        check(unsafe { ffi::katsu_cuda_int8_row_bytes(k, &mut bytes) })?;
+        let (q, scale) = (DeviceBuf::zeros(ctx, n * bytes / 4)?, DeviceBuf::zeros(ctx, n)?);
+        check(unsafe { ffi::katsu_cuda_int8_quantize_weights(ctx.ptr(), weights.ptr, q.ptr as *mut i8, scale.ptr, k, n) })?;
+        Ok(Self { q, scale, k, n })
+    }
+}
+
+/// y[m, n] = x[m, k] w + bias with the rows of x in 8 bits too (katsu_cuda_int8_linear).
+pub fn int8_linear(ctx: &Context, x: &DeviceBuf, w: &Int8Weights, bias: Option<&DeviceBuf>, y: &mut DeviceBuf, m: usize)
+                   -> Result<(), CudaError> {
+    length("x", x, m * w.k)?;
+    length("y", y, m * w.n)?;
+    if let Some(b) = bias {
+        length("bias", b, w.n)?;
+    }
+    check(unsafe {
+        ffi::katsu_cuda_int8_linear(ctx.ptr(), x.ptr, w.q.ptr as *const i8, w.scale.ptr, opt_const(bias), y.ptr, m, w.k, w.n)
+    })
+}
+
+/// The norm over all gradients into a one-element buffer.
+pub fn grad_norm(ctx: &Context, grads: &[&DeviceBuf], norm: &mut DeviceBuf) -> Result<(), CudaError> {
+    length("norm", norm, 1)?;
+    let (g, counts): (Vec<*const f32>, Vec<usize>) = grads.iter().map(|b| (b.ptr as *const f32, b.len)).unzip();
+    check(unsafe { ffi::katsu_cuda_grad_norm(ctx.ptr(), g.as_ptr(), counts.as_ptr(), g.len(), norm.ptr) })
+}
+
+/// Scales the gradients in place so that their norm is at most `max_norm`; `norm` receives it as it was.
+pub fn clip_grads(ctx: &Context, grads: &mut [&mut DeviceBuf], max_norm: f32, norm: &mut DeviceBuf) -> Result<(), CudaError> {
+    length("norm", norm, 1)?;
+    let out: Vec<*mut f32> = grads.iter().map(|b| b.ptr).collect();
+    let g: Vec<*const f32> = out.iter().map(|p| *p as *const f32).collect();
+    let counts: Vec<usize> = grads.iter().map(|b| b.len).collect();
+    check(unsafe { ffi::katsu_cuda_clip_grads(ctx.ptr(), g.as_ptr(), out.as_ptr(), counts.as_ptr(), g.len(), max_norm, norm.ptr) })
+}
+
+/// `clip_grads` and `sgd_step` of all weights in one, the gradients left as they are.
+pub fn sgd_step_clipped(ctx: &Context, weights: &mut [&mut DeviceBuf], grads: &[&DeviceBuf], lr: f32, max_norm: f32,
+                        norm: &mut DeviceBuf) -> Result<(), CudaError> {
+    length("norm", norm, 1)?;
+    if weights.len() != grads.len() {
+        return Err(CudaError { code: ffi::KATSU_ERR_INVALID_ARG, message: "as many weights as gradients".to_string() });
+    }
+    for (w, g) in weights.iter().zip(grads) {
+        length("gradient", g, w.len)?;
+    }
+    let w: Vec<*mut f32> = weights.iter().map(|b| b.ptr).collect();
+    let (g, counts): (Vec<*const f32>, Vec<usize>) = grads.iter().map(|b| (b.ptr as *const f32, b.len)).unzip();
+    check(unsafe {
+        ffi::katsu_cuda_sgd_step_clipped(ctx.ptr(), w.as_ptr(), g.as_ptr(), counts.as_ptr(), g.len(), lr, max_norm, norm.ptr)
+    })
+}
+
 /// Data-parallel gradient exchange: one process per GPU, images sharded over ranks, only parameter
 /// gradients cross devices (dW sums over the batch, conv2d.rs:289).
 pub struct Comm {

@@ -209,8 +209,9 @@ int32_t katsu_cuda_matmul_bwd(katsu_cuda_ctx *ctx, const float *a, const float *
  *     n null        no norm behind the sum; pre_w and pre_b are null
  * post_b and pre_b may be null (no bias).  gate is [gate_rows, cols], gate_rows a divisor of rows: 1 (one value a
  * channel), rows (each row its own), or one row of the gate for every rows / gate_rows rows (sequences of one
- * length).  cols is at least 1; without rows nothing is written.  Outputs alias neither inputs nor each other.
- * Sums are f32: squares above the f32 range (values above 1.8e19) overflow to a norm of 0. */
+ * length).  cols is 1 to 2^30 - 1; without rows nothing is written.  Outputs alias neither inputs nor each other.
+ * A row's infinities and NaNs stay in its row.  Sums are f32: squares above the f32 range (values above 1.8e19)
+ * overflow to a norm of 0; a row without spread needs eps > 0. */
 #define KATSU_NORM_RMS 0
 #define KATSU_NORM_LAYER 1
 int32_t katsu_cuda_block_norm_fwd(katsu_cuda_ctx *ctx, const float *x, const float *h, const float *gate,
@@ -221,7 +222,7 @@ int32_t katsu_cuda_block_norm_fwd(katsu_cuda_ctx *ctx, const float *x, const flo
  * zeros; dn is null exactly where pre_w is).  The statistics of the rows are taken again from r and h.
  *     dx = dr + [gradient through N(r; pre)]        dh = [gradient through the gate and N(h; post)] of dx
  *     dgate [gate_rows, cols], dpost_w, dpost_b, dpre_w, dpre_b [cols]: sums over rows, in an order that the
- *     shape fixes
+ *     shape and the buffers' alignment fix
  * Any output may be null.  `accumulate` is a sum of KATSU_BLOCK_*: those outputs are added to their contents. */
 #define KATSU_BLOCK_DX 1
 #define KATSU_BLOCK_DH 2
@@ -266,8 +267,8 @@ int32_t katsu_cuda_int8_linear(katsu_cuda_ctx *ctx, const float *x, const int8_t
 
 /* ---- the norm over all gradients, and clipping ------------------------------
  * norm = sqrt of the sum of all squares over `tensors` buffers of counts[i] floats (counts of 0 are fine), summed
- * in 64 bits in an order that the counts fix; norm[0] is f32 device memory.  The arrays of addresses and counts
- * are host memory, read before the call returns.  No counterpart in the reference. */
+ * in 64 bits in an order that counts and alignment fix; norm[0] is f32 device memory apart from them.  The arrays
+ * of addresses and counts are host memory, read before the call returns.  No counterpart in the reference. */
 int32_t katsu_cuda_grad_norm(katsu_cuda_ctx *ctx, const float *const *grads, const size_t *counts, size_t tensors,
                              float *norm);
 /* out[i] = grads[i] * min(1, max_norm / norm); out[i] may be grads[i] itself, other overlaps of an output are

@@ -1,4 +1,4 @@
-"""katsu_b200 -- Python face of the B200-native Conv2D / matmul hot path.
+"""katsu_b200 -- Python face of the B200-native Conv2D / matmul hot path and the operators around it.
 
 The names mirror katsu_core's public surface (crates/katsu-core/src/lib.rs:5,8):
 Tensor, Conv2D, Op and the TensorError variants.  Each object is a handle into

@@ -103,31 +103,32 @@ struct Row {
 #pragma unroll
         for (int i = 0; i < N; ++i) v[i] = in(i / W) ? v[i] - mean : 0.f;
     }
-    __device__ __forceinline__ void load(float (&v)[N], const float *at) const {
-        at += W * t;
+    // First value of a piece.  Addresses are a row's own, the same in all threads, and this: a register for all arrays.
+    __device__ __forceinline__ unsigned place(int piece) const { return unsigned(W) * unsigned(t + piece * T); }
+    __device__ __forceinline__ void load(float (&v)[N], const float *row) const {
 #pragma unroll
-        for (int q = 0; q < P; ++q, at += W * T)
+        for (int q = 0; q < P; ++q)
             if constexpr (VEC) {
-                const float4 f = in(q) ? *reinterpret_cast<const float4 *>(at) : make_float4(0.f, 0.f, 0.f, 0.f);
+                const float4 f = in(q) ? *reinterpret_cast<const float4 *>(row + place(q)) : make_float4(0.f, 0.f, 0.f, 0.f);
                 v[4 * q] = f.x; v[4 * q + 1] = f.y; v[4 * q + 2] = f.z; v[4 * q + 3] = f.w;
             } else {
-                v[q] = in(q) ? *at : 0.f;
+                v[q] = in(q) ? row[place(q)] : 0.f;
             }
     }
-    __device__ __forceinline__ void store(const float (&v)[N], float *at, bool add) const {
-        at += W * t;
+    __device__ __forceinline__ void store(const float (&v)[N], float *row, bool add) const {
 #pragma unroll
-        for (int q = 0; q < P; ++q, at += W * T)
+        for (int q = 0; q < P; ++q)
             if (in(q)) {
                 if constexpr (VEC) {
                     float4 f = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+                    float4 *at = reinterpret_cast<float4 *>(row + place(q));
                     if (add) {
-                        const float4 old = *reinterpret_cast<const float4 *>(at);
+                        const float4 old = *at;
                         f.x += old.x; f.y += old.y; f.z += old.z; f.w += old.w;
                     }
-                    *reinterpret_cast<float4 *>(at) = f;
+                    *at = f;
                 } else {
-                    *at = add ? *at + v[q] : v[q];
+                    row[place(q)] = add ? row[place(q)] + v[q] : v[q];
                 }
             }
     }

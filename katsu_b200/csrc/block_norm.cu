@@ -57,13 +57,12 @@ struct Backward {
 constexpr int kThreads = 256;
 
 // Sums of K values over the block, the same in every thread.  `sh` is used by one round; the next round takes another.
-template <int K, int T>
+template <int K>
 __device__ __forceinline__ void block_sums(float (&v)[K], float (*sh)[32]) {
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
-    if (T == 32) return;
     if ((threadIdx.x & 31) == 0)
 #pragma unroll
         for (int k = 0; k < K; ++k) sh[k][threadIdx.x >> 5] = v[k];
@@ -72,7 +71,7 @@ __device__ __forceinline__ void block_sums(float (&v)[K], float (*sh)[32]) {
     for (int k = 0; k < K; ++k) {
         float t = 0.f;
 #pragma unroll
-        for (int q = 0; q < T / 32; ++q) t += sh[k][q];
+        for (int q = 0; q < kThreads / 32; ++q) t += sh[k][q];
         v[k] = t;
     }
 }
@@ -300,8 +299,8 @@ constexpr int kValues = 8;       // a thread's, in the backward
 constexpr int kMostCluster = 4;  // blocks to a row
 
 // Backward of rows that a block (or a cluster of blocks, each with a slab of `width` columns) holds, eight values a thread.  A
-// thread keeps its columns' sums over the block's rows in registers.  What bounds it is the instructions of a row, about 450 a
-// warp at 2048 values and 16 warps to an SM, beside the 2000 clocks that HBM takes for that row on every SM.
+// thread keeps its columns' sums over the block's rows in registers.  What bounds it is the instructions of a row
+// and its two rounds of sums, with 16 warps to an SM, beside the 2000 clocks that HBM takes for 2048 values on every SM.
 //
 // Layer norms on clusters: the mean is each block's own at first, and the sums about it are moved to the row's mean when the
 // blocks exchange them, so that a row has two exchanges like one of RMS norms and not three.
@@ -546,11 +545,11 @@ __global__ void __launch_bounds__(kThreads) norm_fwd_long_kernel(const __grid_co
         if (p.post_w) {
             if (LAYER) {
                 for (int j = threadIdx.x; j < p.cols; j += kThreads) hm[0] += h[j];
-                block_sums<1, kThreads>(hm, sh[0]);
+                block_sums(hm, sh[0]);
                 hm[0] *= inv;
             }
             for (int j = threadIdx.x; j < p.cols; j += kThreads) hs[0] += (h[j] - hm[0]) * (h[j] - hm[0]);
-            block_sums<1, kThreads>(hs, sh[1]);
+            block_sums(hs, sh[1]);
             hs[0] = rsqrtf(hs[0] * inv + p.eps);
         }
         for (int j = threadIdx.x; j < p.cols; j += kThreads) {
@@ -567,11 +566,11 @@ __global__ void __launch_bounds__(kThreads) norm_fwd_long_kernel(const __grid_co
         if (p.n) {
             const float *r = h ? p.r + at : x;  // (a thread reads what it has written itself)
             if (LAYER) {
-                block_sums<1, kThreads>(rm, sh[2]);
+                block_sums(rm, sh[2]);
                 rm[0] *= inv;
                 for (int j = threadIdx.x; j < p.cols; j += kThreads) rs[0] += (r[j] - rm[0]) * (r[j] - rm[0]);
             }
-            block_sums<1, kThreads>(rs, sh[3]);
+            block_sums(rs, sh[3]);
             rs[0] = rsqrtf(rs[0] * inv + p.eps);
             for (int j = threadIdx.x; j < p.cols; j += kThreads)
                 p.n[at + j] = (r[j] - rm[0]) * rs[0] * p.pre_w[j] + (p.pre_b ? p.pre_b[j] : 0.f);
@@ -609,7 +608,7 @@ __global__ void __launch_bounds__(kThreads) norm_bwd_long_kernel(const __grid_co
                 m[0] += r[j];
                 if (p.post_w) m[1] += h[j];
             }
-            block_sums<2, kThreads>(m, sh);
+            block_sums(m, sh);
             m[0] *= inv;
             m[1] *= inv;
         }
@@ -623,7 +622,7 @@ __global__ void __launch_bounds__(kThreads) norm_bwd_long_kernel(const __grid_co
             }
             if (p.post_w) v[1] += (h[j] - m[1]) * (h[j] - m[1]);
         }
-        block_sums<4, kThreads>(v, sh4);
+        block_sums(v, sh4);
         const float rs = rsqrtf(v[0] * inv + p.eps), hs = rsqrtf(v[1] * inv + p.eps);
         const float c_hat = v[2] * rs * inv, c_one = LAYER ? v[3] * inv : 0.f;
         auto full = [&](int j, float *hat) {  // D, and r^
@@ -663,7 +662,7 @@ __global__ void __launch_bounds__(kThreads) norm_bwd_long_kernel(const __grid_co
             }
         }
         if (p.post_w && p.dh) {
-            block_sums<2, kThreads>(q, sh2);
+            block_sums(q, sh2);
             q[0] *= inv;
             q[1] = LAYER ? q[1] * inv : 0.f;
             for (int j = threadIdx.x; j < p.cols; j += kThreads) {
@@ -732,7 +731,7 @@ int32_t start(katsu_cuda_ctx *ctx, void (*kernel)(Params...), unsigned grid, uns
 }
 
 // Blocks to an SM, by the registers of the kernels that hold rows (up to 128 a thread).
-unsigned resident_blocks(unsigned threads) { return threads >= 64 ? 512 / threads : 8; }
+unsigned resident_blocks(unsigned threads) { return 512 / threads; }
 
 // Whether rows are whole 16-byte pieces at 16-byte addresses.
 bool pieces(int cols, std::initializer_list<const void *> pointers) {
@@ -785,20 +784,34 @@ BackwardShape backward_shape(const katsu_cuda_ctx *ctx, const Backward &p, std::
     return s;
 }
 
+using BackwardKernel = void (*)(Backward, int);
+
 template <Sums MODE>
-int32_t start_backward_of(katsu_cuda_ctx *ctx, const Backward &p, const BackwardShape &s, size_t blocks) {
-    auto kernel = s.cluster > 1       ? (s.pieces == FULL ? norm_bwd_kernel<MODE, FULL, true> : norm_bwd_kernel<MODE, WHOLE, true>)
-                  : s.pieces == FULL  ? norm_bwd_kernel<MODE, FULL, false>
-                  : s.pieces == WHOLE ? norm_bwd_kernel<MODE, WHOLE, false> : norm_bwd_kernel<MODE, SINGLES, false>;
-    return katsu_launch_chained(ctx, kernel, (unsigned)blocks * s.cluster, s.threads, 0, s.cluster, p, s.slab);
+BackwardKernel backward_of(const BackwardShape &s) {
+    return s.cluster > 1       ? (s.pieces == FULL ? norm_bwd_kernel<MODE, FULL, true> : norm_bwd_kernel<MODE, WHOLE, true>)
+           : s.pieces == FULL  ? norm_bwd_kernel<MODE, FULL, false>
+           : s.pieces == WHOLE ? norm_bwd_kernel<MODE, WHOLE, false> : norm_bwd_kernel<MODE, SINGLES, false>;
 }
 
-template <bool LAYER>
-int32_t start_backward(katsu_cuda_ctx *ctx, const Backward &p, const BackwardShape &s, size_t blocks) {
-    if (s.slab == 0) return start(ctx, norm_bwd_long_kernel<LAYER>, (unsigned)blocks, kThreads, p);
-    const bool bias = p.post_b || p.partial[DPRE_B] || p.partial[DPOST_B];
-    return LAYER ? start_backward_of<LAYER_BIAS>(ctx, p, s, blocks)
-                 : bias ? start_backward_of<RMS_BIAS>(ctx, p, s, blocks) : start_backward_of<RMS>(ctx, p, s, blocks);
+// Blocks (clusters) that go round at once.  Four SMs of a cluster are of one group of SMs, whose number four need not divide: 33
+// clusters of 512 threads a block, where 148 SMs would have 37, and the last four took as long as the others before them
+// (2048 x 16384: 252 us, 33 clusters 149).
+int32_t blocks_at_once(const katsu_cuda_ctx *ctx, BackwardKernel kernel, const BackwardShape &s, size_t *blocks) {
+    *blocks = s.most_blocks;
+    if (s.cluster <= 2) return KATSU_OK;
+    cudaLaunchAttribute of_cluster = {};
+    of_cluster.id = cudaLaunchAttributeClusterDimension;
+    of_cluster.val.clusterDim.x = s.cluster;
+    of_cluster.val.clusterDim.y = of_cluster.val.clusterDim.z = 1;
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(unsigned(s.most_blocks) * s.cluster, 1, 1);
+    config.blockDim = dim3(s.threads, 1, 1);
+    config.attrs = &of_cluster;
+    config.numAttrs = 1;
+    int most = 0;
+    KATSU_CUDA_TRY(cudaOccupancyMaxActiveClusters(&most, kernel, &config));
+    if (most >= 1 && size_t(most) < *blocks) *blocks = size_t(most);
+    return KATSU_OK;
 }
 
 int32_t check_sizes(size_t rows, size_t cols, const float *gate, size_t gate_rows, int32_t kind, float eps) {
@@ -876,7 +889,13 @@ extern "C" int32_t katsu_cuda_block_norm_bwd(katsu_cuda_ctx *ctx, const float *r
     p.gate_of_row = dgate && gate_rows == rows;
     p.groups = dgate && !p.gate_of_row ? gate_rows : 1;
     const BackwardShape shape = backward_shape(ctx, p, {r, h, gate, post_w, post_b, pre_w, dr, dn, dx, dh, dgate});
-    const size_t want = shape.most_blocks < rows ? shape.most_blocks : rows;
+    const bool layer = kind == KATSU_NORM_LAYER, bias = post_b || dpre_b || dpost_b;
+    const BackwardKernel kernel = layer ? backward_of<LAYER_BIAS>(shape) : bias ? backward_of<RMS_BIAS>(shape) : backward_of<RMS>(shape);
+    // Four rows and more to a block behind the fourth block of an SM: what a block adds up is written and read again (4000 rows of
+    // 256 values: 17 us, with sixteen blocks to an SM 25).
+    size_t want = rows / 4 > size_t(ctx->num_sms) * 4 ? rows / 4 : size_t(ctx->num_sms) * 4;
+    if (want > rows) want = rows;
+    if (want > shape.most_blocks) KATSU_TRY(blocks_at_once(ctx, kernel, shape, &want));
     size_t blocks;
     if (p.gate_of_row || dgate == nullptr || p.groups < want) {
         p.slices = (int)(want / p.groups);  // (a block more than go round at once would double the time)
@@ -903,7 +922,10 @@ extern "C" int32_t katsu_cuda_block_norm_bwd(katsu_cuda_ctx *ctx, const float *r
             scratch += blocks * cols;
         }
     }
-    KATSU_TRY(kind == KATSU_NORM_LAYER ? start_backward<true>(ctx, p, shape, blocks) : start_backward<false>(ctx, p, shape, blocks));
+    if (shape.slab == 0)
+        KATSU_TRY(start(ctx, layer ? norm_bwd_long_kernel<true> : norm_bwd_long_kernel<false>, (unsigned)blocks, kThreads, p));
+    else
+        KATSU_TRY(katsu_launch_chained(ctx, kernel, (unsigned)blocks * shape.cluster, shape.threads, 0, shape.cluster, p, shape.slab));
     if (folds.folds == 0) return KATSU_OK;
     unsigned long long items = 0;
     for (int k = 0; k < folds.folds; ++k) items += folds.f[k].results * katsu_div_up(cols, 32);

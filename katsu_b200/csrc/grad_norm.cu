@@ -14,7 +14,6 @@
 #include <math.h>
 
 #include <algorithm>
-#include <new>
 #include <vector>
 
 #include "common.cuh"

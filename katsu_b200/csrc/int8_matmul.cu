@@ -212,7 +212,7 @@ __global__ void __launch_bounds__(256) int8_fold_kernel(const int *__restrict__ 
     for (size_t i = size_t(blockIdx.x) * blockDim.x + threadIdx.x; i < count; i += size_t(gridDim.x) * blockDim.x) {
         int sum = 0;
 #pragma unroll 16
-        for (int s = 0; s < splits; ++s) sum += __ldg(partial + size_t(s) * count + i);
+        for (int s = 0; s < splits; ++s) sum += __ldcg(partial + size_t(s) * count + i);
         const size_t token = i / channels;
         const unsigned channel = unsigned(i - token * channels);
         y[i] = katsu_int8_result(sum, __ldg(xs + token), __ldg(ws + channel), bias ? __ldg(bias + channel) : 0.f);

@@ -27,8 +27,8 @@ constexpr int kHeld = 8;  // 16-byte pieces
 // T threads to a row, each of which holds kHeld 16-byte pieces: the row's last ones, loaded behind what is read twice, so that
 // their registers are free until then.  WAVES: more blocks than are resident at once (see katsu_int8_quantize).
 template <int T, bool VEC, bool WAVES>
-__global__ void __launch_bounds__(T == 32 ? 256 : T) quantize_rows_kernel(const float *__restrict__ x, int8_t *q, float *scale,
-                                                                          unsigned long long rows, size_t k, size_t pitch) {
+__global__ void __launch_bounds__(T == 32 ? 256 : T, WAVES ? 1 : T == 32 ? 3 : 1024 / T)
+quantize_rows_kernel(const float *__restrict__ x, int8_t *q, float *scale, unsigned long long rows, size_t k, size_t pitch) {
     __shared__ float sh[T / 32];
     if (!WAVES) launch_next();
     launch_wait();
@@ -164,7 +164,7 @@ int32_t katsu_int8_quantize(katsu_cuda_ctx *ctx, const float *x, int8_t *q, floa
     const bool warps = k <= 1024;
     const unsigned threads = warps ? 256 : k <= 4096 ? 128 : k <= 8192 ? 256 : k <= 16384 ? 512 : 1024;
     const size_t blocks = warps ? katsu_div_up(m, 8) : m;
-    const bool waves = blocks > size_t(ctx->num_sms) * (warps ? 3 : 1024 / threads);  // by the kernels' registers
+    const bool waves = blocks > size_t(ctx->num_sms) * (warps ? 3 : 1024 / threads);  // (as the kernel's bounds)
     auto kernel = waves ? (vec ? rows_kernel<true, true>(k) : rows_kernel<false, true>(k))
                          : (vec ? rows_kernel<true, false>(k) : rows_kernel<false, false>(k));
     if (!waves) KATSU_TRY(katsu_prepare_kernel(ctx, (const void *)kernel, 0));

@@ -152,6 +152,7 @@ __device__ __forceinline__ void ask_all_ahead(const float *const (&arrays)[COUNT
 }
 
 constexpr int kMostThreads = 512;
+constexpr int kNarrow = 4;  // values a thread of rows of up to 128
 
 // Sums over the threads of a row; WARP: the row is a warp's.  Rounds take the two sets of places in turn: a thread that
 // writes to a set again has passed the barrier of the round between, and so have that set's readers.
@@ -213,7 +214,7 @@ struct Rounds {
 };
 
 template <int N, Pieces PIECES, bool WARP, bool LAYER>
-__global__ void __launch_bounds__(kMostThreads) norm_fwd_kernel(const __grid_constant__ Forward p) {
+__global__ void __launch_bounds__(N == kNarrow ? 128 : kMostThreads, N == kNarrow ? 8 : 1) norm_fwd_kernel(const __grid_constant__ Forward p) {
     __shared__ Places places;
     launch_next();
     if (!WARP) {
@@ -304,10 +305,9 @@ constexpr int kMostCluster = 4;  // blocks to a row
 //
 // Layer norms on clusters: the mean is each block's own at first, and the sums about it are moved to the row's mean when the
 // blocks exchange them, so that a row has two exchanges like one of RMS norms and not three.
-template <Sums MODE, Pieces PIECES, bool CLUSTER>
-__global__ void __launch_bounds__(kMostThreads) norm_bwd_kernel(const __grid_constant__ Backward p, int slab) {
+template <int N, Sums MODE, Pieces PIECES, bool CLUSTER>
+__global__ void __launch_bounds__(N == kNarrow ? 32 : kMostThreads, N == kNarrow ? 24 : 1) norm_bwd_kernel(const __grid_constant__ Backward p, int slab) {
     constexpr bool LAYER = MODE == LAYER_BIAS, BIAS = MODE != RMS;
-    constexpr int N = kValues;
     __shared__ Places places;
     __shared__ __align__(16) float exchange[2][kMostCluster][8];  // CLUSTER: the blocks' sums of a round
     __shared__ uint64_t arrived[2];
@@ -746,15 +746,17 @@ int32_t start_forward(katsu_cuda_ctx *ctx, Forward p) {
     const unsigned long long sms = ctx->num_sms;
     if (p.cols > kMostThreads * (vec ? 32 : 16))
         return start(ctx, norm_fwd_long_kernel<LAYER>, unsigned(p.rows < sms * 4 ? p.rows : sms * 4), kThreads, p);
-    // 16 values a thread, 32 where that would take more than 512 threads; up to 512 values are one warp's
-    const bool wide = p.cols > kMostThreads * 16, warp = p.cols <= 512;
+    // 16 values a thread, 32 where that would take more than 512 threads; up to 512 values are one warp's, up to 128 with four a
+    // thread and twice the warps to an SM (65536 x 128: AAA us, with sixteen a thread 36)
+    const bool wide = p.cols > kMostThreads * 16, warp = p.cols <= 512, narrow = p.cols <= 32 * kNarrow;
     const unsigned threads = warp ? 128 : unsigned(katsu_div_up(katsu_div_up(p.cols, wide ? 32 : 16), 32)) * 32;
-    const unsigned long long need = warp ? katsu_div_up(p.rows, 4) : p.rows, most = sms * resident_blocks(threads);
+    const unsigned long long need = warp ? katsu_div_up(p.rows, 4) : p.rows, most = sms * (narrow ? 8 : resident_blocks(threads));
     // Rows are asked into L2 ahead where little else of the SM runs under a row's rounds: layer norms have two more of them
     // (16384 x 2048: 90 us, 103 without), rows of more than 4096 values leave an SM to one block (8192 x 5120: 108 us, 127).  Two
     // blocks of RMS norms reach 93 % of HBM's rate without and 87 % with it.
     p.ahead = !warp && (LAYER || (threads > 256 && !wide));
-    auto kernel = wide   ? norm_fwd_kernel<32, WHOLE, false, LAYER>
+    auto kernel = wide     ? norm_fwd_kernel<32, WHOLE, false, LAYER>
+                  : narrow ? (vec ? norm_fwd_kernel<kNarrow, WHOLE, true, LAYER> : norm_fwd_kernel<kNarrow, SINGLES, true, LAYER>)
                   : warp ? (vec ? norm_fwd_kernel<16, WHOLE, true, LAYER> : norm_fwd_kernel<16, SINGLES, true, LAYER>)
                          : (vec ? norm_fwd_kernel<16, WHOLE, false, LAYER> : norm_fwd_kernel<16, SINGLES, false, LAYER>);
     return start(ctx, kernel, unsigned(need < most ? need : most), threads, p);
@@ -765,6 +767,7 @@ struct BackwardShape {
     int slab;  // columns to a block; 0: the kernel for rows of any length
     Pieces pieces;
     unsigned threads, cluster;
+    bool narrow;
     size_t most_blocks;
 };
 
@@ -780,7 +783,8 @@ BackwardShape backward_shape(const katsu_cuda_ctx *ctx, const Backward &p, std::
     s.slab = int(katsu_div_up(katsu_div_up(p.cols, s.cluster), 4)) * 4;
     s.threads = unsigned(katsu_div_up(katsu_div_up(s.slab, kValues), 32)) * 32;
     s.pieces = !vec ? SINGLES : p.cols == int(s.cluster * s.threads) * kValues ? FULL : WHOLE;
-    s.most_blocks = size_t(ctx->num_sms) * resident_blocks(s.threads) / s.cluster;
+    s.narrow = p.cols <= 32 * kNarrow;
+    s.most_blocks = size_t(ctx->num_sms) * (s.narrow ? 24 : resident_blocks(s.threads)) / s.cluster;
     return s;
 }
 
@@ -788,9 +792,10 @@ using BackwardKernel = void (*)(Backward, int);
 
 template <Sums MODE>
 BackwardKernel backward_of(const BackwardShape &s) {
-    return s.cluster > 1       ? (s.pieces == FULL ? norm_bwd_kernel<MODE, FULL, true> : norm_bwd_kernel<MODE, WHOLE, true>)
-           : s.pieces == FULL  ? norm_bwd_kernel<MODE, FULL, false>
-           : s.pieces == WHOLE ? norm_bwd_kernel<MODE, WHOLE, false> : norm_bwd_kernel<MODE, SINGLES, false>;
+    return s.cluster > 1 ? (s.pieces == FULL ? norm_bwd_kernel<kValues, MODE, FULL, true> : norm_bwd_kernel<kValues, MODE, WHOLE, true>)
+           : s.narrow    ? (s.pieces == SINGLES ? norm_bwd_kernel<kNarrow, MODE, SINGLES, false> : norm_bwd_kernel<kNarrow, MODE, WHOLE, false>)
+           : s.pieces == FULL  ? norm_bwd_kernel<kValues, MODE, FULL, false>
+           : s.pieces == WHOLE ? norm_bwd_kernel<kValues, MODE, WHOLE, false> : norm_bwd_kernel<kValues, MODE, SINGLES, false>;
 }
 
 // Blocks (clusters) that go round at once.  Four SMs of a cluster are of one group of SMs, whose number four need not divide: 33

@@ -691,23 +691,31 @@ struct Folds {
 
 constexpr int kFoldThreads = 1024;  // 32 columns by 32 parts at a time: one round of loads for 300 blocks' sums
 
-__global__ void __launch_bounds__(kFoldThreads) norm_fold_kernel(const __grid_constant__ Folds p) {
+// Narrow rows leave few columns and many parts: clusters of SPLIT blocks share an item's parts, and the first block adds up what
+// the others write into its shared memory (backward of 8000 x 128: 15 us, 26 with a block to an item).  The two sets of places take turns: a block that writes to a set again
+// has passed the barrier of the item between, and so has that set's reader.
+template <int SPLIT>
+__global__ void __launch_bounds__(kFoldThreads, 2) norm_fold_kernel(const __grid_constant__ Folds p) {
     __shared__ float sh[32][33];
+    __shared__ float sums[2][SPLIT][32];
     launch_next();
+    if (SPLIT > 1) cluster_sync_all();  // all blocks have begun: their shared memory may be written to
     launch_wait();
     const int lane = threadIdx.x & 31, part = threadIdx.x >> 5;
-    const unsigned tiles = unsigned(p.cols + 31) / 32;
-    unsigned long long item = blockIdx.x;
+    const int rank = SPLIT > 1 ? int(cluster_ctarank()) : 0;
+    const unsigned tiles = unsigned(p.cols + 31) / 32, step = gridDim.x / SPLIT;
+    unsigned long long item = blockIdx.x / SPLIT;
+    int turn = 0;
     for (int k = 0; k < p.folds; ++k) {
         const Fold &f = p.f[k];
-        for (; item < f.results * tiles; item += gridDim.x) {
+        for (; item < f.results * tiles; item += step) {
             const unsigned long long result = item / tiles;
             const int col = int(item - result * tiles) * 32 + lane;
             const float *src = f.partial + result * f.parts * p.cols;
             float s = 0.f;
             if (col < p.cols)
 #pragma unroll 10
-                for (int q = part; q < f.parts; q += 32) s += __ldcg(src + size_t(q) * p.cols + col);
+                for (int q = 32 * rank + part; q < f.parts; q += 32 * SPLIT) s += __ldcg(src + size_t(q) * p.cols + col);
             sh[part][lane] = s;
             __syncthreads();
             // warp `part` adds up column `part` of the tile
@@ -715,7 +723,16 @@ __global__ void __launch_bounds__(kFoldThreads) norm_fold_kernel(const __grid_co
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
             const int mine = int(item - result * tiles) * 32 + part;
-            if (lane == 0 && mine < p.cols) {
+            if (SPLIT > 1) {
+                if (lane == 0) st_cluster(map_to_rank(&sums[turn][rank][part], 0), t);
+                __syncwarp();
+                cluster_sync_all();
+                t = 0.f;
+#pragma unroll
+                for (int q = 0; q < SPLIT; ++q) t += sums[turn][q][part];
+                turn ^= 1;
+            }
+            if (lane == 0 && rank == 0 && mine < p.cols) {
                 float *o = f.out + result * p.cols + mine;
                 *o = f.add ? *o + t : t;
             }
@@ -747,7 +764,7 @@ int32_t start_forward(katsu_cuda_ctx *ctx, Forward p) {
     if (p.cols > kMostThreads * (vec ? 32 : 16))
         return start(ctx, norm_fwd_long_kernel<LAYER>, unsigned(p.rows < sms * 4 ? p.rows : sms * 4), kThreads, p);
     // 16 values a thread, 32 where that would take more than 512 threads; up to 512 values are one warp's, up to 128 with four a
-    // thread and twice the warps to an SM (65536 x 128: AAA us, with sixteen a thread 36)
+    // thread and twice the warps to an SM (65536 x 128: 26 us, with sixteen a thread 36)
     const bool wide = p.cols > kMostThreads * 16, warp = p.cols <= 512, narrow = p.cols <= 32 * kNarrow;
     const unsigned threads = warp ? 128 : unsigned(katsu_div_up(katsu_div_up(p.cols, wide ? 32 : 16), 32)) * 32;
     const unsigned long long need = warp ? katsu_div_up(p.rows, 4) : p.rows, most = sms * (narrow ? 8 : resident_blocks(threads));
@@ -896,11 +913,9 @@ extern "C" int32_t katsu_cuda_block_norm_bwd(katsu_cuda_ctx *ctx, const float *r
     const BackwardShape shape = backward_shape(ctx, p, {r, h, gate, post_w, post_b, pre_w, dr, dn, dx, dh, dgate});
     const bool layer = kind == KATSU_NORM_LAYER, bias = post_b || dpre_b || dpost_b;
     const BackwardKernel kernel = layer ? backward_of<LAYER_BIAS>(shape) : bias ? backward_of<RMS_BIAS>(shape) : backward_of<RMS>(shape);
-    // Four rows and more to a block behind the fourth block of an SM: what a block adds up is written and read again (4000 rows of
-    // 256 values: 17 us, with sixteen blocks to an SM 25).
-    size_t want = rows / 4 > size_t(ctx->num_sms) * 4 ? rows / 4 : size_t(ctx->num_sms) * 4;
+    size_t want = 0;
+    KATSU_TRY(blocks_at_once(ctx, kernel, shape, &want));
     if (want > rows) want = rows;
-    if (want > shape.most_blocks) KATSU_TRY(blocks_at_once(ctx, kernel, shape, &want));
     size_t blocks;
     if (p.gate_of_row || dgate == nullptr || p.groups < want) {
         p.slices = (int)(want / p.groups);  // (a block more than go round at once would double the time)
@@ -935,5 +950,9 @@ extern "C" int32_t katsu_cuda_block_norm_bwd(katsu_cuda_ctx *ctx, const float *r
     unsigned long long items = 0;
     for (int k = 0; k < folds.folds; ++k) items += folds.f[k].results * katsu_div_up(cols, 32);
     const unsigned long long most = (unsigned long long)ctx->num_sms * 2;
-    return start(ctx, norm_fold_kernel, unsigned(items < most ? items : most), kFoldThreads, folds);
+    const unsigned grid = unsigned(items < most ? items : most);
+    // (24 clusters of eight are resident at once)
+    if (blocks >= 512 && items <= 24) return katsu_launch_chained(ctx, norm_fold_kernel<8>, grid * 8, kFoldThreads, 0, 8, folds);
+    if (blocks >= 512 && items <= 48) return katsu_launch_chained(ctx, norm_fold_kernel<4>, grid * 4, kFoldThreads, 0, 4, folds);
+    return start(ctx, norm_fold_kernel<1>, grid, kFoldThreads, folds);
 }

@@ -29,6 +29,10 @@ __device__ __forceinline__ void st_async_v4(const void *local, uint64_t *bar, ui
                  : "memory");
 }
 
+__device__ __forceinline__ void st_cluster(uint32_t addr, float v) {
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+}
+
 // Whole-warp bounded wait (mbar_wait_warp) for what other blocks of the cluster have written.
 __device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t *bar, uint32_t parity) {
     uint32_t done;

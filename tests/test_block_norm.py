@@ -54,7 +54,8 @@ def bwd(ctx, d, a, shape, scale, eps, layer, outs, accumulate=0, shift=0, dr=Tru
 
 
 SHAPES = [(1, 1), (1, 4096), (3, 2), (5, 33), (2, 255), (7, 256), (4, 1024), (6, 1367), (3, 4096), (2, 5120), (3, 8191),
-          (2, 8192), (2, 16388), (1, 40001), (300, 64), (1022, 96), (900, 4), (2500, 7)]
+          (2, 8192), (2, 16388), (1, 40001), (300, 64), (1022, 96), (900, 4), (2500, 7),
+          (1200, 250), (600, 128), (40, 8200), (400, 8452)]
 
 
 @pytest.mark.gpu

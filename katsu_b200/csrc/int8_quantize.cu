@@ -1,12 +1,15 @@
 // Matrices to 8 bits: rows of x (one scale a token) and columns of w (one scale an output channel, kept transposed).
 //
-// Rows: a warp (up to 1024 values) or a block of 128 to 1024 threads takes a row and holds it in registers, 32 values a thread,
-// between the largest magnitude and the quotients; of rows above 32768 values what lies in front of these is read again, from
-// L2.  Bound: HBM, 4 bytes in and 1 out a value (8192 x 8192: 53 us, its floor 52).
+// Rows: a warp (up to 1024 values), a block of 128 to 1024 threads or a cluster of blocks takes a row and holds it in registers, 32
+// values a thread, between the largest magnitude and the quotients; of rows that a block cannot hold what lies in front of
+// these is read again, from L2.  Bound: HBM, 4 bytes in and 1 out a value (8192 x 8192: 53 us, its floor 52).
 //
 // Columns: one launch finds the largest magnitudes of pieces of the columns, another folds them and turns tiles of 128 x 32 over
 // in shared memory; w is read twice.
 #include "int8.cuh"
+#include "sm100_pair.cuh"
+
+using namespace sm100;
 
 namespace {
 
@@ -22,33 +25,34 @@ __device__ __forceinline__ void load4(const float *row, size_t j, size_t k, floa
     }
 }
 
-constexpr int kHeld = 8;  // 16-byte pieces
+constexpr int kHeld = 8;        // 16-byte pieces
+constexpr int kMostBlocks = 8;  // to a row: 131072 values are held
 
-// T threads to a row, each of which holds kHeld 16-byte pieces: the row's last ones, loaded behind what is read twice, so that
-// their registers are free until then.  WAVES: more blocks than are resident at once (see katsu_int8_quantize).
-template <int T, bool VEC, bool WAVES>
-__global__ void __launch_bounds__(T == 32 ? 256 : T, WAVES ? 1 : T == 32 ? 3 : 1024 / T)
+// C blocks of T threads to a row, each thread with kHeld 16-byte pieces: the row's last ones, loaded behind what is read twice, so
+// that their registers are free until then.  WAVES: more blocks than are resident at once (see katsu_int8_quantize).
+template <int T, int C, bool VEC, bool WAVES>
+__global__ void __launch_bounds__(T == 32 ? 256 : T, WAVES && T < 512 ? 1 : T == 32 ? 3 : 1024 / T)
 quantize_rows_kernel(const float *__restrict__ x, int8_t *q, float *scale, unsigned long long rows, size_t k, size_t pitch) {
-    __shared__ float sh[T / 32];
+    __shared__ float sh[T / 32], of_block;
     if (!WAVES) launch_next();
     launch_wait();
-    constexpr int per_block = T == 32 ? 8 : 1, batch = 4 * T * kHeld;
-    const int t = threadIdx.x % T;
-    const unsigned long long row = (unsigned long long)blockIdx.x * per_block + threadIdx.x / T;
+    constexpr int per_block = T == 32 ? 8 : 1, TC = T * C, batch = 4 * TC * kHeld;
+    const int t = threadIdx.x % T + (C > 1 ? int(cluster_ctarank()) * T : 0);
+    const unsigned long long row = C > 1 ? blockIdx.x / C : (unsigned long long)blockIdx.x * per_block + threadIdx.x / T;
     if (row >= rows) return;  // (a warp's rows: the others of the block do not wait)
     const float *src = x + row * k;
-    const size_t twice = (pitch - 1) / batch * batch;  // values in front of the held ones
+    const size_t twice = T == 1024 || C == kMostBlocks ? (pitch - 1) / batch * batch : 0;  // values in front of the held ones
     float most = 0.f;
     for (size_t j0 = 0; j0 < twice; j0 += batch) {
         float v[kHeld][4];
 #pragma unroll
-        for (int i = 0; i < kHeld; ++i) load4<VEC>(src, j0 + 4 * (t + i * T), k, v[i]);
+        for (int i = 0; i < kHeld; ++i) load4<VEC>(src, j0 + 4 * (t + i * TC), k, v[i]);
 #pragma unroll
         for (int i = 0; i < kHeld; ++i) most = katsu_larger4(most, v[i]);
     }
     float v[kHeld][4];
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i) load4<VEC>(src, twice + 4 * (t + i * T), k, v[i]);
+    for (int i = 0; i < kHeld; ++i) load4<VEC>(src, twice + 4 * (t + i * TC), k, v[i]);
 #pragma unroll
     for (int i = 0; i < kHeld; ++i) most = katsu_larger4(most, v[i]);
     most = katsu_larger_of_warp(most);
@@ -58,28 +62,40 @@ quantize_rows_kernel(const float *__restrict__ x, int8_t *q, float *scale, unsig
 #pragma unroll
         for (int w = 0; w < T / 32; ++w) most = katsu_larger(most, sh[w]);
     }
+    if (C > 1) {
+        if (threadIdx.x == 0) of_block = most;
+        __syncwarp();
+        cluster_sync_all();
+#pragma unroll
+        for (int c = 0; c < C; ++c) most = katsu_larger(most, ld_cluster(map_to_rank(&of_block, c)));
+        cluster_arrive();  // (a block leaves when the others have read what it found)
+    }
     const KatsuInt8Scale s = katsu_int8_scale(most);
     if (t == 0) scale[row] = s.scale;
     unsigned *dst = reinterpret_cast<unsigned *>(q + row * pitch);
     bool sure = true;
 #pragma unroll
     for (int i = 0; i < kHeld; ++i) {
-        const size_t j = twice + 4 * (t + i * T);
+        const size_t j = twice + 4 * (t + i * TC);
         const unsigned out = katsu_int8_pack(v[i], s, &sure);
         if (j < pitch) dst[j / 4] = out;
     }
     for (size_t j0 = 0; j0 < twice; j0 += batch) {
 #pragma unroll
-        for (int i = 0; i < kHeld; ++i) load4<VEC>(src, j0 + 4 * (t + i * T), k, v[i]);
+        for (int i = 0; i < kHeld; ++i) load4<VEC>(src, j0 + 4 * (t + i * TC), k, v[i]);
 #pragma unroll
-        for (int i = 0; i < kHeld; ++i) dst[(j0 + 4 * (t + i * T)) / 4] = katsu_int8_pack(v[i], s, &sure);
+        for (int i = 0; i < kHeld; ++i) dst[(j0 + 4 * (t + i * TC)) / 4] = katsu_int8_pack(v[i], s, &sure);
     }
     if (!sure)  // this thread's pieces once more, by the definition
-        for (size_t j = 4 * t; j < pitch; j += 4 * T) {
+        for (size_t j = 4 * t; j < pitch; j += 4 * TC) {
             float w[4];
             load4<VEC>(src, j, k, w);
             dst[j / 4] = katsu_int8_pack_exactly(w, s);
         }
+    if (C > 1) {
+        __syncwarp();
+        cluster_wait();
+    }
 }
 
 // Largest magnitude of every column of w [k, n] over each of `pieces` equal pieces of its rows: [pieces][n].  A block has a piece
@@ -148,27 +164,43 @@ __global__ void __launch_bounds__(256) quantize_columns_kernel(const float *__re
 }  // namespace
 
 template <bool VEC, bool WAVES>
-static void (*rows_kernel(size_t k))(const float *, int8_t *, float *, unsigned long long, size_t, size_t) {
-    return k <= 1024    ? quantize_rows_kernel<32, VEC, WAVES>
-           : k <= 4096  ? quantize_rows_kernel<128, VEC, WAVES>
-           : k <= 8192  ? quantize_rows_kernel<256, VEC, WAVES>
-           : k <= 16384 ? quantize_rows_kernel<512, VEC, WAVES> : quantize_rows_kernel<1024, VEC, WAVES>;
+static void (*rows_kernel(size_t k, unsigned cluster))(const float *, int8_t *, float *, unsigned long long, size_t, size_t) {
+    return cluster == 2   ? quantize_rows_kernel<512, 2, VEC, WAVES>
+           : cluster == 4 ? quantize_rows_kernel<512, 4, VEC, WAVES>
+           : cluster > 4  ? quantize_rows_kernel<512, kMostBlocks, VEC, WAVES>
+           : k <= 1024    ? quantize_rows_kernel<32, 1, VEC, WAVES>
+           : k <= 4096    ? quantize_rows_kernel<128, 1, VEC, WAVES>
+           : k <= 8192    ? quantize_rows_kernel<256, 1, VEC, WAVES>
+           : k <= 16384   ? quantize_rows_kernel<512, 1, VEC, WAVES> : quantize_rows_kernel<1024, 1, VEC, true>;
 }
 
 // A row to a warp or block.  Few rows: the launch is chained, like that of the product behind it, and takes the largest
 // shared-memory partition as that does.  More rows than go round at once: the hardware hands them out as others end, the rounds
 // of one hide behind the loads of others, and the kernel wants its L1 for the loads in flight (8192 x 8192: 53 us, with the
 // largest partition 80).
+//
+// Rows of more than 16384 values: clusters of blocks hold each of them where about all are resident at once (with the product,
+// 30 rows of 65536: 16 us, a block to a row 19).  Else clusters wait for places in one group of SMs and a block to a row is
+// faster, that reads what it cannot hold twice (512 rows of 65536: 54 us, in clusters 57).
 int32_t katsu_int8_quantize(katsu_cuda_ctx *ctx, const float *x, int8_t *q, float *scale, size_t m, size_t k) {
     const bool vec = k % 4 == 0 && (reinterpret_cast<uintptr_t>(x) & 15u) == 0;
     const bool warps = k <= 1024;
-    const unsigned threads = warps ? 256 : k <= 4096 ? 128 : k <= 8192 ? 256 : k <= 16384 ? 512 : 1024;
-    const size_t blocks = warps ? katsu_div_up(m, 8) : m;
-    const bool waves = blocks > size_t(ctx->num_sms) * (warps ? 3 : 1024 / threads);  // (as the kernel's bounds)
-    auto kernel = waves ? (vec ? rows_kernel<true, true>(k) : rows_kernel<false, true>(k))
-                         : (vec ? rows_kernel<true, false>(k) : rows_kernel<false, false>(k));
+    const size_t sms = ctx->num_sms;
+    unsigned threads = warps ? 256 : k <= 4096 ? 128 : k <= 8192 ? 256 : 512, cluster = 1;
+    if (k > 16384) {
+        cluster = k <= 32768 ? 2 : k <= 65536 ? 4 : kMostBlocks;
+        if (m * cluster > sms * 2) {
+            cluster = 1;
+            threads = 1024;
+        }
+    }
+    const size_t blocks = warps ? katsu_div_up(m, 8) : m * cluster;
+    // (as the kernels' bounds; clusters leave some SMs idle)
+    const bool waves = blocks > sms * (warps ? 3 : cluster > 1 ? 1 : 1024 / threads);
+    auto kernel = waves ? (vec ? rows_kernel<true, true>(k, cluster) : rows_kernel<false, true>(k, cluster))
+                         : (vec ? rows_kernel<true, false>(k, cluster) : rows_kernel<false, false>(k, cluster));
     if (!waves) KATSU_TRY(katsu_prepare_kernel(ctx, (const void *)kernel, 0));
-    return katsu_launch(ctx, !waves, kernel, (unsigned)blocks, threads, 0, 1, x, q, scale, m, k, katsu_int8_pitch(k));
+    return katsu_launch(ctx, !waves, kernel, (unsigned)blocks, threads, 0, cluster, x, q, scale, m, k, katsu_int8_pitch(k));
 }
 
 extern "C" int32_t katsu_cuda_int8_row_bytes(size_t k, size_t *out_bytes) {

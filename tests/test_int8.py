@@ -48,7 +48,8 @@ SHAPES = [(1, 1, 1), (1, 16, 1), (1, 4096, 4096), (2, 100, 33), (3, 17, 5), (4, 
           (8, 1024, 515), (1, 20000, 3), (2, 60001, 10), (8, 4096, 1000), (9, 64, 40), (16, 128, 256), (16, 144, 257),
           (33, 500, 100), (64, 4096, 128), (100, 1031, 517), (130, 257, 255), (256, 384, 512), (300, 2047, 515),
           (512, 8192, 10), (1021, 333, 700), (40, 30000, 24), (1, 133144, 2), (12, 133144, 3), (5, 16384, 2056), (160, 20000, 8),
-          (300, 9000, 8), (1300, 1100, 8), (4000, 100, 16), (700, 5000, 12)]
+          (300, 9000, 8), (1300, 1100, 8), (4000, 100, 16), (700, 5000, 12), (100, 20001, 8), (20, 65536, 10), (60, 60001, 8),
+          (25, 70001, 5), (320, 40000, 8)]
 
 
 @pytest.mark.gpu

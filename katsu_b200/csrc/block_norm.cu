@@ -152,7 +152,7 @@ __device__ __forceinline__ void ask_all_ahead(const float *const (&arrays)[COUNT
 }
 
 constexpr int kMostThreads = 512;
-constexpr int kNarrow = 4;  // values a thread of rows of up to 128
+constexpr int kNarrow = 4;  // values a thread of narrow rows and of rows taken one value at a time
 
 // Sums over the threads of a row; WARP: the row is a warp's.  Rounds take the two sets of places in turn: a thread that
 // writes to a set again has passed the barrier of the round between, and so have that set's readers.
@@ -214,7 +214,7 @@ struct Rounds {
 };
 
 template <int N, Pieces PIECES, bool WARP, bool LAYER>
-__global__ void __launch_bounds__(N == kNarrow ? 128 : kMostThreads, N == kNarrow ? 8 : 1) norm_fwd_kernel(const __grid_constant__ Forward p) {
+__global__ void __launch_bounds__(kMostThreads, N == kNarrow ? 2 : 1) norm_fwd_kernel(const __grid_constant__ Forward p) {
     __shared__ Places places;
     launch_next();
     if (!WARP) {
@@ -305,8 +305,9 @@ constexpr int kMostCluster = 4;  // blocks to a row
 //
 // Layer norms on clusters: the mean is each block's own at first, and the sums about it are moved to the row's mean when the
 // blocks exchange them, so that a row has two exchanges like one of RMS norms and not three.
-template <int N, Sums MODE, Pieces PIECES, bool CLUSTER>
-__global__ void __launch_bounds__(N == kNarrow ? 32 : kMostThreads, N == kNarrow ? 24 : 1) norm_bwd_kernel(const __grid_constant__ Backward p, int slab) {
+// Blocks of one warp have no barriers and no places to meet at (200000 x 64: 101 us, with them 131).
+template <int N, int THREADS, Sums MODE, Pieces PIECES, bool CLUSTER>
+__global__ void __launch_bounds__(THREADS, (N == kNarrow ? 768 : kMostThreads) / THREADS) norm_bwd_kernel(const __grid_constant__ Backward p, int slab) {
     constexpr bool LAYER = MODE == LAYER_BIAS, BIAS = MODE != RMS;
     __shared__ Places places;
     __shared__ __align__(16) float exchange[2][kMostCluster][8];  // CLUSTER: the blocks' sums of a round
@@ -315,8 +316,10 @@ __global__ void __launch_bounds__(N == kNarrow ? 32 : kMostThreads, N == kNarrow
     const unsigned blocks_a_row = CLUSTER ? unsigned(p.cols + slab - 1) / unsigned(slab) : 1;
     const int c0 = int(rank) * slab, width = CLUSTER ? min(slab, p.cols - c0) : p.cols;
     launch_next();
-    clear_places(places);
-    __syncthreads();
+    if (THREADS > 32) {
+        clear_places(places);
+        __syncthreads();
+    }
     if (CLUSTER) {
         if (threadIdx.x == 0) {
             mbar_init(&arrived[0], 1);
@@ -337,7 +340,7 @@ __global__ void __launch_bounds__(N == kNarrow ? 32 : kMostThreads, N == kNarrow
     const bool gate_each = p.gate && p.rows_per_gate == 1;
     const float *const ahead[5] = {p.r, p.h, p.dn, p.dr, gate_each ? p.gate : nullptr};
 
-    Rounds<false> rounds = {places, 0};
+    Rounds<THREADS == 32> rounds = {places, 0};
     int turn = 0;
     // 4 * QUADS numbers of every block of the cluster, block q's at the result's [q]: a block writes its own to all.  The set of
     // places and barrier that a block writes to again are free: that block has had the exchange between, to which every block
@@ -763,17 +766,19 @@ int32_t start_forward(katsu_cuda_ctx *ctx, Forward p) {
     const unsigned long long sms = ctx->num_sms;
     if (p.cols > kMostThreads * (vec ? 32 : 16))
         return start(ctx, norm_fwd_long_kernel<LAYER>, unsigned(p.rows < sms * 4 ? p.rows : sms * 4), kThreads, p);
-    // 16 values a thread, 32 where that would take more than 512 threads; up to 512 values are one warp's, up to 128 with four a
-    // thread and twice the warps to an SM (65536 x 128: 26 us, with sixteen a thread 36)
-    const bool wide = p.cols > kMostThreads * 16, warp = p.cols <= 512, narrow = p.cols <= 32 * kNarrow;
-    const unsigned threads = warp ? 128 : unsigned(katsu_div_up(katsu_div_up(p.cols, wide ? 32 : 16), 32)) * 32;
-    const unsigned long long need = warp ? katsu_div_up(p.rows, 4) : p.rows, most = sms * (narrow ? 8 : resident_blocks(threads));
+    // 16 values a thread, 32 where that would take more than 512 threads; up to 512 values are one warp's.  Four a thread, with
+    // twice the warps to an SM, for rows of up to 128 values (65536 x 128: 26 us, with sixteen a thread 36) and rows of up to 2048
+    // that go one value at a time (4000 x 1367, layer norms: 37 us, with sixteen 42).
+    const bool wide = p.cols > kMostThreads * 16, narrow = p.cols <= (vec ? 32 : kMostThreads) * kNarrow, warp = p.cols <= (narrow ? 32 * kNarrow : 512);
+    const unsigned threads = warp ? 128 : unsigned(katsu_div_up(katsu_div_up(p.cols, wide ? 32 : narrow ? kNarrow : 16), 32)) * 32;
+    const unsigned long long need = warp ? katsu_div_up(p.rows, 4) : p.rows, most = sms * (narrow ? 1024 / threads : resident_blocks(threads));
     // Rows are asked into L2 ahead where little else of the SM runs under a row's rounds: layer norms have two more of them
     // (16384 x 2048: 90 us, 103 without), rows of more than 4096 values leave an SM to one block (8192 x 5120: 108 us, 127).  Two
     // blocks of RMS norms reach 93 % of HBM's rate without and 87 % with it.
     p.ahead = !warp && (LAYER || (threads > 256 && !wide));
     auto kernel = wide     ? norm_fwd_kernel<32, WHOLE, false, LAYER>
-                  : narrow ? (vec ? norm_fwd_kernel<kNarrow, WHOLE, true, LAYER> : norm_fwd_kernel<kNarrow, SINGLES, true, LAYER>)
+                  : narrow ? (vec ? norm_fwd_kernel<kNarrow, WHOLE, true, LAYER>
+                               : warp ? norm_fwd_kernel<kNarrow, SINGLES, true, LAYER> : norm_fwd_kernel<kNarrow, SINGLES, false, LAYER>)
                   : warp ? (vec ? norm_fwd_kernel<16, WHOLE, true, LAYER> : norm_fwd_kernel<16, SINGLES, true, LAYER>)
                          : (vec ? norm_fwd_kernel<16, WHOLE, false, LAYER> : norm_fwd_kernel<16, SINGLES, false, LAYER>);
     return start(ctx, kernel, unsigned(need < most ? need : most), threads, p);
@@ -797,11 +802,13 @@ BackwardShape backward_shape(const katsu_cuda_ctx *ctx, const Backward &p, std::
         return s;
     }
     s.cluster = p.cols > 2 * most ? 4 : p.cols > most ? 2 : 1;
+    // Four values a thread as in the forward, here with half as many warps again to an SM: 65536 x 128 45 us, with eight a thread
+    // 51; 4000 x 1367, layer norms, 69 and 81.
+    s.narrow = p.cols <= (vec ? 32 : 384) * kNarrow;
     s.slab = int(katsu_div_up(katsu_div_up(p.cols, s.cluster), 4)) * 4;
-    s.threads = unsigned(katsu_div_up(katsu_div_up(s.slab, kValues), 32)) * 32;
+    s.threads = unsigned(katsu_div_up(katsu_div_up(s.slab, s.narrow ? kNarrow : kValues), 32)) * 32;
     s.pieces = !vec ? SINGLES : p.cols == int(s.cluster * s.threads) * kValues ? FULL : WHOLE;
-    s.narrow = p.cols <= 32 * kNarrow;
-    s.most_blocks = size_t(ctx->num_sms) * (s.narrow ? 24 : resident_blocks(s.threads)) / s.cluster;
+    s.most_blocks = size_t(ctx->num_sms) * (s.narrow ? 768 / s.threads : resident_blocks(s.threads)) / s.cluster;
     return s;
 }
 
@@ -809,10 +816,14 @@ using BackwardKernel = void (*)(Backward, int);
 
 template <Sums MODE>
 BackwardKernel backward_of(const BackwardShape &s) {
-    return s.cluster > 1 ? (s.pieces == FULL ? norm_bwd_kernel<kValues, MODE, FULL, true> : norm_bwd_kernel<kValues, MODE, WHOLE, true>)
-           : s.narrow    ? (s.pieces == SINGLES ? norm_bwd_kernel<kNarrow, MODE, SINGLES, false> : norm_bwd_kernel<kNarrow, MODE, WHOLE, false>)
-           : s.pieces == FULL  ? norm_bwd_kernel<kValues, MODE, FULL, false>
-           : s.pieces == WHOLE ? norm_bwd_kernel<kValues, MODE, WHOLE, false> : norm_bwd_kernel<kValues, MODE, SINGLES, false>;
+    constexpr int most = kMostThreads;
+    if (s.cluster > 1) return s.pieces == FULL ? norm_bwd_kernel<kValues, most, MODE, FULL, true> : norm_bwd_kernel<kValues, most, MODE, WHOLE, true>;
+    if (s.narrow && s.threads == 32)
+        return s.pieces == SINGLES ? norm_bwd_kernel<kNarrow, 32, MODE, SINGLES, false> : norm_bwd_kernel<kNarrow, 32, MODE, WHOLE, false>;
+    if (s.narrow) return norm_bwd_kernel<kNarrow, 384, MODE, SINGLES, false>;
+    if (s.threads == 32) return norm_bwd_kernel<kValues, 32, MODE, WHOLE, false>;
+    return s.pieces == FULL    ? norm_bwd_kernel<kValues, most, MODE, FULL, false>
+           : s.pieces == WHOLE ? norm_bwd_kernel<kValues, most, MODE, WHOLE, false> : norm_bwd_kernel<kValues, most, MODE, SINGLES, false>;
 }
 
 // Blocks (clusters) that go round at once.  Four SMs of a cluster are of one group of SMs, whose number four need not divide: 33

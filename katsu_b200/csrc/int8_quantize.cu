@@ -5,7 +5,7 @@
 // these is read again, from L2.  Bound: HBM, 4 bytes in and 1 out a value (8192 x 8192: 53 us, its floor 52).
 //
 // Columns: one launch finds the largest magnitudes of pieces of the columns, another folds them and turns tiles of 128 x 32 over
-// in shared memory; w is read twice.
+// in shared memory; w is read twice, the second time from L2 where it fits.
 #include "int8.cuh"
 #include "sm100_pair.cuh"
 
@@ -121,43 +121,52 @@ __global__ void __launch_bounds__(256) column_largest_kernel(const float *__rest
     }
 }
 
-// A tile of 128 rows of w by 32 columns, through shared memory, to 32 rows of q.
-__global__ void __launch_bounds__(256) quantize_columns_kernel(const float *__restrict__ w, const float *largest, int8_t *q, float *scale,
-                                                               size_t k, size_t n, size_t pitch, unsigned pieces, unsigned tiles,
-                                                               int waves) {
-    __shared__ float tile[128][33], sh[8][33];
+constexpr int kTileBlocks = 5;  // of the kernel below that an SM holds at once
+
+// A tile of 128 rows of w by 32 columns to 32 rows of q.  A thread has 16 rows of one column, so that it needs one scale (with tiles
+// turned over in f32 and a scale for each of a thread's four columns: 30 us at 4096 x 4096, now 20), and four of their whole
+// numbers are a word of the tile that shared memory turns over.
+__global__ void __launch_bounds__(256, kTileBlocks) quantize_columns_kernel(const float *__restrict__ w, const float *largest, int8_t *q,
+                                                                            float *scale, size_t k, size_t n, size_t pitch,
+                                                                            unsigned pieces, unsigned tiles, int waves) {
+    __shared__ unsigned tile[32][33];  // [column][word]
+    __shared__ float sh[8][32];
     if (!waves) launch_next();
     launch_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const unsigned part = blockIdx.x / tiles;
     const size_t p0 = size_t(part) * 128, col0 = size_t(blockIdx.x - part * tiles) * 32;
+    const bool in = col0 + lane < n;
+    const float *src = w + (p0 + 16 * warp) * n + col0 + lane;
+    float v[4][4];
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-        const size_t p = p0 + warp + 8 * i;
-        tile[warp + 8 * i][lane] = p < k && col0 + lane < n ? __ldg(w + p * n + col0 + lane) : 0.f;
+        v[i >> 2][i & 3] = in && p0 + 16 * warp + i < k ? __ldg(src) : 0.f;
+        src += n;
     }
     float m = 0.f;
-    if (col0 + lane < n)
+    if (in)
         for (unsigned piece = warp; piece < pieces; piece += 8) m = katsu_larger(m, __ldcg(largest + piece * n + col0 + lane));
     sh[warp][lane] = m;
     __syncthreads();
 #pragma unroll
+    for (int j = 0; j < 8; ++j) m = katsu_larger(m, sh[j][lane]);
+    const KatsuInt8Scale s = katsu_int8_scale(m);
+    if (part == 0 && warp == 0 && in) scale[col0 + lane] = s.scale;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        bool sure = true;
+        unsigned out = katsu_int8_pack(v[i], s, &sure);
+        if (!sure) out = katsu_int8_pack_exactly(v[i], s);
+        tile[lane][4 * warp + i] = out;
+    }
+    __syncthreads();
+    const size_t p = p0 + 4 * lane;
+    if (p >= pitch) return;
+#pragma unroll
     for (int i = 0; i < 4; ++i) {
         const size_t col = col0 + warp + 8 * i;
-        if (col >= n) break;
-        float most = 0.f;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) most = katsu_larger(most, sh[j][warp + 8 * i]);
-        const KatsuInt8Scale s = katsu_int8_scale(most);
-        if (part == 0 && lane == 0) scale[col] = s.scale;
-        const size_t p = p0 + 4 * lane;
-        if (p >= pitch) continue;
-        const float v[4] = {tile[4 * lane][warp + 8 * i], tile[4 * lane + 1][warp + 8 * i], tile[4 * lane + 2][warp + 8 * i],
-                            tile[4 * lane + 3][warp + 8 * i]};
-        bool sure = true;
-        unsigned out = katsu_int8_pack(v, s, &sure);
-        if (!sure) out = katsu_int8_pack_exactly(v, s);
-        *reinterpret_cast<unsigned *>(q + col * pitch + p) = out;
+        if (col < n) *reinterpret_cast<unsigned *>(q + col * pitch + p) = tile[warp + 8 * i][lane];
     }
 }
 
@@ -239,7 +248,7 @@ extern "C" int32_t katsu_cuda_int8_quantize_weights(katsu_cuda_ctx *ctx, const f
     if (parts * tiles > 0x7fffffff) return katsu_set_error(KATSU_ERR_UNSUPPORTED, "too many weights");
     float *largest = nullptr;
     KATSU_TRY(katsu_scratch(ctx, pieces * n, &largest));
-    const bool waves_a = pieces * tiles > resident, waves_b = parts * tiles > resident;
+    const bool waves_a = pieces * tiles > resident, waves_b = parts * tiles > size_t(ctx->num_sms) * kTileBlocks;
     KATSU_TRY(katsu_launch(ctx, !waves_a, column_largest_kernel, (unsigned)(pieces * tiles), 256, 0, 1, w, largest, k, n,
                            (unsigned)pieces, (unsigned)tiles, waves_a ? 1 : 0));
     KATSU_TRY(katsu_launch(ctx, !waves_b, quantize_columns_kernel, (unsigned)(parts * tiles), 256, 0, 1, w, largest, q, scale, k, n,

@@ -74,3 +74,34 @@ def test_steps_without_waiting(ctx, rows, cols, layer):
     for how in ("at once", "captured"):
         for (name, v), (_, got) in zip(want, run(ctx, a, rows, cols, layer, how)):
             assert np.array_equal(v, got), (how, name)
+
+
+@pytest.mark.gpu
+def test_two_contexts_at_once():
+    """A host thread to a context, both over their own buffers: what one computes does not depend on the other."""
+    import threading
+
+    from katsu_b200 import cabi
+
+    sizes = [(8, 520), (300, 256)], [(160, 8300), (1, 512)]
+    contexts = [cabi.Context(0) for _ in sizes]
+    try:
+        alone = [[run(c, state(*s), *s, True, "waiting") for s in pair] for c, pair in zip(contexts, sizes)]
+        together = [[], []]
+
+        def drive(i):
+            for s in sizes[i]:
+                together[i].append(run(contexts[i], state(*s), *s, True, "at once"))
+
+        threads = [threading.Thread(target=drive, args=(i,)) for i in range(2)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        for want, got in zip(alone, together):
+            assert len(got) == 2
+            for a, b in zip(want, got):
+                assert all(np.array_equal(v, w) for (_, v), (_, w) in zip(a, b))
+    finally:
+        for c in contexts:
+            c.close()

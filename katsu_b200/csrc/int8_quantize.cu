@@ -183,10 +183,9 @@ static void (*rows_kernel(size_t k, unsigned cluster))(const float *, int8_t *, 
            : k <= 16384   ? quantize_rows_kernel<512, 1, VEC, WAVES> : quantize_rows_kernel<1024, 1, VEC, true>;
 }
 
-// A row to a warp or block.  Few rows: the launch is chained, like that of the product behind it, and takes the largest
-// shared-memory partition as that does.  More rows than go round at once: the hardware hands them out as others end, the rounds
-// of one hide behind the loads of others, and the kernel wants its L1 for the loads in flight (8192 x 8192: 53 us, with the
-// largest partition 80).
+// A row to a warp or block.  Few rows: the launch is chained, like that of the product behind it.  More rows than go round at once:
+// the hardware hands them out as others end, and the rounds of one hide behind the loads of others.  Either way the kernel wants
+// its L1 for the loads in flight (8192 x 8192: 53 us, with the largest shared-memory partition 80; 64 x 8192 3.1 and 4.3).
 //
 // Rows of more than 16384 values: clusters of blocks hold each of them where about all are resident at once (with the product,
 // 30 rows of 65536: 16 us, a block to a row 19).  Else clusters wait for places in one group of SMs and a block to a row is
@@ -207,8 +206,7 @@ int32_t katsu_int8_quantize(katsu_cuda_ctx *ctx, const float *x, int8_t *q, floa
     // (as the kernels' bounds; clusters leave some SMs idle)
     const bool waves = blocks > sms * (warps ? 3 : cluster > 1 ? 1 : 1024 / threads);
     auto kernel = waves ? (vec ? rows_kernel<true, true>(k, cluster) : rows_kernel<false, true>(k, cluster))
-                         : (vec ? rows_kernel<true, false>(k, cluster) : rows_kernel<false, false>(k, cluster));
-    if (!waves) KATSU_TRY(katsu_prepare_kernel(ctx, (const void *)kernel, 0));
+                        : (vec ? rows_kernel<true, false>(k, cluster) : rows_kernel<false, false>(k, cluster));
     return katsu_launch(ctx, !waves, kernel, (unsigned)blocks, threads, 0, cluster, x, q, scale, m, k, katsu_int8_pitch(k));
 }
 

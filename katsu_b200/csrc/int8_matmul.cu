@@ -57,6 +57,10 @@ __device__ __forceinline__ Tile tile_of(int item, const Problem &p) {
     return t;
 }
 
+// PER: k-blocks to a stage.  The issuing thread's waits and releases, once a stage, take about 470 clocks, in which the operands of two
+// or four narrow blocks arrive and are multiplied (1024 x 4096 by 4096 x 512, tiles of 32 tokens: 12.1 us with one, 8.6 with four;
+// by 4096 x 2048, tiles of 128: 13.3 with one, 10.7 with two).  Wider tiles would have three stages or fewer of more than one.
+template <int PER>
 __global__ void __launch_bounds__(THREADS, 1) int8_pair_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Problem p) {
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -68,7 +72,7 @@ __global__ void __launch_bounds__(THREADS, 1) int8_pair_kernel(const __grid_cons
     const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
     const int items = p.m_tiles * p.n_tiles * p.splits;
     const int half = p.bn >> 1;  // columns of B that this block loads
-    const int b_bytes = half * BK, stage_bytes = A_BYTES + b_bytes;
+    const int b_bytes = half * BK, a_bytes = PER * A_BYTES, stage_bytes = PER * (A_BYTES + b_bytes);
     const int stages = min(MAX_STAGES, SMEM_RING / stage_bytes);
     launch_next();
 
@@ -103,13 +107,18 @@ __global__ void __launch_bounds__(THREADS, 1) int8_pair_kernel(const __grid_cons
             const Tile t = tile_of(item, p);
             const int m0 = (2 * t.mt + int(rank)) * BM, n0 = t.nt * p.bn + int(rank) * half;
             const int kb1 = min((t.split + 1) * p.kb_per_split, p.kblocks);
-            for (int kb = t.split * p.kb_per_split; kb < kb1; ++kb) {
+            for (int kb = t.split * p.kb_per_split; kb < kb1; kb += PER) {
                 if (!mbar_wait(&empty[s], phase, p.status, 181)) { ok = false; break; }
-                if (leader) mbar_arrive_expect_tx(&full[s], 2 * stage_bytes);
+                const int count = min(PER, kb1 - kb);
+                if (leader) mbar_arrive_expect_tx(&full[s], 2 * count * (A_BYTES + b_bytes));
                 const uint32_t bar = map_to_rank(&full[s], 0);
                 unsigned char *st = smem + s * stage_bytes;
-                tma_load_3d_pair(st, &maps.w, bar, kb * BK, m0, 0);
-                tma_load_3d_pair(st + A_BYTES, &maps.x, bar, kb * BK, n0, 0);
+#pragma unroll
+                for (int c = 0; c < PER; ++c) {
+                    if (c >= count) break;
+                    tma_load_3d_pair(st + c * A_BYTES, &maps.w, bar, (kb + c) * BK, m0, 0);
+                    tma_load_3d_pair(st + a_bytes + c * b_bytes, &maps.x, bar, (kb + c) * BK, n0, 0);
+                }
                 if (++s == stages) {
                     s = 0;
                     phase ^= 1;
@@ -130,20 +139,26 @@ __global__ void __launch_bounds__(THREADS, 1) int8_pair_kernel(const __grid_cons
             if (!mbar_wait_warp_ready(&acc_empty[b], ((q >> 1) & 1) ^ 1, p.status, 182)) break;
             tc_fence_after_sync();
             const uint32_t acc = tmem_base + uint32_t(b * 256);
-            for (int kb = kb0; kb < kb1; ++kb) {
+            for (int kb = kb0; kb < kb1; kb += PER) {
                 if (!mbar_wait_warp_ready(&full[s], phase, p.status, 183)) { ok = false; break; }
                 tc_fence_after_sync();
                 const uint32_t st = smem_u32(smem + s * stage_bytes);
-                const uint64_t a0 = smem_desc(st, 16, 1024, kLayoutSw128), b0 = smem_desc(st + A_BYTES, 16, 1024, kLayoutSw128);
-                const int steps = kb == p.kblocks - 1 ? p.last_steps : BK / 32;
+                const int count = min(PER, kb1 - kb);
                 if (issue) {
 #pragma unroll
-                    for (int j = 0; j < BK / 32; ++j)
-                        if (j < steps) mma_i8_pair(acc, a0 + j * 2, b0 + j * 2, idesc, kb > kb0 || j > 0);
+                    for (int c = 0; c < PER; ++c) {
+                        if (c >= count) break;
+                        const uint64_t a0 = smem_desc(st + c * A_BYTES, 16, 1024, kLayoutSw128);
+                        const uint64_t b0 = smem_desc(st + a_bytes + c * b_bytes, 16, 1024, kLayoutSw128);
+                        const int steps = kb + c == p.kblocks - 1 ? p.last_steps : BK / 32;
+#pragma unroll
+                        for (int j = 0; j < BK / 32; ++j)
+                            if (j < steps) mma_i8_pair(acc, a0 + j * 2, b0 + j * 2, idesc, kb + c > kb0 || j > 0);
+                    }
                     // The accumulator's release comes last: the blocks leave when it has been drained, and no arrival may be
                     // outstanding then.
                     mma_commit_both(&empty[s]);
-                    if (kb == kb1 - 1) mma_commit_both(&acc_full[b]);
+                    if (kb + count >= kb1) mma_commit_both(&acc_full[b]);
                 }
                 __syncwarp();
                 if (++s == stages) {
@@ -219,9 +234,12 @@ __global__ void __launch_bounds__(256) int8_fold_kernel(const int *__restrict__ 
     }
 }
 
-// Columns a tile and splits of k, by estimated clocks: a k-block costs the tensor pipe 4 * bn / 2 and the fill of
-// (128 + bn / 2) * 128 bytes a block at about 60 bytes a clock; a tile its start and stores besides; splits the writing and
-// folding of their sums.
+int per_stage(int bn) { return bn <= 64 ? 4 : bn <= 160 ? 2 : 1; }
+
+// Columns a tile and splits of k, by estimated clocks.  A k-block costs the tensor pipe 2 * bn, and the fill of (128 + bn / 2) * 128
+// bytes a block at the rate of L2, 60 bytes a clock for each of 148 blocks and at most 75; a stage's waits are its least.  A tile's
+// start is hidden but for the first one's, its stores but for the last one's (27 clocks a column where all blocks store at
+// once); splits cost the writing and folding of their sums.
 struct Plan {
     int bn, splits;
 };
@@ -232,7 +250,7 @@ Plan plan_for(const katsu_cuda_ctx *ctx, size_t m, size_t k, size_t n) {
     double best_cost = 0;
     for (int bn = 32; bn <= 256; bn += 32) {
         const long long tiles = m_tiles * (long long)katsu_div_up(m, bn);
-        const double pipe = 2.0 * bn, fill = (BM + bn / 2) * 128.0 / 60.0, per_kb = (pipe > fill ? pipe : fill) + 30;
+        const double pipe = 2.0 * bn, least = per_stage(bn) == 4 ? 285 : per_stage(bn) == 2 ? 300 : 470;
         for (int w = 0; w <= 2; ++w) {  // unsplit, or as many splits as fill one or two waves
             long long splits = w == 0 ? 1 : (long long)(w * pairs) / tiles;
             if (w > 0 && splits <= 1) continue;
@@ -241,9 +259,11 @@ Plan plan_for(const katsu_cuda_ctx *ctx, size_t m, size_t k, size_t n) {
             if (splits < 1) splits = 1;
             const long long kb = (kblocks + splits - 1) / splits;
             splits = (kblocks + kb - 1) / kb;
-            const double waves = double((tiles * splits + (long long)pairs - 1) / (long long)pairs);
-            double cost = waves * (kb * per_kb + 1200 + bn * 6);
-            if (splits > 1) cost += (splits + 1) * results * 4 / 2500 + 5000;
+            const double items = double(tiles * splits), waves = ceil(items / pairs), active = items < pairs ? items : pairs;
+            const double rate = 60 * pairs / active, fill = (BM + bn / 2) * 128.0 / (rate < 75 ? rate : 75);
+            const double busy = pipe > fill ? pipe : fill, per_kb = (busy > least ? busy : least) + 10;
+            double cost = waves * (kb * per_kb + 200) + 1200 + bn * 27;
+            if (splits > 1) cost += (splits + 1) * results * 4 / 2500 + 4000;
             if (best.bn == 0 || cost < best_cost) {
                 best.bn = bn;
                 best.splits = (int)splits;
@@ -288,8 +308,9 @@ int32_t many(katsu_cuda_ctx *ctx, const Plan &plan, int *partial, const int8_t *
     const long long items = (long long)p.m_tiles * p.n_tiles * p.splits;
     if (items > 0x3fffffff) return katsu_set_error(KATSU_ERR_UNSUPPORTED, "too many tiles");
     const unsigned pairs = (unsigned)(items < ctx->num_sms / 2 ? items : ctx->num_sms / 2);
-    KATSU_TRY(katsu_prepare_kernel(ctx, (const void *)int8_pair_kernel, SMEM));
-    KATSU_TRY(katsu_launch_chained(ctx, int8_pair_kernel, 2 * pairs, THREADS, SMEM, 2, maps, p));
+    auto kernel = per_stage(plan.bn) == 4 ? int8_pair_kernel<4> : per_stage(plan.bn) == 2 ? int8_pair_kernel<2> : int8_pair_kernel<1>;
+    KATSU_TRY(katsu_prepare_kernel(ctx, (const void *)kernel, SMEM));
+    KATSU_TRY(katsu_launch_chained(ctx, kernel, 2 * pairs, THREADS, SMEM, 2, maps, p));
     if (plan.splits == 1) return KATSU_OK;
     size_t blocks = katsu_div_up(m * n, 256);
     if (blocks > size_t(ctx->num_sms) * 8) blocks = size_t(ctx->num_sms) * 8;

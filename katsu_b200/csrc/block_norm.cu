@@ -12,8 +12,8 @@
 //   D  = dr + dv of N(r; pre) under dn                        = dx
 //   du = scale * gate * D,   dgate = sum of scale * D * u,    dh = dv of N(h; post) under du
 //
-// A row belongs to one block.  Sums over rows (weights, biases, gate) are kept a block and folded by a second launch in a
-// fixed order.  Variances are of differences from the mean, in a round of their own: mean(v^2) - m^2 in 32 bits would lose a
+// A row belongs to one warp or block, in the backward above 4096 values to a cluster of blocks.  Sums over rows (weights, biases,
+// gate) are kept a block and folded by a second launch in a fixed order.  Variances are of differences from the mean, in a round of their own: mean(v^2) - m^2 in 32 bits would lose a
 // row whose mean is a thousand times its spread.
 #include <math.h>
 
@@ -692,11 +692,15 @@ struct Folds {
     int cols, folds;
 };
 
-constexpr int kFoldThreads = 1024;  // 32 columns by 32 parts at a time: one round of loads for 300 blocks' sums
+constexpr int kFoldThreads = 1024;  // 32 columns by 32 parts at a time
+// Parts that are on their way together, also where fewer are left: one round for 300 blocks' sums (an unrolled loop takes its last
+// ones one by one, each after the other's way to L2 and back: backward of 300 x 1024 9.5 us, 8.8 so).  Few parts are better off
+// with that loop (30 x 10000: 10.9 us, 13.2 in batches).
+constexpr int kFoldBatch = 10;
 
 // Narrow rows leave few columns and many parts: clusters of SPLIT blocks share an item's parts, and the first block adds up what
-// the others write into its shared memory (backward of 8000 x 128: 15 us, 26 with a block to an item).  The two sets of places take turns: a block that writes to a set again
-// has passed the barrier of the item between, and so has that set's reader.
+// the others write into its shared memory (backward of 8000 x 128: 15 us, 26 with a block to an item).  The two sets of places take
+// turns: a block that writes to a set again has passed the barrier of the item between, and so has that set's reader.
 template <int SPLIT>
 __global__ void __launch_bounds__(kFoldThreads, 2) norm_fold_kernel(const __grid_constant__ Folds p) {
     __shared__ float sh[32][33];
@@ -716,9 +720,20 @@ __global__ void __launch_bounds__(kFoldThreads, 2) norm_fold_kernel(const __grid
             const int col = int(item - result * tiles) * 32 + lane;
             const float *src = f.partial + result * f.parts * p.cols;
             float s = 0.f;
-            if (col < p.cols)
-#pragma unroll 10
+            if (col < p.cols && f.parts > 96 * SPLIT) {
+                for (int q = 32 * rank + part; q < f.parts; q += 32 * SPLIT * kFoldBatch) {
+                    float v[kFoldBatch];
+#pragma unroll
+                    for (int i = 0; i < kFoldBatch; ++i) {
+                        const int at = q + 32 * SPLIT * i;
+                        v[i] = at < f.parts ? __ldcg(src + size_t(at) * p.cols + col) : 0.f;
+                    }
+#pragma unroll
+                    for (int i = 0; i < kFoldBatch; ++i) s += v[i];
+                }
+            } else if (col < p.cols) {
                 for (int q = 32 * rank + part; q < f.parts; q += 32 * SPLIT) s += __ldcg(src + size_t(q) * p.cols + col);
+            }
             sh[part][lane] = s;
             __syncthreads();
             // warp `part` adds up column `part` of the tile

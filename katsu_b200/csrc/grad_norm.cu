@@ -127,9 +127,16 @@ __global__ void __launch_bounds__(kThreads) squares_kernel(const __grid_constant
 }
 
 // The sum of all partials, the same in every block; the caller's threads all get it.
+template <int BATCH>
 __device__ __forceinline__ double fold(const double *partial, int parts) {
     double acc = 0.0;
-    for (int i = threadIdx.x; i < parts; i += kThreads) acc += __ldcg(partial + i);
+    for (int i = threadIdx.x; i < parts; i += BATCH * kThreads) {  // a batch is on its way together, the last one too
+        double v[BATCH];
+#pragma unroll
+        for (int j = 0; j < BATCH; ++j) v[j] = i + j * kThreads < parts ? __ldcg(partial + i + j * kThreads) : 0.0;
+#pragma unroll
+        for (int j = 0; j < BATCH; ++j) acc += v[j];
+    }
     __shared__ double sh[kThreads / 32];
     return block_sum(acc, sh);
 }
@@ -143,7 +150,7 @@ __device__ __forceinline__ float factor_of(double sum, double norm, float max_no
 __global__ void __launch_bounds__(kThreads) norm_kernel(const double *partial, int parts, float max_norm, float *norm, float *factor) {
     launch_next();
     launch_wait();
-    const double sum = fold(partial, parts), total = sqrt(sum);
+    const double sum = fold<16>(partial, parts), total = sqrt(sum);
     if (threadIdx.x != 0) return;
     norm[0] = (float)total;
     if (factor) *factor = factor_of(sum, total, max_norm);
@@ -193,7 +200,7 @@ __global__ void __launch_bounds__(kThreads) apply_kernel(const __grid_constant__
             __syncthreads();
             c = shared_factor;
         } else if (!known) {
-            const double sum = fold(partial, parts), total = sqrt(sum);
+            const double sum = fold<3>(partial, parts), total = sqrt(sum);
             if (norm != nullptr && blockIdx.x == 0 && threadIdx.x == 0) norm[0] = (float)total;
             c = factor_of(sum, total, max_norm);
         }

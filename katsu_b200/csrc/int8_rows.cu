@@ -9,6 +9,7 @@
 namespace {
 
 constexpr int kWarps = 8, kRows = 2, kUnroll = 4;
+constexpr size_t kMostShared = size_t(200) * 1024;  // a block's tokens
 
 template <int M>
 __global__ void __launch_bounds__(kWarps * 32) int8_rows_kernel(const float *__restrict__ x, const int8_t *__restrict__ xq,
@@ -141,7 +142,7 @@ int32_t katsu_int8_few(katsu_cuda_ctx *ctx, const float *x, const int8_t *xq, co
     const size_t pitch = katsu_int8_pitch(k);
     const int tokens = m <= 1 ? 1 : m <= 2 ? 2 : m <= 4 ? 4 : 8;
     const size_t smem = tokens * pitch;
-    if (m > 8 || smem > size_t(200) * 1024 || n > 0x3fffffff) return KATSU_OK;
+    if (m > 8 || smem > kMostShared || n > 0x3fffffff) return KATSU_OK;
     // Rows in 8 bits come to every block as they are; rows in f32 are four times that, and read twice (2 x 8192 by 8192 x 8192:
     // 32 us, 19 with a launch that quantises them once).
     if (x != nullptr && m * k > 8192) return KATSU_OK;
@@ -150,7 +151,9 @@ int32_t katsu_int8_few(katsu_cuda_ctx *ctx, const float *x, const int8_t *xq, co
     if (m > 4 && k * n > (size_t(1) << 25)) return KATSU_OK;
     *handled = 1;
     auto kernel = tokens == 1 ? int8_rows_kernel<1> : tokens == 2 ? int8_rows_kernel<2> : tokens == 4 ? int8_rows_kernel<4> : int8_rows_kernel<8>;
-    if (smem > size_t(48) * 1024) KATSU_TRY(katsu_prepare_kernel(ctx, (const void *)kernel, smem, false));
+    // Without asking, a block's tokens and the kernel's own variables (up to 800 bytes) have 48 KiB together.  All that a launch may
+    // want is asked for once, so that none depends on the launches before it.
+    KATSU_TRY(katsu_prepare_kernel(ctx, (const void *)kernel, kMostShared, false));
     const size_t pairs = katsu_div_up(n, kRows), warps = size_t(ctx->num_sms) * kWarps * 2;
     int share = 1;
     while (share < kWarps && pairs * share * 2 <= warps) share *= 2;

@@ -252,3 +252,44 @@ def test_refusals(anywhere, name, why, args):  # noqa: F811
     assert call(anywhere, *args) == cabi.ERR_INVALID_ARG
     assert why in lib.katsu_cuda_last_error_string().decode()
     assert call(None, *args) == cabi.ERR_INVALID_ARG
+
+
+# Rows of the few-token kernel in shared memory: a launch's dynamic part on both sides of 48 KiB less the kernel's static part, and of
+# 48 KiB itself.  A process of its own for each: the first launch of a kernel must not depend on a larger one before it.
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,k,n", [(1, 49024, 8), (1, 49152, 8), (1, 49153, 8), (2, 24464, 16), (2, 24576, 16), (2, 24577, 16), (3, 12177, 9),
+                                   (4, 12288, 64), (4, 12289, 64), (5, 6033, 33), (8, 6144, 64), (8, 6145, 64)])
+def test_first_call_of_a_process(m, k, n):
+    import os
+    import subprocess
+    import sys
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    run = subprocess.run([sys.executable, __file__, str(m), str(k), str(n)], capture_output=True, text=True, timeout=300,
+                         env=dict(os.environ, PYTHONPATH=root))
+    assert run.returncode == 0, run.stderr[-2000:]
+
+
+def first_call(m, k, n):
+    x, w = values(m, k, 11), values(k, n, 12)
+    xq, xs = block_ref.quantize(x)
+    wq, ws = block_ref.quantize(w.T)
+    laid = np.zeros((n, pitch(k)), np.int8)
+    laid[:, :k] = wq
+    rows = np.zeros((m, pitch(k)), np.int8)
+    rows[:, :k] = xq
+    ctx = cabi.Context(0)
+    with DeviceArrays(ctx, x=x, wq=laid.view(np.float32), ws=ws, xq=rows.view(np.float32), xs=xs) as d:
+        d.alloc("y", m * n, fill=np.nan)
+        ctx.int8_matmul(d["xq"], d["xs"], d["wq"], d["ws"], None, d["y"], m, k, n)
+        check_result(d.get("y").reshape(m, n), xq, xs, wq, ws, None)
+        d.alloc("y2", m * n, fill=np.nan)
+        ctx.int8_linear(d["x"], d["wq"], d["ws"], None, d["y2"], m, k, n)
+        assert np.array_equal(d.get("y2"), d.get("y"))
+    ctx.close()
+
+
+if __name__ == "__main__":
+    import sys
+
+    first_call(*(int(v) for v in sys.argv[1:]))

@@ -298,12 +298,14 @@ int32_t katsu_f16_conv_fwd(katsu_cuda_ctx *ctx, const float *x, const float *w, 
 
 namespace {
 
+constexpr int kFoldBlocks = 4;  // resident blocks of the kernel below per SM
+
 // dw[k][c][ky][kx] (+)= sum over splits of partial[split][k][(ky, column group, column)].  A
 // block handles 32 elements in the partials' order, eight thread groups each add every eighth split.
-__global__ void __launch_bounds__(256)
-f16_dw_fold_kernel(const __grid_constant__ KatsuF16Raw raw, const float *__restrict__ partial, float *dw, int k, int c, int r, int s, int cp, int groups_per_row, int splits, int accumulate) {
+__global__ void __launch_bounds__(256, kFoldBlocks)
+f16_dw_fold_kernel(const __grid_constant__ KatsuF16Raw raw, const float *__restrict__ partial, float *dw, int k, int c, int r, int s, int cp, int groups_per_row, int splits, int accumulate, int waves) {
     __shared__ float sums[8][32];
-    launch_next();
+    if (!waves) launch_next();
     launch_wait();
     const size_t lanes = size_t(r) * groups_per_row * 64, elems = lanes * k;
     const size_t j = size_t(blockIdx.x) * 32 + (threadIdx.x & 31);
@@ -504,9 +506,11 @@ int32_t katsu_f16_conv_bwd(katsu_cuda_ctx *ctx, const float *x, const float *w, 
             p.b_pairs = b_pairs;
             KATSU_TRY(katsu_f16_launch(ctx, KATSU_F16_CONV_DW, mw, p, plan_dw, partial_dw, (long long)dw_count));
             KATSU_TRY(katsu_prepare_kernel(ctx, (const void *)f16_dw_fold_kernel, 0));
-            KATSU_TRY(katsu_launch_chained(ctx, f16_dw_fold_kernel, (unsigned)katsu_div_up(dw_count, (size_t)32), 256, 0, 1,
-                                           raw_of(KatsuF16Raw::DW, x, gr, g, false, gscale, gfactor), partial_dw, dw, (int)k, (int)c, (int)r, (int)s, (int)cp, (int)gpr, plan_dw.splits,
-                                           accumulate));
+            const size_t blocks = katsu_div_up(dw_count, (size_t)32);
+            const bool waves = blocks > size_t(ctx->num_sms) * kFoldBlocks;
+            KATSU_TRY(katsu_launch(ctx, !waves, f16_dw_fold_kernel, (unsigned)blocks, 256, 0, 1,
+                                   raw_of(KatsuF16Raw::DW, x, gr, g, false, gscale, gfactor), partial_dw, dw, (int)k, (int)c, (int)r, (int)s, (int)cp, (int)gpr, plan_dw.splits,
+                                   accumulate, waves ? 1 : 0));
         }
     }
     return KATSU_OK;

@@ -593,7 +593,9 @@ f16_pair_kernel(const __grid_constant__ KatsuF16Maps maps, const __grid_constant
     if (warp == 9) tmem_dealloc_pair(tmem_base, 512);
 }
 
-__global__ void __launch_bounds__(256)
+constexpr int kFoldBlocks = 4;  // resident blocks of the kernel below per SM
+
+__global__ void __launch_bounds__(256, kFoldBlocks)
 f16_fold_kernel(const __grid_constant__ KatsuF16Raw raw, const float *__restrict__ partial, float *out, size_t count, int splits, int accumulate, const float *bias, size_t channels, size_t plane, int relu) {
     launch_next();
     launch_wait();
@@ -715,7 +717,7 @@ int32_t katsu_f16_launch(katsu_cuda_ctx *ctx, KatsuF16Kind kind, const KatsuF16M
 int32_t katsu_f16_fold(katsu_cuda_ctx *ctx, const KatsuF16Raw &raw, const float *partial, float *out, size_t count, int splits,
                        int accumulate, const float *bias, size_t channels, size_t plane, int relu) {
     size_t blocks = katsu_div_up(count, (size_t)256);
-    if (blocks > size_t(ctx->num_sms) * 8) blocks = size_t(ctx->num_sms) * 8;
+    if (blocks > size_t(ctx->num_sms) * kFoldBlocks) blocks = size_t(ctx->num_sms) * kFoldBlocks;
     KATSU_TRY(katsu_prepare_kernel(ctx, (const void *)f16_fold_kernel, 0));
     return katsu_launch_chained(ctx, f16_fold_kernel, (unsigned)blocks, 256, 0, 1, raw, partial, out, count, splits, accumulate, bias,
                                 channels, plane, relu);

@@ -28,6 +28,7 @@ struct AmaxSegment {
 struct AmaxParams {
     AmaxSegment seg[3];
     int segments;
+    int waves;  // more blocks than are resident at once
 };
 
 __device__ __forceinline__ unsigned magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
@@ -96,7 +97,7 @@ __device__ __forceinline__ void amax_tiles(const AmaxSegment &sg, unsigned first
 
 // Magnitudes compare as their bit patterns, which puts infinities and NaNs above every number.
 __global__ void __launch_bounds__(THREADS, AMAX_BLOCKS) amax_kernel(const __grid_constant__ AmaxParams p) {
-    launch_next();
+    if (!p.waves) launch_next();
     launch_wait();
     int si = 0;
     while (si + 1 < p.segments && blockIdx.x >= p.seg[si + 1].first_block) ++si;
@@ -135,6 +136,7 @@ struct StageParams {
     KatsuStageJob job[KATSU_STAGE_JOBS];
     unsigned first_block[KATSU_STAGE_JOBS], blocks[KATSU_STAGE_JOBS];
     int jobs;
+    int waves;  // more blocks than are resident at once
 };
 
 // How the values of one job are written.
@@ -386,7 +388,7 @@ __device__ void stage_weights(const KatsuStageJob &j, const Writer &out, unsigne
 
 __global__ void __launch_bounds__(THREADS, STAGE_BLOCKS) stage_kernel(const __grid_constant__ StageParams p) {
     __shared__ __align__(16) float tile[4096];
-    launch_next();
+    if (!p.waves) launch_next();
     launch_wait();
     int ji = 0;
     while (ji + 1 < p.jobs && blockIdx.x >= p.first_block[ji + 1]) ++ji;
@@ -467,7 +469,8 @@ int32_t katsu_f16_amax(katsu_cuda_ctx *ctx, const KatsuAmaxJob *jobs, int count)
     }
     if (ctx->f16_captured) KATSU_LAUNCH(ctx, clear_kernel, 1, 32, 0, katsu_f16_slot(ctx, 0));
     KATSU_TRY(katsu_prepare_kernel(ctx, (const void *)amax_kernel, 0));
-    return katsu_launch_chained(ctx, amax_kernel, at, THREADS, 0, 1, p);
+    p.waves = at > unsigned(ctx->num_sms) * AMAX_BLOCKS;
+    return katsu_launch(ctx, !p.waves, amax_kernel, at, THREADS, 0, 1, p);
 }
 
 int32_t katsu_f16_stage(katsu_cuda_ctx *ctx, const KatsuF16Call &call, const KatsuStageJob *jobs, int count) {
@@ -502,5 +505,6 @@ int32_t katsu_f16_stage(katsu_cuda_ctx *ctx, const KatsuF16Call &call, const Kat
     }
     if (at > 0x7fffffffu) return katsu_set_error(KATSU_ERR_UNSUPPORTED, "operand too large to stage");
     KATSU_TRY(katsu_prepare_kernel(ctx, (const void *)stage_kernel, 0));
-    return katsu_launch_chained(ctx, stage_kernel, (unsigned)at, THREADS, 0, 1, p);
+    p.waves = at > size_t(ctx->num_sms) * STAGE_BLOCKS;
+    return katsu_launch(ctx, !p.waves, stage_kernel, (unsigned)at, THREADS, 0, 1, p);
 }

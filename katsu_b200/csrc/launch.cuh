@@ -20,8 +20,10 @@ __device__ __forceinline__ void launch_next() { asm volatile("griddepcontrol.lau
 // that partition leaves 28 KiB (a step over 1.2 GB of gradients and weights each: 682 us with it, 506 without).
 int32_t katsu_prepare_kernel(katsu_cuda_ctx *ctx, const void *kernel, size_t smem, bool largest = true);
 
-// early: the launch may start under its predecessor's end.  Only for grids whose blocks are all resident at once: one that the
-// hardware hands out in waves is launched plainly, and its blocks do not call launch_next().
+// early: the launch may start under its predecessor's end.  Only for grids whose blocks the device holds all at once: one that is
+// handed out in waves is launched plainly, and its blocks do not call launch_next().  (One early form in waves hung; why, is not
+// known.)  Blocks are counted for a device without other work.  Beside a predecessor fewer fit at first, and the rest come as its
+// blocks end: these are all running by then, or nothing would start early, and wait for nothing that comes later.
 template <typename... Params, typename... Args>
 int32_t katsu_launch(katsu_cuda_ctx *ctx, bool early, void (*kernel)(Params...), unsigned grid, unsigned block, size_t smem,
                      unsigned cluster, Args &&...args) {

@@ -579,7 +579,8 @@ class BlockNorm:
             self._h = None
 
     def forward(self, x, h, gate=None):
-        """(r, n); n is None without pre.  gate: [..., channels] with a row for every one or more rows of x."""
+        """(r, n); n is None without pre.  gate: [..., channels] with a row for every one or more
+        rows of x in turn; its axes in front are x's first ones, not its last as in broadcasting."""
         r, n = _vp(), _vp()
         _check(_lib.kh_block_norm_forward(self._h, x._h, h._h, gate._h if gate is not None else None, ctypes.byref(r),
                                           ctypes.byref(n)))

@@ -3,6 +3,7 @@
 // each function); every numeric loop of the reference is a C-ABI call here.
 #include "katsu.hpp"
 
+#include <algorithm>
 #include <cmath>
 #include <unordered_map>
 #include <unordered_set>
@@ -975,6 +976,23 @@ void check_weight(const Norm &norm, size_t cols) {
     if (norm.weight().shape()[0] != cols) fail(ErrorKind::InvalidOperand, "a norm's weight must have one value per channel of the last axis");
 }
 
+// Whether broadcasting would read a gate otherwise than as a row for every run of x's rows: its axes fit x's last ones, are not x's
+// first ones (behind which it may have ones), and one of them stands behind an axis that it would be repeated along.
+bool broadcasts_otherwise(const std::vector<size_t> &x, const std::vector<size_t> &gate) {
+    const size_t axes = x.size() - 1;
+    size_t own = gate.size() - 1;
+    while (own > 0 && gate[own - 1] == 1) --own;
+    if (own <= axes && std::equal(gate.begin(), gate.begin() + own, x.begin())) return false;
+    bool repeated = false, otherwise = false;
+    for (size_t i = 0; i < axes; ++i) {
+        const size_t size = i + gate.size() < x.size() ? 1 : gate[i + gate.size() - x.size()];
+        if (size != 1 && size != x[i]) return false;  // does not broadcast
+        if (size != 1 && repeated) otherwise = true;
+        if (size == 1 && x[i] != 1) repeated = true;
+    }
+    return otherwise;
+}
+
 const float *data_or_null(const Tensor &t) { return t.defined() ? t.device_data() : nullptr; }
 
 Op norm_op(const Norm &norm) {
@@ -1029,6 +1047,8 @@ std::pair<Tensor, Tensor> BlockNorm::forward(const Tensor &x, const Tensor &h, c
     if (gate.defined()) {
         if (gate.rank() == 0 || gate.shape().back() != cols || gate.numel() == 0 || rows % (gate.numel() / cols) != 0)
             fail(ErrorKind::InvalidOperand, "a gate's last axis must be that of x, and its rows must divide those of x");
+        if (broadcasts_otherwise(x.shape(), gate.shape()))
+            fail(ErrorKind::InvalidOperand, "a gate's axes must be the first ones of x, not its last");
         gate_rows = gate.numel() / cols;
     }
     auto r = uninit_buffer(x.numel());

@@ -242,8 +242,9 @@ class BlockNorm {
     const std::optional<Norm> &post() const { return post_; }
     const std::optional<Norm> &pre() const { return pre_; }
     float scale() const { return scale_; }
-    // gate: undefined, or [..., cols] whose rows divide those of x (katsu_cuda_block_norm_fwd).  The second tensor is
-    // undefined without `pre`.
+    // gate: undefined, or [..., cols] with a row for every run of x's rows: one, one each, or a number that divides theirs.  Its axes
+    // in front are x's first ones ([batch, cols] or [batch, 1, cols] for [batch, length, cols]); a shape that fits x's last axes by
+    // broadcasting and means other rows there is refused.  The second tensor is undefined without `pre`.
     std::pair<Tensor, Tensor> forward(const Tensor &x, const Tensor &h, const Tensor &gate) const;
 
    private:

@@ -589,7 +589,8 @@ class BlockNorm:
 
 class Int8Linear:
     """x @ weights + bias in 8-bit integers with a scale for every row of x and every output channel, for serving.  The
-    weights [k, n] are quantised here, once; forward returns a leaf that no gradient passes."""
+    weights [k, n] are quantised and the bias is copied here, once: later steps of the tensors are not seen.  forward returns a
+    leaf that no gradient passes."""
 
     def __init__(self, weights, bias=None):
         out = _vp()

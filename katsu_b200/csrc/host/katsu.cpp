@@ -1091,7 +1091,10 @@ Int8Linear Int8Linear::from_weights(const Tensor &weights, const Tensor &bias) {
         fail(ErrorKind::InvalidOperand, "bias must have one value per output channel");
     if (layer.k_ == 0 || layer.k_ > KATSU_INT8_MAX_K)
         fail(ErrorKind::InvalidOperand, "the 8-bit product sums 1 to " + std::to_string(KATSU_INT8_MAX_K) + " values");
-    layer.bias_ = bias;
+    if (bias.defined()) {  // a copy: a later step of the tensor would leave weights and bias of different steps
+        layer.bias_ = uninit_buffer(layer.n_);
+        if (layer.n_) check(katsu_cuda_d2d(device_context(), layer.bias_->ptr, bias.device_data(), layer.n_));
+    }
     size_t pitch = 0;
     check(katsu_cuda_int8_row_bytes(layer.k_, &pitch));
     layer.q_ = uninit_buffer(element_count({layer.n_, pitch / sizeof(float)}));
@@ -1109,7 +1112,7 @@ Tensor Int8Linear::forward(const Tensor &x) const {
     auto out = uninit_buffer(element_count({m, n_}));
     if (out->count)
         check(katsu_cuda_int8_linear(device_context(), x.device_data(), reinterpret_cast<const int8_t *>(q_->ptr), scale_->ptr,
-                                     data_or_null(bias_), out->ptr, m, k_, n_));
+                                     bias_ ? bias_->ptr : nullptr, out->ptr, m, k_, n_));
     return Tensor::make_node(std::move(out), {m, n_}, Op{}, {});
 }
 

@@ -252,8 +252,8 @@ class BlockNorm {
     float scale_;
 };
 
-// x w + bias with w [k, n] and the rows of x [m, k] in 8 bits (katsu_cuda_int8_linear), for serving: the weights are quantised
-// once, later changes of the tensor are not seen, and what forward returns is a leaf that no gradient passes.
+// x w + bias with w [k, n] and the rows of x [m, k] in 8 bits (katsu_cuda_int8_linear), for serving: the weights are quantised and
+// the bias is copied once, later changes of the tensors are not seen, and what forward returns is a leaf that no gradient passes.
 class Int8Linear {
    public:
     static Int8Linear from_weights(const Tensor &weights, const Tensor &bias);
@@ -263,8 +263,7 @@ class Int8Linear {
 
    private:
     size_t k_ = 0, n_ = 0;
-    std::shared_ptr<DeviceBuffer> q_, scale_;
-    Tensor bias_;
+    std::shared_ptr<DeviceBuffer> q_, scale_, bias_;  // bias_ null: none
 };
 
 // The norm over the gradients of all `tensors`, each listed once, as a leaf of one element; clipping them to max_norm in place;

@@ -621,13 +621,13 @@ class Int8Linear:
 
 
 def _handles(tensors):
-    tensors = list(tensors)
+    """Array and number of the handles of a list of tensors, which the caller holds until the library has returned."""
     return (_vp * len(tensors))(*(t._h for t in tensors)), len(tensors)
 
 
 def grad_norm(tensors):
     """The norm over the gradients of all `tensors`, as a Tensor of one element that stays on the device until it is read."""
-    lib, out = _load(), _vp()
+    lib, out, tensors = _load(), _vp(), list(tensors)
     _check(lib.kh_grad_norm(*_handles(tensors), ctypes.byref(out)))
     return Tensor._wrap(out.value)
 
@@ -635,7 +635,7 @@ def grad_norm(tensors):
 def clip_grad_norm(tensors, max_norm):
     """Scales the gradients of all `tensors` in place so that their norm is at most max_norm; returns the norm before.
     Gradients that hold an infinity or a NaN stay as they are."""
-    lib, out = _load(), _vp()
+    lib, out, tensors = _load(), _vp(), list(tensors)
     _check(lib.kh_clip_grad_norm(*_handles(tensors), float(max_norm), ctypes.byref(out)))
     return Tensor._wrap(out.value)
 
@@ -643,6 +643,6 @@ def clip_grad_norm(tensors, max_norm):
 def sgd_step_clipped(tensors, lr, max_norm):
     """clip_grad_norm and sgd_step of all `tensors` in two launches; the gradients stay as they are.  Returns the norm.
     Where a gradient holds an infinity or a NaN no tensor changes."""
-    lib, out = _load(), _vp()
+    lib, out, tensors = _load(), _vp(), list(tensors)
     _check(lib.kh_sgd_step_clipped(*_handles(tensors), float(lr), float(max_norm), ctypes.byref(out)))
     return Tensor._wrap(out.value)

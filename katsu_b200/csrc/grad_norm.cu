@@ -334,6 +334,7 @@ int32_t checked(katsu_cuda_ctx *ctx, What what, const float *const *grads, float
                 size_t tensors, float lr, float max_norm, float *norm) {
     KATSU_REQUIRE(ctx != nullptr, "null context");
     KATSU_REQUIRE(norm != nullptr, "norm is null");
+    KATSU_REQUIRE(((uintptr_t)norm & 3u) == 0, "norm is not at a whole float");
     KATSU_REQUIRE(tensors == 0 || (grads != nullptr && counts != nullptr), "null array of gradients or counts");
     KATSU_REQUIRE(tensors == 0 || what == NORM_ONLY || dst != nullptr, "null array of outputs or weights");
     KATSU_REQUIRE(what == NORM_ONLY || max_norm >= 0.f, "max_norm must be 0 or more");

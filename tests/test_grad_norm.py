@@ -236,3 +236,13 @@ def test_lists_of_different_lengths_are_refused():
                  lambda c: c.sgd_step_clipped([1, 2], [1], [3], 0.1, 1.0, 4), lambda c: c.clip_grads([1], [1], [3, 3], 1.0, 4)):
         with pytest.raises(ValueError):
             call(Nothing())
+
+
+@pytest.mark.parametrize("norm", [0x90001, 0x90002, 0x90003])
+def test_a_norm_between_two_floats_is_refused(anywhere, norm):  # noqa: F811
+    lib = cabi.load()
+    (w, c), (g, _) = arrays([0x10000], [4]), arrays([0x20000], [4])
+    for call in (lambda: lib.katsu_cuda_grad_norm(anywhere, g, c, 1, norm), lambda: lib.katsu_cuda_clip_grads(anywhere, g, w, c, 1, 1.0, norm),
+                 lambda: lib.katsu_cuda_sgd_step_clipped(anywhere, w, g, c, 1, 0.1, 1.0, norm)):
+        assert call() == cabi.ERR_INVALID_ARG
+        assert "whole float" in lib.katsu_cuda_last_error_string().decode()

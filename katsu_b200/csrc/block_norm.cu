@@ -794,7 +794,7 @@ int32_t start_forward(katsu_cuda_ctx *ctx, Forward p) {
     auto kernel = wide     ? norm_fwd_kernel<32, WHOLE, false, LAYER>
                   : narrow ? (vec ? norm_fwd_kernel<kNarrow, WHOLE, true, LAYER>
                                : warp ? norm_fwd_kernel<kNarrow, SINGLES, true, LAYER> : norm_fwd_kernel<kNarrow, SINGLES, false, LAYER>)
-                  : warp ? (vec ? norm_fwd_kernel<16, WHOLE, true, LAYER> : norm_fwd_kernel<16, SINGLES, true, LAYER>)
+                  : warp ? norm_fwd_kernel<16, WHOLE, true, LAYER>  // (single values: narrow)
                          : (vec ? norm_fwd_kernel<16, WHOLE, false, LAYER> : norm_fwd_kernel<16, SINGLES, false, LAYER>);
     return start(ctx, kernel, unsigned(need < most ? need : most), threads, p);
 }

@@ -263,7 +263,7 @@ enum What { NORM_ONLY, CLIPPED, STEPPED };
 template <int N>
 int32_t run(katsu_cuda_ctx *ctx, What what, const float *const *grads, float *const *dst, const size_t *counts, size_t tensors,
             float lr, float max_norm, float *norm) {
-    static thread_local Tensors<N> t;  // (too large for some hosts' stacks)
+    Tensors<N> t;
     // Partial sums of a launch: more blocks than go round at once, which the hardware hands out as others end, read 15 % faster
     // than each SM's share in one piece (1.2 GB: 170 us, 186), and 9 500 numbers are folded in 4 us.
     const unsigned most = unsigned(ctx->num_sms) * 64;

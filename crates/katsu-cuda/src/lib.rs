@@ -415,8 +415,15 @@ impl BlockNorm {
     fn kind(&self) -> i32 {
         if self.layer { ffi::KATSU_NORM_LAYER } else { ffi::KATSU_NORM_RMS }
     }
-    fn gate_rows(&self, gate: Option<&DeviceBuf>) -> usize {
-        gate.map_or(0, |g| if self.cols == 0 { 0 } else { g.len / self.cols })
+    fn gate_rows(&self, gate: Option<&DeviceBuf>) -> Result<usize, CudaError> {
+        match gate {
+            None => Ok(0),
+            Some(g) if self.cols != 0 && g.len != 0 && g.len % self.cols == 0 => Ok(g.len / self.cols),
+            Some(g) => Err(CudaError {
+                code: ffi::KATSU_ERR_INVALID_ARG,
+                message: format!("gate: {} elements are no whole rows of {}", g.len, self.cols),
+            }),
+        }
     }
     fn weights(&self, w: Option<NormWeights<'_>>) -> Result<(*const f32, *const f32), CudaError> {
         if let Some(w) = w {
@@ -438,8 +445,9 @@ pub fn block_norm_forward(ctx: &Context, x: &DeviceBuf, h: Option<&DeviceBuf>, g
         length("x, h, r or n", buf, count)?;
     }
     let ((post_w, post_b), (pre_w, pre_b)) = (g.weights(post)?, g.weights(pre)?);
+    let gate_rows = g.gate_rows(gate)?;
     check(unsafe {
-        ffi::katsu_cuda_block_norm_fwd(ctx.ptr(), x.ptr, opt_const(h), opt_const(gate), g.gate_rows(gate), post_w, post_b, pre_w,
+        ffi::katsu_cuda_block_norm_fwd(ctx.ptr(), x.ptr, opt_const(h), opt_const(gate), gate_rows, post_w, post_b, pre_w,
                                        pre_b, g.scale, g.eps, g.kind(), opt_mut(r), opt_mut(n), g.rows, g.cols)
     })
 }
@@ -473,8 +481,9 @@ pub fn block_norm_backward(ctx: &Context, r: &DeviceBuf, h: Option<&DeviceBuf>, 
         length("gate gradient", dgate, gate.len)?;
     }
     let (post_w, post_b) = g.weights(post)?;
+    let gate_rows = g.gate_rows(gate)?;
     check(unsafe {
-        ffi::katsu_cuda_block_norm_bwd(ctx.ptr(), r.ptr, opt_const(h), opt_const(gate), g.gate_rows(gate), post_w, post_b,
+        ffi::katsu_cuda_block_norm_bwd(ctx.ptr(), r.ptr, opt_const(h), opt_const(gate), gate_rows, post_w, post_b,
                                        opt_const(pre_weight), g.scale, g.eps, g.kind(), opt_const(dr), opt_const(dn), opt_mut(out.x),
                                        opt_mut(out.h), opt_mut(out.gate), opt_mut(out.post_weight), opt_mut(out.post_bias),
                                        opt_mut(out.pre_weight), opt_mut(out.pre_bias), g.rows, g.cols, accumulate)

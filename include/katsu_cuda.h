@@ -247,7 +247,8 @@ int32_t katsu_cuda_block_norm_bwd(katsu_cuda_ctx *ctx, const float *r, const flo
  * A row (column of w) of zeros has scale 0; one that holds an infinity or a NaN has a NaN for its scale, and so
  * for its results.
  * A quantised matrix of `rows` rows of k values is int8_t [rows][katsu_cuda_int8_row_bytes], the bytes behind k
- * zero, at a 16-byte aligned address; w [k, n] is kept transposed, one row for an output channel. */
+ * zero, at a 16-byte aligned address; w [k, n] is kept transposed, one row for an output channel.  Outputs overlap
+ * neither inputs nor each other. */
 #define KATSU_INT8_MAX_K 133144
 /* k rounded up to whole 16-byte units. */
 int32_t katsu_cuda_int8_row_bytes(size_t k, size_t *out_bytes);

@@ -862,6 +862,13 @@ int32_t blocks_at_once(const katsu_cuda_ctx *ctx, BackwardKernel kernel, const B
     return KATSU_OK;
 }
 
+struct Extent {
+    const float *at;
+    size_t bytes;
+};
+
+bool overlap(const Extent &a, const Extent &b) { return katsu_overlap(a.at, a.bytes, b.at, b.bytes); }
+
 int32_t check_sizes(size_t rows, size_t cols, const float *gate, size_t gate_rows, int32_t kind, float eps) {
     KATSU_REQUIRE(kind == KATSU_NORM_RMS || kind == KATSU_NORM_LAYER, "unknown kind of norm");
     KATSU_REQUIRE(eps >= 0.f && eps < INFINITY, "eps must be 0 or more, and finite");
@@ -887,9 +894,11 @@ extern "C" int32_t katsu_cuda_block_norm_fwd(katsu_cuda_ctx *ctx, const float *x
     KATSU_REQUIRE((h != nullptr) == (r != nullptr) && (r || n), "nothing to compute, or h without r");
     if (rows == 0) return katsu_bind(ctx);
     KATSU_REQUIRE(x != nullptr, "x is null");
-    for (const float *in : {x, h, gate, post_w, post_b, pre_w, pre_b})
-        KATSU_REQUIRE(in == nullptr || (in != r && in != n), "an output is an input too");
-    KATSU_REQUIRE(r != n, "r and n are the same buffer");
+    const size_t all = rows * cols * sizeof(float), channels = cols * sizeof(float), gates = gate_rows * channels;
+    const Extent ins[] = {{x, all}, {h, all}, {gate, gates}, {post_w, channels}, {post_b, channels}, {pre_w, channels}, {pre_b, channels}};
+    for (const Extent &in : ins)
+        KATSU_REQUIRE(!overlap(in, {r, all}) && !overlap(in, {n, all}), "an output is an input too, or overlaps one");
+    KATSU_REQUIRE(!overlap({r, all}, {n, all}), "r and n are the same buffer, or overlap");
     KATSU_TRY(katsu_bind(ctx));
     Forward p = {x, h, gate, post_w, post_b, pre_w, pre_b, r, n, scale, eps, rows, gate ? rows / gate_rows : 1, (int)cols, 0};
     return kind == KATSU_NORM_LAYER ? start_forward<true>(ctx, p) : start_forward<false>(ctx, p);
@@ -909,12 +918,12 @@ extern "C" int32_t katsu_cuda_block_norm_bwd(katsu_cuda_ctx *ctx, const float *r
     KATSU_REQUIRE(gate != nullptr || !dgate, "dgate without a gate");
     KATSU_REQUIRE((pre_w != nullptr) == (dn != nullptr) || rows == 0, "dn and pre_w go together");
     KATSU_REQUIRE(pre_w != nullptr || (!dpre_w && !dpre_b), "dpre_w or dpre_b without pre_w");
-    float *const outs[] = {dx, dh, dgate, dpost_w, dpost_b, dpre_w, dpre_b};
+    const size_t all = rows * cols * sizeof(float), channels = cols * sizeof(float), gates = gate_rows * channels;
+    const Extent outs[] = {{dx, all}, {dh, all}, {dgate, gates}, {dpost_w, channels}, {dpost_b, channels}, {dpre_w, channels}, {dpre_b, channels}};
+    const Extent ins[] = {{r, all}, {h, all}, {gate, gates}, {post_w, channels}, {post_b, channels}, {pre_w, channels}, {dr, all}, {dn, all}};
     for (size_t i = 0; i < 7; ++i) {
-        if (outs[i] == nullptr) continue;
-        for (size_t j = 0; j < i; ++j) KATSU_REQUIRE(outs[i] != outs[j], "two outputs are the same buffer");
-        for (const float *in : {r, h, gate, post_w, post_b, pre_w, dr, dn})
-            KATSU_REQUIRE(in != outs[i], "an output is an input too");
+        for (size_t j = 0; j < i; ++j) KATSU_REQUIRE(!overlap(outs[i], outs[j]), "two outputs are the same buffer, or overlap");
+        for (const Extent &in : ins) KATSU_REQUIRE(!overlap(in, outs[i]), "an output is an input too, or overlaps one");
     }
     const int adds[SUMS] = {accumulate & KATSU_BLOCK_DPRE_W, accumulate & KATSU_BLOCK_DPRE_B, accumulate & KATSU_BLOCK_DPOST_W,
                             accumulate & KATSU_BLOCK_DPOST_B, accumulate & KATSU_BLOCK_DGATE};

@@ -124,6 +124,12 @@ __device__ __forceinline__ float *katsu_dynamic_smem() {
 
 static inline size_t katsu_div_up(size_t a, size_t b) { return (a + b - 1) / b; }
 
+// Whether two buffers (null: none) share a byte.
+static inline bool katsu_overlap(const void *a, size_t a_bytes, const void *b, size_t b_bytes) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return a != nullptr && b != nullptr && x < y + b_bytes && y < x + a_bytes;
+}
+
 // Internal entry points shared between translation units.
 int32_t katsu_conv_direct_fwd(katsu_cuda_ctx *ctx, const float *x, const float *w, float *y,
                               size_t n, size_t c, size_t h, size_t wd, size_t k, size_t r, size_t s,

@@ -328,6 +328,17 @@ int32_t check(const int8_t *wq, const float *ws, const float *y, size_t m, size_
     return KATSU_OK;
 }
 
+// x: `x_bytes` of tokens, in 8 bits with scales xs or in f32.
+int32_t check_apart(const float *y, const void *x, size_t x_bytes, const float *xs, const int8_t *wq, const float *ws,
+                    const float *bias, size_t m, size_t k, size_t n) {
+    const size_t bytes = m * n * sizeof(float), channels = n * sizeof(float);
+    const bool apart = !katsu_overlap(y, bytes, x, x_bytes) && !katsu_overlap(y, bytes, xs, m * sizeof(float)) &&
+                       !katsu_overlap(y, bytes, wq, n * katsu_int8_pitch(k)) && !katsu_overlap(y, bytes, ws, channels) &&
+                       !katsu_overlap(y, bytes, bias, channels);
+    KATSU_REQUIRE(apart, "y is an input too, or overlaps one");
+    return KATSU_OK;
+}
+
 }  // namespace
 
 extern "C" int32_t katsu_cuda_int8_matmul(katsu_cuda_ctx *ctx, const int8_t *xq, const float *xs, const int8_t *wq,
@@ -336,8 +347,7 @@ extern "C" int32_t katsu_cuda_int8_matmul(katsu_cuda_ctx *ctx, const int8_t *xq,
     KATSU_TRY(check(wq, ws, y, m, k, n));
     if (m == 0 || n == 0) return katsu_bind(ctx);
     KATSU_REQUIRE(xq != nullptr && xs != nullptr, "null buffer");
-    for (const void *in : {(const void *)xq, (const void *)xs, (const void *)wq, (const void *)ws, (const void *)bias})
-        KATSU_REQUIRE(in != y, "y is an input too");
+    KATSU_TRY(check_apart(y, xq, m * katsu_int8_pitch(k), xs, wq, ws, bias, m, k, n));
     KATSU_REQUIRE((reinterpret_cast<uintptr_t>(xq) & 15u) == 0, "a quantised matrix must be 16-byte aligned");
     KATSU_TRY(katsu_bind(ctx));
     int handled = 0;
@@ -355,8 +365,7 @@ extern "C" int32_t katsu_cuda_int8_linear(katsu_cuda_ctx *ctx, const float *x, c
     KATSU_TRY(check(wq, ws, y, m, k, n));
     if (m == 0 || n == 0) return katsu_bind(ctx);
     KATSU_REQUIRE(x != nullptr, "null buffer");
-    for (const void *in : {(const void *)x, (const void *)wq, (const void *)ws, (const void *)bias})
-        KATSU_REQUIRE(in != y, "y is an input too");
+    KATSU_TRY(check_apart(y, x, m * k * sizeof(float), nullptr, wq, ws, bias, m, k, n));
     KATSU_TRY(katsu_bind(ctx));
     int handled = 0;
     KATSU_TRY(katsu_int8_few(ctx, x, nullptr, nullptr, wq, ws, bias, y, m, k, n, &handled));

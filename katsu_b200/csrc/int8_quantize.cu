@@ -217,6 +217,14 @@ extern "C" int32_t katsu_cuda_int8_row_bytes(size_t k, size_t *out_bytes) {
     return KATSU_OK;
 }
 
+// `rows` rows of k values to 8 bits.
+static int32_t check_apart(const float *v, const int8_t *q, const float *scale, size_t rows, size_t k) {
+    const size_t in = rows * k * sizeof(float), out = rows * katsu_int8_pitch(k), scales = rows * sizeof(float);
+    const bool apart = !katsu_overlap(q, out, v, in) && !katsu_overlap(scale, scales, v, in) && !katsu_overlap(q, out, scale, scales);
+    KATSU_REQUIRE(apart, "the input and the outputs overlap");
+    return KATSU_OK;
+}
+
 extern "C" int32_t katsu_cuda_int8_quantize_rows(katsu_cuda_ctx *ctx, const float *x, int8_t *q, float *scale, size_t m,
                                                  size_t k) {
     KATSU_REQUIRE(ctx != nullptr, "null context");
@@ -225,6 +233,7 @@ extern "C" int32_t katsu_cuda_int8_quantize_rows(katsu_cuda_ctx *ctx, const floa
     if (m == 0) return katsu_bind(ctx);
     KATSU_REQUIRE(x != nullptr && q != nullptr && scale != nullptr, "null buffer");
     KATSU_REQUIRE((reinterpret_cast<uintptr_t>(q) & 15u) == 0, "a quantised matrix must be 16-byte aligned");
+    KATSU_TRY(check_apart(x, q, scale, m, k));
     KATSU_TRY(katsu_bind(ctx));
     return katsu_int8_quantize(ctx, x, q, scale, m, k);
 }
@@ -237,6 +246,7 @@ extern "C" int32_t katsu_cuda_int8_quantize_weights(katsu_cuda_ctx *ctx, const f
     if (n == 0) return katsu_bind(ctx);
     KATSU_REQUIRE(w != nullptr && q != nullptr && scale != nullptr, "null buffer");
     KATSU_REQUIRE((reinterpret_cast<uintptr_t>(q) & 15u) == 0, "a quantised matrix must be 16-byte aligned");
+    KATSU_TRY(check_apart(w, q, scale, n, k));
     KATSU_TRY(katsu_bind(ctx));
     const size_t tiles = katsu_div_up(n, 32), parts = katsu_div_up(k, 128), resident = size_t(ctx->num_sms) * 8;
     // pieces of at least 64 rows, about eight blocks to an SM

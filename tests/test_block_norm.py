@@ -375,3 +375,34 @@ def test_backward_refuses(anywhere, why, change):
     handle = None if "ctx" in change else anywhere
     assert lib.katsu_cuda_block_norm_bwd(handle, *(args[n] for n in names)) == cabi.ERR_INVALID_ARG
     assert why in lib.katsu_cuda_last_error_string().decode()
+
+
+# rows = 4, cols = 8: x, h, r, n and their gradients 128 bytes, weights 32, a gate of two rows 64
+@pytest.mark.parametrize("why,args", [
+    ("output is an input", (A, B, None, 0, C, None, None, None, 1.0, 1e-6, 0, A + 124, None, 4, 8)),
+    ("output is an input", (A, B, None, 0, C, None, None, None, 1.0, 1e-6, 0, B - 124, None, 4, 8)),
+    ("output is an input", (A, B, None, 0, C, None, None, None, 1.0, 1e-6, 0, C + 28, None, 4, 8)),
+    ("output is an input", (A, B, C, 2, None, None, A, None, 1.0, 1e-6, 0, D, C + 60, 4, 8)),
+    ("output is an input", (A, None, None, 0, None, None, C, B, 1.0, 1e-6, 0, None, B - 124, 4, 8)),
+    ("same buffer", (A, B, None, 0, None, None, C, None, 1.0, 1e-6, 0, D, D + 124, 4, 8)),
+    ("same buffer", (A, B, None, 0, None, None, C, None, 1.0, 1e-6, 0, D, D - 124, 4, 8)),
+])
+def test_forward_refuses_overlaps(anywhere, why, args):
+    lib = cabi.load()
+    assert lib.katsu_cuda_block_norm_fwd(anywhere, *args) == cabi.ERR_INVALID_ARG
+    assert why in lib.katsu_cuda_last_error_string().decode()
+
+
+@pytest.mark.parametrize("why,change", [
+    ("two outputs", {"dx": 0x9000, "dh": 0x907c}), ("two outputs", {"dpre_w": 0x9000, "dpre_b": 0x901c}),
+    ("two outputs", {"dgate": 0x9000, "dpost_w": 0x903c}), ("output is an input", {"dx": 0x4000 - 124}),
+    ("output is an input", {"dh": "dn"}), ("output is an input", {"dgate": "post_w"}), ("output is an input", {"dpost_b": "gate"})])
+def test_backward_refuses_overlaps(anywhere, why, change):
+    names = ["r", "h", "gate", "gate_rows", "post_w", "post_b", "pre_w", "scale", "eps", "kind", "dr", "dn", "dx", "dh", "dgate",
+             "dpost_w", "dpost_b", "dpre_w", "dpre_b", "rows", "cols", "accumulate"]
+    args = {n: 0x100000 + 0x1000 * i for i, n in enumerate(names)}
+    args.update(r=0x4000, gate_rows=2, scale=1.0, eps=1e-6, kind=1, rows=4, cols=8, accumulate=0)
+    args.update({k: args[v] + 4 if isinstance(v, str) else v for k, v in change.items()})
+    lib = cabi.load()
+    assert lib.katsu_cuda_block_norm_bwd(anywhere, *(args[n] for n in names)) == cabi.ERR_INVALID_ARG
+    assert why in lib.katsu_cuda_last_error_string().decode()

@@ -254,6 +254,23 @@ def test_refusals(anywhere, name, why, args):  # noqa: F811
     assert call(None, *args) == cabi.ERR_INVALID_ARG
 
 
+# m = 8, k = 20, n = 6: x 640 bytes, y 192, a quantised row 32
+@pytest.mark.parametrize("name,args", [
+    ("linear", (A[0], A[1], A[2], None, A[0] + 636, 8, 20, 6)), ("linear", (A[0], A[1], A[2], None, A[0] - 188, 8, 20, 6)),
+    ("linear", (A[0], A[1], A[2], None, A[1] + 188, 8, 20, 6)), ("linear", (A[0], A[1], A[2], None, A[2] + 20, 8, 20, 6)),
+    ("linear", (A[0], A[1], A[2], A[3], A[3] - 188, 8, 20, 6)), ("matmul", (A[0], A[4], A[1], A[2], A[3], A[0] + 252, 8, 20, 6)),
+    ("matmul", (A[0], A[4], A[1], A[2], A[3], A[4] + 28, 8, 20, 6)), ("quantize_rows", (A[0], A[0], A[1], 8, 20)),
+    ("quantize_rows", (A[0], A[0] + 624, A[1], 8, 20)), ("quantize_rows", (A[0], A[0] - 240, A[1], 8, 20)),
+    ("quantize_rows", (A[0], A[1], A[0] + 636, 8, 20)), ("quantize_rows", (A[0], A[1], A[1] + 252, 8, 20)),
+    ("quantize_weights", (A[0], A[0] + 464, A[1], 20, 6)), ("quantize_weights", (A[0], A[1], A[0] - 20, 20, 6)),
+    ("quantize_weights", (A[0], A[1], A[1] - 20, 20, 6)),
+])
+def test_overlaps_are_refused(anywhere, name, args):  # noqa: F811
+    lib = cabi.load()
+    assert getattr(lib, "katsu_cuda_int8_" + name)(anywhere, *args) == cabi.ERR_INVALID_ARG
+    assert "input" in lib.katsu_cuda_last_error_string().decode()
+
+
 # Rows of the few-token kernel in shared memory: a launch's dynamic part on both sides of 48 KiB less the kernel's static part, and of
 # 48 KiB itself.  A process of its own for each: the first launch of a kernel must not depend on a larger one before it.
 @pytest.mark.gpu

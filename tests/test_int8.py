@@ -191,6 +191,26 @@ def test_nothing_to_do(ctx, m, n):
         assert (d.get("y") == 2).all()
 
 
+# With 148 SMs: tiles of 32 to 256 tokens, each in two or more rounds (accumulators and the ring's stages go from tile to tile, the last
+# round is not full), and tiles of 128 to 256 with k split.
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,k,n", [(1600, 230, 544), (3372, 247, 584), (3501, 278, 515), (4027, 262, 1319), (2500, 1300, 2100), (4063, 268, 1627),
+                                   (2000, 700, 3000), (4195, 266, 2105), (4271, 270, 2798), (3905, 290, 4441), (1161, 5792, 282), (774, 12396, 274),
+                                   (536, 18790, 522), (1296, 17479, 269), (1748, 17120, 258)])
+def test_many_tokens(ctx, m, k, n):
+    x, w, bias = values(m, k, 13), values(k, n, 14), values(1, n, 15)[0]
+    xq, xs = block_ref.quantize(x)
+    wq, ws = block_ref.quantize(w.T)
+    with DeviceArrays(ctx, x=x, w=w, bias=bias) as d:
+        for name, count in (("wq", floats(n, k)), ("ws", n), ("y", m * n + 8)):
+            d.alloc(name, count, fill=np.nan)
+        ctx.int8_quantize_weights(d["w"], d["wq"], d["ws"], k, n)
+        ctx.int8_linear(d["x"], d["wq"], d["ws"], d["bias"], d["y"], m, k, n)
+        y = d.get("y")
+    assert np.isnan(y[m * n:]).all()
+    check_result(y[:m * n].reshape(m, n), xq.astype(np.float64), xs, wq.astype(np.float64), ws, bias)  # (sums below 2^53 are exact)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("m,k,n", [(1, 4096, 512), (8, 8192, 300), (300, 1024, 600), (32, 8192, 256)])
 def test_replayed_and_on_other_streams(m, k, n):

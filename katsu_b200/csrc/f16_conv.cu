@@ -301,32 +301,37 @@ namespace {
 constexpr int kFoldBlocks = 4;  // resident blocks of the kernel below per SM
 
 // dw[k][c][ky][kx] (+)= sum over splits of partial[split][k][(ky, column group, column)].  A
-// block handles 32 elements in the partials' order, eight thread groups each add every eighth split.
+// block handles 32 elements at a time in the partials' order, eight thread groups each add every eighth split.
 __global__ void __launch_bounds__(256, kFoldBlocks)
 f16_dw_fold_kernel(const __grid_constant__ KatsuF16Raw raw, const float *__restrict__ partial, float *dw, int k, int c, int r, int s, int cp, int groups_per_row, int splits, int accumulate, int waves) {
-    __shared__ float sums[8][32];
+    __shared__ float sums[2][8][32];
     if (!waves) launch_next();
     launch_wait();
     const size_t lanes = size_t(r) * groups_per_row * 64, elems = lanes * k;
-    const size_t j = size_t(blockIdx.x) * 32 + (threadIdx.x & 31);
     const int part = threadIdx.x >> 5;
-    float v = 0.f;
-    if (j < elems)
+    int turn = 0;  // (a warp that writes to a set again has passed the barrier between, and so has that set's reader)
+    for (size_t first = size_t(blockIdx.x) * 32; first < elems; first += size_t(gridDim.x) * 32, turn ^= 1) {
+        const size_t j = first + (threadIdx.x & 31);
+        float v = 0.f;
+        if (j < elems)
 #pragma unroll 4
-        for (int q = part; q < splits; q += 8) v += __ldg(partial + size_t(q) * elems + j);
-    sums[part][threadIdx.x & 31] = v;
-    __syncthreads();
-    if (part != 0 || j >= elems) return;
-    float total = sums[0][threadIdx.x];
+            for (int q = part; q < splits; q += 8) v += __ldg(partial + size_t(q) * elems + j);
+        sums[turn][part][threadIdx.x & 31] = v;
+        __syncthreads();
+        if (part == 0 && j < elems) {
+            float total = sums[turn][0][threadIdx.x];
 #pragma unroll
-    for (int q = 1; q < 8; ++q) total += sums[q][threadIdx.x];
-    const int o = int(j / lanes), m = int(j - size_t(o) * lanes);
-    const int ky = m / (groups_per_row * 64), col = m - ky * groups_per_row * 64;
-    const int kx = col / cp, cc = col - kx * cp;
-    if (kx >= s || cc >= c) return;
-    if (raw.form != KatsuF16Raw::NONE && !katsu_is_number(total) && katsu_f16_mixed(raw, ky, kx)) total = katsu_f16_exact(raw, o, cc, ky, kx);
-    float *dst = dw + ((size_t(o) * c + cc) * r + ky) * s + kx;
-    *dst = accumulate ? *dst + total : total;
+            for (int q = 1; q < 8; ++q) total += sums[turn][q][threadIdx.x];
+            const int o = int(j / lanes), m = int(j - size_t(o) * lanes);
+            const int ky = m / (groups_per_row * 64), col = m - ky * groups_per_row * 64;
+            const int kx = col / cp, cc = col - kx * cp;
+            if (kx < s && cc < c) {
+                if (raw.form != KatsuF16Raw::NONE && !katsu_is_number(total) && katsu_f16_mixed(raw, ky, kx)) total = katsu_f16_exact(raw, o, cc, ky, kx);
+                float *dst = dw + ((size_t(o) * c + cc) * r + ky) * s + kx;
+                *dst = accumulate ? *dst + total : total;
+            }
+        }
+    }
 }
 
 }  // namespace
@@ -506,9 +511,9 @@ int32_t katsu_f16_conv_bwd(katsu_cuda_ctx *ctx, const float *x, const float *w, 
             p.b_pairs = b_pairs;
             KATSU_TRY(katsu_f16_launch(ctx, KATSU_F16_CONV_DW, mw, p, plan_dw, partial_dw, (long long)dw_count));
             KATSU_TRY(katsu_prepare_kernel(ctx, (const void *)f16_dw_fold_kernel, 0));
-            const size_t blocks = katsu_div_up(dw_count, (size_t)32);
-            const bool waves = blocks > size_t(ctx->num_sms) * kFoldBlocks;
-            KATSU_TRY(katsu_launch(ctx, !waves, f16_dw_fold_kernel, (unsigned)blocks, 256, 0, 1,
+            const size_t want = katsu_div_up(dw_count, (size_t)32), resident = size_t(ctx->num_sms) * kFoldBlocks;
+            const bool waves = want > resident * KATSU_ROUNDS;
+            KATSU_TRY(katsu_launch(ctx, !waves, f16_dw_fold_kernel, (unsigned)(waves || want < resident ? want : resident), 256, 0, 1,
                                    raw_of(KatsuF16Raw::DW, x, gr, g, false, gscale, gfactor), partial_dw, dw, (int)k, (int)c, (int)r, (int)s, (int)cp, (int)gpr, plan_dw.splits,
                                    accumulate, waves ? 1 : 0));
         }

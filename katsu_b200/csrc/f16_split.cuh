@@ -147,6 +147,9 @@ struct KatsuStageJob {
 int32_t katsu_f16_amax(katsu_cuda_ctx *ctx, const KatsuAmaxJob *jobs, int count);
 // Writes up to KATSU_STAGE_JOBS operands' planes, one launch.
 constexpr int KATSU_STAGE_JOBS = 4;
+// Work for up to this many times the resident blocks goes to these, in launches that may start early (1021 x 2047 by 2047 x 515 with both
+// gradients: 88 us, in waves 92); more goes in waves (a 128 x 256 x 56 layer with both gradients: 3.88 ms, on resident blocks 4.02).
+constexpr size_t KATSU_ROUNDS = 4;
 int32_t katsu_f16_stage(katsu_cuda_ctx *ctx, const KatsuF16Call &call, const KatsuStageJob *jobs, int count);
 
 // Planes of the narrow form in the context's mode, and of room for either form.

@@ -28,7 +28,7 @@ struct AmaxSegment {
 struct AmaxParams {
     AmaxSegment seg[3];
     int segments;
-    int waves;  // more blocks than are resident at once
+    int waves;
 };
 
 __device__ __forceinline__ unsigned magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
@@ -136,7 +136,7 @@ struct StageParams {
     KatsuStageJob job[KATSU_STAGE_JOBS];
     unsigned first_block[KATSU_STAGE_JOBS], blocks[KATSU_STAGE_JOBS];
     int jobs;
-    int waves;  // more blocks than are resident at once
+    int waves;
 };
 
 // How the values of one job are written.
@@ -449,10 +449,29 @@ KatsuF16Call katsu_f16_call(const katsu_cuda_ctx *ctx, const KatsuF16Info *a, co
     return KatsuF16Call{{a, b, c}, ctx->precision == KATSU_MODE_3XTF32 ? 17 : 28, nullptr, 1.f};
 }
 
+// Blocks of the parts of a launch, whose loops go over what their blocks leave.  Work for up to KATSU_ROUNDS times the resident blocks is
+// shared out to these, so that the launch may start early (launch.cuh); with more, every part has its own `most` blocks, the
+// launch goes in waves, and the hardware hands out the next part's blocks as those of the one before end.
+static unsigned share_blocks(const size_t *want, const size_t *most, int parts, size_t resident, unsigned *first, unsigned *blocks, int *waves) {
+    size_t sum = 0;
+    unsigned at = 0;
+    for (int i = 0; i < parts; ++i) sum += want[i];
+    const bool shared = sum > resident && sum <= resident * KATSU_ROUNDS;
+    for (int i = 0; i < parts; ++i) {
+        size_t own = want[i] < most[i] ? want[i] : most[i];
+        if (shared && own > 0) own = want[i] * (resident - parts) / sum + 1;
+        first[i] = at;
+        blocks[i] = (unsigned)own;
+        at += blocks[i];
+    }
+    *waves = at > resident;
+    return at;
+}
+
 int32_t katsu_f16_amax(katsu_cuda_ctx *ctx, const KatsuAmaxJob *jobs, int count) {
     AmaxParams p;
     p.segments = count;
-    unsigned at = 0;
+    size_t want[3], most[3];
     for (int i = 0; i < count; ++i) {
         AmaxSegment &s = p.seg[i];
         s.job = jobs[i];
@@ -462,14 +481,17 @@ int32_t katsu_f16_amax(katsu_cuda_ctx *ctx, const KatsuAmaxJob *jobs, int count)
         s.longer = jobs[i].rows % s.strips;
         s.col_tiles = (jobs[i].cols + (s.vec ? 127 : 31)) / (s.vec ? 128 : 32);
         size_t blocks = katsu_div_up(size_t(jobs[i].images) * s.strips * s.col_tiles, (size_t)(THREADS / 32));
-        if (blocks > size_t(ctx->num_sms) * AMAX_BLOCKS) blocks = size_t(ctx->num_sms) * AMAX_BLOCKS;
-        s.first_block = at;
-        s.blocks = (unsigned)blocks;
-        at += s.blocks;
+        want[i] = blocks;
+        most[i] = size_t(ctx->num_sms) * AMAX_BLOCKS;
+    }
+    unsigned first[3], blocks[3];
+    const unsigned at = share_blocks(want, most, count, size_t(ctx->num_sms) * AMAX_BLOCKS, first, blocks, &p.waves);
+    for (int i = 0; i < count; ++i) {
+        p.seg[i].first_block = first[i];
+        p.seg[i].blocks = blocks[i];
     }
     if (ctx->f16_captured) KATSU_LAUNCH(ctx, clear_kernel, 1, 32, 0, katsu_f16_slot(ctx, 0));
     KATSU_TRY(katsu_prepare_kernel(ctx, (const void *)amax_kernel, 0));
-    p.waves = at > unsigned(ctx->num_sms) * AMAX_BLOCKS;
     return katsu_launch(ctx, !p.waves, amax_kernel, at, THREADS, 0, 1, p);
 }
 
@@ -479,7 +501,7 @@ int32_t katsu_f16_stage(katsu_cuda_ctx *ctx, const KatsuF16Call &call, const Kat
     p.narrow_planes = katsu_f16_narrow_planes(ctx);
     p.clear = ctx->f16_captured ? nullptr : slots(ctx, ctx->f16_set ^ 1);
     p.jobs = count;
-    size_t at = 0;
+    size_t want[KATSU_STAGE_JOBS], most[KATSU_STAGE_JOBS];
     for (int i = 0; i < count; ++i) {
         const KatsuStageJob &j = jobs[i];
         p.job[i] = j;
@@ -489,22 +511,19 @@ int32_t katsu_f16_stage(katsu_cuda_ctx *ctx, const KatsuF16Call &call, const Kat
             const size_t ct = tile_channels(j.c);
             blocks = size_t(j.n) * katsu_div_up(hw, 4096 / ct) * katsu_div_up((size_t)j.c, ct);
             if (blocks > 0x3fffffff) return katsu_set_error(KATSU_ERR_UNSUPPORTED, "operand too large to stage");
-            if (blocks > size_t(ctx->num_sms) * STAGE_BLOCKS) blocks = size_t(ctx->num_sms) * STAGE_BLOCKS;
         } else {
             const size_t units = j.kind == KATSU_STAGE_NHWC ? size_t(j.n) * hw * (j.cp / 8)
                                  : j.kind == KATSU_STAGE_ROWS ? size_t(j.n) * (j.cp / 8)
                                                               : size_t(weight_planes(j)) * weight_rows(j) * (j.width / 8);
             blocks = katsu_div_up(units, (size_t)THREADS);
-            if (blocks > size_t(ctx->num_sms) * 64) blocks = size_t(ctx->num_sms) * 64;
         }
         // (as many blocks would do nothing but start and end when the copy is not needed: 30 us for 25 000)
         if (j.only_if_mixed && blocks > (size_t)ctx->num_sms) blocks = (size_t)ctx->num_sms;
-        p.first_block[i] = (unsigned)at;
-        p.blocks[i] = (unsigned)blocks;
-        at += blocks;
+        want[i] = blocks;
+        // (a tile's block loads the next one under its stores)
+        most[i] = size_t(ctx->num_sms) * (j.kind == KATSU_STAGE_NHWC && j.c > 16 ? STAGE_BLOCKS : 64);
     }
-    if (at > 0x7fffffffu) return katsu_set_error(KATSU_ERR_UNSUPPORTED, "operand too large to stage");
+    const unsigned at = share_blocks(want, most, count, size_t(ctx->num_sms) * STAGE_BLOCKS, p.first_block, p.blocks, &p.waves);
     KATSU_TRY(katsu_prepare_kernel(ctx, (const void *)stage_kernel, 0));
-    p.waves = at > size_t(ctx->num_sms) * STAGE_BLOCKS;
-    return katsu_launch(ctx, !p.waves, stage_kernel, (unsigned)at, THREADS, 0, 1, p);
+    return katsu_launch(ctx, !p.waves, stage_kernel, at, THREADS, 0, 1, p);
 }

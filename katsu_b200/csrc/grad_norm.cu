@@ -159,7 +159,7 @@ __global__ void __launch_bounds__(kThreads) norm_kernel(const double *partial, i
 // g and the product are rounded as katsu_cuda_clip_grads followed by katsu_cuda_sgd_step round them.
 template <Apply OP>
 __device__ __forceinline__ float applied(float g, float w, float c, float lr) {
-    const float clipped = __fmul_rn(g, c);
+    const float clipped = OP == CLIP && c == 1.f ? g : __fmul_rn(g, c);  // (a product with 1 is not all of a NaN's bits)
     return OP == CLIP ? clipped : w - __fmul_rn(lr, clipped);
 }
 

@@ -246,3 +246,18 @@ def test_a_norm_between_two_floats_is_refused(anywhere, norm):  # noqa: F811
                  lambda: lib.katsu_cuda_sgd_step_clipped(anywhere, w, g, c, 1, 0.1, 1.0, norm)):
         assert call() == cabi.ERR_INVALID_ARG
         assert "whole float" in lib.katsu_cuda_last_error_string().decode()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("sizes", [[1001], [5000, 9001, 3]], ids=str)
+@pytest.mark.parametrize("shift", [0, 1])
+def test_values_that_stay_keep_their_bits(ctx, sizes, shift):
+    """Below the limit and beside a gradient that is no number: signs of zeros, NaNs' bits and the smallest numbers arrive as they are."""
+    bits = np.random.default_rng(11).integers(0, 2 ** 32, sum(sizes), dtype=np.uint32)
+    small = np.where(np.arange(bits.size) % 3 == 0, bits & np.uint32(0x80000000), bits & np.uint32(0x807fffff))
+    for v in (bits, small):  # any values, NaNs among them; zeros and subnormal numbers
+        with DeviceArrays(ctx, g=v.view(np.float32), n=np.zeros(1)) as d:
+            d.alloc("out", bits.size + 4, fill=0.0)
+            ctx.clip_grads(places(d["g"], sizes), places(d["out"] + 4 * shift, sizes), sizes, 1.0, d["n"])
+            assert np.array_equal(d.get("out")[shift:shift + bits.size].view(np.uint32), v)
+            assert np.isnan(d.get("n")[0]) == (v is bits)

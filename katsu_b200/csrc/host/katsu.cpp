@@ -7,6 +7,7 @@
 #include <cmath>
 #include <unordered_map>
 #include <unordered_set>
+#include <utility>
 
 #include "katsu_cuda.h"
 
@@ -193,6 +194,7 @@ struct TensorNode {
     mutable int staged_mode = -1;
     // values are parents[0] * parents[0], not computed yet (set by Tensor::mul when fusion is on)
     mutable bool lazy_square = false;
+    mutable std::vector<std::weak_ptr<TensorNode>> squares;  // DeviceBuffer::squares until there is a buffer
     mutable std::shared_ptr<DeviceBuffer> grad_dev;  // null == None (unless grad_sym holds it)
     mutable std::shared_ptr<Adjoint> grad_sym;       // a gradient still in symbolic form
     mutable std::vector<float> grad_host;
@@ -210,8 +212,18 @@ struct TensorNode {
                 // (from pageable memory: the call returns once the values have been staged)
                 check(katsu_cuda_h2d(device_context(), buffer->ptr, host.data(), numel));
             }
+            buffer->squares = std::move(squares);
+            squares.clear();
             dev = std::move(buffer);
         }
+        return dev->ptr;
+    }
+
+    // The values' address for a step in place: what still refers to the values as they are is computed first.
+    float *stepped() const {
+        device();
+        for (const std::weak_ptr<TensorNode> &square : std::exchange(dev->squares, {}))
+            if (const auto node = square.lock()) node->device();
         return dev->ptr;
     }
 
@@ -372,6 +384,9 @@ Tensor Tensor::make_lazy_square(const Tensor &parent) {
     node->op.kind = Op::Mul;
     node->parents = {parent, parent};
     node->lazy_square = true;
+    auto &squares = parent.node_->dev ? parent.node_->dev->squares : parent.node_->squares;
+    squares.erase(std::remove_if(squares.begin(), squares.end(), [](const auto &square) { return square.expired(); }), squares.end());
+    squares.push_back(node);
     return Tensor(std::move(node));
 }
 
@@ -379,7 +394,7 @@ void Tensor::sgd_step(float lr) const {
     if (node_->borrows != 0) fail(ErrorKind::GradientBorrowed);
     if (!node_->has_grad()) fail(ErrorKind::Device, "sgd_step needs a gradient: run backward first");
     const float *gradient = node_->dense_grad()->ptr;
-    float *values = const_cast<float *>(node_->device());
+    float *values = node_->stepped();
     if (numel()) check(katsu_cuda_sgd_step(device_context(), values, gradient, lr, numel()));
     node_->host_valid = false;  // the host mirror is refilled from the device on the next data()
     node_->staged.reset();      // as is the copy for convolutions, by the next one
@@ -1173,7 +1188,7 @@ Tensor sgd_step_clipped(const std::vector<Tensor> &tensors, float lr, float max_
     std::vector<size_t> counts;
     for (const Tensor &t : tensors) {
         grads.push_back(t.node()->dense_grad()->ptr);
-        weights.push_back(const_cast<float *>(t.node()->device()));
+        weights.push_back(t.node()->stepped());
         counts.push_back(t.numel());
     }
     auto norm = uninit_buffer(1);

@@ -104,6 +104,8 @@ struct DeviceBuffer {
     ~DeviceBuffer();
     DeviceBuffer(const DeviceBuffer &) = delete;
     DeviceBuffer &operator=(const DeviceBuffer &) = delete;
+    // Squares of these values that may not be computed yet (Tensor::mul): a step in place computes them first.
+    std::vector<std::weak_ptr<TensorNode>> squares;
 };
 
 // Guard returned by Tensor::grad(): while alive, backward and zero_grad on the

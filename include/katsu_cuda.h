@@ -73,7 +73,8 @@ int32_t katsu_cuda_get_precision(katsu_cuda_ctx *ctx, int32_t *out_mode);
 const char *katsu_cuda_last_error_string(void);
 /* Number of kernels this context has launched so far (for benchmark reports). */
 int32_t katsu_cuda_launch_count(katsu_cuda_ctx *ctx, uint64_t *out_count);
-/* Raw cudaStream_t of the context, for callers that interleave their own work. */
+/* Raw cudaStream_t of the context, for callers that interleave their own work.  Calls captured from it refer to the
+ * context's workspace, as its other calls do: replays wait for these and for each other (the same stream, or events). */
 int32_t katsu_cuda_stream(katsu_cuda_ctx *ctx, void **out_stream);
 
 /* ---- memory ------------------------------------------------------------ */
@@ -211,7 +212,7 @@ int32_t katsu_cuda_matmul_bwd(katsu_cuda_ctx *ctx, const float *a, const float *
  * channel), rows (each row its own), or one row of the gate for every rows / gate_rows rows (sequences of one
  * length).  cols is 1 to 2^30 - 1; without rows nothing is written.  Outputs alias neither inputs nor each other.
  * A row's infinities and NaNs stay in its row.  Sums are f32: squares above the f32 range (values above 1.8e19)
- * overflow to a norm of 0; a row without spread needs eps > 0. */
+ * overflow to a norm of 0; a row without spread, or of values below 1e-19 only, needs eps > 0. */
 #define KATSU_NORM_RMS 0
 #define KATSU_NORM_LAYER 1
 int32_t katsu_cuda_block_norm_fwd(katsu_cuda_ctx *ctx, const float *x, const float *h, const float *gate,
@@ -222,7 +223,7 @@ int32_t katsu_cuda_block_norm_fwd(katsu_cuda_ctx *ctx, const float *x, const flo
  * zeros; dn is null exactly where pre_w is).  The statistics of the rows are taken again from r and h.
  *     dx = dr + [gradient through N(r; pre)]        dh = [gradient through the gate and N(h; post)] of dx
  *     dgate [gate_rows, cols], dpost_w, dpost_b, dpre_w, dpre_b [cols]: sums over rows, in an order that the
- *     shape and the buffers' alignment fix
+ *     shape and the buffers' alignment fix; zeros where there are no rows
  * Any output may be null.  `accumulate` is a sum of KATSU_BLOCK_*: those outputs are added to their contents. */
 #define KATSU_BLOCK_DX 1
 #define KATSU_BLOCK_DH 2

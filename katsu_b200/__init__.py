@@ -641,7 +641,7 @@ def clip_grad_norm(tensors, max_norm):
 
 
 def sgd_step_clipped(tensors, lr, max_norm):
-    """clip_grad_norm and sgd_step of all `tensors` in two launches; the gradients stay as they are.  Returns the norm.
+    """clip_grad_norm and sgd_step of all `tensors` in one call; the gradients stay as they are.  Returns the norm.
     Where a gradient holds an infinity or a NaN no tensor changes."""
     lib, out, tensors = _load(), _vp(), list(tensors)
     _check(lib.kh_sgd_step_clipped(*_handles(tensors), float(lr), float(max_norm), ctypes.byref(out)))

@@ -35,6 +35,8 @@ pub const KATSU_BLOCK_DPOST_B: i32 = 16;
 pub const KATSU_BLOCK_DPRE_W: i32 = 32;
 pub const KATSU_BLOCK_DPRE_B: i32 = 64;
 pub const KATSU_INT8_MAX_K: i32 = 133144;
+pub const KATSU_DISTILL_MAX_TOP: i32 = 1024;
+pub const KATSU_LOGITS_MAX_BIASES: i32 = 1024;
 pub const KATSU_COMM_ID_BYTES: usize = 128;
 pub const KATSU_SUM_STATIC_MAX_COUNT: usize = 1 << 30;
 
@@ -81,6 +83,12 @@ extern "C" {
     pub fn katsu_cuda_grad_norm(ctx: *mut Ctx, grads: *const *const f32, counts: *const usize, tensors: usize, norm: *mut f32) -> i32;
     pub fn katsu_cuda_clip_grads(ctx: *mut Ctx, grads: *const *const f32, out: *const *mut f32, counts: *const usize, tensors: usize, max_norm: f32, norm: *mut f32) -> i32;
     pub fn katsu_cuda_sgd_step_clipped(ctx: *mut Ctx, weights: *const *mut f32, grads: *const *const f32, counts: *const usize, tensors: usize, lr: f32, max_norm: f32, norm: *mut f32) -> i32;
+    pub fn katsu_cuda_embed_fwd(ctx: *mut Ctx, table: *const f32, tokens: *const i32, scale: f32, y: *mut f32, count: usize, vocab: usize, cols: usize) -> i32;
+    pub fn katsu_cuda_int8_embed(ctx: *mut Ctx, q: *const i8, rows_scale: *const f32, tokens: *const i32, scale: f32, y: *mut f32, count: usize, vocab: usize, cols: usize) -> i32;
+    pub fn katsu_cuda_embed_bwd(ctx: *mut Ctx, tokens: *const i32, dy: *const f32, scale: f32, dtable: *mut f32, count: usize, vocab: usize, cols: usize, accumulate: i32) -> i32;
+    pub fn katsu_cuda_distill_fwd(ctx: *mut Ctx, logits: *const f32, teacher: *const f32, index: *const i32, labels: *const i32, weight: *const f32, temperature: f32, soft: f32, hard: f32, loss: *mut f32, rows: usize, vocab: usize, top: usize) -> i32;
+    pub fn katsu_cuda_distill_bwd(ctx: *mut Ctx, logits: *const f32, teacher: *const f32, index: *const i32, labels: *const i32, weight: *const f32, temperature: f32, soft: f32, hard: f32, g: *const f32, loss: *mut f32, dlogits: *mut f32, rows: usize, vocab: usize, top: usize, accumulate: i32) -> i32;
+    pub fn katsu_cuda_adjust_logits(ctx: *mut Ctx, logits: *const f32, history: *const i32, prompts: *const i32, lengths: *const i32, repetition: *const f32, presence: *const f32, frequency: *const f32, bias_tokens: *const i32, bias: *const f32, allowed: *const u32, out: *mut f32, rows: usize, vocab: usize, history_cols: usize, biases: usize) -> i32;
     pub fn katsu_cuda_add(ctx: *mut Ctx, a: *const f32, b: *const f32, out: *mut f32, count: usize) -> i32;
     pub fn katsu_cuda_mul(ctx: *mut Ctx, a: *const f32, b: *const f32, out: *mut f32, count: usize) -> i32;
     pub fn katsu_cuda_sum(ctx: *mut Ctx, a: *const f32, out: *mut f32, count: usize) -> i32;

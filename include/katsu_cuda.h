@@ -12,7 +12,7 @@
  *    aborts or prints.  katsu_cuda_last_error_string() describes the most
  *    recent failure on the calling thread.
  *  - all tensors are contiguous row-major f32 (the 8-bit matrices of the integer
- *    product apart); device pointers come from katsu_cuda_alloc (or any
+ *    product and lists of tokens apart); device pointers come from katsu_cuda_alloc (or any
  *    cudaMalloc'ed memory on the context's device).
  *  - sizes are size_t like the reference's usize; the caller has already run
  *    the reference's shape validation (Geometry::new, matmul rank checks);
@@ -283,6 +283,65 @@ int32_t katsu_cuda_clip_grads(katsu_cuda_ctx *ctx, const float *const *grads, fl
  * or NaN no weight changes.  Weights overlap neither gradients nor each other. */
 int32_t katsu_cuda_sgd_step_clipped(katsu_cuda_ctx *ctx, float *const *weights, const float *const *grads,
                                     const size_t *counts, size_t tensors, float lr, float max_norm, float *norm);
+
+/* ---- the two ends of a language model -----------------------------------------
+ * No counterpart in the reference.  Tokens are int32_t in device memory (katsu_cuda_alloc's 4-byte elements), 0 to
+ * vocab - 1; what stands for no token (padding, a list's unused places) is any other number.  vocab and the numbers of
+ * tokens and rows are below 2^31.  Outputs overlap neither inputs nor each other unless a function says so.
+ *
+ * Lookup: y[i] = scale * table[tokens[i]] for `count` tokens and a table [vocab, cols]; a row of zeros where tokens[i]
+ * is no token. */
+int32_t katsu_cuda_embed_fwd(katsu_cuda_ctx *ctx, const float *table, const int32_t *tokens, float scale, float *y,
+                             size_t count, size_t vocab, size_t cols);
+/* The same from a table in 8 bits, y[i][j] = (q[tokens[i]][j] * rows_scale[tokens[i]]) * scale: q [vocab][row bytes of
+ * cols] and rows_scale [vocab] as katsu_cuda_int8_quantize_weights leaves them for w [cols, vocab] (a head whose weights
+ * are the table too), or katsu_cuda_int8_quantize_rows for a table [vocab, cols]. */
+int32_t katsu_cuda_int8_embed(katsu_cuda_ctx *ctx, const int8_t *q, const float *rows_scale, const int32_t *tokens,
+                              float scale, float *y, size_t count, size_t vocab, size_t cols);
+/* Gradient of the lookup's table: dtable[v] = scale * (sum of dy[i] over all i with tokens[i] == v), in an order that
+ * `tokens` alone fixes: the same bits every time.  Rows of other tokens are zeros.  accumulate != 0: added to dtable
+ * instead, whose other rows are not touched. */
+int32_t katsu_cuda_embed_bwd(katsu_cuda_ctx *ctx, const int32_t *tokens, const float *dy, float scale, float *dtable,
+                             size_t count, size_t vocab, size_t cols, int32_t accumulate);
+
+/* Loss of logits z [rows, vocab] against a teacher's top logits and against labels, for every row:
+ *     p = softmax(teacher / T) over the row's `top` entries, q = softmax(z / T) over the vocabulary (T = temperature)
+ *     loss = weight * (soft T^2 sum_j p_j (log p_j - log q[index_j]) - hard log softmax(z)[label])
+ * teacher and index are [rows, top], top at most KATSU_DISTILL_MAX_TOP.  Entries whose index is no token are left out,
+ * and a token that is listed twice has both probabilities.  Without an entry that counts (none listed, all teacher
+ * logits -infinity) a row's soft part is 0, without a label its hard part.  labels may be null (none), weight null (1).
+ * A row of weight 0 is not read: its loss is 0 and its gradient zeros, as they are without either part.  Other rows keep
+ * infinities and NaNs to themselves: a logit of -infinity is a token of probability 0 (the loss is infinite where the teacher or the label asks
+ * for it), other infinities and NaNs make the row NaN, and so do -infinities only. */
+#define KATSU_DISTILL_MAX_TOP 1024
+int32_t katsu_cuda_distill_fwd(katsu_cuda_ctx *ctx, const float *logits, const float *teacher, const int32_t *index,
+                               const int32_t *labels, const float *weight, float temperature, float soft, float hard,
+                               float *loss, size_t rows, size_t vocab, size_t top);
+/* dlogits = g[row] * weight * (soft T (q - p) + hard (softmax(z) - [v == label])): the gradient of sum_row g * loss.
+ * g [rows] may be null (1).  loss [rows] may be null; otherwise it receives the loss as well, so that a training step
+ * reads the logits once for both.  dlogits may be `logits` itself; accumulate != 0 adds to dlogits (then not `logits`). */
+int32_t katsu_cuda_distill_bwd(katsu_cuda_ctx *ctx, const float *logits, const float *teacher, const int32_t *index,
+                               const int32_t *labels, const float *weight, float temperature, float soft, float hard,
+                               const float *g, float *loss, float *dlogits, size_t rows, size_t vocab, size_t top,
+                               int32_t accumulate);
+
+/* Logits [rows, vocab] of a served model before a token is picked from them; for every row and token, in this order:
+ *     repetition   v > 0 ? v / repetition : v * repetition for tokens of the row's history
+ *     counts       v - (frequency * count + presence) for tokens that are `count` > 0 times in its generated part
+ *     biases       v + the values that the row's list has for the token
+ *     allowed      -infinity where the token's bit is 0, whatever v is
+ * history [rows, history_cols]: the first lengths[row] entries are the row's tokens (null: all), of which the first
+ * prompts[row] are its prompt (null: none) and the rest generated; lengths are cut off at 0 and history_cols, prompts at
+ * 0 and the length.  repetition, presence, frequency [rows] may be null (1, 0, 0); history is null with history_cols 0.
+ * bias_tokens and bias [rows, biases], at most KATSU_LOGITS_MAX_BIASES (null with biases 0): values of one token are
+ * added up first.  allowed: bit v % 32 of word v / 32 of [rows][(vocab + 31) / 32], null: every token.
+ * out may be `logits` itself. */
+#define KATSU_LOGITS_MAX_BIASES 1024
+int32_t katsu_cuda_adjust_logits(katsu_cuda_ctx *ctx, const float *logits, const int32_t *history, const int32_t *prompts,
+                                 const int32_t *lengths, const float *repetition, const float *presence,
+                                 const float *frequency, const int32_t *bias_tokens, const float *bias,
+                                 const uint32_t *allowed, float *out, size_t rows, size_t vocab, size_t history_cols,
+                                 size_t biases);
 
 /* ---- streaming ops that keep the autograd graph on the device ---------- */
 /* out = a + b / out = a * b; Tensor::elementwise, tensor.rs:226-233. */

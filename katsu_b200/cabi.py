@@ -24,6 +24,7 @@ COMM_ID_BYTES = 128
 NORM_RMS, NORM_LAYER = 0, 1
 BLOCK_DX, BLOCK_DH, BLOCK_DGATE, BLOCK_DPOST_W, BLOCK_DPOST_B, BLOCK_DPRE_W, BLOCK_DPRE_B = (1 << i for i in range(7))
 INT8_MAX_K = 133144
+DISTILL_MAX_TOP, LOGITS_MAX_BIASES = 1024, 1024
 
 _c_float_p = ctypes.POINTER(ctypes.c_float)
 _sz = ctypes.c_size_t
@@ -77,6 +78,12 @@ SIGNATURES = {
     "katsu_cuda_grad_norm": [_ctx, ctypes.POINTER(_ptr), ctypes.POINTER(_sz), _sz, _ptr],
     "katsu_cuda_clip_grads": [_ctx, ctypes.POINTER(_ptr), ctypes.POINTER(_ptr), ctypes.POINTER(_sz), _sz, _f32, _ptr],
     "katsu_cuda_sgd_step_clipped": [_ctx, ctypes.POINTER(_ptr), ctypes.POINTER(_ptr), ctypes.POINTER(_sz), _sz, _f32, _f32, _ptr],
+    "katsu_cuda_embed_fwd": [_ctx, _ptr, _ptr, _f32, _ptr, _sz, _sz, _sz],
+    "katsu_cuda_int8_embed": [_ctx, _ptr, _ptr, _ptr, _f32, _ptr, _sz, _sz, _sz],
+    "katsu_cuda_embed_bwd": [_ctx, _ptr, _ptr, _f32, _ptr, _sz, _sz, _sz, _i32],
+    "katsu_cuda_distill_fwd": [_ctx] + [_ptr] * 5 + [_f32] * 3 + [_ptr] + [_sz] * 3,
+    "katsu_cuda_distill_bwd": [_ctx] + [_ptr] * 5 + [_f32] * 3 + [_ptr] * 3 + [_sz] * 3 + [_i32],
+    "katsu_cuda_adjust_logits": [_ctx] + [_ptr] * 11 + [_sz] * 4,
     "katsu_cuda_add": [_ctx, _ptr, _ptr, _ptr, _sz],
     "katsu_cuda_mul": [_ctx, _ptr, _ptr, _ptr, _sz],
     "katsu_cuda_sum": [_ctx, _ptr, _ptr, _sz],
@@ -328,3 +335,27 @@ class Context:
             raise ValueError(f"{len(grads)} gradients, but {len(weights)} weights")
         self.call("katsu_cuda_sgd_step_clipped", self._addresses(weights), self._addresses(grads),
                   self._counts(counts, len(grads)), len(grads), lr, max_norm, norm)
+
+    # -- the two ends of a language model: tokens are device addresses of int32 values ----------
+    def embed_fwd(self, table, tokens, scale, y, count, vocab, cols) -> None:
+        check(self.lib.katsu_cuda_embed_fwd(self.handle, table, tokens, scale, y, count, vocab, cols))
+
+    def int8_embed(self, q, rows_scale, tokens, scale, y, count, vocab, cols) -> None:
+        check(self.lib.katsu_cuda_int8_embed(self.handle, q, rows_scale, tokens, scale, y, count, vocab, cols))
+
+    def embed_bwd(self, tokens, dy, scale, dtable, count, vocab, cols, accumulate=0) -> None:
+        check(self.lib.katsu_cuda_embed_bwd(self.handle, tokens, dy, scale, dtable, count, vocab, cols, accumulate))
+
+    def distill_fwd(self, logits, teacher, index, labels, weight, temperature, soft, hard, loss, rows, vocab, top) -> None:
+        check(self.lib.katsu_cuda_distill_fwd(self.handle, logits, teacher, index, labels, weight, temperature, soft, hard, loss,
+                                              rows, vocab, top))
+
+    def distill_bwd(self, logits, teacher, index, labels, weight, temperature, soft, hard, g, loss, dlogits, rows, vocab, top,
+                    accumulate=0) -> None:
+        check(self.lib.katsu_cuda_distill_bwd(self.handle, logits, teacher, index, labels, weight, temperature, soft, hard, g, loss,
+                                              dlogits, rows, vocab, top, accumulate))
+
+    def adjust_logits(self, logits, history, prompts, lengths, repetition, presence, frequency, bias_tokens, bias, allowed, out,
+                      rows, vocab, history_cols, biases) -> None:
+        check(self.lib.katsu_cuda_adjust_logits(self.handle, logits, history, prompts, lengths, repetition, presence, frequency,
+                                                bias_tokens, bias, allowed, out, rows, vocab, history_cols, biases))

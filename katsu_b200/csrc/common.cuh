@@ -130,6 +130,9 @@ static inline bool katsu_overlap(const void *a, size_t a_bytes, const void *b, s
     return a != nullptr && b != nullptr && x < y + b_bytes && y < x + a_bytes;
 }
 
+// Whether an address (null: none) is that of a whole 4-byte element.
+static inline bool katsu_whole(const void *p) { return reinterpret_cast<uintptr_t>(p) % 4 == 0; }
+
 // Internal entry points shared between translation units.
 int32_t katsu_conv_direct_fwd(katsu_cuda_ctx *ctx, const float *x, const float *w, float *y,
                               size_t n, size_t c, size_t h, size_t wd, size_t k, size_t r, size_t s,

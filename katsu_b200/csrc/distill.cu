@@ -1,0 +1,374 @@
+// Loss of logits against a teacher's top logits and against labels, and its gradient.
+//
+//   p = softmax(t / T) over the listed entries      q = softmax(z / T), s = softmax(z) over the vocabulary
+//   loss = w (soft T^2 sum_j p_j (log p_j - log q_idx(j)) - hard log s_label)
+//   dz   = g w (soft T (q - p) + hard (s - [v = label]))
+//
+// Bound: HBM, z once and dz once.  A row is held in the registers of a block (32 values a thread), or of a cluster of up to
+// eight blocks, from its only read to the gradient's write; blocks exchange their largest value and sums through shared memory
+// of the cluster.  Sums of exponentials are relative to a warp's largest value, joined in a tree, so that a row of 1e5 values
+// adds up 32 numbers behind each other at most.  The gradient of listed tokens (a few of a row) is written again behind
+// the row's, from sums over the list in its order: no atomics.
+#include <float.h>
+#include <math.h>
+
+#include <algorithm>
+
+#include "common.cuh"
+#include "launch.cuh"
+#include "sm100_pair.cuh"
+
+namespace {
+
+constexpr int kHeld = 8;  // 16-byte accesses a thread holds
+constexpr int kMostCluster = 8;
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct Distill {
+    const float *logits, *teacher, *weight, *g;
+    const int *index, *labels;
+    float *loss, *dlogits;
+    float temperature, soft, hard;
+    float c0, c1;  // log2(e) / T and log2(e)
+    unsigned rows, vocab, top, blocks;  // blocks of a row
+    int accumulate;
+};
+
+struct Sums {
+    float m, s0, s1;  // largest value; sums of exp((z - m) / T) and of exp(z - m)
+};
+
+// A warp or block without a value above -infinity counts from the lowest number, which leaves its sums 0.
+__device__ __forceinline__ float base_of(float m) { return fmaxf(m, -FLT_MAX); }
+__device__ __forceinline__ float ex(float d, float c) { return exp2f(d * c); }
+
+template <bool TWO>
+__device__ __forceinline__ Sums join(const Distill &a, Sums x, Sums y) {
+    Sums r;
+    r.m = fmaxf(x.m, y.m);
+    const float b = base_of(r.m), dx = base_of(x.m) - b, dy = base_of(y.m) - b;
+    r.s0 = x.s0 * ex(dx, a.c0) + y.s0 * ex(dy, a.c0);
+    r.s1 = TWO ? x.s1 * ex(dx, a.c1) + y.s1 * ex(dy, a.c1) : 0.f;
+    return r;
+}
+
+template <bool TWO>
+__device__ __forceinline__ Sums join_lanes(const Distill &a, Sums x, int lanes) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        if (o >= lanes) continue;
+        Sums y;
+        y.m = __shfl_xor_sync(0xffffffffu, x.m, o);
+        y.s0 = __shfl_xor_sync(0xffffffffu, x.s0, o);
+        y.s1 = TWO ? __shfl_xor_sync(0xffffffffu, x.s1, o) : 0.f;
+        x = join<TWO>(a, x, y);
+    }
+    return x;
+}
+
+__device__ __forceinline__ float largest_of_warp(float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+
+__device__ __forceinline__ float sum_of_warp(float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+__device__ __forceinline__ double sum_of_warp(double v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+// The row's entries and, as the last one, its label: in shared memory, written by the first warp.
+struct Entries {
+    int *token;  // -1 where it is none
+    float *e;    // exp((t - largest t) / T), 0 for the label
+    float *z;    // the token's logit
+    float *t;    // t - largest t
+};
+
+// Four values from place 4 u - lead of a row of `vocab`; what is outside of it is -infinity.
+__device__ __forceinline__ float4 load_row(const float *row, unsigned u, unsigned lead, unsigned vocab) {
+    const long long first = 4ll * u - lead;
+    if (first >= 0 && first + 4 <= vocab) return *reinterpret_cast<const float4 *>(row + first);
+    float v[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) v[c] = first + c >= 0 && first + c < vocab ? row[first + c] : -INFINITY;
+    return make_float4(v[0], v[1], v[2], v[3]);
+}
+
+// GRAD: writes the gradient (and the loss where it is asked for).  TWO: sums at the temperature and at 1; otherwise one set of
+// sums is both.  ONCE: the row fits the registers; otherwise it is read again for the gradient.
+template <int THREADS, bool GRAD, bool TWO, bool ONCE>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) distill_kernel(Distill a) {
+    extern __shared__ float dynamic[];
+    __shared__ Sums of_warp[THREADS / 32];
+    __shared__ Sums of_block[kMostCluster];
+    __shared__ float teacher_sum;
+    const unsigned lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const unsigned row = blockIdx.x / a.blocks, rank = blockIdx.x % a.blocks;
+    const float weight = a.weight ? a.weight[row] : 1.f;
+    const float *z = a.logits + size_t(row) * a.vocab;
+    float *dz = GRAD ? a.dlogits + size_t(row) * a.vocab : nullptr;
+    const unsigned lead = unsigned(reinterpret_cast<uintptr_t>(z) >> 2) & 3u, out_lead = unsigned(reinterpret_cast<uintptr_t>(dz) >> 2) & 3u;
+    const unsigned units = (a.vocab + lead + 3) / 4, share = (units + a.blocks - 1) / a.blocks;
+    const unsigned begin = min(units, rank * share), end = min(units, begin + share);
+    if (weight == 0.f) {  // (all blocks of the row)
+        if (GRAD && !a.accumulate) {
+            const unsigned v0 = max(4 * begin, lead) - lead, v1 = min(4 * end - lead, a.vocab);
+            if (begin < end)
+                for (unsigned v = v0 + threadIdx.x; v < v1; v += THREADS) dz[v] = 0.f;
+        }
+        if (a.loss && rank == 0 && threadIdx.x == 0) a.loss[row] = 0.f;
+        return;
+    }
+    if (a.blocks > 1) sm100::cluster_arrive();
+    float4 v[kHeld];
+    auto fetch = [&](unsigned from) {
+#pragma unroll
+        for (int q = 0; q < kHeld; ++q) {
+            const unsigned u = from + q * THREADS + threadIdx.x;
+            v[q] = u < end ? load_row(z, u, lead, a.vocab) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        }
+    };
+    fetch(begin);
+    // ---- the teacher's entries ----
+    const unsigned listed = a.top + 1;
+    const Entries entries = {reinterpret_cast<int *>(dynamic), dynamic + listed, dynamic + 2 * listed, dynamic + 3 * listed};
+    if (warp == 0) {
+        float most = -INFINITY;
+        for (unsigned j = lane; j < a.top; j += 32) {
+            const int token = a.index[size_t(row) * a.top + j];
+            const bool there = unsigned(token) < a.vocab;
+            const float t = there ? a.teacher[size_t(row) * a.top + j] : -INFINITY;
+            entries.token[j] = there ? token : -1;
+            entries.z[j] = there ? z[token] : 0.f;
+            entries.t[j] = t;
+            most = fmaxf(most, t);
+        }
+        most = base_of(largest_of_warp(most));
+        float sum = 0.f;
+        for (unsigned j = lane; j < a.top; j += 32) {
+            const float t = entries.t[j] - most, e = entries.token[j] >= 0 ? expf(t / a.temperature) : 0.f;
+            entries.t[j] = t;
+            entries.e[j] = e;
+            sum += e;
+        }
+        sum = sum_of_warp(sum);
+        if (lane == 0) {
+            const int label = a.labels ? a.labels[row] : -1;
+            const bool there = unsigned(label) < a.vocab;
+            entries.token[a.top] = there ? label : -1;
+            entries.z[a.top] = there ? z[label] : 0.f;
+            entries.e[a.top] = 0.f;
+            teacher_sum = sum;
+        }
+        __syncwarp();
+    }
+    // ---- largest value and sums of the row ----
+    Sums s = {-INFINITY, 0.f, 0.f};
+    for (unsigned from = begin;;) {
+        float most = -INFINITY;
+#pragma unroll
+        for (int q = 0; q < kHeld; ++q) most = fmaxf(most, fmaxf(fmaxf(v[q].x, v[q].y), fmaxf(v[q].z, v[q].w)));
+        Sums here = {largest_of_warp(most), 0.f, 0.f};
+        const float b = base_of(here.m);
+#pragma unroll
+        for (int q = 0; q < kHeld; ++q) {
+            here.s0 += ex(v[q].x - b, a.c0) + ex(v[q].y - b, a.c0) + (ex(v[q].z - b, a.c0) + ex(v[q].w - b, a.c0));
+            if (TWO) here.s1 += ex(v[q].x - b, a.c1) + ex(v[q].y - b, a.c1) + (ex(v[q].z - b, a.c1) + ex(v[q].w - b, a.c1));
+        }
+        s = ONCE ? here : join<TWO>(a, s, here);
+        if (ONCE) break;
+        from += kHeld * THREADS;
+        if (from >= end) break;
+        fetch(from);
+    }
+    s.s0 = sum_of_warp(s.s0);
+    if (TWO) s.s1 = sum_of_warp(s.s1);
+    if (lane == 0) of_warp[warp] = s;
+    __syncthreads();
+    s = join_lanes<TWO>(a, of_warp[lane % (THREADS / 32)], THREADS / 32);
+    if (a.blocks > 1) {
+        sm100::cluster_wait();  // the others run: their shared memory is there
+        if (warp == 0 && lane < a.blocks) {
+            const uint32_t at = sm100::map_to_rank(&of_block[rank], lane);
+            sm100::st_cluster(at, s.m);
+            sm100::st_cluster(at + 4, s.s0);
+            sm100::st_cluster(at + 8, s.s1);
+        }
+        __syncwarp();
+        sm100::cluster_sync_all();
+        s = of_block[0];
+        for (unsigned r = 1; r < a.blocks; ++r) s = join<TWO>(a, s, of_block[r]);
+    }
+    const float b = base_of(s.m), s1 = TWO ? s.s1 : s.s0;
+    const bool taught = a.soft != 0.f && !(teacher_sum == 0.f);
+    const bool labelled = a.hard != 0.f && entries.token[a.top] >= 0;
+    if (a.loss && rank == 0 && warp == 0) {
+        // log p_j - log q_j = (t_j - largest t - (z_j - b)) / T - log sum e + log s0: differences that nearly cancel, in 64 bits
+        double total = 0.0, apart = 0.0;
+        for (unsigned j = lane; j < a.top; j += 32) {
+            const double e = entries.e[j];
+            total += e;
+            if (e != 0.0) apart += e * (double(entries.t[j]) - (double(entries.z[j]) - double(b)));
+        }
+        total = sum_of_warp(total);
+        apart = sum_of_warp(apart);
+        if (lane == 0) {
+            double loss = 0.0;
+            const double T = a.temperature;
+            if (taught) loss += a.soft * (T * T) * (apart / total / T - log(total) + log(double(s.s0)));
+            if (labelled) loss += a.hard * (double(b) + log(double(s1)) - double(entries.z[a.top]));
+            a.loss[row] = float(weight * loss);
+        }
+    }
+    if (!GRAD) return;
+    // ---- the gradient ----
+    const float of_row = weight * (a.g ? a.g[row] : 1.f);
+    const float soft = taught ? of_row * a.soft * a.temperature : 0.f, hard = labelled ? of_row * a.hard : 0.f;
+    const float k0 = TWO ? soft / s.s0 : (soft + hard) / s.s0, k1 = TWO ? hard / s1 : 0.f;
+    const bool none = !taught && !labelled;  // such a row has a loss of 0, whatever it holds
+    auto slope = [&](float value) {
+        if (none) return 0.f;
+        const float d = value - b;
+        float r = k0 * ex(d, a.c0);
+        if (TWO) r += k1 * ex(d, a.c1);
+        return r;
+    };
+    for (unsigned from = begin;;) {
+        if (!ONCE) fetch(from);
+#pragma unroll
+        for (int q = 0; q < kHeld; ++q) {
+            const unsigned u = from + q * THREADS + threadIdx.x;
+            if (u >= end) continue;
+            const long long first = 4ll * u - lead;
+            float d[4] = {slope(v[q].x), slope(v[q].y), slope(v[q].z), slope(v[q].w)};
+            if (out_lead == lead && first >= 0 && first + 4 <= a.vocab) {
+                float4 *dst = reinterpret_cast<float4 *>(dz + first);
+                if (a.accumulate) {
+                    const float4 old = *dst;
+                    d[0] += old.x, d[1] += old.y, d[2] += old.z, d[3] += old.w;
+                }
+                *dst = make_float4(d[0], d[1], d[2], d[3]);
+            } else {
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    if (first + c >= 0 && first + c < a.vocab) dz[first + c] = a.accumulate ? dz[first + c] + d[c] : d[c];
+            }
+        }
+        from += kHeld * THREADS;
+        if (ONCE || from >= end) break;
+    }
+    __syncthreads();
+    // listed tokens of this block's part, each by its first entry
+    const unsigned v0 = max(4 * begin, lead) - lead, v1 = begin < end ? min(4 * end - lead, a.vocab) : v0;
+    for (unsigned j = threadIdx.x; j < listed; j += THREADS) {
+        const unsigned token = unsigned(entries.token[j]);
+        if (token < v0 || token >= v1) continue;
+        bool first = true;
+        float e = 0.f;
+        for (unsigned i = 0; i < listed; ++i) {
+            if (unsigned(entries.token[i]) != token) continue;
+            first = first && i >= j;
+            e += entries.e[i];
+        }
+        if (!first) continue;
+        float d = 0.f;
+        if (taught) d = soft * (e / teacher_sum);
+        if (token == unsigned(entries.token[a.top])) d += hard;
+        if (a.accumulate) dz[token] -= d;
+        else dz[token] = slope(entries.z[j]) - d;
+    }
+}
+
+template <int THREADS, bool GRAD, bool TWO, bool ONCE>
+int32_t launch(katsu_cuda_ctx *ctx, const Distill &a) {
+    const size_t smem = 4 * sizeof(float) * (size_t(a.top) + 1), blocks = size_t(a.rows) * a.blocks;
+    if (blocks > 0x7fffffffu) return katsu_set_error(KATSU_ERR_UNSUPPORTED, "%u rows of %u logits in one loss", a.rows, a.vocab);
+    return katsu_launch(ctx, false, distill_kernel<THREADS, GRAD, TWO, ONCE>, unsigned(blocks), THREADS, smem, a.blocks, a);
+}
+
+template <int THREADS, bool GRAD>
+int32_t launch_for(katsu_cuda_ctx *ctx, const Distill &a, bool two, bool once) {
+    if (two) return once ? launch<THREADS, GRAD, true, true>(ctx, a) : launch<THREADS, GRAD, true, false>(ctx, a);
+    return once ? launch<THREADS, GRAD, false, true>(ctx, a) : launch<THREADS, GRAD, false, false>(ctx, a);
+}
+
+template <bool GRAD>
+int32_t run(katsu_cuda_ctx *ctx, Distill a) {
+    if (a.soft == 0.f || a.top == 0) {  // labels alone: one set of sums, at 1
+        a.soft = 0.f;
+        a.temperature = 1.f;
+        a.top = 0;
+    }
+    a.c1 = kLog2e;
+    a.c0 = kLog2e / a.temperature;
+    const bool two = a.hard != 0.f && a.soft != 0.f && a.temperature != 1.f;
+    // blocks of as few threads as hold a row, then clusters of the largest
+    const size_t units = (size_t(a.vocab) + 3 + 3) / 4;
+    const size_t threads = units <= 128 * kHeld ? 128 : units <= 256 * kHeld ? 256 : 512;
+    a.blocks = 1;
+    while (a.blocks < kMostCluster && units > a.blocks * threads * kHeld) a.blocks *= 2;
+    const bool once = units <= a.blocks * threads * kHeld;
+    return threads == 128 ? launch_for<128, GRAD>(ctx, a, two, once)
+         : threads == 256 ? launch_for<256, GRAD>(ctx, a, two, once) : launch_for<512, GRAD>(ctx, a, two, once);
+}
+
+// The checks of both calls.  loss is null where it is not asked for, dlogits in the forward.
+int32_t check(const katsu_cuda_ctx *ctx, const Distill &a, size_t rows, size_t vocab, size_t top) {
+    KATSU_REQUIRE(ctx != nullptr, "null context");
+    KATSU_REQUIRE(rows <= 0x7fffffffu && vocab <= 0x7fffffffu, "rows and vocab are below 2^31");
+    KATSU_REQUIRE(top <= KATSU_DISTILL_MAX_TOP, "at most KATSU_DISTILL_MAX_TOP entries of a row");
+    KATSU_REQUIRE(a.temperature > 0.f && isfinite(a.temperature), "temperature must be above 0, and finite");
+    KATSU_REQUIRE(isfinite(a.soft) && isfinite(a.hard), "soft and hard must be finite");
+    if (rows == 0) return KATSU_OK;
+    KATSU_REQUIRE(vocab != 0, "a loss needs a vocabulary");
+    KATSU_REQUIRE(a.logits != nullptr, "logits is null");
+    KATSU_REQUIRE(top == 0 || a.soft == 0.f || (a.teacher != nullptr && a.index != nullptr), "teacher or index is null");
+    const struct {
+        const void *p;
+        size_t bytes;
+    } in[] = {{a.teacher, 4 * rows * top}, {a.index, 4 * rows * top}, {a.labels, 4 * rows}, {a.weight, 4 * rows}, {a.g, 4 * rows},
+              {a.logits, 4 * rows * vocab}}, out[] = {{a.loss, 4 * rows}, {a.dlogits, 4 * rows * vocab}};
+    for (const auto &o : out) {
+        KATSU_REQUIRE(katsu_whole(o.p), "an address is not that of a whole element");
+        for (const auto &i : in) {
+            KATSU_REQUIRE(katsu_whole(i.p), "an address is not that of a whole element");
+            KATSU_REQUIRE((o.p == a.dlogits && i.p == a.logits && o.p == i.p && !a.accumulate) || !katsu_overlap(o.p, o.bytes, i.p, i.bytes),
+                          "an output is an input too, or overlaps one");
+        }
+    }
+    KATSU_REQUIRE(!katsu_overlap(out[0].p, out[0].bytes, out[1].p, out[1].bytes), "loss and dlogits overlap");
+    return KATSU_OK;
+}
+
+}  // namespace
+
+extern "C" int32_t katsu_cuda_distill_fwd(katsu_cuda_ctx *ctx, const float *logits, const float *teacher, const int32_t *index,
+                                          const int32_t *labels, const float *weight, float temperature, float soft, float hard,
+                                          float *loss, size_t rows, size_t vocab, size_t top) {
+    const Distill a = {logits, teacher, weight, nullptr, index, labels, loss, nullptr, temperature, soft, hard,
+                       0.f, 0.f, unsigned(rows), unsigned(vocab), unsigned(top), 1, 0};
+    KATSU_TRY(check(ctx, a, rows, vocab, top));
+    KATSU_REQUIRE(loss != nullptr || rows == 0, "loss is null");
+    KATSU_TRY(katsu_bind(ctx));
+    return rows ? run<false>(ctx, a) : KATSU_OK;
+}
+
+extern "C" int32_t katsu_cuda_distill_bwd(katsu_cuda_ctx *ctx, const float *logits, const float *teacher, const int32_t *index,
+                                          const int32_t *labels, const float *weight, float temperature, float soft, float hard,
+                                          const float *g, float *loss, float *dlogits, size_t rows, size_t vocab, size_t top,
+                                          int32_t accumulate) {
+    const Distill a = {logits, teacher, weight, g, index, labels, loss, dlogits, temperature, soft, hard,
+                       0.f, 0.f, unsigned(rows), unsigned(vocab), unsigned(top), 1, accumulate != 0};
+    KATSU_TRY(check(ctx, a, rows, vocab, top));
+    KATSU_REQUIRE(dlogits != nullptr || rows == 0, "dlogits is null");
+    KATSU_TRY(katsu_bind(ctx));
+    return rows ? run<true>(ctx, a) : KATSU_OK;
+}

@@ -20,7 +20,7 @@
 
 namespace {
 
-constexpr int kHeld = 8;  // 16-byte accesses a thread holds
+constexpr int kHeld = 4;  // 16-byte accesses of a thread on their way together
 constexpr int kMostCluster = 8;
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -40,7 +40,12 @@ struct Sums {
 
 // A warp or block without a value above -infinity counts from the lowest number, which leaves its sums 0.
 __device__ __forceinline__ float base_of(float m) { return fmaxf(m, -FLT_MAX); }
-__device__ __forceinline__ float ex(float d, float c) { return exp2f(d * c); }
+// 2^(d c), zero where that is no normal number
+__device__ __forceinline__ float ex(float d, float c) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d * c));
+    return r;
+}
 
 template <bool TWO>
 __device__ __forceinline__ Sums join(const Distill &a, Sums x, Sums y) {
@@ -92,20 +97,32 @@ struct Entries {
     float *t;    // t - largest t
 };
 
-// Four values from place 4 u - lead of a row of `vocab`; what is outside of it is -infinity.
-__device__ __forceinline__ float4 load_row(const float *row, unsigned u, unsigned lead, unsigned vocab) {
-    const long long first = 4ll * u - lead;
-    if (first >= 0 && first + 4 <= vocab) return *reinterpret_cast<const float4 *>(row + first);
-    float v[4];
-#pragma unroll
-    for (int c = 0; c < 4; ++c) v[c] = first + c >= 0 && first + c < vocab ? row[first + c] : -INFINITY;
-    return make_float4(v[0], v[1], v[2], v[3]);
-}
+// A row as whole 16-byte units, and up to three values in front of the first and behind the last one, which the first block of
+// the row takes, a value a thread.
+struct Row {
+    unsigned head, units, edge;  // values in front; units; values in front and behind
+    unsigned begin, end;         // the block's units
 
-// GRAD: writes the gradient (and the loss where it is asked for).  TWO: sums at the temperature and at 1; otherwise one set of
-// sums is both.  ONCE: the row fits the registers; otherwise it is read again for the gradient.
-template <int THREADS, bool GRAD, bool TWO, bool ONCE>
-__global__ void __launch_bounds__(THREADS, 1024 / THREADS) distill_kernel(Distill a) {
+    __device__ Row(const float *z, unsigned vocab, unsigned rank, unsigned blocks) {
+        head = min(vocab, (0u - unsigned(reinterpret_cast<uintptr_t>(z) >> 2)) & 3u);
+        units = (vocab - head) / 4;
+        edge = rank ? 0 : vocab - 4 * units;
+        const unsigned share = (units + blocks - 1) / blocks;
+        begin = min(units, rank * share);
+        end = min(units, begin + share);
+    }
+    __device__ unsigned edge_token(unsigned i) const { return i < head ? i : 4 * units + i; }
+    __device__ bool has(unsigned token) const {
+        const unsigned place = token - head;
+        if (token >= head && place < 4 * units) return place >= 4 * begin && place < 4 * end;
+        return edge != 0;
+    }
+};
+
+// THREADS threads go through the row, the warp behind them through its entries.  GRAD: writes the gradient (and the loss where it is
+// asked for).  TWO: sums at the temperature and at 1; otherwise one set of sums is both.
+template <int THREADS, bool GRAD, bool TWO>
+__global__ void __launch_bounds__(THREADS + 32, 65536 / ((THREADS + 32) * 40)) distill_kernel(Distill a) {
     extern __shared__ float dynamic[];
     __shared__ Sums of_warp[THREADS / 32];
     __shared__ Sums of_block[kMostCluster];
@@ -115,32 +132,22 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) distill_kernel(Distil
     const float weight = a.weight ? a.weight[row] : 1.f;
     const float *z = a.logits + size_t(row) * a.vocab;
     float *dz = GRAD ? a.dlogits + size_t(row) * a.vocab : nullptr;
-    const unsigned lead = unsigned(reinterpret_cast<uintptr_t>(z) >> 2) & 3u, out_lead = unsigned(reinterpret_cast<uintptr_t>(dz) >> 2) & 3u;
-    const unsigned units = (a.vocab + lead + 3) / 4, share = (units + a.blocks - 1) / a.blocks;
-    const unsigned begin = min(units, rank * share), end = min(units, begin + share);
+    const Row part(z, a.vocab, rank, a.blocks);
+    const float4 *body = reinterpret_cast<const float4 *>(z + part.head);
+    auto zeros = [&] {
+        for (unsigned v = part.head + 4 * part.begin + threadIdx.x; v < part.head + 4 * part.end; v += THREADS + 32) dz[v] = 0.f;
+        if (threadIdx.x < part.edge) dz[part.edge_token(threadIdx.x)] = 0.f;
+    };
     if (weight == 0.f) {  // (all blocks of the row)
-        if (GRAD && !a.accumulate) {
-            const unsigned v0 = max(4 * begin, lead) - lead, v1 = min(4 * end - lead, a.vocab);
-            if (begin < end)
-                for (unsigned v = v0 + threadIdx.x; v < v1; v += THREADS) dz[v] = 0.f;
-        }
+        if (GRAD && !a.accumulate) zeros();
         if (a.loss && rank == 0 && threadIdx.x == 0) a.loss[row] = 0.f;
         return;
     }
     if (a.blocks > 1) sm100::cluster_arrive();
-    float4 v[kHeld];
-    auto fetch = [&](unsigned from) {
-#pragma unroll
-        for (int q = 0; q < kHeld; ++q) {
-            const unsigned u = from + q * THREADS + threadIdx.x;
-            v[q] = u < end ? load_row(z, u, lead, a.vocab) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-        }
-    };
-    fetch(begin);
-    // ---- the teacher's entries ----
     const unsigned listed = a.top + 1;
     const Entries entries = {reinterpret_cast<int *>(dynamic), dynamic + listed, dynamic + 2 * listed, dynamic + 3 * listed};
-    if (warp == 0) {
+    if (warp == THREADS / 32) {
+        // ---- the teacher's entries ----
         float most = -INFINITY;
         for (unsigned j = lane; j < a.top; j += 32) {
             const int token = a.index[size_t(row) * a.top + j];
@@ -168,32 +175,43 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) distill_kernel(Distil
             entries.e[a.top] = 0.f;
             teacher_sum = sum;
         }
-        __syncwarp();
-    }
-    // ---- largest value and sums of the row ----
-    Sums s = {-INFINITY, 0.f, 0.f};
-    for (unsigned from = begin;;) {
-        float most = -INFINITY;
+    } else {
+        // ---- largest value and sums of the row: a thread's own, then the warp's ----
+        Sums s = {threadIdx.x < part.edge ? z[part.edge_token(threadIdx.x)] : -INFINITY, 0.f, 0.f};
+        s.s0 = s.s1 = ex(s.m - base_of(s.m), a.c0);
+        auto take = [&](const float4 (&v)[kHeld]) {
+            float most = s.m;
 #pragma unroll
-        for (int q = 0; q < kHeld; ++q) most = fmaxf(most, fmaxf(fmaxf(v[q].x, v[q].y), fmaxf(v[q].z, v[q].w)));
-        Sums here = {largest_of_warp(most), 0.f, 0.f};
-        const float b = base_of(here.m);
+            for (int q = 0; q < kHeld; ++q) most = fmaxf(most, fmaxf(fmaxf(v[q].x, v[q].y), fmaxf(v[q].z, v[q].w)));
+            const float b = base_of(most), d = base_of(s.m) - b;
+            s.s0 *= ex(d, a.c0);
+            if (TWO) s.s1 *= ex(d, a.c1);
+            s.m = most;
 #pragma unroll
-        for (int q = 0; q < kHeld; ++q) {
-            here.s0 += ex(v[q].x - b, a.c0) + ex(v[q].y - b, a.c0) + (ex(v[q].z - b, a.c0) + ex(v[q].w - b, a.c0));
-            if (TWO) here.s1 += ex(v[q].x - b, a.c1) + ex(v[q].y - b, a.c1) + (ex(v[q].z - b, a.c1) + ex(v[q].w - b, a.c1));
+            for (int q = 0; q < kHeld; ++q) {
+                s.s0 += ex(v[q].x - b, a.c0) + ex(v[q].y - b, a.c0) + (ex(v[q].z - b, a.c0) + ex(v[q].w - b, a.c0));
+                if (TWO) s.s1 += ex(v[q].x - b, a.c1) + ex(v[q].y - b, a.c1) + (ex(v[q].z - b, a.c1) + ex(v[q].w - b, a.c1));
+            }
+        };
+        unsigned u = part.begin + threadIdx.x;
+        for (; u + (kHeld - 1) * THREADS < part.end; u += kHeld * THREADS) {
+            float4 v[kHeld];
+#pragma unroll
+            for (int q = 0; q < kHeld; ++q) v[q] = body[u + q * THREADS];
+            take(v);
         }
-        s = ONCE ? here : join<TWO>(a, s, here);
-        if (ONCE) break;
-        from += kHeld * THREADS;
-        if (from >= end) break;
-        fetch(from);
+        if (u < part.end) {
+            float4 v[kHeld];
+#pragma unroll
+            for (int q = 0; q < kHeld; ++q)
+                v[q] = u + q * THREADS < part.end ? body[u + q * THREADS] : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+            take(v);
+        }
+        s = join_lanes<TWO>(a, s, 32);
+        if (lane == 0) of_warp[warp] = s;
     }
-    s.s0 = sum_of_warp(s.s0);
-    if (TWO) s.s1 = sum_of_warp(s.s1);
-    if (lane == 0) of_warp[warp] = s;
     __syncthreads();
-    s = join_lanes<TWO>(a, of_warp[lane % (THREADS / 32)], THREADS / 32);
+    Sums s = join_lanes<TWO>(a, of_warp[lane % (THREADS / 32)], THREADS / 32);
     if (a.blocks > 1) {
         sm100::cluster_wait();  // the others run: their shared memory is there
         if (warp == 0 && lane < a.blocks) {
@@ -210,7 +228,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) distill_kernel(Distil
     const float b = base_of(s.m), s1 = TWO ? s.s1 : s.s0;
     const bool taught = a.soft != 0.f && !(teacher_sum == 0.f);
     const bool labelled = a.hard != 0.f && entries.token[a.top] >= 0;
-    if (a.loss && rank == 0 && warp == 0) {
+    if (a.loss && rank == 0 && warp == THREADS / 32) {
         // log p_j - log q_j = (t_j - largest t - (z_j - b)) / T - log sum e + log s0: differences that nearly cancel, in 64 bits
         double total = 0.0, apart = 0.0;
         for (unsigned j = lane; j < a.top; j += 32) {
@@ -233,44 +251,63 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) distill_kernel(Distil
     const float of_row = weight * (a.g ? a.g[row] : 1.f);
     const float soft = taught ? of_row * a.soft * a.temperature : 0.f, hard = labelled ? of_row * a.hard : 0.f;
     const float k0 = TWO ? soft / s.s0 : (soft + hard) / s.s0, k1 = TWO ? hard / s1 : 0.f;
-    const bool none = !taught && !labelled;  // such a row has a loss of 0, whatever it holds
+    if (!taught && !labelled) {  // such a row has a loss of 0, whatever it holds
+        if (!a.accumulate) zeros();
+        return;
+    }
     auto slope = [&](float value) {
-        if (none) return 0.f;
         const float d = value - b;
         float r = k0 * ex(d, a.c0);
         if (TWO) r += k1 * ex(d, a.c1);
         return r;
     };
-    for (unsigned from = begin;;) {
-        if (!ONCE) fetch(from);
-#pragma unroll
-        for (int q = 0; q < kHeld; ++q) {
-            const unsigned u = from + q * THREADS + threadIdx.x;
-            if (u >= end) continue;
-            const long long first = 4ll * u - lead;
-            float d[4] = {slope(v[q].x), slope(v[q].y), slope(v[q].z), slope(v[q].w)};
-            if (out_lead == lead && first >= 0 && first + 4 <= a.vocab) {
-                float4 *dst = reinterpret_cast<float4 *>(dz + first);
+    if (warp < THREADS / 32) {
+        float4 *out = reinterpret_cast<float4 *>(dz + part.head);
+        const bool whole = (reinterpret_cast<uintptr_t>(out) & 15u) == 0;  // the gradient's rows lie as the logits' do
+        auto put = [&](unsigned u, float4 v) {
+            v = make_float4(slope(v.x), slope(v.y), slope(v.z), slope(v.w));
+            if (whole) {
                 if (a.accumulate) {
-                    const float4 old = *dst;
-                    d[0] += old.x, d[1] += old.y, d[2] += old.z, d[3] += old.w;
+                    const float4 old = out[u];
+                    v.x += old.x, v.y += old.y, v.z += old.z, v.w += old.w;
                 }
-                *dst = make_float4(d[0], d[1], d[2], d[3]);
+                out[u] = v;
             } else {
-#pragma unroll
-                for (int c = 0; c < 4; ++c)
-                    if (first + c >= 0 && first + c < a.vocab) dz[first + c] = a.accumulate ? dz[first + c] + d[c] : d[c];
+                float *at = dz + part.head + 4 * size_t(u);
+                at[0] = a.accumulate ? at[0] + v.x : v.x;
+                at[1] = a.accumulate ? at[1] + v.y : v.y;
+                at[2] = a.accumulate ? at[2] + v.z : v.z;
+                at[3] = a.accumulate ? at[3] + v.w : v.w;
             }
+        };
+        if (threadIdx.x < part.edge) {
+            const unsigned token = part.edge_token(threadIdx.x);
+            const float d = slope(z[token]);
+            dz[token] = a.accumulate ? dz[token] + d : d;
         }
-        from += kHeld * THREADS;
-        if (ONCE || from >= end) break;
+        unsigned u = part.begin + threadIdx.x;
+        for (; u + (kHeld - 1) * THREADS < part.end; u += kHeld * THREADS) {
+            float4 v[kHeld];
+#pragma unroll
+            for (int q = 0; q < kHeld; ++q) v[q] = body[u + q * THREADS];
+#pragma unroll
+            for (int q = 0; q < kHeld; ++q) put(u + q * THREADS, v[q]);
+        }
+        if (u < part.end) {
+            float4 v[kHeld];
+#pragma unroll
+            for (int q = 0; q < kHeld; ++q)
+                if (u + q * THREADS < part.end) v[q] = body[u + q * THREADS];
+#pragma unroll
+            for (int q = 0; q < kHeld; ++q)
+                if (u + q * THREADS < part.end) put(u + q * THREADS, v[q]);
+        }
     }
     __syncthreads();
     // listed tokens of this block's part, each by its first entry
-    const unsigned v0 = max(4 * begin, lead) - lead, v1 = begin < end ? min(4 * end - lead, a.vocab) : v0;
-    for (unsigned j = threadIdx.x; j < listed; j += THREADS) {
+    for (unsigned j = threadIdx.x; j < listed; j += THREADS + 32) {
         const unsigned token = unsigned(entries.token[j]);
-        if (token < v0 || token >= v1) continue;
+        if (token >= a.vocab || !part.has(token)) continue;
         bool first = true;
         float e = 0.f;
         for (unsigned i = 0; i < listed; ++i) {
@@ -287,17 +324,11 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) distill_kernel(Distil
     }
 }
 
-template <int THREADS, bool GRAD, bool TWO, bool ONCE>
+template <int THREADS, bool GRAD, bool TWO>
 int32_t launch(katsu_cuda_ctx *ctx, const Distill &a) {
     const size_t smem = 4 * sizeof(float) * (size_t(a.top) + 1), blocks = size_t(a.rows) * a.blocks;
     if (blocks > 0x7fffffffu) return katsu_set_error(KATSU_ERR_UNSUPPORTED, "%u rows of %u logits in one loss", a.rows, a.vocab);
-    return katsu_launch(ctx, false, distill_kernel<THREADS, GRAD, TWO, ONCE>, unsigned(blocks), THREADS, smem, a.blocks, a);
-}
-
-template <int THREADS, bool GRAD>
-int32_t launch_for(katsu_cuda_ctx *ctx, const Distill &a, bool two, bool once) {
-    if (two) return once ? launch<THREADS, GRAD, true, true>(ctx, a) : launch<THREADS, GRAD, true, false>(ctx, a);
-    return once ? launch<THREADS, GRAD, false, true>(ctx, a) : launch<THREADS, GRAD, false, false>(ctx, a);
+    return katsu_launch(ctx, false, distill_kernel<THREADS, GRAD, TWO>, unsigned(blocks), THREADS + 32, smem, a.blocks, a);
 }
 
 template <bool GRAD>
@@ -310,14 +341,14 @@ int32_t run(katsu_cuda_ctx *ctx, Distill a) {
     a.c1 = kLog2e;
     a.c0 = kLog2e / a.temperature;
     const bool two = a.hard != 0.f && a.soft != 0.f && a.temperature != 1.f;
-    // blocks of as few threads as hold a row, then clusters of the largest
-    const size_t units = (size_t(a.vocab) + 3 + 3) / 4;
-    const size_t threads = units <= 128 * kHeld ? 128 : units <= 256 * kHeld ? 256 : 512;
+    const size_t units = (size_t(a.vocab) + 3) / 4;
+    const int threads = units <= 2048 ? 128 : units <= 8192 ? 256 : 512;
     a.blocks = 1;
-    while (a.blocks < kMostCluster && units > a.blocks * threads * kHeld) a.blocks *= 2;
-    const bool once = units <= a.blocks * threads * kHeld;
-    return threads == 128 ? launch_for<128, GRAD>(ctx, a, two, once)
-         : threads == 256 ? launch_for<256, GRAD>(ctx, a, two, once) : launch_for<512, GRAD>(ctx, a, two, once);
+    // few rows: blocks share them; a gradient's rows in L2 between their two readings
+    while (a.blocks < kMostCluster && (size_t(a.rows) * a.blocks < size_t(2) * ctx->num_sms || (GRAD && units > a.blocks * size_t(4096))) && units > size_t(a.blocks) * 2 * threads * kHeld)
+        a.blocks *= 2;
+    if (two) return threads == 128 ? launch<128, GRAD, true>(ctx, a) : threads == 256 ? launch<256, GRAD, true>(ctx, a) : launch<512, GRAD, true>(ctx, a);
+    return threads == 128 ? launch<128, GRAD, false>(ctx, a) : threads == 256 ? launch<256, GRAD, false>(ctx, a) : launch<512, GRAD, false>(ctx, a);
 }
 
 // The checks of both calls.  loss is null where it is not asked for, dlogits in the forward.

@@ -57,16 +57,20 @@ __device__ __forceinline__ Sums join(const Distill &a, Sums x, Sums y) {
     return r;
 }
 
-template <bool TWO>
-__device__ __forceinline__ Sums join_lanes(const Distill &a, Sums x, int lanes) {
+// Joins those of LANES neighbouring lanes: the largest value first, every lane's sums counted from it, then their sum.
+template <bool TWO, int LANES>
+__device__ __forceinline__ Sums join_lanes(const Distill &a, Sums x) {
+    float most = x.m;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        if (o >= lanes) continue;
-        Sums y;
-        y.m = __shfl_xor_sync(0xffffffffu, x.m, o);
-        y.s0 = __shfl_xor_sync(0xffffffffu, x.s0, o);
-        y.s1 = TWO ? __shfl_xor_sync(0xffffffffu, x.s1, o) : 0.f;
-        x = join<TWO>(a, x, y);
+    for (int o = LANES / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+    const float d = base_of(x.m) - base_of(most);
+    x.m = most;
+    x.s0 *= ex(d, a.c0);
+    if (TWO) x.s1 *= ex(d, a.c1);
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) {
+        x.s0 += __shfl_xor_sync(0xffffffffu, x.s0, o);
+        if (TWO) x.s1 += __shfl_xor_sync(0xffffffffu, x.s1, o);
     }
     return x;
 }
@@ -129,7 +133,7 @@ __global__ void __launch_bounds__(THREADS + 32, 65536 / ((THREADS + 32) * 40)) d
     __shared__ float teacher_sum;
     const unsigned lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const unsigned row = blockIdx.x / a.blocks, rank = blockIdx.x % a.blocks;
-    const float weight = a.weight ? a.weight[row] : 1.f;
+    const float weight = a.weight ? a.weight[row] : 1.f, of_row = GRAD && a.g ? a.g[row] : 1.f;
     const float *z = a.logits + size_t(row) * a.vocab;
     float *dz = GRAD ? a.dlogits + size_t(row) * a.vocab : nullptr;
     const Row part(z, a.vocab, rank, a.blocks);
@@ -148,6 +152,7 @@ __global__ void __launch_bounds__(THREADS + 32, 65536 / ((THREADS + 32) * 40)) d
     const Entries entries = {reinterpret_cast<int *>(dynamic), dynamic + listed, dynamic + 2 * listed, dynamic + 3 * listed};
     if (warp == THREADS / 32) {
         // ---- the teacher's entries ----
+        const int label = a.labels ? a.labels[row] : -1;
         float most = -INFINITY;
         for (unsigned j = lane; j < a.top; j += 32) {
             const int token = a.index[size_t(row) * a.top + j];
@@ -168,7 +173,6 @@ __global__ void __launch_bounds__(THREADS + 32, 65536 / ((THREADS + 32) * 40)) d
         }
         sum = sum_of_warp(sum);
         if (lane == 0) {
-            const int label = a.labels ? a.labels[row] : -1;
             const bool there = unsigned(label) < a.vocab;
             entries.token[a.top] = there ? label : -1;
             entries.z[a.top] = there ? z[label] : 0.f;
@@ -207,11 +211,11 @@ __global__ void __launch_bounds__(THREADS + 32, 65536 / ((THREADS + 32) * 40)) d
                 v[q] = u + q * THREADS < part.end ? body[u + q * THREADS] : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
             take(v);
         }
-        s = join_lanes<TWO>(a, s, 32);
+        s = join_lanes<TWO, 32>(a, s);
         if (lane == 0) of_warp[warp] = s;
     }
     __syncthreads();
-    Sums s = join_lanes<TWO>(a, of_warp[lane % (THREADS / 32)], THREADS / 32);
+    Sums s = join_lanes<TWO, THREADS / 32>(a, of_warp[lane % (THREADS / 32)]);
     if (a.blocks > 1) {
         sm100::cluster_wait();  // the others run: their shared memory is there
         if (warp == 0 && lane < a.blocks) {
@@ -248,8 +252,7 @@ __global__ void __launch_bounds__(THREADS + 32, 65536 / ((THREADS + 32) * 40)) d
     }
     if (!GRAD) return;
     // ---- the gradient ----
-    const float of_row = weight * (a.g ? a.g[row] : 1.f);
-    const float soft = taught ? of_row * a.soft * a.temperature : 0.f, hard = labelled ? of_row * a.hard : 0.f;
+    const float scale = weight * of_row, soft = taught ? scale * a.soft * a.temperature : 0.f, hard = labelled ? scale * a.hard : 0.f;
     const float k0 = TWO ? soft / s.s0 : (soft + hard) / s.s0, k1 = TWO ? hard / s1 : 0.f;
     if (!taught && !labelled) {  // such a row has a loss of 0, whatever it holds
         if (!a.accumulate) zeros();
@@ -271,7 +274,7 @@ __global__ void __launch_bounds__(THREADS + 32, 65536 / ((THREADS + 32) * 40)) d
                     const float4 old = out[u];
                     v.x += old.x, v.y += old.y, v.z += old.z, v.w += old.w;
                 }
-                out[u] = v;
+                __stcs(out + u, v);
             } else {
                 float *at = dz + part.head + 4 * size_t(u);
                 at[0] = a.accumulate ? at[0] + v.x : v.x;
@@ -289,7 +292,7 @@ __global__ void __launch_bounds__(THREADS + 32, 65536 / ((THREADS + 32) * 40)) d
         for (; u + (kHeld - 1) * THREADS < part.end; u += kHeld * THREADS) {
             float4 v[kHeld];
 #pragma unroll
-            for (int q = 0; q < kHeld; ++q) v[q] = body[u + q * THREADS];
+            for (int q = 0; q < kHeld; ++q) v[q] = __ldcs(body + u + q * THREADS);
 #pragma unroll
             for (int q = 0; q < kHeld; ++q) put(u + q * THREADS, v[q]);
         }
@@ -297,7 +300,7 @@ __global__ void __launch_bounds__(THREADS + 32, 65536 / ((THREADS + 32) * 40)) d
             float4 v[kHeld];
 #pragma unroll
             for (int q = 0; q < kHeld; ++q)
-                if (u + q * THREADS < part.end) v[q] = body[u + q * THREADS];
+                if (u + q * THREADS < part.end) v[q] = __ldcs(body + u + q * THREADS);
 #pragma unroll
             for (int q = 0; q < kHeld; ++q)
                 if (u + q * THREADS < part.end) put(u + q * THREADS, v[q]);
@@ -342,13 +345,13 @@ int32_t run(katsu_cuda_ctx *ctx, Distill a) {
     a.c0 = kLog2e / a.temperature;
     const bool two = a.hard != 0.f && a.soft != 0.f && a.temperature != 1.f;
     const size_t units = (size_t(a.vocab) + 3) / 4;
-    const int threads = units <= 2048 ? 128 : units <= 8192 ? 256 : 512;
+    const int threads = units <= 2048 ? 128 : 256;
     a.blocks = 1;
     // few rows: blocks share them; a gradient's rows in L2 between their two readings
     while (a.blocks < kMostCluster && (size_t(a.rows) * a.blocks < size_t(2) * ctx->num_sms || (GRAD && units > a.blocks * size_t(4096))) && units > size_t(a.blocks) * 2 * threads * kHeld)
         a.blocks *= 2;
-    if (two) return threads == 128 ? launch<128, GRAD, true>(ctx, a) : threads == 256 ? launch<256, GRAD, true>(ctx, a) : launch<512, GRAD, true>(ctx, a);
-    return threads == 128 ? launch<128, GRAD, false>(ctx, a) : threads == 256 ? launch<256, GRAD, false>(ctx, a) : launch<512, GRAD, false>(ctx, a);
+    if (two) return threads == 128 ? launch<128, GRAD, true>(ctx, a) : launch<256, GRAD, true>(ctx, a);
+    return threads == 128 ? launch<128, GRAD, false>(ctx, a) : launch<256, GRAD, false>(ctx, a);
 }
 
 // The checks of both calls.  loss is null where it is not asked for, dlogits in the forward.

@@ -3,7 +3,7 @@
 //   y[i] = scale * table[t_i]                        dtable[v] (+)= scale * sum over i with t_i = v of dy[i]
 //
 // The lookup reads the rows of the tokens and writes y: HBM.  The gradient sorts the tokens (positions of one token in
-// ascending order behind each other), cuts the sorted list into pieces of kPiece and adds up each piece on its own, whatever
+// ascending order behind each other), cuts the sorted list into pieces of 8 to 64 and adds up each piece on its own, whatever
 // the tokens are: a token of a tenth of all positions costs what a thousand rare ones cost.  Runs that lie in one piece are
 // written as they end; what a piece has of a run that began in front of it or goes on behind it is kept beside the table
 // and folded by a second launch in the pieces' order.  No floating-point atomics: the same tokens give the same bits.
@@ -40,8 +40,8 @@ __device__ __forceinline__ void store(float *p, const Values<VEC> &r) {
 }
 
 // ---- lookup ----------------------------------------------------------------------------------------------------------
-// A row is `units` accesses of VEC values; 1 << shift threads share a row (a block's slab of 4 << shift accesses of it, where
-// it is longer).  Four accesses of a thread are on their way together.
+// A row is `units` accesses of VEC values; 1 << shift threads share a row, four accesses each (a block's slab of 1024 accesses of
+// it, where it is longer): a thread's four are on their way together (100 000 rows of 64 values: 10.5 us with one access a thread).
 struct Rows {
     unsigned count, units, slabs;
     int shift;
@@ -52,7 +52,7 @@ Rows rows_of(size_t count, size_t units) {
     r.count = unsigned(count);
     r.units = unsigned(units);
     r.shift = 0;
-    while (r.shift < 8 && (size_t(1) << r.shift) < units) ++r.shift;
+    while (r.shift < 8 && (size_t(4) << r.shift) < units) ++r.shift;
     r.slabs = unsigned(katsu_div_up(units, size_t(4) << r.shift));
     return r;
 }
@@ -87,7 +87,7 @@ __global__ void __launch_bounds__(kThreads) embed_kernel(const void *table, cons
                 v[q].v[0] = row[u];
             }
         } else {
-            v[q] = load<VEC>(static_cast<const float *>(table) + size_t(token) * cols + size_t(u) * VEC);
+            v[q] = load<VEC>(static_cast<const float *>(table) + size_t(token) * pitch + size_t(u) * VEC);
         }
     }
 #pragma unroll
@@ -100,17 +100,65 @@ __global__ void __launch_bounds__(kThreads) embed_kernel(const void *table, cons
     }
 }
 
+// Rows that are not whole 16-byte units: y is written by 16 bytes from its own boundary on, whatever rows these are of, and the
+// table is read value by value.  Fewer than 2^32 values in all.
+template <bool INT8>
+__global__ void __launch_bounds__(kThreads) embed_flat_kernel(const void *table, const float *rows_scale, const int *tokens, float scale,
+                                                              float *y, unsigned values, unsigned vocab, size_t pitch, unsigned cols, int waves) {
+    if (!waves) launch_next();
+    launch_wait();
+    const unsigned lead = unsigned(reinterpret_cast<uintptr_t>(y) >> 2) & 3u;
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        // places are counted from the boundary at or in front of y; those in front of it are numbers above `values`
+        const unsigned long long place = 4ull * ((unsigned long long)blockIdx.x * (2 * kThreads) + q * kThreads + threadIdx.x);
+        if (place >= (unsigned long long)values + lead) return;
+        const unsigned first = unsigned(place) - lead;
+        float v[4];
+        unsigned row = (first < values ? first : 0) / cols, col = (first < values ? first : 0) - row * cols;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            v[c] = 0.f;
+            if (first + c >= values) continue;
+            const unsigned token = unsigned(tokens[row]);
+            if (token < vocab) {
+                if (INT8) v[c] = (float(static_cast<const int8_t *>(table)[size_t(token) * pitch + col]) * rows_scale[token]) * scale;
+                else v[c] = static_cast<const float *>(table)[size_t(token) * pitch + col] * scale;
+            }
+            if (++col == cols) {
+                col = 0;
+                ++row;
+            }
+        }
+        if (first < values && values - first >= 4) {
+            *reinterpret_cast<float4 *>(y + first) = make_float4(v[0], v[1], v[2], v[3]);
+        } else {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                if (first + c < values) y[first + c] = v[c];
+        }
+    }
+}
+
 bool vectors(const void *p, size_t cols) { return cols % 4 == 0 && reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
-template <int VEC, bool INT8>
-int32_t launch_lookup(katsu_cuda_ctx *ctx, const void *table, const float *rows_scale, const int *tokens, float scale, float *y,
-                      size_t count, size_t vocab, size_t pitch, size_t cols) {
-    const Rows rows = rows_of(count, cols / VEC);
+// pitch: bytes (8-bit rows) or values (others) from one row of the table to the next
+template <bool INT8>
+int32_t lookup(katsu_cuda_ctx *ctx, const void *table, const float *rows_scale, const int *tokens, float scale, float *y, size_t count,
+               size_t vocab, size_t pitch, size_t cols) {
+    const bool whole = vectors(y, cols) && (INT8 || vectors(table, cols));
+    if (!whole && count * cols < 0xfffffff0u) {
+        const size_t blocks = katsu_div_up(count * cols + 3, size_t(8) * kThreads);
+        const bool waves = blocks > size_t(2) * ctx->num_sms;
+        return katsu_launch(ctx, !waves, embed_flat_kernel<INT8>, unsigned(blocks), kThreads, 0, 1, table, rows_scale, tokens, scale, y,
+                            unsigned(count * cols), unsigned(vocab), pitch, unsigned(cols), int(waves));
+    }
+    const Rows rows = rows_of(count, whole ? cols / 4 : cols);
     const size_t blocks = katsu_div_up(count, kThreads >> rows.shift) * rows.slabs;
     if (blocks > 0x7fffffffu) return katsu_set_error(KATSU_ERR_UNSUPPORTED, "%zu rows of %zu values in one lookup", count, cols);
     const bool waves = blocks > size_t(2) * ctx->num_sms;
-    return katsu_launch(ctx, !waves, embed_kernel<VEC, INT8>, unsigned(blocks), kThreads, 0, 1, table, rows_scale, tokens, scale, y, rows,
-                        unsigned(vocab), pitch, cols, int(waves));
+    return katsu_launch(ctx, !waves, whole ? embed_kernel<4, INT8> : embed_kernel<1, INT8>, unsigned(blocks), kThreads, 0, 1, table, rows_scale,
+                        tokens, scale, y, rows, unsigned(vocab), pitch, cols, int(waves));
 }
 
 // ---- sorting the tokens --------------------------------------------------------------------------------------------------
@@ -120,19 +168,22 @@ constexpr int kRanked = 32, kMostRanked = 8192;
 __device__ __forceinline__ unsigned key_of(int token, unsigned vocab) { return min(unsigned(token), vocab); }
 
 // Up to 8192 tokens: the place of a token is the number of tokens that belong in front of it.  A block counts for 32 of them,
-// its warps over an eighth of the list each: 64 comparisons a lane and cycle of the GPU, one launch (8192 tokens: 67 million
-// comparisons).
-__global__ void __launch_bounds__(256) rank_kernel(const int *tokens, unsigned count, unsigned vocab, unsigned *keys, int *position) {
+// its warps over a sixteenth of the list each, 32 comparisons a lane for four loads of 16 bytes: one launch, 67 million
+// comparisons for 8192 tokens.
+constexpr int kRankThreads = 512;
+
+__global__ void __launch_bounds__(kRankThreads) rank_kernel(const int *tokens, unsigned count, unsigned vocab, unsigned *keys, int *position) {
     __shared__ __align__(16) unsigned all[kMostRanked];
-    __shared__ int partial[8][kRanked];
+    __shared__ int partial[kRankThreads / 32][kRanked];
     launch_next();
     launch_wait();
     const unsigned tiles = (count + 31) / 32, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    for (unsigned j = threadIdx.x; j < tiles * 32; j += 256) all[j] = j < count ? key_of(tokens[j], vocab) : 0xffffffffu;
+#pragma unroll 4
+    for (unsigned j = threadIdx.x; j < tiles * 32; j += kRankThreads) all[j] = j < count ? key_of(tokens[j], vocab) : 0xffffffffu;
     __syncthreads();
     const unsigned i = blockIdx.x * kRanked + lane, key = all[i];
     int before = 0;
-    for (unsigned tile = warp; tile < tiles; tile += 8) {
+    for (unsigned tile = warp; tile < tiles; tile += kRankThreads / 32) {
         const uint4 *of_tile = reinterpret_cast<const uint4 *>(all + 32 * tile);
         const unsigned limit = key + (tile < blockIdx.x ? 1 : 0);  // in front: equal ones count too
 #pragma unroll
@@ -141,20 +192,26 @@ __global__ void __launch_bounds__(256) rank_kernel(const int *tokens, unsigned c
             before += (k.x < limit) + (k.y < limit) + (k.z < limit) + (k.w < limit);
         }
         if (tile == blockIdx.x)
-            for (unsigned j = 0; j < lane; ++j) before += all[32 * tile + j] == key;
+#pragma unroll
+            for (unsigned q = 0; q < 8; ++q) {
+                const uint4 k = of_tile[q];
+                before += (k.x == key && 4 * q < lane) + (k.y == key && 4 * q + 1 < lane) + (k.z == key && 4 * q + 2 < lane) +
+                          (k.w == key && 4 * q + 3 < lane);
+            }
     }
     partial[warp][lane] = before;
     __syncthreads();
     if (warp != 0 || i >= count) return;
     int place = 0;
 #pragma unroll
-    for (int w = 0; w < 8; ++w) place += partial[w][lane];
+    for (int w = 0; w < kRankThreads / 32; ++w) place += partial[w][lane];
     keys[place] = key;
     position[place] = int(i);
 }
 
-// More: passes over digits of up to 10 bits from the lowest on, two launches each.  A block has `tile` of the keys.
-constexpr int kDigits = 1024, kSorters = 128;
+// More: passes over digits of two to ten bits from the lowest on, a launch each, behind one that counts the first pass's digits; a
+// pass counts those of the next where it puts the keys.  A block has `tile` of the keys, a multiple of kTile.
+constexpr int kDigits = 1024, kSorters = 128, kTile = 2048;
 
 struct Pass {
     const int *tokens;                              // first pass
@@ -166,8 +223,8 @@ struct Pass {
 
 __device__ __forceinline__ unsigned pass_key(const Pass &p, unsigned i) { return p.tokens ? key_of(p.tokens[i], p.vocab) : p.keys[i]; }
 
-// digits[block][digit]: how many of the block's keys have the digit.
-__global__ void __launch_bounds__(256) digits_kernel(Pass p, unsigned *digits) {
+// digits[block][digit]: how many of the block's keys have the digit.  next: zeros, for the pass behind.
+__global__ void __launch_bounds__(256) digits_kernel(Pass p, unsigned *digits, unsigned *next) {
     __shared__ unsigned mine[kDigits];
     launch_next();
     const unsigned values = 1u << p.bits, mask = values - 1;
@@ -175,39 +232,74 @@ __global__ void __launch_bounds__(256) digits_kernel(Pass p, unsigned *digits) {
     __syncthreads();
     launch_wait();
     const unsigned begin = blockIdx.x * p.tile, end = min(p.count, begin + p.tile);
+#pragma unroll 8
     for (unsigned i = begin + threadIdx.x; i < end; i += 256) atomicAdd(&mine[(pass_key(p, i) >> p.shift) & mask], 1u);
     __syncthreads();
-    for (unsigned d = threadIdx.x; d < values; d += 256) digits[blockIdx.x * values + d] = mine[d];
+    for (unsigned d = threadIdx.x; d < values; d += 256) {
+        digits[blockIdx.x * values + d] = mine[d];
+        next[blockIdx.x * values + d] = 0;
+    }
 }
 
-// Moves the block's keys to their places.  A warp takes an eighth of them in order, so that equal digits keep theirs.
-__global__ void __launch_bounds__(256) scatter_kernel(Pass p, const unsigned *digits, unsigned *keys, int *position) {
-    __shared__ unsigned place[8][kDigits];
+// Moves the block's keys to their places, and counts the next pass's digits there (next, null: this is the last one; behind: zeros
+// for the one behind that).  A warp takes an eighth of them in order, so that equal digits keep theirs; eight keys
+// a lane are on their way together.
+__global__ void __launch_bounds__(256) scatter_kernel(Pass p, const unsigned *digits, unsigned *next, unsigned *behind, unsigned *keys, int *position) {
+    __shared__ __align__(16) unsigned place[8][kDigits];
+    __shared__ __align__(16) unsigned all[kDigits], front[kDigits];
     __shared__ unsigned sums[8];
     launch_next();
-    launch_wait();
     const unsigned values = 1u << p.bits, mask = values - 1, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    for (unsigned d = threadIdx.x; d < 8 * kDigits; d += 256) (&place[0][0])[d] = 0;
+    for (unsigned d = lane; d < values; d += 32) place[warp][d] = 0;
+    for (unsigned d = threadIdx.x; d < kDigits; d += 256) all[d] = front[d] = 0;
     __syncthreads();
+    launch_wait();
     const unsigned share = p.tile / 8, begin = min(p.count, blockIdx.x * p.tile + warp * share), end = min(p.count, begin + share);
-    for (unsigned i = begin + lane; i < end; i += 32) atomicAdd(&place[warp][(pass_key(p, i) >> p.shift) & mask], 1u);
-    __syncthreads();
-    // a thread's four digits: keys of each in all blocks and in those in front of this one
-    unsigned all[4] = {0, 0, 0, 0}, front[4] = {0, 0, 0, 0};
-    const unsigned d0 = 4 * threadIdx.x;
-    if (d0 < values) {
-#pragma unroll 8
-        for (unsigned b = 0; b < gridDim.x; ++b) {
-            const unsigned *of_block = digits + size_t(b) * values + d0;
+    if (behind)
+        for (unsigned d = threadIdx.x; d < values; d += 256) behind[blockIdx.x * values + d] = 0;
+    unsigned key[8];
+    int at[8];
+    auto fetch = [&](unsigned from) {
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const unsigned n = d0 + q < values ? of_block[q] : 0;
-                all[q] += n;
-                front[q] += b < blockIdx.x ? n : 0;
-            }
+        for (int q = 0; q < 8; ++q) {
+            const unsigned i = from + 32 * q + lane;
+            key[q] = i < end ? pass_key(p, i) : 0xffffffffu;  // (no key: keys are at most 2^31 - 1)
+            at[q] = p.tokens ? int(i) : i < end ? p.position[i] : 0;
+        }
+    };
+    fetch(begin);
+    // keys of each digit in all blocks and in those in front of this one: four digits a thread, the blocks shared out among threads
+    const unsigned quads = values / 4, parts = 256 / quads, quad = threadIdx.x % quads;
+    uint4 sum_all = make_uint4(0, 0, 0, 0), sum_front = sum_all;
+    for (unsigned b0 = threadIdx.x / quads; b0 < gridDim.x; b0 += 8 * parts) {
+        uint4 n[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+            const unsigned b = b0 + q * parts;
+            n[q] = b < gridDim.x ? *reinterpret_cast<const uint4 *>(digits + size_t(b) * values + 4 * quad) : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+            sum_all.x += n[q].x, sum_all.y += n[q].y, sum_all.z += n[q].z, sum_all.w += n[q].w;
+            if (b0 + q * parts < blockIdx.x) sum_front.x += n[q].x, sum_front.y += n[q].y, sum_front.z += n[q].z, sum_front.w += n[q].w;
         }
     }
-    unsigned sum = all[0] + all[1] + all[2] + all[3], scan = sum;
+    const unsigned of_all[4] = {sum_all.x, sum_all.y, sum_all.z, sum_all.w}, of_front[4] = {sum_front.x, sum_front.y, sum_front.z, sum_front.w};
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        atomicAdd(&all[4 * quad + q], of_all[q]);
+        atomicAdd(&front[4 * quad + q], of_front[q]);
+    }
+    for (unsigned from = begin; from < end; from += 256) {
+        if (from != begin) fetch(from);
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+            if (key[q] != 0xffffffffu) atomicAdd(&place[warp][(key[q] >> p.shift) & mask], 1u);
+    }
+    __syncthreads();
+    const uint4 mine = reinterpret_cast<const uint4 *>(all)[threadIdx.x];  // zeros behind the digits
+    unsigned scan = mine.x + mine.y + mine.z + mine.w;
+    const unsigned sum = scan;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const unsigned other = __shfl_up_sync(0xffffffffu, scan, o);
@@ -217,47 +309,61 @@ __global__ void __launch_bounds__(256) scatter_kernel(Pass p, const unsigned *di
     __syncthreads();
     unsigned first = scan - sum;
     for (unsigned w = 0; w < warp; ++w) first += sums[w];
-    if (d0 < values) {
+    if (4 * threadIdx.x < values) {
+        const uint4 in_front = reinterpret_cast<const uint4 *>(front)[threadIdx.x];
+        uint4 from = make_uint4(first + in_front.x, first + mine.x + in_front.y, first + mine.x + mine.y + in_front.z,
+                                first + mine.x + mine.y + mine.z + in_front.w);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            unsigned at = first + front[q];
-            if (d0 + q < values)
-                for (int w = 0; w < 8; ++w) {
-                    const unsigned n = place[w][d0 + q];
-                    place[w][d0 + q] = at;
-                    at += n;
-                }
-            first += all[q];
+        for (int w = 0; w < 8; ++w) {
+            uint4 *at = reinterpret_cast<uint4 *>(place[w]) + threadIdx.x;
+            const uint4 n = *at;
+            *at = from;
+            from.x += n.x, from.y += n.y, from.z += n.z, from.w += n.w;
         }
     }
     __syncthreads();
-    for (unsigned i0 = begin; i0 < end; i0 += 32) {
-        const unsigned i = i0 + lane;
-        const bool valid = i < end;
-        const unsigned key = valid ? pass_key(p, i) : 0, digit = valid ? (key >> p.shift) & mask : 0xffffffffu;
-        const unsigned same = __match_any_sync(0xffffffffu, digit), ahead = __popc(same & ((1u << lane) - 1));
-        unsigned at = 0;
-        if (valid) at = place[warp][digit] + ahead;
-        __syncwarp();
-        if (valid && ahead == 0) place[warp][digit] += __popc(same);
-        __syncwarp();
-        if (!valid) continue;
-        keys[at] = key;
-        position[at] = p.tokens ? int(i) : p.position[i];
+    const bool again = end - begin > 256;
+    for (unsigned from = begin; from < end; from += 256) {
+        if (again) fetch(from);
+        unsigned same[8];  // lanes with the same digit, by a vote on each of its bits: matching takes a step for each different one
+#pragma unroll
+        for (int q = 0; q < 8; ++q) same[q] = __ballot_sync(0xffffffffu, key[q] != 0xffffffffu);
+        for (int bit = p.shift; bit < p.shift + p.bits; ++bit)
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                const unsigned ones = __ballot_sync(0xffffffffu, key[q] >> bit & 1);
+                same[q] &= key[q] >> bit & 1 ? ones : ~ones;
+            }
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+            const bool valid = key[q] != 0xffffffffu;
+            const unsigned digit = (key[q] >> p.shift) & mask, ahead = __popc(same[q] & ((1u << lane) - 1));
+            unsigned to = 0;
+            if (valid) to = place[warp][digit] + ahead;
+            __syncwarp();
+            if (valid && ahead == 0) place[warp][digit] = to + __popc(same[q]);
+            __syncwarp();
+            if (!valid) continue;
+            keys[to] = key[q];
+            position[to] = at[q];
+            if (next) atomicAdd(next + size_t(to / p.tile) * values + (key[q] >> (p.shift + p.bits) & mask), 1u);
+        }
     }
 }
 
 // ---- the gradient ----------------------------------------------------------------------------------------------------------
-constexpr int kPiece = 32, kGradThreads = 128;
+constexpr int kGradThreads = 128, kMostPiece = 64, kDirect = 256;
 
 struct Grad {
+    const int *tokens;  // few tokens: unsorted
     const unsigned *keys;
     const int *position;
     const float *dy;
     float *dtable, *kept;  // kept [piece][2][pitch]: of the run that began in front; of the one that goes on behind
     float scale;
-    unsigned count, vocab, units, slabs, pieces, piece_blocks, fill_rows;
-    int shift, accumulate;
+    unsigned count, vocab, units, slabs, piece, pieces, piece_blocks, fill_rows;
+    int shift, waves;
+    bool accumulate;
     size_t cols, pitch;
 };
 
@@ -273,23 +379,112 @@ __device__ __forceinline__ unsigned lower_bound(const unsigned *keys, unsigned c
 }
 
 template <int VEC>
-__device__ __forceinline__ void write_row(const Grad &g, unsigned key, unsigned u, Values<VEC> sum) {
-    float *dst = g.dtable + size_t(key) * g.cols + size_t(u) * VEC;
-    Values<VEC> old;
-    if (g.accumulate) old = load<VEC>(dst);
+__device__ __forceinline__ float *row_of(const Grad &g, unsigned key, unsigned u) {
+    return g.dtable + size_t(key) * g.cols + size_t(u) * VEC;
+}
+
+template <int VEC>
+__device__ __forceinline__ Values<VEC> zero_values() {
+    Values<VEC> r;
 #pragma unroll
-    for (int c = 0; c < VEC; ++c) sum.v[c] = g.accumulate ? fmaf(g.scale, sum.v[c], old.v[c]) : g.scale * sum.v[c];
+    for (int c = 0; c < VEC; ++c) r.v[c] = 0.f;
+    return r;
+}
+
+// sum = scale * sum, added to what the table has where that is asked for
+template <int VEC, bool ADD>
+__device__ __forceinline__ void write_row(const Grad &g, float *dst, Values<VEC> sum, const Values<VEC> &old) {
+#pragma unroll
+    for (int c = 0; c < VEC; ++c) sum.v[c] = ADD ? fmaf(g.scale, sum.v[c], old.v[c]) : g.scale * sum.v[c];
     store<VEC>(dst, sum);
+}
+
+// Zeros for rows row0 .. row0 + rows - 1 but for those that are `there`, by 16 bytes from the first boundary of a row on.
+__device__ __forceinline__ void fill_rows(const Grad &g, const bool *there, unsigned row0, unsigned rows) {
+    const unsigned width = 1u << g.shift, groups = kGradThreads >> g.shift, lane = threadIdx.x & (width - 1);
+    for (unsigned r = threadIdx.x >> g.shift; r < rows; r += groups) {
+        if (there[r]) continue;
+        float *row = g.dtable + size_t(row0 + r) * g.cols;
+        const unsigned cols = unsigned(g.cols), head = min(cols, (0u - unsigned(reinterpret_cast<uintptr_t>(row) >> 2)) & 3u), units = (cols - head) / 4;
+        if (lane < head) row[lane] = 0.f;
+        float4 *body = reinterpret_cast<float4 *>(row + head);
+        for (unsigned u = lane; u < units; u += width) body[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (lane < cols - head - 4 * units) row[head + 4 * units + lane] = 0.f;
+    }
+}
+
+// Up to kDirect tokens, without sorting: a group of 1 << shift threads takes the run of one token, if that is its first place.
+template <int VEC, bool ADD>
+__global__ void __launch_bounds__(kGradThreads) embed_direct_kernel(Grad g) {
+    __shared__ __align__(16) unsigned keys[kDirect];
+    __shared__ bool there[kGradThreads];
+    if (!g.waves) launch_next();
+    launch_wait();
+    for (unsigned j = threadIdx.x; j < kDirect; j += kGradThreads) keys[j] = j < g.count ? key_of(g.tokens[j], g.vocab) : 0xffffffffu;
+    there[threadIdx.x] = false;
+    __syncthreads();
+    if (blockIdx.x >= g.piece_blocks) {
+        const unsigned row0 = (blockIdx.x - g.piece_blocks) * g.fill_rows, rows = min(g.fill_rows, g.vocab - row0);
+        for (unsigned j = threadIdx.x; j < kDirect; j += kGradThreads)
+            if (keys[j] - row0 < rows) there[keys[j] - row0] = true;
+        __syncthreads();
+        fill_rows(g, there, row0, rows);
+        return;
+    }
+    const unsigned groups = kGradThreads >> g.shift, i = blockIdx.x / g.slabs * groups + (threadIdx.x >> g.shift);
+    const unsigned u = ((blockIdx.x % g.slabs) << g.shift) + (threadIdx.x & ((1u << g.shift) - 1));
+    if (i >= g.count || u >= g.units) return;
+    const unsigned key = keys[i];
+    if (key >= g.vocab) return;
+    // places of the token: the next one from `from` on in `same`, the 64 places of one word after the other
+    auto word = [&](unsigned from) {
+        unsigned long long same = 0;
+#pragma unroll 4
+        for (unsigned j = 0; j < 64; j += 4) {
+            const uint4 k = *reinterpret_cast<const uint4 *>(keys + from + j);
+            same |= (unsigned long long)((k.x == key) | (k.y == key) << 1 | (k.z == key) << 2 | (k.w == key) << 3) << j;
+        }
+        return same;
+    };
+    unsigned from = i & ~63u;
+    unsigned long long same = word(from);
+    if (same << (63 - (i & 63)) << 1) return;  // an earlier place, in this word or in those in front of it
+    for (unsigned front = 0; front < from; front += 64)
+        if (word(front)) return;
+    float *dst = row_of<VEC>(g, key, u);
+    const Values<VEC> old = ADD ? load<VEC>(dst) : zero_values<VEC>();
+    Values<VEC> sum = zero_values<VEC>();
+    for (;;) {
+        while (!same && from + 64 < g.count) same = word(from += 64);
+        if (!same) break;
+        Values<VEC> v[8];
+        int taken = 0;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+            if (!same) continue;
+            v[q] = load<VEC>(g.dy + size_t(from + __ffsll((long long)same) - 1) * g.cols + size_t(u) * VEC);
+            same &= same - 1;
+            taken = q + 1;
+        }
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+            if (q < taken)
+#pragma unroll
+                for (int c = 0; c < VEC; ++c) sum.v[c] += v[q].v[c];
+    }
+    write_row<VEC, ADD>(g, dst, sum, old);
 }
 
 // Blocks 0 .. piece_blocks - 1: a group of 1 << shift threads adds up a piece (a slab of 1 << shift accesses of its rows); the
 // blocks behind them write zeros to fill_rows rows of the table each, but for those of tokens that are there.
-template <int VEC>
-__global__ void __launch_bounds__(kGradThreads) embed_grad_kernel(Grad g) {
+template <int VEC, bool ADD>
+__global__ void __launch_bounds__(kGradThreads, ADD ? 5 : 8) embed_grad_kernel(Grad g) {
     const unsigned width = 1u << g.shift, groups = kGradThreads >> g.shift, mine = threadIdx.x >> g.shift, lane = threadIdx.x & (width - 1);
-    __shared__ unsigned keys[kGradThreads / 4 * kPiece + 2];
-    __shared__ int position[kGradThreads / 4 * kPiece];
+    extern __shared__ unsigned keys[];  // of the block's pieces, their positions behind them
+    int *position = reinterpret_cast<int *>(keys + groups * g.piece + 2);
     __shared__ bool there[kGradThreads];
+    if (!g.waves) launch_next();
+    launch_wait();
     if (blockIdx.x >= g.piece_blocks) {
         const unsigned row0 = (blockIdx.x - g.piece_blocks) * g.fill_rows, rows = min(g.fill_rows, g.vocab - row0);
         if (threadIdx.x < rows) {
@@ -297,18 +492,11 @@ __global__ void __launch_bounds__(kGradThreads) embed_grad_kernel(Grad g) {
             there[threadIdx.x] = at < g.count && g.keys[at] == key;
         }
         __syncthreads();
-        Values<VEC> zero;
-#pragma unroll
-        for (int c = 0; c < VEC; ++c) zero.v[c] = 0.f;
-        for (unsigned r = mine; r < rows; r += groups) {
-            if (there[r]) continue;
-            float *row = g.dtable + size_t(row0 + r) * g.cols;
-            for (unsigned u = lane; u < g.units; u += width) store<VEC>(row + size_t(u) * VEC, zero);
-        }
+        fill_rows(g, there, row0, rows);
         return;
     }
-    const unsigned slab = blockIdx.x % g.slabs, piece0 = blockIdx.x / g.slabs * groups, begin0 = piece0 * kPiece;
-    const unsigned staged = min(groups * kPiece, g.count - begin0);
+    const unsigned slab = blockIdx.x % g.slabs, piece0 = blockIdx.x / g.slabs * groups, begin0 = piece0 * g.piece;
+    const unsigned staged = min(groups * g.piece, g.count - begin0);
     // keys[1 + j] is that of place begin0 + j; one in front and one behind as well, ~0 where there is none
     for (unsigned j = threadIdx.x; j < staged; j += kGradThreads) {
         keys[1 + j] = g.keys[begin0 + j];
@@ -317,19 +505,22 @@ __global__ void __launch_bounds__(kGradThreads) embed_grad_kernel(Grad g) {
     if (threadIdx.x == 0) keys[0] = begin0 ? g.keys[begin0 - 1] : ~0u;
     if (threadIdx.x == 1) keys[1 + staged] = begin0 + staged < g.count ? g.keys[begin0 + staged] : ~0u;
     __syncthreads();
-    const unsigned piece = piece0 + mine, u = slab * width + lane, j0 = mine * kPiece;
+    const unsigned piece = piece0 + mine, u = slab * width + lane, j0 = mine * g.piece;
     if (piece >= g.pieces || u >= g.units) return;
-    const unsigned j1 = min(staged, j0 + kPiece);
+    const unsigned j1 = min(staged, j0 + g.piece);
     float *kept = g.kept + size_t(piece) * 2 * g.pitch + size_t(u) * VEC;
     bool began = keys[j0] != keys[j0 + 1];  // the current run began in this piece
-    Values<VEC> sum;
-#pragma unroll
-    for (int c = 0; c < VEC; ++c) sum.v[c] = 0.f;
+    Values<VEC> sum = zero_values<VEC>();
     for (unsigned j = j0; j < j1; j += 8) {
-        Values<VEC> v[8];
+        Values<VEC> v[8], old[8];
 #pragma unroll
         for (int q = 0; q < 8; ++q)
             if (j + q < j1) v[q] = load<VEC>(g.dy + size_t(position[j + q]) * g.cols + size_t(u) * VEC);
+        if (ADD)  // rows that end here, asked for with the others: one by one they took a trip to memory each
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+                if (j + q < j1 && keys[2 + j + q] != keys[1 + j + q] && keys[1 + j + q] < g.vocab)
+                    old[q] = load<VEC>(row_of<VEC>(g, keys[1 + j + q], u));
 #pragma unroll
         for (int q = 0; q < 8; ++q) {
             if (j + q >= j1) continue;
@@ -339,43 +530,56 @@ __global__ void __launch_bounds__(kGradThreads) embed_grad_kernel(Grad g) {
             const bool ends = keys[2 + j + q] != key;
             if (!ends && j + q + 1 < j1) continue;
             if (key < g.vocab) {
-                if (ends && began) write_row<VEC>(g, key, u, sum);
+                if (ends && began) write_row<VEC, ADD>(g, row_of<VEC>(g, key, u), sum, old[q]);
                 else store<VEC>(kept + (began ? g.pitch : 0), sum);
             }
             began = true;
-#pragma unroll
-            for (int c = 0; c < VEC; ++c) sum.v[c] = 0.f;
+            sum = zero_values<VEC>();
         }
     }
 }
 
 // Runs of more than one piece: what their first piece kept behind, and what every later one kept in front.
-template <int VEC>
+template <int VEC, bool ADD>
 __global__ void __launch_bounds__(kGradThreads) embed_fold_kernel(Grad g) {
     const unsigned width = 1u << g.shift, groups = kGradThreads >> g.shift, lane = threadIdx.x & (width - 1);
+    if (!g.waves) launch_next();
+    launch_wait();
     const unsigned piece = blockIdx.x / g.slabs * groups + (threadIdx.x >> g.shift), u = blockIdx.x % g.slabs * width + lane;
-    if (piece + 1 >= g.pieces || u >= g.units) return;
-    const unsigned begin = piece * kPiece, next = begin + kPiece, key = g.keys[next - 1];
-    if (key >= g.vocab || g.keys[next] != key) return;
-    if (begin && g.keys[begin - 1] == key && g.keys[begin] == key) return;  // began in front of this piece
-    const unsigned end = next + lower_bound(g.keys + next, g.count - next, key + 1), last = (end - 1) / kPiece;
+    const unsigned begin = piece * g.piece, next = begin + g.piece;
+    if (piece + 1 >= g.pieces) return;
+    const unsigned front = begin ? g.keys[begin - 1] : ~0u, first = g.keys[begin], key = g.keys[next - 1], behind = g.keys[next];
+    if (key != behind || key >= g.vocab || (front == key && first == key)) return;  // (all threads of the group) not a run that began here and goes on
+    // the pieces that the run passes through whole: the threads of the group that are in one warp look at one each
+    const unsigned looking = min(width, 32u), mask = looking == 32 ? ~0u : ((1u << looking) - 1) << (threadIdx.x & 31 & ~(looking - 1));
+    unsigned last = piece + 1;
+    for (;;) {
+        const unsigned p = last + (lane & (looking - 1));
+        const bool goes_on = p + 1 < g.pieces && g.keys[(p + 1) * g.piece] == key;
+        const unsigned through = __popc(__ballot_sync(mask, goes_on) & mask);
+        last += through;
+        if (through < looking) break;
+    }
+    if (u >= g.units) return;
     const float *kept = g.kept + size_t(u) * VEC;
+    float *dst = row_of<VEC>(g, key, u);
+    const Values<VEC> old = ADD ? load<VEC>(dst) : zero_values<VEC>();
     Values<VEC> sum = load<VEC>(kept + (size_t(piece) * 2 + 1) * g.pitch);
-    for (unsigned p = piece + 1; p <= last; p += 8) {
-        Values<VEC> v[8];
+    for (unsigned p = piece + 1; p <= last; p += 16) {
+        Values<VEC> v[16];
 #pragma unroll
-        for (int q = 0; q < 8; ++q)
+        for (int q = 0; q < 16; ++q)
             if (p + q <= last) v[q] = load<VEC>(kept + size_t(p + q) * 2 * g.pitch);
 #pragma unroll
-        for (int q = 0; q < 8; ++q)
+        for (int q = 0; q < 16; ++q)
             if (p + q <= last)
 #pragma unroll
                 for (int c = 0; c < VEC; ++c) sum.v[c] += v[q].v[c];
     }
-    write_row<VEC>(g, key, u, sum);
+    write_row<VEC, ADD>(g, dst, sum, old);
 }
 
-template <int VEC>
+template <int VEC, bool ADD>
 int32_t launch_grad(katsu_cuda_ctx *ctx, Grad g) {
     g.units = unsigned(g.cols / VEC);
     g.shift = 2;
@@ -383,14 +587,22 @@ int32_t launch_grad(katsu_cuda_ctx *ctx, Grad g) {
     g.slabs = (g.units + (1u << g.shift) - 1) >> g.shift;
     const size_t groups = kGradThreads >> g.shift, piece_blocks = katsu_div_up(g.pieces, groups) * g.slabs;
     g.fill_rows = unsigned(std::min<size_t>(kGradThreads, std::max<size_t>(1, 16384 / g.cols)));
-    const size_t fill_blocks = g.accumulate ? 0 : katsu_div_up(g.vocab, g.fill_rows);
-    if (piece_blocks + fill_blocks > 0x7fffffffu)
+    const size_t fill_blocks = ADD ? 0 : katsu_div_up(g.vocab, g.fill_rows), blocks = piece_blocks + fill_blocks;
+    if (blocks > 0x7fffffffu)
         return katsu_set_error(KATSU_ERR_UNSUPPORTED, "%u tokens with rows of %zu values in one gradient", g.count, g.cols);
     g.piece_blocks = unsigned(piece_blocks);
-    if (piece_blocks + fill_blocks)
-        KATSU_LAUNCH(ctx, embed_grad_kernel<VEC>, unsigned(piece_blocks + fill_blocks), kGradThreads, 0, g);
-    if (g.pieces > 1) KATSU_LAUNCH(ctx, embed_fold_kernel<VEC>, unsigned(piece_blocks), kGradThreads, 0, g);
-    return KATSU_OK;
+    const size_t resident = size_t(4) * ctx->num_sms;  // (of 128 threads with up to 128 registers)
+    g.waves = blocks > resident;
+    if (g.tokens) return katsu_launch(ctx, !g.waves, embed_direct_kernel<VEC, ADD>, unsigned(blocks), kGradThreads, 0, 1, g);
+    KATSU_TRY(katsu_launch(ctx, !g.waves, embed_grad_kernel<VEC, ADD>, unsigned(blocks), kGradThreads, (2 * groups * g.piece + 2) * sizeof(unsigned), 1, g));
+    if (g.pieces == 1) return KATSU_OK;
+    g.waves = piece_blocks > resident;
+    return katsu_launch(ctx, !g.waves, embed_fold_kernel<VEC, ADD>, g.piece_blocks, kGradThreads, 0, 1, g);
+}
+
+int32_t launch_grad_for(katsu_cuda_ctx *ctx, const Grad &g, bool vec) {
+    if (g.accumulate) return vec ? launch_grad<4, true>(ctx, g) : launch_grad<1, true>(ctx, g);
+    return vec ? launch_grad<4, false>(ctx, g) : launch_grad<1, false>(ctx, g);
 }
 
 // Leaves the sorted keys and their positions in two of the four arrays of `count` words at `work`.
@@ -400,18 +612,20 @@ int32_t sort_tokens(katsu_cuda_ctx *ctx, const int *tokens, unsigned count, unsi
     int *position_of_side[2] = {reinterpret_cast<int *>(work + count), reinterpret_cast<int *>(work + 3 * size_t(count))};
     int side = 0;
     if (count <= kMostRanked) {
-        KATSU_TRY(katsu_launch_chained(ctx, rank_kernel, (count + kRanked - 1) / kRanked, 256, 0, 1, tokens, count, vocab, key_of_side[0],
+        KATSU_TRY(katsu_launch_chained(ctx, rank_kernel, (count + kRanked - 1) / kRanked, kRankThreads, 0, 1, tokens, count, vocab, key_of_side[0],
                                        position_of_side[0]));
     } else {
         unsigned *digits = work + 4 * size_t(count);
-        const int bits = 32 - __builtin_clz(vocab), passes = (bits + 9) / 10, of_pass = (bits + passes - 1) / passes;
-        const unsigned blocks = std::min<unsigned>(kSorters, (count + 2047) / 2048), tile = ((count + blocks - 1) / blocks + 255) / 256 * 256;
+        const int bits = 32 - __builtin_clz(vocab), passes = (bits + 9) / 10, of_pass = std::max(2, (bits + passes - 1) / passes);
+        const unsigned blocks = std::min<unsigned>(kSorters, (count + kTile - 1) / kTile), tile = ((count + blocks - 1) / blocks + kTile - 1) / kTile * kTile;
         const unsigned grid = (count + tile - 1) / tile;
+        unsigned *of_pass_digits[3] = {digits, digits + kSorters * kDigits, digits + 2 * kSorters * kDigits};
         for (int pass = 0; pass < passes; ++pass, side ^= 1) {
             Pass p = {pass ? nullptr : tokens, key_of_side[side ^ 1], position_of_side[side ^ 1], count, vocab, tile, pass * of_pass, of_pass};
-            KATSU_TRY(katsu_launch_chained(ctx, digits_kernel, grid, 256, 0, 1, p, digits));
-            KATSU_TRY(katsu_launch_chained(ctx, scatter_kernel, grid, 256, 0, 1, p, static_cast<const unsigned *>(digits), key_of_side[side],
-                                           position_of_side[side]));
+            if (pass == 0) KATSU_TRY(katsu_launch_chained(ctx, digits_kernel, grid, 256, 0, 1, p, of_pass_digits[0], of_pass_digits[1]));
+            KATSU_TRY(katsu_launch_chained(ctx, scatter_kernel, grid, 256, 0, 1, p, static_cast<const unsigned *>(of_pass_digits[pass % 3]),
+                                           pass + 1 < passes ? of_pass_digits[(pass + 1) % 3] : nullptr,
+                                           pass + 2 < passes ? of_pass_digits[(pass + 2) % 3] : nullptr, key_of_side[side], position_of_side[side]));
         }
         side ^= 1;
     }
@@ -439,9 +653,7 @@ extern "C" int32_t katsu_cuda_embed_fwd(katsu_cuda_ctx *ctx, const float *table,
     KATSU_REQUIRE(!katsu_overlap(y, 4 * count * cols, table, 4 * vocab * cols) && !katsu_overlap(y, 4 * count * cols, tokens, 4 * count),
                   "y overlaps an input");
     KATSU_TRY(katsu_bind(ctx));
-    return vectors(table, cols) && vectors(y, cols)
-               ? launch_lookup<4, false>(ctx, table, nullptr, tokens, scale, y, count, vocab, 0, cols)
-               : launch_lookup<1, false>(ctx, table, nullptr, tokens, scale, y, count, vocab, 0, cols);
+    return lookup<false>(ctx, table, nullptr, tokens, scale, y, count, vocab, cols, cols);
 }
 
 extern "C" int32_t katsu_cuda_int8_embed(katsu_cuda_ctx *ctx, const int8_t *q, const float *rows_scale, const int32_t *tokens,
@@ -457,8 +669,7 @@ extern "C" int32_t katsu_cuda_int8_embed(katsu_cuda_ctx *ctx, const int8_t *q, c
     KATSU_REQUIRE(!katsu_overlap(y, bytes, q, vocab * pitch) && !katsu_overlap(y, bytes, rows_scale, 4 * vocab) &&
                       !katsu_overlap(y, bytes, tokens, 4 * count), "y overlaps an input");
     KATSU_TRY(katsu_bind(ctx));
-    return vectors(y, cols) ? launch_lookup<4, true>(ctx, q, rows_scale, tokens, scale, y, count, vocab, pitch, cols)
-                            : launch_lookup<1, true>(ctx, q, rows_scale, tokens, scale, y, count, vocab, pitch, cols);
+    return lookup<true>(ctx, q, rows_scale, tokens, scale, y, count, vocab, pitch, cols);
 }
 
 extern "C" int32_t katsu_cuda_embed_bwd(katsu_cuda_ctx *ctx, const int32_t *tokens, const float *dy, float scale, float *dtable,
@@ -477,14 +688,23 @@ extern "C" int32_t katsu_cuda_embed_bwd(katsu_cuda_ctx *ctx, const int32_t *toke
     g.scale = scale;
     g.count = unsigned(count);
     g.vocab = unsigned(vocab);
-    g.pieces = unsigned(katsu_div_up(count, kPiece));
     g.accumulate = accumulate != 0;
     g.cols = cols;
     g.pitch = (cols + 3) / 4 * 4;
-    const size_t sorting = (4 * count + size_t(kSorters) * kDigits + 3) / 4 * 4;
+    const bool vec = vectors(dy, cols) && vectors(dtable, cols);
+    if (count <= kDirect) {
+        g.tokens = tokens;
+        g.pieces = g.count;
+        return launch_grad_for(ctx, g, vec);
+    }
+    // A piece is a chain of loads, eight at a time; the fold of a run one of its pieces, sixteen at a time.  With a fifteenth of the
+    // tokens alike both are short at pieces of 8 to 64.  Where the rows are many bytes, short pieces write too many sums beside the table.
+    g.piece = count * cols >= size_t(1) << 22 ? (count <= 32768 ? 32 : kMostPiece) : count <= 4096 ? 8 : count <= 16384 ? 16 : count <= 65536 ? 32 : kMostPiece;
+    g.pieces = unsigned(katsu_div_up(count, g.piece));
+    const size_t sorting = 4 * count + 3 * size_t(kSorters) * kDigits;
     float *work = nullptr;
     KATSU_TRY(katsu_scratch(ctx, sorting + size_t(g.pieces) * 2 * g.pitch, &work));
     g.kept = work + sorting;
     KATSU_TRY(sort_tokens(ctx, tokens, g.count, g.vocab, reinterpret_cast<unsigned *>(work), &g.keys, &g.position));
-    return vectors(dy, cols) && vectors(dtable, cols) ? launch_grad<4>(ctx, g) : launch_grad<1>(ctx, g);
+    return launch_grad_for(ctx, g, vec);
 }

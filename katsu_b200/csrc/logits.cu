@@ -2,130 +2,185 @@
 //
 //   v = z / r or z r for tokens of the history      v -= f count + a for generated ones      v += biases      v = -inf if not allowed
 //
-// Bound: HBM, logits in (of allowed tokens) and out.  A block has a slice of a row: it counts the history's tokens of its slice in
-// shared memory (whole numbers: atomics in any order give the same counts) while the slice's logits are on their way, and
-// writes the slice once.  Tokens with biases, a few of a row, are written again behind it from the row's list in its order.
+// Bound: HBM, logits in (of allowed tokens) and out; few rows: a chain of loads.  A block has a slice of a row: it counts the
+// history's tokens of its slice in shared memory (whole numbers: atomics in any order give the same counts) while the slice's
+// logits are on their way, and writes the slice once.  Tokens with biases, a few of a row, are written again behind it from the
+// row's list in its order.  In place only what changes is read and written.
 #include <math.h>
+
+#include <algorithm>
 
 #include "common.cuh"
 #include "launch.cuh"
 
 namespace {
 
-constexpr int kThreads = 256, kHeld = 8;
-constexpr unsigned kSlice = 4 * kThreads * kHeld;  // tokens of a block
-constexpr unsigned kInPrompt = 0x80000000u;        // beside the count of generated ones
+constexpr int kThreads = 256, kBlocks = 4;  // blocks of an SM
+constexpr int kHeld = 4;                    // 16-byte accesses of a thread on their way together
+constexpr unsigned kStep = 4 * kThreads, kMostSlice = 16 * kStep;
 
 struct Adjust {
     const float *logits, *repetition, *presence, *frequency, *bias;
     const int *history, *prompts, *lengths, *bias_tokens;
     const unsigned *allowed;
     float *out;
-    unsigned rows, vocab, history_cols, biases, words, slices;
+    unsigned rows, vocab, history_cols, biases, words, slices, slice;  // slice: tokens of a block, a multiple of kStep
+    int waves;
 };
 
 struct Penalties {
     float repetition, presence, frequency;
 };
 
-__device__ __forceinline__ float penalised(float v, unsigned seen, const Penalties &p) {
-    if (seen == 0) return v;
-    v = v > 0.f ? v / p.repetition : v * p.repetition;
-    const unsigned count = seen & ~kInPrompt;
-    return count ? v - fmaf(p.frequency, float(count), p.presence) : v;
-}
+// A token's place: how often it is in the generated part, and a bit above for the prompt.  Two places share a word where the history
+// has less than 2^15 tokens.
+template <bool WIDE>
+struct Place {
+    static constexpr unsigned kPrompt = WIDE ? 0x80000000u : 0x8000u;
+    static __device__ __forceinline__ void count(unsigned *seen, unsigned place, bool prompt) {
+        if (WIDE) {
+            if (prompt) atomicOr(&seen[place], kPrompt);
+            else atomicAdd(&seen[place], 1u);
+        } else {
+            const unsigned up = 16 * (place & 1);
+            if (prompt) atomicOr(&seen[place >> 1], kPrompt << up);
+            else atomicAdd(&seen[place >> 1], 1u << up);
+        }
+    }
+    static __device__ __forceinline__ unsigned one(const unsigned *seen, unsigned place) {
+        return WIDE ? seen[place] : seen[place >> 1] >> (16 * (place & 1)) & 0xffffu;
+    }
+    // four places from a multiple of four on
+    static __device__ __forceinline__ uint4 four(const unsigned *seen, unsigned place) {
+        if (WIDE) return *reinterpret_cast<const uint4 *>(seen + place);
+        const uint2 two = *reinterpret_cast<const uint2 *>(seen + place / 2);
+        return make_uint4(two.x & 0xffffu, two.x >> 16, two.y & 0xffffu, two.y >> 16);
+    }
+    static __device__ __forceinline__ float penalised(float v, unsigned seen, const Penalties &p) {
+        if (seen == 0) return v;
+        v = v > 0.f ? v / p.repetition : v * p.repetition;
+        const unsigned count = seen & ~kPrompt;
+        return count ? v - fmaf(p.frequency, float(count), p.presence) : v;
+    }
+};
 
-__global__ void __launch_bounds__(kThreads) adjust_kernel(Adjust a) {
-    extern __shared__ __align__(16) unsigned seen[];  // [kSlice + 4], behind it the row's biases
+template <bool WIDE>
+__global__ void __launch_bounds__(kThreads, kBlocks) adjust_kernel(Adjust a) {
+    using P = Place<WIDE>;
+    extern __shared__ __align__(16) unsigned seen[];  // behind the places the row's biases
+    if (!a.waves) launch_next();
+    launch_wait();
     const unsigned row = blockIdx.x / a.slices, slice = blockIdx.x % a.slices;
     const float *z = a.logits + size_t(row) * a.vocab;
     float *out = a.out + size_t(row) * a.vocab;
+    const bool in_place = z == out;
     const unsigned *words = a.allowed ? a.allowed + size_t(row) * a.words : nullptr;
-    // The slice's places are counted from the 16-byte boundary at or in front of the row.
-    const unsigned lead = unsigned(reinterpret_cast<uintptr_t>(z) >> 2) & 3u, out_lead = unsigned(reinterpret_cast<uintptr_t>(out) >> 2) & 3u;
-    const long long base = (long long)slice * kSlice - lead;  // token of the slice's place 0 (negative: none)
-    // bit c: place 4 u + c is a token that is allowed
-    auto allowed = [&](long long first) {
-        unsigned bits = 0;
+    // The slice's places are counted from the 16-byte boundary at or in front of the row: base is the token of place 0.  Tokens are
+    // taken modulo 2^32, so that the up to three places in front of the row are numbers above the vocabulary.
+    const unsigned lead = unsigned(reinterpret_cast<uintptr_t>(z) >> 2) & 3u, base = slice * a.slice - lead;
+    const bool inside = base < a.vocab && a.vocab - base >= a.slice;  // (of all the slice's places)
+    const bool whole = (unsigned(reinterpret_cast<uintptr_t>(out) >> 2) & 3u) == lead;
+    // which of an access's tokens are allowed: bit c of token + c
+    auto allowed = [&](unsigned token) {
+        unsigned bits = 15;
+        if (inside) {
+            if (words) {
+                const unsigned shift = token & 31, low = words[token >> 5], high = shift > 28 ? words[(token >> 5) + 1] : 0;
+                bits = __funnelshift_r(low, high, shift) & 15;
+            }
+        } else {
+            bits = 0;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            const long long token = first + c;
-            if (token < 0 || token >= a.vocab) continue;
-            if (!words || (words[token >> 5] >> (token & 31) & 1u)) bits |= 1u << c;
+            for (unsigned c = 0; c < 4; ++c)
+                if (token + c < a.vocab && (!words || (words[(token + c) >> 5] >> ((token + c) & 31) & 1u))) bits |= 1u << c;
         }
         return bits;
     };
-    float4 v[kHeld];
+    auto fetch = [&](unsigned token, unsigned bits) {
+        if (bits == 0) return make_float4(0.f, 0.f, 0.f, 0.f);
+        if (inside) return *reinterpret_cast<const float4 *>(z + token);
+        return make_float4(bits & 1 ? z[token] : 0.f, bits & 2 ? z[token + 1] : 0.f, bits & 4 ? z[token + 2] : 0.f, bits & 8 ? z[token + 3] : 0.f);
+    };
     unsigned bits[kHeld];
+    float4 v[kHeld];
+    auto ask = [&](unsigned from) {
 #pragma unroll
-    for (int q = 0; q < kHeld; ++q) {
-        const long long first = base + 4ll * (q * kThreads + threadIdx.x);
-        bits[q] = allowed(first);
-        v[q] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (bits[q] == 0) continue;
-        if (first >= 0 && first + 4 <= a.vocab) {
-            v[q] = *reinterpret_cast<const float4 *>(z + first);
-        } else {
-            float one[4];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) one[c] = bits[q] >> c & 1u ? z[first + c] : 0.f;
-            v[q] = make_float4(one[0], one[1], one[2], one[3]);
+        for (int q = 0; q < kHeld; ++q) {
+            const unsigned place = from + q * kStep;
+            bits[q] = place < a.slice ? allowed(base + place) : 0;
         }
-    }
-    Penalties p = {1.f, 0.f, 0.f};
-    float *bias = reinterpret_cast<float *>(seen + kSlice), *bias_z = bias + a.biases;
+        if (!in_place)
+#pragma unroll
+            for (int q = 0; q < kHeld; ++q) v[q] = fetch(base + from + q * kStep, bits[q]);
+    };
+    ask(4 * threadIdx.x);
+    // ---- the history's tokens and the biases of the slice ----
+    const unsigned words_of_slice = !a.history ? 0 : WIDE ? a.slice : a.slice / 2;
+    float *bias = reinterpret_cast<float *>(seen + words_of_slice), *bias_z = bias + a.biases;
     int *bias_tokens = reinterpret_cast<int *>(bias_z + a.biases);
-    if (a.history) {
-        for (unsigned i = threadIdx.x; i < kSlice / 4; i += kThreads) reinterpret_cast<uint4 *>(seen)[i] = make_uint4(0, 0, 0, 0);
-        if (a.repetition) p.repetition = a.repetition[row];
-        if (a.presence) p.presence = a.presence[row];
-        if (a.frequency) p.frequency = a.frequency[row];
-    }
+    if (a.history)
+        for (unsigned i = threadIdx.x; i < words_of_slice / 4; i += kThreads) reinterpret_cast<uint4 *>(seen)[i] = make_uint4(0, 0, 0, 0);
     for (unsigned j = threadIdx.x; j < a.biases; j += kThreads) {
-        const long long token = a.bias_tokens[size_t(row) * a.biases + j];
-        const bool mine = token >= 0 && token < a.vocab && token >= base && token < base + kSlice;
+        const unsigned token = unsigned(a.bias_tokens[size_t(row) * a.biases + j]);
+        const bool mine = token < a.vocab && token - base < a.slice;
         bias_tokens[j] = mine ? int(token) : -1;
         bias[j] = a.bias[size_t(row) * a.biases + j];
         bias_z[j] = mine ? z[token] : 0.f;
     }
-    __syncthreads();
+    Penalties p = {1.f, 0.f, 0.f};
     if (a.history) {
+        const int *history = a.history + size_t(row) * a.history_cols;
         const unsigned length = a.lengths ? unsigned(min(max(a.lengths[row], 0), int(a.history_cols))) : a.history_cols;
         const unsigned prompt = a.prompts ? unsigned(min(max(a.prompts[row], 0), int(length))) : 0;
-        const int *history = a.history + size_t(row) * a.history_cols;
-#pragma unroll 8
-        for (unsigned i = threadIdx.x; i < length; i += kThreads) {
-            const int token = history[i];
-            const long long place = token - base;
-            if (token < 0 || unsigned(token) >= a.vocab || place < 0 || place >= kSlice) continue;
-            if (i < prompt) atomicOr(&seen[place], kInPrompt);
-            else atomicAdd(&seen[place], 1u);
-        }
+        if (a.repetition) p.repetition = a.repetition[row];
+        if (a.presence) p.presence = a.presence[row];
+        if (a.frequency) p.frequency = a.frequency[row];
         __syncthreads();
+        for (unsigned i = threadIdx.x; i < length; i += 8 * kThreads) {
+            int token[8];
+#pragma unroll
+            for (int q = 0; q < 8; ++q) token[q] = i + q * kThreads < length ? history[i + q * kThreads] : -1;
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+                if (unsigned(token[q]) < a.vocab && unsigned(token[q]) - base < a.slice) P::count(seen, unsigned(token[q]) - base, i + q * kThreads < prompt);
+        }
     }
+    if (a.history || a.biases) __syncthreads();
+    // ---- the slice ----
+    for (unsigned from = 4 * threadIdx.x;;) {
 #pragma unroll
-    for (int q = 0; q < kHeld; ++q) {
-        const unsigned place = 4 * (q * kThreads + threadIdx.x);
-        const long long first = base + place;
-        if (first + 3 < 0 || first >= a.vocab) continue;
-        float r[4] = {v[q].x, v[q].y, v[q].z, v[q].w};
-        if (a.history) {
-            const uint4 s = *reinterpret_cast<const uint4 *>(seen + place);
-            r[0] = penalised(r[0], s.x, p);
-            r[1] = penalised(r[1], s.y, p);
-            r[2] = penalised(r[2], s.z, p);
-            r[3] = penalised(r[3], s.w, p);
+        for (int q = 0; q < kHeld; ++q) {
+            const unsigned place = from + q * kStep, token = base + place;
+            if (place >= a.slice) continue;
+            uint4 s = make_uint4(0, 0, 0, 0);
+            if (a.history) s = P::four(seen, place);
+            const bool touched = (s.x | s.y | s.z | s.w) != 0;
+            if (in_place) {
+                if (bits[q] == 15 && !touched) continue;
+                v[q] = fetch(token, bits[q]);
+            }
+            if (touched) {
+                v[q].x = P::penalised(v[q].x, s.x, p);
+                v[q].y = P::penalised(v[q].y, s.y, p);
+                v[q].z = P::penalised(v[q].z, s.z, p);
+                v[q].w = P::penalised(v[q].w, s.w, p);
+            }
+            if (!(bits[q] & 1)) v[q].x = -INFINITY;
+            if (!(bits[q] & 2)) v[q].y = -INFINITY;
+            if (!(bits[q] & 4)) v[q].z = -INFINITY;
+            if (!(bits[q] & 8)) v[q].w = -INFINITY;
+            if (inside && whole) {
+                *reinterpret_cast<float4 *>(out + token) = v[q];
+            } else {
+                if (token < a.vocab) out[token] = v[q].x;
+                if (token + 1 < a.vocab) out[token + 1] = v[q].y;
+                if (token + 2 < a.vocab) out[token + 2] = v[q].z;
+                if (token + 3 < a.vocab) out[token + 3] = v[q].w;
+            }
         }
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-            if (!(bits[q] >> c & 1u)) r[c] = -INFINITY;
-        if (out_lead == lead && first >= 0 && first + 4 <= a.vocab) {
-            *reinterpret_cast<float4 *>(out + first) = make_float4(r[0], r[1], r[2], r[3]);
-        } else {
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-                if (first + c >= 0 && first + c < a.vocab) out[first + c] = r[c];
-        }
+        from += kHeld * kStep;
+        if (from >= a.slice) break;
+        ask(from);
     }
     if (a.biases == 0) return;
     __syncthreads();
@@ -139,8 +194,21 @@ __global__ void __launch_bounds__(kThreads) adjust_kernel(Adjust a) {
             first = first && i >= j;
             sum += bias[i];
         }
-        if (first) out[token] = (a.history ? penalised(bias_z[j], seen[token - base], p) : bias_z[j]) + sum;
+        if (first) out[token] = (a.history ? P::penalised(bias_z[j], P::one(seen, unsigned(token) - base), p) : bias_z[j]) + sum;
     }
+}
+
+template <bool WIDE>
+int32_t launch(katsu_cuda_ctx *ctx, Adjust a) {
+    // One round of blocks, as every block looks at the row's whole history; slices are bounded by the shared memory for their places.
+    const size_t places = size_t(a.vocab) + 3, resident = size_t(kBlocks) * ctx->num_sms, wanted = std::max<size_t>(1, resident / a.rows);
+    a.slice = unsigned(std::min<size_t>(kMostSlice, katsu_div_up(katsu_div_up(places, wanted), kStep) * kStep));
+    a.slices = unsigned(katsu_div_up(places, a.slice));
+    const size_t blocks = size_t(a.rows) * a.slices, smem = (a.history ? (WIDE ? 4 : 2) * size_t(a.slice) : 0) + 12 * size_t(a.biases);
+    if (blocks > 0x7fffffffu) return katsu_set_error(KATSU_ERR_UNSUPPORTED, "%u rows of %u logits in one call", a.rows, a.vocab);
+    KATSU_TRY(katsu_prepare_kernel(ctx, reinterpret_cast<const void *>(adjust_kernel<WIDE>), smem, false));
+    a.waves = blocks > size_t(2) * ctx->num_sms;
+    return katsu_launch(ctx, !a.waves, adjust_kernel<WIDE>, unsigned(blocks), kThreads, smem, 1, a);
 }
 
 }  // namespace
@@ -167,12 +235,9 @@ extern "C" int32_t katsu_cuda_adjust_logits(katsu_cuda_ctx *ctx, const float *lo
         KATSU_REQUIRE(katsu_whole(i.p) && katsu_whole(out), "an address is not that of a whole element");
         KATSU_REQUIRE((i.p == logits && out == logits) || !katsu_overlap(out, bytes, i.p, i.bytes), "out overlaps an input");
     }
-    Adjust a = {logits, repetition, presence, frequency, bias, history_cols ? history : nullptr, prompts, lengths, bias_tokens, allowed, out,
-                unsigned(rows), unsigned(vocab), unsigned(history_cols), unsigned(biases), unsigned(words),
-                unsigned((vocab + 3 + kSlice - 1) / kSlice)};
-    const size_t blocks = rows * a.slices, smem = 4 * size_t(kSlice) + 12 * biases;
-    if (blocks > 0x7fffffffu) return katsu_set_error(KATSU_ERR_UNSUPPORTED, "%zu rows of %zu logits in one call", rows, vocab);
     KATSU_TRY(katsu_bind(ctx));
-    KATSU_LAUNCH(ctx, adjust_kernel, unsigned(blocks), kThreads, smem, a);
-    return KATSU_OK;
+    const Adjust a = {logits, repetition, presence, frequency, bias, history_cols ? history : nullptr, prompts, lengths, bias_tokens, allowed, out,
+                      unsigned(rows), unsigned(vocab), unsigned(history_cols), unsigned(biases), unsigned(words), 0, 0, 0};
+    const bool wide = history_cols >= 1 << 15;
+    return wide ? launch<true>(ctx, a) : launch<false>(ctx, a);
 }

@@ -77,8 +77,11 @@ def test_lookup_of_no_tokens_and_in_no_table(ctx):
         assert not d.get("y").any()
 
 
-# counts around a piece of 32 places, and around 8192, where the sort changes; vocabularies of one to three digits of a sort
-GRADS = [(1, 1, 1, "one"), (2, 3, 5, "zipf"), (31, 1, 4, "one"), (32, 2, 4, "uniform"), (33, 1, 7, "one"), (64, 9, 16, "sorted"),
+# counts up to and above 256, to which tokens are not sorted, around 8192, where the sort changes, and 4096 to 65536, where pieces grow; vocabularies of
+# one to three digits of a sort
+GRADS = [(127, 9, 24, "zipf"), (128, 3, 40, "one"), (128, 500, 513, "holes"), (129, 3, 40, "one"), (256, 2, 516, "uniform"), (256, 90, 64, "zipf"), (257, 2, 516, "uniform"), (255, 1, 3, "one"), (160, 1, 12, "one"), (161, 300, 515, "holes"),
+         (4096, 30, 20, "zipf"), (16384, 2, 12, "uniform"), (16385, 9, 12, "zipf"), (65537, 5, 4, "zipf"), (32768, 3, 8, "one"), (32769, 3, 8, "one"), (32800, 100, 132, "zipf"), (50000, 2, 1, "uniform"),
+         (1, 1, 1, "one"), (2, 3, 5, "zipf"), (31, 1, 4, "one"), (32, 2, 4, "uniform"), (33, 1, 7, "one"), (64, 9, 16, "sorted"),
          (65, 200, 36, "holes"), (100, 40, 515, "zipf"), (1000, 10, 64, "zipf"), (1000, 5000, 1030, "uniform"), (300, 7, 4100, "zipf"),
          (4097, 100, 20, "one"), (8191, 1000, 8, "zipf"), (8192, 50, 12, "holes"), (8193, 1023, 12, "zipf"), (8193, 1024, 5, "holes"),
          (9000, 1, 33, "one"), (20000, 70000, 4, "zipf"), (30001, 3000, 40, "sorted"), (70000, 500, 3, "uniform"), (12345, 1 << 20, 4, "zipf"),

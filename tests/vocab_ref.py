@@ -25,14 +25,14 @@ def embed(table, tokens, scale):
 
 
 def embed_grad(tokens, dy, scale, vocab):
-    """The gradient, and what the sums of every row may be off: a value passes the additions of its piece of 32 places and those of
-    the pieces of its run, and the product with the scale rounds once more."""
+    """The gradient, and what the sums of every row may be off: a value passes the additions of its piece (8 to 64 places; 256 tokens
+    are one) and those of the pieces of its run, and the product with the scale rounds once more."""
     there = valid(tokens, vocab)
     want, size = np.zeros((vocab, dy.shape[1])), np.zeros((vocab, dy.shape[1]))
     np.add.at(want, tokens[there], dy[there].astype(np.float64))
     np.add.at(size, tokens[there], np.abs(dy[there].astype(np.float64)))
     run = np.bincount(tokens[there], minlength=vocab)
-    roundings = np.minimum(run, 32) + np.ceil(run / 32) + 2
+    roundings = np.minimum(run, 256) + np.ceil(run / 8) + 2
     return want * scale, 1.01 * U * roundings[:, None] * size * abs(scale) + 2.0 ** -149
 
 

@@ -16,7 +16,7 @@
 namespace {
 
 constexpr int kThreads = 256, kBlocks = 4;  // blocks of an SM
-constexpr int kHeld = 4;                    // 16-byte accesses of a thread on their way together
+constexpr int kHeld = 4, kAhead = 8;        // 16-byte accesses of a thread, and tokens of the history, on their way together
 constexpr unsigned kStep = 4 * kThreads, kMostSlice = 16 * kStep;
 
 struct Adjust {
@@ -24,7 +24,8 @@ struct Adjust {
     const int *history, *prompts, *lengths, *bias_tokens;
     const unsigned *allowed;
     float *out;
-    unsigned rows, vocab, history_cols, biases, words, slices, slice;  // slice: tokens of a block, a multiple of kStep
+    unsigned rows, vocab, history_cols, biases, words, slices;
+    unsigned slice, places, masks;  // tokens of a block, a multiple of kStep; words of its places and of its part of the mask
     int waves;
 };
 
@@ -67,7 +68,7 @@ struct Place {
 template <bool WIDE>
 __global__ void __launch_bounds__(kThreads, kBlocks) adjust_kernel(Adjust a) {
     using P = Place<WIDE>;
-    extern __shared__ __align__(16) unsigned seen[];  // behind the places the row's biases
+    extern __shared__ __align__(16) unsigned seen[];  // the places; the slice's words of the mask; the row's biases
     if (!a.waves) launch_next();
     launch_wait();
     const unsigned row = blockIdx.x / a.slices, slice = blockIdx.x % a.slices;
@@ -80,19 +81,29 @@ __global__ void __launch_bounds__(kThreads, kBlocks) adjust_kernel(Adjust a) {
     const unsigned lead = unsigned(reinterpret_cast<uintptr_t>(z) >> 2) & 3u, base = slice * a.slice - lead;
     const bool inside = base < a.vocab && a.vocab - base >= a.slice;  // (of all the slice's places)
     const bool whole = (unsigned(reinterpret_cast<uintptr_t>(out) >> 2) & 3u) == lead;
+    // ---- what does not wait for anything: the slice's words of the mask and the history's first tokens ----
+    unsigned *mask = seen + a.places;
+    const unsigned word0 = base < a.vocab ? base >> 5 : 0;
+    if (words)
+        for (unsigned i = threadIdx.x; i < a.slice / 32 + 2; i += kThreads) mask[i] = word0 + i < a.words ? words[word0 + i] : 0;
+    const int *history = a.history ? a.history + size_t(row) * a.history_cols : nullptr;
+    int first[kAhead];
+    if (history)
+#pragma unroll
+        for (int q = 0; q < kAhead; ++q) first[q] = threadIdx.x + q * kThreads < a.history_cols ? history[threadIdx.x + q * kThreads] : -1;
+    for (unsigned i = threadIdx.x; i < a.places / 4; i += kThreads) reinterpret_cast<uint4 *>(seen)[i] = make_uint4(0, 0, 0, 0);
+    if (words) __syncthreads();
     // which of an access's tokens are allowed: bit c of token + c
     auto allowed = [&](unsigned token) {
         unsigned bits = 15;
-        if (inside) {
-            if (words) {
-                const unsigned shift = token & 31, low = words[token >> 5], high = shift > 28 ? words[(token >> 5) + 1] : 0;
-                bits = __funnelshift_r(low, high, shift) & 15;
-            }
-        } else {
+        if (!inside) {
             bits = 0;
 #pragma unroll
             for (unsigned c = 0; c < 4; ++c)
-                if (token + c < a.vocab && (!words || (words[(token + c) >> 5] >> ((token + c) & 31) & 1u))) bits |= 1u << c;
+                if (token + c < a.vocab && (!words || (mask[((token + c) >> 5) - word0] >> ((token + c) & 31) & 1u))) bits |= 1u << c;
+        } else if (words) {
+            const unsigned *at = mask + ((token >> 5) - word0);
+            bits = __funnelshift_r(at[0], at[1], token & 31) & 15;
         }
         return bits;
     };
@@ -101,25 +112,20 @@ __global__ void __launch_bounds__(kThreads, kBlocks) adjust_kernel(Adjust a) {
         if (inside) return *reinterpret_cast<const float4 *>(z + token);
         return make_float4(bits & 1 ? z[token] : 0.f, bits & 2 ? z[token + 1] : 0.f, bits & 4 ? z[token + 2] : 0.f, bits & 8 ? z[token + 3] : 0.f);
     };
-    unsigned bits[kHeld];
     float4 v[kHeld];
+    unsigned bits[kHeld];
     auto ask = [&](unsigned from) {
 #pragma unroll
         for (int q = 0; q < kHeld; ++q) {
             const unsigned place = from + q * kStep;
             bits[q] = place < a.slice ? allowed(base + place) : 0;
+            if (!in_place) v[q] = fetch(base + place, bits[q]);
         }
-        if (!in_place)
-#pragma unroll
-            for (int q = 0; q < kHeld; ++q) v[q] = fetch(base + from + q * kStep, bits[q]);
     };
     ask(4 * threadIdx.x);
     // ---- the history's tokens and the biases of the slice ----
-    const unsigned words_of_slice = !a.history ? 0 : WIDE ? a.slice : a.slice / 2;
-    float *bias = reinterpret_cast<float *>(seen + words_of_slice), *bias_z = bias + a.biases;
+    float *bias = reinterpret_cast<float *>(mask + a.masks), *bias_z = bias + a.biases;
     int *bias_tokens = reinterpret_cast<int *>(bias_z + a.biases);
-    if (a.history)
-        for (unsigned i = threadIdx.x; i < words_of_slice / 4; i += kThreads) reinterpret_cast<uint4 *>(seen)[i] = make_uint4(0, 0, 0, 0);
     for (unsigned j = threadIdx.x; j < a.biases; j += kThreads) {
         const unsigned token = unsigned(a.bias_tokens[size_t(row) * a.biases + j]);
         const bool mine = token < a.vocab && token - base < a.slice;
@@ -128,36 +134,38 @@ __global__ void __launch_bounds__(kThreads, kBlocks) adjust_kernel(Adjust a) {
         bias_z[j] = mine ? z[token] : 0.f;
     }
     Penalties p = {1.f, 0.f, 0.f};
-    if (a.history) {
-        const int *history = a.history + size_t(row) * a.history_cols;
+    if (history) {
         const unsigned length = a.lengths ? unsigned(min(max(a.lengths[row], 0), int(a.history_cols))) : a.history_cols;
         const unsigned prompt = a.prompts ? unsigned(min(max(a.prompts[row], 0), int(length))) : 0;
         if (a.repetition) p.repetition = a.repetition[row];
         if (a.presence) p.presence = a.presence[row];
         if (a.frequency) p.frequency = a.frequency[row];
         __syncthreads();
-        for (unsigned i = threadIdx.x; i < length; i += 8 * kThreads) {
-            int token[8];
+        for (unsigned i = threadIdx.x; i < length; i += kAhead * kThreads) {
+            int token[kAhead];
 #pragma unroll
-            for (int q = 0; q < 8; ++q) token[q] = i + q * kThreads < length ? history[i + q * kThreads] : -1;
+            for (int q = 0; q < kAhead; ++q) {
+                const unsigned at = i + q * kThreads;
+                token[q] = at >= length ? -1 : i == threadIdx.x ? first[q] : history[at];
+            }
 #pragma unroll
-            for (int q = 0; q < 8; ++q)
+            for (int q = 0; q < kAhead; ++q)
                 if (unsigned(token[q]) < a.vocab && unsigned(token[q]) - base < a.slice) P::count(seen, unsigned(token[q]) - base, i + q * kThreads < prompt);
         }
     }
-    if (a.history || a.biases) __syncthreads();
+    if (history || a.biases) __syncthreads();
     // ---- the slice ----
     for (unsigned from = 4 * threadIdx.x;;) {
 #pragma unroll
         for (int q = 0; q < kHeld; ++q) {
-            const unsigned place = from + q * kStep, token = base + place;
+            const unsigned place = from + q * kStep, token = base + place, can = bits[q];
             if (place >= a.slice) continue;
             uint4 s = make_uint4(0, 0, 0, 0);
-            if (a.history) s = P::four(seen, place);
+            if (history) s = P::four(seen, place);
             const bool touched = (s.x | s.y | s.z | s.w) != 0;
             if (in_place) {
-                if (bits[q] == 15 && !touched) continue;
-                v[q] = fetch(token, bits[q]);
+                if (can == 15 && !touched) continue;
+                v[q] = fetch(token, can);
             }
             if (touched) {
                 v[q].x = P::penalised(v[q].x, s.x, p);
@@ -165,10 +173,10 @@ __global__ void __launch_bounds__(kThreads, kBlocks) adjust_kernel(Adjust a) {
                 v[q].z = P::penalised(v[q].z, s.z, p);
                 v[q].w = P::penalised(v[q].w, s.w, p);
             }
-            if (!(bits[q] & 1)) v[q].x = -INFINITY;
-            if (!(bits[q] & 2)) v[q].y = -INFINITY;
-            if (!(bits[q] & 4)) v[q].z = -INFINITY;
-            if (!(bits[q] & 8)) v[q].w = -INFINITY;
+            if (!(can & 1)) v[q].x = -INFINITY;
+            if (!(can & 2)) v[q].y = -INFINITY;
+            if (!(can & 4)) v[q].z = -INFINITY;
+            if (!(can & 8)) v[q].w = -INFINITY;
             if (inside && whole) {
                 *reinterpret_cast<float4 *>(out + token) = v[q];
             } else {
@@ -186,7 +194,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) adjust_kernel(Adjust a) {
     __syncthreads();
     for (unsigned j = threadIdx.x; j < a.biases; j += kThreads) {
         const int token = bias_tokens[j];
-        if (token < 0 || (words && !(words[token >> 5] >> (token & 31) & 1u))) continue;
+        if (token < 0 || (words && !(mask[(token >> 5) - word0] >> (token & 31) & 1u))) continue;
         bool first = true;
         float sum = 0.f;
         for (unsigned i = 0; i < a.biases; ++i) {
@@ -194,7 +202,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) adjust_kernel(Adjust a) {
             first = first && i >= j;
             sum += bias[i];
         }
-        if (first) out[token] = (a.history ? P::penalised(bias_z[j], P::one(seen, unsigned(token) - base), p) : bias_z[j]) + sum;
+        if (first) out[token] = (history ? P::penalised(bias_z[j], P::one(seen, unsigned(token) - base), p) : bias_z[j]) + sum;
     }
 }
 
@@ -204,7 +212,9 @@ int32_t launch(katsu_cuda_ctx *ctx, Adjust a) {
     const size_t places = size_t(a.vocab) + 3, resident = size_t(kBlocks) * ctx->num_sms, wanted = std::max<size_t>(1, resident / a.rows);
     a.slice = unsigned(std::min<size_t>(kMostSlice, katsu_div_up(katsu_div_up(places, wanted), kStep) * kStep));
     a.slices = unsigned(katsu_div_up(places, a.slice));
-    const size_t blocks = size_t(a.rows) * a.slices, smem = (a.history ? (WIDE ? 4 : 2) * size_t(a.slice) : 0) + 12 * size_t(a.biases);
+    a.places = !a.history ? 0 : WIDE ? a.slice : a.slice / 2;
+    a.masks = a.allowed ? a.slice / 32 + 2 : 0;
+    const size_t blocks = size_t(a.rows) * a.slices, smem = 4 * (size_t(a.places) + a.masks + 3 * size_t(a.biases));
     if (blocks > 0x7fffffffu) return katsu_set_error(KATSU_ERR_UNSUPPORTED, "%u rows of %u logits in one call", a.rows, a.vocab);
     KATSU_TRY(katsu_prepare_kernel(ctx, reinterpret_cast<const void *>(adjust_kernel<WIDE>), smem, false));
     a.waves = blocks > size_t(2) * ctx->num_sms;
@@ -237,7 +247,7 @@ extern "C" int32_t katsu_cuda_adjust_logits(katsu_cuda_ctx *ctx, const float *lo
     }
     KATSU_TRY(katsu_bind(ctx));
     const Adjust a = {logits, repetition, presence, frequency, bias, history_cols ? history : nullptr, prompts, lengths, bias_tokens, allowed, out,
-                      unsigned(rows), unsigned(vocab), unsigned(history_cols), unsigned(biases), unsigned(words), 0, 0, 0};
+                      unsigned(rows), unsigned(vocab), unsigned(history_cols), unsigned(biases), unsigned(words), 0, 0, 0, 0, 0};
     const bool wide = history_cols >= 1 << 15;
     return wide ? launch<true>(ctx, a) : launch<false>(ctx, a);
 }

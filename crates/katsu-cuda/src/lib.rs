@@ -522,6 +522,164 @@ pub fn int8_linear(ctx: &Context, x: &DeviceBuf, w: &Int8Weights, bias: Option<&
     })
 }
 
+/// Tokens (32-bit whole numbers) on the device; what is no token of a vocabulary, negative numbers for one, stands for none.
+pub struct TokenBuf {
+    words: DeviceBuf,
+}
+
+impl TokenBuf {
+    pub fn from_host(ctx: &Context, tokens: &[i32]) -> Result<Self, CudaError> {
+        let words = DeviceBuf::zeros(ctx, tokens.len())?;
+        // h2d copies 4-byte elements as they are; `tokens` may be dropped right away
+        check(unsafe { ffi::katsu_cuda_h2d(ctx.ptr(), words.ptr, tokens.as_ptr() as *const f32, tokens.len()) })?;
+        ctx.sync()?;
+        Ok(Self { words })
+    }
+    pub fn len(&self) -> usize {
+        self.words.len
+    }
+    pub fn is_empty(&self) -> bool {
+        self.words.len == 0
+    }
+    fn ptr(&self) -> *const i32 {
+        self.words.ptr as *const i32
+    }
+}
+
+fn opt_tokens(tokens: Option<&TokenBuf>) -> *const i32 {
+    tokens.map_or(ptr::null(), |t| t.ptr())
+}
+
+/// y[i] = scale * table[tokens[i]] for a table [vocab, cols].
+pub fn embed_forward(ctx: &Context, table: &DeviceBuf, tokens: &TokenBuf, scale: f32, y: &mut DeviceBuf, vocab: usize, cols: usize)
+                     -> Result<(), CudaError> {
+    length("table", table, vocab * cols)?;
+    length("y", y, tokens.len() * cols)?;
+    check(unsafe { ffi::katsu_cuda_embed_fwd(ctx.ptr(), table.ptr, tokens.ptr(), scale, y.ptr, tokens.len(), vocab, cols) })
+}
+
+/// dtable[v] (+)= scale * sum of dy[i] over the tokens that are v.
+pub fn embed_backward(ctx: &Context, tokens: &TokenBuf, dy: &DeviceBuf, scale: f32, dtable: &mut DeviceBuf, vocab: usize, cols: usize,
+                      accumulate: bool) -> Result<(), CudaError> {
+    length("dy", dy, tokens.len() * cols)?;
+    length("dtable", dtable, vocab * cols)?;
+    check(unsafe {
+        ffi::katsu_cuda_embed_bwd(ctx.ptr(), tokens.ptr(), dy.ptr, scale, dtable.ptr, tokens.len(), vocab, cols, accumulate as i32)
+    })
+}
+
+/// `embed_forward` from the 8-bit weights [k, n] of a head that are the table of its n tokens too: y is [tokens, k].
+pub fn int8_embed(ctx: &Context, w: &Int8Weights, tokens: &TokenBuf, scale: f32, y: &mut DeviceBuf) -> Result<(), CudaError> {
+    length("y", y, tokens.len() * w.k)?;
+    check(unsafe {
+        ffi::katsu_cuda_int8_embed(ctx.ptr(), w.q.ptr as *const i8, w.scale.ptr, tokens.ptr(), scale, y.ptr, tokens.len(), w.n, w.k)
+    })
+}
+
+/// Loss against a teacher's top logits (rows of `top`) and against labels, for every row of logits; see katsu_cuda_distill_fwd.
+#[derive(Clone, Copy)]
+pub struct Distill<'a> {
+    pub logits: &'a DeviceBuf,
+    /// Logits and their tokens.
+    pub teacher: Option<(&'a DeviceBuf, &'a TokenBuf)>,
+    pub labels: Option<&'a TokenBuf>,
+    pub weight: Option<&'a DeviceBuf>,
+    pub temperature: f32,
+    pub soft: f32,
+    pub hard: f32,
+    pub rows: usize,
+    pub vocab: usize,
+    pub top: usize,
+}
+
+impl Distill<'_> {
+    fn check(&self) -> Result<(), CudaError> {
+        length("logits", self.logits, self.rows * self.vocab)?;
+        if let Some((teacher, index)) = self.teacher {
+            length("teacher", teacher, self.rows * self.top)?;
+            length("index", &index.words, self.rows * self.top)?;
+        }
+        if let Some(labels) = self.labels {
+            length("labels", &labels.words, self.rows)?;
+        }
+        self.weight.map_or(Ok(()), |w| length("weight", w, self.rows))
+    }
+    fn top(&self) -> usize {
+        self.teacher.map_or(0, |_| self.top)
+    }
+}
+
+/// loss [rows].
+pub fn distill_forward(ctx: &Context, d: &Distill<'_>, loss: &mut DeviceBuf) -> Result<(), CudaError> {
+    d.check()?;
+    length("loss", loss, d.rows)?;
+    check(unsafe {
+        ffi::katsu_cuda_distill_fwd(ctx.ptr(), d.logits.ptr, opt_const(d.teacher.map(|t| t.0)), opt_tokens(d.teacher.map(|t| t.1)),
+                                    opt_tokens(d.labels), opt_const(d.weight), d.temperature, d.soft, d.hard, loss.ptr, d.rows, d.vocab, d.top())
+    })
+}
+
+/// dlogits (+)= gradient of the sum of grad * loss; `loss` is written too where it is given, from the same reading of the logits.
+pub fn distill_backward(ctx: &Context, d: &Distill<'_>, grad: Option<&DeviceBuf>, loss: Option<&mut DeviceBuf>, dlogits: &mut DeviceBuf,
+                        accumulate: bool) -> Result<(), CudaError> {
+    d.check()?;
+    for buf in [grad, loss.as_deref()].into_iter().flatten() {
+        length("grad or loss", buf, d.rows)?;
+    }
+    length("dlogits", dlogits, d.rows * d.vocab)?;
+    check(unsafe {
+        ffi::katsu_cuda_distill_bwd(ctx.ptr(), d.logits.ptr, opt_const(d.teacher.map(|t| t.0)), opt_tokens(d.teacher.map(|t| t.1)),
+                                    opt_tokens(d.labels), opt_const(d.weight), d.temperature, d.soft, d.hard, opt_const(grad), opt_mut(loss),
+                                    dlogits.ptr, d.rows, d.vocab, d.top(), accumulate as i32)
+    })
+}
+
+/// What `adjust_logits` does to every row of logits; `None` leaves a part out.
+#[derive(Clone, Copy, Default)]
+pub struct LogitAdjustments<'a> {
+    /// Tokens [rows, history_cols], and how many of a row's there are and are its prompt.
+    pub history: Option<&'a TokenBuf>,
+    pub lengths: Option<&'a TokenBuf>,
+    pub prompts: Option<&'a TokenBuf>,
+    pub repetition: Option<&'a DeviceBuf>,
+    pub presence: Option<&'a DeviceBuf>,
+    pub frequency: Option<&'a DeviceBuf>,
+    /// Tokens and values [rows, biases].
+    pub bias: Option<(&'a TokenBuf, &'a DeviceBuf)>,
+    /// Bits in words [rows, (vocab + 31) / 32].
+    pub allowed: Option<&'a TokenBuf>,
+}
+
+/// out = the logits [rows, vocab] behind penalties, biases and mask (katsu_cuda_adjust_logits).
+pub fn adjust_logits(ctx: &Context, logits: &DeviceBuf, a: &LogitAdjustments<'_>, out: &mut DeviceBuf, rows: usize, vocab: usize)
+                     -> Result<(), CudaError> {
+    length("logits", logits, rows * vocab)?;
+    length("out", out, rows * vocab)?;
+    for tokens in [a.lengths, a.prompts].into_iter().flatten() {
+        length("lengths or prompts", &tokens.words, rows)?;
+    }
+    for buf in [a.repetition, a.presence, a.frequency].into_iter().flatten() {
+        length("penalties", buf, rows)?;
+    }
+    let of_row = |len: usize| if rows == 0 { 0 } else { len / rows };
+    let (cols, biases) = (a.history.map_or(0, |h| of_row(h.len())), a.bias.map_or(0, |b| of_row(b.1.len())));
+    if let Some(h) = a.history {
+        length("history", &h.words, rows * cols)?;
+    }
+    if let Some((tokens, values)) = a.bias {
+        length("bias", values, rows * biases)?;
+        length("bias tokens", &tokens.words, rows * biases)?;
+    }
+    if let Some(words) = a.allowed {
+        length("allowed", &words.words, rows * ((vocab + 31) / 32))?;
+    }
+    check(unsafe {
+        ffi::katsu_cuda_adjust_logits(ctx.ptr(), logits.ptr, opt_tokens(a.history), opt_tokens(a.prompts), opt_tokens(a.lengths),
+                                      opt_const(a.repetition), opt_const(a.presence), opt_const(a.frequency), opt_tokens(a.bias.map(|b| b.0)),
+                                      opt_const(a.bias.map(|b| b.1)), opt_tokens(a.allowed) as *const u32, out.ptr, rows, vocab, cols, biases)
+    })
+}
+
 /// The norm over all gradients into a one-element buffer.
 pub fn grad_norm(ctx: &Context, grads: &[&DeviceBuf], norm: &mut DeviceBuf) -> Result<(), CudaError> {
     length("norm", norm, 1)?;

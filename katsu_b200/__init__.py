@@ -22,7 +22,7 @@ HOST_LIB_PATH = os.path.join(_PKG, "lib", "libkatsu_host.so")
 USIZE_MAX = (1 << 64) - 1
 
 __all__ = [
-    "Tensor", "Conv2D", "Norm", "BlockNorm", "Int8Linear", "grad_norm", "clip_grad_norm", "sgd_step_clipped", "Op", "TensorError", "ShapeOverflow", "InvalidConv", "MissingForward",
+    "Tensor", "Conv2D", "Norm", "BlockNorm", "Int8Linear", "Embedding", "DistillLoss", "adjust_logits", "grad_norm", "clip_grad_norm", "sgd_step_clipped", "Op", "TensorError", "ShapeOverflow", "InvalidConv", "MissingForward",
     "NonScalarBackward", "GradientBorrowed", "DataLength", "ShapeMismatch", "RankMismatch",
     "MatmulMismatch", "Allocation", "DeviceError", "InvalidOperand", "set_device", "set_precision", "synchronize",
     "set_loss_fusion", "loss_fusion",
@@ -107,7 +107,7 @@ class DeviceError(TensorError):
 
 
 class InvalidOperand(TensorError):
-    """An operand that a norm, the 8-bit product or clipping does not take (an addition, like these)."""
+    """An operand that a norm, the 8-bit product, clipping, a lookup, a loss or adjust_logits does not take (an addition, like these)."""
 
 
 _ERRORS = {1: ShapeOverflow, 2: InvalidConv, 3: MissingForward, 4: NonScalarBackward, 5: GradientBorrowed,
@@ -164,6 +164,12 @@ def _load():
             "kh_block_norm_new": [_vp, _vp, ctypes.c_float, ctypes.POINTER(_vp)],
             "kh_block_norm_forward": [_vp, _vp, _vp, _vp, ctypes.POINTER(_vp), ctypes.POINTER(_vp)],
             "kh_int8_from_weights": [_vp, _vp, ctypes.POINTER(_vp)], "kh_int8_forward": [_vp, _vp, ctypes.POINTER(_vp)],
+            "kh_embedding_new": [_vp, ctypes.c_float, ctypes.POINTER(_vp)],
+            "kh_embedding_forward": [_vp, _vp, _sz, _szp, _sz, ctypes.POINTER(_vp)],
+            "kh_int8_embed": [_vp, _vp, _sz, _szp, _sz, ctypes.c_float, ctypes.POINTER(_vp)],
+            "kh_distill_new": [ctypes.c_float] * 3 + [ctypes.POINTER(_vp)],
+            "kh_distill_forward": [_vp, _vp, _vp, _vp, _sz, _vp, _sz, _vp, ctypes.POINTER(_vp)],
+            "kh_adjust_logits": [_vp] + [_vp, _sz] * 9 + [ctypes.POINTER(_vp)],
             "kh_grad_norm": [ctypes.POINTER(_vp), _sz, ctypes.POINTER(_vp)],
             "kh_clip_grad_norm": [ctypes.POINTER(_vp), _sz, ctypes.c_float, ctypes.POINTER(_vp)],
             "kh_sgd_step_clipped": [ctypes.POINTER(_vp), _sz, ctypes.c_float, ctypes.c_float, ctypes.POINTER(_vp)],
@@ -182,6 +188,8 @@ def _load():
             ("kh_tensor_op_norm", [_vp] + [ctypes.POINTER(ctypes.c_float)] * 2 + [ctypes.POINTER(ctypes.c_int)] * 3, None),
             ("kh_norm_free", [_vp], None), ("kh_block_norm_free", [_vp], None), ("kh_int8_free", [_vp], None),
             ("kh_int8_features", [_vp, _szp, _szp], None),
+            ("kh_embedding_free", [_vp], None), ("kh_distill_free", [_vp], None),
+            ("kh_tensor_op_distill", [_vp] + [ctypes.POINTER(ctypes.c_float)] * 3, None),
         ]:
             fn = getattr(lib, name)
             fn.argtypes, fn.restype = argtypes, restype
@@ -238,18 +246,20 @@ def context() -> int:
 
 
 # ---------------------------------------------------------------------------
-# Op (tensor.rs:85-93, plus Reshape, Norm and BlockSum)
+# Op (tensor.rs:85-93, plus Reshape, Norm, BlockSum, Embed and Distill)
 # ---------------------------------------------------------------------------
 class Op:
-    _KINDS = ["Leaf", "Add", "Mul", "Matmul", "Conv2D", "Sum", "Reshape", "Norm", "BlockSum"]
+    _KINDS = ["Leaf", "Add", "Mul", "Matmul", "Conv2D", "Sum", "Reshape", "Norm", "BlockSum", "Embed", "Distill"]
 
     def __init__(self, kind, stride=None, padding=None, bias=False, relu=False, scale=None, eps=None, layer=False, gate=False,
-                 post=False):
+                 post=False, temperature=None, soft=None, hard=None):
         self.kind, self.stride, self.padding, self.bias, self.relu = kind, stride, padding, bias, relu
         self.scale, self.eps, self.layer, self.gate, self.post = scale, eps, layer, gate, post
+        self.temperature, self.soft, self.hard = temperature, soft, hard
 
     def _key(self):
-        return (self.kind, self.stride, self.padding, self.bias, self.relu, self.scale, self.eps, self.layer, self.gate, self.post)
+        return (self.kind, self.stride, self.padding, self.bias, self.relu, self.scale, self.eps, self.layer, self.gate, self.post,
+                self.temperature, self.soft, self.hard)
 
     def __eq__(self, other):
         return isinstance(other, Op) and self._key() == other._key()
@@ -265,6 +275,10 @@ class Op:
             flags = "".join(f", {name}" for name in ("layer", "gate", "post", "bias") if getattr(self, name))
             scale = f"scale: {self.scale}, " if self.kind == "BlockSum" else ""
             return f"{self.kind} {{ {scale}eps: {self.eps}{flags} }}"
+        if self.kind == "Embed":
+            return f"Embed {{ scale: {self.scale} }}"
+        if self.kind == "Distill":
+            return f"Distill {{ temperature: {self.temperature}, soft: {self.soft}, hard: {self.hard} }}"
         return self.kind
 
     @staticmethod
@@ -360,6 +374,14 @@ class Tensor:
         kind, stride, padding = ctypes.c_int(), _sz(), _sz()
         _lib.kh_tensor_op(self._h, ctypes.byref(kind), ctypes.byref(stride), ctypes.byref(padding))
         name = Op._KINDS[kind.value]
+        if name == "Embed":
+            scale, eps, flags = ctypes.c_float(), ctypes.c_float(), [ctypes.c_int() for _ in range(3)]
+            _lib.kh_tensor_op_norm(self._h, *(ctypes.byref(v) for v in (scale, eps, *flags)))
+            return Op(name, scale=scale.value)
+        if name == "Distill":
+            t, soft, hard = (ctypes.c_float() for _ in range(3))
+            _lib.kh_tensor_op_distill(self._h, *(ctypes.byref(v) for v in (t, soft, hard)))
+            return Op(name, temperature=t.value, soft=soft.value, hard=hard.value)
         if name not in ("Conv2D", "Norm", "BlockSum"):
             return Op(name)
         bias, relu = ctypes.c_int(), ctypes.c_int()
@@ -618,6 +640,113 @@ class Int8Linear:
         out = _vp()
         _check(_lib.kh_int8_forward(self._h, x._h, ctypes.byref(out)))
         return Tensor._wrap(out.value)
+
+    def embed(self, tokens, scale=1.0):
+        """scale * weights[:, token] for every token, from the same 8 bits: the lookup of a model whose head's weights are its
+        tokens' table too.  A leaf [..., in_features]; a negative token is none."""
+        out, (data, count, dims, rank, _keep) = _vp(), _token_args(tokens)
+        _check(_lib.kh_int8_embed(self._h, data, count, dims, rank, float(scale), ctypes.byref(out)))
+        return Tensor._wrap(out.value)
+
+
+# ---------------------------------------------------------------------------
+# Additions: the two ends of a language model
+# ---------------------------------------------------------------------------
+def _whole(values, what):
+    """Whole numbers as a contiguous int32 array; what does not fit 32 bits is no token either way."""
+    array = np.asarray(values)
+    if array.size == 0:
+        return np.zeros(array.shape, np.int32)
+    if array.dtype.kind not in "iub":
+        raise InvalidOperand(f"invalid operand: {what} must be whole numbers, got {array.dtype}")
+    if array.dtype.kind == "u":
+        array = np.minimum(array, np.uint64(2 ** 31 - 1))
+    return np.array(np.clip(array.astype(np.int64), -(2 ** 31), 2 ** 31 - 1), dtype=np.int32, order="C").reshape(array.shape)
+
+
+def _token_args(tokens):
+    array = _whole(tokens, "tokens")
+    dims, rank = _shape_args(array.shape)
+    return array.ctypes.data, array.size, dims, rank, array
+
+
+class Embedding:
+    """scale * table[token] for tokens of any shape, and the gradient of the table [vocab, cols].  A negative token (padding) is a
+    row of zeros without a gradient."""
+
+    def __init__(self, table, scale=1.0):
+        out = _vp()
+        _check(_load().kh_embedding_new(table._h, float(scale), ctypes.byref(out)))
+        self._h = out.value
+
+    def __del__(self):
+        h = getattr(self, "_h", None)
+        if h and _lib is not None:
+            _lib.kh_embedding_free(h)
+            self._h = None
+
+    def forward(self, tokens):
+        """[..., cols] for whole numbers [...]."""
+        out, (data, count, dims, rank, _keep) = _vp(), _token_args(tokens)
+        _check(_lib.kh_embedding_forward(self._h, data, count, dims, rank, ctypes.byref(out)))
+        return Tensor._wrap(out.value)
+
+
+class DistillLoss:
+    """The loss of every row of logits [..., vocab]: weight * (soft T^2 KL(p, q) + hard * cross entropy of the label), p the teacher's
+    softmax(t / T) over its listed entries and q = softmax(logits / T) over the vocabulary."""
+
+    def __init__(self, temperature=1.0, soft=1.0, hard=0.0):
+        out = _vp()
+        _check(_load().kh_distill_new(float(temperature), float(soft), float(hard), ctypes.byref(out)))
+        self._h = out.value
+
+    def __del__(self):
+        h = getattr(self, "_h", None)
+        if h and _lib is not None:
+            _lib.kh_distill_free(h)
+            self._h = None
+
+    def forward(self, logits, teacher=None, index=None, labels=None, weight=None):
+        """A Tensor [...].  teacher: a Tensor [..., top] of logits, index: their tokens (negative: left out); labels: a token for
+        every row (negative: none); weight: a Tensor with a value for every row.  The gradient reaches the logits alone."""
+        out = _vp()
+        indices, labels = _whole([] if index is None else index, "index"), _whole([] if labels is None else labels, "labels")
+        _check(_lib.kh_distill_forward(self._h, logits._h, teacher._h if teacher is not None else None, indices.ctypes.data, indices.size,
+                                       labels.ctypes.data, labels.size, weight._h if weight is not None else None, ctypes.byref(out)))
+        return Tensor._wrap(out.value)
+
+
+def adjust_logits(logits, history=None, lengths=None, prompts=None, repetition=None, presence=None, frequency=None, bias_tokens=None,
+                  bias=None, allowed=None):
+    """Logits [rows, vocab] (or [vocab]) as a server changes them before it picks a token, as a new leaf.
+
+    history [rows, n]: tokens, of which lengths [rows] are a row's (all) and the first prompts [rows] of these its prompt (none);
+    repetition divides positive and multiplies other logits of its tokens, frequency * count + presence is taken off those of
+    generated ones (numbers, or one for every row); bias_tokens and bias [rows, n]: values to be added; allowed [rows, vocab]:
+    where it is not true the logit becomes -infinity, whatever it was."""
+    lib, out, shape = _load(), _vp(), logits.shape()
+    rows = 1 if len(shape) == 1 else shape[0] if shape else 0
+
+    def per_row(v):
+        return np.zeros(0, np.float32) if v is None else np.ascontiguousarray(np.full(rows, v) if np.ndim(v) == 0 else v, dtype=np.float32).reshape(-1)
+
+    none = np.zeros(0, np.int32)
+    words = none
+    if allowed is not None:
+        allowed = np.asarray(allowed, dtype=bool)
+        if list(allowed.shape) != shape:
+            raise InvalidOperand("invalid operand: allowed must have the logits' shape")
+        allowed = allowed.reshape(rows, -1)
+        bits = np.zeros((rows, (allowed.shape[1] + 31) // 32 * 32), bool)
+        bits[:, : allowed.shape[1]] = allowed
+        words = np.ascontiguousarray(np.packbits(bits, axis=1, bitorder="little")).view("<u4")
+    arrays = [none if history is None else _whole(history, "history"), none if prompts is None else _whole(prompts, "prompts"),
+              none if lengths is None else _whole(lengths, "lengths"), per_row(repetition), per_row(presence), per_row(frequency),
+              none if bias_tokens is None else _whole(bias_tokens, "bias_tokens"),
+              np.zeros(0, np.float32) if bias is None else np.ascontiguousarray(bias, dtype=np.float32).reshape(-1), words]
+    _check(lib.kh_adjust_logits(logits._h, *(x for a in arrays for x in (a.ctypes.data, a.size)), ctypes.byref(out)))
+    return Tensor._wrap(out.value)
 
 
 def _handles(tensors):

@@ -12,6 +12,8 @@
 
 using katsu::BlockNorm;
 using katsu::Conv2D;
+using katsu::DistillLoss;
+using katsu::Embedding;
 using katsu::Int8Linear;
 using katsu::Norm;
 using katsu::Tensor;
@@ -50,6 +52,10 @@ int guarded(F &&body) {
     }
 }
 
+template <typename V>
+std::vector<V> values(const V *data, size_t count) {
+    return count ? std::vector<V>(data, data + count) : std::vector<V>();
+}
 std::vector<size_t> shape_vec(const size_t *shape, size_t rank) { return std::vector<size_t>(shape, shape + rank); }
 
 Tensor &T(void *h) { return *static_cast<Tensor *>(h); }
@@ -306,6 +312,48 @@ int kh_int8_forward(void *h, void *x, void **out) {
 void kh_int8_features(void *h, size_t *in, size_t *out) {
     *in = static_cast<Int8Linear *>(h)->in_features();
     *out = static_cast<Int8Linear *>(h)->out_features();
+}
+
+// ---- the two ends of a language model ---------------------------------------------
+int kh_embedding_new(void *table, float scale, void **out) {
+    return guarded([&] { *out = new Embedding(T(table), scale); });
+}
+void kh_embedding_free(void *h) { delete static_cast<Embedding *>(h); }
+int kh_embedding_forward(void *h, const int32_t *tokens, size_t count, const size_t *shape, size_t rank, void **out) {
+    return guarded([&] { *out = box(static_cast<Embedding *>(h)->forward(values(tokens, count), shape_vec(shape, rank))); });
+}
+int kh_int8_embed(void *h, const int32_t *tokens, size_t count, const size_t *shape, size_t rank, float scale, void **out) {
+    return guarded([&] { *out = box(static_cast<Int8Linear *>(h)->embed(values(tokens, count), shape_vec(shape, rank), scale)); });
+}
+int kh_distill_new(float temperature, float soft, float hard, void **out) {
+    return guarded([&] { *out = new DistillLoss(temperature, soft, hard); });
+}
+void kh_distill_free(void *h) { delete static_cast<DistillLoss *>(h); }
+// teacher, labels and weight may be NULL.
+int kh_distill_forward(void *h, void *logits, void *teacher, const int32_t *index, size_t indices, const int32_t *labels, size_t label_count,
+                       void *weight, void **out) {
+    return guarded([&] {
+        *out = box(static_cast<DistillLoss *>(h)->forward(T(logits), optional_tensor(teacher), values(index, indices), values(labels, label_count),
+                                                          optional_tensor(weight)));
+    });
+}
+// Every array may be NULL with a count of 0.
+int kh_adjust_logits(void *logits, const int32_t *history, size_t tokens, const int32_t *prompts, size_t prompt_count, const int32_t *lengths,
+                     size_t length_count, const float *repetition, size_t repetitions, const float *presence, size_t presences,
+                     const float *frequency, size_t frequencies, const int32_t *bias_tokens, size_t bias_token_count, const float *bias,
+                     size_t biases, const uint32_t *allowed, size_t words, void **out) {
+    return guarded([&] {
+        const katsu::LogitAdjustments a = {values(history, tokens),         values(prompts, prompt_count),   values(lengths, length_count),
+                                           values(repetition, repetitions), values(presence, presences),     values(frequency, frequencies),
+                                           values(bias_tokens, bias_token_count), values(bias, biases),      values(allowed, words)};
+        *out = box(katsu::adjust_logits(T(logits), a));
+    });
+}
+void kh_tensor_op_distill(void *h, float *temperature, float *soft, float *hard) {
+    const katsu::Op op = T(h).op();
+    *temperature = op.temperature;
+    *soft = op.soft;
+    *hard = op.hard;
 }
 
 // ---- all gradients of a step ----------------------------------------------------

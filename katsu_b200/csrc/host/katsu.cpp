@@ -195,6 +195,7 @@ struct TensorNode {
     // values are parents[0] * parents[0], not computed yet (set by Tensor::mul when fusion is on)
     mutable bool lazy_square = false;
     mutable std::vector<std::weak_ptr<TensorNode>> squares;  // DeviceBuffer::squares until there is a buffer
+    std::vector<std::shared_ptr<DeviceBuffer>> kept;  // what Embed and Distill read again in their backward
     mutable std::shared_ptr<DeviceBuffer> grad_dev;  // null == None (unless grad_sym holds it)
     mutable std::shared_ptr<Adjoint> grad_sym;       // a gradient still in symbolic form
     mutable std::vector<float> grad_host;
@@ -510,6 +511,10 @@ std::shared_ptr<DeviceBuffer> device_one() {
     return *one;
 }
 
+// Buffers of an operator's other operands; null where there is none.
+const float *floats_of(const std::shared_ptr<DeviceBuffer> &buffer) { return buffer ? buffer->ptr : nullptr; }
+const int32_t *ints_of(const std::shared_ptr<DeviceBuffer> &buffer) { return reinterpret_cast<const int32_t *>(floats_of(buffer)); }
+
 // Rows and columns of a norm's values: the last axis is normalised.
 size_t last_axis(const std::vector<size_t> &shape) { return shape.back(); }
 size_t rows_of(const Tensor &t) { return t.numel() ? t.numel() / last_axis(t.shape()) : 0; }
@@ -756,6 +761,31 @@ void op_backward(const Tensor &node, Adjoint &own, Pending &pending, Touched &to
             own.tail = Tensor();
             own.tail_grad.reset();
             block_backward(node, &node, tail.defined() ? &tail : nullptr, dr, dn ? dn->ptr : nullptr, own, pending, touched);
+            return;
+        }
+        case Op::Embed: {
+            const Tensor &table = parents[0];
+            const size_t cols = table.shape()[1];
+            const int add = touched.count(table.id()) ? 1 : 0;
+            Adjoint &target = pending.at(table.id());
+            float *to = add ? target.to_add() : target.to_overwrite();
+            check(katsu_cuda_embed_bwd(ctx, ints_of(node.node()->kept[0]), own.to_dense(), op.scale, to, cols ? node.numel() / cols : 0,
+                                       table.shape()[0], cols, add));
+            touched.insert(table.id());
+            return;
+        }
+        case Op::Distill: {
+            const Tensor &logits = parents[0];
+            if (logits.numel() == 0) return;
+            const auto &kept = node.node()->kept;  // teacher, index, labels, weight
+            const size_t vocab = last_axis(logits.shape()), rows = rows_of(logits);
+            const int add = touched.count(logits.id()) ? 1 : 0;
+            Adjoint &target = pending.at(logits.id());
+            float *to = add ? target.to_add() : target.to_overwrite();
+            check(katsu_cuda_distill_bwd(ctx, logits.device_data(), floats_of(kept[0]), ints_of(kept[1]), ints_of(kept[2]), floats_of(kept[3]),
+                                         op.temperature, op.soft, op.hard, own.to_dense(), nullptr, to, rows, vocab,
+                                         kept[0] ? kept[0]->count / rows : 0, add));
+            touched.insert(logits.id());
             return;
         }
         case Op::Matmul: {
@@ -1129,6 +1159,147 @@ Tensor Int8Linear::forward(const Tensor &x) const {
         check(katsu_cuda_int8_linear(device_context(), x.device_data(), reinterpret_cast<const int8_t *>(q_->ptr), scale_->ptr,
                                      bias_ ? bias_->ptr : nullptr, out->ptr, m, k_, n_));
     return Tensor::make_node(std::move(out), {m, n_}, Op{}, {});
+}
+
+// ---------------------------------------------------------------------------
+// the two ends of a language model
+// ---------------------------------------------------------------------------
+namespace {
+
+static_assert(sizeof(float) == sizeof(int32_t), "buffers of tokens are allocated as floats");
+
+// Host values in device memory; null where there are none.
+template <typename T>
+std::shared_ptr<DeviceBuffer> uploaded(const std::vector<T> &values) {
+    if (values.empty()) return nullptr;
+    auto buffer = uninit_buffer(values.size());
+    // (from pageable memory: the call returns once the values have been staged)
+    check(katsu_cuda_h2d(device_context(), buffer->ptr, reinterpret_cast<const float *>(values.data()), values.size()));
+    return buffer;
+}
+
+void check_tokens(const std::vector<int32_t> &tokens, size_t vocab, const char *what) {
+    for (const int32_t token : tokens)
+        if (token >= 0 && static_cast<size_t>(token) >= vocab)
+            fail(ErrorKind::InvalidOperand, std::string(what) + " " + std::to_string(token) + " of a vocabulary of " + std::to_string(vocab));
+}
+
+std::vector<size_t> with_axis(std::vector<size_t> shape, size_t cols) {
+    shape.push_back(cols);
+    return shape;
+}
+
+}  // namespace
+
+Embedding::Embedding(Tensor table, float scale) : table_(std::move(table)), scale_(scale) {
+    if (table_.rank() != 2) fail(ErrorKind::RankMismatch, "", 2, table_.rank());
+}
+
+Tensor Embedding::forward(const std::vector<int32_t> &tokens, const std::vector<size_t> &shape) const {
+    const size_t count = element_count(shape), vocab = table_.shape()[0], cols = table_.shape()[1];
+    if (tokens.size() != count) fail(ErrorKind::DataLength, "", count, tokens.size());
+    check_tokens(tokens, vocab, "token");
+    auto out = uninit_buffer(element_count(with_axis(shape, cols)));
+    auto on_device = uploaded(tokens);
+    if (out->count)
+        check(katsu_cuda_embed_fwd(device_context(), table_.device_data(), ints_of(on_device), scale_, out->ptr, count, vocab, cols));
+    Op op;
+    op.kind = Op::Embed;
+    op.scale = scale_;
+    Tensor node = Tensor::make_node(std::move(out), with_axis(shape, cols), op, {table_});
+    node.node()->kept = {std::move(on_device)};
+    return node;
+}
+
+Tensor Int8Linear::embed(const std::vector<int32_t> &tokens, const std::vector<size_t> &shape, float scale) const {
+    const size_t count = element_count(shape);
+    if (tokens.size() != count) fail(ErrorKind::DataLength, "", count, tokens.size());
+    check_tokens(tokens, n_, "token");
+    auto out = uninit_buffer(element_count(with_axis(shape, k_)));
+    const auto on_device = uploaded(tokens);
+    if (out->count)
+        check(katsu_cuda_int8_embed(device_context(), reinterpret_cast<const int8_t *>(q_->ptr), scale_->ptr, ints_of(on_device), scale,
+                                    out->ptr, count, n_, k_));
+    return Tensor::make_node(std::move(out), with_axis(shape, k_), Op{}, {});
+}
+
+DistillLoss::DistillLoss(float temperature, float soft, float hard) : temperature_(temperature), soft_(soft), hard_(hard) {
+    if (!(temperature > 0.f) || std::isinf(temperature)) fail(ErrorKind::InvalidOperand, "temperature must be above 0, and finite");
+    if (!std::isfinite(soft) || !std::isfinite(hard)) fail(ErrorKind::InvalidOperand, "soft and hard must be finite");
+}
+
+Tensor DistillLoss::forward(const Tensor &logits, const Tensor &teacher, const std::vector<int32_t> &index, const std::vector<int32_t> &labels,
+                            const Tensor &weight) const {
+    if (logits.rank() == 0 || logits.shape().back() == 0) fail(ErrorKind::InvalidOperand, "a loss needs logits with a last axis of at least one value");
+    const size_t vocab = logits.shape().back(), rows = logits.numel() / vocab;
+    const std::vector<size_t> shape(logits.shape().begin(), logits.shape().end() - 1);
+    size_t top = 0;
+    if (teacher.defined()) {
+        if (teacher.rank() != logits.rank() || !std::equal(shape.begin(), shape.end(), teacher.shape().begin()))
+            fail(ErrorKind::InvalidOperand, "a teacher's axes must be those of the logits, but for the last");
+        top = teacher.shape().back();
+        if (top > KATSU_DISTILL_MAX_TOP) fail(ErrorKind::InvalidOperand, "a teacher has at most " + std::to_string(KATSU_DISTILL_MAX_TOP) + " entries a row");
+    }
+    if (index.size() != rows * top) fail(ErrorKind::DataLength, "", rows * top, index.size());
+    if (!labels.empty() && labels.size() != rows) fail(ErrorKind::DataLength, "", rows, labels.size());
+    if (weight.defined() && weight.numel() != rows) fail(ErrorKind::DataLength, "", rows, weight.numel());
+    check_tokens(index, vocab, "index");
+    check_tokens(labels, vocab, "label");
+    auto loss = uninit_buffer(rows);
+    std::vector<std::shared_ptr<DeviceBuffer>> kept(4);
+    if (rows && top) {
+        teacher.device_data();
+        kept[0] = teacher.node()->dev;
+        kept[1] = uploaded(index);
+    }
+    kept[2] = uploaded(labels);
+    if (rows && weight.defined()) {
+        weight.device_data();
+        kept[3] = weight.node()->dev;
+    }
+    if (rows)
+        check(katsu_cuda_distill_fwd(device_context(), logits.device_data(), floats_of(kept[0]), ints_of(kept[1]), ints_of(kept[2]),
+                                     floats_of(kept[3]), temperature_, soft_, hard_, loss->ptr, rows, vocab, top));
+    Op op;
+    op.kind = Op::Distill;
+    op.temperature = temperature_;
+    op.soft = soft_;
+    op.hard = hard_;
+    Tensor node = Tensor::make_node(std::move(loss), shape, op, {logits});
+    node.node()->kept = std::move(kept);
+    return node;
+}
+
+Tensor adjust_logits(const Tensor &logits, const LogitAdjustments &a) {
+    if (logits.rank() != 1 && logits.rank() != 2) fail(ErrorKind::RankMismatch, "", logits.rank(), 2);
+    const size_t vocab = logits.shape().back(), rows = logits.rank() == 1 ? 1 : logits.shape()[0];
+    auto per_row = [&](size_t size, const char *what) {
+        if (size != 0 && size != rows) fail(ErrorKind::InvalidOperand, std::string(what) + " must have one value for every row of logits");
+    };
+    auto row_length = [&](size_t size, const char *what) {
+        if (rows == 0 ? size != 0 : size % rows != 0) fail(ErrorKind::InvalidOperand, std::string(what) + " must have rows of one length for every row of logits");
+        return rows ? size / rows : 0;
+    };
+    const size_t cols = row_length(a.history.size(), "history"), biases = row_length(a.bias.size(), "bias");
+    per_row(a.prompts.size(), "prompts");
+    per_row(a.lengths.size(), "lengths");
+    per_row(a.repetition.size(), "repetition");
+    per_row(a.presence.size(), "presence");
+    per_row(a.frequency.size(), "frequency");
+    if (a.bias_tokens.size() != a.bias.size()) fail(ErrorKind::DataLength, "", a.bias.size(), a.bias_tokens.size());
+    if (biases > KATSU_LOGITS_MAX_BIASES) fail(ErrorKind::InvalidOperand, "at most " + std::to_string(KATSU_LOGITS_MAX_BIASES) + " biases a row");
+    if (!a.allowed.empty() && a.allowed.size() != rows * ((vocab + 31) / 32)) fail(ErrorKind::DataLength, "", rows * ((vocab + 31) / 32), a.allowed.size());
+    check_tokens(a.history, vocab, "token");
+    check_tokens(a.bias_tokens, vocab, "token");
+    auto out = uninit_buffer(logits.numel());
+    const auto history = uploaded(a.history), prompts = uploaded(a.prompts), lengths = uploaded(a.lengths), repetition = uploaded(a.repetition),
+               presence = uploaded(a.presence), frequency = uploaded(a.frequency), bias_tokens = uploaded(a.bias_tokens), bias = uploaded(a.bias),
+               allowed = uploaded(a.allowed);
+    if (out->count)
+        check(katsu_cuda_adjust_logits(device_context(), logits.device_data(), ints_of(history), ints_of(prompts), ints_of(lengths),
+                                       floats_of(repetition), floats_of(presence), floats_of(frequency), ints_of(bias_tokens), floats_of(bias),
+                                       reinterpret_cast<const uint32_t *>(floats_of(allowed)), out->ptr, rows, vocab, cols, biases));
+    return Tensor::make_node(std::move(out), logits.shape(), Op{}, {});
 }
 
 // ---------------------------------------------------------------------------

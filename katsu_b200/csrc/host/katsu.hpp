@@ -40,7 +40,7 @@ enum class ErrorKind : int {
     MatmulMismatch,
     Allocation,
     Device,  // addition: a CUDA / library failure (no counterpart in the CPU-only reference)
-    InvalidOperand,  // addition: an operand that a norm, the 8-bit product or clipping does not take
+    InvalidOperand,  // addition: an operand that an operator of a language model (Norm and those below it) does not take
 };
 
 // tensor.rs:9-82.  `a` and `b` carry the two numbers of DataLength
@@ -53,9 +53,10 @@ struct TensorError {
     std::string to_string() const;  // the reference's Display text
 };
 
-// tensor.rs:85-93 plus Reshape (the reference has no view op), Norm and BlockSum (class Norm, class BlockNorm).
+// tensor.rs:85-93 plus Reshape (the reference has no view op), Norm and BlockSum (class Norm, class BlockNorm), Embed and Distill
+// (class Embedding, class DistillLoss).
 struct Op {
-    enum Kind : int { Leaf = 0, Add, Mul, Matmul, Conv2D, Sum, Reshape, Norm, BlockSum };
+    enum Kind : int { Leaf = 0, Add, Mul, Matmul, Conv2D, Sum, Reshape, Norm, BlockSum, Embed, Distill };
     Kind kind = Leaf;
     size_t stride = 0, padding = 0;  // Conv2D only
     // Conv2D only, additions (docs/roadmap.md:18-26 names bias and ReLU as the next layer features):
@@ -65,9 +66,12 @@ struct Op {
     // weight of the norm behind the block and, with `bias`, its bias).
     float scale = 1.f, eps = 0.f;
     bool layer = false, gate = false, post = false;
+    // Embed (parent: the table; scale above) and Distill (parent: the logits).
+    float temperature = 1.f, soft = 0.f, hard = 0.f;
     bool operator==(const Op &o) const {
         return kind == o.kind && stride == o.stride && padding == o.padding && bias == o.bias && relu == o.relu &&
-               scale == o.scale && eps == o.eps && layer == o.layer && gate == o.gate && post == o.post;
+               scale == o.scale && eps == o.eps && layer == o.layer && gate == o.gate && post == o.post &&
+               temperature == o.temperature && soft == o.soft && hard == o.hard;
     }
 };
 
@@ -260,6 +264,9 @@ class Int8Linear {
    public:
     static Int8Linear from_weights(const Tensor &weights, const Tensor &bias);
     Tensor forward(const Tensor &x) const;
+    // Rows of the weights' transpose for tokens (Embedding::forward): scale * w[:, token] of a head whose weights are the table of the
+    // model's tokens too, from the same 8 bits (katsu_cuda_int8_embed).  A leaf.
+    Tensor embed(const std::vector<int32_t> &tokens, const std::vector<size_t> &shape, float scale) const;
     size_t in_features() const { return k_; }
     size_t out_features() const { return n_; }
 
@@ -267,6 +274,52 @@ class Int8Linear {
     size_t k_ = 0, n_ = 0;
     std::shared_ptr<DeviceBuffer> q_, scale_, bias_;  // bias_ null: none
 };
+
+// The two ends of a language model.
+//
+// scale * table[token] for tokens of any shape, and the gradient of the table [vocab, cols] (katsu_cuda_embed_fwd, _bwd).
+class Embedding {
+   public:
+    Embedding(Tensor table, float scale);
+    const Tensor &table() const { return table_; }
+    float scale() const { return scale_; }
+    // [shape..., cols]; a negative token is none: a row of zeros without a gradient.
+    Tensor forward(const std::vector<int32_t> &tokens, const std::vector<size_t> &shape) const;
+
+   private:
+    Tensor table_;
+    float scale_;
+};
+
+// The loss of every row of logits [..., vocab] against a teacher's top logits and against labels (katsu_cuda_distill_fwd, _bwd):
+// weight * (soft T^2 KL(softmax(teacher / T) over its entries, softmax(logits / T)) + hard * cross entropy of the label).
+class DistillLoss {
+   public:
+    DistillLoss(float temperature, float soft, float hard);
+    float temperature() const { return temperature_; }
+    float soft() const { return soft_; }
+    float hard() const { return hard_; }
+    // teacher: undefined, or [..., top] with a token of `index` for every entry (negative: the entry is left out).  labels: empty, or one
+    // for every row (negative: none).  weight: undefined (1), or one for every row.  The result is [...]; a gradient reaches the logits
+    // alone.
+    Tensor forward(const Tensor &logits, const Tensor &teacher, const std::vector<int32_t> &index, const std::vector<int32_t> &labels,
+                   const Tensor &weight) const;
+
+   private:
+    float temperature_, soft_, hard_;
+};
+
+// What katsu_cuda_adjust_logits does to logits [rows, vocab] (or [vocab]) of a served model.  Empty vectors leave a part out; the others
+// have a value for every row, `history` and the biases a row of one length for every row, `allowed` (vocab + 31) / 32 words.
+struct LogitAdjustments {
+    std::vector<int32_t> history, prompts, lengths;  // tokens; negative ones are none
+    std::vector<float> repetition, presence, frequency;
+    std::vector<int32_t> bias_tokens;
+    std::vector<float> bias;
+    std::vector<uint32_t> allowed;
+};
+// A leaf of the logits' shape; the logits stay as they are.
+Tensor adjust_logits(const Tensor &logits, const LogitAdjustments &adjustments);
 
 // The norm over the gradients of all `tensors`, each listed once, as a leaf of one element; clipping them to max_norm in place;
 // and the SGD step with clipped gradients, which stay as they are (katsu_cuda_grad_norm, _clip_grads, _sgd_step_clipped).

@@ -318,8 +318,8 @@ int32_t katsu_cuda_distill_fwd(katsu_cuda_ctx *ctx, const float *logits, const f
                                const int32_t *labels, const float *weight, float temperature, float soft, float hard,
                                float *loss, size_t rows, size_t vocab, size_t top);
 /* dlogits = g[row] * weight * (soft T (q - p) + hard (softmax(z) - [v == label])): the gradient of sum_row g * loss.
- * g [rows] may be null (1).  loss [rows] may be null; otherwise it receives the loss as well, so that a training step
- * reads the logits once for both.  dlogits may be `logits` itself; accumulate != 0 adds to dlogits (then not `logits`). */
+ * g [rows] may be null (1).  loss [rows] may be null; otherwise it receives the loss as well (of long rows to the roundings
+ * of another order of sums than the call above takes), so that a training step reads the logits once for both.  dlogits may be `logits` itself; accumulate != 0 adds to dlogits (then not `logits`). */
 int32_t katsu_cuda_distill_bwd(katsu_cuda_ctx *ctx, const float *logits, const float *teacher, const int32_t *index,
                                const int32_t *labels, const float *weight, float temperature, float soft, float hard,
                                const float *g, float *loss, float *dlogits, size_t rows, size_t vocab, size_t top,

@@ -56,8 +56,8 @@ def check(ctx, a, T=1.0, soft=1.0, hard=0.0, labels=True, weight=True, g=True, *
                                       T, soft, hard, a["g"] if g else None)
     fwd, bwd, got = run(ctx, a, T, soft, hard, labels=labels, weight=weight, g=g, **more)
     ref.assert_near(fwd, want, off, "loss")
-    if more.get("loss", True):
-        assert np.array_equal(fwd, bwd, equal_nan=True)
+    if more.get("loss", True):  # (the two calls cut long rows into different parts: their sums agree to roundings, not bit for bit)
+        ref.assert_near(bwd, want, off, "loss beside the gradient")
     if more.get("accumulate") is not None:
         before = more["accumulate"].astype(np.float64)
         # added to twice at listed tokens: the row's part, then the list's

@@ -305,7 +305,7 @@ int32_t katsu_cuda_embed_bwd(katsu_cuda_ctx *ctx, const int32_t *tokens, const f
                              size_t count, size_t vocab, size_t cols, int32_t accumulate);
 
 /* Loss of logits z [rows, vocab] against a teacher's top logits and against labels, for every row:
- *     p = softmax(teacher / T) over the row's `top` entries, q = softmax(z / T) over the vocabulary (T = temperature)
+ *     p = softmax(teacher / T) over the row's `top` entries, q = softmax(z / T) over the vocabulary (T = temperature, a normal number)
  *     loss = weight * (soft T^2 sum_j p_j (log p_j - log q[index_j]) - hard log softmax(z)[label])
  * teacher and index are [rows, top], top at most KATSU_DISTILL_MAX_TOP.  Entries whose index is no token are left out,
  * and a token that is listed twice has both probabilities.  Without an entry that counts (none listed, all teacher

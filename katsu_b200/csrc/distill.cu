@@ -31,7 +31,7 @@ struct Distill {
     float temperature, soft, hard;
     float c0, c1;  // log2(e) / T and log2(e)
     unsigned rows, vocab, top, blocks;  // blocks of a row
-    int accumulate;
+    int accumulate, waves;
 };
 
 struct Sums {
@@ -123,14 +123,19 @@ struct Row {
     }
 };
 
+// Blocks of an SM, by 40 registers a thread.
+constexpr int blocks_of_sm(int threads) { return 65536 / ((threads + 32) * 40); }
+
 // THREADS threads go through the row, the warp behind them through its entries.  GRAD: writes the gradient (and the loss where it is
 // asked for).  TWO: sums at the temperature and at 1; otherwise one set of sums is both.
 template <int THREADS, bool GRAD, bool TWO>
-__global__ void __launch_bounds__(THREADS + 32, 65536 / ((THREADS + 32) * 40)) distill_kernel(Distill a) {
+__global__ void __launch_bounds__(THREADS + 32, blocks_of_sm(THREADS)) distill_kernel(Distill a) {
     extern __shared__ float dynamic[];
     __shared__ Sums of_warp[THREADS / 32];
     __shared__ Sums of_block[kMostCluster];
     __shared__ float teacher_sum;
+    if (!a.waves) launch_next();
+    launch_wait();
     const unsigned lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const unsigned row = blockIdx.x / a.blocks, rank = blockIdx.x % a.blocks;
     const float weight = a.weight ? a.weight[row] : 1.f, of_row = GRAD && a.g ? a.g[row] : 1.f;
@@ -328,10 +333,12 @@ __global__ void __launch_bounds__(THREADS + 32, 65536 / ((THREADS + 32) * 40)) d
 }
 
 template <int THREADS, bool GRAD, bool TWO>
-int32_t launch(katsu_cuda_ctx *ctx, const Distill &a) {
+int32_t launch(katsu_cuda_ctx *ctx, Distill a) {
     const size_t smem = 4 * sizeof(float) * (size_t(a.top) + 1), blocks = size_t(a.rows) * a.blocks;
     if (blocks > 0x7fffffffu) return katsu_set_error(KATSU_ERR_UNSUPPORTED, "%u rows of %u logits in one loss", a.rows, a.vocab);
-    return katsu_launch(ctx, false, distill_kernel<THREADS, GRAD, TWO>, unsigned(blocks), THREADS + 32, smem, a.blocks, a);
+    const size_t per_sm = std::min<size_t>(blocks_of_sm(THREADS), katsu_shared_per_sm() / (smem + 2048));
+    a.waves = blocks > (a.blocks > 1 ? size_t(ctx->num_sms) * 3 / 4 : per_sm * ctx->num_sms);  // (not every group of SMs is filled by clusters)
+    return katsu_launch(ctx, !a.waves, distill_kernel<THREADS, GRAD, TWO>, unsigned(blocks), THREADS + 32, smem, a.blocks, a);
 }
 
 template <bool GRAD>
@@ -366,7 +373,7 @@ int32_t check(const katsu_cuda_ctx *ctx, const Distill &a, size_t rows, size_t v
     KATSU_REQUIRE(ctx != nullptr, "null context");
     KATSU_REQUIRE(rows <= 0x7fffffffu && vocab <= 0x7fffffffu, "rows and vocab are below 2^31");
     KATSU_REQUIRE(top <= KATSU_DISTILL_MAX_TOP, "at most KATSU_DISTILL_MAX_TOP entries of a row");
-    KATSU_REQUIRE(a.temperature > 0.f && isfinite(a.temperature), "temperature must be above 0, and finite");
+    KATSU_REQUIRE(a.temperature >= FLT_MIN && isfinite(a.temperature), "temperature must be above 0, and finite");  // (its reciprocal too)
     KATSU_REQUIRE(isfinite(a.soft) && isfinite(a.hard), "soft and hard must be finite");
     if (rows == 0) return KATSU_OK;
     KATSU_REQUIRE(vocab != 0, "a loss needs a vocabulary");
@@ -395,7 +402,7 @@ extern "C" int32_t katsu_cuda_distill_fwd(katsu_cuda_ctx *ctx, const float *logi
                                           const int32_t *labels, const float *weight, float temperature, float soft, float hard,
                                           float *loss, size_t rows, size_t vocab, size_t top) {
     const Distill a = {logits, teacher, weight, nullptr, index, labels, loss, nullptr, temperature, soft, hard,
-                       0.f, 0.f, unsigned(rows), unsigned(vocab), unsigned(top), 1, 0};
+                       0.f, 0.f, unsigned(rows), unsigned(vocab), unsigned(top), 1, 0, 0};
     KATSU_TRY(check(ctx, a, rows, vocab, top));
     KATSU_REQUIRE(loss != nullptr || rows == 0, "loss is null");
     KATSU_TRY(katsu_bind(ctx));
@@ -407,7 +414,7 @@ extern "C" int32_t katsu_cuda_distill_bwd(katsu_cuda_ctx *ctx, const float *logi
                                           const float *g, float *loss, float *dlogits, size_t rows, size_t vocab, size_t top,
                                           int32_t accumulate) {
     const Distill a = {logits, teacher, weight, g, index, labels, loss, dlogits, temperature, soft, hard,
-                       0.f, 0.f, unsigned(rows), unsigned(vocab), unsigned(top), 1, accumulate != 0};
+                       0.f, 0.f, unsigned(rows), unsigned(vocab), unsigned(top), 1, accumulate != 0, 0};
     KATSU_TRY(check(ctx, a, rows, vocab, top));
     KATSU_REQUIRE(dlogits != nullptr || rows == 0, "dlogits is null");
     KATSU_TRY(katsu_bind(ctx));

@@ -14,7 +14,7 @@
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256, kLookups = 8;  // of a lookup, and its blocks of an SM
 
 template <int VEC>
 struct Values {
@@ -59,7 +59,7 @@ Rows rows_of(size_t count, size_t units) {
 
 // INT8: the table's rows are int8_t of `pitch` bytes with a scale each, four values a load.
 template <int VEC, bool INT8>
-__global__ void __launch_bounds__(kThreads) embed_kernel(const void *table, const float *rows_scale, const int *tokens, float scale,
+__global__ void __launch_bounds__(kThreads, kLookups) embed_kernel(const void *table, const float *rows_scale, const int *tokens, float scale,
                                                          float *y, Rows rows, unsigned vocab, size_t pitch, size_t cols, int waves) {
     if (!waves) launch_next();
     launch_wait();
@@ -103,7 +103,7 @@ __global__ void __launch_bounds__(kThreads) embed_kernel(const void *table, cons
 // Rows that are not whole 16-byte units: y is written by 16 bytes from its own boundary on, whatever rows these are of, and the
 // table is read value by value.  Fewer than 2^32 values in all.
 template <bool INT8>
-__global__ void __launch_bounds__(kThreads) embed_flat_kernel(const void *table, const float *rows_scale, const int *tokens, float scale,
+__global__ void __launch_bounds__(kThreads, kLookups) embed_flat_kernel(const void *table, const float *rows_scale, const int *tokens, float scale,
                                                               float *y, unsigned values, unsigned vocab, size_t pitch, unsigned cols, int waves) {
     if (!waves) launch_next();
     launch_wait();
@@ -149,14 +149,14 @@ int32_t lookup(katsu_cuda_ctx *ctx, const void *table, const float *rows_scale, 
     const bool whole = vectors(y, cols) && (INT8 || vectors(table, cols));
     if (!whole && count * cols < 0xfffffff0u) {
         const size_t blocks = katsu_div_up(count * cols + 3, size_t(8) * kThreads);
-        const bool waves = blocks > size_t(2) * ctx->num_sms;
+        const bool waves = blocks > size_t(kLookups) * ctx->num_sms;
         return katsu_launch(ctx, !waves, embed_flat_kernel<INT8>, unsigned(blocks), kThreads, 0, 1, table, rows_scale, tokens, scale, y,
                             unsigned(count * cols), unsigned(vocab), pitch, unsigned(cols), int(waves));
     }
     const Rows rows = rows_of(count, whole ? cols / 4 : cols);
     const size_t blocks = katsu_div_up(count, kThreads >> rows.shift) * rows.slabs;
     if (blocks > 0x7fffffffu) return katsu_set_error(KATSU_ERR_UNSUPPORTED, "%zu rows of %zu values in one lookup", count, cols);
-    const bool waves = blocks > size_t(2) * ctx->num_sms;
+    const bool waves = blocks > size_t(kLookups) * ctx->num_sms;
     return katsu_launch(ctx, !waves, whole ? embed_kernel<4, INT8> : embed_kernel<1, INT8>, unsigned(blocks), kThreads, 0, 1, table, rows_scale,
                         tokens, scale, y, rows, unsigned(vocab), pitch, cols, int(waves));
 }
@@ -363,7 +363,7 @@ struct Grad {
     float scale;
     unsigned count, vocab, units, slabs, piece, pieces, piece_blocks, fill_rows;
     int shift, waves;
-    bool accumulate;
+    bool accumulate, bundles;
     size_t cols, pitch;
 };
 
@@ -539,7 +539,56 @@ __global__ void __launch_bounds__(kGradThreads, ADD ? 5 : 8) embed_grad_kernel(G
     }
 }
 
-// Runs of more than one piece: what their first piece kept behind, and what every later one kept in front.
+// Long runs (a padding token is half of a batch): kBundle pieces that one run fills, from a multiple of kBundle on, are added up into
+// the place of the first one, by as many blocks as there are such bundles.  Where the run fills them, both kernels find the same.
+constexpr unsigned kBundle = 32;
+
+__device__ __forceinline__ bool bundle_of_run(const Grad &g, unsigned first, unsigned key) {
+    const unsigned long long end = ((unsigned long long)first + kBundle) * g.piece;
+    return end <= g.count && g.keys[end - 1] == key;  // (a piece of the run is `first`, and not its first one)
+}
+
+// The sum of what the pieces kept in front, sixteen on their way together.  next(&piece): whether there is another one, and which.
+template <int VEC, typename Next>
+__device__ __forceinline__ void add_kept(const Grad &g, unsigned u, Values<VEC> *sum, Next &&next) {
+    for (bool more = true; more;) {
+        Values<VEC> v[16];
+        int taken = 0;
+#pragma unroll
+        for (int q = 0; q < 16; ++q) {
+            unsigned piece;
+            more = more && next(&piece);
+            if (!more) continue;
+            v[q] = load<VEC>(g.kept + size_t(piece) * 2 * g.pitch + size_t(u) * VEC);
+            taken = q + 1;
+        }
+#pragma unroll
+        for (int q = 0; q < 16; ++q)
+            if (q < taken)
+#pragma unroll
+                for (int c = 0; c < VEC; ++c) sum->v[c] += v[q].v[c];
+    }
+}
+
+template <int VEC>
+__global__ void __launch_bounds__(kGradThreads) embed_bundle_kernel(Grad g) {
+    const unsigned width = 1u << g.shift, groups = kGradThreads >> g.shift, lane = threadIdx.x & (width - 1);
+    if (!g.waves) launch_next();
+    launch_wait();
+    const unsigned first = (blockIdx.x / g.slabs * groups + (threadIdx.x >> g.shift)) * kBundle, u = blockIdx.x % g.slabs * width + lane;
+    if (first == 0 || first >= g.pieces || u >= g.units) return;
+    const unsigned key = g.keys[first * g.piece];
+    if (key >= g.vocab || g.keys[first * g.piece - 1] != key || !bundle_of_run(g, first, key)) return;
+    Values<VEC> sum = zero_values<VEC>();
+    unsigned at = first;
+    add_kept<VEC>(g, u, &sum, [&](unsigned *piece) {
+        *piece = at++;
+        return *piece < first + kBundle;
+    });
+    store<VEC>(g.kept + size_t(first) * 2 * g.pitch + size_t(u) * VEC, sum);
+}
+
+// Runs of more than one piece: what their first piece kept behind, and what every later one (or bundle) kept in front.
 template <int VEC, bool ADD>
 __global__ void __launch_bounds__(kGradThreads) embed_fold_kernel(Grad g) {
     const unsigned width = 1u << g.shift, groups = kGradThreads >> g.shift, lane = threadIdx.x & (width - 1);
@@ -561,21 +610,16 @@ __global__ void __launch_bounds__(kGradThreads) embed_fold_kernel(Grad g) {
         if (through < looking) break;
     }
     if (u >= g.units) return;
-    const float *kept = g.kept + size_t(u) * VEC;
     float *dst = row_of<VEC>(g, key, u);
     const Values<VEC> old = ADD ? load<VEC>(dst) : zero_values<VEC>();
-    Values<VEC> sum = load<VEC>(kept + (size_t(piece) * 2 + 1) * g.pitch);
-    for (unsigned p = piece + 1; p <= last; p += 16) {
-        Values<VEC> v[16];
-#pragma unroll
-        for (int q = 0; q < 16; ++q)
-            if (p + q <= last) v[q] = load<VEC>(kept + size_t(p + q) * 2 * g.pitch);
-#pragma unroll
-        for (int q = 0; q < 16; ++q)
-            if (p + q <= last)
-#pragma unroll
-                for (int c = 0; c < VEC; ++c) sum.v[c] += v[q].v[c];
-    }
+    Values<VEC> sum = load<VEC>(g.kept + (size_t(piece) * 2 + 1) * g.pitch + size_t(u) * VEC);
+    unsigned at = piece + 1;
+    add_kept<VEC>(g, u, &sum, [&](unsigned *p) {
+        *p = at;
+        const bool bundled = g.bundles && at % kBundle == 0 && (at + kBundle <= last || (at + kBundle - 1 == last && bundle_of_run(g, at, key)));
+        at += bundled ? kBundle : 1;
+        return *p <= last;
+    });
     write_row<VEC, ADD>(g, dst, sum, old);
 }
 
@@ -596,6 +640,13 @@ int32_t launch_grad(katsu_cuda_ctx *ctx, Grad g) {
     if (g.tokens) return katsu_launch(ctx, !g.waves, embed_direct_kernel<VEC, ADD>, unsigned(blocks), kGradThreads, 0, 1, g);
     KATSU_TRY(katsu_launch(ctx, !g.waves, embed_grad_kernel<VEC, ADD>, unsigned(blocks), kGradThreads, (2 * groups * g.piece + 2) * sizeof(unsigned), 1, g));
     if (g.pieces == 1) return KATSU_OK;
+    // (below 512 pieces a run's fold is short beside another launch)
+    g.bundles = g.pieces >= 512;
+    if (g.bundles) {
+        const size_t bundle_blocks = katsu_div_up(katsu_div_up(g.pieces, kBundle), groups) * g.slabs;
+        g.waves = bundle_blocks > resident;
+        KATSU_TRY(katsu_launch(ctx, !g.waves, embed_bundle_kernel<VEC>, unsigned(bundle_blocks), kGradThreads, 0, 1, g));
+    }
     g.waves = piece_blocks > resident;
     return katsu_launch(ctx, !g.waves, embed_fold_kernel<VEC, ADD>, g.piece_blocks, kGradThreads, 0, 1, g);
 }

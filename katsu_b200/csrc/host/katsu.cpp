@@ -1224,7 +1224,7 @@ Tensor Int8Linear::embed(const std::vector<int32_t> &tokens, const std::vector<s
 }
 
 DistillLoss::DistillLoss(float temperature, float soft, float hard) : temperature_(temperature), soft_(soft), hard_(hard) {
-    if (!(temperature > 0.f) || std::isinf(temperature)) fail(ErrorKind::InvalidOperand, "temperature must be above 0, and finite");
+    if (!(temperature > 0.f) || !std::isnormal(temperature)) fail(ErrorKind::InvalidOperand, "temperature must be above 0, and finite");
     if (!std::isfinite(soft) || !std::isfinite(hard)) fail(ErrorKind::InvalidOperand, "soft and hard must be finite");
 }
 

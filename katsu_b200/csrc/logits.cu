@@ -217,7 +217,8 @@ int32_t launch(katsu_cuda_ctx *ctx, Adjust a) {
     const size_t blocks = size_t(a.rows) * a.slices, smem = 4 * (size_t(a.places) + a.masks + 3 * size_t(a.biases));
     if (blocks > 0x7fffffffu) return katsu_set_error(KATSU_ERR_UNSUPPORTED, "%u rows of %u logits in one call", a.rows, a.vocab);
     KATSU_TRY(katsu_prepare_kernel(ctx, reinterpret_cast<const void *>(adjust_kernel<WIDE>), smem, false));
-    a.waves = blocks > size_t(2) * ctx->num_sms;
+    const size_t per_sm = std::min<size_t>(kBlocks, katsu_shared_per_sm() / (smem + 1024));
+    a.waves = blocks > per_sm * ctx->num_sms;
     return katsu_launch(ctx, !a.waves, adjust_kernel<WIDE>, unsigned(blocks), kThreads, smem, 1, a);
 }
 

@@ -18,6 +18,11 @@ def some_tokens(rng, count, vocab, how="zipf"):
     if how == "holes":
         tokens[rng.random(count) < 0.3] = -1
         tokens[: min(count, 4)] = [vocab, *NONE][: min(count, 4)]
+    if how == "half":  # a padding token
+        tokens[rng.random(count) < 0.7] = min(1, vocab - 1)
+    if how == "blocks":  # runs that end with whole pieces and bundles of them
+        tokens = np.arange(count) * vocab // count
+        rng.shuffle(tokens)
     if how == "sorted":
         tokens.sort()
     return tokens
@@ -77,9 +82,10 @@ def test_lookup_of_no_tokens_and_in_no_table(ctx):
         assert not d.get("y").any()
 
 
-# counts up to and above 256, to which tokens are not sorted, around 8192, where the sort changes, and 4096 to 65536, where pieces grow; vocabularies of
+# counts up to and above 256, to which tokens are not sorted, around 8192, where the sort changes, and 4096 to 65536, where pieces grow; runs of more than 32 pieces; vocabularies of
 # one to three digits of a sort
 GRADS = [(127, 9, 24, "zipf"), (128, 3, 40, "one"), (128, 500, 513, "holes"), (129, 3, 40, "one"), (256, 2, 516, "uniform"), (256, 90, 64, "zipf"), (257, 2, 516, "uniform"), (255, 1, 3, "one"), (160, 1, 12, "one"), (161, 300, 515, "holes"),
+         (40000, 5, 8, "half"), (40000, 2, 1030, "half"), (66000, 3, 36, "half"), (16384 + 512, 2, 8, "blocks"), (65536, 4, 12, "blocks"),
          (4096, 30, 20, "zipf"), (16384, 2, 12, "uniform"), (16385, 9, 12, "zipf"), (65537, 5, 4, "zipf"), (32768, 3, 8, "one"), (32769, 3, 8, "one"), (32800, 100, 132, "zipf"), (50000, 2, 1, "uniform"),
          (1, 1, 1, "one"), (2, 3, 5, "zipf"), (31, 1, 4, "one"), (32, 2, 4, "uniform"), (33, 1, 7, "one"), (64, 9, 16, "sorted"),
          (65, 200, 36, "holes"), (100, 40, 515, "zipf"), (1000, 10, 64, "zipf"), (1000, 5000, 1030, "uniform"), (300, 7, 4100, "zipf"),

@@ -116,6 +116,20 @@ __global__ void __launch_bounds__(kThreads, kLookups) embed_flat_kernel(const vo
         const unsigned first = unsigned(place) - lead;
         float v[4];
         unsigned row = (first < values ? first : 0) / cols, col = (first < values ? first : 0) - row * cols;
+        if (first < values && cols - col >= 4) {  // four of one row
+            const unsigned token = unsigned(tokens[row]);
+            const size_t at = size_t(token) * pitch + col;
+            const bool there = token < vocab;
+            const float of_row = INT8 && there ? rows_scale[token] : 1.f;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                if (!there) v[c] = 0.f;
+                else if (INT8) v[c] = (float(static_cast<const int8_t *>(table)[at + c]) * of_row) * scale;
+                else v[c] = static_cast<const float *>(table)[at + c] * scale;
+            }
+            *reinterpret_cast<float4 *>(y + first) = make_float4(v[0], v[1], v[2], v[3]);
+            continue;
+        }
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
             v[c] = 0.f;
@@ -353,6 +367,7 @@ __global__ void __launch_bounds__(256) scatter_kernel(Pass p, const unsigned *di
 
 // ---- the gradient ----------------------------------------------------------------------------------------------------------
 constexpr int kGradThreads = 128, kMostPiece = 64, kDirect = 256;
+constexpr int kApart = 2;
 
 struct Grad {
     const int *tokens;  // few tokens: unsorted
@@ -361,8 +376,8 @@ struct Grad {
     const float *dy;
     float *dtable, *kept;  // kept [piece][2][pitch]: of the run that began in front; of the one that goes on behind
     float scale;
-    unsigned count, vocab, units, slabs, piece, pieces, piece_blocks, fill_rows;
-    int shift, waves;
+    unsigned count, vocab, units, slabs, slab_cols, piece, pieces, piece_blocks, fill_rows;
+    int shift, fill_shift, waves;
     bool accumulate, bundles;
     size_t cols, pitch;
 };
@@ -378,43 +393,83 @@ __device__ __forceinline__ unsigned lower_bound(const unsigned *keys, unsigned c
     return lo;
 }
 
-template <int VEC>
-__device__ __forceinline__ float *row_of(const Grad &g, unsigned key, unsigned u) {
-    return g.dtable + size_t(key) * g.cols + size_t(u) * VEC;
-}
+// A thread's N values of a row, in slab `slab` of it and at place `lane` of the group: 16 bytes of rows that are whole 16-byte units
+// (WHOLE), else kApart values a group's width apart, so that a warp's accesses lie side by side.  One, two and four of them: 90, 74 and
+// 72 us for 30 000 rows of 1001, 60, 67 and 86 for 100 000 rows of 61.
+template <bool WHOLE, int N>
+struct Part {
+    size_t at;
+    unsigned step;
+    int count;  // how many of the N there are
 
-template <int VEC>
-__device__ __forceinline__ Values<VEC> zero_values() {
-    Values<VEC> r;
+    __device__ __forceinline__ Part(const Grad &g, unsigned slab, unsigned lane) {
+        step = 1u << g.shift;
+        if (WHOLE) {
+            const unsigned u = (slab << g.shift) + lane;
+            at = 4 * size_t(u);
+            count = u < g.units ? N : 0;
+        } else {
+            const unsigned first = slab * g.slab_cols, cols = unsigned(min(size_t(g.slab_cols), g.cols - first));
+            at = size_t(first) + lane;
+            count = lane < cols ? int((cols - lane + step - 1) >> g.shift) : 0;
+        }
+    }
+    __device__ __forceinline__ Values<N> load(const float *row) const {
+        if constexpr (WHOLE) return ::load<4>(row + at);
+        Values<N> r;
 #pragma unroll
-    for (int c = 0; c < VEC; ++c) r.v[c] = 0.f;
+        for (int c = 0; c < N; ++c) r.v[c] = c < count ? row[at + c * step] : 0.f;
+        return r;
+    }
+    __device__ __forceinline__ void store(float *row, const Values<N> &r) const {
+        if constexpr (WHOLE) ::store<4>(row + at, r);
+        else
+#pragma unroll
+            for (int c = 0; c < N; ++c)
+                if (c < count) row[at + c * step] = r.v[c];
+    }
+};
+
+__device__ __forceinline__ float *row_of(const Grad &g, unsigned key) { return g.dtable + size_t(key) * g.cols; }
+
+template <int N>
+__device__ __forceinline__ Values<N> zero_values() {
+    Values<N> r;
+#pragma unroll
+    for (int c = 0; c < N; ++c) r.v[c] = 0.f;
     return r;
 }
 
-// sum = scale * sum, added to what the table has where that is asked for
-template <int VEC, bool ADD>
-__device__ __forceinline__ void write_row(const Grad &g, float *dst, Values<VEC> sum, const Values<VEC> &old) {
+template <int N>
+__device__ __forceinline__ void add_values(Values<N> *sum, const Values<N> &v) {
 #pragma unroll
-    for (int c = 0; c < VEC; ++c) sum.v[c] = ADD ? fmaf(g.scale, sum.v[c], old.v[c]) : g.scale * sum.v[c];
-    store<VEC>(dst, sum);
+    for (int c = 0; c < N; ++c) sum->v[c] += v.v[c];
+}
+
+// sum = scale * sum, added to what the table has where that is asked for
+template <bool WHOLE, int N, bool ADD>
+__device__ __forceinline__ void write_row(const Grad &g, const Part<WHOLE, N> &part, float *row, Values<N> sum, const Values<N> &old) {
+#pragma unroll
+    for (int c = 0; c < N; ++c) sum.v[c] = ADD ? fmaf(g.scale, sum.v[c], old.v[c]) : g.scale * sum.v[c];
+    part.store(row, sum);
 }
 
 // Zeros for rows row0 .. row0 + rows - 1 but for those that are `there`, by 16 bytes from the first boundary of a row on.
 __device__ __forceinline__ void fill_rows(const Grad &g, const bool *there, unsigned row0, unsigned rows) {
-    const unsigned width = 1u << g.shift, groups = kGradThreads >> g.shift, lane = threadIdx.x & (width - 1);
-    for (unsigned r = threadIdx.x >> g.shift; r < rows; r += groups) {
+    const unsigned width = 1u << g.fill_shift, groups = kGradThreads >> g.fill_shift, lane = threadIdx.x & (width - 1);
+    for (unsigned r = threadIdx.x >> g.fill_shift; r < rows; r += groups) {
         if (there[r]) continue;
         float *row = g.dtable + size_t(row0 + r) * g.cols;
         const unsigned cols = unsigned(g.cols), head = min(cols, (0u - unsigned(reinterpret_cast<uintptr_t>(row) >> 2)) & 3u), units = (cols - head) / 4;
-        if (lane < head) row[lane] = 0.f;
+        for (unsigned c = lane; c < head; c += width) row[c] = 0.f;
         float4 *body = reinterpret_cast<float4 *>(row + head);
         for (unsigned u = lane; u < units; u += width) body[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (lane < cols - head - 4 * units) row[head + 4 * units + lane] = 0.f;
+        for (unsigned c = head + 4 * units + lane; c < cols; c += width) row[c] = 0.f;
     }
 }
 
 // Up to kDirect tokens, without sorting: a group of 1 << shift threads takes the run of one token, if that is its first place.
-template <int VEC, bool ADD>
+template <bool WHOLE, int N, bool ADD>
 __global__ void __launch_bounds__(kGradThreads) embed_direct_kernel(Grad g) {
     __shared__ __align__(16) unsigned keys[kDirect];
     __shared__ bool there[kGradThreads];
@@ -432,8 +487,8 @@ __global__ void __launch_bounds__(kGradThreads) embed_direct_kernel(Grad g) {
         return;
     }
     const unsigned groups = kGradThreads >> g.shift, i = blockIdx.x / g.slabs * groups + (threadIdx.x >> g.shift);
-    const unsigned u = ((blockIdx.x % g.slabs) << g.shift) + (threadIdx.x & ((1u << g.shift) - 1));
-    if (i >= g.count || u >= g.units) return;
+    const Part<WHOLE, N> part(g, blockIdx.x % g.slabs, threadIdx.x & ((1u << g.shift) - 1));
+    if (i >= g.count || part.count == 0) return;
     const unsigned key = keys[i];
     if (key >= g.vocab) return;
     // places of the token: the next one from `from` on in `same`, the 64 places of one word after the other
@@ -451,33 +506,32 @@ __global__ void __launch_bounds__(kGradThreads) embed_direct_kernel(Grad g) {
     if (same << (63 - (i & 63)) << 1) return;  // an earlier place, in this word or in those in front of it
     for (unsigned front = 0; front < from; front += 64)
         if (word(front)) return;
-    float *dst = row_of<VEC>(g, key, u);
-    const Values<VEC> old = ADD ? load<VEC>(dst) : zero_values<VEC>();
-    Values<VEC> sum = zero_values<VEC>();
+    float *dst = row_of(g, key);
+    const Values<N> old = ADD ? part.load(dst) : zero_values<N>();
+    Values<N> sum = zero_values<N>();
     for (;;) {
         while (!same && from + 64 < g.count) same = word(from += 64);
         if (!same) break;
-        Values<VEC> v[8];
+        Values<N> v[8];
         int taken = 0;
 #pragma unroll
         for (int q = 0; q < 8; ++q) {
             if (!same) continue;
-            v[q] = load<VEC>(g.dy + size_t(from + __ffsll((long long)same) - 1) * g.cols + size_t(u) * VEC);
+            v[q] = part.load(g.dy + size_t(from + __ffsll((long long)same) - 1) * g.cols);
             same &= same - 1;
             taken = q + 1;
         }
 #pragma unroll
         for (int q = 0; q < 8; ++q)
             if (q < taken)
-#pragma unroll
-                for (int c = 0; c < VEC; ++c) sum.v[c] += v[q].v[c];
+                add_values(&sum, v[q]);
     }
-    write_row<VEC, ADD>(g, dst, sum, old);
+    write_row<WHOLE, N, ADD>(g, part, dst, sum, old);
 }
 
 // Blocks 0 .. piece_blocks - 1: a group of 1 << shift threads adds up a piece (a slab of 1 << shift accesses of its rows); the
 // blocks behind them write zeros to fill_rows rows of the table each, but for those of tokens that are there.
-template <int VEC, bool ADD>
+template <bool WHOLE, int N, bool ADD>
 __global__ void __launch_bounds__(kGradThreads, ADD ? 5 : 8) embed_grad_kernel(Grad g) {
     const unsigned width = 1u << g.shift, groups = kGradThreads >> g.shift, mine = threadIdx.x >> g.shift, lane = threadIdx.x & (width - 1);
     extern __shared__ unsigned keys[];  // of the block's pieces, their positions behind them
@@ -505,36 +559,36 @@ __global__ void __launch_bounds__(kGradThreads, ADD ? 5 : 8) embed_grad_kernel(G
     if (threadIdx.x == 0) keys[0] = begin0 ? g.keys[begin0 - 1] : ~0u;
     if (threadIdx.x == 1) keys[1 + staged] = begin0 + staged < g.count ? g.keys[begin0 + staged] : ~0u;
     __syncthreads();
-    const unsigned piece = piece0 + mine, u = slab * width + lane, j0 = mine * g.piece;
-    if (piece >= g.pieces || u >= g.units) return;
+    const unsigned piece = piece0 + mine, j0 = mine * g.piece;
+    const Part<WHOLE, N> part(g, slab, lane);
+    if (piece >= g.pieces || part.count == 0) return;
     const unsigned j1 = min(staged, j0 + g.piece);
-    float *kept = g.kept + size_t(piece) * 2 * g.pitch + size_t(u) * VEC;
+    float *kept = g.kept + size_t(piece) * 2 * g.pitch;
     bool began = keys[j0] != keys[j0 + 1];  // the current run began in this piece
-    Values<VEC> sum = zero_values<VEC>();
+    Values<N> sum = zero_values<N>();
     for (unsigned j = j0; j < j1; j += 8) {
-        Values<VEC> v[8], old[8];
+        Values<N> v[8], old[8];
 #pragma unroll
         for (int q = 0; q < 8; ++q)
-            if (j + q < j1) v[q] = load<VEC>(g.dy + size_t(position[j + q]) * g.cols + size_t(u) * VEC);
+            if (j + q < j1) v[q] = part.load(g.dy + size_t(position[j + q]) * g.cols);
         if (ADD)  // rows that end here, asked for with the others: one by one they took a trip to memory each
 #pragma unroll
             for (int q = 0; q < 8; ++q)
                 if (j + q < j1 && keys[2 + j + q] != keys[1 + j + q] && keys[1 + j + q] < g.vocab)
-                    old[q] = load<VEC>(row_of<VEC>(g, keys[1 + j + q], u));
+                    old[q] = part.load(row_of(g, keys[1 + j + q]));
 #pragma unroll
         for (int q = 0; q < 8; ++q) {
             if (j + q >= j1) continue;
-#pragma unroll
-            for (int c = 0; c < VEC; ++c) sum.v[c] += v[q].v[c];
+            add_values(&sum, v[q]);
             const unsigned key = keys[1 + j + q];
             const bool ends = keys[2 + j + q] != key;
             if (!ends && j + q + 1 < j1) continue;
             if (key < g.vocab) {
-                if (ends && began) write_row<VEC, ADD>(g, row_of<VEC>(g, key, u), sum, old[q]);
-                else store<VEC>(kept + (began ? g.pitch : 0), sum);
+                if (ends && began) write_row<WHOLE, N, ADD>(g, part, row_of(g, key), sum, old[q]);
+                else part.store(kept + (began ? g.pitch : 0), sum);
             }
             began = true;
-            sum = zero_values<VEC>();
+            sum = zero_values<N>();
         }
     }
 }
@@ -549,52 +603,52 @@ __device__ __forceinline__ bool bundle_of_run(const Grad &g, unsigned first, uns
 }
 
 // The sum of what the pieces kept in front, sixteen on their way together.  next(&piece): whether there is another one, and which.
-template <int VEC, typename Next>
-__device__ __forceinline__ void add_kept(const Grad &g, unsigned u, Values<VEC> *sum, Next &&next) {
+template <bool WHOLE, int N, typename Next>
+__device__ __forceinline__ void add_kept(const Grad &g, const Part<WHOLE, N> &part, Values<N> *sum, Next &&next) {
     for (bool more = true; more;) {
-        Values<VEC> v[16];
+        Values<N> v[16];
         int taken = 0;
 #pragma unroll
         for (int q = 0; q < 16; ++q) {
             unsigned piece;
             more = more && next(&piece);
             if (!more) continue;
-            v[q] = load<VEC>(g.kept + size_t(piece) * 2 * g.pitch + size_t(u) * VEC);
+            v[q] = part.load(g.kept + size_t(piece) * 2 * g.pitch);
             taken = q + 1;
         }
 #pragma unroll
         for (int q = 0; q < 16; ++q)
             if (q < taken)
-#pragma unroll
-                for (int c = 0; c < VEC; ++c) sum->v[c] += v[q].v[c];
+                add_values(sum, v[q]);
     }
 }
 
-template <int VEC>
+template <bool WHOLE, int N>
 __global__ void __launch_bounds__(kGradThreads) embed_bundle_kernel(Grad g) {
-    const unsigned width = 1u << g.shift, groups = kGradThreads >> g.shift, lane = threadIdx.x & (width - 1);
+    const unsigned groups = kGradThreads >> g.shift;
     if (!g.waves) launch_next();
     launch_wait();
-    const unsigned first = (blockIdx.x / g.slabs * groups + (threadIdx.x >> g.shift)) * kBundle, u = blockIdx.x % g.slabs * width + lane;
-    if (first == 0 || first >= g.pieces || u >= g.units) return;
+    const unsigned first = (blockIdx.x / g.slabs * groups + (threadIdx.x >> g.shift)) * kBundle;
+    const Part<WHOLE, N> part(g, blockIdx.x % g.slabs, threadIdx.x & ((1u << g.shift) - 1));
+    if (first == 0 || first >= g.pieces || part.count == 0) return;
     const unsigned key = g.keys[first * g.piece];
     if (key >= g.vocab || g.keys[first * g.piece - 1] != key || !bundle_of_run(g, first, key)) return;
-    Values<VEC> sum = zero_values<VEC>();
+    Values<N> sum = zero_values<N>();
     unsigned at = first;
-    add_kept<VEC>(g, u, &sum, [&](unsigned *piece) {
+    add_kept(g, part, &sum, [&](unsigned *piece) {
         *piece = at++;
         return *piece < first + kBundle;
     });
-    store<VEC>(g.kept + size_t(first) * 2 * g.pitch + size_t(u) * VEC, sum);
+    part.store(g.kept + size_t(first) * 2 * g.pitch, sum);
 }
 
 // Runs of more than one piece: what their first piece kept behind, and what every later one (or bundle) kept in front.
-template <int VEC, bool ADD>
+template <bool WHOLE, int N, bool ADD>
 __global__ void __launch_bounds__(kGradThreads) embed_fold_kernel(Grad g) {
     const unsigned width = 1u << g.shift, groups = kGradThreads >> g.shift, lane = threadIdx.x & (width - 1);
     if (!g.waves) launch_next();
     launch_wait();
-    const unsigned piece = blockIdx.x / g.slabs * groups + (threadIdx.x >> g.shift), u = blockIdx.x % g.slabs * width + lane;
+    const unsigned piece = blockIdx.x / g.slabs * groups + (threadIdx.x >> g.shift);
     const unsigned begin = piece * g.piece, next = begin + g.piece;
     if (piece + 1 >= g.pieces) return;
     const unsigned front = begin ? g.keys[begin - 1] : ~0u, first = g.keys[begin], key = g.keys[next - 1], behind = g.keys[next];
@@ -609,51 +663,57 @@ __global__ void __launch_bounds__(kGradThreads) embed_fold_kernel(Grad g) {
         last += through;
         if (through < looking) break;
     }
-    if (u >= g.units) return;
-    float *dst = row_of<VEC>(g, key, u);
-    const Values<VEC> old = ADD ? load<VEC>(dst) : zero_values<VEC>();
-    Values<VEC> sum = load<VEC>(g.kept + (size_t(piece) * 2 + 1) * g.pitch + size_t(u) * VEC);
+    const Part<WHOLE, N> part(g, blockIdx.x % g.slabs, lane);
+    if (part.count == 0) return;
+    float *dst = row_of(g, key);
+    const Values<N> old = ADD ? part.load(dst) : zero_values<N>();
+    Values<N> sum = part.load(g.kept + (size_t(piece) * 2 + 1) * g.pitch);
     unsigned at = piece + 1;
-    add_kept<VEC>(g, u, &sum, [&](unsigned *p) {
+    add_kept(g, part, &sum, [&](unsigned *p) {
         *p = at;
         const bool bundled = g.bundles && at % kBundle == 0 && (at + kBundle <= last || (at + kBundle - 1 == last && bundle_of_run(g, at, key)));
         at += bundled ? kBundle : 1;
         return *p <= last;
     });
-    write_row<VEC, ADD>(g, dst, sum, old);
+    write_row<WHOLE, N, ADD>(g, part, dst, sum, old);
 }
 
-template <int VEC, bool ADD>
+template <bool WHOLE, int N, bool ADD>
 int32_t launch_grad(katsu_cuda_ctx *ctx, Grad g) {
-    g.units = unsigned(g.cols / VEC);
+    g.units = unsigned(katsu_div_up(g.cols, N));
     g.shift = 2;
     while ((1 << g.shift) < kGradThreads && (1u << g.shift) < g.units) ++g.shift;
     g.slabs = (g.units + (1u << g.shift) - 1) >> g.shift;
+    g.slab_cols = unsigned(katsu_div_up(g.cols, g.slabs));
     const size_t groups = kGradThreads >> g.shift, piece_blocks = katsu_div_up(g.pieces, groups) * g.slabs;
-    g.fill_rows = unsigned(std::min<size_t>(kGradThreads, std::max<size_t>(1, 16384 / g.cols)));
+    // zeros: about 64 KiB a block, less where that leaves SMs without one; two accesses of a thread to a row
+    const size_t shared_out = katsu_div_up(g.vocab, size_t(8) * ctx->num_sms);
+    g.fill_rows = unsigned(std::max<size_t>(1, std::min({size_t(kGradThreads), 16384 / g.cols, shared_out})));
+    g.fill_shift = 0;
+    while ((1 << g.fill_shift) < kGradThreads && (size_t(8) << g.fill_shift) < g.cols) ++g.fill_shift;
     const size_t fill_blocks = ADD ? 0 : katsu_div_up(g.vocab, g.fill_rows), blocks = piece_blocks + fill_blocks;
     if (blocks > 0x7fffffffu)
         return katsu_set_error(KATSU_ERR_UNSUPPORTED, "%u tokens with rows of %zu values in one gradient", g.count, g.cols);
     g.piece_blocks = unsigned(piece_blocks);
     const size_t resident = size_t(4) * ctx->num_sms;  // (of 128 threads with up to 128 registers)
     g.waves = blocks > resident;
-    if (g.tokens) return katsu_launch(ctx, !g.waves, embed_direct_kernel<VEC, ADD>, unsigned(blocks), kGradThreads, 0, 1, g);
-    KATSU_TRY(katsu_launch(ctx, !g.waves, embed_grad_kernel<VEC, ADD>, unsigned(blocks), kGradThreads, (2 * groups * g.piece + 2) * sizeof(unsigned), 1, g));
+    if (g.tokens) return katsu_launch(ctx, !g.waves, embed_direct_kernel<WHOLE, N, ADD>, unsigned(blocks), kGradThreads, 0, 1, g);
+    KATSU_TRY(katsu_launch(ctx, !g.waves, embed_grad_kernel<WHOLE, N, ADD>, unsigned(blocks), kGradThreads, (2 * groups * g.piece + 2) * sizeof(unsigned), 1, g));
     if (g.pieces == 1) return KATSU_OK;
     // (below 512 pieces a run's fold is short beside another launch)
     g.bundles = g.pieces >= 512;
     if (g.bundles) {
         const size_t bundle_blocks = katsu_div_up(katsu_div_up(g.pieces, kBundle), groups) * g.slabs;
         g.waves = bundle_blocks > resident;
-        KATSU_TRY(katsu_launch(ctx, !g.waves, embed_bundle_kernel<VEC>, unsigned(bundle_blocks), kGradThreads, 0, 1, g));
+        KATSU_TRY(katsu_launch(ctx, !g.waves, embed_bundle_kernel<WHOLE, N>, unsigned(bundle_blocks), kGradThreads, 0, 1, g));
     }
     g.waves = piece_blocks > resident;
-    return katsu_launch(ctx, !g.waves, embed_fold_kernel<VEC, ADD>, g.piece_blocks, kGradThreads, 0, 1, g);
+    return katsu_launch(ctx, !g.waves, embed_fold_kernel<WHOLE, N, ADD>, g.piece_blocks, kGradThreads, 0, 1, g);
 }
 
-int32_t launch_grad_for(katsu_cuda_ctx *ctx, const Grad &g, bool vec) {
-    if (g.accumulate) return vec ? launch_grad<4, true>(ctx, g) : launch_grad<1, true>(ctx, g);
-    return vec ? launch_grad<4, false>(ctx, g) : launch_grad<1, false>(ctx, g);
+int32_t launch_grad_for(katsu_cuda_ctx *ctx, const Grad &g, bool whole) {
+    if (g.accumulate) return whole ? launch_grad<true, 4, true>(ctx, g) : launch_grad<false, kApart, true>(ctx, g);
+    return whole ? launch_grad<true, 4, false>(ctx, g) : launch_grad<false, kApart, false>(ctx, g);
 }
 
 // Leaves the sorted keys and their positions in two of the four arrays of `count` words at `work`.
@@ -742,11 +802,11 @@ extern "C" int32_t katsu_cuda_embed_bwd(katsu_cuda_ctx *ctx, const int32_t *toke
     g.accumulate = accumulate != 0;
     g.cols = cols;
     g.pitch = (cols + 3) / 4 * 4;
-    const bool vec = vectors(dy, cols) && vectors(dtable, cols);
+    const bool whole = vectors(dy, cols) && vectors(dtable, cols);
     if (count <= kDirect) {
         g.tokens = tokens;
         g.pieces = g.count;
-        return launch_grad_for(ctx, g, vec);
+        return launch_grad_for(ctx, g, whole);
     }
     // A piece is a chain of loads, eight at a time; the fold of a run one of its pieces, sixteen at a time.  With a fifteenth of the
     // tokens alike both are short at pieces of 8 to 64.  Where the rows are many bytes, short pieces write too many sums beside the table.
@@ -757,5 +817,5 @@ extern "C" int32_t katsu_cuda_embed_bwd(katsu_cuda_ctx *ctx, const int32_t *toke
     KATSU_TRY(katsu_scratch(ctx, sorting + size_t(g.pieces) * 2 * g.pitch, &work));
     g.kept = work + sorting;
     KATSU_TRY(sort_tokens(ctx, tokens, g.count, g.vocab, reinterpret_cast<unsigned *>(work), &g.keys, &g.position));
-    return launch_grad_for(ctx, g, vec);
+    return launch_grad_for(ctx, g, whole);
 }

@@ -17,7 +17,7 @@ namespace {
 
 constexpr int kThreads = 256, kBlocks = 4;  // blocks of an SM
 constexpr int kHeld = 4, kAhead = 8;        // 16-byte accesses of a thread, and tokens of the history, on their way together
-constexpr unsigned kStep = 4 * kThreads, kMostSlice = 16 * kStep;
+constexpr unsigned kStep = 4 * kThreads, kMostSlice = 16 * kStep, kEdge = 8;  // kEdge: places for the edge
 
 struct Adjust {
     const float *logits, *repetition, *presence, *frequency, *bias;
@@ -76,14 +76,20 @@ __global__ void __launch_bounds__(kThreads, kBlocks) adjust_kernel(Adjust a) {
     float *out = a.out + size_t(row) * a.vocab;
     const bool in_place = z == out;
     const unsigned *words = a.allowed ? a.allowed + size_t(row) * a.words : nullptr;
-    // The slice's places are counted from the 16-byte boundary at or in front of the row: base is the token of place 0.  Tokens are
-    // taken modulo 2^32, so that the up to three places in front of the row are numbers above the vocabulary.
-    const unsigned lead = unsigned(reinterpret_cast<uintptr_t>(z) >> 2) & 3u, base = slice * a.slice - lead;
-    const bool inside = base < a.vocab && a.vocab - base >= a.slice;  // (of all the slice's places)
-    const bool whole = (unsigned(reinterpret_cast<uintptr_t>(out) >> 2) & 3u) == lead;
-    // ---- what does not wait for anything: the slice's words of the mask and the history's first tokens ----
+    // A row is whole 16-byte units, cut into slices, and up to three tokens in front of the first and behind the last unit.  These, the
+    // edge, go with the first slice: their places are behind the slice's.
+    const unsigned head = min(a.vocab, (0u - unsigned(reinterpret_cast<uintptr_t>(z) >> 2)) & 3u), body = (a.vocab - head) & ~3u;
+    const unsigned edge = slice ? 0 : a.vocab - body, begin = min(body, slice * a.slice), here = min(body - begin, a.slice);
+    const unsigned base = head + begin;  // token of place 0; places 0 .. here - 1 are base, base + 1, ..
+    auto edge_token = [&](unsigned i) { return i < head ? i : body + i; };
+    auto place_of = [&](unsigned token) {  // ~0u: not of this block
+        if (token - base < here) return token - base;
+        if (token >= a.vocab || edge == 0 || (token >= head && token < head + body)) return ~0u;
+        return a.slice + (token < head ? token : token - body);
+    };
+    // ---- what does not wait for anything: the slice's words of the mask, the history's first tokens ----
     unsigned *mask = seen + a.places;
-    const unsigned word0 = base < a.vocab ? base >> 5 : 0;
+    const unsigned word0 = base >> 5;
     if (words)
         for (unsigned i = threadIdx.x; i < a.slice / 32 + 2; i += kThreads) mask[i] = word0 + i < a.words ? words[word0 + i] : 0;
     const int *history = a.history ? a.history + size_t(row) * a.history_cols : nullptr;
@@ -93,33 +99,21 @@ __global__ void __launch_bounds__(kThreads, kBlocks) adjust_kernel(Adjust a) {
         for (int q = 0; q < kAhead; ++q) first[q] = threadIdx.x + q * kThreads < a.history_cols ? history[threadIdx.x + q * kThreads] : -1;
     for (unsigned i = threadIdx.x; i < a.places / 4; i += kThreads) reinterpret_cast<uint4 *>(seen)[i] = make_uint4(0, 0, 0, 0);
     if (words) __syncthreads();
-    // which of an access's tokens are allowed: bit c of token + c
-    auto allowed = [&](unsigned token) {
-        unsigned bits = 15;
-        if (!inside) {
-            bits = 0;
-#pragma unroll
-            for (unsigned c = 0; c < 4; ++c)
-                if (token + c < a.vocab && (!words || (mask[((token + c) >> 5) - word0] >> ((token + c) & 31) & 1u))) bits |= 1u << c;
-        } else if (words) {
-            const unsigned *at = mask + ((token >> 5) - word0);
-            bits = __funnelshift_r(at[0], at[1], token & 31) & 15;
-        }
-        return bits;
+    // of the four tokens from place p on: bit c is that of place p + c
+    auto allowed = [&](unsigned p) {
+        if (!words) return 15u;
+        const unsigned token = base + p, *at = mask + ((token >> 5) - word0);
+        return __funnelshift_r(at[0], at[1], token & 31) & 15;
     };
-    auto fetch = [&](unsigned token, unsigned bits) {
-        if (bits == 0) return make_float4(0.f, 0.f, 0.f, 0.f);
-        if (inside) return *reinterpret_cast<const float4 *>(z + token);
-        return make_float4(bits & 1 ? z[token] : 0.f, bits & 2 ? z[token + 1] : 0.f, bits & 4 ? z[token + 2] : 0.f, bits & 8 ? z[token + 3] : 0.f);
-    };
+    const float4 *units = reinterpret_cast<const float4 *>(z + base);
     float4 v[kHeld];
     unsigned bits[kHeld];
     auto ask = [&](unsigned from) {
 #pragma unroll
         for (int q = 0; q < kHeld; ++q) {
-            const unsigned place = from + q * kStep;
-            bits[q] = place < a.slice ? allowed(base + place) : 0;
-            if (!in_place) v[q] = fetch(base + place, bits[q]);
+            const unsigned p = from + q * kStep;
+            bits[q] = p < here ? allowed(p) : 0;
+            if (bits[q] && !in_place) v[q] = units[p / 4];
         }
     };
     ask(4 * threadIdx.x);
@@ -128,7 +122,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) adjust_kernel(Adjust a) {
     int *bias_tokens = reinterpret_cast<int *>(bias_z + a.biases);
     for (unsigned j = threadIdx.x; j < a.biases; j += kThreads) {
         const unsigned token = unsigned(a.bias_tokens[size_t(row) * a.biases + j]);
-        const bool mine = token < a.vocab && token - base < a.slice;
+        const bool mine = place_of(token) != ~0u;
         bias_tokens[j] = mine ? int(token) : -1;
         bias[j] = a.bias[size_t(row) * a.biases + j];
         bias_z[j] = mine ? z[token] : 0.f;
@@ -149,23 +143,38 @@ __global__ void __launch_bounds__(kThreads, kBlocks) adjust_kernel(Adjust a) {
                 token[q] = at >= length ? -1 : i == threadIdx.x ? first[q] : history[at];
             }
 #pragma unroll
-            for (int q = 0; q < kAhead; ++q)
-                if (unsigned(token[q]) < a.vocab && unsigned(token[q]) - base < a.slice) P::count(seen, unsigned(token[q]) - base, i + q * kThreads < prompt);
+            for (int q = 0; q < kAhead; ++q) {
+                const unsigned place = unsigned(token[q]) - base;
+                if (place < here) P::count(seen, place, i + q * kThreads < prompt);
+            }
+            if (edge)
+#pragma unroll
+                for (int q = 0; q < kAhead; ++q) {
+                    const unsigned t = unsigned(token[q]);
+                    if (t < head || t - (head + body) < edge - head) P::count(seen, a.slice + (t < head ? t : t - body), i + q * kThreads < prompt);
+                }
         }
     }
     if (history || a.biases) __syncthreads();
-    // ---- the slice ----
-    for (unsigned from = 4 * threadIdx.x;;) {
+    // ---- the edge, and the slice ----
+    auto is_allowed = [&](unsigned token) { return !words || (words[token >> 5] >> (token & 31) & 1u); };
+    if (threadIdx.x < edge) {
+        const unsigned token = edge_token(threadIdx.x);
+        const float value = z[token];
+        out[token] = !is_allowed(token) ? -INFINITY : history ? P::penalised(value, P::one(seen, place_of(token)), p) : value;
+    }
+    const bool whole = (reinterpret_cast<uintptr_t>(out + base) & 15u) == 0;
+    for (unsigned from = 4 * threadIdx.x; from < here;) {
 #pragma unroll
         for (int q = 0; q < kHeld; ++q) {
-            const unsigned place = from + q * kStep, token = base + place, can = bits[q];
-            if (place >= a.slice) continue;
+            const unsigned place = from + q * kStep, can = bits[q];
+            if (place >= here) continue;
             uint4 s = make_uint4(0, 0, 0, 0);
             if (history) s = P::four(seen, place);
             const bool touched = (s.x | s.y | s.z | s.w) != 0;
             if (in_place) {
                 if (can == 15 && !touched) continue;
-                v[q] = fetch(token, can);
+                if (can) v[q] = units[place / 4];
             }
             if (touched) {
                 v[q].x = P::penalised(v[q].x, s.x, p);
@@ -177,24 +186,24 @@ __global__ void __launch_bounds__(kThreads, kBlocks) adjust_kernel(Adjust a) {
             if (!(can & 2)) v[q].y = -INFINITY;
             if (!(can & 4)) v[q].z = -INFINITY;
             if (!(can & 8)) v[q].w = -INFINITY;
-            if (inside && whole) {
-                *reinterpret_cast<float4 *>(out + token) = v[q];
+            float *to = out + base + place;
+            if (whole) {
+                *reinterpret_cast<float4 *>(to) = v[q];
             } else {
-                if (token < a.vocab) out[token] = v[q].x;
-                if (token + 1 < a.vocab) out[token + 1] = v[q].y;
-                if (token + 2 < a.vocab) out[token + 2] = v[q].z;
-                if (token + 3 < a.vocab) out[token + 3] = v[q].w;
+                to[0] = v[q].x;
+                to[1] = v[q].y;
+                to[2] = v[q].z;
+                to[3] = v[q].w;
             }
         }
         from += kHeld * kStep;
-        if (from >= a.slice) break;
         ask(from);
     }
     if (a.biases == 0) return;
     __syncthreads();
     for (unsigned j = threadIdx.x; j < a.biases; j += kThreads) {
         const int token = bias_tokens[j];
-        if (token < 0 || (words && !(mask[(token >> 5) - word0] >> (token & 31) & 1u))) continue;
+        if (token < 0 || !is_allowed(unsigned(token))) continue;
         bool first = true;
         float sum = 0.f;
         for (unsigned i = 0; i < a.biases; ++i) {
@@ -202,17 +211,17 @@ __global__ void __launch_bounds__(kThreads, kBlocks) adjust_kernel(Adjust a) {
             first = first && i >= j;
             sum += bias[i];
         }
-        if (first) out[token] = (history ? P::penalised(bias_z[j], P::one(seen, unsigned(token) - base), p) : bias_z[j]) + sum;
+        if (first) out[token] = (history ? P::penalised(bias_z[j], P::one(seen, place_of(unsigned(token))), p) : bias_z[j]) + sum;
     }
 }
 
 template <bool WIDE>
 int32_t launch(katsu_cuda_ctx *ctx, Adjust a) {
     // One round of blocks, as every block looks at the row's whole history; slices are bounded by the shared memory for their places.
-    const size_t places = size_t(a.vocab) + 3, resident = size_t(kBlocks) * ctx->num_sms, wanted = std::max<size_t>(1, resident / a.rows);
-    a.slice = unsigned(std::min<size_t>(kMostSlice, katsu_div_up(katsu_div_up(places, wanted), kStep) * kStep));
-    a.slices = unsigned(katsu_div_up(places, a.slice));
-    a.places = !a.history ? 0 : WIDE ? a.slice : a.slice / 2;
+    const size_t resident = size_t(kBlocks) * ctx->num_sms, wanted = std::max<size_t>(1, resident / a.rows);
+    a.slice = unsigned(std::min<size_t>(kMostSlice, katsu_div_up(katsu_div_up(a.vocab, wanted), kStep) * kStep));
+    a.slices = unsigned(katsu_div_up(a.vocab, a.slice));
+    a.places = !a.history ? 0 : WIDE ? a.slice + kEdge : (a.slice + kEdge) / 2;
     a.masks = a.allowed ? a.slice / 32 + 2 : 0;
     const size_t blocks = size_t(a.rows) * a.slices, smem = 4 * (size_t(a.places) + a.masks + 3 * size_t(a.biases));
     if (blocks > 0x7fffffffu) return katsu_set_error(KATSU_ERR_UNSUPPORTED, "%u rows of %u logits in one call", a.rows, a.vocab);

@@ -4,11 +4,15 @@
 //   loss = w (soft T^2 sum_j p_j (log p_j - log q_idx(j)) - hard log s_label)
 //   dz   = g w (soft T (q - p) + hard (s - [v = label]))
 //
-// Bound: HBM, z once and dz once.  A row is held in the registers of a block (32 values a thread), or of a cluster of up to
-// eight blocks, from its only read to the gradient's write; blocks exchange their largest value and sums through shared memory
-// of the cluster.  Sums of exponentials are relative to a warp's largest value, joined in a tree, so that a row of 1e5 values
-// adds up 32 numbers behind each other at most.  The gradient of listed tokens (a few of a row) is written again behind
-// the row's, from sums over the list in its order: no atomics.
+// Bound: HBM, z once and dz once (4096 x 32768, T = 2, labels too: loss 82 us, 5.9 TB/s; with the gradient 184 us, 5.6 TB/s; L2 has
+// every row of the gradient's second reading).  Short or few rows: a block's chain of loads, votes and exchanges, 4 to 6 us.
+//
+// Blocks stream their row, threads with sums of their own (a largest value, sums of exponentials counted from it), four 16-byte loads
+// on their way and five blocks of 256 threads to an SM: rows held in the registers of two blocks of 512 threads took five times as
+// long, as nothing was on its way while a block exchanged its sums.  Threads, warps, blocks and the blocks of a cluster join their sums
+// in a tree.  A warp beside the others goes through the row's list and label, whose loads follow each other.  The gradient reads the
+// row again, from L2: threads and blocks are chosen so that the rows of all resident blocks fit there.  The gradient of listed tokens,
+// a few of a row, is written again behind the row's, from sums over the list in its order: no atomics.
 #include <float.h>
 #include <math.h>
 
@@ -93,7 +97,7 @@ __device__ __forceinline__ double sum_of_warp(double v) {
     return v;
 }
 
-// The row's entries and, as the last one, its label: in shared memory, written by the first warp.
+// The row's entries and, as the last one, its label: in shared memory, written by the warp behind the others.
 struct Entries {
     int *token;  // -1 where it is none
     float *e;    // exp((t - largest t) / T), 0 for the label
@@ -358,7 +362,8 @@ int32_t run(katsu_cuda_ctx *ctx, Distill a) {
     const int threads = units <= 1024 && a.rows >= size_t(16) * ctx->num_sms ? 64 : units <= 2048 ? 128 : GRAD && units > 4096 ? 512 : 256;
     a.blocks = 1;
     // Blocks of a row: more where there are few rows; a gradient's, so that all that are resident have their rows in L2.
-    while (a.blocks < kMostCluster && (size_t(a.rows) * a.blocks < size_t(2) * ctx->num_sms || (GRAD && units > a.blocks * size_t(8192))) && units > size_t(a.blocks) * 2 * threads * kHeld)
+    while (a.blocks < kMostCluster && units > size_t(a.blocks) * 2 * threads * kHeld &&
+           (size_t(a.rows) * a.blocks < size_t(2) * ctx->num_sms || (GRAD && units > a.blocks * size_t(8192))))
         a.blocks *= 2;
     switch (threads) {
         case 64: return two ? launch<64, GRAD, true>(ctx, a) : launch<64, GRAD, false>(ctx, a);

@@ -49,14 +49,16 @@ def distill(z, teacher, index, labels, weight, T, soft, hard, g=None):
     """loss and gradient of every row, and how far off f32 may be.
 
     An exponential of x = (z - largest) / T is off by U (6 + 4 |x|), relatively: its function 2 ulp, and roundings of z - largest,
-    1 / T and the product.  A row's sum of them has 60 further roundings on a value's way at most (8 of the thread, 5 of the warp, the rest joins
-    of warps and blocks, each with an exponential).  p has the same terms with fewer additions."""
+    1 / T and the product.  A row's sum of them has 60 further roundings on a value's way at most in joins of lanes, warps and blocks, each
+    with an exponential, and those of its thread: an addition for every 1024 tokens, and a product with an exponential where the largest
+    value changes, at most for every 4096.  p has the same terms with fewer additions."""
     z = z.astype(np.float64)
     rows, vocab = z.shape
     top = index.shape[1]
     w = np.ones(rows) if weight is None else weight.astype(np.float64)
     g = np.ones(rows) if g is None else g.astype(np.float64)
     loss, off = np.zeros(rows), np.zeros(rows)
+    sums = 66 + vocab / 1024 + 6 * vocab / 4096
     dz, doff = np.zeros((rows, vocab)), np.zeros((rows, vocab))
     if soft == 0 or top == 0:
         soft, T = 0.0, 1.0
@@ -72,9 +74,9 @@ def distill(z, teacher, index, labels, weight, T, soft, hard, g=None):
             e = np.exp(t - t.max()) if there.any() and t.max() > -np.inf else np.zeros(top)
             taught, labelled = bool(soft != 0 and e.sum() != 0), bool(hard != 0 and labels is not None and valid(labels[i], vocab))
             spread = np.nansum(q[i] * np.where(np.isfinite(x[i]), x[i], 0))
-            sum_q = U * (66 + 4 * spread)
+            sum_q = U * (sums + 4 * spread)
             spread1 = np.nansum(s[i] * np.where(np.isfinite(x1[i]), x1[i], 0))
-            sum_s = U * (66 + 4 * spread1)
+            sum_s = U * (sums + 4 * spread1)
             if taught:
                 p = e / e.sum()
                 at = index[i][there & (p > 0)]

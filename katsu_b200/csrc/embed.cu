@@ -380,7 +380,7 @@ struct Grad {
     const float *dy;
     float *dtable, *kept;  // kept [piece][2][pitch]: of the run that began in front; of the one that goes on behind
     float scale;
-    unsigned count, vocab, units, slabs, slab_cols, piece, pieces, piece_blocks, fill_rows;
+    unsigned count, vocab, units, slabs, piece, pieces, piece_blocks, fill_rows;
     int shift, fill_shift, waves;
     bool accumulate, bundles;
     size_t cols, pitch;
@@ -398,8 +398,8 @@ __device__ __forceinline__ unsigned lower_bound(const unsigned *keys, unsigned c
 }
 
 // A thread's N values of a row, in slab `slab` of it and at place `lane` of the group: 16 bytes of rows that are whole 16-byte units
-// (WHOLE), else kApart values a group's width apart, so that a warp's accesses lie side by side.  One, two and four of them: 90, 74 and
-// 72 us for 30 000 rows of 1001, 60, 67 and 86 for 100 000 rows of 61.
+// (WHOLE), else kApart values a group's width apart, so that a warp's accesses lie side by side.  One, two and four of them: 91, 75 and
+// 72 us for 30 000 rows of 1001, 58, 65 and 84 for 100 000 rows of 61.
 template <bool WHOLE, int N>
 struct Part {
     size_t at;
@@ -413,9 +413,8 @@ struct Part {
             at = 4 * size_t(u);
             count = u < g.units ? N : 0;
         } else {
-            const unsigned first = slab * g.slab_cols, cols = unsigned(min(size_t(g.slab_cols), g.cols - first));
-            at = size_t(first) + lane;
-            count = lane < cols ? int((cols - lane + step - 1) >> g.shift) : 0;
+            at = size_t(slab) * N * step + lane;
+            count = at < g.cols ? int(min((unsigned(g.cols - at) + step - 1) >> g.shift, unsigned(N))) : 0;
         }
     }
     __device__ __forceinline__ Values<N> load(const float *row) const {
@@ -682,13 +681,25 @@ __global__ void __launch_bounds__(kGradThreads) embed_fold_kernel(Grad g) {
     write_row<WHOLE, N, ADD>(g, part, dst, sum, old);
 }
 
+// Threads of a group, and slabs of a row, at n values a thread.
+struct Width {
+    unsigned units, slabs;
+    int shift;
+};
+
+Width width_of(size_t cols, size_t n) {
+    Width w = {unsigned(katsu_div_up(cols, n)), 1, 2};
+    while ((1 << w.shift) < kGradThreads && (1u << w.shift) < w.units) ++w.shift;
+    w.slabs = (w.units + (1u << w.shift) - 1) >> w.shift;
+    return w;
+}
+
 template <bool WHOLE, int N, bool ADD>
 int32_t launch_grad(katsu_cuda_ctx *ctx, Grad g) {
-    g.units = unsigned(katsu_div_up(g.cols, N));
-    g.shift = 2;
-    while ((1 << g.shift) < kGradThreads && (1u << g.shift) < g.units) ++g.shift;
-    g.slabs = (g.units + (1u << g.shift) - 1) >> g.shift;
-    g.slab_cols = unsigned(katsu_div_up(g.cols, g.slabs));
+    const Width width = width_of(g.cols, N);
+    g.units = width.units;
+    g.shift = width.shift;
+    g.slabs = width.slabs;
     const size_t groups = kGradThreads >> g.shift, piece_blocks = katsu_div_up(g.pieces, groups) * g.slabs;
     // zeros: about 64 KiB a block, less where that leaves SMs without one; two accesses of a thread to a row
     const size_t shared_out = katsu_div_up(g.vocab, size_t(8) * ctx->num_sms);
@@ -812,9 +823,12 @@ extern "C" int32_t katsu_cuda_embed_bwd(katsu_cuda_ctx *ctx, const int32_t *toke
         g.pieces = g.count;
         return launch_grad_for(ctx, g, whole);
     }
-    // A piece is a chain of loads, eight at a time; the fold of a run one of its pieces, sixteen at a time.  With a fifteenth of the
-    // tokens alike both are short at pieces of 8 to 64.  Where the rows are many bytes, short pieces write too many sums beside the table.
-    g.piece = count * cols >= size_t(1) << 22 ? (count <= 32768 ? 32 : kMostPiece) : count <= 4096 ? 8 : count <= 16384 ? 16 : count <= 65536 ? 32 : kMostPiece;
+    // A piece is a chain of loads, eight at a time: short ones, as long as their blocks are not more than three rounds.  Where the rows
+    // are many bytes, pieces below 32 write too many sums beside the table.
+    const Width width = width_of(cols, whole ? 4 : kApart);
+    g.piece = count * cols >= size_t(1) << 22 ? 32 : count <= 4096 ? 8 : 16;
+    while (g.piece < kMostPiece && katsu_div_up(katsu_div_up(count, g.piece), kGradThreads >> width.shift) * width.slabs > size_t(16) * ctx->num_sms)
+        g.piece *= 2;
     g.pieces = unsigned(katsu_div_up(count, g.piece));
     const size_t sorting = 4 * count + 3 * size_t(kSorters) * kDigits;
     float *work = nullptr;

@@ -82,7 +82,7 @@ def test_lookup_of_no_tokens_and_in_no_table(ctx):
         assert not d.get("y").any()
 
 
-# counts up to and above 256, to which tokens are not sorted, around 8192, where the sort changes, and 4096 to 65536, where pieces grow; runs of more than 32 pieces; vocabularies of
+# counts up to and above 256, to which tokens are not sorted, around 8192, where the sort changes, and 4096 and more, where pieces grow; runs of more than 32 pieces; vocabularies of
 # one to three digits of a sort
 GRADS = [(127, 9, 24, "zipf"), (128, 3, 40, "one"), (128, 500, 513, "holes"), (129, 3, 40, "one"), (256, 2, 516, "uniform"), (256, 90, 64, "zipf"), (257, 2, 516, "uniform"), (255, 1, 3, "one"), (160, 1, 12, "one"), (161, 300, 515, "holes"),
          (40000, 5, 8, "half"), (40000, 2, 1030, "half"), (66000, 3, 36, "half"), (16384 + 512, 2, 8, "blocks"), (65536, 4, 12, "blocks"),

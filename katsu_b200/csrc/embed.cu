@@ -9,8 +9,8 @@
 // ones cost.  Runs that lie in one piece are written as they end; what a piece has of a run that began in front of it or goes on behind
 // it is kept beside the table and folded in the pieces' order by a launch behind, in two steps where runs may be long.  Rows without
 // a token get zeros from blocks of the pieces' launch.  No floating-point atomics: the same tokens give the same bits.  Bound: HBM for
-// large gradients (65536 x 2048 into a table of as many rows: 157 us of 199, 6.8 TB/s with what L2 keeps; sorting 26, folding 16),
-// three launches one behind the other for small ones (3001 x 515: 17 us).
+// large gradients (65536 x 2048 into a table of as many rows: 152 us of 198, 7.1 TB/s with what L2 keeps; sorting 25, folding 19),
+// three launches one behind the other for small ones (3001 x 515: 15.5 us).
 #include <algorithm>
 
 #include "common.cuh"
@@ -399,7 +399,7 @@ __device__ __forceinline__ unsigned lower_bound(const unsigned *keys, unsigned c
 
 // A thread's N values of a row, in slab `slab` of it and at place `lane` of the group: 16 bytes of rows that are whole 16-byte units
 // (WHOLE), else kApart values a group's width apart, so that a warp's accesses lie side by side.  One, two and four of them: 91, 75 and
-// 72 us for 30 000 rows of 1001, 58, 65 and 84 for 100 000 rows of 61.
+// 72 us for 30 000 rows of 1001, 58, 65 and 84 for 100 000 rows of 61 (longer pieces than today's, with which two take 65 us of 30 000).
 template <bool WHOLE, int N>
 struct Part {
     size_t at;

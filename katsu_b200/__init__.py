@@ -733,11 +733,11 @@ def adjust_logits(logits, history=None, lengths=None, prompts=None, repetition=N
 
     none = np.zeros(0, np.int32)
     words = none
-    if allowed is not None:
+    if allowed is not None and len(shape) in (1, 2):  # (other ranks are refused below)
         allowed = np.asarray(allowed, dtype=bool)
         if list(allowed.shape) != shape:
             raise InvalidOperand("invalid operand: allowed must have the logits' shape")
-        allowed = allowed.reshape(rows, -1)
+        allowed = allowed.reshape(rows, shape[-1])
         bits = np.zeros((rows, (allowed.shape[1] + 31) // 32 * 32), bool)
         bits[:, : allowed.shape[1]] = allowed
         words = np.ascontiguousarray(np.packbits(bits, axis=1, bitorder="little")).view("<u4")

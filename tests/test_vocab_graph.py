@@ -209,3 +209,18 @@ def test_nothing_to_do():
     assert y.shape() == [2, 4] and not y.data().any()
     y.sum().backward()
     assert t.grad() is not None and t.grad().size == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [[0, 5], [2, 0], [0, 0], [0]])
+def test_masks_of_nothing(shape):
+    out = K.adjust_logits(K.Tensor.zeros(shape), allowed=np.zeros(shape, bool), repetition=1.5)
+    assert out.shape() == shape and out.data().size == 0
+    with pytest.raises(K.InvalidOperand):
+        K.adjust_logits(K.Tensor.zeros(shape), allowed=np.zeros([*shape, 1], bool))
+
+
+@pytest.mark.parametrize("shape", [[], [2, 3, 4]])
+def test_masks_of_other_ranks(shape):
+    with pytest.raises(K.RankMismatch):
+        K.adjust_logits(K.Tensor.zeros(shape), allowed=np.ones(shape, bool))

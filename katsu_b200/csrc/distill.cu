@@ -4,7 +4,7 @@
 //   loss = w (soft T^2 sum_j p_j (log p_j - log q_idx(j)) - hard log s_label)
 //   dz   = g w (soft T (q - p) + hard (s - [v = label]))
 //
-// Bound: HBM, z once and dz once (4096 x 32768, T = 2, labels too: loss 82 us, 5.9 TB/s; with the gradient 184 us, 5.6 TB/s; L2 has
+// Bound: HBM, z once and dz once (4096 x 32768, T = 2, labels too: loss 82 us, 5.9 TB/s; with the gradient 180 us, 5.7 TB/s; L2 has
 // every row of the gradient's second reading).  Short or few rows: a block's chain of loads, votes and exchanges, 4 to 6 us.
 //
 // Blocks stream their row, threads with sums of their own (a largest value, sums of exponentials counted from it), four 16-byte loads
@@ -12,7 +12,8 @@
 // long, as nothing was on its way while a block exchanged its sums.  Threads, warps, blocks and the blocks of a cluster join their sums
 // in a tree.  A warp beside the others goes through the row's list and label, whose loads follow each other.  The gradient reads the
 // row again, from L2: threads and blocks are chosen so that the rows of all resident blocks fit there.  The gradient of listed tokens,
-// a few of a row, is written again behind the row's, from sums over the list in its order: no atomics.
+// a few of a row, is written again behind the row's, by a token's first entry, which a table in shared memory finds, from a sum over the
+// list in its order: the same bits every time (comparing all entries took 1631 us of 4096 x 32768 with 1000 of them, now 300).
 #include <float.h>
 #include <math.h>
 
@@ -35,6 +36,7 @@ struct Distill {
     float temperature, soft, hard;
     float c0, c1;  // log2(e) / T and log2(e)
     unsigned rows, vocab, top, blocks;  // blocks of a row
+    unsigned places;  // of the gradient's table of listed tokens, a power of two
     int accumulate, waves;
 };
 
@@ -103,7 +105,45 @@ struct Entries {
     float *e;    // exp((t - largest t) / T), 0 for the label
     float *z;    // the token's logit
     float *t;    // t - largest t
+    // the gradient's:
+    int *place;  // the token's place in the table
+    int *table;  // the first entry of every token; kAgain: later ones have a part of its probability
 };
+constexpr int kAgain = 1 << 16;
+// Entries that the list's warp puts into the table alone, while the others go through the row; longer lists all threads behind it.  4096 x
+// 32768 with its gradient: 200 entries 196 us alone, 209 by all; 400 entries 230 and 225, and of 64 rows 18 and 13.
+constexpr unsigned kAlone = 256;
+
+// Puts entry j into the table, by open addressing: what is there is an entry of the same token, or another place is tried (the table has
+// half as many places again as entries).  The order in which threads come changes where a token is, not what is found.
+__device__ __forceinline__ void insert(const Entries &entries, unsigned j, unsigned places) {
+    const int token = entries.token[j];
+    if (token < 0) return;
+    unsigned at = unsigned(token) * 0x9e3779b1u >> (__clz(places) + 1);  // the hash's uppermost bits
+    for (;;) {
+        const int there = atomicCAS(&entries.table[at], -1, int(j));
+        if (there < 0) break;
+        if (entries.token[there] == token) {
+            atomicMin(&entries.table[at], int(j));
+            break;
+        }
+        at = (at + 1) & (places - 1);
+    }
+    entries.place[j] = int(at);
+}
+
+// Marks the first entry of entry j's token if that is another one and j's probability is not 0.
+__device__ __forceinline__ void mark(const Entries &entries, unsigned j) {
+    if (entries.token[j] < 0 || entries.e[j] == 0.f) return;
+    int *first = entries.table + entries.place[j];
+    if ((*first & ~kAgain) != int(j)) atomicOr(first, kAgain);
+}
+
+// Copies 4 bytes to shared memory; wait_copies() waits for those of the thread.
+__device__ __forceinline__ void copy_word(void *to, const void *from) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(uint32_t(__cvta_generic_to_shared(to))), "l"(from) : "memory");
+}
+__device__ __forceinline__ void wait_copies() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 // A row as whole 16-byte units, and up to three values in front of the first and behind the last one, which the first block of
 // the row takes, a value a thread.
@@ -134,7 +174,7 @@ constexpr int blocks_of_sm(int threads) { return 65536 / ((threads + 32) * 40); 
 // asked for).  TWO: sums at the temperature and at 1; otherwise one set of sums is both.
 template <int THREADS, bool GRAD, bool TWO>
 __global__ void __launch_bounds__(THREADS + 32, blocks_of_sm(THREADS)) distill_kernel(Distill a) {
-    extern __shared__ float dynamic[];
+    extern __shared__ __align__(16) float dynamic[];
     __shared__ Sums of_warp[THREADS / 32];
     __shared__ Sums of_block[kMostCluster];
     __shared__ float teacher_sum;
@@ -157,23 +197,35 @@ __global__ void __launch_bounds__(THREADS + 32, blocks_of_sm(THREADS)) distill_k
         return;
     }
     if (a.blocks > 1) sm100::cluster_arrive();
-    const unsigned listed = a.top + 1;
-    const Entries entries = {reinterpret_cast<int *>(dynamic), dynamic + listed, dynamic + 2 * listed, dynamic + 3 * listed};
+    const unsigned listed = a.top + 1, array = (listed + 3) & ~3u;  // (tokens are read by 16 bytes)
+    int *const ints = reinterpret_cast<int *>(dynamic);
+    const Entries entries = {ints, dynamic + array, dynamic + 2 * array, dynamic + 3 * array, ints + 4 * array, ints + 5 * array};
     if (warp == THREADS / 32) {
         // ---- the teacher's entries ----
         const int label = a.labels ? a.labels[row] : -1;
+        // (copies, all on their way together: with 1000 entries the loss of 4096 x 32768 took 149 us by loads, 119 by copies)
+        for (unsigned j = lane; j < a.top; j += 32) {
+            copy_word(entries.token + j, a.index + size_t(row) * a.top + j);
+            copy_word(entries.t + j, a.teacher + size_t(row) * a.top + j);
+        }
+        if (GRAD)
+            for (unsigned i = lane; i < a.places; i += 32) entries.table[i] = -1;
+        wait_copies();
         float most = -INFINITY;
         for (unsigned j = lane; j < a.top; j += 32) {
-            const int token = a.index[size_t(row) * a.top + j];
-            const bool there = unsigned(token) < a.vocab;
-            const float t = there ? a.teacher[size_t(row) * a.top + j] : -INFINITY;
-            entries.token[j] = there ? token : -1;
-            entries.z[j] = there ? z[token] : 0.f;
-            entries.t[j] = t;
-            most = fmaxf(most, t);
+            const int token = entries.token[j];
+            if (unsigned(token) < a.vocab) {
+                copy_word(entries.z + j, z + token);
+                most = fmaxf(most, entries.t[j]);
+            } else {
+                entries.token[j] = -1;
+                entries.z[j] = 0.f;
+                entries.t[j] = -INFINITY;
+            }
         }
         most = base_of(largest_of_warp(most));
         float sum = 0.f;
+#pragma unroll 2
         for (unsigned j = lane; j < a.top; j += 32) {
             const float t = entries.t[j] - most, e = entries.token[j] >= 0 ? expf(t / a.temperature) : 0.f;
             entries.t[j] = t;
@@ -187,6 +239,14 @@ __global__ void __launch_bounds__(THREADS + 32, blocks_of_sm(THREADS)) distill_k
             entries.z[a.top] = there ? z[label] : 0.f;
             entries.e[a.top] = 0.f;
             teacher_sum = sum;
+        }
+        if (lane > 0 && a.top + lane < array) entries.token[a.top + lane] = -1;
+        wait_copies();
+        if (GRAD && a.top <= kAlone) {
+            __syncwarp();
+            for (unsigned j = lane; j < listed; j += 32) insert(entries, j, a.places);
+            __syncwarp();
+            for (unsigned j = lane; j < listed; j += 32) mark(entries, j);
         }
     } else {
         // ---- largest value and sums of the row: a thread's own, then the warp's ----
@@ -224,6 +284,8 @@ __global__ void __launch_bounds__(THREADS + 32, blocks_of_sm(THREADS)) distill_k
         if (lane == 0) of_warp[warp] = s;
     }
     __syncthreads();
+    if (GRAD && a.top > kAlone)
+        for (unsigned j = threadIdx.x; j < listed; j += THREADS + 32) insert(entries, j, a.places);
     Sums s = join_lanes<TWO, THREADS / 32>(a, of_warp[lane % (THREADS / 32)]);
     if (a.blocks > 1) {
         sm100::cluster_wait();  // the others run: their shared memory is there
@@ -316,18 +378,25 @@ __global__ void __launch_bounds__(THREADS + 32, blocks_of_sm(THREADS)) distill_k
         }
     }
     __syncthreads();
+    if (a.top > kAlone) {
+        for (unsigned j = threadIdx.x; j < listed; j += THREADS + 32) mark(entries, j);
+        __syncthreads();
+    }
     // listed tokens of this block's part, each by its first entry
     for (unsigned j = threadIdx.x; j < listed; j += THREADS + 32) {
         const unsigned token = unsigned(entries.token[j]);
         if (token >= a.vocab || !part.has(token)) continue;
-        bool first = true;
-        float e = 0.f;
-        for (unsigned i = 0; i < listed; ++i) {
-            if (unsigned(entries.token[i]) != token) continue;
-            first = first && i >= j;
-            e += entries.e[i];
-        }
-        if (!first) continue;
+        const int first = entries.table[entries.place[j]];
+        if ((first & ~kAgain) != int(j)) continue;
+        float e = entries.e[j];
+        if (first & kAgain)
+            for (unsigned i = j & ~3u; i < listed; i += 4) {
+                const int4 four = *reinterpret_cast<const int4 *>(entries.token + i);
+                if (unsigned(four.x) == token && i > j) e += entries.e[i];
+                if (unsigned(four.y) == token && i + 1 > j) e += entries.e[i + 1];
+                if (unsigned(four.z) == token && i + 2 > j) e += entries.e[i + 2];
+                if (unsigned(four.w) == token && i + 3 > j) e += entries.e[i + 3];
+            }
         float d = 0.f;
         if (taught) d = soft * (e / teacher_sum);
         if (token == unsigned(entries.token[a.top])) d += hard;
@@ -338,7 +407,10 @@ __global__ void __launch_bounds__(THREADS + 32, blocks_of_sm(THREADS)) distill_k
 
 template <int THREADS, bool GRAD, bool TWO>
 int32_t launch(katsu_cuda_ctx *ctx, Distill a) {
-    const size_t smem = 4 * sizeof(float) * (size_t(a.top) + 1), blocks = size_t(a.rows) * a.blocks;
+    const size_t listed = size_t(a.top) + 1;
+    a.places = 64;
+    while (2 * a.places < 3 * listed) a.places *= 2;
+    const size_t array = (listed + 3) / 4 * 4, smem = sizeof(float) * (GRAD ? 5 * array + a.places : 4 * array), blocks = size_t(a.rows) * a.blocks;
     if (blocks > 0x7fffffffu) return katsu_set_error(KATSU_ERR_UNSUPPORTED, "%u rows of %u logits in one loss", a.rows, a.vocab);
     const size_t per_sm = std::min<size_t>(blocks_of_sm(THREADS), katsu_shared_per_sm() / (smem + 2048));
     a.waves = blocks > (a.blocks > 1 ? size_t(ctx->num_sms) * 3 / 4 : per_sm * ctx->num_sms);  // (not every group of SMs is filled by clusters)
@@ -407,7 +479,7 @@ extern "C" int32_t katsu_cuda_distill_fwd(katsu_cuda_ctx *ctx, const float *logi
                                           const int32_t *labels, const float *weight, float temperature, float soft, float hard,
                                           float *loss, size_t rows, size_t vocab, size_t top) {
     const Distill a = {logits, teacher, weight, nullptr, index, labels, loss, nullptr, temperature, soft, hard,
-                       0.f, 0.f, unsigned(rows), unsigned(vocab), unsigned(top), 1, 0, 0};
+                       0.f, 0.f, unsigned(rows), unsigned(vocab), unsigned(top), 1, 0, 0, 0};
     KATSU_TRY(check(ctx, a, rows, vocab, top));
     KATSU_REQUIRE(loss != nullptr || rows == 0, "loss is null");
     KATSU_TRY(katsu_bind(ctx));
@@ -419,7 +491,7 @@ extern "C" int32_t katsu_cuda_distill_bwd(katsu_cuda_ctx *ctx, const float *logi
                                           const float *g, float *loss, float *dlogits, size_t rows, size_t vocab, size_t top,
                                           int32_t accumulate) {
     const Distill a = {logits, teacher, weight, g, index, labels, loss, dlogits, temperature, soft, hard,
-                       0.f, 0.f, unsigned(rows), unsigned(vocab), unsigned(top), 1, accumulate != 0, 0};
+                       0.f, 0.f, unsigned(rows), unsigned(vocab), unsigned(top), 1, 0, accumulate != 0, 0};
     KATSU_TRY(check(ctx, a, rows, vocab, top));
     KATSU_REQUIRE(dlogits != nullptr || rows == 0, "dlogits is null");
     KATSU_TRY(katsu_bind(ctx));

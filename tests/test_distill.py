@@ -79,6 +79,31 @@ def test_loss_and_gradient(ctx, rows, vocab, top, T, soft, hard):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("vocab,top", [(1003, 64), (1003, 1000), (4100, 1024), (40001, 1023), (140000, 1024)])
+def test_tokens_listed_many_times(ctx, vocab, top):
+    """A row of one token only, of two tokens in turn, of pairs far apart, of pairs next to each other, of few tokens at random, and one
+    whose places behind the tenth are filled up with a token at a teacher's logit of -infinity."""
+    a = inputs(7, vocab, top, seed=3)
+    rng, j = np.random.default_rng(vocab), np.arange(top)
+    pairs = rng.permutation(vocab)[:top]
+    a["index"] = np.stack([np.full(top, vocab - 1), j % 2, pairs[j % (top // 2)], pairs[j // 2], rng.integers(0, 40, top), np.where(j < 10, j + 5, 7), pairs])
+    a["teacher"][5, 10:] = -np.inf
+    a["labels"] = np.array([vocab - 1, 1, pairs[0], -1, 7, 7, pairs[-1]])
+    a["weight"][:] = 1.5
+    listed = np.stack([np.bincount(i, minlength=vocab) for i in a["index"]])
+    for T, soft, hard in ((1.0, 1.0, 0.0), (2.0, 0.5, 0.5)):
+        want, off, dz, doff = ref.distill(a["z"], a["teacher"], a["index"], a["labels"], a["weight"], T, soft, hard, a["g"])
+        # a token's probability is a sum of as many roundings as it is listed times, of at most 1
+        doff = doff + np.abs(a["g"] * a["weight"])[:, None] * soft * T * ref.U * listed
+        first = run(ctx, a, T, soft, hard)
+        ref.assert_near(first[0], want, off, "loss")
+        ref.assert_near(first[1], want, off, "loss beside the gradient")
+        ref.assert_near(first[2], dz, doff, "gradient")
+        for x, y in zip(first, run(ctx, a, T, soft, hard)):
+            assert np.array_equal(x, y)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("T,hard", [(1.0, 0.0), (2.0, 0.5)])
 @pytest.mark.parametrize("rows,vocab", [(2, 131073), (1, 262150), (1, 400003)])
 def test_rows_that_are_read_twice(ctx, rows, vocab, T, hard):

@@ -299,7 +299,7 @@ int32_t katsu_cuda_embed_fwd(katsu_cuda_ctx *ctx, const float *table, const int3
 int32_t katsu_cuda_int8_embed(katsu_cuda_ctx *ctx, const int8_t *q, const float *rows_scale, const int32_t *tokens,
                               float scale, float *y, size_t count, size_t vocab, size_t cols);
 /* Gradient of the lookup's table: dtable[v] = scale * (sum of dy[i] over all i with tokens[i] == v), in an order that
- * `tokens` alone fixes: the same bits every time.  Rows of other tokens are zeros.  accumulate != 0: added to dtable
+ * the tokens and the sizes alone fix: the same bits every time.  Rows of other tokens are zeros.  accumulate != 0: added to dtable
  * instead, whose other rows are not touched. */
 int32_t katsu_cuda_embed_bwd(katsu_cuda_ctx *ctx, const int32_t *tokens, const float *dy, float scale, float *dtable,
                              size_t count, size_t vocab, size_t cols, int32_t accumulate);

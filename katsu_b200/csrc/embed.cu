@@ -824,8 +824,8 @@ extern "C" int32_t katsu_cuda_embed_bwd(katsu_cuda_ctx *ctx, const int32_t *toke
         return launch_grad_for(ctx, g, whole);
     }
     // A piece is a chain of loads, eight at a time: short ones, as long as their blocks are not more than three rounds.  Where the rows
-    // are many bytes, pieces below 32 write too many sums beside the table.
-    const Width width = width_of(cols, whole ? 4 : kApart);
+    // are many bytes, pieces below 32 write too many sums beside the table.  (Sizes decide, not addresses: the order of the sums is theirs.)
+    const Width width = width_of(cols, cols % 4 ? kApart : 4);
     g.piece = count * cols >= size_t(1) << 22 ? 32 : count <= 4096 ? 8 : 16;
     while (g.piece < kMostPiece && katsu_div_up(katsu_div_up(count, g.piece), kGradThreads >> width.shift) * width.slabs > size_t(16) * ctx->num_sms)
         g.piece *= 2;

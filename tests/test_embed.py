@@ -137,6 +137,13 @@ def test_gradient_at_any_address(ctx, count, vocab, cols, shift):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("count,cols", [(50000, 512), (40000, 260), (20000, 16), (100000, 20)])
+def test_gradient_of_many_tokens_at_any_address(ctx, count, cols):
+    """The same bits, where rows that are whole 16-byte units have other threads than those that are not."""
+    assert np.array_equal(check_grad(ctx, count, 300, cols, "zipf", 1, 0), check_grad(ctx, count, 300, cols, "zipf", 0, 0))
+
+
+@pytest.mark.gpu
 def test_gradient_of_no_tokens(ctx):
     with DeviceArrays(ctx, t=ref.device_ints([-1] * 40), dy=np.ones(160)) as d:
         for count in (0, 40):

@@ -382,6 +382,7 @@ struct Grad {
     float scale;
     unsigned count, vocab, units, slabs, piece, pieces, piece_blocks, fill_rows;
     int shift, fill_shift, waves;
+    unsigned parts;  // of a run that are folded side by side
     bool accumulate, bundles;
     size_t cols, pitch;
 };
@@ -645,40 +646,62 @@ __global__ void __launch_bounds__(kGradThreads) embed_bundle_kernel(Grad g) {
     part.store(g.kept + size_t(first) * 2 * g.pitch, sum);
 }
 
-// Runs of more than one piece: what their first piece kept behind, and what every later one (or bundle) kept in front.
+// Runs of more than one piece: what their first piece kept behind, and what every later one (or bundle) kept in front.  A run has a
+// group of threads, a warp at least: of rows of fewer threads as many neighbouring parts of the run as fit there are added up at once
+// (100 000 x 16: 8 us; 32 where a run had four threads that looked at four pieces at a time).
 template <bool WHOLE, int N, bool ADD>
 __global__ void __launch_bounds__(kGradThreads) embed_fold_kernel(Grad g) {
-    const unsigned width = 1u << g.shift, groups = kGradThreads >> g.shift, lane = threadIdx.x & (width - 1);
+    const int shift = max(g.shift, 5);
+    const unsigned groups = kGradThreads >> shift, lane = threadIdx.x & 31, width = 1u << g.shift;
     if (!g.waves) launch_next();
     launch_wait();
-    const unsigned piece = blockIdx.x / g.slabs * groups + (threadIdx.x >> g.shift);
+    const unsigned piece = blockIdx.x / g.slabs * groups + (threadIdx.x >> shift);
     const unsigned begin = piece * g.piece, next = begin + g.piece;
     if (piece + 1 >= g.pieces) return;
     const unsigned front = begin ? g.keys[begin - 1] : ~0u, first = g.keys[begin], key = g.keys[next - 1], behind = g.keys[next];
     if (key != behind || key >= g.vocab || (front == key && first == key)) return;  // (all threads of the group) not a run that began here and goes on
-    // the pieces that the run passes through whole: the threads of the group that are in one warp look at one each
-    const unsigned looking = min(width, 32u), mask = looking == 32 ? ~0u : ((1u << looking) - 1) << (threadIdx.x & 31 & ~(looking - 1));
-    unsigned last = piece + 1;
+    // the last piece that begins with the token: 32 pieces at a time, from one step to the next 32 times as far, and back
+    unsigned last = piece + 1, step = 1;
+    auto through = [&] {
+        const unsigned long long p = last + (lane + 1ull) * step;
+        return unsigned(__popc(__ballot_sync(~0u, p < g.pieces && g.keys[p * g.piece] == key)));
+    };
+    unsigned far = through();
     for (;;) {
-        const unsigned p = last + (lane & (looking - 1));
-        const bool goes_on = p + 1 < g.pieces && g.keys[(p + 1) * g.piece] == key;
-        const unsigned through = __popc(__ballot_sync(mask, goes_on) & mask);
-        last += through;
-        if (through < looking) break;
+        last += far * step;
+        if (far < 32) break;
+        step *= 32;
+        far = through();
     }
-    const Part<WHOLE, N> part(g, blockIdx.x % g.slabs, lane);
-    if (part.count == 0) return;
+    while (step > 1) {
+        step /= 32;
+        last += through() * step;
+    }
+    const Part<WHOLE, N> part(g, blockIdx.x % g.slabs, threadIdx.x & (width - 1));
+    const unsigned parts = g.parts, mine = parts > 1 ? lane >> g.shift : 0;  // (bundles are of one part)
+    const bool there = part.count != 0 && mine < parts;
+    const unsigned base = g.bundles ? (piece + 1) / kBundle * kBundle : piece + 1, bundle = g.bundles ? kBundle : 1;
+    const unsigned share = ((last - base) / parts / bundle + 1) * bundle;
     float *dst = row_of(g, key);
-    const Values<N> old = ADD ? part.load(dst) : zero_values<N>();
-    Values<N> sum = part.load(g.kept + (size_t(piece) * 2 + 1) * g.pitch);
-    unsigned at = piece + 1;
-    add_kept(g, part, &sum, [&](unsigned *p) {
-        *p = at;
-        const bool bundled = g.bundles && at % kBundle == 0 && (at + kBundle <= last || (at + kBundle - 1 == last && bundle_of_run(g, at, key)));
-        at += bundled ? kBundle : 1;
-        return *p <= last;
-    });
-    write_row<WHOLE, N, ADD>(g, part, dst, sum, old);
+    const Values<N> old = ADD && there && mine == 0 ? part.load(dst) : zero_values<N>();
+    Values<N> sum = there && mine == 0 ? part.load(g.kept + (size_t(piece) * 2 + 1) * g.pitch) : zero_values<N>();
+    unsigned at = max(piece + 1, base + mine * share);
+    const unsigned end = min(last, base + mine * share + share - 1);
+    if (there)
+        add_kept(g, part, &sum, [&](unsigned *p) {
+            *p = at;
+            const bool bundled = g.bundles && at % kBundle == 0 && (at + kBundle <= last || (at + kBundle - 1 == last && bundle_of_run(g, at, key)));
+            at += bundled ? kBundle : 1;
+            return *p <= end;
+        });
+    if (parts > 1)
+        for (unsigned o = parts * width / 2; o >= width; o >>= 1) {
+            Values<N> other;
+#pragma unroll
+            for (int c = 0; c < N; ++c) other.v[c] = __shfl_xor_sync(~0u, sum.v[c], o);
+            add_values(&sum, other);
+        }
+    if (there && mine == 0) write_row<WHOLE, N, ADD>(g, part, dst, sum, old);
 }
 
 // Threads of a group, and slabs of a row, at n values a thread.
@@ -715,15 +738,20 @@ int32_t launch_grad(katsu_cuda_ctx *ctx, Grad g) {
     if (g.tokens) return katsu_launch(ctx, !g.waves, embed_direct_kernel<WHOLE, N, ADD>, unsigned(blocks), kGradThreads, 0, 1, g);
     KATSU_TRY(katsu_launch(ctx, !g.waves, embed_grad_kernel<WHOLE, N, ADD>, unsigned(blocks), kGradThreads, (2 * groups * g.piece + 2) * sizeof(unsigned), 1, g));
     if (g.pieces == 1) return KATSU_OK;
-    // (below 512 pieces a run's fold is short beside another launch)
-    g.bundles = g.pieces >= 512;
+    // (below 512 pieces for each part of a run its fold is short beside another launch)
+    const int fold_shift = std::max(g.shift, 5);
+    g.parts = 32u >> std::min(5, width_of(g.cols, kApart).shift);  // (as many as rows of either kind have: the order is that of sizes)
+    g.bundles = g.pieces >= 512 * g.parts;
     if (g.bundles) {
         const size_t bundle_blocks = katsu_div_up(katsu_div_up(g.pieces, kBundle), groups) * g.slabs;
         g.waves = bundle_blocks > resident;
         KATSU_TRY(katsu_launch(ctx, !g.waves, embed_bundle_kernel<WHOLE, N>, unsigned(bundle_blocks), kGradThreads, 0, 1, g));
     }
-    g.waves = piece_blocks > resident;
-    return katsu_launch(ctx, !g.waves, embed_fold_kernel<WHOLE, N, ADD>, g.piece_blocks, kGradThreads, 0, 1, g);
+    const size_t fold_blocks = katsu_div_up(g.pieces, size_t(kGradThreads) >> fold_shift) * g.slabs;
+    if (fold_blocks > 0x7fffffffu)
+        return katsu_set_error(KATSU_ERR_UNSUPPORTED, "%u tokens with rows of %zu values in one gradient", g.count, g.cols);
+    g.waves = fold_blocks > resident;
+    return katsu_launch(ctx, !g.waves, embed_fold_kernel<WHOLE, N, ADD>, unsigned(fold_blocks), kGradThreads, 0, 1, g);
 }
 
 int32_t launch_grad_for(katsu_cuda_ctx *ctx, const Grad &g, bool whole) {

@@ -21,6 +21,7 @@
 
 #include "common.cuh"
 #include "launch.cuh"
+#include "listed.cuh"
 #include "sm100_pair.cuh"
 
 namespace {
@@ -105,39 +106,10 @@ struct Entries {
     float *e;    // exp((t - largest t) / T), 0 for the label
     float *z;    // the token's logit
     float *t;    // t - largest t
-    // the gradient's:
-    int *place;  // the token's place in the table
-    int *table;  // the first entry of every token; kAgain: later ones have a part of its probability
 };
-constexpr int kAgain = 1 << 16;
 // Entries that the list's warp puts into the table alone, while the others go through the row; longer lists all threads behind it.  4096 x
 // 32768 with its gradient: 200 entries 196 us alone, 209 by all; 400 entries 230 and 225, and of 64 rows 18 and 13.
 constexpr unsigned kAlone = 256;
-
-// Puts entry j into the table, by open addressing: what is there is an entry of the same token, or another place is tried (the table has
-// half as many places again as entries).  The order in which threads come changes where a token is, not what is found.
-__device__ __forceinline__ void insert(const Entries &entries, unsigned j, unsigned places) {
-    const int token = entries.token[j];
-    if (token < 0) return;
-    unsigned at = unsigned(token) * 0x9e3779b1u >> (__clz(places) + 1);  // the hash's uppermost bits
-    for (;;) {
-        const int there = atomicCAS(&entries.table[at], -1, int(j));
-        if (there < 0) break;
-        if (entries.token[there] == token) {
-            atomicMin(&entries.table[at], int(j));
-            break;
-        }
-        at = (at + 1) & (places - 1);
-    }
-    entries.place[j] = int(at);
-}
-
-// Marks the first entry of entry j's token if that is another one and j's probability is not 0.
-__device__ __forceinline__ void mark(const Entries &entries, unsigned j) {
-    if (entries.token[j] < 0 || entries.e[j] == 0.f) return;
-    int *first = entries.table + entries.place[j];
-    if ((*first & ~kAgain) != int(j)) atomicOr(first, kAgain);
-}
 
 // Copies 4 bytes to shared memory; wait_copies() waits for those of the thread.
 __device__ __forceinline__ void copy_word(void *to, const void *from) {
@@ -199,7 +171,8 @@ __global__ void __launch_bounds__(THREADS + 32, blocks_of_sm(THREADS)) distill_k
     if (a.blocks > 1) sm100::cluster_arrive();
     const unsigned listed = a.top + 1, array = (listed + 3) & ~3u;  // (tokens are read by 16 bytes)
     int *const ints = reinterpret_cast<int *>(dynamic);
-    const Entries entries = {ints, dynamic + array, dynamic + 2 * array, dynamic + 3 * array, ints + 4 * array, ints + 5 * array};
+    const Entries entries = {ints, dynamic + array, dynamic + 2 * array, dynamic + 3 * array};
+    const Listed tokens = {ints, ints + 4 * array, ints + 5 * array, a.places, listed};  // (the gradient's)
     if (warp == THREADS / 32) {
         // ---- the teacher's entries ----
         const int label = a.labels ? a.labels[row] : -1;
@@ -209,7 +182,7 @@ __global__ void __launch_bounds__(THREADS + 32, blocks_of_sm(THREADS)) distill_k
             copy_word(entries.t + j, a.teacher + size_t(row) * a.top + j);
         }
         if (GRAD)
-            for (unsigned i = lane; i < a.places; i += 32) entries.table[i] = -1;
+            for (unsigned i = lane; i < a.places; i += 32) tokens.table[i] = -1;
         wait_copies();
         float most = -INFINITY;
         for (unsigned j = lane; j < a.top; j += 32) {
@@ -244,9 +217,9 @@ __global__ void __launch_bounds__(THREADS + 32, blocks_of_sm(THREADS)) distill_k
         wait_copies();
         if (GRAD && a.top <= kAlone) {
             __syncwarp();
-            for (unsigned j = lane; j < listed; j += 32) insert(entries, j, a.places);
+            for (unsigned j = lane; j < listed; j += 32) tokens.insert(j);
             __syncwarp();
-            for (unsigned j = lane; j < listed; j += 32) mark(entries, j);
+            for (unsigned j = lane; j < listed; j += 32) tokens.mark(j, entries.e[j]);
         }
     } else {
         // ---- largest value and sums of the row: a thread's own, then the warp's ----
@@ -285,7 +258,7 @@ __global__ void __launch_bounds__(THREADS + 32, blocks_of_sm(THREADS)) distill_k
     }
     __syncthreads();
     if (GRAD && a.top > kAlone)
-        for (unsigned j = threadIdx.x; j < listed; j += THREADS + 32) insert(entries, j, a.places);
+        for (unsigned j = threadIdx.x; j < listed; j += THREADS + 32) tokens.insert(j);
     Sums s = join_lanes<TWO, THREADS / 32>(a, of_warp[lane % (THREADS / 32)]);
     if (a.blocks > 1) {
         sm100::cluster_wait();  // the others run: their shared memory is there
@@ -379,26 +352,16 @@ __global__ void __launch_bounds__(THREADS + 32, blocks_of_sm(THREADS)) distill_k
     }
     __syncthreads();
     if (a.top > kAlone) {
-        for (unsigned j = threadIdx.x; j < listed; j += THREADS + 32) mark(entries, j);
+        for (unsigned j = threadIdx.x; j < listed; j += THREADS + 32) tokens.mark(j, entries.e[j]);
         __syncthreads();
     }
     // listed tokens of this block's part, each by its first entry
     for (unsigned j = threadIdx.x; j < listed; j += THREADS + 32) {
         const unsigned token = unsigned(entries.token[j]);
         if (token >= a.vocab || !part.has(token)) continue;
-        const int first = entries.table[entries.place[j]];
-        if ((first & ~kAgain) != int(j)) continue;
-        float e = entries.e[j];
-        if (first & kAgain)
-            for (unsigned i = j & ~3u; i < listed; i += 4) {
-                const int4 four = *reinterpret_cast<const int4 *>(entries.token + i);
-                if (unsigned(four.x) == token && i > j) e += entries.e[i];
-                if (unsigned(four.y) == token && i + 1 > j) e += entries.e[i + 1];
-                if (unsigned(four.z) == token && i + 2 > j) e += entries.e[i + 2];
-                if (unsigned(four.w) == token && i + 3 > j) e += entries.e[i + 3];
-            }
+        if (!tokens.is_first(j)) continue;
         float d = 0.f;
-        if (taught) d = soft * (e / teacher_sum);
+        if (taught) d = soft * (tokens.sum(j, entries.e) / teacher_sum);
         if (token == unsigned(entries.token[a.top])) d += hard;
         if (a.accumulate) dz[token] -= d;
         else dz[token] = slope(entries.z[j]) - d;
@@ -408,8 +371,7 @@ __global__ void __launch_bounds__(THREADS + 32, blocks_of_sm(THREADS)) distill_k
 template <int THREADS, bool GRAD, bool TWO>
 int32_t launch(katsu_cuda_ctx *ctx, Distill a) {
     const size_t listed = size_t(a.top) + 1;
-    a.places = 64;
-    while (2 * a.places < 3 * listed) a.places *= 2;
+    a.places = listed_places(listed);
     const size_t array = (listed + 3) / 4 * 4, smem = sizeof(float) * (GRAD ? 5 * array + a.places : 4 * array), blocks = size_t(a.rows) * a.blocks;
     if (blocks > 0x7fffffffu) return katsu_set_error(KATSU_ERR_UNSUPPORTED, "%u rows of %u logits in one loss", a.rows, a.vocab);
     const size_t per_sm = std::min<size_t>(blocks_of_sm(THREADS), katsu_shared_per_sm() / (smem + 2048));

@@ -4,20 +4,24 @@
 //
 // Bound: HBM, logits in (of allowed tokens) and out; few rows: a chain of loads.  A block has a slice of a row: it counts the
 // history's tokens of its slice in shared memory (whole numbers: atomics in any order give the same counts) while the slice's
-// logits are on their way, and writes the slice once.  Tokens with biases, a few of a row, are written again behind it from the
-// row's list in its order.  In place only what changes is read and written.  512 x 100003: 73 us, 5.6 TB/s; 64 x 131072 with histories of
-// 4096 tokens 18 us, 14 of them without a history; under a grammar, with biases, 21.
+// logits are on their way, and writes the slice once.  Tokens with biases, a few of a row, are written again behind it, by a token's
+// first entry, with the sum over the row's list in its order.  In place only what changes is read and written.  512 x 100003: 65 us without
+// a history, 6.3 TB/s; 64 x 131072 with histories of 4096 tokens 18 us, 14 without; under a grammar, with biases, 21.
 #include <math.h>
 
 #include <algorithm>
 
 #include "common.cuh"
 #include "launch.cuh"
+#include "listed.cuh"
 
 namespace {
 
 constexpr int kThreads = 256, kBlocks = 4;  // blocks of an SM
 constexpr int kHeld = 4, kAhead = 8;        // 16-byte accesses of a thread, and tokens of the history, on their way together
+// Biases of a row above which a token's first entry is found by a table, in a kernel of its own: 64 x 131072 with histories of 4096 tokens,
+// 150 biases 23 us by comparing all entries and 24 by a table, 300 39 and 31, 1000 211 and 62.
+constexpr unsigned kCompared = 200;
 constexpr unsigned kStep = 4 * kThreads, kMostSlice = 16 * kStep, kEdge = 8;  // kEdge: places for the edge
 
 struct Adjust {
@@ -27,6 +31,7 @@ struct Adjust {
     float *out;
     unsigned rows, vocab, history_cols, biases, words, slices;
     unsigned slice, places, masks;  // tokens of a block, a multiple of kStep; words of its places and of its part of the mask
+    unsigned listed, firsts;        // words of a list of the biases, and of the table of their first entries
     int waves;
 };
 
@@ -66,7 +71,8 @@ struct Place {
     }
 };
 
-template <bool WIDE>
+// TABLE: many biases
+template <bool WIDE, bool TABLE>
 __global__ void __launch_bounds__(kThreads, kBlocks) adjust_kernel(Adjust a) {
     using P = Place<WIDE>;
     extern __shared__ __align__(16) unsigned seen[];  // the places; the slice's words of the mask; the row's biases
@@ -119,8 +125,13 @@ __global__ void __launch_bounds__(kThreads, kBlocks) adjust_kernel(Adjust a) {
     };
     ask(4 * threadIdx.x);
     // ---- the history's tokens and the biases of the slice ----
-    float *bias = reinterpret_cast<float *>(mask + a.masks), *bias_z = bias + a.biases;
-    int *bias_tokens = reinterpret_cast<int *>(bias_z + a.biases);
+    float *bias = reinterpret_cast<float *>(mask + a.masks), *bias_z = bias + a.listed;
+    int *bias_tokens = reinterpret_cast<int *>(bias_z + a.listed);
+    const Listed tokens = {bias_tokens, bias_tokens + a.listed, bias_tokens + 2 * a.listed, a.firsts, a.biases};
+    if (TABLE) {
+        for (unsigned i = threadIdx.x; i < a.firsts; i += kThreads) tokens.table[i] = -1;
+        if (threadIdx.x < a.listed - a.biases) bias_tokens[a.biases + threadIdx.x] = -1;
+    }
     for (unsigned j = threadIdx.x; j < a.biases; j += kThreads) {
         const unsigned token = unsigned(a.bias_tokens[size_t(row) * a.biases + j]);
         const bool mine = place_of(token) != ~0u;
@@ -157,6 +168,8 @@ __global__ void __launch_bounds__(kThreads, kBlocks) adjust_kernel(Adjust a) {
         }
     }
     if (history || a.biases) __syncthreads();
+    if (TABLE)
+        for (unsigned j = threadIdx.x; j < a.biases; j += kThreads) tokens.insert(j);
     // ---- the edge, and the slice ----
     auto is_allowed = [&](unsigned token) { return !words || (words[token >> 5] >> (token & 31) & 1u); };
     if (threadIdx.x < edge) {
@@ -202,34 +215,45 @@ __global__ void __launch_bounds__(kThreads, kBlocks) adjust_kernel(Adjust a) {
     }
     if (a.biases == 0) return;
     __syncthreads();
+    if (TABLE) {
+        for (unsigned j = threadIdx.x; j < a.biases; j += kThreads) tokens.mark(j, bias[j]);
+        __syncthreads();
+    }
     for (unsigned j = threadIdx.x; j < a.biases; j += kThreads) {
         const int token = bias_tokens[j];
         if (token < 0 || !is_allowed(unsigned(token))) continue;
         bool first = true;
         float sum = 0.f;
-        for (unsigned i = 0; i < a.biases; ++i) {
-            if (bias_tokens[i] != token) continue;
-            first = first && i >= j;
-            sum += bias[i];
+        if (TABLE) {
+            first = tokens.is_first(j);
+            if (first) sum += tokens.sum(j, bias);
+        } else {
+            for (unsigned i = 0; i < a.biases; ++i) {
+                if (bias_tokens[i] != token) continue;
+                first = first && i >= j;
+                sum += bias[i];
+            }
         }
         if (first) out[token] = (history ? P::penalised(bias_z[j], P::one(seen, place_of(unsigned(token))), p) : bias_z[j]) + sum;
     }
 }
 
-template <bool WIDE>
+template <bool WIDE, bool TABLE>
 int32_t launch(katsu_cuda_ctx *ctx, Adjust a) {
     // One round of blocks, as every block looks at the row's whole history; slices are bounded by the shared memory for their places.
     const size_t resident = size_t(kBlocks) * ctx->num_sms, wanted = std::max<size_t>(1, resident / a.rows);
     a.slice = unsigned(std::min<size_t>(kMostSlice, katsu_div_up(katsu_div_up(a.vocab, wanted), kStep) * kStep));
     a.slices = unsigned(katsu_div_up(a.vocab, a.slice));
     a.places = !a.history ? 0 : WIDE ? a.slice + kEdge : (a.slice + kEdge) / 2;
-    a.masks = a.allowed ? a.slice / 32 + 2 : 0;
-    const size_t blocks = size_t(a.rows) * a.slices, smem = 4 * (size_t(a.places) + a.masks + 3 * size_t(a.biases));
+    a.masks = a.allowed ? a.slice / 32 + (TABLE ? 4 : 2) : 0;
+    a.listed = TABLE ? (a.biases + 3) / 4 * 4 : a.biases;  // (the table's tokens are read by 16 bytes)
+    a.firsts = TABLE ? listed_places(a.biases) : 0;
+    const size_t blocks = size_t(a.rows) * a.slices, smem = 4 * (size_t(a.places) + a.masks + (TABLE ? 4 : 3) * size_t(a.listed) + a.firsts);
     if (blocks > 0x7fffffffu) return katsu_set_error(KATSU_ERR_UNSUPPORTED, "%u rows of %u logits in one call", a.rows, a.vocab);
-    KATSU_TRY(katsu_prepare_kernel(ctx, reinterpret_cast<const void *>(adjust_kernel<WIDE>), smem, false));
+    KATSU_TRY(katsu_prepare_kernel(ctx, reinterpret_cast<const void *>(adjust_kernel<WIDE, TABLE>), smem, false));
     const size_t per_sm = std::min<size_t>(kBlocks, katsu_shared_per_sm() / (smem + 1024));
     a.waves = blocks > per_sm * ctx->num_sms;
-    return katsu_launch(ctx, !a.waves, adjust_kernel<WIDE>, unsigned(blocks), kThreads, smem, 1, a);
+    return katsu_launch(ctx, !a.waves, adjust_kernel<WIDE, TABLE>, unsigned(blocks), kThreads, smem, 1, a);
 }
 
 }  // namespace
@@ -258,7 +282,8 @@ extern "C" int32_t katsu_cuda_adjust_logits(katsu_cuda_ctx *ctx, const float *lo
     }
     KATSU_TRY(katsu_bind(ctx));
     const Adjust a = {logits, repetition, presence, frequency, bias, history_cols ? history : nullptr, prompts, lengths, bias_tokens, allowed, out,
-                      unsigned(rows), unsigned(vocab), unsigned(history_cols), unsigned(biases), unsigned(words), 0, 0, 0, 0, 0};
+                      unsigned(rows), unsigned(vocab), unsigned(history_cols), unsigned(biases), unsigned(words), 0, 0, 0, 0, 0, 0, 0};
     const bool wide = history_cols >= 1 << 15;
-    return wide ? launch<true>(ctx, a) : launch<false>(ctx, a);
+    if (biases > kCompared) return wide ? launch<true, true>(ctx, a) : launch<false, true>(ctx, a);
+    return wide ? launch<true, false>(ctx, a) : launch<false, false>(ctx, a);
 }

@@ -102,6 +102,21 @@ def test_parts_that_are_left_out(ctx, without):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("vocab,biases", [(1003, 5), (1003, 1000), (9000, 1024), (140001, 1021)])
+@pytest.mark.parametrize("cols,allowed", [(0, None), (50, 0.7)])
+def test_tokens_with_many_biases(ctx, vocab, biases, cols, allowed):
+    """A row of one token only, of two in turn, of pairs far apart and of pairs next to each other, of few tokens at random with biases of 0
+    among them, and of different tokens."""
+    a = inputs(6, vocab, cols, biases, allowed, seed=8)
+    rng, j = np.random.default_rng(vocab), np.arange(biases)
+    some = np.resize(rng.permutation(vocab), biases)
+    a["bias_tokens"] = np.stack([np.full(biases, vocab - 1), j % 2, some[j % (biases // 2)], some[j // 2], rng.integers(0, 40, biases), some])
+    a["bias"][4, ::3] = 0.0
+    got = check(ctx, a)
+    assert np.array_equal(got, check(ctx, a, in_place=True)) and np.array_equal(got, check(ctx, a, shift=3))
+
+
+@pytest.mark.gpu
 def test_untouched_logits_keep_their_bits(ctx):
     bits = np.random.default_rng(4).integers(0, 2 ** 32, (3, 5000), dtype=np.uint32)
     a = inputs(3, 5000, 40, 0, None)

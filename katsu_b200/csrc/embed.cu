@@ -646,6 +646,45 @@ __global__ void __launch_bounds__(kGradThreads) embed_bundle_kernel(Grad g) {
     part.store(g.kept + size_t(first) * 2 * g.pitch, sum);
 }
 
+// Threads of a group, and slabs of a row, at n values a thread.
+struct Width {
+    unsigned units, slabs;
+    int shift;
+};
+
+constexpr Width width_of(size_t cols, size_t n) {
+    Width w = {unsigned((cols + n - 1) / n), 1, 2};
+    while ((1 << w.shift) < kGradThreads && (1u << w.shift) < w.units) ++w.shift;
+    w.slabs = (w.units + (1u << w.shift) - 1) >> w.shift;
+    return w;
+}
+
+// Parts of a run that its fold's warp adds up side by side: as many as rows of either kind have groups in a warp (the order is that of
+// sizes).  A lane takes part fold_part(lane, shift), and none where that is not below the parts: rows that are whole 16-byte units have
+// groups of half the size.
+constexpr unsigned fold_parts(size_t cols) { return 32u >> std::min(5, width_of(cols, kApart).shift); }
+__host__ __device__ constexpr unsigned fold_part(unsigned lane, int shift) { return lane >> shift; }
+
+// Every value of a part of a run has one lane, whatever rows of up to a warp's width are, and there is a lane for all of them.
+constexpr bool folds_each_value_once(size_t cols, size_t n) {
+    const Width width = width_of(cols, n);
+    for (unsigned part = 0; part < fold_parts(cols); ++part)
+        for (unsigned unit = 0; unit < width.units; ++unit) {
+            int lanes = 0;
+            for (unsigned lane = 0; lane < 32; ++lane)
+                lanes += fold_part(lane, width.shift) == part && (lane & ((1u << width.shift) - 1)) == unit;
+            if (lanes != 1) return false;
+        }
+    return true;
+}
+
+constexpr bool folds_of_a_warp_are_right() {
+    for (size_t cols = 1; cols <= 32 * kApart; ++cols)
+        if (!folds_each_value_once(cols, kApart) || (cols % 4 == 0 && !folds_each_value_once(cols, 4))) return false;
+    return true;
+}
+static_assert(folds_of_a_warp_are_right(), "a value of a run is folded by one lane");
+
 // Runs of more than one piece: what their first piece kept behind, and what every later one (or bundle) kept in front.  A run has a
 // group of threads, a warp at least: of rows of fewer threads as many neighbouring parts of the run as fit there are added up at once
 // (100 000 x 16: 8 us; 32 where a run had four threads that looked at four pieces at a time).
@@ -678,7 +717,7 @@ __global__ void __launch_bounds__(kGradThreads) embed_fold_kernel(Grad g) {
         last += through() * step;
     }
     const Part<WHOLE, N> part(g, blockIdx.x % g.slabs, threadIdx.x & (width - 1));
-    const unsigned parts = g.parts, mine = parts > 1 ? lane >> g.shift : 0;  // (bundles are of one part)
+    const unsigned parts = g.parts, mine = fold_part(lane, g.shift);
     const bool there = part.count != 0 && mine < parts;
     const unsigned base = g.bundles ? (piece + 1) / kBundle * kBundle : piece + 1, bundle = g.bundles ? kBundle : 1;
     const unsigned share = ((last - base) / parts / bundle + 1) * bundle;
@@ -704,19 +743,6 @@ __global__ void __launch_bounds__(kGradThreads) embed_fold_kernel(Grad g) {
     if (there && mine == 0) write_row<WHOLE, N, ADD>(g, part, dst, sum, old);
 }
 
-// Threads of a group, and slabs of a row, at n values a thread.
-struct Width {
-    unsigned units, slabs;
-    int shift;
-};
-
-Width width_of(size_t cols, size_t n) {
-    Width w = {unsigned(katsu_div_up(cols, n)), 1, 2};
-    while ((1 << w.shift) < kGradThreads && (1u << w.shift) < w.units) ++w.shift;
-    w.slabs = (w.units + (1u << w.shift) - 1) >> w.shift;
-    return w;
-}
-
 template <bool WHOLE, int N, bool ADD>
 int32_t launch_grad(katsu_cuda_ctx *ctx, Grad g) {
     const Width width = width_of(g.cols, N);
@@ -740,7 +766,7 @@ int32_t launch_grad(katsu_cuda_ctx *ctx, Grad g) {
     if (g.pieces == 1) return KATSU_OK;
     // (below 512 pieces for each part of a run its fold is short beside another launch)
     const int fold_shift = std::max(g.shift, 5);
-    g.parts = 32u >> std::min(5, width_of(g.cols, kApart).shift);  // (as many as rows of either kind have: the order is that of sizes)
+    g.parts = fold_parts(g.cols);
     g.bundles = g.pieces >= 512 * g.parts;
     if (g.bundles) {
         const size_t bundle_blocks = katsu_div_up(katsu_div_up(g.pieces, kBundle), groups) * g.slabs;

@@ -421,14 +421,15 @@ int32_t check(const katsu_cuda_ctx *ctx, const Distill &a, size_t rows, size_t v
     const struct {
         const void *p;
         size_t bytes;
-    } in[] = {{a.teacher, 4 * rows * top}, {a.index, 4 * rows * top}, {a.labels, 4 * rows}, {a.weight, 4 * rows}, {a.g, 4 * rows},
-              {a.logits, 4 * rows * vocab}}, out[] = {{a.loss, 4 * rows}, {a.dlogits, 4 * rows * vocab}};
+    } in[] = {{a.logits, 4 * rows * vocab}, {a.teacher, 4 * rows * top}, {a.index, 4 * rows * top}, {a.labels, 4 * rows}, {a.weight, 4 * rows},
+              {a.g, 4 * rows}}, out[] = {{a.dlogits, 4 * rows * vocab}, {a.loss, 4 * rows}};
     for (const auto &o : out) {
         KATSU_REQUIRE(katsu_whole(o.p), "an address is not that of a whole element");
         for (const auto &i : in) {
+            // the logits' place: of the gradient and these two operands alone, whatever else is at their address
+            const bool in_place = &o == out && &i == in && o.p == i.p && !a.accumulate;
             KATSU_REQUIRE(katsu_whole(i.p), "an address is not that of a whole element");
-            KATSU_REQUIRE((o.p == a.dlogits && i.p == a.logits && o.p == i.p && !a.accumulate) || !katsu_overlap(o.p, o.bytes, i.p, i.bytes),
-                          "an output is an input too, or overlaps one");
+            KATSU_REQUIRE(in_place || !katsu_overlap(o.p, o.bytes, i.p, i.bytes), "an output is an input too, or overlaps one");
         }
     }
     KATSU_REQUIRE(!katsu_overlap(out[0].p, out[0].bytes, out[1].p, out[1].bytes), "loss and dlogits overlap");

@@ -278,7 +278,8 @@ extern "C" int32_t katsu_cuda_adjust_logits(katsu_cuda_ctx *ctx, const float *lo
               {presence, 4 * rows}, {frequency, 4 * rows}, {bias_tokens, 4 * rows * biases}, {bias, 4 * rows * biases}, {allowed, 4 * rows * words}};
     for (const auto &i : in) {
         KATSU_REQUIRE(katsu_whole(i.p) && katsu_whole(out), "an address is not that of a whole element");
-        KATSU_REQUIRE((i.p == logits && out == logits) || !katsu_overlap(out, bytes, i.p, i.bytes), "out overlaps an input");
+        // (out may be the logits' place: of this operand alone, whatever else is at their address)
+        KATSU_REQUIRE((&i == in && out == logits) || !katsu_overlap(out, bytes, i.p, i.bytes), "out overlaps an input");
     }
     KATSU_TRY(katsu_bind(ctx));
     const Adjust a = {logits, repetition, presence, frequency, bias, history_cols ? history : nullptr, prompts, lengths, bias_tokens, allowed, out,

@@ -719,17 +719,22 @@ class DistillLoss:
 
 def adjust_logits(logits, history=None, lengths=None, prompts=None, repetition=None, presence=None, frequency=None, bias_tokens=None,
                   bias=None, allowed=None):
-    """Logits [rows, vocab] (or [vocab]) as a server changes them before it picks a token, as a new leaf.
+    """Logits [rows, vocab] (or [vocab], one row) as a server changes them before it picks a token, as a new leaf.
 
-    history [rows, n]: tokens, of which lengths [rows] are a row's (all) and the first prompts [rows] of these its prompt (none);
-    repetition divides positive and multiplies other logits of its tokens, frequency * count + presence is taken off those of
-    generated ones (numbers, or one for every row); bias_tokens and bias [rows, n]: values to be added; allowed [rows, vocab]:
-    where it is not true the logit becomes -infinity, whatever it was."""
+    history [rows, n] (of one row also [n], as the biases): tokens, of which lengths [rows] are a row's (all) and the first prompts
+    [rows] of these its prompt (none); repetition divides positive and multiplies other logits of its tokens, frequency * count +
+    presence is taken off those of generated ones (numbers, or one for every row); bias_tokens and bias [rows, n]: values to be added;
+    allowed [rows, vocab]: where it is not true the logit becomes -infinity, whatever it was."""
     lib, out, shape = _load(), _vp(), logits.shape()
     rows = 1 if len(shape) == 1 else shape[0] if shape else 0
 
     def per_row(v):
         return np.zeros(0, np.float32) if v is None else np.ascontiguousarray(np.full(rows, v) if np.ndim(v) == 0 else v, dtype=np.float32).reshape(-1)
+
+    def of_rows(v, what):
+        if v.size and len(shape) in (1, 2) and not (v.shape[:-1] == (rows,) or (v.ndim < 2 and rows == 1)):
+            raise InvalidOperand(f"invalid operand: {what} must be [{rows}, n], a list for every row of logits, got {list(v.shape)}")
+        return v
 
     none = np.zeros(0, np.int32)
     words = none
@@ -741,10 +746,10 @@ def adjust_logits(logits, history=None, lengths=None, prompts=None, repetition=N
         bits = np.zeros((rows, (allowed.shape[1] + 31) // 32 * 32), bool)
         bits[:, : allowed.shape[1]] = allowed
         words = np.ascontiguousarray(np.packbits(bits, axis=1, bitorder="little")).view("<u4")
-    arrays = [none if history is None else _whole(history, "history"), none if prompts is None else _whole(prompts, "prompts"),
+    arrays = [none if history is None else of_rows(_whole(history, "history"), "history"), none if prompts is None else _whole(prompts, "prompts"),
               none if lengths is None else _whole(lengths, "lengths"), per_row(repetition), per_row(presence), per_row(frequency),
-              none if bias_tokens is None else _whole(bias_tokens, "bias_tokens"),
-              np.zeros(0, np.float32) if bias is None else np.ascontiguousarray(bias, dtype=np.float32).reshape(-1), words]
+              none if bias_tokens is None else of_rows(_whole(bias_tokens, "bias_tokens"), "bias_tokens"),
+              np.zeros(0, np.float32) if bias is None else of_rows(np.asarray(bias, dtype=np.float32, order="C"), "bias"), words]
     _check(lib.kh_adjust_logits(logits._h, *(x for a in arrays for x in (a.ctypes.data, a.size)), ctypes.byref(out)))
     return Tensor._wrap(out.value)
 

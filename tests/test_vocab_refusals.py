@@ -1,6 +1,10 @@
-"""Calls at a language model's two ends that have to be refused: outputs in the place of an input that is not the logits."""
+"""Calls at a language model's two ends that have to be refused: outputs in the place of an input that is not the logits, lists of other
+axes than the rows that they are for."""
+import numpy as np
 import pytest
 
+import katsu_b200 as K
+import vocab_ref as ref
 from katsu_b200 import cabi
 from test_adjust_logits import BASE as LOGITS
 from test_adjust_logits import NAMES as LOGITS_NAMES
@@ -24,3 +28,41 @@ def test_logits_adjusted_in_place_and_in_that_of_another_input(anywhere, other):
     lib = cabi.load()
     assert lib.katsu_cuda_adjust_logits(anywhere, *(args[n] for n in LOGITS_NAMES)) == cabi.ERR_INVALID_ARG
     assert "overlaps" in lib.katsu_cuda_last_error_string().decode()
+
+
+LISTS = {"history": lambda *shape: {"history": np.zeros(shape, int)},
+         "biases": lambda *shape: {"bias_tokens": np.zeros(shape, int), "bias": np.zeros(shape)}}
+
+
+@pytest.mark.parametrize("of", LISTS.values(), ids=LISTS)
+@pytest.mark.parametrize("shape", [(100,), (1, 100), (100, 1), (8, 4), (2, 8), (4,), (4, 3, 2), (2, 2, 3), (1, 4, 5)], ids=str)
+def test_lists_that_are_not_a_row_of_logits_each(of, shape):
+    """One list for all rows, a transposed one, or more axes: their sizes divide by the rows."""
+    with pytest.raises(K.InvalidOperand, match="a list for every row"):
+        K.adjust_logits(K.Tensor.zeros([4, 9]), **of(*shape))
+
+
+@pytest.mark.parametrize("logits,shape", [([9], (2, 3)), ([9], (3, 1)), ([1, 9], (3, 1)), ([1, 9], (1, 1, 3))], ids=str)
+def test_lists_of_other_rows_than_the_one(logits, shape):
+    for of in LISTS.values():
+        with pytest.raises(K.InvalidOperand, match="a list for every row"):
+            K.adjust_logits(K.Tensor.zeros(logits), **of(*shape))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("logits", [[50], [1, 50]], ids=str)
+@pytest.mark.parametrize("shape", [(7,), (1, 7)], ids=str)
+def test_lists_of_one_row(logits, shape):
+    rng = np.random.default_rng(2)
+    z, history, tokens, bias = (rng.standard_normal(50).astype(np.float32), rng.integers(0, 50, 7), rng.integers(0, 50, 7),
+                                rng.standard_normal(7).astype(np.float32))
+    got = K.adjust_logits(K.Tensor(z, logits), history.reshape(shape), repetition=1.5, bias_tokens=tokens.reshape(shape), bias=bias.reshape(shape))
+    ref.assert_near(got.data(), *ref.adjust(z[None], history[None], None, None, np.float32([1.5]), None, None, tokens[None], bias[None], None))
+
+
+@pytest.mark.gpu
+def test_lists_of_nothing():
+    z = np.arange(12, dtype=np.float32)
+    for empty in ([], np.zeros((3, 0), int), np.zeros((0, 5), int)):
+        got = K.adjust_logits(K.Tensor(z, [3, 4]), history=empty, bias_tokens=empty, bias=empty)
+        assert np.array_equal(got.data(), z)

@@ -670,6 +670,18 @@ def _token_args(tokens):
     return array.ctypes.data, array.size, dims, rank, array
 
 
+def _in_order(values, axes, what):
+    """`values`, unless they are as many as `axes` have but lie in another order than these: of other axes than result from putting
+    neighbouring ones together on either side.  (Other numbers of them are the library's to refuse.)"""
+    def ends(shape):  # how many values a step along each axis passes
+        return set(np.cumprod([1, *reversed(shape)]).tolist())
+
+    mine, theirs = ends(values.shape), ends(axes)
+    if values.size and max(mine) == max(theirs) and not (mine <= theirs or theirs <= mine):
+        raise InvalidOperand(f"invalid operand: {what} must have the axes {list(axes)}, got {list(values.shape)}")
+    return values
+
+
 class Embedding:
     """scale * table[token] for tokens of any shape, and the gradient of the table [vocab, cols].  A negative token (padding) is a
     row of zeros without a gradient."""
@@ -709,9 +721,12 @@ class DistillLoss:
 
     def forward(self, logits, teacher=None, index=None, labels=None, weight=None):
         """A Tensor [...].  teacher: a Tensor [..., top] of logits, index: their tokens (negative: left out); labels: a token for
-        every row (negative: none); weight: a Tensor with a value for every row.  The gradient reaches the logits alone."""
+        every row (negative: none); weight: a Tensor with a value for every row.  Each has the axes of the logits' rows, or these put
+        together ([rows]) or apart.  The gradient reaches the logits alone."""
         out = _vp()
         indices, labels = _whole([] if index is None else index, "index"), _whole([] if labels is None else labels, "labels")
+        _in_order(indices, teacher.shape() if teacher is not None else [], "index")
+        _in_order(labels, logits.shape()[:-1], "labels")
         _check(_lib.kh_distill_forward(self._h, logits._h, teacher._h if teacher is not None else None, indices.ctypes.data, indices.size,
                                        labels.ctypes.data, labels.size, weight._h if weight is not None else None, ctypes.byref(out)))
         return Tensor._wrap(out.value)

@@ -5,6 +5,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <set>
 #include <unordered_map>
 #include <unordered_set>
 #include <utility>
@@ -1184,6 +1185,18 @@ void check_tokens(const std::vector<int32_t> &tokens, size_t vocab, const char *
             fail(ErrorKind::InvalidOperand, std::string(what) + " " + std::to_string(token) + " of a vocabulary of " + std::to_string(vocab));
 }
 
+// Whether as many values of axes `a` as those of axes `b` lie in one order: the axes of one are neighbouring ones of the other, put together.
+bool in_order(const std::vector<size_t> &a, const std::vector<size_t> &b) {
+    auto ends = [](const std::vector<size_t> &shape) {  // how many values a step along each axis passes
+        std::set<size_t> steps = {1};
+        size_t step = 1;
+        for (auto axis = shape.rbegin(); axis != shape.rend(); ++axis) steps.insert(step *= *axis);
+        return steps;
+    };
+    const std::set<size_t> x = ends(a), y = ends(b);
+    return std::includes(x.begin(), x.end(), y.begin(), y.end()) || std::includes(y.begin(), y.end(), x.begin(), x.end());
+}
+
 std::vector<size_t> with_axis(std::vector<size_t> shape, size_t cols) {
     shape.push_back(cols);
     return shape;
@@ -1243,6 +1256,7 @@ Tensor DistillLoss::forward(const Tensor &logits, const Tensor &teacher, const s
     if (index.size() != rows * top) fail(ErrorKind::DataLength, "", rows * top, index.size());
     if (!labels.empty() && labels.size() != rows) fail(ErrorKind::DataLength, "", rows, labels.size());
     if (weight.defined() && weight.numel() != rows) fail(ErrorKind::DataLength, "", rows, weight.numel());
+    if (rows && weight.defined() && !in_order(weight.shape(), shape)) fail(ErrorKind::InvalidOperand, "weight must have the axes of the logits, but for the last");
     check_tokens(index, vocab, "index");
     check_tokens(labels, vocab, "label");
     auto loss = uninit_buffer(rows);

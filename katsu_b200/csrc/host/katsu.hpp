@@ -300,8 +300,8 @@ class DistillLoss {
     float soft() const { return soft_; }
     float hard() const { return hard_; }
     // teacher: undefined, or [..., top] with a token of `index` for every entry (negative: the entry is left out).  labels: empty, or one
-    // for every row (negative: none).  weight: undefined (1), or one for every row.  The result is [...]; a gradient reaches the logits
-    // alone.
+    // for every row (negative: none).  weight: undefined (1), or one for every row, of the rows' axes or these put together or apart.  The
+    // result is [...]; a gradient reaches the logits alone.
     Tensor forward(const Tensor &logits, const Tensor &teacher, const std::vector<int32_t> &index, const std::vector<int32_t> &labels,
                    const Tensor &weight) const;
 

@@ -66,3 +66,45 @@ def test_lists_of_nothing():
     for empty in ([], np.zeros((3, 0), int), np.zeros((0, 5), int)):
         got = K.adjust_logits(K.Tensor(z, [3, 4]), history=empty, bias_tokens=empty, bias=empty)
         assert np.array_equal(got.data(), z)
+
+
+# logits [2, 3, 9] against a teacher [2, 3, 4]: axes whose sizes multiply to the right number, in another order
+@pytest.mark.parametrize("what,shape", [("index", (3, 2, 4)), ("index", (4, 6)), ("index", (3, 8)), ("index", (4, 3, 2)), ("index", (6, 2, 2)),
+                                        ("index", (8, 3)), ("labels", (3, 2)), ("labels", (1, 3, 1, 2)), ("weight", [3, 2]),
+                                        ("weight", [3, 1, 2])], ids=str)
+def test_rows_in_another_order(what, shape):
+    args = {"teacher": K.Tensor.zeros([2, 3, 4]), "index": np.zeros((2, 3, 4), int)}
+    args[what] = K.Tensor.zeros(shape) if what == "weight" else np.zeros(shape, int)
+    with pytest.raises(K.InvalidOperand, match=f"{what} must have"):
+        K.DistillLoss().forward(K.Tensor.zeros([2, 3, 9]), **args)
+
+
+@pytest.mark.parametrize("shape", [(4, 6), (8, 3), (12, 2), (4, 3, 2)], ids=str)
+def test_lists_of_another_order_than_the_teachers(shape):
+    with pytest.raises(K.InvalidOperand, match="index must have"):
+        K.DistillLoss().forward(K.Tensor.zeros([6, 9]), K.Tensor.zeros([6, 4]), np.zeros(shape, int))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("index,labels,weight", [((2, 3, 4), (2, 3), [2, 3]), ((6, 4), (6,), [6]), ((24,), (6,), [2, 3, 1]), ((2, 1, 3, 4), (1, 2, 3), [1, 2, 3]), ((2, 12), (2, 3, 1), [1, 6])])
+def test_rows_in_order(index, labels, weight):
+    """Axes of one value, and axes that are put together, change no order."""
+    rng = np.random.default_rng(7)
+    z, teacher, at, label = (rng.standard_normal((6, 9)).astype(np.float32), rng.standard_normal((6, 4)).astype(np.float32),
+                             rng.integers(-1, 9, (6, 4)), rng.integers(-1, 9, 6))
+    w = rng.random(6).astype(np.float32)
+    loss = K.DistillLoss(2.0, 0.5, 0.5).forward(K.Tensor(z, [2, 3, 9]), K.Tensor(teacher, [2, 3, 4]), at.reshape(index), label.reshape(labels),
+                                               K.Tensor(w, weight))
+    assert loss.shape() == [2, 3]
+    want, off, _, _ = ref.distill(z, teacher, at, label, w, 2.0, 0.5, 0.5)
+    ref.assert_near(loss.data(), want, off)
+
+
+@pytest.mark.gpu
+def test_rows_of_more_axes_than_the_logits():
+    """Labels and weights [2, 3] of logits that were made [6, 9] for a product."""
+    rng = np.random.default_rng(8)
+    z, label, w = rng.standard_normal((6, 9)).astype(np.float32), rng.integers(-1, 9, 6), rng.random(6).astype(np.float32)
+    loss = K.DistillLoss(1.0, 0.0, 1.0).forward(K.Tensor(z, [6, 9]), labels=label.reshape(2, 3), weight=K.Tensor(w, [2, 3]))
+    want, off, _, _ = ref.distill(z, np.zeros((6, 0)), np.zeros((6, 0), int), label, w, 1.0, 0.0, 1.0)
+    ref.assert_near(loss.data(), want, off)

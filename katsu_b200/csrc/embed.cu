@@ -188,9 +188,9 @@ __device__ __forceinline__ unsigned key_of(int token, unsigned vocab) { return m
 // Up to 8192 tokens: the place of a token is the number of tokens that belong in front of it.  A block counts for 32 of them,
 // its warps over a sixteenth of the list each, 32 comparisons a lane for eight loads of 16 bytes that all lanes share: one launch
 // (3001 tokens 6 us, 8192 13; two lists side by side in a warp, for twice the blocks, took twice the time).
-constexpr int kRankThreads = 512;
+constexpr int kRankThreads = 512, kRankBlocks = 2;  // blocks of an SM: all 256 of a list are resident, so that each launch may start early
 
-__global__ void __launch_bounds__(kRankThreads) rank_kernel(const int *tokens, unsigned count, unsigned vocab, unsigned *keys, int *position) {
+__global__ void __launch_bounds__(kRankThreads, kRankBlocks) rank_kernel(const int *tokens, unsigned count, unsigned vocab, unsigned *keys, int *position) {
     __shared__ __align__(16) unsigned all[kMostRanked];
     __shared__ int partial[kRankThreads / 32][kRanked];
     launch_next();
@@ -242,7 +242,7 @@ struct Pass {
 __device__ __forceinline__ unsigned pass_key(const Pass &p, unsigned i) { return p.tokens ? key_of(p.tokens[i], p.vocab) : p.keys[i]; }
 
 // digits[block][digit]: how many of the block's keys have the digit.  next: zeros, for the pass behind.
-__global__ void __launch_bounds__(256) digits_kernel(Pass p, unsigned *digits, unsigned *next) {
+__global__ void __launch_bounds__(256, 1) digits_kernel(Pass p, unsigned *digits, unsigned *next) {
     __shared__ unsigned mine[kDigits];
     launch_next();
     const unsigned values = 1u << p.bits, mask = values - 1;
@@ -262,7 +262,7 @@ __global__ void __launch_bounds__(256) digits_kernel(Pass p, unsigned *digits, u
 // Moves the block's keys to their places, and counts the next pass's digits there (next, null: this is the last one; behind: zeros
 // for the one behind that).  A warp takes an eighth of them in order, so that equal digits keep theirs; eight keys a lane are on their
 // way together.  65536 tokens: 10 to 12 us a pass, most of it the chain of loads, counts and scans; counting 3.
-__global__ void __launch_bounds__(256) scatter_kernel(Pass p, const unsigned *digits, unsigned *next, unsigned *behind, unsigned *keys, int *position) {
+__global__ void __launch_bounds__(256, 1) scatter_kernel(Pass p, const unsigned *digits, unsigned *next, unsigned *behind, unsigned *keys, int *position) {
     __shared__ __align__(16) unsigned place[8][kDigits];
     __shared__ __align__(16) unsigned all[kDigits], front[kDigits];
     __shared__ unsigned sums[8];
@@ -371,6 +371,13 @@ __global__ void __launch_bounds__(256) scatter_kernel(Pass p, const unsigned *di
 
 // ---- the gradient ----------------------------------------------------------------------------------------------------------
 constexpr int kGradThreads = 128, kMostPiece = 64, kDirect = 256;
+// Blocks of an SM that the gradient's launches count with, where they ask whether one may start early; its kernels leave registers for
+// these and more.
+constexpr int kGradBlocks = 4, kPieceBlocks = 8, kAddBlocks = 5, kFoldBlocks = 5;
+// (few tokens of odd rows: 9 to 12 within 5 % of each other, 16, which spills, 200 tokens x 101 added 7.5 us instead of 5.9)
+constexpr int direct_blocks(bool whole, bool add) { return whole ? 8 : add ? 10 : 12; }
+static_assert(std::min({kPieceBlocks, kAddBlocks, kFoldBlocks, direct_blocks(true, true)}) >= kGradBlocks,
+              "launches that start early have all their blocks resident");
 constexpr int kApart = 2;
 
 struct Grad {
@@ -474,7 +481,7 @@ __device__ __forceinline__ void fill_rows(const Grad &g, const bool *there, unsi
 
 // Up to kDirect tokens, without sorting: a group of 1 << shift threads takes the run of one token, if that is its first place.
 template <bool WHOLE, int N, bool ADD>
-__global__ void __launch_bounds__(kGradThreads) embed_direct_kernel(Grad g) {
+__global__ void __launch_bounds__(kGradThreads, direct_blocks(WHOLE, ADD)) embed_direct_kernel(Grad g) {
     __shared__ __align__(16) unsigned keys[kDirect];
     __shared__ bool there[kGradThreads];
     if (!g.waves) launch_next();
@@ -536,7 +543,7 @@ __global__ void __launch_bounds__(kGradThreads) embed_direct_kernel(Grad g) {
 // Blocks 0 .. piece_blocks - 1: a group of 1 << shift threads adds up a piece (a slab of 1 << shift accesses of its rows); the
 // blocks behind them write zeros to fill_rows rows of the table each, but for those of tokens that are there.
 template <bool WHOLE, int N, bool ADD>
-__global__ void __launch_bounds__(kGradThreads, ADD ? 5 : 8) embed_grad_kernel(Grad g) {
+__global__ void __launch_bounds__(kGradThreads, ADD ? kAddBlocks : kPieceBlocks) embed_grad_kernel(Grad g) {
     const unsigned width = 1u << g.shift, groups = kGradThreads >> g.shift, mine = threadIdx.x >> g.shift, lane = threadIdx.x & (width - 1);
     extern __shared__ unsigned keys[];  // of the block's pieces, their positions behind them
     int *position = reinterpret_cast<int *>(keys + groups * g.piece + 2);
@@ -628,7 +635,7 @@ __device__ __forceinline__ void add_kept(const Grad &g, const Part<WHOLE, N> &pa
 }
 
 template <bool WHOLE, int N>
-__global__ void __launch_bounds__(kGradThreads) embed_bundle_kernel(Grad g) {
+__global__ void __launch_bounds__(kGradThreads, kFoldBlocks) embed_bundle_kernel(Grad g) {
     const unsigned groups = kGradThreads >> g.shift;
     if (!g.waves) launch_next();
     launch_wait();
@@ -689,7 +696,7 @@ static_assert(folds_of_a_warp_are_right(), "a value of a run is folded by one la
 // group of threads, a warp at least: of rows of fewer threads as many neighbouring parts of the run as fit there are added up at once
 // (100 000 x 16: 8 us; 32 where a run had four threads that looked at four pieces at a time).
 template <bool WHOLE, int N, bool ADD>
-__global__ void __launch_bounds__(kGradThreads) embed_fold_kernel(Grad g) {
+__global__ void __launch_bounds__(kGradThreads, kFoldBlocks) embed_fold_kernel(Grad g) {
     const int shift = max(g.shift, 5);
     const unsigned groups = kGradThreads >> shift, lane = threadIdx.x & 31, width = 1u << g.shift;
     if (!g.waves) launch_next();
@@ -759,7 +766,7 @@ int32_t launch_grad(katsu_cuda_ctx *ctx, Grad g) {
     if (blocks > 0x7fffffffu)
         return katsu_set_error(KATSU_ERR_UNSUPPORTED, "%u tokens with rows of %zu values in one gradient", g.count, g.cols);
     g.piece_blocks = unsigned(piece_blocks);
-    const size_t resident = size_t(4) * ctx->num_sms;  // (of 128 threads with up to 128 registers)
+    const size_t resident = size_t(kGradBlocks) * ctx->num_sms;
     g.waves = blocks > resident;
     if (g.tokens) return katsu_launch(ctx, !g.waves, embed_direct_kernel<WHOLE, N, ADD>, unsigned(blocks), kGradThreads, 0, 1, g);
     KATSU_TRY(katsu_launch(ctx, !g.waves, embed_grad_kernel<WHOLE, N, ADD>, unsigned(blocks), kGradThreads, (2 * groups * g.piece + 2) * sizeof(unsigned), 1, g));

@@ -5,7 +5,7 @@ import pytest
 
 import vocab_ref as ref
 from parity_util import DeviceArrays
-from test_embed import some_tokens
+from test_embed import GRADS, some_tokens
 
 
 def whole_numbers(rng, shape):
@@ -25,10 +25,14 @@ def sums_of(tokens, dy, vocab):
     return want
 
 
-def check(ctx, count, vocab, cols, how, accumulate, shift=0, seed=0):
+def check(ctx, count, vocab, cols, how, accumulate, shift=0):
+    rng = np.random.default_rng([count, vocab, cols])
+    check_tokens(ctx, some_tokens(rng, count, vocab, how), vocab, cols, rng, accumulate, shift)
+
+
+def check_tokens(ctx, tokens, vocab, cols, rng, accumulate=1, shift=0):
     """Twice, as what threads write at the same time need not come out alike."""
-    rng = np.random.default_rng([seed, count, vocab, cols])
-    tokens, dy, before = some_tokens(rng, count, vocab, how), whole_numbers(rng, (count, cols)), whole_numbers(rng, (vocab, cols))
+    count, dy, before = len(tokens), whole_numbers(rng, (len(tokens), cols)), whole_numbers(rng, (vocab, cols))
     want = sums_of(tokens, dy, vocab) * 0.5 + (before if accumulate else 0)
     assert np.abs(want).max() + 3 < 2 ** 22  # (halves of numbers below 2^24 are numbers of f32)
     edge = np.full(4, 7.0, np.float32)
@@ -52,3 +56,28 @@ def check(ctx, count, vocab, cols, how, accumulate, shift=0, seed=0):
 @pytest.mark.parametrize("cols", [4, 8, 12, 16, 20, 28, 32, 33, 36, 40, 44, 48, 52, 56, 60, 63, 64, 65, 68, 128])
 def test_runs_over_many_pieces_in_narrow_rows(ctx, cols, count, vocab, how, shift, accumulate):
     check(ctx, count, vocab, cols, how, accumulate, shift)
+
+
+# Counts on both sides of those where the gradient takes another way, runs of many pieces, bundles and parts among them
+@pytest.mark.gpu
+@pytest.mark.parametrize("accumulate", [0, 1])
+@pytest.mark.parametrize("count,vocab,cols,how", GRADS + [
+    (1000003, 7, 4, "half"), (400000, 3, 17, "one"), (400000, 40, 64, "blocks"), (131072, 1, 130, "one"), (262144, 16, 16, "blocks"), (50000, 9, 40, "half")])
+def test_every_sum(ctx, count, vocab, cols, how, accumulate):
+    check(ctx, count, vocab, cols, how, accumulate)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cols", [4, 12, 24, 48, 64, 200])
+@pytest.mark.parametrize("off", [-1, 0, 1])
+@pytest.mark.parametrize("piece", [8, 16, 32])
+def test_runs_that_end_around_pieces_and_bundles(ctx, piece, off, cols):
+    """Runs of 1, 2, 31 to 33 and 64 pieces behind each other, a token more or less than whole ones."""
+    lengths = [max(1, piece * n + off) for n in (1, 2, 31, 32, 33, 64, 1, 0, 96, 5)]
+    tokens = np.repeat(np.arange(len(lengths)), lengths)
+    for start in (0, 1, 7):  # what is no token sorts behind; a token in front moves all ends
+        keys = np.concatenate([np.zeros(start, int), tokens + 1])
+        rng = np.random.default_rng([piece, cols, start])
+        order = rng.permutation(len(keys))
+        for times in (1, 9):  # (longer lists have longer pieces)
+            check_tokens(ctx, np.tile(keys[order], times), len(lengths) + 1, cols, rng)

@@ -139,7 +139,11 @@ struct Row {
     }
 };
 
-// Blocks of an SM, by 40 registers a thread.
+// Blocks of an SM: five of 256 threads, which have 40 registers each; 17, 10 and 3 of 64, 128 and 512, which are 51 warps, three more than
+// fit with 40, and so have 32: the gradient with both sums then keeps 68 bytes a thread in local memory, the loss up to 28.  More warps are
+// worth that.  Two blocks of 512 threads, with 56 registers and nothing in local memory, take 194 us for 4096 x 32768 instead of 180, 206
+// instead of 189 for 2000 x 65536; 9 of 128 and 16 of 64 threads with 40 registers 41 instead of 38 for 8192 x 1003, 227 instead of 213 for
+// 100 000 x 50.
 constexpr int blocks_of_sm(int threads) { return 65536 / ((threads + 32) * 40); }
 
 // THREADS threads go through the row, the warp behind them through its entries.  GRAD: writes the gradient (and the loss where it is

@@ -294,7 +294,8 @@ __global__ void __launch_bounds__(THREADS + 32, blocks_of_sm(THREADS)) distill_k
             double loss = 0.0;
             const double T = a.temperature;
             if (taught) loss += a.soft * (T * T) * (apart / total / T - log(total) + log(double(s.s0)));
-            if (labelled) loss += a.hard * (double(b) + log(double(s1)) - double(entries.z[a.top]));
+            // (the difference first: next to logits of a mask's lowest number the logarithm is nothing)
+            if (labelled) loss += a.hard * ((double(b) - double(entries.z[a.top])) + log(double(s1)));
             a.loss[row] = float(weight * loss);
         }
     }

@@ -53,3 +53,21 @@ def test_short_rows(ctx, rows, vocab, top, T, soft, hard):
 def test_long_rows(ctx, rows, vocab, top, T, soft, hard):
     want = Formula(inputs(rows, vocab, top), T, soft, hard)
     assert np.array_equal(want.check(ctx), want.check(ctx, in_place=True))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,soft,hard", [(1.0, 0.0, 1.0), (1.0, 0.5, 0.5), (2.0, 0.5, 1.0), (0.5, 1.0, 0.3)])
+@pytest.mark.parametrize("vocab", [2, 50, 1003, 40001])
+def test_logits_that_are_large_and_alike(ctx, vocab, T, soft, hard):
+    """Rows of one number, a mask's lowest one among them, and rows of a few numbers far from 0: the loss is that of their differences."""
+    a = inputs(12, vocab, 4)
+    low = np.finfo(np.float32).min
+    for row, value in enumerate([low, -1e30, 1e30, -low, 3e20, -2.0 ** 60, low, 1e9]):
+        a["z"][row] = value
+    a["z"][8] = np.where(np.arange(vocab) % 2, 1e30, low)           # half of them masked, the others alike
+    a["z"][9] = 2.0 ** 40 + 2.0 ** 18 * (np.arange(vocab) % 3)      # steps of the numbers there
+    a["z"][10] = -2.0 ** 26 + 4.0 * (np.arange(vocab) % 5)
+    a["index"][8], a["labels"][8] = 1, 1
+    a["labels"][:8] = np.arange(8) % vocab
+    a["weight"][:], a["teacher"] = 1.0, np.random.default_rng(1).standard_normal(a["teacher"].shape).astype(np.float32)
+    Formula(a, T, soft, hard).check(ctx)

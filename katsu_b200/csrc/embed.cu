@@ -9,8 +9,8 @@
 // ones cost.  Runs that lie in one piece are written as they end; what a piece has of a run that began in front of it or goes on behind
 // it is kept beside the table and folded in the pieces' order by a launch behind, in two steps where runs may be long.  Rows without
 // a token get zeros from blocks of the pieces' launch.  No floating-point atomics: the same tokens give the same bits.  Bound: HBM for
-// large gradients (65536 x 2048 into a table of as many rows: 152 us of 198, 7.1 TB/s with what L2 keeps; sorting 25, folding 19),
-// three launches one behind the other for small ones (3001 x 515: 15.5 us).
+// large gradients (65536 x 2048 into a table of as many rows: 154 us of 196, 7.0 TB/s with what L2 keeps; sorting 21, folding 19),
+// three launches one behind the other for small ones (3001 x 515: 15.3 us).
 #include <algorithm>
 
 #include "common.cuh"
@@ -261,7 +261,7 @@ __global__ void __launch_bounds__(256, 1) digits_kernel(Pass p, unsigned *digits
 
 // Moves the block's keys to their places, and counts the next pass's digits there (next, null: this is the last one; behind: zeros
 // for the one behind that).  A warp takes an eighth of them in order, so that equal digits keep theirs; eight keys a lane are on their
-// way together.  65536 tokens: 10 to 12 us a pass, most of it the chain of loads, counts and scans; counting 3.
+// way together.  65536 tokens: 8 to 10 us a pass, most of it the chain of loads, counts and scans; counting 3.
 __global__ void __launch_bounds__(256, 1) scatter_kernel(Pass p, const unsigned *digits, unsigned *next, unsigned *behind, unsigned *keys, int *position) {
     __shared__ __align__(16) unsigned place[8][kDigits];
     __shared__ __align__(16) unsigned all[kDigits], front[kDigits];
